@@ -30,6 +30,9 @@ extern "C" {
 
 #define GLAD_DTYPE_F32 0
 #define GLAD_DTYPE_F16 1
+#define GLAD_DTYPE_BF16 2   /* rms_norm and w4_linear only */
+#define GLAD_DTYPE_I8 3     /* 8-bit activations: two's complement */
+#define GLAD_DTYPE_E4M3 4   /* 8-bit activations: 4 exponent, 3 mantissa bits, no infinities */
 
 #define GLAD_ACT_STATIC 0   /* qrt QuantLinear act_mode="static"  (qrt/qlinear.py:132-135) */
 #define GLAD_ACT_DYNAMIC 1  /* qrt QuantLinear act_mode="dynamic" (qrt/qlinear.py:125-131) */
@@ -380,6 +383,71 @@ int glad_w4a16_mlp_forward(const GladW4Linear* mlp, const void* x, int64_t M, in
 int glad_actor_forward_w4a16(const GladActorWeights* w, const GladW4Linear* mlp, const void* obs,
                              int obs_dtype, int64_t B, int64_t ld_obs, int act_mode, float* mean_out,
                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- root-mean-square norm (no counterpart in the reference) -----------------
+ * Rows x [rows, cols] (f32, f16 or bf16, row stride ldx elements), optionally
+ * plus a residual of x's type or f32:
+ *   h = x + residual, rounded to the residual's type    (h = x without one)
+ *   rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight
+ * weight [cols] has x's type or f32, or is NULL (ones). y has x's type, sum_out
+ * (h) the residual's; both contiguous. residual and sum_out go together.
+ * rstd_out (NULL or f32 [rows]) is what the backward pass reads. Statistics
+ * and products are f32. cols 1..32768.                                      */
+int glad_rms_norm_forward(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr,
+                          const void* weight, int w_dtype, int64_t rows, int cols, float eps, void* y, void* sum_out,
+                          float* rstd_out, void* stream);
+
+/* The same norm with an 8-bit output q [rows, cols] (GLAD_DTYPE_I8 or
+ * GLAD_DTYPE_E4M3) of the unrounded y: q = round_half_even(y * (1/s)), |q| at
+ * most Q = 127 (i8) or 448 (e4m3).
+ *   given_scale (device f32 [1]): s is that scale for the whole tensor;
+ *   group 0: one scale a row, s = max|y| / Q, 1 for a row of zeros; scales [rows];
+ *   group 32, 64, 128: one scale for that many columns, the last group of a row
+ *     may be shorter; scales [rows, ceil(cols / group)].
+ * A NaN in a row (group) makes its scale NaN; its i8 code is 0.              */
+int glad_rms_norm_quant(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr,
+                        const void* weight, int w_dtype, int64_t rows, int cols, float eps, int q_dtype, int group,
+                        const float* given_scale, void* q, float* scales, void* sum_out, void* stream);
+
+/* Backward pass of glad_rms_norm_forward. dy [rows, cols] of x's type (x_dtype),
+ * dsum (the gradient of sum_out, NULL: none) and h of the sum's type (h_dtype;
+ * x's without a residual), rstd of the forward pass. With g = dy * weight:
+ *   d = dsum + rstd * (g - h * rstd^2 * mean(g * h))
+ * dx (x's type) and dresidual (the sum's type) are d; dweight = sum over rows of
+ * dy * h * rstd (the weight's type). Any of the three may be NULL. dweight is
+ * summed in a fixed order: the same call gives the same bits. The workspace
+ * is needed for dweight only; its contents need no initialisation.          */
+size_t glad_rms_norm_backward_workspace_size(int64_t rows, int cols);
+int glad_rms_norm_backward(const void* dy, int x_dtype, int64_t lddy, const void* dsum, int h_dtype, int64_t lddsum,
+                           const void* h, int64_t ldh, const void* weight, int w_dtype, const float* rstd,
+                           int64_t rows, int cols, void* dx, void* dresidual, void* dweight, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* ---- 4-bit linear of any shape (no counterpart in the reference) ---------------
+ * y[m, n] = sum_g xs[m, g] * scales[n, g] * sum_{k in group g} x[m, k] * q[n, k] + bias[n]
+ * with q int4 in [-8, 7] and one f16 scale for `group` (32, 64 or 128)
+ * consecutive inputs of a row. `tiles` and `scales` hold the weight in blocks:
+ *   tiles  [ceil(N/16)][KB][32][4] u32, KB = ceil(K / b) * b / 64, b = max(64, group):
+ *          word j of lane 4*r + c of block (t, kb) holds rows n = 16t + r and
+ *          n + 8, inputs k = 64 kb + 32 (j >> 1) + 8 c + 4 (j & 1) + (0..3); nibble i
+ *          (bits 4i..4i+3) is row n + 8 (i & 1), input k + 2 ((i >> 1) & 1) + (i >> 2);
+ *          zero past N and K
+ *   scales [ceil(N/16)][KB * 64 / group][16] f16, zero past N and K
+ * x [M, K] (row stride ldx elements): f16 or bf16 with x_scale NULL; i8 or e4m3
+ * with x_scale f32: one for all rows (x_scale_rows 0), one a row (x_scale_groups
+ * 1) or one a row and group (x_scale_groups = ceil(K / group), rows contiguous).
+ * y [M, N] contiguous, f16, bf16 or f32; bias [N] of y's type or NULL. The inner
+ * sums are exact products accumulated in f32. K is even. No workspace.        */
+typedef struct GladW4Weight {
+  const void* tiles;    /* 16-byte aligned */
+  const void* scales;   /* 16-byte aligned */
+  int32_t in_features, out_features, group;
+} GladW4Weight;
+size_t glad_w4_tiles_bytes(int in_features, int out_features, int group);
+size_t glad_w4_scales_bytes(int in_features, int out_features, int group);
+int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, int64_t M, int64_t ldx,
+                           const float* x_scale, int x_scale_rows, int x_scale_groups, const void* bias, void* y,
+                           int y_dtype, void* stream);
 
 /* ---- weight refresh (qrt/runtime.py:195-271) ------------------------------- */
 

@@ -5,6 +5,7 @@ sm_100 part, every entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
@@ -23,6 +24,11 @@ GLAD_ERR_WORKSPACE = -5
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2
+DTYPE_I8 = 3
+DTYPE_E4M3 = 4
+DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.int8: DTYPE_I8,
+          torch.float8_e4m3fn: DTYPE_E4M3}
 ACT_STATIC = 0
 ACT_DYNAMIC = 1
 ACT_MODES = {"static": ACT_STATIC, "dynamic": ACT_DYNAMIC}
@@ -85,6 +91,11 @@ class GladW4Linear(Structure):
                 ("out_features", c_int)]
 
 
+class GladW4Weight(Structure):
+    _fields_ = [("tiles", c_void_p), ("scales", c_void_p), ("in_features", c_int32), ("out_features", c_int32),
+                ("group", c_int32)]
+
+
 class GladPackItem(Structure):
     _fields_ = [("tensor", c_void_p), ("nbytes", c_size_t), ("offset", c_size_t)]
 
@@ -139,6 +150,18 @@ SIGNATURES = {
     "glad_actor_kernel_count": (c_int, [c_int64, c_int]),
     "glad_workspace_status": (c_int, [c_void_p, POINTER(c_uint32), c_void_p]),
     "glad_debug_mlp_barrier": (c_int, [c_uint32, c_uint64]),
+    "glad_rms_norm_forward": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
+                                      c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "glad_rms_norm_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
+                                    c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "glad_rms_norm_backward_workspace_size": (c_size_t, [c_int64, c_int]),
+    "glad_rms_norm_backward": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64,
+                                       c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_void_p]),
+    "glad_w4_tiles_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "glad_w4_scales_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "glad_w4_linear_forward": (c_int, [POINTER(GladW4Weight), c_void_p, c_int, c_int64, c_int64, c_void_p, c_int,
+                                       c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "glad_requant_qlinear": (c_int, [POINTER(GladQLinearSrc), c_int, c_void_p]),
     "glad_requant_qcnn": (c_int, [POINTER(GladQCNNSrc), c_void_p]),
     "glad_cast_copy": (c_int, [POINTER(GladCastCopy), c_int, c_void_p]),
@@ -180,6 +203,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def device_guard(device: torch.device):
+    """Launches go to the tensors' device; a no-op when it is the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
+
+
+_NO_GUARD = contextlib.nullcontext()
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:

@@ -1,0 +1,188 @@
+"""4-bit linear of any shape, for few rows to many: int4 weights with one fp16 scale a group of inputs.
+
+The weight format is ``quantize_w4``'s (rl_quant_b200/w4a16.py, the format of the W4A16 actor MLP) with groups of
+32, 64 or 128; ``pack_w4`` lays it out once in the order the kernel streams it (include/glad_b200.h, GladW4Weight).
+Rows are fp16 or bf16, or 8-bit codes with scales as ``rms_norm_quant`` writes them. Products are exact, sums fp32 and
+the group's scale multiplies the group's sum: y = sum_g s[n,g] * (sum_k x[m,k] q[n,k]) + b, rounded once.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import _native as N
+from .w4a16 import quantize_w4
+
+GROUPS = (32, 64, 128)
+_OUT = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _shapes(in_features: int, out_features: int, group: int):
+    """(row tiles, 64-input blocks, padded groups) of the laid-out weight."""
+    b = max(64, group)
+    kb = -(-in_features // b) * b // 64
+    return -(-out_features // 16), kb, kb * 64 // group
+
+
+class W4Weight:
+    """A laid-out 4-bit weight [out_features, in_features]: ``tiles`` (uint8) and ``scales`` (fp16) on one device."""
+
+    __slots__ = ("tiles", "scales", "in_features", "out_features", "group")
+
+    def __init__(self, tiles, scales, in_features, out_features, group):
+        if group not in GROUPS:
+            raise ValueError(f"group must be one of {GROUPS}, got {group}")
+        if in_features < 2 or in_features % 2:
+            raise ValueError(f"in_features must be even, got {in_features}")
+        t, kb, gp = _shapes(in_features, out_features, group)
+        if tiles.dtype != torch.uint8 or tuple(tiles.shape) != (t, kb, 512) or not tiles.is_contiguous():
+            raise ValueError(f"tiles must be contiguous uint8 [{t}, {kb}, 512]")
+        if scales.dtype != torch.float16 or tuple(scales.shape) != (t, gp, 16) or not scales.is_contiguous():
+            raise ValueError(f"scales must be contiguous float16 [{t}, {gp}, 16]")
+        if tiles.device != scales.device:
+            raise ValueError(f"tiles on {tiles.device}, scales on {scales.device}")
+        self.tiles, self.scales = tiles, scales
+        self.in_features, self.out_features, self.group = in_features, out_features, group
+
+
+@torch.no_grad()
+def pack_w4(packed: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4Weight:
+    """``quantize_w4``'s (packed uint8 [N, K/2], scales fp16 [N, ceil(K/group)]) as a ``W4Weight``."""
+    if group not in GROUPS:
+        raise ValueError(f"group must be one of {GROUPS}, got {group}")
+    if packed.dtype != torch.uint8 or packed.dim() != 2 or packed.shape[0] < 1 or packed.shape[1] < 1:
+        raise ValueError("packed must be uint8 [N, K/2]")
+    n, k = packed.shape[0], 2 * packed.shape[1]
+    if scales.dtype != torch.float16 or tuple(scales.shape) != (n, -(-k // group)):
+        raise ValueError(f"scales must be float16 [{n}, {-(-k // group)}]")
+    t, kb, gp = _shapes(k, n, group)
+    q = torch.zeros(t * 16, kb * 64, dtype=torch.uint8, device=packed.device)
+    q[:n, 0:k:2] = packed & 15
+    q[:n, 1:k:2] = packed >> 4
+    # [t, row half, row, kb, j/2, c, j%2, k/2, k%2] -> byte (k/2 + 2 (k%2)) of word j, row half in the nibble
+    v = q.view(t, 2, 8, kb, 2, 4, 2, 2, 2)
+    b = (v[:, 0] | (v[:, 1] << 4)).permute(0, 2, 1, 4, 3, 5, 7, 6)
+    s = torch.zeros(t * 16, gp, dtype=torch.float16, device=scales.device)
+    s[:n, :scales.shape[1]] = scales
+    return W4Weight(b.reshape(t, kb, 512).contiguous(), s.view(t, 16, gp).permute(0, 2, 1).contiguous(), k, n, group)
+
+
+@torch.no_grad()
+def unpack_w4(weight: W4Weight):
+    """The inverse of ``pack_w4``: (packed, scales)."""
+    t, kb, gp = _shapes(weight.in_features, weight.out_features, weight.group)
+    b = weight.tiles.view(t, kb, 8, 4, 2, 2, 2, 2).permute(0, 2, 1, 4, 3, 5, 7, 6)
+    q = torch.stack((b & 15, b >> 4), dim=1).reshape(t * 16, kb * 64)[:weight.out_features, :weight.in_features]
+    packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
+    g = -(-weight.in_features // weight.group)
+    s = weight.scales.permute(0, 2, 1).reshape(t * 16, gp)[:weight.out_features, :g].contiguous()
+    return packed, s
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = None,
+              x_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """x [..., K] times the weight's transpose, plus bias: y [..., N].
+
+    x float16 or bfloat16 (``x_scale`` None, ``out_dtype`` x's by default), or int8 / float8_e4m3fn codes with a float32
+    ``x_scale`` of one value, [..., 1] (one a row) or [..., ceil(K / group)] (one a row and group of the weight) and
+    ``out_dtype`` named. out_dtype float16, bfloat16 or float32; bias [N] has it. Inference only."""
+    K, n = weight.in_features, weight.out_features
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"x {tuple(x.shape)} does not match in_features {K}")
+    eight = x.dtype in (torch.int8, torch.float8_e4m3fn)
+    if not eight and x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"x is {x.dtype}; expected float16, bfloat16, int8 or float8_e4m3fn")
+    if out_dtype is None:
+        if eight:
+            raise ValueError("8-bit rows need out_dtype")
+        out_dtype = x.dtype
+    if out_dtype not in _OUT:
+        raise TypeError(f"out_dtype is {out_dtype}; expected float16, bfloat16 or float32")
+    per_row = groups = 0
+    if eight:
+        if x_scale is None:
+            raise ValueError("8-bit rows need x_scale")
+        if x_scale.dtype != torch.float32:
+            raise TypeError(f"x_scale is {x_scale.dtype}; expected float32")
+        if x_scale.numel() != 1 or x_scale.shape == x.shape[:-1] + (1,):
+            g = -(-K // weight.group)
+            if x_scale.shape == x.shape[:-1] + (1,):
+                per_row, groups = 1, 1
+            elif x_scale.shape == x.shape[:-1] + (g,):
+                per_row, groups = 1, g
+            else:
+                raise ValueError(f"x_scale {tuple(x_scale.shape)}: one value, {tuple(x.shape[:-1]) + (1,)} or "
+                                 f"{tuple(x.shape[:-1]) + (g,)}")
+            if not x_scale.is_contiguous():
+                x_scale = x_scale.contiguous()
+    elif x_scale is not None:
+        raise ValueError("x_scale is for 8-bit rows")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != out_dtype):
+        raise ValueError(f"bias must be {out_dtype} [{n}]")
+    for t in (weight.tiles, bias, x_scale):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"tensors on {x.device} and {t.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("w4_linear has no gradient; use torch.no_grad()")
+    N.require_cuda(x)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
+    w = N.GladW4Weight(weight.tiles.data_ptr(), weight.scales.data_ptr(), K, n, weight.group)
+    with N.device_guard(x.device):
+        N.check(N.load().glad_w4_linear_forward(
+            w, x2.data_ptr(), N.DTYPES[x.dtype], x2.shape[0], x2.stride(0), N.ptr(x_scale), per_row, groups,
+            N.ptr(bias), y.data_ptr(), N.DTYPES[out_dtype], N.stream_handle(x.device)), "w4_linear")
+    return y
+
+
+class W4Linear(nn.Module):
+    """``nn.Linear`` with 4-bit weights at inference and its own Parameters in training, like ``QuantLinear``:
+    with gradients enabled the forward is ``F.linear`` on the source layer's weight and bias; without, ``w4_linear`` on
+    the laid-out copy, which ``requantize_`` rewrites in place (captured CUDA graphs stay valid).
+    ``forward(q, x_scale)`` takes 8-bit rows."""
+
+    def __init__(self, linear: nn.Linear, group: int = 64):
+        super().__init__()
+        if group not in GROUPS:
+            raise ValueError(f"group must be one of {GROUPS}, got {group}")
+        if linear.in_features % 2:
+            raise ValueError(f"in_features={linear.in_features} is odd")
+        self.in_features, self.out_features, self.group = linear.in_features, linear.out_features, group
+        # the source layer's Parameters, transferred (optimiser references stay valid)
+        self.weight = linear.weight
+        self.bias = linear.bias
+        t, kb, gp = _shapes(self.in_features, self.out_features, group)
+        dev = linear.weight.device
+        self.register_buffer("tiles", torch.zeros(t, kb, 512, dtype=torch.uint8, device=dev))
+        self.register_buffer("scales", torch.zeros(t, gp, 16, dtype=torch.float16, device=dev))
+        self.requantize_()
+
+    @torch.no_grad()
+    def requantize_(self):
+        """Refresh the 4-bit copy from the current weight, in place."""
+        w = pack_w4(*quantize_w4(self.weight, self.group), self.group)
+        self.tiles.copy_(w.tiles)
+        self.scales.copy_(w.scales)
+        return self
+
+    def w4(self) -> W4Weight:
+        return W4Weight(self.tiles, self.scales, self.in_features, self.out_features, self.group)
+
+    def forward(self, x, x_scale=None, out_dtype=None):
+        if torch.is_grad_enabled() and x_scale is None:
+            return F.linear(x, self.weight, self.bias)
+        if out_dtype is None and x_scale is not None:
+            out_dtype = self.weight.dtype
+        bias = self.bias
+        if bias is not None:
+            bias = bias.to(out_dtype or x.dtype)
+        with torch.no_grad():
+            return w4_linear(x, self.w4(), bias, x_scale, out_dtype)
+
+    def extra_repr(self):
+        return f"in={self.in_features}, out={self.out_features}, group={self.group}, bias={self.bias is not None}"

@@ -1,0 +1,401 @@
+"""rms_norm / rms_norm_quant against the formula in 64 bits.
+
+Tolerances, fixed before the first run: a row's sum of squares is at most 32 adds a thread and 10 levels of a tree, each
+off by 2^-24 of the running sum of positive terms, and enters 1/rms by half; square root, quotient and two products add
+2^-24 each. So y is off by at most F32 = 64 * 2^-24 relative before it is rounded (half a step, finfo.eps / 2). The
+row sums of the backward pass have terms of both signs: 64 * 2^-24 of the sum of their magnitudes."""
+import numpy as np
+import pytest
+import torch
+
+from rl_quant_b200 import _native as N
+from rl_quant_b200.norm import MAX_COLS, RMSNorm, rms_norm, rms_norm_quant
+
+F32 = 64 * 2.0 ** -24
+EPS = 1e-6
+PAIRS = [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32),
+         (torch.float16, torch.float32), (torch.bfloat16, torch.float32)]
+gpu = pytest.mark.gpu
+
+
+def half_step(t):
+    return 0.0 if t == torch.float32 else torch.finfo(t).eps / 2
+
+
+def tiny(t):          # half the spacing of the subnormal numbers
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def rows(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+def ref_norm(h, w, eps=EPS):
+    h = h.double()
+    rstd = 1.0 / torch.sqrt((h * h).mean(-1, keepdim=True) + eps)
+    return h * rstd * (1.0 if w is None else w.double()), rstd
+
+
+def check_y(y, ref):
+    tol = (half_step(y.dtype) * (1 + F32) + F32) * ref.abs() + tiny(y.dtype)
+    assert ((y.double() - ref).abs() <= tol).all()
+
+
+# widths: one column, a lone vector, off every vector width, one and two words a thread, the largest
+SIZES = [(1, 1), (3, 8), (1, 2048), (2, 1000), (5, 1111), (1, 8192), (300, 264), (700, 1301), (600, 4096), (1, 32768),
+         (2, 16391), (299, 32767), (310, 20000)]
+
+
+@gpu
+@pytest.mark.parametrize("x_t,r_t", PAIRS)
+@pytest.mark.parametrize("shape", SIZES)
+def test_forward(shape, x_t, r_t):
+    x, r = rows(shape, x_t, 1), rows(shape, r_t, 2, 5.0)
+    for w in (None, rows(shape[1:], x_t, 3), rows(shape[1:], torch.float32, 4)):
+        y = rms_norm(x, w, eps=EPS)
+        assert y.dtype == x_t and y.shape == x.shape
+        check_y(y, ref_norm(x, w)[0])
+    y, h = rms_norm(x, w, residual=r, eps=EPS)
+    assert h.dtype == r_t and torch.equal(h, (x.float() + r.float()).to(r_t))
+    check_y(y, ref_norm(h, w)[0])
+
+
+def grads(h, w, dy, dh, x_t, r_t):
+    """64-bit gradients and the magnitudes their roundings scale with."""
+    C = h.shape[-1]
+    h, dy = h.double(), dy.double()
+    rstd = 1.0 / torch.sqrt((h * h).mean(-1, keepdim=True) + EPS)
+    g = dy * (1.0 if w is None else w.double())
+    d = rstd * (g - h * rstd ** 2 * (g * h).sum(-1, keepdim=True) / C)
+    mag = rstd * (g.abs() + h.abs() * rstd ** 2 * (g * h).abs().sum(-1, keepdim=True) / C)
+    if dh is not None:
+        d, mag = d + dh.double(), mag + dh.double().abs()
+    unit = h * rstd
+    return d, mag, (dy * unit).sum(0), (dy * unit).abs().sum(0)
+
+
+@gpu
+@pytest.mark.parametrize("x_t,r_t", PAIRS)
+@pytest.mark.parametrize("shape", SIZES + [(2500, 72), (1200, 512), (1, 32)])
+@pytest.mark.parametrize("with_res", [False, True])
+def test_backward(shape, x_t, r_t, with_res):
+    if not with_res and r_t != x_t:
+        pytest.skip("the residual's type without a residual")
+    for w_t in {x_t, torch.float32}:
+        x = rows(shape, x_t, 1).requires_grad_()
+        w = (1 + 0.3 * rows(shape[1:], torch.float32, 3)).to(w_t).requires_grad_()
+        r = rows(shape, r_t, 2, 5.0).requires_grad_() if with_res else None
+        dy, dh = rows(shape, x_t, 5), rows(shape, r_t, 6) if with_res else None
+        if with_res:
+            y, h = rms_norm(x, w, residual=r, eps=EPS)
+            dx, dw, dr = torch.autograd.grad((y, h), (x, w, r), (dy, dh))
+        else:
+            y, h = rms_norm(x, w, eps=EPS), x
+            (dx, dw), dr = torch.autograd.grad(y, (x, w), dy), None
+        check_y(y.detach(), ref_norm(h.detach(), w.detach())[0])
+        d, mag, dw_ref, dw_mag = grads(h.detach(), w.detach(), dy, dh, x_t, r_t)
+        for got, t in ((dx, x_t), (dr, r_t)):
+            if got is not None:
+                assert got.dtype == t
+                tol = half_step(t) * d.abs() + 2 * F32 * mag + tiny(t)
+                assert ((got.double() - d).abs() <= tol).all()
+        assert dw.dtype == w_t
+        tol = half_step(w_t) * dw_ref.abs() + (shape[0] + 64) * 2.0 ** -24 * dw_mag * (1 + half_step(w_t)) \
+            + F32 * dw_mag + tiny(w_t)
+        assert ((dw.double() - dw_ref).abs() <= tol).all()
+
+
+@gpu
+def test_gradient_against_differences():
+    """Central differences of the scalar sum(dy * y + dh * h) along random directions, all in fp32: the step 2^-6 leaves a
+    truncation error of order 2^-12 and a rounding error of order 2^-24 * 2^6 * sqrt(n), far below the 1% asked."""
+    x, w, r = rows((6, 200), torch.float32, 1), 1 + 0.3 * rows((200,), torch.float32, 2), rows((6, 200), torch.float32, 3)
+    dy, dh = rows((6, 200), torch.float32, 4), rows((6, 200), torch.float32, 5)
+    leaves = [t.clone().requires_grad_() for t in (x, w, r)]
+    y, h = rms_norm(leaves[0], leaves[1], residual=leaves[2], eps=EPS)
+    got = torch.autograd.grad((y, h), leaves, (dy, dh))
+
+    def f(x, w, r):
+        y, h = rms_norm(x, w, residual=r, eps=EPS)
+        return float((y.double() * dy.double()).sum() + (h.double() * dh.double()).sum())
+
+    e = 2.0 ** -6
+    for i in range(3):
+        v = rows((x, w, r)[i].shape, torch.float32, 10 + i)
+        up, dn = [x, w, r], [x, w, r]
+        up[i], dn[i] = up[i] + e * v, dn[i] - e * v
+        num = (f(*up) - f(*dn)) / (2 * e)
+        ana = float((got[i].double() * v.double()).sum())
+        assert abs(num - ana) <= 0.01 * float((got[i].double().abs() * v.double().abs()).sum() / 8 + abs(ana))
+
+
+@gpu
+def test_backward_parts():
+    """One of the two outputs used alone, gradients asked for singly, no weight."""
+    x, r = rows((40, 96), torch.bfloat16, 1).requires_grad_(), rows((40, 96), torch.bfloat16, 2).requires_grad_()
+    w = rows((96,), torch.bfloat16, 3).requires_grad_()
+    g = rows((40, 96), torch.bfloat16, 4)
+    y, h = rms_norm(x, w, residual=r)
+    full = torch.autograd.grad((y, h), (x, w, r), (g, torch.zeros_like(g)), retain_graph=True)
+    only_y = torch.autograd.grad(y, (x, w, r), g, retain_graph=True)
+    for a, b in zip(full, only_y):
+        assert torch.equal(a, b)
+    for i, leaf in enumerate((x, w, r)):
+        assert torch.equal(torch.autograd.grad(y, leaf, g, retain_graph=True)[0], full[i])
+    dx, dr = torch.autograd.grad(h, (x, r), g, retain_graph=True)
+    assert torch.equal(dx, g) and torch.equal(dr, g)
+    x2 = x.detach().float().requires_grad_()
+    y2, h2 = rms_norm(x2, residual=r.detach().float())
+    d, mag, _, _ = grads(h2.detach(), None, g.float(), None, torch.float32, torch.float32)
+    (dx2,) = torch.autograd.grad(y2, x2, g.float())
+    assert ((dx2.double() - d).abs() <= 2 * F32 * mag).all()
+    # leaves accumulate: two uses of one weight
+    w2 = w.detach().clone().requires_grad_()
+    (rms_norm(x.detach(), w2) + rms_norm(r.detach(), w2)).backward(g)
+    assert w2.grad.shape == (96,)
+
+
+@gpu
+def test_deterministic_and_empty():
+    x, w = rows((3000, 1024), torch.bfloat16, 1).requires_grad_(), rows((1024,), torch.float32, 2).requires_grad_()
+    g = rows((3000, 1024), torch.bfloat16, 3)
+    a = torch.autograd.grad(rms_norm(x, w), (x, w), g)
+    b = torch.autograd.grad(rms_norm(x, w), (x, w), g)
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+    e = torch.empty(0, 1024, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    y, h = rms_norm(e, w, residual=e.detach())
+    assert y.shape == h.shape == (0, 1024)
+    dx, dw = torch.autograd.grad(y, (e, w), torch.empty_like(y))
+    assert dx.shape == (0, 1024) and float(dw.abs().max()) == 0.0
+    q, s = rms_norm_quant(e.detach(), w.detach())
+    assert q.shape == (0, 1024) and s.shape == (0, 1)
+
+
+@gpu
+@pytest.mark.parametrize("x_t", [torch.float16, torch.float32])
+def test_strides_and_alignment(x_t):
+    """Rows inside a wider tensor, every start within a 16-byte line, transposed and 3-d inputs."""
+    base = rows((64, 700), x_t, 1)
+    w = rows((512,), torch.float32, 2)
+    for at in (0, 1, 3, 8):
+        x = base[:, at:at + 512]
+        y, h = rms_norm(x, w[:512], residual=base[:, 150:662])
+        assert torch.equal(h, (x.float() + base[:, 150:662].float()).to(x_t))
+        check_y(y, ref_norm(h, w)[0])
+        q, s = rms_norm_quant(x, w, group=64)
+        q2, s2 = rms_norm_quant(x.contiguous(), w, group=64)
+        # rows off 16 bytes are read one element at a time, so the two sums of squares run in other orders; each y is
+        # within F32 of the exact value: scales within 2 F32 of one another, each code nearest to its own y / s
+        assert ((s - s2).abs() <= 2 * F32 * s2).all()
+        y, _ = ref_norm(x, w)
+        for codes, scales in ((q, s), (q2, s2)):
+            check_codes(codes, scales.double().repeat_interleave(64, 1), y, torch.int8)
+    t = base.t()[:, :33]
+    check_y(rms_norm(t), ref_norm(t, None)[0])
+    b3 = base[:, :512].reshape(8, 8, 512).transpose(0, 1)
+    check_y(rms_norm(b3, w), ref_norm(b3, w)[0])
+    one = base[0, :512]
+    check_y(rms_norm(one, w), ref_norm(one, w)[0])
+    ws = torch.stack((w, w), dim=1)[:, 0]
+    assert torch.equal(rms_norm(one, ws), rms_norm(one, w))
+    xg = base[:, 1:513].detach().requires_grad_()
+    dy = base[:, 100:612]
+    (dx,) = torch.autograd.grad(rms_norm(xg, w), xg, dy)
+    d, mag, _, _ = grads(xg.detach(), w, dy, None, x_t, x_t)
+    assert ((dx.double() - d).abs() <= half_step(x_t) * d.abs() + 2 * F32 * mag + tiny(x_t)).all()
+
+
+QMAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def check_codes(q, s_cols, y, out):
+    """Each code is a nearest one to y / s: within half a step plus the fp32 error of y / s."""
+    t = y / s_cols
+    Q = QMAX[out]
+    t = t.clamp(-Q, Q)
+    d = (q.double() - t).abs()
+    if out == torch.int8:
+        assert (d <= 0.5 + 2 * F32 * Q).all()
+    else:
+        assert (d <= (2.0 ** -4 + 2 * F32) * t.abs() + 2.0 ** -10).all()
+
+
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("x_t,r_t", PAIRS)
+@pytest.mark.parametrize("shape", SIZES)
+def test_quant(shape, x_t, r_t, out):
+    x, r, w = rows(shape, x_t, 1), rows(shape, r_t, 2, 5.0), rows(shape[1:], torch.float32, 3)
+    R, C = shape
+    for group in (0, 32, 64, 128):
+        q, s, h = rms_norm_quant(x, w, residual=r, eps=EPS, out_dtype=out, group=group)
+        assert q.dtype == out and torch.equal(h, (x.float() + r.float()).to(r_t))
+        y, _ = ref_norm(h, w)
+        width = group or C
+        G = -(-C // width)
+        assert s.shape == (R, G)
+        pad = torch.zeros(R, G * width, dtype=torch.float64, device="cuda")
+        pad[:, :C] = y.abs()
+        ref = pad.view(R, G, width).amax(-1) / QMAX[out]
+        ref = torch.where(ref > 0, ref, torch.ones_like(ref))
+        assert ((s.double() - ref).abs() <= 2 * F32 * ref).all()
+        check_codes(q, s.double().repeat_interleave(width, 1)[:, :C], y, out)
+    given = torch.tensor(3.0 / QMAX[out], device="cuda")
+    q, s = rms_norm_quant(x, w, eps=EPS, out_dtype=out, scale=given)
+    assert s is given
+    check_codes(q, given.double(), ref_norm(x, w)[0], out)
+
+
+@gpu
+def test_quant_zero_and_nonfinite_rows():
+    x = rows((6, 256), torch.float32, 1)
+    x[0] = 0
+    x[1, :64] = 0
+    x[2, 5] = float("nan")
+    x[3, 7] = float("inf")
+    x[4] = 3e38                      # the sum of squares overflows: y is 0
+    for out in QMAX:
+        q, s = rms_norm_quant(x, out_dtype=out)
+        assert float(s[0]) == 1.0 and not q[0].float().any()
+        assert bool(torch.isnan(s[2])) and bool(torch.isnan(s[3]))
+        assert float(s[4]) == 1.0 and not q[4].float().any()
+        assert torch.isfinite(s[[1, 5]]).all() and float(q[5].float().abs().max()) == QMAX[out]
+        q, s = rms_norm_quant(x, out_dtype=out, group=64)
+        assert float(s[1, 0]) == 1.0 and not q[1, :64].float().any() and bool(torch.isnan(s[2]).all())
+    tiny_rows = torch.full((2, 64), 1e-38, device="cuda")
+    q, s = rms_norm_quant(tiny_rows, eps=1.0)          # a scale below the smallest normal number
+    assert torch.isfinite(s).all() and (q.abs() >= 120).all()
+
+
+@gpu
+def test_streams_graph_and_64_bit_offsets():
+    x, w = rows((50, 1000), torch.float16, 1), rows((1000,), torch.float16, 2)
+    want = rms_norm(x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = rms_norm(x, w)
+    s.synchronize()
+    assert torch.equal(got, want)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dy = rows((50, 1000), torch.float16, 3)
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            torch.autograd.grad(rms_norm(xs, ws), (xs, ws), dy)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = rms_norm(xs, ws)
+        dx, dw = torch.autograd.grad(y, (xs, ws), dy)
+        q, sc, h = rms_norm_quant(xs.detach(), ws.detach(), residual=dy)
+    with torch.no_grad():
+        xs.copy_(rows((50, 1000), torch.float16, 9))
+    g.replay()
+    torch.cuda.synchronize()
+    y = y.detach()
+    assert torch.equal(y, rms_norm(xs.detach(), ws.detach()))
+    x2, w2 = xs.detach().clone().requires_grad_(), ws.detach().clone().requires_grad_()
+    dx2, dw2 = torch.autograd.grad(rms_norm(x2, w2), (x2, w2), dy)
+    assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
+    for a, b in zip((q, sc, h), rms_norm_quant(xs.detach(), ws.detach(), residual=dy)):
+        assert torch.equal(a, b)
+    # rows past 2^31 elements
+    big = torch.zeros(70000, 32768, dtype=torch.bfloat16, device="cuda")
+    big[-1] = rows((32768,), torch.bfloat16, 4)
+    y = rms_norm(big)
+    check_y(y[-1], ref_norm(big[-1], None)[0])
+    q, s = rms_norm_quant(big, group=128)
+    q1, s1 = rms_norm_quant(big[-1:].clone(), group=128)
+    assert torch.equal(q[-1:], q1) and torch.equal(s[-1:], s1)
+
+
+@gpu
+def test_module():
+    src = torch.nn.RMSNorm(320, eps=1e-5, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        src.weight.copy_(rows((320,), torch.bfloat16, 1))
+    m = RMSNorm.from_torch(src)
+    assert m.weight is src.weight
+    x = rows((9, 320), torch.bfloat16, 2)
+    check_y(m(x).detach(), ref_norm(x, src.weight.detach(), 1e-5)[0])
+    with torch.no_grad():
+        q, s = m.quant(x, out_dtype=torch.float8_e4m3fn, group=64)
+    assert q.shape == x.shape and s.shape == (9, 5)
+
+
+# -- refusals (no GPU) -----------------------------------------------------------------------------
+
+
+def test_refusals():
+    x = torch.zeros(4, 64)
+    for bad, kw in ((TypeError, dict(x=x.to(torch.float64))), (TypeError, dict(x=x.to(torch.int8))),
+                    (ValueError, dict(x=torch.zeros(4, 0))), (ValueError, dict(x=torch.zeros(1, MAX_COLS + 1))),
+                    (ValueError, dict(x=torch.tensor(1.0))),
+                    (ValueError, dict(x=x, weight=torch.zeros(63))), (ValueError, dict(x=x, weight=torch.zeros(4, 64))),
+                    (TypeError, dict(x=x, weight=torch.zeros(64, dtype=torch.float16))),
+                    (ValueError, dict(x=x, residual=torch.zeros(64))),
+                    (ValueError, dict(x=x, residual=torch.zeros(1, 64))),
+                    (TypeError, dict(x=x, residual=x.half())),
+                    (TypeError, dict(x=x.half(), residual=x.bfloat16())),
+                    (ValueError, dict(x=x, eps=-1.0)), (ValueError, dict(x=x, eps=float("nan"))),
+                    (ValueError, dict(x=x, residual=x.to("meta"))), (RuntimeError, dict(x=x))):
+        with pytest.raises(bad):
+            rms_norm(**kw)
+        with pytest.raises(bad):
+            rms_norm_quant(**kw)
+    with pytest.raises(TypeError):
+        rms_norm_quant(x, out_dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        rms_norm_quant(x, group=16)
+    with pytest.raises(ValueError):
+        rms_norm_quant(x, group=64, scale=torch.tensor(1.0))
+    with pytest.raises(ValueError):
+        rms_norm_quant(x, scale=torch.ones(2))
+    with pytest.raises(ValueError):
+        rms_norm_quant(x, scale=torch.ones(1, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rms_norm_quant(x.clone().requires_grad_())
+    with pytest.raises(ValueError):
+        RMSNorm.from_torch(torch.nn.RMSNorm((4, 8), eps=1e-6))
+    with pytest.raises(ValueError):
+        RMSNorm.from_torch(torch.nn.RMSNorm(8, elementwise_affine=False))
+
+
+def test_abi_refusals():
+    lib = N.load()
+    a = np.zeros(4096, np.float32).ctypes.data // 16 * 16 + 16          # an address that no call may reach
+
+    def fwd(x=a, xt=N.DTYPE_F16, ld=64, r=None, rt=0, ldr=64, w=None, wt=0, rows=2, cols=64, eps=1e-6, y=a, h=None):
+        return lib.glad_rms_norm_forward(x, xt, ld, r, rt, ldr, w, wt, rows, cols, eps, y, h, None, None)
+
+    bad = N.GLAD_ERR_INVALID_ARG
+    assert fwd(rows=0) == N.GLAD_OK
+    for kw in (dict(x=None), dict(y=None), dict(xt=N.DTYPE_I8), dict(xt=77), dict(ld=63), dict(cols=0), dict(cols=32769),
+               dict(rows=-1), dict(rows=1 << 31), dict(eps=-1.0), dict(eps=float("nan")), dict(x=a + 1), dict(y=a + 1),
+               dict(w=a, wt=N.DTYPE_BF16), dict(w=a + 1, wt=N.DTYPE_F16), dict(r=a, rt=N.DTYPE_F16),
+               dict(h=a), dict(r=a, rt=N.DTYPE_BF16, h=a), dict(r=a, rt=N.DTYPE_F16, h=a, ldr=8),
+               dict(r=a, rt=N.DTYPE_F32, h=a + 2)):
+        assert fwd(**kw) == bad, kw
+        assert lib.glad_last_error()
+
+    def qnt(qt=N.DTYPE_I8, group=0, given=None, q=a, s=a, rows=2):
+        return lib.glad_rms_norm_quant(a, N.DTYPE_F16, 64, None, 0, 0, None, 0, rows, 64, 1e-6, qt, group, given, q, s,
+                                       None, None)
+
+    assert qnt(rows=0) == N.GLAD_OK
+    for kw in (dict(qt=N.DTYPE_F16), dict(group=1), dict(group=256), dict(given=a, group=64), dict(s=None), dict(q=None),
+               dict(s=a + 2), dict(given=a + 1)):
+        assert qnt(**kw) == bad, kw
+
+    def bwd(dy=a, ds=None, h=a, ht=N.DTYPE_F16, w=a, rstd=a, dx=a, dr=None, dw=None, ws=None, n=0, rows=2, ld=64):
+        return lib.glad_rms_norm_backward(dy, N.DTYPE_F16, ld, ds, ht, 64, h, 64, w, N.DTYPE_F16, rstd, rows, 64, dx, dr,
+                                          dw, ws, n, None)
+
+    need = lib.glad_rms_norm_backward_workspace_size(2, 64)
+    assert need >= 8 * 64 * 4 and lib.glad_rms_norm_backward_workspace_size(0, 64) == 0
+    assert lib.glad_rms_norm_backward_workspace_size(1 << 30, 64) < 1 << 20
+    for kw in (dict(dy=None), dict(h=None), dict(rstd=None), dict(dx=None), dict(ht=N.DTYPE_BF16), dict(dw=a, w=None),
+               dict(ld=8), dict(dx=a + 1), dict(rows=-1)):
+        assert bwd(**kw) == bad, kw
+    assert bwd(dw=a, ws=None) == bwd(dw=a, ws=a, n=need - 1) == bwd(dw=a, ws=a + 8, n=need) == N.GLAD_ERR_WORKSPACE

@@ -1,0 +1,423 @@
+"""w4_linear / W4Linear against the definition in 64 bits.
+
+Tolerance, fixed before the first run: the products x * q are exact; a tensor-core sum keeps at least 24 bits of its
+largest term, so each of at most K/16 steps, 64 joins and scale products is off by at most 2^-23 of the sum of
+magnitudes S = sum |x q| s xs seen so far, in all (K/16 + 64) * 2^-23 * S; the result is rounded once (half a step)."""
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+from rl_quant_b200 import _native as N
+from rl_quant_b200 import swap
+from rl_quant_b200.norm import RMSNorm, rms_norm_quant
+from rl_quant_b200.w4a16 import quantize_w4
+from rl_quant_b200.w4linear import W4Linear, W4Weight, pack_w4, unpack_w4, w4_linear
+
+gpu = pytest.mark.gpu
+F16, BF16, I8, E4M3 = torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn
+
+
+def weight(n, k, group, seed, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-8, 8, (n, k), generator=g).to(torch.int8)
+    packed = ((q[:, 0::2] & 15) | ((q[:, 1::2] & 15) << 4)).view(torch.uint8)
+    s = ((0.5 + torch.rand(n, -(-k // group), generator=g)) * 0.02).half()
+    return q.to(device), packed.to(device), s.to(device)
+
+
+def rows(m, k, t, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g)
+    if t == I8:
+        return (x * 40).round().clamp(-128, 127).to(I8).cuda()
+    if t == E4M3:
+        return (x * 90).clamp(-448, 448).to(E4M3).cuda()
+    return x.to(t).cuda()
+
+
+def check(y, x, q, s, group, bias=None, xs=None):
+    k = q.shape[1]
+    col = torch.arange(k, device=q.device) // group
+    W = q.double() * s.double()[:, col]
+    xd = x.double()
+    if xs is not None:
+        xd = xd * (xs.double()[:, col] if xs.dim() == 2 and xs.shape[1] > 1 else xs.double())
+    ref, S = xd @ W.T, xd.abs() @ W.abs().T
+    if bias is not None:
+        ref, S = ref + bias.double(), S + bias.double().abs()
+    step = 0.0 if y.dtype == torch.float32 else torch.finfo(y.dtype).eps / 2
+    tol = step * ref.abs() + (k / 16 + 64) * 2.0 ** -23 * S * (1 + step) + torch.finfo(y.dtype).smallest_normal * step
+    assert torch.isfinite(y).all()
+    assert ((y.double() - ref).abs() <= tol).all(), float(((y.double() - ref).abs() / tol.clamp_min(1e-30)).max())
+
+
+# rows from one to several tiles of every kind, sizes off every tile
+M_SIZES = [1, 2, 7, 8, 9, 16, 17, 31, 33, 64, 65, 100, 129, 200, 300, 1000]
+SHAPES = [(16, 64), (1, 2), (29, 128), (777, 1002), (512, 224), (130, 4096), (4096, 320), (17, 16384)]
+
+
+@gpu
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_16_bit_rows(n, k, group):
+    q, packed, s = weight(n, k, group, n + k)
+    w = pack_w4(packed, s, group)
+    for i, m in enumerate(M_SIZES):
+        t = (F16, BF16)[i % 2]
+        x = rows(m, k, t, m)
+        bias = rows(1, n, t, 7)[0] if i % 3 else None
+        y = w4_linear(x, w, bias)
+        assert y.dtype == t and y.shape == (m, n)
+        check(y, x, q, s, group, bias)
+    for t in (F16, BF16):
+        for m in (1, 20, 150):
+            x = rows(m, k, t, m)
+            for out in (F16, BF16, torch.float32):
+                check(w4_linear(x, w, out_dtype=out), x, q, s, group)
+
+
+@gpu
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("t", [I8, E4M3])
+def test_8_bit_rows(n, k, group, t):
+    q, packed, s = weight(n, k, group, n + k)
+    w = pack_w4(packed, s, group)
+    G = -(-k // group)
+    for i, m in enumerate(M_SIZES):
+        x = rows(m, k, t, m)
+        for j, xs in enumerate((torch.tensor(0.01, device="cuda"), 0.01 * (0.5 + torch.rand(m, 1, device="cuda")),
+                                0.01 * (0.5 + torch.rand(m, G, device="cuda")))):
+            out = (F16, BF16, torch.float32)[(i + j) % 3]
+            bias = rows(1, n, out, 7)[0] if (i + j) % 2 else None
+            check(w4_linear(x, w, bias, x_scale=xs, out_dtype=out), x, q, s, group, bias, xs)
+
+
+@gpu
+def test_every_code_and_extremes():
+    """Every weight code at every place of a word; the largest magnitudes of each input type; signed zeros."""
+    k, group = 256, 64
+    for v in range(-8, 8):
+        q = torch.full((16, k), v, dtype=torch.int8)
+        q[torch.arange(16), torch.arange(16) * 16 + 3] = -8
+        packed = ((q[:, 0::2] & 15) | ((q[:, 1::2] & 15) << 4)).view(torch.uint8).cuda()
+        s = torch.full((16, 4), 0.125, dtype=F16, device="cuda")
+        w = pack_w4(packed, s, group)
+        for m in (3, 40):
+            x = rows(m, k, F16, v + 50)
+            check(w4_linear(x, w), x, q.cuda(), s, group)
+            x8 = rows(m, k, I8, v + 90)
+            x8[0] = -128
+            x8[1] = 127
+            one = torch.tensor(1.0, device="cuda")
+            check(w4_linear(x8, w, x_scale=one, out_dtype=torch.float32), x8, q.cuda(), s, group, None, one)
+            xe = rows(m, k, E4M3, v)
+            xe[0] = torch.full((k,), 448.0, device="cuda").to(E4M3)
+            xe[1] = torch.full((k,), 2.0 ** -9, device="cuda").to(E4M3)
+            check(w4_linear(xe, w, x_scale=one, out_dtype=torch.float32), xe, q.cuda(), s, group, None, one)
+
+
+@gpu
+def test_identity_rows_pick_weights():
+    """A unit row picks one column of the weight exactly, for every column: the layout end to end."""
+    n, k, group = 40, 192, 32
+    q, packed, s = weight(n, k, group, 5)
+    w = pack_w4(packed, s, group)
+    W = (q.float() * s.float()[:, torch.arange(k, device="cuda") // group])
+    for t in (F16, BF16):
+        assert torch.equal(w4_linear(torch.eye(k, device="cuda").to(t), w, out_dtype=torch.float32), W.T)
+    one = torch.tensor(1.0, device="cuda")
+    for t in (I8, E4M3):
+        x = torch.eye(k, device="cuda").to(t)
+        for lo, hi in ((0, k), (3, 4), (5, 18)):
+            assert torch.equal(w4_linear(x[lo:hi], w, x_scale=one, out_dtype=torch.float32), W.T[lo:hi])
+
+
+@gpu
+def test_nonfinite_rows_stay_apart():
+    """A row with NaN or infinities spoils its own outputs only; zero scales give zeros."""
+    q, packed, s = weight(48, 320, 64, 1)
+    w = pack_w4(packed, s, 64)
+    for m in (4, 12, 90, 260):
+        x = rows(m, 320, F16, m)
+        clean = w4_linear(x, w)
+        x[1, 17] = float("nan")
+        x[2, 300] = float("inf")
+        y = w4_linear(x, w)
+        keep = [i for i in range(m) if i not in (1, 2)]
+        assert torch.equal(y[keep], clean[keep])
+        assert torch.isnan(y[1]).all() and not torch.isfinite(y[2][q[:, 300] != 0]).any()
+    w0 = pack_w4(packed, torch.zeros_like(s), 64)
+    assert not w4_linear(rows(5, 320, BF16, 1), w0).any()
+
+
+@gpu
+@pytest.mark.parametrize("t", [F16, I8])
+def test_strides_alignment_and_shapes(t):
+    q, packed, s = weight(100, 192, 64, 1)
+    w = pack_w4(packed, s, 64)
+    base = rows(70, 500, t, 2)
+    xs = torch.rand(70, 1, device="cuda") if t == I8 else None
+    kw = dict(x_scale=xs, out_dtype=F16) if t == I8 else {}
+    for at in (0, 1, 2, 8, 16):
+        for m in (1, 5, 70):
+            k2 = dict(kw, x_scale=xs[:m]) if xs is not None else kw
+            x = base[:m, at:at + 192]
+            assert torch.equal(w4_linear(x, w, **k2), w4_linear(x.contiguous(), w, **k2))
+    x = base[:, :192].t().contiguous().t()
+    assert torch.equal(w4_linear(x, w, **kw), w4_linear(x.contiguous(), w, **kw))
+    x3 = base[:, :192].reshape(7, 10, 192)
+    k3 = dict(kw, x_scale=xs.view(7, 10, 1)) if xs is not None else kw
+    assert torch.equal(w4_linear(x3, w, **k3).view(70, 100), w4_linear(base[:, :192], w, **kw))
+    k1 = dict(kw, x_scale=xs[0]) if xs is not None else kw
+    assert w4_linear(base[0, :192], w, **k1).shape == (100,)
+    k0 = dict(kw, x_scale=xs[:0]) if xs is not None else kw
+    assert w4_linear(base[:0, :192], w, **k0).shape == (0, 100)
+    if xs is not None:
+        g = torch.rand(70, 6, device="cuda")[:, ::2]
+        assert torch.equal(w4_linear(base[:, :192], w, x_scale=g, out_dtype=F16),
+                           w4_linear(base[:, :192], w, x_scale=g.contiguous(), out_dtype=F16))
+
+
+@gpu
+def test_streams_graph_repeat():
+    q, packed, s = weight(512, 2048, 128, 1)
+    w = pack_w4(packed, s, 128)
+    for m in (1, 24, 200):
+        x = rows(m, 2048, BF16, 2)
+        want = w4_linear(x, w)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = [w4_linear(x, w) for _ in range(3)]
+        main = [w4_linear(x, w) for _ in range(3)]        # at the same time on two streams
+        side.synchronize()
+        assert all(torch.equal(y, want) for y in got + main)
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                y = w4_linear(x, w)
+            graphs.append((g, y))
+        x.copy_(rows(m, 2048, BF16, 3))
+        for g, _ in graphs:
+            g.replay()
+        want = w4_linear(x, w)
+        assert all(torch.equal(y, want) for _, y in graphs)
+
+
+@gpu
+def test_64_bit_offsets():
+    """An output past 2^31 elements and rows past 2^31 elements apart."""
+    q, packed, s = weight(16384, 64, 32, 1)
+    w = pack_w4(packed, s, 32)
+    x = rows(140000, 64, F16, 1)
+    y = w4_linear(x, w)
+    check(y[-100:], x[-100:], q, s, 32)
+    big = torch.zeros(3, 1 << 30, dtype=F16, device="cuda")
+    big[:, :64] = rows(3, 64, F16, 2)
+    check(w4_linear(big[:, :64], w), big[:, :64], q, s, 32)
+    del y, big
+
+
+class Block(nn.Module):
+    """Residual block of two linears behind a norm, as a policy's trunk has it."""
+
+    def __init__(self, d, f):
+        super().__init__()
+        self.norm, self.up, self.down = nn.RMSNorm(d, eps=1e-6), nn.Linear(d, f), nn.Linear(f, d)
+
+    def forward(self, x, res):
+        y, h = self.norm(x, res)
+        return self.down(torch.nn.functional.elu(self.up(y))), h
+
+
+def block(seed=0):
+    torch.manual_seed(seed)
+    return Block(256, 640).cuda().half()
+
+
+@gpu
+def test_block_serves_and_trains():
+    """The operators together: swapped block at inference (16-bit and int8 rows) and in training, refreshed in place."""
+    b = block()
+    params = {n: p for n, p in b.named_parameters()}
+    swapped = swap.apply(b, {"up": {"bits": 4, "group": 32}, "down": {"bits": 4}})
+    norms = swap.apply_norm(b)
+    assert isinstance(b.up, W4Linear) and b.up.group == 32 and b.down.group == 64 and isinstance(b.norm, RMSNorm)
+    assert all(params[n] is p for n, p in b.named_parameters())
+    x, res = rows(5, 256, F16, 1), rows(5, 256, F16, 2)
+    with torch.no_grad():
+        y, h = b(x, res)
+        n16 = b.norm(x, res)[0]
+        up = w4_linear(n16, b.up.w4(), b.up.bias)
+        assert torch.equal(y, w4_linear(torch.nn.functional.elu(up), b.down.w4(), b.down.bias))
+        # the int8 form: the product of the codes is the product of the values they stand for
+        q, s, h2 = b.norm.quant(x, res, group=32)
+        assert torch.equal(h, h2)
+        packed, sc = quantize_w4(b.up.weight, 32)
+        codes = torch.stack((packed & 15, packed >> 4), -1).view(640, 256).to(torch.int8)
+        codes = torch.where(codes > 7, codes - 16, codes)
+        got = b.up(q, x_scale=s)
+        assert got.dtype == F16
+        check(got, q, codes, sc, 32, b.up.bias, s)
+        # ... and near the 16-bit form: a code is off by half a step of s at most
+        step = s.float().amax() / 2
+        W = (codes.float() * sc.float()[:, torch.arange(256, device="cuda") // 32]).abs().sum(1)
+        assert ((got.float() - up.float()).abs() <= step * W + 2.0 ** -9 * up.float().abs() + 0.02).all()
+        ptr, before = b.up.tiles.data_ptr(), y.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            yg, _ = b(x, res)
+        b.up.weight.mul_(0.5)
+        b.up.requantize_()
+        g.replay()
+        assert b.up.tiles.data_ptr() == ptr
+        assert torch.equal(yg, b(x, res)[0]) and not torch.equal(yg, before)
+    # training: the plain layers' gradients
+    ref = block()
+    with torch.no_grad():
+        ref.up.weight.mul_(0.5)
+    out, h = b(x, res)
+    out.float().square().sum().backward()
+    yr, hr = ref.norm(x + res), x + res
+    ref.down(torch.nn.functional.elu(ref.up(yr))).float().square().sum().backward()
+    for (n, p), (_, r) in zip(b.named_parameters(), ref.named_parameters()):
+        d = (p.grad.float() - r.grad.float()).norm() / r.grad.float().norm()
+        assert d <= 2.0 ** -8, (n, float(d))       # fp16 gradients of fp16 activations, each rounded to 2^-11
+    swap.restore(b, swapped)
+    swap.restore_norm(b, norms)
+    assert type(b.up) is nn.Linear and type(b.norm) is nn.RMSNorm and all(params[n] is p for n, p in b.named_parameters())
+
+
+@gpu
+def test_runner_refreshes_w4_layers():
+    """InferenceRunner's weight hand-over reaches W4Linear layers (refresh_quant, eager and graphed)."""
+    from rl_quant_b200 import InferenceRunner
+
+    class Policy(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.actor = nn.Sequential(nn.Linear(64, 96), nn.ELU(), nn.Linear(96, 8))
+
+    p = Policy().cuda().half()
+    swap.apply(p, {"actor.0": {"bits": 4}})
+    run = InferenceRunner.__new__(InferenceRunner)
+    run.model, run._g_refresh = p, None
+    run._quant_layers = [m for m in p.modules() if m is not p and hasattr(m, "requantize_")]
+    for graph in (False, True, True):
+        with torch.no_grad():
+            p.actor[0].weight.normal_()
+        run.refresh_quant(use_graph=graph)
+        want = pack_w4(*quantize_w4(p.actor[0].weight, 64), 64)
+        assert torch.equal(p.actor[0].tiles, want.tiles) and torch.equal(p.actor[0].scales, want.scales)
+
+
+# -- no GPU ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 2, 32), (16, 64, 64), (29, 130, 128), (40, 192, 32), (33, 100, 64)])
+def test_layout(n, k, group):
+    """tiles and scales as include/glad_b200.h words them, element by element; the round trip."""
+    q, packed, s = weight(n, k, group, 3, "cpu")
+    w = pack_w4(packed, s, group)
+    lib = N.load()
+    assert w.tiles.numel() == lib.glad_w4_tiles_bytes(k, n, group)
+    assert w.scales.numel() * 2 == lib.glad_w4_scales_bytes(k, n, group)
+    words = w.tiles.numpy().reshape(w.tiles.shape[0], w.tiles.shape[1], 128, 4).view(np.uint32).reshape(
+        w.tiles.shape[0], w.tiles.shape[1], 32, 4)
+    seen = np.zeros((w.tiles.shape[0] * 16, w.tiles.shape[1] * 64), np.int64)
+    for t in range(words.shape[0]):
+        for kb in range(words.shape[1]):
+            for lane in range(32):
+                r, c = lane >> 2, lane & 3
+                for j in range(4):
+                    for i in range(8):
+                        row = 16 * t + r + 8 * (i & 1)
+                        col = 64 * kb + 32 * (j >> 1) + 8 * c + 4 * (j & 1) + 2 * ((i >> 1) & 1) + (i >> 2)
+                        v = (int(words[t, kb, lane, j]) >> (4 * i)) & 15
+                        seen[row, col] = v - 16 if v > 7 else v
+    assert np.array_equal(seen[:n, :k], q.numpy()) and not seen[n:].any() and not seen[:, k:].any()
+    g = s.shape[1]
+    flat = w.scales.permute(0, 2, 1).reshape(-1, w.scales.shape[1])
+    assert torch.equal(flat[:n, :g], s) and not flat[n:].any() and not flat[:, g:].any()
+    p2, s2 = unpack_w4(w)
+    assert torch.equal(p2, packed) and torch.equal(s2, s)
+
+
+def test_refusals():
+    q, packed, s = weight(24, 128, 64, 1, "cpu")
+    w = pack_w4(packed, s, 64)
+    x = torch.zeros(3, 128, dtype=F16)
+    x8 = x.to(I8)
+    one, row, grp = torch.ones(()), torch.ones(3, 1), torch.ones(3, 2)
+    for bad, args, kw in (
+            (ValueError, (x[:, :126], w), {}), (TypeError, (x.float(), w), {}), (TypeError, (x.to(torch.uint8), w), {}),
+            (ValueError, (torch.tensor(1.0), w), {}), (TypeError, (x, w), dict(out_dtype=torch.float64)),
+            (ValueError, (x, w), dict(x_scale=one)), (ValueError, (x8, w), dict(out_dtype=F16)),
+            (ValueError, (x8, w), dict(x_scale=row)), (TypeError, (x8, w), dict(x_scale=row.half(), out_dtype=F16)),
+            (ValueError, (x8, w), dict(x_scale=torch.ones(3), out_dtype=F16)),
+            (ValueError, (x8, w), dict(x_scale=torch.ones(3, 3), out_dtype=F16)),
+            (ValueError, (x8, w), dict(x_scale=torch.ones(1, 2), out_dtype=F16)),
+            (ValueError, (x, w, torch.zeros(23, dtype=F16)), {}), (ValueError, (x, w, torch.zeros(24)), {}),
+            (ValueError, (x.to("meta"), w), {}), (RuntimeError, (x, w), {}),
+            (RuntimeError, (x8, w), dict(x_scale=grp, out_dtype=F16)),
+            (RuntimeError, (x.clone().requires_grad_(), w), {})):
+        with pytest.raises(bad):
+            w4_linear(*args, **kw)
+    for args in ((packed, s, 16), (packed.view(I8), s, 64), (packed, s.float(), 64), (packed, s[:, :1], 64),
+                 (packed, s, 32), (packed[:, :0], s[:, :0], 64), (packed[0], s, 64)):
+        with pytest.raises(ValueError):
+            pack_w4(*args)
+    for args in ((w.tiles, w.scales, 127, 24, 64), (w.tiles, w.scales, 128, 24, 48), (w.tiles, w.scales, 128, 33, 64),
+                 (w.tiles[:, :1], w.scales, 128, 24, 64), (w.tiles, w.scales.float(), 128, 24, 64)):
+        with pytest.raises(ValueError):
+            W4Weight(*args)
+    with pytest.raises(ValueError):
+        W4Linear(nn.Linear(7, 3))
+    with pytest.raises(ValueError):
+        W4Linear(nn.Linear(8, 3), group=8)
+    with pytest.raises(ValueError):
+        swap.apply(nn.Sequential(nn.Linear(8, 3)), {"0": {"bits": 3}})
+    with pytest.raises(ValueError):
+        swap.apply(nn.Sequential(nn.Linear(8, 3)), {"0": {"bits": 4, "s_z": 0.1}})
+
+
+def test_swap_and_restore_on_cpu():
+    m = nn.Sequential(nn.RMSNorm(64, eps=1e-6), nn.Linear(64, 40), nn.ELU(), nn.Linear(40, 3, bias=False)).eval()
+    params = list(m.parameters())
+    x = torch.randn(5, 64)
+    want = m(x)
+    sw = swap.apply(m, {"1": {"bits": 4}, "3": {"bits": 4, "group": 128}})
+    nm = swap.apply_norm(m, ["0"])
+    assert [type(l) for l in m] == [RMSNorm, W4Linear, nn.ELU, W4Linear] and not m[1].training
+    assert all(a is b for a, b in zip(params, m.parameters()))
+    p, s = unpack_w4(m[1].w4())
+    p2, s2 = quantize_w4(m[1].weight, 64)
+    assert torch.equal(p, p2) and torch.equal(s, s2)
+    swap.restore(m, sw)
+    swap.restore_norm(m, nm)
+    assert [type(l) for l in m] == [nn.RMSNorm, nn.Linear, nn.ELU, nn.Linear] and torch.equal(m(x), want)
+    assert all(a is b for a, b in zip(params, m.parameters())) and m[0].eps == 1e-6
+
+
+def test_abi_refusals():
+    lib = N.load()
+    a = np.zeros(8192, np.float32).ctypes.data // 16 * 16 + 16          # an address that no call may reach
+
+    def call(tiles=a, scales=a, k=128, n=24, group=64, x=a, t=N.DTYPE_F16, m=2, ld=128, xs=None, xr=0, xg=0, b=None, y=a,
+             yt=N.DTYPE_F16):
+        return lib.glad_w4_linear_forward(N.GladW4Weight(tiles, scales, k, n, group), x, t, m, ld, xs, xr, xg, b, y, yt,
+                                          None)
+
+    assert call(m=0) == N.GLAD_OK
+    for kw in (dict(tiles=None), dict(scales=None), dict(tiles=a + 8), dict(scales=a + 2), dict(k=127), dict(k=0),
+               dict(k=1 << 21), dict(n=0), dict(n=1 << 21), dict(group=16), dict(x=None), dict(y=None), dict(x=a + 1),
+               dict(y=a + 1), dict(b=a + 1), dict(t=N.DTYPE_F32), dict(t=9), dict(yt=N.DTYPE_I8), dict(m=-1),
+               dict(m=(1 << 20) + 1), dict(ld=64), dict(xs=a), dict(t=N.DTYPE_I8), dict(t=N.DTYPE_I8, xs=a + 2),
+               dict(t=N.DTYPE_I8, xs=a, xr=1, xg=3), dict(t=N.DTYPE_I8, xs=a, xr=0, xg=2),
+               dict(t=N.DTYPE_E4M3, xs=a, xr=2, xg=1)):
+        assert call(**kw) == N.GLAD_ERR_INVALID_ARG, kw
+        assert lib.glad_last_error()
+    assert lib.glad_w4_tiles_bytes(127, 8, 64) == 0 and lib.glad_w4_scales_bytes(128, 8, 48) == 0
