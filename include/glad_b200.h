@@ -427,12 +427,13 @@ int glad_rms_norm_backward(const void* dy, int x_dtype, int64_t lddy, const void
  * y[m, n] = sum_g xs[m, g] * scales[n, g] * sum_{k in group g} x[m, k] * q[n, k] + bias[n]
  * with q int4 in [-8, 7] and one f16 scale for `group` (32, 64 or 128)
  * consecutive inputs of a row. `tiles` and `scales` hold the weight in blocks:
- *   tiles  [ceil(N/16)][KB][32][4] u32, KB = ceil(K / b) * b / 64, b = max(64, group):
+ *   tiles  [ceil(N/16)][KB][32][4] u32, KB = 2 ceil(K / 128):
  *          word j of lane 4*r + c of block (t, kb) holds rows n = 16t + r and
  *          n + 8, inputs k = 64 kb + 32 (j >> 1) + 8 c + 4 (j & 1) + (0..3); nibble i
  *          (bits 4i..4i+3) is row n + 8 (i & 1), input k + 2 ((i >> 1) & 1) + (i >> 2);
  *          zero past N and K
- *   scales [ceil(N/16)][KB * 64 / group][16] f16, zero past N and K
+ *   scales [ceil(N/16)][KB * 64 / group][8][2] f16: rows 16t + r and 16t + r + 8 of a
+ *          group side by side; zero past N and K
  * x [M, K] (row stride ldx elements): f16 or bf16 with x_scale NULL; i8 or e4m3
  * with x_scale f32: one for all rows (x_scale_rows 0), one a row (x_scale_groups
  * 1) or one a row and group (x_scale_groups = ceil(K / group), rows contiguous).
@@ -448,6 +449,13 @@ size_t glad_w4_scales_bytes(int in_features, int out_features, int group);
 int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, int64_t M, int64_t ldx,
                            const float* x_scale, int x_scale_rows, int x_scale_groups, const void* bias, void* y,
                            int y_dtype, void* stream);
+
+/* Device-side status word of glad_w4_linear_forward on the current device: 0, or
+ * GLAD_DEVERR_* bits when a bounded wait inside a kernel ran out since the last
+ * call of this function, in which case that call's outputs are not valid; reads
+ * and clears it and returns GLAD_ERR_DEVICE when it was not 0. Synchronises
+ * `stream`.                                                                 */
+int glad_w4_linear_status(uint32_t* status, void* stream);
 
 /* ---- weight refresh (qrt/runtime.py:195-271) ------------------------------- */
 

@@ -5,7 +5,6 @@ sm_100 part, every entry point raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
@@ -162,6 +161,7 @@ SIGNATURES = {
     "glad_w4_scales_bytes": (c_size_t, [c_int, c_int, c_int]),
     "glad_w4_linear_forward": (c_int, [POINTER(GladW4Weight), c_void_p, c_int, c_int64, c_int64, c_void_p, c_int,
                                        c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "glad_w4_linear_status": (c_int, [POINTER(c_uint32), c_void_p]),
     "glad_requant_qlinear": (c_int, [POINTER(GladQLinearSrc), c_int, c_void_p]),
     "glad_requant_qcnn": (c_int, [POINTER(GladQCNNSrc), c_void_p]),
     "glad_cast_copy": (c_int, [POINTER(GladCastCopy), c_int, c_void_p]),
@@ -205,14 +205,17 @@ def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def device_guard(device: torch.device):
-    """Launches go to the tensors' device; a no-op when it is the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+# The current stream's handle by device index: what stream_handle returns without building a Stream object (0.1 us
+# instead of 2.2 us, a fifth of a small call's host time).
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or stream_handle
 
 
-_NO_GUARD = contextlib.nullcontext()
+def on_device(fn, index: int, *args) -> int:
+    """``fn(*args, current stream of device index)`` with that device current."""
+    if index == torch.cuda.current_device():
+        return fn(*args, raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, raw_stream(index))
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:

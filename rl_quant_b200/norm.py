@@ -16,30 +16,33 @@ import torch.nn as nn
 
 from . import _native as N
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_CODE = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 MAX_COLS = 32768
 
 
 def _check(x, weight, residual, eps):
-    if x.dtype not in _FLOATS:
-        raise TypeError(f"x is {x.dtype}; expected float32, float16 or bfloat16")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_COLS:
-        raise ValueError(f"x must have 1..{MAX_COLS} columns, got shape {tuple(x.shape)}")
+    dt, shape = x.dtype, x.shape
+    if dt not in _CODE:
+        raise TypeError(f"x is {dt}; expected float32, float16 or bfloat16")
+    if not shape or not 1 <= shape[-1] <= MAX_COLS:
+        raise ValueError(f"x must have 1..{MAX_COLS} columns, got shape {tuple(shape)}")
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0, got {eps}")
+    dev = x.device
     if weight is not None:
-        if weight.shape != x.shape[-1:]:
-            raise ValueError(f"weight {tuple(weight.shape)} does not match {x.shape[-1]} columns")
-        if weight.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"weight is {weight.dtype}; expected {x.dtype} or float32")
+        if weight.shape != shape[-1:]:
+            raise ValueError(f"weight {tuple(weight.shape)} does not match {shape[-1]} columns")
+        if weight.dtype != dt and weight.dtype != torch.float32:
+            raise TypeError(f"weight is {weight.dtype}; expected {dt} or float32")
+        if weight.device != dev:
+            raise ValueError(f"tensors on {dev} and {weight.device}")
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"residual is {residual.dtype}; expected {x.dtype} or float32")
-    for t in (weight, residual):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"tensors on {x.device} and {t.device}")
+        if residual.shape != shape:
+            raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(shape)}")
+        if residual.dtype != dt and residual.dtype != torch.float32:
+            raise TypeError(f"residual is {residual.dtype}; expected {dt} or float32")
+        if residual.device != dev:
+            raise ValueError(f"tensors on {dev} and {residual.device}")
     N.require_cuda(x)
 
 
@@ -49,63 +52,83 @@ def _rows(t):
     return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
 
 
-def _forward(x, weight, residual, eps, rstd):
-    """(y, h or None) as rows; ``rstd`` None or f32 [rows] to fill."""
+def _like(t, dtype=None):
+    """Contiguous and uninitialised, of t's shape (empty_like is the cheaper call)."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
+def _inputs(x, weight, residual):
+    """The first arguments of both forward entry points, the tensors they point into and the sum's buffer."""
     x2 = _rows(x)
     rows, cols = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    r2 = h = None
+    wp, wt, rp, rt, ldr, h, r2 = None, 0, None, 0, 0, None, None
+    if weight is not None:
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        wp, wt = weight.data_ptr(), _CODE[weight.dtype]
     if residual is not None:
         r2 = _rows(residual)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    with N.device_guard(x.device):
-        N.check(N.load().glad_rms_norm_forward(
-            x2.data_ptr(), N.DTYPES[x.dtype], x2.stride(0), N.ptr(r2), N.DTYPES[h.dtype] if h is not None else 0,
-            r2.stride(0) if r2 is not None else 0, N.ptr(w), N.DTYPES[w.dtype] if w is not None else 0, rows, cols,
-            eps, y.data_ptr(), N.ptr(h), N.ptr(rstd), N.stream_handle(x.device)), "rms_norm")
+        rp, rt, ldr = r2.data_ptr(), _CODE[residual.dtype], r2.stride(0)
+        h = _like(residual)
+    args = (x2.data_ptr(), _CODE[x.dtype], x2.stride(0), rp, rt, ldr, wp, wt, rows, cols)
+    return args, (x2, weight, r2), h
+
+
+def _forward(x, weight, residual, eps, rstd):
+    """(y, h or None); ``rstd`` None or f32 [rows] to fill."""
+    args, keep, h = _inputs(x, weight, residual)
+    y = _like(x)
+    rc = N.on_device(N.load().glad_rms_norm_forward, x.device.index, *args, eps, y.data_ptr(),
+                     None if h is None else h.data_ptr(), None if rstd is None else rstd.data_ptr())
+    if rc:
+        N.check(rc, "rms_norm")
     return y, h
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
         y, h = _forward(x, weight, residual, eps, rstd)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.x_dtype = x.dtype
         ctx.set_materialize_grads(False)
-        return (y, h) if h is not None else y
+        return y if h is None else (y, h)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
         h, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r, _ = ctx.needs_input_grad
+        x_t, h_t = ctx.x_dtype, h.dtype
         if dy is None:      # only the sum was used
-            return (dsum.to(ctx.x_dtype) if need_x and dsum is not None else None, None,
-                    dsum if need_r else None, None)
+            return (dsum.to(x_t) if need_x and dsum is not None else None, None, dsum if need_r else None, None)
         h2, dy2 = _rows(h), _rows(dy)
-        ds2 = _rows(dsum) if dsum is not None else None
         rows, cols = h2.shape
-        dev = h.device
-        same = h.dtype == ctx.x_dtype       # one gradient serves x and the residual
-        dx = torch.empty(h.shape, dtype=ctx.x_dtype, device=dev) if need_x or (need_r and same) else None
-        dr = torch.empty(h.shape, dtype=h.dtype, device=dev) if need_r and not same else None
-        dw = ws = w = None
+        dx = dr = dw = ws = ds2 = None
+        wp, wt, dwp, wsp, wsn, dsp, ldds = None, 0, None, None, 0, None, 0
+        if need_x or (need_r and x_t == h_t):       # one gradient serves x and a residual of its type
+            dx = _like(dy)
+        if need_r:
+            dr = dx if x_t == h_t else _like(h)
+        if dsum is not None:
+            ds2 = _rows(dsum)
+            dsp, ldds = ds2.data_ptr(), ds2.stride(0)
         if weight is not None:
-            w = weight if weight.is_contiguous() else weight.contiguous()
+            if not weight.is_contiguous():
+                weight = weight.contiguous()
+            wp, wt = weight.data_ptr(), _CODE[weight.dtype]
             if need_w:
-                dw = torch.empty(cols, dtype=weight.dtype, device=dev)
-                ws = torch.empty(N.load().glad_rms_norm_backward_workspace_size(rows, cols), dtype=torch.uint8,
-                                 device=dev)
-        with N.device_guard(dev):
-            N.check(N.load().glad_rms_norm_backward(
-                dy2.data_ptr(), N.DTYPES[ctx.x_dtype], dy2.stride(0), N.ptr(ds2), N.DTYPES[h.dtype],
-                ds2.stride(0) if ds2 is not None else 0, h2.data_ptr(), h2.stride(0), N.ptr(w),
-                N.DTYPES[w.dtype] if w is not None else 0, rstd.data_ptr(), rows, cols, N.ptr(dx), N.ptr(dr),
-                N.ptr(dw), N.ptr(ws), ws.numel() if ws is not None else 0, N.stream_handle(dev)), "rms_norm backward")
-        return dx if need_x else None, dw, (dx if same else dr) if need_r else None, None
+                wsn = N.load().glad_rms_norm_backward_workspace_size(rows, cols)
+                dw, ws = torch.empty_like(weight), rstd.new_empty(wsn // 4)
+                dwp, wsp = dw.data_ptr(), ws.data_ptr()
+        rc = N.on_device(N.load().glad_rms_norm_backward, h.device.index, dy2.data_ptr(), _CODE[x_t], dy2.stride(0), dsp,
+                         _CODE[h_t], ldds, h2.data_ptr(), h2.stride(0), wp, wt, rstd.data_ptr(), rows, cols,
+                         None if dx is None else dx.data_ptr(), None if dr is None or dr is dx else dr.data_ptr(), dwp,
+                         wsp, wsn)
+        if rc:
+            N.check(rc, "rms_norm backward")
+        return dx if need_x else None, dw, dr, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
@@ -132,7 +155,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
     columns of a row (s [..., ceil(C / group)]), 1 where the maximum is 0. ``scale`` a float32 tensor of one value: that
     scale for all (static calibration), returned as s. Inference only: inputs that require a gradient are refused
     while gradients are enabled (``rms_norm`` is the form that trains)."""
-    if out_dtype not in (torch.int8, torch.float8_e4m3fn):
+    if out_dtype != torch.int8 and out_dtype != torch.float8_e4m3fn:
         raise TypeError(f"out_dtype is {out_dtype}; expected int8 or float8_e4m3fn")
     if group not in (0, 32, 64, 128):
         raise ValueError(f"group must be 0, 32, 64 or 128, got {group}")
@@ -144,23 +167,17 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_quant has no gradient; use rms_norm, or torch.no_grad()")
     _check(x, weight, residual, eps)
-    x2 = _rows(x)
-    rows, cols = x2.shape
-    q = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    args, keep, h = _inputs(x, weight, residual)
+    q = _like(x, out_dtype)
     s = scale
     if s is None:
-        s = torch.empty(x.shape[:-1] + (1 if group == 0 else -(-cols // group),), dtype=torch.float32, device=x.device)
-    r2 = h = None
-    if residual is not None:
-        r2 = _rows(residual)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    with N.device_guard(x.device):
-        N.check(N.load().glad_rms_norm_quant(
-            x2.data_ptr(), N.DTYPES[x.dtype], x2.stride(0), N.ptr(r2), N.DTYPES[h.dtype] if h is not None else 0,
-            r2.stride(0) if r2 is not None else 0, N.ptr(w), N.DTYPES[w.dtype] if w is not None else 0, rows, cols,
-            eps, N.DTYPES[out_dtype], group, N.ptr(scale), q.data_ptr(), None if scale is not None else s.data_ptr(),
-            N.ptr(h), N.stream_handle(x.device)), "rms_norm_quant")
+        s = x.new_empty(x.shape[:-1] + (-(-x.shape[-1] // group) if group else 1,), dtype=torch.float32)
+    rc = N.on_device(N.load().glad_rms_norm_quant, x.device.index, *args, eps,
+                     N.DTYPE_I8 if out_dtype == torch.int8 else N.DTYPE_E4M3, group,
+                     None if scale is None else scale.data_ptr(), q.data_ptr(), None if scale is not None else s.data_ptr(),
+                     None if h is None else h.data_ptr())
+    if rc:
+        N.check(rc, "rms_norm_quant")
     return (q, s) if h is None else (q, s, h)
 
 

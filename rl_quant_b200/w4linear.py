@@ -20,8 +20,7 @@ _OUT = (torch.float16, torch.bfloat16, torch.float32)
 
 def _shapes(in_features: int, out_features: int, group: int):
     """(row tiles, 64-input blocks, padded groups) of the laid-out weight."""
-    b = max(64, group)
-    kb = -(-in_features // b) * b // 64
+    kb = -(-in_features // 128) * 2
     return -(-out_features // 16), kb, kb * 64 // group
 
 
@@ -65,7 +64,8 @@ def pack_w4(packed: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4We
     b = (v[:, 0] | (v[:, 1] << 4)).permute(0, 2, 1, 4, 3, 5, 7, 6)
     s = torch.zeros(t * 16, gp, dtype=torch.float16, device=scales.device)
     s[:n, :scales.shape[1]] = scales
-    return W4Weight(b.reshape(t, kb, 512).contiguous(), s.view(t, 16, gp).permute(0, 2, 1).contiguous(), k, n, group)
+    return W4Weight(b.reshape(t, kb, 512).contiguous(), s.view(t, 2, 8, gp).permute(0, 3, 2, 1).reshape(t, gp, 16).contiguous(),
+                    k, n, group)
 
 
 @torch.no_grad()
@@ -76,7 +76,7 @@ def unpack_w4(weight: W4Weight):
     q = torch.stack((b & 15, b >> 4), dim=1).reshape(t * 16, kb * 64)[:weight.out_features, :weight.in_features]
     packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
     g = -(-weight.in_features // weight.group)
-    s = weight.scales.permute(0, 2, 1).reshape(t * 16, gp)[:weight.out_features, :g].contiguous()
+    s = weight.scales.view(t, gp, 8, 2).permute(0, 3, 2, 1).reshape(t * 16, gp)[:weight.out_features, :g].contiguous()
     return packed, s
 
 
@@ -131,12 +131,13 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
         x2 = x2.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
+    y = x.new_empty(x.shape[:-1] + (n,), dtype=out_dtype)
     w = N.GladW4Weight(weight.tiles.data_ptr(), weight.scales.data_ptr(), K, n, weight.group)
-    with N.device_guard(x.device):
-        N.check(N.load().glad_w4_linear_forward(
-            w, x2.data_ptr(), N.DTYPES[x.dtype], x2.shape[0], x2.stride(0), N.ptr(x_scale), per_row, groups,
-            N.ptr(bias), y.data_ptr(), N.DTYPES[out_dtype], N.stream_handle(x.device)), "w4_linear")
+    rc = N.on_device(N.load().glad_w4_linear_forward, x.device.index, w, x2.data_ptr(), N.DTYPES[x.dtype], x2.shape[0],
+                     x2.stride(0), None if x_scale is None else x_scale.data_ptr(), per_row, groups,
+                     None if bias is None else bias.data_ptr(), y.data_ptr(), N.DTYPES[out_dtype])
+    if rc:
+        N.check(rc, "w4_linear")
     return y
 
 

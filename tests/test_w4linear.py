@@ -340,7 +340,7 @@ def test_layout(n, k, group):
                         seen[row, col] = v - 16 if v > 7 else v
     assert np.array_equal(seen[:n, :k], q.numpy()) and not seen[n:].any() and not seen[:, k:].any()
     g = s.shape[1]
-    flat = w.scales.permute(0, 2, 1).reshape(-1, w.scales.shape[1])
+    flat = torch.stack([w.scales[i // 16, :, 2 * (i % 8) + i % 16 // 8] for i in range(16 * w.scales.shape[0])])
     assert torch.equal(flat[:n, :g], s) and not flat[n:].any() and not flat[:, g:].any()
     p2, s2 = unpack_w4(w)
     assert torch.equal(p2, packed) and torch.equal(s2, s)
