@@ -7,6 +7,7 @@
 // four half2 registers with one logic operation and one half operation each:
 // 0x6400 | u is the half 1024 + u, exact for 4-bit u. Products q * x are exact and the sum of
 // a group is fp32; the scale multiplies the group's sum, so no weight is ever rounded.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -30,11 +31,12 @@ struct W4Params {
   const float* xs;          // scales of 8-bit rows or null
   int xs_rows, xs_groups;   // 0/0: none or one value; 1/1: a row; 1/G: a row and group
   int x_fast;               // rows can be read 8 inputs at a time
-  int x_smem;               // few rows: x is staged in shared memory
   int splits;               // many rows: blocks that share a tile's inputs
+  int x_tma;                // many rows: x is read by TMA
   const void* bias;
   void* y;
   int y_dtype;
+  int y_vec;                // four columns of y can be stored at once
 };
 
 struct e4m3_t { uint8_t v; };
@@ -70,18 +72,6 @@ __device__ __forceinline__ void unpack_w4(uint32_t w, uint32_t (&a)[4]) {
     a[2] = h2_sub((w & 0x000f000fu) ^ 0x64086408u, 0x64086408u);
     a[3] = h2_fma((w & 0x00f000f0u) ^ 0x64806480u, 0x2c002c00u, 0xd480d480u);
   }
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Inputs [k, k + 8) of one row as stored: 16 bytes of 16-bit inputs, 8 bytes of 8-bit ones (in
@@ -158,53 +148,132 @@ __device__ __forceinline__ void store_y(const W4Params& p, int64_t m, int n, flo
   }
 }
 
+// Four neighbouring columns; one store where the row allows it.
+__device__ __forceinline__ void store_y4(const W4Params& p, int64_t m, int n, const float (&v)[4]) {
+  if (!p.y_vec || n + 4 > p.N) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < p.N) store_y(p, m, n + e, v[e]);
+    return;
+  }
+  float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t at = m * p.N + n;
+  if (p.y_dtype == GLAD_DTYPE_F32) {
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = static_cast<const float*>(p.bias)[n + e];
+    }
+    *reinterpret_cast<float4*>(static_cast<float*>(p.y) + at) =
+        make_float4(v[0] + b[0], v[1] + b[1], v[2] + b[2], v[3] + b[3]);
+  } else if (p.y_dtype == GLAD_DTYPE_F16) {
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = __half2float(static_cast<const __half*>(p.bias)[n + e]);
+    }
+    __half2 h[2] = {__floats2half2_rn(v[0] + b[0], v[1] + b[1]), __floats2half2_rn(v[2] + b[2], v[3] + b[3])};
+    *reinterpret_cast<uint2*>(static_cast<__half*>(p.y) + at) = *reinterpret_cast<uint2*>(h);
+  } else {
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n + e]);
+    }
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0] + b[0], v[1] + b[1]),
+                           __floats2bfloat162_rn(v[2] + b[2], v[3] + b[3])};
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.y) + at) = *reinterpret_cast<uint2*>(h);
+  }
+}
+
 // ---- few rows (up to 8 NT): weight streaming ------------------------------------------------
 // One persistent block per SM walks 16-column tiles; its 16 warps split the inputs in units of
 // 128 and join their sums in warp order once a tile. Each warp streams its own units (1 KB of
 // weights and 128/GROUP * 32 bytes of scales) through a private shared-memory ring of
-// cp.async copies kRing - 1 units ahead, across tile borders, so about 64 KB are in flight on
-// an SM whatever the warps wait for. x is staged once in shared memory when it fits.
-constexpr int kRowWarps = 16, kRing = 5;
+// cp.async copies kRing - 1 units ahead, across tile borders, so about 48 KB are in flight on
+// an SM whatever the warps wait for. x is staged once in shared memory when it fits, in the form the
+// products take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
+// a word's nibbles come apart). Rows past M read row M - 1: their sums are never stored.
+constexpr int kRowWarps = 16, kRing = 4;
 constexpr int kRowThreads = kRowWarps * 32;
 
-template <int GROUP>
-struct RowRing {
+template <int NT, int GROUP>
+struct RowSmem {
   static constexpr int kScales = 128 / GROUP;           // groups of a unit
   static constexpr int kWarpSlot = 1024 + kScales * 32;
-  static constexpr int kBytes = kRing * kRowWarps * kWarpSlot;
-};
-template <int NT>
-struct RowPart {                                         // two buffers of every warp's sums
-  static constexpr int kBytes = 2 * kRowWarps * 8 * NT * 17 * 4;
+  static constexpr int kRingBytes = kRing * kRowWarps * kWarpSlot;
+  static constexpr int kBuffers = NT == 1 ? 2 : 1;      // of every warp's sums
+  static constexpr int kPart = kRowWarps * 8 * NT * 17;
+  static constexpr int kFixed = kRingBytes + kBuffers * kPart * 4;
 };
 
-template <typename TX, int NT, int GROUP>
+// D = A * B + 0 / D += A * B, m16n8k16 (f16, bf16 -> f32) and m16n8k32 (s8 -> s32).
+template <bool BF16, bool FIRST>
+__device__ __forceinline__ void mma_rows(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (FIRST) {
+    if constexpr (BF16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  } else {
+    if constexpr (BF16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+template <bool FIRST>
+__device__ __forceinline__ void mma_rows_i8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (FIRST)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The 4-bit pieces of a word as int8 times 16 (the nibble in the byte's high half): rows r and r + 8.
+__device__ __forceinline__ uint32_t w4_low16(uint32_t w) { return (w << 4) & 0xf0f0f0f0u; }
+__device__ __forceinline__ uint32_t w4_high16(uint32_t w) { return w & 0xf0f0f0f0u; }
+__device__ __forceinline__ uint32_t swap_mid(uint32_t v) { return __byte_perm(v, 0, 0x3120); }
+
+template <typename TX, int NT, int GROUP, bool XS>
 __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
-  using Ring = RowRing<GROUP>;
-  constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value;
-  constexpr int SG = Ring::kScales, XB = (int)sizeof(TX);
+  using L = RowSmem<NT, GROUP>;
+  constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
+  constexpr int SG = L::kScales, XP = I8 ? 8 : 16;       // bytes of eight staged inputs
   extern __shared__ __align__(16) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem + Ring::kBytes);
-  uint8_t* xs = smem + Ring::kBytes + RowPart<NT>::kBytes;
+  float* part = reinterpret_cast<float*>(smem + L::kRingBytes);
+  uint8_t* xs = smem + L::kFixed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int T = (p.N + 15) / 16, U = p.KB / 2, M = (int)p.M;
   const int u0 = (int)((int64_t)warp * U / kRowWarps), u1 = (int)((int64_t)(warp + 1) * U / kRowWarps);
-  uint8_t* ring = smem + warp * (kRing * Ring::kWarpSlot);
+  uint8_t* ring = smem + warp * (kRing * L::kWarpSlot);
 
-  int pt = blockIdx.x, pu = u0;                          // the next unit to fetch
+  // the next unit to fetch: tile pt, unit pu
+  int pt = u0 < u1 ? blockIdx.x : T, pu = u0;
+  const uint4* wsrc = p.tiles + ((int64_t)pt * U + pu) * 64 + lane;
+  const uint8_t* ssrc = reinterpret_cast<const uint8_t*>(p.scales) + ((int64_t)pt * U + pu) * (SG * 32) + lane * 16;
+  const int64_t skip = (int64_t)gridDim.x * U - (u1 - u0);   // units from the end of this tile's share to the next tile's
   auto fetch = [&](int slot) {
-    if (pt < T && u0 < u1) {
-      uint8_t* dst = ring + slot * Ring::kWarpSlot;
-      const uint4* src = p.tiles + ((int64_t)pt * p.KB + 2 * pu) * 32 + lane;
-      cp_async16(dst + lane * 16, src);
-      cp_async16(dst + 512 + lane * 16, src + 32);
-      if (lane < SG * 2) {
-        const uint8_t* sc = reinterpret_cast<const uint8_t*>(p.scales) + ((int64_t)pt * U + pu) * (SG * 32);
-        cp_async16(dst + 1024 + lane * 16, sc + lane * 16);
-      }
+    if (pt < T) {
+      uint8_t* dst = ring + slot * L::kWarpSlot + lane * 16;
+      cp_async16(dst, wsrc);
+      cp_async16(dst + 512, wsrc + 32);
+      if (lane < SG * 2) cp_async16(dst + 1024, ssrc);
+      wsrc += 64;
+      ssrc += SG * 32;
       if (++pu == u1) {
         pu = u0;
         pt += gridDim.x;
+        wsrc += skip * 64;
+        ssrc += skip * (SG * 32);
       }
     }
     cp_async_commit();
@@ -214,83 +283,111 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) fetch(i);
 
-  if (p.x_smem) {
+  auto staged = [&](uint4 v) -> uint4 {
+    if constexpr (I8) return make_uint4(swap_mid(v.x), swap_mid(v.y), 0, 0);
+    else return to_halves<TX>(v);
+  };
+  if constexpr (XS) {
     // [32-input block][row][32 inputs]: a warp's reads of eight rows are contiguous
     const int pieces = p.KB * 8 * M;
     for (int i = threadIdx.x; i < pieces; i += kRowThreads) {
       const int m = i / (p.KB * 8), k8 = i - m * (p.KB * 8);
-      const uint4 v = load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k8 * 8, p.K, p.x_fast);
-      uint8_t* dst = xs + (((k8 >> 2) * M + m) * 4 + (k8 & 3)) * (8 * XB);
-      if constexpr (XB == 2) *reinterpret_cast<uint4*>(dst) = v;
-      else *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+      const uint4 v = staged(load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k8 * 8, p.K, p.x_fast));
+      uint8_t* dst = xs + (((k8 >> 2) * M + m) * 4 + (k8 & 3)) * XP;
+      if constexpr (I8) *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+      else *reinterpret_cast<uint4*>(dst) = v;
     }
     __syncthreads();
   }
-  auto get_x = [&](int m, int k32) -> uint4 {            // inputs 32 k32 + 8 c .. + 7 of row m
-    if (m >= M) return make_uint4(0, 0, 0, 0);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (p.x_smem) {
-      const uint8_t* src = xs + ((k32 * M + m) * 4 + c) * (8 * XB);
-      if constexpr (XB == 2) {
-        v = *reinterpret_cast<const uint4*>(src);
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(src);
-        v.x = u.x, v.y = u.y;
-      }
-    } else {
-      v = load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k32 * 32 + 8 * c, p.K, p.x_fast);
-    }
-    return to_halves<TX>(v);
-  };
+  const uint8_t* xrow[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int m = min(8 * j + r, M - 1);
+    xrow[j] = xs + (m * 4 + c) * XP;
+  }
+  const int xstep = M * 4 * XP;                          // bytes of 32 inputs of all rows
 
-  int slot = 0, parity = 0;
+  int slot = 0, buffer = 0;
   for (int t = blockIdx.x; t < T; t += gridDim.x) {
-    float acc[NT][4], g[NT][4];
+    float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = g[j][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
     for (int u = u0; u < u1; ++u) {
       cp_async_wait_group<kRing - 2>();
       __syncwarp();
-      fetch(slot == 0 ? kRing - 1 : slot - 1);           // the slot that every lane has just left
-      const uint8_t* in = ring + slot * Ring::kWarpSlot;
-      slot = slot + 1 == kRing ? 0 : slot + 1;
+      fetch((slot + kRing - 1) % kRing);                 // the slot that every lane has just left
+      const uint8_t* in = ring + slot * L::kWarpSlot;
+      slot = (slot + 1) % kRing;
+      uint4 w4[2] = {*reinterpret_cast<const uint4*>(in + lane * 16),
+                     *reinterpret_cast<const uint4*>(in + 512 + lane * 16)};
+      const uint32_t w[8] = {w4[0].x, w4[0].y, w4[0].z, w4[0].w, w4[1].x, w4[1].y, w4[1].z, w4[1].w};
+      float g[NT][4];
+      int gi8[NT][4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {                      // 32 inputs at a time
-        const uint2 w = *reinterpret_cast<const uint2*>(in + (q >> 1) * 512 + lane * 16 + (q & 1) * 8);
-        uint32_t a0[4], a1[4];
-        unpack_w4<BF16>(w.x, a0);
-        unpack_w4<BF16>(w.y, a1);
+        constexpr int QG = GROUP / 32;
+        uint4 x[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const uint4 x = get_x(8 * j + r, 4 * u + q);
-          mma_16816<BF16>(g[j], a0, x.x, x.y);
-          mma_16816<BF16>(g[j], a1, x.z, x.w);
+          if constexpr (XS) {
+            const uint8_t* src = xrow[j] + (4 * u + q) * xstep;
+            if constexpr (I8) {
+              const uint2 v = *reinterpret_cast<const uint2*>(src);
+              x[j] = make_uint4(v.x, v.y, 0, 0);
+            } else {
+              x[j] = *reinterpret_cast<const uint4*>(src);
+            }
+          } else {
+            x[j] = staged(load_raw8<TX>(static_cast<const TX*>(p.x) + min(8 * j + r, M - 1) * p.ldx,
+                                        (4 * u + q) * 32 + 8 * c, p.K, p.x_fast));
+          }
         }
-        if ((q + 1) % (GROUP / 32) == 0) {
-          const int gi = q / (GROUP / 32);
-          const float2 s = __half22float2(*reinterpret_cast<const __half2*>(in + 1024 + gi * 32 + r * 4));
+        if constexpr (I8) {
+          const uint32_t a[4] = {w4_low16(w[2 * q]), w4_high16(w[2 * q]), w4_low16(w[2 * q + 1]), w4_high16(w[2 * q + 1])};
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            float x0 = 1.0f, x1 = 1.0f;
-            if (p.xs_groups > 1) {
-              const int m = 8 * j + 2 * c, xg = u * SG + gi;
-              x0 = (m < M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
-              x1 = (m + 1 < M && xg < p.xs_groups) ? p.xs[(m + 1) * p.xs_groups + xg] : 0.0f;
-            }
-            acc[j][0] = fmaf(__fmul_rn(s.x, x0), g[j][0], acc[j][0]);
-            acc[j][1] = fmaf(__fmul_rn(s.x, x1), g[j][1], acc[j][1]);
-            acc[j][2] = fmaf(__fmul_rn(s.y, x0), g[j][2], acc[j][2]);
-            acc[j][3] = fmaf(__fmul_rn(s.y, x1), g[j][3], acc[j][3]);
+            if (q % QG == 0) mma_rows_i8<true>(gi8[j], a, x[j].x, x[j].y);
+            else mma_rows_i8<false>(gi8[j], a, x[j].x, x[j].y);
+          }
+        } else {
+          uint32_t a0[4], a1[4];
+          unpack_w4<BF16>(w[2 * q], a0);
+          unpack_w4<BF16>(w[2 * q + 1], a1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) g[j][e] = 0.0f;
+          for (int j = 0; j < NT; ++j) {
+            if (q % QG == 0) mma_rows<BF16, true>(g[j], a0, x[j].x, x[j].y);
+            else mma_rows<BF16, false>(g[j], a0, x[j].x, x[j].y);
+            mma_rows<BF16, false>(g[j], a1, x[j].z, x[j].w);
+          }
+        }
+        if ((q + 1) % QG == 0) {
+          const int gi = q / QG;
+          float2 s = __half22float2(*reinterpret_cast<const __half2*>(in + 1024 + gi * 32 + r * 4));
+          if constexpr (I8) s.x *= 0.0625f, s.y *= 0.0625f;   // the codes were multiplied by 16
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if constexpr (I8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) g[j][e] = i2f_small(gi8[j][e]);   // below 2^21
+            }
+            if (sizeof(TX) == 1 && p.xs_groups > 1) {
+              const int m = 8 * j + 2 * c, xg = u * SG + gi;
+              const float x0 = (m < M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
+              const float x1 = (m + 1 < M && xg < p.xs_groups) ? p.xs[(m + 1) * p.xs_groups + xg] : 0.0f;
+              g[j][0] *= x0, g[j][1] *= x1, g[j][2] *= x0, g[j][3] *= x1;
+            }
+            acc[j][0] = fmaf(s.x, g[j][0], acc[j][0]);
+            acc[j][1] = fmaf(s.x, g[j][1], acc[j][1]);
+            acc[j][2] = fmaf(s.y, g[j][2], acc[j][2]);
+            acc[j][3] = fmaf(s.y, g[j][3], acc[j][3]);
           }
         }
       }
     }
-    // the buffer written now was last read two tiles ago, before the previous tile's barrier
-    float* mine = part + (parity * kRowWarps + warp) * (8 * NT * 17);
+    // with two buffers, the one written now was last read before the previous tile's barrier
+    float* mine = part + buffer * L::kPart + warp * (8 * NT * 17);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       mine[(8 * j + 2 * c) * 17 + r] = acc[j][0];
@@ -301,53 +398,58 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
     __syncthreads();
     const int row = threadIdx.x >> 4, col = threadIdx.x & 15, n = 16 * t + col;
     if (row < 8 * NT && row < M && n < p.N) {
-      const float* all = part + parity * kRowWarps * (8 * NT * 17) + row * 17 + col;
+      const float* all = part + buffer * L::kPart + row * 17 + col;
       float v = 0.0f;
 #pragma unroll
       for (int k = 0; k < kRowWarps; ++k) v += all[k * (8 * NT * 17)];
       if (p.xs != nullptr && p.xs_groups <= 1) v *= p.xs[p.xs_rows ? row : 0];
       store_y(p, row, n, v);
     }
-    parity ^= 1;
+    if constexpr (L::kBuffers == 2) buffer ^= 1;
+    else __syncthreads();
   }
 }
 
 // ---- many rows: tcgen05 -----------------------------------------------------------------------
-// A block computes 128 output columns x MT rows; D[n, m] lives in tensor memory, n its lanes. Per
-// stage of 128 inputs, 16 warps turn the packed weights into the fp16 (bf16) A operand in shared
-// memory while one thread issues the products of the stage before. Every group of inputs has an
-// accumulator of its own (ND in rotation): the warps read it back, scale it by s[n, g] (a lane's
-// own row: one value a thread) and add it to fp32 sums in registers, so the weights need no
-// rounding; that costs one multiply-add per output and group, as much issue time as the tensor
-// core needs for 64 inputs at fp16 rate. The inputs of x are copied NS - 1 stages ahead, the
-// packed weights PD stages ahead by bulk copies. Blocks of a cluster split the inputs when there are
-// fewer tiles than SMs and join their sums through distributed shared memory in rank order.
+// A block computes 128 output columns x MT rows; D[n, m] lives in tensor memory, n its lanes. The
+// inputs go in stages of 128 bytes a row (64 of 16 bits, 128 of 8 bits: one swizzle atom). A loader
+// thread brings the packed weights (bulk copies, PD units of 128 inputs ahead) and the x tile (TMA,
+// NS stages); 16 warps turn the weights into the A operand in shared memory, in x's own type: f16 or
+// bf16, int8 times 16, or e4m3, all exact; one thread issues the products. Every group of inputs has
+// an accumulator of its own (ND in rotation): the 16 warps read it back, scale it by s[n, g] (a
+// lane's own row: one value a thread) and add it to fp32 sums in registers, so the weights need no
+// rounding; that costs one multiply-add an output and group, at groups of 64 half of the
+// tensor core's time for them at fp16 rate. Blocks of a cluster split the inputs when there are fewer
+// tiles than SMs and join their sums through distributed shared memory in rank order.
 constexpr int kTileWarps = 16;
-constexpr int kTileThreads = (kTileWarps + 2) * 32;      // + the MMA warp + the weight loader
+constexpr int kTileThreads = (kTileWarps + 3) * 32;      // + the MMA warp + two loaders
 
 __device__ unsigned int g_w4_status;
 
-template <int MT, int GROUP>
+template <int XB, int MT, int GROUP>                     // XB: bytes of an input
 struct Tile {
-  static constexpr int NS = MT == 256 ? 2 : 3;
+  static constexpr int SPU = XB;                         // stages of a unit (128 inputs)
+  static constexpr int NS = MT == 256 ? 4 : 6;
   static constexpr int PD = MT == 256 ? 2 : MT == 128 ? 3 : 6;
   static constexpr int ND = MT == 256 ? 2 : 4;
-  static constexpr int SG = 128 / GROUP;
-  static constexpr int kA = 128 * 256, kB = MT * 256, kStage = kA + kB;
-  static constexpr int kSlot = 8192 + 8 * SG * 32;       // packed weights and scales of a stage
-  static constexpr int kXs = 3 * SG * MT * 4;            // x scales of three stages
-  static constexpr int kRed = MT * 128 * 4;
-  static constexpr int kSmem = NS * kStage + PD * kSlot + kXs + 256 + 1024;
+  static constexpr int SG = 128 / GROUP;                 // groups of a unit
+  static constexpr int SPG = GROUP * XB / 32;            // products (32 bytes of inputs) of a group
+  static constexpr int kA = 128 * 128, kB = MT * 128, kStage = kA + kB;
+  static constexpr int kSlot = 8192 + 8 * SG * 32;       // packed weights and scales of a unit
+  static constexpr int kXs = XB == 1 ? 3 * SG * MT * 4 : 0;   // x scales of three units
+  static constexpr int kSmem = NS * kStage + PD * kSlot + kXs + 512 + 1024;
   static constexpr int kCols = ND * MT;
-  static_assert(kRed <= NS * kStage, "the sums are joined in the stage buffers");
+  static_assert(MT * 128 * 4 <= NS * kStage, "the sums are joined in the stage buffers");
   static_assert(kSmem <= 232448, "shared memory of one block");
+  static_assert((2 * NS + 2 * PD + 2 * ND) * 8 + 8 <= 512, "barrier area");
 };
 
 __device__ __noinline__ bool w4_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   while (!*abort) {
-    if (mbar_try_wait(bar, parity)) return true;
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
     if (global_timer_ns() - t0 > 2000000000ull) {
       *abort = 1;
       atomicOr(&g_w4_status, kDevErrMmaTimeout);
@@ -356,17 +458,33 @@ __device__ __noinline__ bool w4_wait(uint64_t* bar, uint32_t parity, volatile in
   return false;
 }
 
-// K-major operand with 128-byte swizzle: rows of 128 bytes (64 halves), 8-row groups 1024 bytes apart,
-// the 16-byte piece i of row r at i ^ (r & 7).
+// K-major operand with 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart, the 16-byte
+// piece i of row r at i ^ (r & 7).
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) |
          ((uint64_t)2 << 61);
 }
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// x tile: 128 bytes of MT rows, zero outside the tensor, swizzled as desc_sw128 reads it.
+__device__ __forceinline__ void tma_x(uint32_t dst, const CUtensorMap* map, int k, int m, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(k), "r"(m), "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void st_shared_v2(uint32_t dst, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(a), "r"(b) : "memory");
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
@@ -375,35 +493,65 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
+// The eight weights of a word as bytes in the operand's type: lo = row r, hi = row r + 8, inputs
+// k .. k + 3 in order.
+template <bool E4M3>
+__device__ __forceinline__ void unpack_w4_bytes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (!E4M3) {
+    lo = swap_mid(w4_low16(w));
+    hi = swap_mid(w4_high16(w));
+  } else {
+    // e4m3 of 0..7 and of -8..-1, picked by the low three bits, chosen by the top bit
+    const uint32_t idx = w & 0x77777777u, neg = (w >> 3) & 0x11111111u;
+    uint32_t v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t i = idx >> (16 * h), n = neg >> (16 * h);
+      const uint32_t pos = __byte_perm(0x44403800u, 0x4e4c4a48u, i);
+      const uint32_t ng = __byte_perm(0xcaccced0u, 0xb8c0c4c8u, i);
+      const uint32_t m = __byte_perm(0x0000ff00u, 0, n);
+      v[h] = (ng & m) | (pos & ~m);
+    }
+    // v[0]: (r, k) (r+8, k) (r, k+2) (r+8, k+2); v[1]: the same for k+1, k+3
+    lo = __byte_perm(v[0], v[1], 0x6240);
+    hi = __byte_perm(v[0], v[1], 0x7351);
+  }
+}
+
 template <typename TX, int MT, int GROUP>
-__global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_constant__ W4Params p) {
-  using L = Tile<MT, GROUP>;
-  constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value;
-  constexpr int SG = L::SG, NC = MT / 4, XP = MT / 32;   // columns, 16-byte x pieces of a thread
+__global__ void __launch_bounds__(kTileThreads, 1)
+    w4_tile_kernel(const __grid_constant__ W4Params p, const __grid_constant__ CUtensorMap xmap) {
+  using L = Tile<(int)sizeof(TX), MT, GROUP>;
+  constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
+  constexpr bool E4M3 = std::is_same<TX, e4m3_t>::value;
+  constexpr int XB = (int)sizeof(TX), SG = L::SG, SPU = L::SPU, NC = MT / 4, KS = 128 / XB;   // KS: inputs of a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* slots = smem + L::NS * L::kStage;
   float* xsc = reinterpret_cast<float*>(slots + L::PD * L::kSlot);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xsc) + L::kXs);   // [NS]
-  uint64_t* wfull = full + L::NS;                                                           // [PD]
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xsc) + L::kXs);   // [NS] operands written
+  uint64_t* empty = full + L::NS;                                                           // [NS] products done
+  uint64_t* wfull = empty + L::NS;                                                          // [PD]
   uint64_t* wempty = wfull + L::PD;                                                         // [PD]
   uint64_t* dfull = wempty + L::PD;                                                         // [ND]
   uint64_t* dempty = dfull + L::ND;                                                         // [ND]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dempty + L::ND);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((L::NS + 2 * L::PD + 2 * L::ND) * 8 + 8 <= 256, "barrier area");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = p.splits, rank = S > 1 ? (int)cluster_ctarank() : 0;
   const int nt = blockIdx.x / S;
   const int64_t m0 = (int64_t)blockIdx.y * MT;
-  const int ST = p.KB / 2, st0 = (int)((int64_t)rank * ST / S), st1 = (int)((int64_t)(rank + 1) * ST / S);
-  const int count = st1 - st0;
+  const int U = p.KB / 2, un0 = (int)((int64_t)rank * U / S), un1 = (int)((int64_t)(rank + 1) * U / S);
+  const int units = un1 - un0;
   const int live16 = min(8, (p.N + 15) / 16 - nt * 8);   // 16-column tiles that exist
 
   if (warp == kTileWarps) tmem_alloc(tmem_slot, L::kCols);
   if (tid == 0) {
-    for (int i = 0; i < L::NS; ++i) mbar_init(&full[i], kTileWarps);
+    for (int i = 0; i < L::NS; ++i) {
+      mbar_init(&full[i], kTileWarps + (p.x_tma ? 1 : 0));
+      mbar_init(&empty[i], 1);
+    }
     for (int i = 0; i < L::PD; ++i) {
       mbar_init(&wfull[i], 1);
       mbar_init(&wempty[i], kTileWarps);
@@ -428,51 +576,67 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
   grid_dep_launch();
 
   if (warp == kTileWarps + 1) {
-    // ---- packed weights and scales, PD stages ahead
+    // ---- packed weights and scales
     if (lane == 0) {
       const uint8_t* wsrc = reinterpret_cast<const uint8_t*>(p.tiles);
       const uint8_t* ssrc = reinterpret_cast<const uint8_t*>(p.scales);
-      int issued = 0;
-      for (int i = 0; i < count; ++i, ++issued) {
+      int i = 0;
+      for (; i < units; ++i) {
         const int slot = i % L::PD;
         if (i >= L::PD && !w4_wait(&wempty[slot], (i / L::PD - 1) & 1, abort)) break;
         uint8_t* dst = slots + slot * L::kSlot;
         mbar_arrive_expect_tx(&wfull[slot], (uint32_t)live16 * (1024 + SG * 32));
         for (int b = 0; b < live16; ++b) {
-          const int64_t t = (int64_t)nt * 8 + b, st = st0 + i;
-          bulk_copy_g2s(dst + b * 1024, wsrc + (t * p.KB + 2 * st) * 512, 1024, &wfull[slot]);
-          bulk_copy_g2s(dst + 8192 + b * (SG * 32), ssrc + (t * ST + st) * (SG * 32), SG * 32, &wfull[slot]);
+          const int64_t at = ((int64_t)nt * 8 + b) * U + un0 + i;
+          bulk_copy_g2s(dst + b * 1024, wsrc + at * 1024, 1024, &wfull[slot]);
+          bulk_copy_g2s(dst + 8192 + b * (SG * 32), ssrc + at * (SG * 32), SG * 32, &wfull[slot]);
         }
       }
-      // copies that were issued land before the block leaves
-      for (int i = max(0, issued - L::PD); i < issued && *abort; ++i)
-        mbar_wait_bounded(&wfull[i % L::PD], (i / L::PD) & 1);
+      // after a failure: copies that were issued land before the block leaves
+      for (int k = max(0, i - L::PD); k < i && *abort; ++k) mbar_wait_bounded(&wfull[k % L::PD], (k / L::PD) & 1);
+    }
+  } else if (warp == kTileWarps + 2) {
+    // ---- x tiles
+    if (lane == 0 && p.x_tma) {
+      const uint32_t base = smem_u32(smem);
+      const int stages = units * SPU;
+      int i = 0;
+      for (; i < stages; ++i) {
+        const int st = i % L::NS;
+        if (i >= L::NS && !w4_wait(&empty[st], (i / L::NS - 1) & 1, abort)) break;
+        mbar_arrive_expect_tx(&full[st], L::kB);
+        tma_x(base + st * L::kStage + L::kA, &xmap, un0 * 128 + i * KS, (int)m0, &full[st]);
+      }
+      for (int k = max(0, i - L::NS); k < i && *abort; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1);
     }
   } else if (warp == kTileWarps) {
     // ---- products
     if (lane == 0) {
-      constexpr uint32_t idesc = idesc_f16(128, MT) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+      constexpr uint32_t idesc = I8 ? idesc_i8(128, MT) : idesc_f16(128, MT) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t base = smem_u32(smem);
-      int gi = 0;
-      for (int i = 0; i < count; ++i) {
-        if (!w4_wait(&full[i % L::NS], (i / L::NS) & 1, abort)) break;
+      const int stages = units * SPU;
+      int gi = 0;                                        // groups begun
+      bool ok = true;
+      for (int i = 0; ok && i < stages; ++i) {
+        if (!(ok = w4_wait(&full[i % L::NS], (i / L::NS) & 1, abort))) break;
         tc_fence_after();
-        const uint32_t a = base + (i % L::NS) * L::kStage, b = a + L::kA;
-        bool ok = true;
+        const uint64_t a = desc_sw128(base + (i % L::NS) * L::kStage);
+        const uint64_t b = desc_sw128(base + (i % L::NS) * L::kStage + L::kA);
 #pragma unroll
-        for (int j = 0; j < SG; ++j, ++gi) {
-          const int d = gi % L::ND;
-          if (gi >= L::ND && !(ok = w4_wait(&dempty[d], (gi / L::ND - 1) & 1, abort))) break;
-          tc_fence_after();
-#pragma unroll
-          for (int q = 0; q < GROUP / 16; ++q) {
-            const int k16 = j * (GROUP / 16) + q;
-            mma_f16(tmem + d * MT, desc_sw128(a + (k16 >> 2) * 16384 + (k16 & 3) * 32),
-                    desc_sw128(b + (k16 >> 2) * (MT * 128) + (k16 & 3) * 32), idesc, q > 0 ? 1u : 0u);
+        for (int q = 0; q < 4; ++q) {                    // 32 bytes of inputs
+          const int in_group = (i * 4 + q) % L::SPG;
+          if (in_group == 0) {
+            if (gi >= L::ND && !(ok = w4_wait(&dempty[gi % L::ND], (gi / L::ND - 1) & 1, abort))) break;
+            tc_fence_after();
+            ++gi;
           }
-          mma_commit(&dfull[d]);
+          const uint32_t d = tmem + ((gi - 1) % L::ND) * MT;
+          if constexpr (I8) mma_i8(d, a + 2 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
+          else if constexpr (E4M3) mma_f8(d, a + 2 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
+          else mma_f16(d, a + 2 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
+          if (in_group == L::SPG - 1) mma_commit(&dfull[(gi - 1) % L::ND]);
         }
-        if (!ok) break;
+        if (ok) mma_commit(&empty[i % L::NS]);
       }
       // after a failure: products that were issued end before their operands go
       for (int k = max(0, gi - L::ND); k < gi && *abort; ++k) mbar_wait_bounded(&dfull[k % L::ND], (k / L::ND) & 1);
@@ -481,93 +645,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
     // ---- operands, sums
     const int r = lane >> 2, c = lane & 3, q4 = warp & 3, col0 = (warp >> 2) * NC;
     const uint32_t sbase = smem_u32(smem);
-    const uint32_t a_row = (uint32_t)((warp >> 1) * 16 + r) * 128 + (warp & 1) * 16384;
     const int my_n16 = q4 * 2 + (lane >> 4), my_s = (lane & 7) * 2 + ((lane >> 3) & 1);
+    const bool by_group = XB == 1 && p.xs_groups > 1;
     float acc[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
     float sc[SG], sc_next[SG];
-    uint2 raw[sizeof(TX) == 1 ? XP : 1];
     float xs_reg[2] = {0.0f, 0.0f};
-    constexpr int XD = L::NS - 1;
-
-    auto x_dst = [&](int i, int piece) -> uint32_t {     // stage i, this thread's piece
-      const int id = piece * 512 + tid, row = id >> 4, k8 = id & 15;
-      return sbase + (i % L::NS) * L::kStage + L::kA + (k8 >> 3) * (MT * 128) + row * 128 + (((k8 & 7) ^ (row & 7)) << 4);
-    };
-    auto x_issue = [&](int i) {                          // 16-bit rows: asynchronous copies of stage i
-      if constexpr (sizeof(TX) == 2) {
-        if (p.x_fast && i < count) {
-#pragma unroll
-          for (int e = 0; e < XP; ++e) {
-            const int id = e * 512 + tid;
-            const int64_t m = m0 + (id >> 4);
-            const int k = (st0 + i) * 128 + (id & 15) * 8;
-            const bool live = m < p.M && k < p.K;
-            cp_async16_zfill(x_dst(i, e), static_cast<const TX*>(p.x) + (live ? m * p.ldx + k : 0), live);
-          }
-        }
-        cp_async_commit();
-      }
-    };
-    auto x_load = [&](int i) {                           // 8-bit rows: stage i into registers
-      if constexpr (sizeof(TX) == 1) {
-        if (i < count) {
-#pragma unroll
-          for (int e = 0; e < XP; ++e) {
-            const int id = e * 512 + tid;
-            const int64_t m = m0 + (id >> 4);
-            const int k = (st0 + i) * 128 + (id & 15) * 8;
-            raw[e] = make_uint2(0, 0);
-            if (m < p.M) {
-              const uint4 v = load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k, p.K, p.x_fast);
-              raw[e] = make_uint2(v.x, v.y);
-            }
-          }
-          if (p.xs_groups > 1) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int id = e * 512 + tid, g = id / MT;
-              const int64_t m = m0 + id % MT;
-              const int xg = (st0 + i) * SG + g;
-              xs_reg[e] = (g < SG && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
-            }
-          }
-        }
-      }
-    };
-    auto x_finish = [&](int i) {                         // stage i of x is in shared memory
-      if constexpr (sizeof(TX) == 1) {
-#pragma unroll
-        for (int e = 0; e < XP; ++e) {
-          const uint4 h = to_halves<TX>(make_uint4(raw[e].x, raw[e].y, 0, 0));
-          st_shared_v4(x_dst(i, e), h.x, h.y, h.z, h.w);
-        }
-        if (p.xs_groups > 1) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (e * 512 + tid < SG * MT) xsc[(i % 3) * (SG * MT) + e * 512 + tid] = xs_reg[e];
-        }
-      } else if (p.x_fast) {
-        cp_async_wait_group<XD - 1>();
-      } else {
-#pragma unroll 1
-        for (int e = 0; e < XP; ++e) {
-          const int id = e * 512 + tid;
-          const int64_t m = m0 + (id >> 4);
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (m < p.M)
-            v = load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, (st0 + i) * 128 + (id & 15) * 8, p.K, false);
-          st_shared_v4(x_dst(i, e), v.x, v.y, v.z, v.w);
-        }
-      }
-    };
     bool ok = true;
-    auto sums = [&](int i) {                             // add the groups of stage i
+
+    // x that TMA cannot read (rows off 16 bytes): stage i by guarded loads
+    auto copy_x = [&](int i) {
+      const uint32_t b = sbase + (i % L::NS) * L::kStage + L::kA;
+#pragma unroll 1
+      for (int id = tid; id < MT * 8; id += kTileWarps * 32) {
+        const int row = id >> 3, piece = id & 7;
+        const int k = un0 * 128 + i * KS + piece * (16 / XB);
+        const int64_t m = m0 + row;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (m < p.M) {
+          const TX* src = static_cast<const TX*>(p.x) + m * p.ldx;
+          v = load_raw8<TX>(src, k, p.K, false);
+          if constexpr (XB == 1) {
+            const uint4 u = load_raw8<TX>(src, k + 8, p.K, false);
+            v.z = u.x, v.w = u.y;
+          }
+        }
+        st_shared_v4(b + row * 128 + ((piece ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
+      }
+    };
+    auto load_xs = [&](int u) {                          // x scales of unit u into registers
+      if (by_group && u < units) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int id = e * 512 + tid, g = id / MT;
+          const int64_t m = m0 + id % MT;
+          const int xg = (un0 + u) * SG + g;
+          xs_reg[e] = (g < SG && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
+        }
+      }
+    };
+    auto sums = [&](int u) {                             // add the groups of unit u
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
-        const int gi = i * SG + j, d = gi % L::ND;
-        if (!ok || !(ok = w4_wait(&dfull[d], (gi / L::ND) & 1, abort))) return;
+        const int gi = u * SG + j, d = gi % L::ND;
+        if (ok) ok = w4_wait(&dfull[d], (gi / L::ND) & 1, abort);
+        if (!ok) return;
         tc_fence_after();
         constexpr int CH = NC < 16 ? NC : 16;
 #pragma unroll
@@ -577,20 +700,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
           if constexpr (CH == 16) tmem_ld16(at, v);
           else tmem_ld8(at, v);
           tmem_ld_wait();
-          if (sizeof(TX) == 1 && p.xs_groups > 1) {
-            const float4* xv = reinterpret_cast<const float4*>(xsc + (i % 3) * (SG * MT) + j * MT + col0 + cb);
+          float f[CH];
+#pragma unroll
+          for (int e = 0; e < CH; ++e) f[e] = I8 ? i2f_small((int)v[e]) : __uint_as_float(v[e]);   // |int| < 2^22
+          if (by_group) {
+            const float4* xv = reinterpret_cast<const float4*>(xsc + (u % 3) * (SG * MT) + j * MT + col0 + cb);
 #pragma unroll
             for (int e = 0; e < CH; e += 4) {
-              const float4 f = xv[e / 4];
-              acc[cb + e] = fmaf(__fmul_rn(sc[j], f.x), __uint_as_float(v[e]), acc[cb + e]);
-              acc[cb + e + 1] = fmaf(__fmul_rn(sc[j], f.y), __uint_as_float(v[e + 1]), acc[cb + e + 1]);
-              acc[cb + e + 2] = fmaf(__fmul_rn(sc[j], f.z), __uint_as_float(v[e + 2]), acc[cb + e + 2]);
-              acc[cb + e + 3] = fmaf(__fmul_rn(sc[j], f.w), __uint_as_float(v[e + 3]), acc[cb + e + 3]);
+              const float4 x = xv[e / 4];
+              f[e] *= x.x, f[e + 1] *= x.y, f[e + 2] *= x.z, f[e + 3] *= x.w;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < CH; ++e) acc[cb + e] = fmaf(sc[j], __uint_as_float(v[e]), acc[cb + e]);
           }
+#pragma unroll
+          for (int e = 0; e < CH; ++e) acc[cb + e] = fmaf(sc[j], f[e], acc[cb + e]);
         }
         tc_fence_before();
         __syncwarp();
@@ -598,48 +720,70 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
       }
     };
 
-#pragma unroll
-    for (int i = 0; i < XD; ++i) x_issue(i);
-    x_load(0);
-    for (int i = 0; i < count; ++i) {
-      const int slot = i % L::PD;
+    load_xs(0);
+    for (int u = 0; u < units; ++u) {
+      const int slot = u % L::PD;
       // after a failure the loop runs on without waiting, so that every warp meets the same barriers
-      if (ok) ok = w4_wait(&wfull[slot], (i / L::PD) & 1, abort);
+      if (ok) ok = w4_wait(&wfull[slot], (u / L::PD) & 1, abort);
       const uint8_t* in = slots + slot * L::kSlot;
-      const uint4 w4 = *reinterpret_cast<const uint4*>(in + warp * 512 + lane * 16);
 #pragma unroll
-      for (int j = 0; j < SG; ++j)
+      for (int j = 0; j < SG; ++j) {
         sc_next[j] = __half2float(*reinterpret_cast<const __half*>(in + 8192 + my_n16 * (SG * 32) + j * 32 + my_s * 2));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&wempty[slot]);
-      // odd rows store their two pieces in the other order: eight lanes then fill all banks
-      const uint32_t a = sbase + (i % L::NS) * L::kStage + a_row;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int half = h ^ (r & 1);
-        uint32_t b0[4], b1[4];
-        unpack_w4<BF16>(half ? w4.z : w4.x, b0);
-        unpack_w4<BF16>(half ? w4.w : w4.y, b1);
-        const uint32_t at = a + (uint32_t)(((half * 4 + c) ^ r) << 4);
-        st_shared_v4(at, b0[0], b0[2], b1[0], b1[2]);
-        st_shared_v4(at + 1024, b0[1], b0[3], b1[1], b1[3]);
+        if (I8) sc_next[j] *= 0.0625f;                   // the operand is 16 q
       }
-      x_finish(i);
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[i % L::NS]);
-      if (sizeof(TX) == 1 && p.xs_groups > 1) named_bar_sync(1, kTileWarps * 32);
-      if (i > 0) sums(i - 1);
+      // The stage's buffers are free: it holds NS / SPU >= 2 units, and the sums of the unit
+      // before the last were taken.
+#pragma unroll
+      for (int h = 0; h < SPU; ++h) {
+        const int i = u * SPU + h;
+        const uint32_t a = sbase + (i % L::NS) * L::kStage;
+        if constexpr (XB == 2) {
+          // warp: 16 rows x one 64-byte half of the stage, the half swapped in odd rows, so that
+          // eight lanes' 16-byte stores fill all banks
+          const int half = (warp & 1) ^ (r & 1);
+          const uint2 w = *reinterpret_cast<const uint2*>(in + (warp >> 1) * 1024 + h * 512 + lane * 16 + half * 8);
+          uint32_t b0[4], b1[4];
+          unpack_w4<BF16>(w.x, b0);
+          unpack_w4<BF16>(w.y, b1);
+          const uint32_t at = a + ((warp >> 1) * 16 + r) * 128 + (uint32_t)(((half * 4 + c) ^ r) << 4);
+          st_shared_v4(at, b0[0], b0[2], b1[0], b1[2]);
+          st_shared_v4(at + 1024, b0[1], b0[3], b1[1], b1[3]);
+        } else {
+          // warp: 16 rows x 64 inputs (bytes); a lane's eight inputs are half of a 16-byte piece
+          const uint4 w = *reinterpret_cast<const uint4*>(in + warp * 512 + lane * 16);
+          const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t lo[2], hi[2];
+            unpack_w4_bytes<E4M3>(word[2 * q], lo[0], hi[0]);
+            unpack_w4_bytes<E4M3>(word[2 * q + 1], lo[1], hi[1]);
+            const int piece = (warp & 1) * 4 + q * 2 + (c >> 1);
+            const uint32_t at = a + ((warp >> 1) * 16 + r) * 128 + (uint32_t)((piece ^ r) << 4) + (c & 1) * 8;
+            st_shared_v2(at, lo[0], lo[1]);
+            st_shared_v2(at + 1024, hi[0], hi[1]);
+          }
+        }
+        if (!p.x_tma) copy_x(i);
+        if (h == SPU - 1 && by_group) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (e * 512 + tid < SG * MT) xsc[(u % 3) * (SG * MT) + e * 512 + tid] = xs_reg[e];
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[i % L::NS]);
+      }
+      if (lane == 0) mbar_arrive(&wempty[slot]);
+      if (by_group) named_bar_sync(1, kTileWarps * 32);
+      load_xs(u + 1);
+      if (u > 0) sums(u - 1);
 #pragma unroll
       for (int j = 0; j < SG; ++j) sc[j] = sc_next[j];
-      x_issue(i + XD);                                   // the products of stage i - 1 are done
-      x_load(i + 1);
     }
-    if (count > 0 && ok) sums(count - 1);
-    cp_async_wait_all();
-    // the stage buffers are free: every product is done
-    float* red = reinterpret_cast<float*>(smem) + 32 * q4 + lane;
+    if (units > 0) sums(units - 1);
+    // every product is done: the stage buffers are free
     named_bar_sync(1, kTileWarps * 32);
+    float* red = reinterpret_cast<float*>(smem) + 32 * q4 + lane;
 #pragma unroll
     for (int i = 0; i < NC; ++i) red[(col0 + i) * 128] = acc[i];
   }
@@ -663,9 +807,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) w4_tile_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] *= s;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) store_y(p, m, n + e, v[e]);
+      store_y4(p, m, n, v);
     }
   }
   if (S > 1) cluster_sync_all();
@@ -690,32 +832,68 @@ int w4_sms() {
   return cache[dev];
 }
 
-template <typename TX, int NT, int GROUP>
-cudaError_t launch_rows(W4Params p, cudaStream_t st) {
+template <typename TX, int NT, int GROUP, bool XS>
+cudaError_t launch_rows_x(const W4Params& p, size_t smem, cudaStream_t st) {
   static bool done[64] = {false};
-  cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP>, done);
+  const cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP, XS>, done);
   if (e != cudaSuccess) return e;
-  const size_t fixed = RowRing<GROUP>::kBytes + RowPart<NT>::kBytes, limit = 232448;
-  const size_t x = (size_t)p.KB * 64 * sizeof(TX) * (size_t)p.M;
-  p.x_smem = fixed + x <= limit;
   const int tiles = (p.N + 15) / 16, sms = w4_sms();
-  return launch_k(w4_rows_kernel<TX, NT, GROUP>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowThreads),
-                  fixed + (p.x_smem ? x : 0), st, true, p);
+  return launch_k(w4_rows_kernel<TX, NT, GROUP, XS>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowThreads), smem,
+                  st, true, p);
+}
+template <typename TX, int NT, int GROUP>
+cudaError_t launch_rows(const W4Params& p, cudaStream_t st) {
+  const size_t fixed = RowSmem<NT, GROUP>::kFixed, limit = 232448;
+  const size_t x = (size_t)p.KB * 64 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M;
+  if (fixed + x <= limit) return launch_rows_x<TX, NT, GROUP, true>(p, fixed + x, st);
+  return launch_rows_x<TX, NT, GROUP, false>(p, fixed, st);
+}
+
+// The driver's tensor-map encoder, looked up once.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+// x as a 2-d tensor read in boxes of 128 bytes x `rows`; false where TMA cannot read it (base or rows
+// off 16 bytes).
+bool x_tensor_map(CUtensorMap* map, const W4Params& p, size_t xb, CUtensorMapDataType type, int rows) {
+  if ((reinterpret_cast<uintptr_t>(p.x) & 15) || (p.ldx * (int64_t)xb) % 16 != 0 || encode_tiled() == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.ldx * xb};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / xb), (cuuint32_t)rows}, one[2] = {1, 1};
+  return encode_tiled()(map, type, 2, const_cast<void*>(p.x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename TX, int MT, int GROUP>
 cudaError_t launch_tile(W4Params p, cudaStream_t st) {
+  using L = Tile<(int)sizeof(TX), MT, GROUP>;
   static bool done[64] = {false};
   cudaError_t e = allow_max_smem((const void*)w4_tile_kernel<TX, MT, GROUP>, done);
   if (e != cudaSuccess) return e;
-  const int nt = (p.N + 127) / 128, mt = (int)((p.M + MT - 1) / MT), stages = p.KB / 2, sms = w4_sms();
+  const int nt = (p.N + 127) / 128, mt = (int)((p.M + MT - 1) / MT), units = p.KB / 2, sms = w4_sms();
   int s = 1;
-  while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && stages >= 8 * s) s *= 2;
+  while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 8 * s) s *= 2;
   p.splits = s;
+  CUtensorMap map{};
+  const CUtensorMapDataType type = sizeof(TX) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : std::is_same<TX, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  p.x_tma = x_tensor_map(&map, p, sizeof(TX), type, MT);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(nt * s), (unsigned)mt);
   cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = Tile<MT, GROUP>::kSmem;
+  cfg.dynamicSmemBytes = L::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -724,7 +902,7 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, w4_tile_kernel<TX, MT, GROUP>, p);
+  return cudaLaunchKernelEx(&cfg, w4_tile_kernel<TX, MT, GROUP>, p, map);
 }
 
 template <typename TX, int GROUP>
@@ -833,6 +1011,7 @@ int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, in
   p.bias = bias;
   p.y = y;
   p.y_dtype = y_dtype;
+  p.y_vec = N % 4 == 0 && on(y, 4 * yb);
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (x_dtype == GLAD_DTYPE_F16) e = launch_w4<__half>(p, st);
