@@ -429,7 +429,7 @@ int glad_rms_norm_backward(const void* dy, int x_dtype, int64_t lddy, const void
  * consecutive inputs of a row. `tiles` and `scales` hold the weight in blocks:
  *   tiles  [ceil(N/16)][KB][32][4] u32, KB = 2 ceil(K / 128):
  *          word j of lane 4*r + c of block (t, kb) holds rows n = 16t + r and
- *          n + 8, inputs k = 64 kb + 32 (j >> 1) + 8 c + 4 (j & 1) + (0..3); nibble i
+ *          n + 8, inputs k = 64 kb + 16 j + 4 c + (0..3); nibble i
  *          (bits 4i..4i+3) is row n + 8 (i & 1), input k + 2 ((i >> 1) & 1) + (i >> 2);
  *          zero past N and K
  *   scales [ceil(N/16)][KB * 64 / group][8][2] f16: rows 16t + r and 16t + r + 8 of a

@@ -188,8 +188,8 @@ __device__ __forceinline__ void store_y4(const W4Params& p, int64_t m, int n, co
 // 128 and join their sums in warp order once a tile. Each warp streams its own units (1 KB of
 // weights and 128/GROUP * 32 bytes of scales) through a private shared-memory ring of
 // cp.async copies kRing - 1 units ahead, across tile borders, so about 48 KB are in flight on
-// an SM whatever the warps wait for. x is staged once in shared memory when it fits, in the form the
-// products take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
+// an SM whatever the warps wait for. x is staged once in shared memory, in the form the products
+// take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
 // a word's nibbles come apart). Rows past M read row M - 1: their sums are never stored.
 constexpr int kRowWarps = 16, kRing = 4;
 constexpr int kRowThreads = kRowWarps * 32;
@@ -243,7 +243,7 @@ __device__ __forceinline__ uint32_t w4_low16(uint32_t w) { return (w << 4) & 0xf
 __device__ __forceinline__ uint32_t w4_high16(uint32_t w) { return w & 0xf0f0f0f0u; }
 __device__ __forceinline__ uint32_t swap_mid(uint32_t v) { return __byte_perm(v, 0, 0x3120); }
 
-template <typename TX, int NT, int GROUP, bool XS>
+template <typename TX, int NT, int GROUP>
 __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
   using L = RowSmem<NT, GROUP>;
   constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
@@ -287,15 +287,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
     if constexpr (I8) return make_uint4(swap_mid(v.x), swap_mid(v.y), 0, 0);
     else return to_halves<TX>(v);
   };
-  if constexpr (XS) {
-    // [32-input block][row][32 inputs]: a warp's reads of eight rows are contiguous
+  {
+    // [32-input block][row][lane c of four][inputs 4c..4c+3, 16+4c..]: a warp's reads of eight rows are contiguous
     const int pieces = p.KB * 8 * M;
     for (int i = threadIdx.x; i < pieces; i += kRowThreads) {
       const int m = i / (p.KB * 8), k8 = i - m * (p.KB * 8);
       const uint4 v = staged(load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k8 * 8, p.K, p.x_fast));
-      uint8_t* dst = xs + (((k8 >> 2) * M + m) * 4 + (k8 & 3)) * XP;
-      if constexpr (I8) *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
-      else *reinterpret_cast<uint4*>(dst) = v;
+      uint8_t* dst = xs + (((k8 >> 2) * M + m) * 4 + (k8 & 1) * 2) * XP + ((k8 >> 1) & 1) * (XP / 2);
+      if constexpr (I8) {
+        *reinterpret_cast<uint32_t*>(dst) = v.x;
+        *reinterpret_cast<uint32_t*>(dst + XP) = v.y;
+      } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2*>(dst + XP) = make_uint2(v.z, v.w);
+      }
     }
     __syncthreads();
   }
@@ -331,17 +336,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
         uint4 x[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          if constexpr (XS) {
-            const uint8_t* src = xrow[j] + (4 * u + q) * xstep;
-            if constexpr (I8) {
-              const uint2 v = *reinterpret_cast<const uint2*>(src);
-              x[j] = make_uint4(v.x, v.y, 0, 0);
-            } else {
-              x[j] = *reinterpret_cast<const uint4*>(src);
-            }
+          const uint8_t* src = xrow[j] + (4 * u + q) * xstep;
+          if constexpr (I8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            x[j] = make_uint4(v.x, v.y, 0, 0);
           } else {
-            x[j] = staged(load_raw8<TX>(static_cast<const TX*>(p.x) + min(8 * j + r, M - 1) * p.ldx,
-                                        (4 * u + q) * 32 + 8 * c, p.K, p.x_fast));
+            x[j] = *reinterpret_cast<const uint4*>(src);
           }
         }
         if constexpr (I8) {
@@ -412,40 +412,48 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
 
 // ---- many rows: tcgen05 -----------------------------------------------------------------------
 // A block computes 128 output columns x MT rows; D[n, m] lives in tensor memory, n its lanes. The
-// inputs go in stages of 128 bytes a row (64 of 16 bits, 128 of 8 bits: one swizzle atom). A loader
-// thread brings the packed weights (bulk copies, PD units of 128 inputs ahead) and the x tile (TMA,
-// NS stages); 16 warps turn the weights into the A operand in shared memory, in x's own type: f16 or
-// bf16, int8 times 16, or e4m3, all exact; one thread issues the products. Every group of inputs has
-// an accumulator of its own (ND in rotation): the 16 warps read it back, scale it by s[n, g] (a
-// lane's own row: one value a thread) and add it to fp32 sums in registers, so the weights need no
-// rounding; that costs one multiply-add an output and group, at groups of 64 half of the
-// tensor core's time for them at fp16 rate. Blocks of a cluster split the inputs when there are fewer
-// tiles than SMs and join their sums through distributed shared memory in rank order.
-constexpr int kTileWarps = 16;
-constexpr int kTileThreads = (kTileWarps + 3) * 32;      // + the MMA warp + two loaders
-
+// inputs go in stages of 128 bytes a row (64 of 16 bits, 128 of 8 bits: one swizzle atom). Roles by
+// warp: one brings the packed weights (bulk copies, PD units of 128 inputs ahead), one the x tile
+// (TMA, NS stages ahead); two teams of four unpack the weights of alternate units, in x's own type:
+// f16 or bf16, int8 times 16, or e4m3, all exact, and store them in tensor memory as the A operand (a
+// warp's fragment order is the order of its 16x256b / 16x128b stores), so shared memory, whose
+// bandwidth bounded the same kernel with A in it, carries only x; two issue the products of
+// alternate groups. Every group of inputs has an accumulator of its own (ND in rotation): SW warps
+// read it back, scale it by s[n, g] (a lane's own row: one value a thread) and add it to fp32 sums in
+// registers, so the weights need no rounding; that costs one multiply-add an output and group, at
+// groups of 64 half of the tensor core's time for them at fp16 rate. Blocks of a cluster split the
+// inputs when there are fewer tiles than SMs, send their sums to the rows' owners through
+// distributed shared memory and add them in rank order.
 __device__ unsigned int g_w4_status;
 
 template <int XB, int MT, int GROUP>                     // XB: bytes of an input
 struct Tile {
   static constexpr int SPU = XB;                         // stages of a unit (128 inputs)
-  static constexpr int NS = MT == 256 ? 4 : 6;
-  static constexpr int PD = MT == 256 ? 2 : MT == 128 ? 3 : 6;
-  static constexpr int ND = MT == 256 ? 2 : 4;
+  static constexpr int NS = 8;                           // NS, PD, ND even: see the waits
+  static constexpr int PD = 4;
+  static constexpr int ND = MT == 128 ? 2 : 4;
   static constexpr int SG = 128 / GROUP;                 // groups of a unit
   static constexpr int SPG = GROUP * XB / 32;            // products (32 bytes of inputs) of a group
-  static constexpr int kA = 128 * 128, kB = MT * 128, kStage = kA + kB;
-  static constexpr int kSlot = 8192 + 8 * SG * 32;       // packed weights and scales of a unit
-  static constexpr int kXs = XB == 1 ? 3 * SG * MT * 4 : 0;   // x scales of three units
+  static constexpr int SW = MT == 128 ? 16 : 4;          // warps that take the sums
+  static constexpr int DW = 8;                           // warps that unpack
+  static constexpr int kThreads = (SW + DW + 4) * 32;
+  static constexpr int NC = MT * 4 / SW;                 // columns of a sums thread
+  static constexpr int kStage = MT * 128;                // x of a stage
+  static constexpr int kSlot = 8192;                     // packed weights of a unit
+  static constexpr int kXs = XB == 1 ? SW * SG * NC * 4 : 0;       // x scales of a unit, a copy a warp
   static constexpr int kSmem = NS * kStage + PD * kSlot + kXs + 512 + 1024;
-  static constexpr int kCols = ND * MT;
-  static_assert(MT * 128 * 4 <= NS * kStage, "the sums are joined in the stage buffers");
+  static constexpr int kACol = ND * MT;                  // first tensor-memory column of A: 32 a stage
+  static constexpr int kCols = ND * MT + NS * 32 <= 256 ? 256 : 512;
+  static_assert(ND * MT + NS * 32 <= kCols, "tensor memory");
+  static_assert(2 * MT * 512 <= NS * kStage, "the sums are sent and joined in the stage buffers");
   static_assert(kSmem <= 232448, "shared memory of one block");
-  static_assert((2 * NS + 2 * PD + 2 * ND) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 * NS + 2 * PD + 2 * ND + 1) * 8 + 8 <= 512, "barrier area");
 };
 
-__device__ __noinline__ bool w4_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
+// Wait for a phase, 2 s at most. The timer is read only after many tries: a read costs more than most waits.
+__device__ __forceinline__ bool w4_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  for (int i = 0; i < 1000; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   while (!*abort) {
     for (int i = 0; i < 64; ++i)
@@ -457,6 +465,9 @@ __device__ __noinline__ bool w4_wait(uint64_t* bar, uint32_t parity, volatile in
   }
   return false;
 }
+__device__ __forceinline__ bool w4_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_try_wait(bar, parity) || w4_wait_slow(bar, parity, abort);
+}
 
 // K-major operand with 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart, the 16-byte
 // piece i of row r at i ^ (r & 7).
@@ -464,15 +475,36 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) |
          ((uint64_t)2 << 61);
 }
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
+// D (+)= A (tensor memory) * B^T from a converged warp: 32 bytes of inputs.
+#define W4_MMA_TS(name, kind)                                                                                \
+  __device__ __forceinline__ void name(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) { \
+    asm volatile(                                                                                            \
+        "{\n\t.reg .pred p, e;\n\t"                                                                           \
+        "elect.sync _|e, 0xffffffff;\n\t"                                                                      \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                            \
+        "@e tcgen05.mma.cta_group::1.kind::" kind " [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),                        \
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)                                                              \
+        : "memory");                                                                                         \
+  }
+W4_MMA_TS(mma_ts_f16, "f16")
+W4_MMA_TS(mma_ts_i8, "i8")
+W4_MMA_TS(mma_ts_f8, "f8f6f4")
+#undef W4_MMA_TS
+// 16 lanes x 32 (16) columns: thread 4g + q gives, of every 8 (4) columns, lane g's columns 2q, 2q + 1
+// (q) and the same of lane g + 8.
+__device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // x tile: 128 bytes of MT rows, zero outside the tensor, swizzled as desc_sw128 reads it.
 __device__ __forceinline__ void tma_x(uint32_t dst, const CUtensorMap* map, int k, int m, uint64_t* bar) {
   asm volatile(
@@ -483,14 +515,12 @@ __device__ __forceinline__ void tma_x(uint32_t dst, const CUtensorMap* map, int 
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ void st_shared_v2(uint32_t dst, uint32_t a, uint32_t b) {
-  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(a), "r"(b) : "memory");
-}
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+// Shared memory of this block -> the same or another block of the cluster; counted on the receiver's barrier.
+__device__ __forceinline__ void bulk_copy_s2c(uint32_t dst_cluster, uint32_t src, uint32_t bytes, uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_cluster),
+      "r"(src), "r"(bytes), "r"(bar_cluster)
+      : "memory");
 }
 
 // The eight weights of a word as bytes in the operand's type: lo = row r, hi = row r + 8, inputs
@@ -519,23 +549,25 @@ __device__ __forceinline__ void unpack_w4_bytes(uint32_t w, uint32_t& lo, uint32
 }
 
 template <typename TX, int MT, int GROUP>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     w4_tile_kernel(const __grid_constant__ W4Params p, const __grid_constant__ CUtensorMap xmap) {
   using L = Tile<(int)sizeof(TX), MT, GROUP>;
   constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
   constexpr bool E4M3 = std::is_same<TX, e4m3_t>::value;
-  constexpr int XB = (int)sizeof(TX), SG = L::SG, SPU = L::SPU, NC = MT / 4, KS = 128 / XB;   // KS: inputs of a stage
+  constexpr int XB = (int)sizeof(TX), SG = L::SG, SPU = L::SPU, NC = L::NC, KS = 128 / XB;   // KS: inputs of a stage
+  constexpr int SW = L::SW, DW = L::DW, CTL = SW + DW;   // first control warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* slots = smem + L::NS * L::kStage;
   float* xsc = reinterpret_cast<float*>(slots + L::PD * L::kSlot);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xsc) + L::kXs);   // [NS] operands written
-  uint64_t* empty = full + L::NS;                                                           // [NS] products done
-  uint64_t* wfull = empty + L::NS;                                                          // [PD]
-  uint64_t* wempty = wfull + L::PD;                                                         // [PD]
-  uint64_t* dfull = wempty + L::PD;                                                         // [ND]
-  uint64_t* dempty = dfull + L::ND;                                                         // [ND]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dempty + L::ND);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xsc) + L::kXs);
+  uint64_t* empty = full + L::NS;                        // [NS] products done; full: operands written
+  uint64_t* wfull = empty + L::NS;                       // [PD]
+  uint64_t* wempty = wfull + L::PD;                      // [PD]
+  uint64_t* dfull = wempty + L::PD;                      // [ND]
+  uint64_t* dempty = dfull + L::ND;                      // [ND]
+  uint64_t* joined = dempty + L::ND;                     // sums of the cluster's other blocks are here
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -546,25 +578,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int units = un1 - un0;
   const int live16 = min(8, (p.N + 15) / 16 - nt * 8);   // 16-column tiles that exist
 
-  if (warp == kTileWarps) tmem_alloc(tmem_slot, L::kCols);
+  if (warp == CTL) tmem_alloc(tmem_slot, L::kCols);
   if (tid == 0) {
     for (int i = 0; i < L::NS; ++i) {
-      mbar_init(&full[i], kTileWarps + (p.x_tma ? 1 : 0));
-      mbar_init(&empty[i], 1);
+      mbar_init(&full[i], 4 + (p.x_tma ? 1 : 0));
+      mbar_init(&empty[i], L::SPG < 4 ? 2 : 1);
     }
     for (int i = 0; i < L::PD; ++i) {
       mbar_init(&wfull[i], 1);
-      mbar_init(&wempty[i], kTileWarps);
+      mbar_init(&wempty[i], 4);
     }
     for (int i = 0; i < L::ND; ++i) {
       mbar_init(&dfull[i], 1);
-      mbar_init(&dempty[i], kTileWarps);
+      mbar_init(&dempty[i], SW);
     }
+    mbar_init(joined, 1);
     fence_mbar_init();
     *abort = 0;
   }
   if (live16 < 8) {                                      // columns past the weight: zeros that nothing overwrites
-    for (int i = tid; i < L::PD * L::kSlot / 16; i += kTileThreads)
+    for (int i = tid; i < L::PD * L::kSlot / 16; i += L::kThreads)
       reinterpret_cast<uint4*>(slots)[i] = make_uint4(0, 0, 0, 0);
     fence_async_smem();
   }
@@ -575,90 +608,80 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   grid_dep_wait();
   grid_dep_launch();
 
-  if (warp == kTileWarps + 1) {
-    // ---- packed weights and scales
-    if (lane == 0) {
-      const uint8_t* wsrc = reinterpret_cast<const uint8_t*>(p.tiles);
-      const uint8_t* ssrc = reinterpret_cast<const uint8_t*>(p.scales);
+  if (warp >= CTL) {
+    if (warp == CTL + 2) {
+      // ---- packed weights, one lane a 16-column tile
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.tiles) + (((int64_t)nt * 8 + lane) * U + un0) * 1024;
       int i = 0;
-      for (; i < units; ++i) {
+      for (; i < units; ++i, src += 1024) {
         const int slot = i % L::PD;
-        if (i >= L::PD && !w4_wait(&wempty[slot], (i / L::PD - 1) & 1, abort)) break;
-        uint8_t* dst = slots + slot * L::kSlot;
-        mbar_arrive_expect_tx(&wfull[slot], (uint32_t)live16 * (1024 + SG * 32));
-        for (int b = 0; b < live16; ++b) {
-          const int64_t at = ((int64_t)nt * 8 + b) * U + un0 + i;
-          bulk_copy_g2s(dst + b * 1024, wsrc + at * 1024, 1024, &wfull[slot]);
-          bulk_copy_g2s(dst + 8192 + b * (SG * 32), ssrc + at * (SG * 32), SG * 32, &wfull[slot]);
-        }
+        if (i >= L::PD && !__all_sync(0xffffffffu, w4_wait(&wempty[slot], (i / L::PD - 1) & 1, abort))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&wfull[slot], (uint32_t)live16 * 1024);
+        __syncwarp();
+        if (lane < live16) bulk_copy_g2s(slots + slot * L::kSlot + lane * 1024, src, 1024, &wfull[slot]);
       }
       // after a failure: copies that were issued land before the block leaves
       for (int k = max(0, i - L::PD); k < i && *abort; ++k) mbar_wait_bounded(&wfull[k % L::PD], (k / L::PD) & 1);
-    }
-  } else if (warp == kTileWarps + 2) {
-    // ---- x tiles
-    if (lane == 0 && p.x_tma) {
-      const uint32_t base = smem_u32(smem);
-      const int stages = units * SPU;
-      int i = 0;
-      for (; i < stages; ++i) {
-        const int st = i % L::NS;
-        if (i >= L::NS && !w4_wait(&empty[st], (i / L::NS - 1) & 1, abort)) break;
-        mbar_arrive_expect_tx(&full[st], L::kB);
-        tma_x(base + st * L::kStage + L::kA, &xmap, un0 * 128 + i * KS, (int)m0, &full[st]);
+    } else if (warp == CTL + 3) {
+      // ---- x tiles
+      if (lane == 0 && p.x_tma) {
+        const uint32_t base = smem_u32(smem);
+        const int stages = units * SPU;
+        int i = 0;
+        for (; i < stages; ++i) {
+          const int st = i % L::NS;
+          if (i >= L::NS && !w4_wait(&empty[st], (i / L::NS - 1) & 1, abort)) break;
+          mbar_arrive_expect_tx(&full[st], L::kStage);
+          tma_x(base + st * L::kStage, &xmap, un0 * 128 + i * KS, (int)m0, &full[st]);
+        }
+        for (int k = max(0, i - L::NS); k < i && *abort; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1);
       }
-      for (int k = max(0, i - L::NS); k < i && *abort; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1);
-    }
-  } else if (warp == kTileWarps) {
-    // ---- products
-    if (lane == 0) {
+    } else {
+      // ---- products of every second group. Each barrier's phases are all met by the warps that wait on
+      // it: a stage holds one group or a part (its buffer is always the same warp's, NS and ND being
+      // even) or several (both warps wait for it).
       constexpr uint32_t idesc = I8 ? idesc_i8(128, MT) : idesc_f16(128, MT) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t base = smem_u32(smem);
-      const int stages = units * SPU;
-      int gi = 0;                                        // groups begun
+      const int stages = units * SPU, me = warp - CTL;
       bool ok = true;
       for (int i = 0; ok && i < stages; ++i) {
-        if (!(ok = w4_wait(&full[i % L::NS], (i / L::NS) & 1, abort))) break;
+        if (L::SPG >= 4 && ((i * 4 / L::SPG) & 1) != me) continue;
+        ok = __all_sync(0xffffffffu, w4_wait(&full[i % L::NS], (i / L::NS) & 1, abort));
         tc_fence_after();
-        const uint64_t a = desc_sw128(base + (i % L::NS) * L::kStage);
-        const uint64_t b = desc_sw128(base + (i % L::NS) * L::kStage + L::kA);
+        const uint32_t a = tmem + L::kACol + (i % L::NS) * 32;
+        const uint64_t b = desc_sw128(base + (i % L::NS) * L::kStage);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {                    // 32 bytes of inputs
-          const int in_group = (i * 4 + q) % L::SPG;
-          if (in_group == 0) {
-            if (gi >= L::ND && !(ok = w4_wait(&dempty[gi % L::ND], (gi / L::ND - 1) & 1, abort))) break;
+          const int in_group = (i * 4 + q) % L::SPG, gi = (i * 4 + q) / L::SPG, d = gi % L::ND;
+          if (L::SPG < 4 && (gi & 1) != me) continue;
+          if (in_group == 0 && gi >= L::ND) {
+            if (ok) ok = __all_sync(0xffffffffu, w4_wait(&dempty[d], (gi / L::ND - 1) & 1, abort));
             tc_fence_after();
-            ++gi;
           }
-          const uint32_t d = tmem + ((gi - 1) % L::ND) * MT;
-          if constexpr (I8) mma_i8(d, a + 2 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
-          else if constexpr (E4M3) mma_f8(d, a + 2 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
-          else mma_f16(d, a + 2 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
-          if (in_group == L::SPG - 1) mma_commit(&dfull[(gi - 1) % L::ND]);
+          if (ok) {
+            if constexpr (I8) mma_ts_i8(tmem + d * MT, a + 8 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
+            else if constexpr (E4M3) mma_ts_f8(tmem + d * MT, a + 8 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
+            else mma_ts_f16(tmem + d * MT, a + 8 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
+            if (in_group == L::SPG - 1) mma_commit_warp(&dfull[d]);
+          }
         }
-        if (ok) mma_commit(&empty[i % L::NS]);
+        if (ok) mma_commit_warp(&empty[i % L::NS]);
       }
       // after a failure: products that were issued end before their operands go
-      for (int k = max(0, gi - L::ND); k < gi && *abort; ++k) mbar_wait_bounded(&dfull[k % L::ND], (k / L::ND) & 1);
+      if (*abort)
+        for (int d = 0; d < L::ND; ++d) mbar_wait_bounded(&dfull[d], 0, 10000000ull);
     }
-  } else {
-    // ---- operands, sums
-    const int r = lane >> 2, c = lane & 3, q4 = warp & 3, col0 = (warp >> 2) * NC;
+  } else if (warp >= SW) {
+    // ---- A operand
+    const int dw = warp & 3;                             // SW is a multiple of four: also the lane quarter
     const uint32_t sbase = smem_u32(smem);
-    const int my_n16 = q4 * 2 + (lane >> 4), my_s = (lane & 7) * 2 + ((lane >> 3) & 1);
-    const bool by_group = XB == 1 && p.xs_groups > 1;
-    float acc[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
-    float sc[SG], sc_next[SG];
-    float xs_reg[2] = {0.0f, 0.0f};
     bool ok = true;
 
     // x that TMA cannot read (rows off 16 bytes): stage i by guarded loads
     auto copy_x = [&](int i) {
-      const uint32_t b = sbase + (i % L::NS) * L::kStage + L::kA;
+      const uint32_t b = sbase + (i % L::NS) * L::kStage;
 #pragma unroll 1
-      for (int id = tid; id < MT * 8; id += kTileWarps * 32) {
+      for (int id = dw * 32 + lane; id < MT * 8; id += 128) {
         const int row = id >> 3, piece = id & 7;
         const int k = un0 * 128 + i * KS + piece * (16 / XB);
         const int64_t m = m0 + row;
@@ -674,134 +697,179 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         st_shared_v4(b + row * 128 + ((piece ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
       }
     };
-    auto load_xs = [&](int u) {                          // x scales of unit u into registers
-      if (by_group && u < units) {
+    for (int u = (warp - SW) >> 2; u < units; u += 2) {    // PD, NS even: a team meets all phases of its slots
+      const int slot = u % L::PD;
+      if (ok) ok = w4_wait(&wfull[slot], (u / L::PD) & 1, abort);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int id = e * 512 + tid, g = id / MT;
-          const int64_t m = m0 + id % MT;
+      for (int h = 0; h < SPU; ++h) {
+        const int i = u * SPU + h;
+        if (ok && i >= L::NS) ok = w4_wait(&empty[i % L::NS], (i / L::NS - 1) & 1, abort);
+      }
+      if (!ok) break;
+      tc_fence_after();
+      const uint8_t* in = slots + slot * L::kSlot;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n16 = dw * 2 + (e & 1), kb = e >> 1;   // 16 rows x 64 inputs
+        const uint4 w = *reinterpret_cast<const uint4*>(in + n16 * 1024 + kb * 512 + lane * 16);
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t at = tmem + ((uint32_t)(16 * n16) << 16) + L::kACol;
+        if constexpr (XB == 2) {
+          uint32_t v[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {                  // 16 inputs: (row r: 2 registers) (row r + 8: 2)
+            uint32_t a[4];
+            unpack_w4<BF16>(word[j], a);
+            v[4 * j] = a[0], v[4 * j + 1] = a[2], v[4 * j + 2] = a[1], v[4 * j + 3] = a[3];
+          }
+          tmem_st_16x256b_x4(at + ((u * 2 + kb) % L::NS) * 32, v);
+        } else {
+          uint32_t v[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) unpack_w4_bytes<E4M3>(word[j], v[2 * j], v[2 * j + 1]);
+          tmem_st_16x128b_x4(at + (u % L::NS) * 32 + kb * 16, v);
+        }
+      }
+      if (!p.x_tma) {
+#pragma unroll
+        for (int h = 0; h < SPU; ++h) copy_x(u * SPU + h);
+        fence_async_smem();
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&wempty[slot]);
+#pragma unroll
+        for (int h = 0; h < SPU; ++h) mbar_arrive(&full[(u * SPU + h) % L::NS]);
+      }
+    }
+  } else {
+    // ---- sums
+    const int q4 = warp & 3, col0 = (warp >> 2) * NC;
+    const bool by_group = XB == 1 && p.xs_groups > 1;
+    const bool row_live = q4 * 2 + (lane >> 4) < live16;
+    // this thread's row of the weight scales
+    const __half* sp = p.scales + (((int64_t)nt * 8 + q4 * 2 + (lane >> 4)) * U + un0) * (SG * 16) + (lane & 7) * 2 +
+                       ((lane >> 3) & 1);
+    constexpr int XN = XB == 1 ? SG * NC / 32 : 1;       // x scales of a unit a lane fetches
+    float* my_xs = xsc + warp * (SG * NC);
+    float acc[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
+    __half s_next[SG], s_after[SG];
+    float xs_next[XN];
+    bool ok = true;
+    auto load_s = [&](int u, __half (&s)[SG]) {
+#pragma unroll
+      for (int j = 0; j < SG; ++j) s[j] = (u < units && row_live) ? sp[(u * SG + j) * 16] : __half(0.0f);
+    };
+    auto load_xs = [&](int u) {
+      if constexpr (XB == 1) {
+#pragma unroll
+        for (int e = 0; e < XN; ++e) {
+          const int id = e * 32 + lane, g = id / NC;
+          const int64_t m = m0 + col0 + id % NC;
           const int xg = (un0 + u) * SG + g;
-          xs_reg[e] = (g < SG && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
+          xs_next[e] = (by_group && u < units && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
         }
       }
     };
-    auto sums = [&](int u) {                             // add the groups of unit u
+    load_s(0, s_next);
+    load_s(1, s_after);
+    load_xs(0);
+    for (int u = 0; ok && u < units; ++u) {
+      float sc[SG];
+#pragma unroll
+      for (int j = 0; j < SG; ++j) {
+        sc[j] = __half2float(s_next[j]) * (I8 ? 0.0625f : 1.0f);   // the int8 operand is 16 q
+        s_next[j] = s_after[j];
+      }
+      load_s(u + 2, s_after);
+      if constexpr (XB == 1) {
+        if (by_group) {
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < XN; ++e) my_xs[e * 32 + lane] = xs_next[e];
+          __syncwarp();
+          load_xs(u + 1);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
         const int gi = u * SG + j, d = gi % L::ND;
         if (ok) ok = w4_wait(&dfull[d], (gi / L::ND) & 1, abort);
-        if (!ok) return;
         tc_fence_after();
-        constexpr int CH = NC < 16 ? NC : 16;
+        // one piece of 16 columns is read while the one before is added, where registers allow it
+        constexpr int CH = 16, PIECES = NC / CH, AHEAD = MT == 128 ? 0 : 1;
+        const uint32_t at = tmem + ((uint32_t)(32 * q4) << 16) + d * MT + col0;
+        uint32_t v[AHEAD + 1][CH];
+        if (AHEAD) tmem_ld16(at, v[0]);
 #pragma unroll
-        for (int cb = 0; cb < NC; cb += CH) {
-          uint32_t v[CH];
-          const uint32_t at = tmem + ((uint32_t)(32 * q4) << 16) + d * MT + col0 + cb;
-          if constexpr (CH == 16) tmem_ld16(at, v);
-          else tmem_ld8(at, v);
+        for (int k = 0; k < PIECES; ++k) {
+          if (!AHEAD) tmem_ld16(at + k * CH, v[0]);
           tmem_ld_wait();
-          float f[CH];
+          if (AHEAD && k + 1 < PIECES) tmem_ld16(at + (k + 1) * CH, v[(k + 1) & AHEAD]);
+          uint32_t (&w)[CH] = v[k & AHEAD];
+          if constexpr (XB == 1) {
 #pragma unroll
-          for (int e = 0; e < CH; ++e) f[e] = I8 ? i2f_small((int)v[e]) : __uint_as_float(v[e]);   // |int| < 2^22
-          if (by_group) {
-            const float4* xv = reinterpret_cast<const float4*>(xsc + (u % 3) * (SG * MT) + j * MT + col0 + cb);
+            for (int e = 0; e < CH; ++e)
+              if (I8) w[e] = __float_as_uint(i2f_small((int)w[e]));      // |int| < 2^22
+            if (by_group) {
+              const float4* xv = reinterpret_cast<const float4*>(my_xs + j * NC + k * CH);
 #pragma unroll
-            for (int e = 0; e < CH; e += 4) {
-              const float4 x = xv[e / 4];
-              f[e] *= x.x, f[e + 1] *= x.y, f[e + 2] *= x.z, f[e + 3] *= x.w;
+              for (int e = 0; e < CH; e += 4) {
+                const float4 x = xv[e / 4];
+                w[e] = __float_as_uint(__uint_as_float(w[e]) * x.x);
+                w[e + 1] = __float_as_uint(__uint_as_float(w[e + 1]) * x.y);
+                w[e + 2] = __float_as_uint(__uint_as_float(w[e + 2]) * x.z);
+                w[e + 3] = __float_as_uint(__uint_as_float(w[e + 3]) * x.w);
+              }
             }
           }
 #pragma unroll
-          for (int e = 0; e < CH; ++e) acc[cb + e] = fmaf(sc[j], f[e], acc[cb + e]);
+          for (int e = 0; e < CH; ++e) acc[k * CH + e] = fmaf(sc[j], __uint_as_float(w[e]), acc[k * CH + e]);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&dempty[d]);
       }
-    };
-
-    load_xs(0);
-    for (int u = 0; u < units; ++u) {
-      const int slot = u % L::PD;
-      // after a failure the loop runs on without waiting, so that every warp meets the same barriers
-      if (ok) ok = w4_wait(&wfull[slot], (u / L::PD) & 1, abort);
-      const uint8_t* in = slots + slot * L::kSlot;
-#pragma unroll
-      for (int j = 0; j < SG; ++j) {
-        sc_next[j] = __half2float(*reinterpret_cast<const __half*>(in + 8192 + my_n16 * (SG * 32) + j * 32 + my_s * 2));
-        if (I8) sc_next[j] *= 0.0625f;                   // the operand is 16 q
-      }
-      // The stage's buffers are free: it holds NS / SPU >= 2 units, and the sums of the unit
-      // before the last were taken.
-#pragma unroll
-      for (int h = 0; h < SPU; ++h) {
-        const int i = u * SPU + h;
-        const uint32_t a = sbase + (i % L::NS) * L::kStage;
-        if constexpr (XB == 2) {
-          // warp: 16 rows x one 64-byte half of the stage, the half swapped in odd rows, so that
-          // eight lanes' 16-byte stores fill all banks
-          const int half = (warp & 1) ^ (r & 1);
-          const uint2 w = *reinterpret_cast<const uint2*>(in + (warp >> 1) * 1024 + h * 512 + lane * 16 + half * 8);
-          uint32_t b0[4], b1[4];
-          unpack_w4<BF16>(w.x, b0);
-          unpack_w4<BF16>(w.y, b1);
-          const uint32_t at = a + ((warp >> 1) * 16 + r) * 128 + (uint32_t)(((half * 4 + c) ^ r) << 4);
-          st_shared_v4(at, b0[0], b0[2], b1[0], b1[2]);
-          st_shared_v4(at + 1024, b0[1], b0[3], b1[1], b1[3]);
-        } else {
-          // warp: 16 rows x 64 inputs (bytes); a lane's eight inputs are half of a 16-byte piece
-          const uint4 w = *reinterpret_cast<const uint4*>(in + warp * 512 + lane * 16);
-          const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t lo[2], hi[2];
-            unpack_w4_bytes<E4M3>(word[2 * q], lo[0], hi[0]);
-            unpack_w4_bytes<E4M3>(word[2 * q + 1], lo[1], hi[1]);
-            const int piece = (warp & 1) * 4 + q * 2 + (c >> 1);
-            const uint32_t at = a + ((warp >> 1) * 16 + r) * 128 + (uint32_t)((piece ^ r) << 4) + (c & 1) * 8;
-            st_shared_v2(at, lo[0], lo[1]);
-            st_shared_v2(at + 1024, hi[0], hi[1]);
-          }
-        }
-        if (!p.x_tma) copy_x(i);
-        if (h == SPU - 1 && by_group) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (e * 512 + tid < SG * MT) xsc[(u % 3) * (SG * MT) + e * 512 + tid] = xs_reg[e];
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[i % L::NS]);
-      }
-      if (lane == 0) mbar_arrive(&wempty[slot]);
-      if (by_group) named_bar_sync(1, kTileWarps * 32);
-      load_xs(u + 1);
-      if (u > 0) sums(u - 1);
-#pragma unroll
-      for (int j = 0; j < SG; ++j) sc[j] = sc_next[j];
     }
-    if (units > 0) sums(units - 1);
-    // every product is done: the stage buffers are free
-    named_bar_sync(1, kTileWarps * 32);
-    float* red = reinterpret_cast<float*>(smem) + 32 * q4 + lane;
+    // every product is done, so the stage buffers are free: [m][n]
+    float* mine = reinterpret_cast<float*>(smem) + 32 * q4 + lane;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) red[(col0 + i) * 128] = acc[i];
+    for (int i = 0; i < NC; ++i) mine[(col0 + i) * 128] = acc[i];
+    if (S > 1) fence_async_smem();
   }
-  __syncthreads();
-  if (S > 1) cluster_sync_all();
-  if (warp < kTileWarps && !*abort) {
-    const int rows = MT / S;
-    const uint32_t red = smem_u32(smem) + lane * 16;
+  __syncwarp();
+  // Rows m of rank k's share are contiguous: one copy a receiver, into [source rank][m of the owner][n]
+  // behind the sums, once every block of the cluster has left its stage buffers.
+  const int own = MT / S;
+  const float* sums = reinterpret_cast<const float*>(smem) + lane * 4;
+  if (S > 1) {
+    cluster_sync_all();
+    sums += MT * 128;
+    if (tid == 0) mbar_arrive_expect_tx(joined, MT * 512);
+    if (tid < S)
+      bulk_copy_s2c(mapa_shared(smem_u32(smem) + (MT + rank * own) * 512, tid), smem_u32(smem) + tid * own * 512, own * 512,
+                    mapa_shared(smem_u32(joined), tid));
+    if (!w4_wait(joined, 0, abort)) mbar_wait_bounded(joined, 0);
+  } else {
+    __syncthreads();
+  }
+  if (!*abort) {
     const int n = nt * 128 + 4 * lane;
-    for (int i = warp; i < rows; i += kTileWarps) {
-      const int row = rank * rows + i;
-      const int64_t m = m0 + row;
+    for (int i = warp; i < own; i += L::kThreads / 32) {
+      const int64_t m = m0 + rank * own + i;
       if (m >= p.M || n >= p.N) continue;
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int k = 0; k < S; ++k) {
-        const float4 f = ld_cluster_f4(S > 1 ? mapa_shared(red + row * 512, k) : red + row * 512);
-        v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-      }
+      float4 f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < S) f[k] = *reinterpret_cast<const float4*>(sums + (k * own + i) * 128);
+      float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
+#pragma unroll
+      for (int k = 1; k < 8; ++k)
+        if (k < S) v[0] += f[k].x, v[1] += f[k].y, v[2] += f[k].z, v[3] += f[k].w;
       if (p.xs != nullptr && p.xs_groups <= 1) {
         const float s = p.xs[p.xs_rows ? m : 0];
 #pragma unroll
@@ -810,10 +878,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       store_y4(p, m, n, v);
     }
   }
-  if (S > 1) cluster_sync_all();
+  if (S > 1) cluster_sync_all();                         // the others have received what this block sent
   tc_fence_before();
   __syncthreads();
-  if (warp == kTileWarps) {
+  if (warp == CTL) {
     tc_fence_after();
     tmem_dealloc(tmem, L::kCols);
   }
@@ -832,21 +900,14 @@ int w4_sms() {
   return cache[dev];
 }
 
-template <typename TX, int NT, int GROUP, bool XS>
-cudaError_t launch_rows_x(const W4Params& p, size_t smem, cudaStream_t st) {
+template <typename TX, int NT, int GROUP>
+cudaError_t launch_rows(const W4Params& p, size_t x_bytes, cudaStream_t st) {
   static bool done[64] = {false};
-  const cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP, XS>, done);
+  const cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP>, done);
   if (e != cudaSuccess) return e;
   const int tiles = (p.N + 15) / 16, sms = w4_sms();
-  return launch_k(w4_rows_kernel<TX, NT, GROUP, XS>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowThreads), smem,
-                  st, true, p);
-}
-template <typename TX, int NT, int GROUP>
-cudaError_t launch_rows(const W4Params& p, cudaStream_t st) {
-  const size_t fixed = RowSmem<NT, GROUP>::kFixed, limit = 232448;
-  const size_t x = (size_t)p.KB * 64 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M;
-  if (fixed + x <= limit) return launch_rows_x<TX, NT, GROUP, true>(p, fixed + x, st);
-  return launch_rows_x<TX, NT, GROUP, false>(p, fixed, st);
+  return launch_k(w4_rows_kernel<TX, NT, GROUP>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowThreads),
+                  RowSmem<NT, GROUP>::kFixed + x_bytes, st, true, p);
 }
 
 // The driver's tensor-map encoder, looked up once.
@@ -867,8 +928,9 @@ EncodeTiled encode_tiled() {
 // x as a 2-d tensor read in boxes of 128 bytes x `rows`; false where TMA cannot read it (base or rows
 // off 16 bytes).
 bool x_tensor_map(CUtensorMap* map, const W4Params& p, size_t xb, CUtensorMapDataType type, int rows) {
-  if ((reinterpret_cast<uintptr_t>(p.x) & 15) || (p.ldx * (int64_t)xb) % 16 != 0 || encode_tiled() == nullptr) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.ldx * xb};
+  const int64_t pitch = p.M > 1 ? p.ldx * (int64_t)xb : (p.K * (int64_t)xb + 15) / 16 * 16;
+  if ((reinterpret_cast<uintptr_t>(p.x) & 15) || pitch % 16 != 0 || encode_tiled() == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)pitch};
   const cuuint32_t box[2] = {(cuuint32_t)(128 / xb), (cuuint32_t)rows}, one[2] = {1, 1};
   return encode_tiled()(map, type, 2, const_cast<void*>(p.x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -883,7 +945,7 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int nt = (p.N + 127) / 128, mt = (int)((p.M + MT - 1) / MT), units = p.KB / 2, sms = w4_sms();
   int s = 1;
-  while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 8 * s) s *= 2;
+  while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 4 * s) s *= 2;
   p.splits = s;
   CUtensorMap map{};
   const CUtensorMapDataType type = sizeof(TX) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
@@ -892,7 +954,7 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
   p.x_tma = x_tensor_map(&map, p, sizeof(TX), type, MT);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(nt * s), (unsigned)mt);
-  cfg.blockDim = dim3(kTileThreads);
+  cfg.blockDim = dim3(L::kThreads);
   cfg.dynamicSmemBytes = L::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -907,12 +969,13 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
 
 template <typename TX, int GROUP>
 cudaError_t launch_group(const W4Params& p, cudaStream_t st) {
-  if (p.M <= 8) return launch_rows<TX, 1, GROUP>(p, st);
-  if (p.M <= 16) return launch_rows<TX, 2, GROUP>(p, st);
+  // x in shared memory as the products take it
+  const size_t x = (size_t)p.KB * 64 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M, limit = 232448;
+  if (p.M <= 8 && RowSmem<1, GROUP>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP>(p, x, st);
+  if (p.M <= 16 && RowSmem<2, GROUP>::kFixed + x <= limit) return launch_rows<TX, 2, GROUP>(p, x, st);
   if (p.M <= 32) return launch_tile<TX, 32, GROUP>(p, st);
   if (p.M <= 64) return launch_tile<TX, 64, GROUP>(p, st);
-  if (p.M <= 128) return launch_tile<TX, 128, GROUP>(p, st);
-  return launch_tile<TX, 256, GROUP>(p, st);
+  return launch_tile<TX, 128, GROUP>(p, st);
 }
 template <typename TX>
 cudaError_t launch_w4(const W4Params& p, cudaStream_t st) {

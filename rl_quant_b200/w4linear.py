@@ -59,9 +59,9 @@ def pack_w4(packed: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4We
     q = torch.zeros(t * 16, kb * 64, dtype=torch.uint8, device=packed.device)
     q[:n, 0:k:2] = packed & 15
     q[:n, 1:k:2] = packed >> 4
-    # [t, row half, row, kb, j/2, c, j%2, k/2, k%2] -> byte (k/2 + 2 (k%2)) of word j, row half in the nibble
-    v = q.view(t, 2, 8, kb, 2, 4, 2, 2, 2)
-    b = (v[:, 0] | (v[:, 1] << 4)).permute(0, 2, 1, 4, 3, 5, 7, 6)
+    # [t, row half, row, kb, j, c, k/2, k%2] -> byte (k/2 + 2 (k%2)) of word j, row half in the nibble
+    v = q.view(t, 2, 8, kb, 4, 4, 2, 2)
+    b = (v[:, 0] | (v[:, 1] << 4)).permute(0, 2, 1, 4, 3, 6, 5)
     s = torch.zeros(t * 16, gp, dtype=torch.float16, device=scales.device)
     s[:n, :scales.shape[1]] = scales
     return W4Weight(b.reshape(t, kb, 512).contiguous(), s.view(t, 2, 8, gp).permute(0, 3, 2, 1).reshape(t, gp, 16).contiguous(),
@@ -72,7 +72,7 @@ def pack_w4(packed: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4We
 def unpack_w4(weight: W4Weight):
     """The inverse of ``pack_w4``: (packed, scales)."""
     t, kb, gp = _shapes(weight.in_features, weight.out_features, weight.group)
-    b = weight.tiles.view(t, kb, 8, 4, 2, 2, 2, 2).permute(0, 2, 1, 4, 3, 5, 7, 6)
+    b = weight.tiles.view(t, kb, 8, 4, 4, 2, 2).permute(0, 2, 1, 4, 3, 6, 5)
     q = torch.stack((b & 15, b >> 4), dim=1).reshape(t * 16, kb * 64)[:weight.out_features, :weight.in_features]
     packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
     g = -(-weight.in_features // weight.group)

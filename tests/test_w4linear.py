@@ -335,7 +335,7 @@ def test_layout(n, k, group):
                 for j in range(4):
                     for i in range(8):
                         row = 16 * t + r + 8 * (i & 1)
-                        col = 64 * kb + 32 * (j >> 1) + 8 * c + 4 * (j & 1) + 2 * ((i >> 1) & 1) + (i >> 2)
+                        col = 64 * kb + 16 * j + 4 * c + 2 * ((i >> 1) & 1) + (i >> 2)
                         v = (int(words[t, kb, lane, j]) >> (4 * i)) & 15
                         seen[row, col] = v - 16 if v > 7 else v
     assert np.array_equal(seen[:n, :k], q.numpy()) and not seen[n:].any() and not seen[:, k:].any()
