@@ -427,13 +427,12 @@ int glad_rms_norm_backward(const void* dy, int x_dtype, int64_t lddy, const void
  * y[m, n] = sum_g xs[m, g] * scales[n, g] * sum_{k in group g} x[m, k] * q[n, k] + bias[n]
  * with q int4 in [-8, 7] and one f16 scale for `group` (32, 64 or 128)
  * consecutive inputs of a row. `tiles` and `scales` hold the weight in blocks:
- *   tiles  [ceil(N/16)][KB][32][4] u32, KB = 2 ceil(K / 128):
- *          word j of lane 4*r + c of block (t, kb) holds rows n = 16t + r and
- *          n + 8, inputs k = 64 kb + 16 j + 4 c + (0..3); nibble i
- *          (bits 4i..4i+3) is row n + 8 (i & 1), input k + 2 ((i >> 1) & 1) + (i >> 2);
- *          zero past N and K
- *   scales [ceil(N/16)][KB * 64 / group][8][2] f16: rows 16t + r and 16t + r + 8 of a
- *          group side by side; zero past N and K
+ *   tiles  [ceil(N/128)][ceil(K/128)][8][2][32][4] u32: word j of lane 4*r + c of block
+ *          (t, u, b, kb) holds rows n = 128t + 16b + r and n + 8, inputs
+ *          k = 128u + 64kb + 16j + 4c + (0..3); nibble i (bits 4i..4i+3) is row
+ *          n + 8 (i & 1), input k + 2 ((i >> 1) & 1) + (i >> 2); zero past N and K
+ *   scales [ceil(N/128)][ceil(K/128)][8][128 / group][8][2] f16: rows 128t + 16b + r and
+ *          the same + 8 of a group side by side; zero past N and K
  * x [M, K] (row stride ldx elements): f16 or bf16 with x_scale NULL; i8 or e4m3
  * with x_scale f32: one for all rows (x_scale_rows 0), one a row (x_scale_groups
  * 1) or one a row and group (x_scale_groups = ceil(K / group), rows contiguous).

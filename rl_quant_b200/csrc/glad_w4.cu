@@ -1,8 +1,8 @@
 // Rows times 4-bit weights with group scales:
 //   y[m, n] = sum_g xs[m, g] * s[n, g] * sum_{k in group g} x[m, k] * q[n, k] + b[n]
 //
-// The weights are streamed once in the order the kernel reads them (include/glad_b200.h:
-// GladW4Weight), 512 contiguous bytes a warp load: 16 rows x 64 inputs. A 32-bit word is
+// The weights are streamed once in the order the kernels read them (include/glad_b200.h: GladW4Weight):
+// 8 KB for 128 rows x 128 inputs, in it 1 KB for 16 rows, 512 bytes a warp load: 16 rows x 64 inputs. A 32-bit word is
 // one lane's share of the A operand of a 16x8x16 tensor-core product, so a word becomes
 // four half2 registers with one logic operation and one half operation each:
 // 0x6400 | u is the half 1024 + u, exact for 4-bit u. Products q * x are exact and the sum of
@@ -25,7 +25,7 @@ namespace {
 struct W4Params {
   const uint4* tiles;
   const __half* scales;
-  int N, K, KB, group;      // KB: 64-input blocks, an even number
+  int N, K, U, group;       // U: units of 128 inputs
   const void* x;
   int64_t M, ldx;
   const float* xs;          // scales of 8-bit rows or null
@@ -252,28 +252,32 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
   float* part = reinterpret_cast<float*>(smem + L::kRingBytes);
   uint8_t* xs = smem + L::kFixed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int T = (p.N + 15) / 16, U = p.KB / 2, M = (int)p.M;
+  const int T = (p.N + 15) / 16, U = p.U, M = (int)p.M;
   const int u0 = (int)((int64_t)warp * U / kRowWarps), u1 = (int)((int64_t)(warp + 1) * U / kRowWarps);
   uint8_t* ring = smem + warp * (kRing * L::kWarpSlot);
 
   // the next unit to fetch: tile pt, unit pu
   int pt = u0 < u1 ? blockIdx.x : T, pu = u0;
-  const uint4* wsrc = p.tiles + ((int64_t)pt * U + pu) * 64 + lane;
-  const uint8_t* ssrc = reinterpret_cast<const uint8_t*>(p.scales) + ((int64_t)pt * U + pu) * (SG * 32) + lane * 16;
-  const int64_t skip = (int64_t)gridDim.x * U - (u1 - u0);   // units from the end of this tile's share to the next tile's
+  const uint4* wsrc = nullptr;
+  const uint8_t* ssrc = nullptr;
+  auto seek = [&]() {
+    const int64_t at = ((int64_t)(pt >> 3) * U + pu) * 8 + (pt & 7);   // 1 KB blocks
+    wsrc = p.tiles + at * 64 + lane;
+    ssrc = reinterpret_cast<const uint8_t*>(p.scales) + at * (SG * 32) + lane * 16;
+  };
+  seek();
   auto fetch = [&](int slot) {
     if (pt < T) {
       uint8_t* dst = ring + slot * L::kWarpSlot + lane * 16;
       cp_async16(dst, wsrc);
       cp_async16(dst + 512, wsrc + 32);
       if (lane < SG * 2) cp_async16(dst + 1024, ssrc);
-      wsrc += 64;
-      ssrc += SG * 32;
+      wsrc += 8 * 64;
+      ssrc += 8 * SG * 32;
       if (++pu == u1) {
         pu = u0;
         pt += gridDim.x;
-        wsrc += skip * 64;
-        ssrc += skip * (SG * 32);
+        seek();
       }
     }
     cp_async_commit();
@@ -289,9 +293,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
   };
   {
     // [32-input block][row][lane c of four][inputs 4c..4c+3, 16+4c..]: a warp's reads of eight rows are contiguous
-    const int pieces = p.KB * 8 * M;
+    const int pieces = U * 16 * M;
     for (int i = threadIdx.x; i < pieces; i += kRowThreads) {
-      const int m = i / (p.KB * 8), k8 = i - m * (p.KB * 8);
+      const int m = i / (U * 16), k8 = i - m * (U * 16);
       const uint4 v = staged(load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k8 * 8, p.K, p.x_fast));
       uint8_t* dst = xs + (((k8 >> 2) * M + m) * 4 + (k8 & 1) * 2) * XP + ((k8 >> 1) & 1) * (XP / 2);
       if constexpr (I8) {
@@ -414,11 +418,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
 // A block computes 128 output columns x MT rows; D[n, m] lives in tensor memory, n its lanes. The
 // inputs go in stages of 128 bytes a row (64 of 16 bits, 128 of 8 bits: one swizzle atom). Roles by
 // warp: one brings the packed weights (bulk copies, PD units of 128 inputs ahead), one the x tile
-// (TMA, NS stages ahead); two teams of four unpack the weights of alternate units, in x's own type:
+// (TMA, NS stages ahead); teams of four unpack the weights of a unit each, in x's own type:
 // f16 or bf16, int8 times 16, or e4m3, all exact, and store them in tensor memory as the A operand (a
 // warp's fragment order is the order of its 16x256b / 16x128b stores), so shared memory, whose
-// bandwidth bounded the same kernel with A in it, carries only x; two issue the products of
-// alternate groups. Every group of inputs has an accumulator of its own (ND in rotation): SW warps
+// bandwidth bounded the same kernel with A in it, carries only x; MW issue the products of
+// groups in turn. Every group of inputs has an accumulator of its own (ND in rotation): SW warps
 // read it back, scale it by s[n, g] (a lane's own row: one value a thread) and add it to fp32 sums in
 // registers, so the weights need no rounding; that costs one multiply-add an output and group, at
 // groups of 64 half of the tensor core's time for them at fp16 rate. Blocks of a cluster split the
@@ -434,9 +438,10 @@ struct Tile {
   static constexpr int ND = MT == 128 ? 2 : 4;
   static constexpr int SG = 128 / GROUP;                 // groups of a unit
   static constexpr int SPG = GROUP * XB / 32;            // products (32 bytes of inputs) of a group
-  static constexpr int SW = MT == 128 ? 16 : 4;          // warps that take the sums
+  static constexpr int MW = MT == 128 ? 2 : 4;           // warps that issue products
+  static constexpr int SW = MT == 128 ? 16 : 8;          // warps that take the sums
   static constexpr int DW = 8;                           // warps that unpack
-  static constexpr int kThreads = (SW + DW + 4) * 32;
+  static constexpr int kThreads = (SW + DW + MW + 2) * 32;
   static constexpr int NC = MT * 4 / SW;                 // columns of a sums thread
   static constexpr int kStage = MT * 128;                // x of a stage
   static constexpr int kSlot = 8192;                     // packed weights of a unit
@@ -445,6 +450,7 @@ struct Tile {
   static constexpr int kACol = ND * MT;                  // first tensor-memory column of A: 32 a stage
   static constexpr int kCols = ND * MT + NS * 32 <= 256 ? 256 : 512;
   static_assert(ND * MT + NS * 32 <= kCols, "tensor memory");
+  static_assert(NS % (2 * MW) == 0 && ND % MW == 0 && PD % (DW / 4) == 0 && NS % (SPU * DW / 4) == 0, "phases");
   static_assert(2 * MT * 512 <= NS * kStage, "the sums are sent and joined in the stage buffers");
   static_assert(kSmem <= 232448, "shared memory of one block");
   static_assert((2 * NS + 2 * PD + 2 * ND + 1) * 8 + 8 <= 512, "barrier area");
@@ -496,13 +502,11 @@ __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_
   asm volatile(
       "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 __device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // x tile: 128 bytes of MT rows, zero outside the tensor, swizzled as desc_sw128 reads it.
@@ -515,6 +519,11 @@ __device__ __forceinline__ void tma_x(uint32_t dst, const CUtensorMap* map, int 
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// Cluster barrier in two halves, without ordering of memory accesses.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // Shared memory of this block -> the same or another block of the cluster; counted on the receiver's barrier.
 __device__ __forceinline__ void bulk_copy_s2c(uint32_t dst_cluster, uint32_t src, uint32_t bytes, uint32_t bar_cluster) {
   asm volatile(
@@ -574,15 +583,14 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   const int S = p.splits, rank = S > 1 ? (int)cluster_ctarank() : 0;
   const int nt = blockIdx.x / S;
   const int64_t m0 = (int64_t)blockIdx.y * MT;
-  const int U = p.KB / 2, un0 = (int)((int64_t)rank * U / S), un1 = (int)((int64_t)(rank + 1) * U / S);
+  const int U = p.U, un0 = (int)((int64_t)rank * U / S), un1 = (int)((int64_t)(rank + 1) * U / S);
   const int units = un1 - un0;
-  const int live16 = min(8, (p.N + 15) / 16 - nt * 8);   // 16-column tiles that exist
 
   if (warp == CTL) tmem_alloc(tmem_slot, L::kCols);
   if (tid == 0) {
     for (int i = 0; i < L::NS; ++i) {
       mbar_init(&full[i], 4 + (p.x_tma ? 1 : 0));
-      mbar_init(&empty[i], L::SPG < 4 ? 2 : 1);
+      mbar_init(&empty[i], L::SPG >= 4 ? 1 : 4 / L::SPG < L::MW ? 4 / L::SPG : L::MW);
     }
     for (int i = 0; i < L::PD; ++i) {
       mbar_init(&wfull[i], 1);
@@ -596,11 +604,6 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     fence_mbar_init();
     *abort = 0;
   }
-  if (live16 < 8) {                                      // columns past the weight: zeros that nothing overwrites
-    for (int i = tid; i < L::PD * L::kSlot / 16; i += L::kThreads)
-      reinterpret_cast<uint4*>(slots)[i] = make_uint4(0, 0, 0, 0);
-    fence_async_smem();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -609,20 +612,21 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   grid_dep_launch();
 
   if (warp >= CTL) {
-    if (warp == CTL + 2) {
-      // ---- packed weights, one lane a 16-column tile
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.tiles) + (((int64_t)nt * 8 + lane) * U + un0) * 1024;
-      int i = 0;
-      for (; i < units; ++i, src += 1024) {
-        const int slot = i % L::PD;
-        if (i >= L::PD && !__all_sync(0xffffffffu, w4_wait(&wempty[slot], (i / L::PD - 1) & 1, abort))) break;
-        if (lane == 0) mbar_arrive_expect_tx(&wfull[slot], (uint32_t)live16 * 1024);
-        __syncwarp();
-        if (lane < live16) bulk_copy_g2s(slots + slot * L::kSlot + lane * 1024, src, 1024, &wfull[slot]);
+    if (warp == CTL + L::MW) {
+      // ---- packed weights
+      if (lane == 0) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(p.tiles) + ((int64_t)nt * U + un0) * 8192;
+        int i = 0;
+        for (; i < units; ++i, src += 8192) {
+          const int slot = i % L::PD;
+          if (i >= L::PD && !w4_wait(&wempty[slot], (i / L::PD - 1) & 1, abort)) break;
+          mbar_arrive_expect_tx(&wfull[slot], 8192);
+          bulk_copy_g2s(slots + slot * L::kSlot, src, 8192, &wfull[slot]);
+        }
+        // after a failure: copies that were issued land before the block leaves
+        for (int k = max(0, i - L::PD); k < i && *abort; ++k) mbar_wait_bounded(&wfull[k % L::PD], (k / L::PD) & 1);
       }
-      // after a failure: copies that were issued land before the block leaves
-      for (int k = max(0, i - L::PD); k < i && *abort; ++k) mbar_wait_bounded(&wfull[k % L::PD], (k / L::PD) & 1);
-    } else if (warp == CTL + 3) {
+    } else if (warp == CTL + L::MW + 1) {
       // ---- x tiles
       if (lane == 0 && p.x_tma) {
         const uint32_t base = smem_u32(smem);
@@ -637,15 +641,17 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
         for (int k = max(0, i - L::NS); k < i && *abort; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1);
       }
     } else {
-      // ---- products of every second group. Each barrier's phases are all met by the warps that wait on
-      // it: a stage holds one group or a part (its buffer is always the same warp's, NS and ND being
-      // even) or several (both warps wait for it).
+      // ---- products of every MW-th group. A wait must meet every phase of its barrier (phases are told apart
+      // by parity alone): NS and ND being multiples of MW, a stage's and an accumulator's buffers are always
+      // the same warps'.
       constexpr uint32_t idesc = I8 ? idesc_i8(128, MT) : idesc_f16(128, MT) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t base = smem_u32(smem);
       const int stages = units * SPU, me = warp - CTL;
       bool ok = true;
       for (int i = 0; ok && i < stages; ++i) {
-        if (L::SPG >= 4 && ((i * 4 / L::SPG) & 1) != me) continue;
+        // the warps of a stage: its one group's, or those of its 4 / SPG groups
+        if (L::SPG >= 4 ? (i * 4 / L::SPG) % L::MW != me : (me - i * 4 / L::SPG % L::MW + L::MW) % L::MW >= 4 / L::SPG)
+          continue;
         ok = __all_sync(0xffffffffu, w4_wait(&full[i % L::NS], (i / L::NS) & 1, abort));
         tc_fence_after();
         const uint32_t a = tmem + L::kACol + (i % L::NS) * 32;
@@ -653,7 +659,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {                    // 32 bytes of inputs
           const int in_group = (i * 4 + q) % L::SPG, gi = (i * 4 + q) / L::SPG, d = gi % L::ND;
-          if (L::SPG < 4 && (gi & 1) != me) continue;
+          if (L::SPG < 4 && gi % L::MW != me) continue;
           if (in_group == 0 && gi >= L::ND) {
             if (ok) ok = __all_sync(0xffffffffu, w4_wait(&dempty[d], (gi / L::ND - 1) & 1, abort));
             tc_fence_after();
@@ -697,7 +703,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
         st_shared_v4(b + row * 128 + ((piece ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
       }
     };
-    for (int u = (warp - SW) >> 2; u < units; u += 2) {    // PD, NS even: a team meets all phases of its slots
+    for (int u = (warp - SW) >> 2; u < units; u += DW / 4) {   // a team meets all phases of its slots
       const int slot = u % L::PD;
       if (ok) ok = w4_wait(&wfull[slot], (u / L::PD) & 1, abort);
 #pragma unroll
@@ -708,10 +714,14 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const uint8_t* in = slots + slot * L::kSlot;
+      uint4 packed[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        packed[e] = *reinterpret_cast<const uint4*>(in + (dw * 2 + (e & 1)) * 1024 + (e >> 1) * 512 + lane * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int n16 = dw * 2 + (e & 1), kb = e >> 1;   // 16 rows x 64 inputs
-        const uint4 w = *reinterpret_cast<const uint4*>(in + n16 * 1024 + kb * 512 + lane * 16);
+        const uint4 w = packed[e];
         const uint32_t word[4] = {w.x, w.y, w.z, w.w};
         const uint32_t at = tmem + ((uint32_t)(16 * n16) << 16) + L::kACol;
         if constexpr (XB == 2) {
@@ -748,11 +758,10 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     // ---- sums
     const int q4 = warp & 3, col0 = (warp >> 2) * NC;
     const bool by_group = XB == 1 && p.xs_groups > 1;
-    const bool row_live = q4 * 2 + (lane >> 4) < live16;
     // this thread's row of the weight scales
-    const __half* sp = p.scales + (((int64_t)nt * 8 + q4 * 2 + (lane >> 4)) * U + un0) * (SG * 16) + (lane & 7) * 2 +
+    const __half* sp = p.scales + (((int64_t)nt * U + un0) * 8 + q4 * 2 + (lane >> 4)) * (SG * 16) + (lane & 7) * 2 +
                        ((lane >> 3) & 1);
-    constexpr int XN = XB == 1 ? SG * NC / 32 : 1;       // x scales of a unit a lane fetches
+    constexpr int XN = XB == 1 ? (SG * NC + 31) / 32 : 1;            // x scales of a unit a lane fetches
     float* my_xs = xsc + warp * (SG * NC);
     float acc[NC];
 #pragma unroll
@@ -762,7 +771,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     bool ok = true;
     auto load_s = [&](int u, __half (&s)[SG]) {
 #pragma unroll
-      for (int j = 0; j < SG; ++j) s[j] = (u < units && row_live) ? sp[(u * SG + j) * 16] : __half(0.0f);
+      for (int j = 0; j < SG; ++j) s[j] = u < units ? sp[(u * 8 * SG + j) * 16] : __half(0.0f);
     };
     auto load_xs = [&](int u) {
       if constexpr (XB == 1) {
@@ -771,7 +780,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
           const int id = e * 32 + lane, g = id / NC;
           const int64_t m = m0 + col0 + id % NC;
           const int xg = (un0 + u) * SG + g;
-          xs_next[e] = (by_group && u < units && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
+          xs_next[e] = (by_group && u < units && g < SG && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
         }
       }
     };
@@ -790,7 +799,8 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
         if (by_group) {
           __syncwarp();
 #pragma unroll
-          for (int e = 0; e < XN; ++e) my_xs[e * 32 + lane] = xs_next[e];
+          for (int e = 0; e < XN; ++e)
+            if (e * 32 + lane < SG * NC) my_xs[e * 32 + lane] = xs_next[e];
           __syncwarp();
           load_xs(u + 1);
         }
@@ -854,6 +864,8 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       bulk_copy_s2c(mapa_shared(smem_u32(smem) + (MT + rank * own) * 512, tid), smem_u32(smem) + tid * own * 512, own * 512,
                     mapa_shared(smem_u32(joined), tid));
     if (!w4_wait(joined, 0, abort)) mbar_wait_bounded(joined, 0);
+    __syncwarp();
+    cluster_arrive_relaxed();                            // this block has received all that is sent to it
   } else {
     __syncthreads();
   }
@@ -878,7 +890,8 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       store_y4(p, m, n, v);
     }
   }
-  if (S > 1) cluster_sync_all();                         // the others have received what this block sent
+  __syncwarp();
+  if (S > 1) cluster_wait();                             // the others have received what this block sent
   tc_fence_before();
   __syncthreads();
   if (warp == CTL) {
@@ -943,7 +956,7 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
   static bool done[64] = {false};
   cudaError_t e = allow_max_smem((const void*)w4_tile_kernel<TX, MT, GROUP>, done);
   if (e != cudaSuccess) return e;
-  const int nt = (p.N + 127) / 128, mt = (int)((p.M + MT - 1) / MT), units = p.KB / 2, sms = w4_sms();
+  const int nt = (p.N + 127) / 128, mt = (int)((p.M + MT - 1) / MT), units = p.U, sms = w4_sms();
   int s = 1;
   while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 4 * s) s *= 2;
   p.splits = s;
@@ -970,7 +983,7 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
 template <typename TX, int GROUP>
 cudaError_t launch_group(const W4Params& p, cudaStream_t st) {
   // x in shared memory as the products take it
-  const size_t x = (size_t)p.KB * 64 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M, limit = 232448;
+  const size_t x = (size_t)p.U * 128 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M, limit = 232448;
   if (p.M <= 8 && RowSmem<1, GROUP>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP>(p, x, st);
   if (p.M <= 16 && RowSmem<2, GROUP>::kFixed + x <= limit) return launch_rows<TX, 2, GROUP>(p, x, st);
   if (p.M <= 32) return launch_tile<TX, 32, GROUP>(p, st);
@@ -994,7 +1007,7 @@ bool shape_ok(int K, int N, int group) {
   return K >= 2 && K % 2 == 0 && K <= (1 << 20) && N >= 1 && N <= (1 << 20) &&
          (group == 32 || group == 64 || group == 128);
 }
-int64_t blocks64(int K) { return (int64_t)((K + 127) / 128) * 2; }
+int units(int K) { return (K + 127) / 128; }
 
 }  // namespace
 }  // namespace glad
@@ -1005,12 +1018,12 @@ extern "C" {
 
 size_t glad_w4_tiles_bytes(int in_features, int out_features, int group) {
   if (!shape_ok(in_features, out_features, group)) return 0;
-  return (size_t)((out_features + 15) / 16) * (size_t)blocks64(in_features) * 512;
+  return (size_t)((out_features + 127) / 128) * (size_t)units(in_features) * 8192;
 }
 
 size_t glad_w4_scales_bytes(int in_features, int out_features, int group) {
   if (!shape_ok(in_features, out_features, group)) return 0;
-  return (size_t)((out_features + 15) / 16) * (size_t)(blocks64(in_features) * 64 / group) * 32;
+  return (size_t)((out_features + 127) / 128) * (size_t)units(in_features) * 8 * (size_t)(128 / group) * 32;
 }
 
 int glad_w4_linear_status(uint32_t* status, void* stream) {
@@ -1062,7 +1075,7 @@ int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, in
   p.scales = static_cast<const __half*>(w->scales);
   p.N = N;
   p.K = K;
-  p.KB = (int)blocks64(K);
+  p.U = units(K);
   p.group = w->group;
   p.x = x;
   p.M = M;

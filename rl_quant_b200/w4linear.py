@@ -19,9 +19,9 @@ _OUT = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def _shapes(in_features: int, out_features: int, group: int):
-    """(row tiles, 64-input blocks, padded groups) of the laid-out weight."""
-    kb = -(-in_features // 128) * 2
-    return -(-out_features // 16), kb, kb * 64 // group
+    """Shapes of the laid-out weight: tiles (uint8), scales (fp16)."""
+    t, u = -(-out_features // 128), -(-in_features // 128)
+    return (t, u, 8192), (t, u, 8, 128 // group * 16)
 
 
 class W4Weight:
@@ -34,11 +34,11 @@ class W4Weight:
             raise ValueError(f"group must be one of {GROUPS}, got {group}")
         if in_features < 2 or in_features % 2:
             raise ValueError(f"in_features must be even, got {in_features}")
-        t, kb, gp = _shapes(in_features, out_features, group)
-        if tiles.dtype != torch.uint8 or tuple(tiles.shape) != (t, kb, 512) or not tiles.is_contiguous():
-            raise ValueError(f"tiles must be contiguous uint8 [{t}, {kb}, 512]")
-        if scales.dtype != torch.float16 or tuple(scales.shape) != (t, gp, 16) or not scales.is_contiguous():
-            raise ValueError(f"scales must be contiguous float16 [{t}, {gp}, 16]")
+        t_shape, s_shape = _shapes(in_features, out_features, group)
+        if tiles.dtype != torch.uint8 or tuple(tiles.shape) != t_shape or not tiles.is_contiguous():
+            raise ValueError(f"tiles must be contiguous uint8 {t_shape}")
+        if scales.dtype != torch.float16 or tuple(scales.shape) != s_shape or not scales.is_contiguous():
+            raise ValueError(f"scales must be contiguous float16 {s_shape}")
         if tiles.device != scales.device:
             raise ValueError(f"tiles on {tiles.device}, scales on {scales.device}")
         self.tiles, self.scales = tiles, scales
@@ -55,29 +55,30 @@ def pack_w4(packed: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4We
     n, k = packed.shape[0], 2 * packed.shape[1]
     if scales.dtype != torch.float16 or tuple(scales.shape) != (n, -(-k // group)):
         raise ValueError(f"scales must be float16 [{n}, {-(-k // group)}]")
-    t, kb, gp = _shapes(k, n, group)
-    q = torch.zeros(t * 16, kb * 64, dtype=torch.uint8, device=packed.device)
+    (t, u, _), s_shape = _shapes(k, n, group)
+    g = 128 // group
+    q = torch.zeros(t * 128, u * 128, dtype=torch.uint8, device=packed.device)
     q[:n, 0:k:2] = packed & 15
     q[:n, 1:k:2] = packed >> 4
-    # [t, row half, row, kb, j, c, k/2, k%2] -> byte (k/2 + 2 (k%2)) of word j, row half in the nibble
-    v = q.view(t, 2, 8, kb, 4, 4, 2, 2)
-    b = (v[:, 0] | (v[:, 1] << 4)).permute(0, 2, 1, 4, 3, 6, 5)
-    s = torch.zeros(t * 16, gp, dtype=torch.float16, device=scales.device)
+    # [t, n16, row half, row, unit, kb, j, c, k/2, k%2] -> byte (k/2 + 2 (k%2)) of word j, row half in the nibble
+    v = q.view(t, 8, 2, 8, u, 2, 4, 4, 2, 2)
+    b = (v[:, :, 0] | (v[:, :, 1] << 4)).permute(0, 3, 1, 4, 2, 6, 5, 8, 7)
+    s = torch.zeros(t * 128, u * g, dtype=torch.float16, device=scales.device)
     s[:n, :scales.shape[1]] = scales
-    return W4Weight(b.reshape(t, kb, 512).contiguous(), s.view(t, 2, 8, gp).permute(0, 3, 2, 1).reshape(t, gp, 16).contiguous(),
-                    k, n, group)
+    s = s.view(t, 8, 2, 8, u, g).permute(0, 4, 1, 5, 3, 2)
+    return W4Weight(b.reshape(t, u, 8192).contiguous(), s.reshape(s_shape).contiguous(), k, n, group)
 
 
 @torch.no_grad()
 def unpack_w4(weight: W4Weight):
     """The inverse of ``pack_w4``: (packed, scales)."""
-    t, kb, gp = _shapes(weight.in_features, weight.out_features, weight.group)
-    b = weight.tiles.view(t, kb, 8, 4, 4, 2, 2).permute(0, 2, 1, 4, 3, 6, 5)
-    q = torch.stack((b & 15, b >> 4), dim=1).reshape(t * 16, kb * 64)[:weight.out_features, :weight.in_features]
+    (t, u, _), _ = _shapes(weight.in_features, weight.out_features, weight.group)
+    n, k, g = weight.out_features, weight.in_features, 128 // weight.group
+    b = weight.tiles.view(t, u, 8, 2, 8, 4, 4, 2, 2).permute(0, 2, 4, 1, 3, 6, 5, 8, 7)
+    q = torch.stack((b & 15, b >> 4), dim=2).reshape(t * 128, u * 128)[:n, :k]
     packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
-    g = -(-weight.in_features // weight.group)
-    s = weight.scales.view(t, gp, 8, 2).permute(0, 3, 2, 1).reshape(t * 16, gp)[:weight.out_features, :g].contiguous()
-    return packed, s
+    s = weight.scales.view(t, u, 8, g, 8, 2).permute(0, 2, 5, 4, 1, 3).reshape(t * 128, u * g)
+    return packed, s[:n, :-(-k // weight.group)].contiguous()
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = None,
@@ -157,10 +158,10 @@ class W4Linear(nn.Module):
         # the source layer's Parameters, transferred (optimiser references stay valid)
         self.weight = linear.weight
         self.bias = linear.bias
-        t, kb, gp = _shapes(self.in_features, self.out_features, group)
+        t_shape, s_shape = _shapes(self.in_features, self.out_features, group)
         dev = linear.weight.device
-        self.register_buffer("tiles", torch.zeros(t, kb, 512, dtype=torch.uint8, device=dev))
-        self.register_buffer("scales", torch.zeros(t, gp, 16, dtype=torch.float16, device=dev))
+        self.register_buffer("tiles", torch.zeros(t_shape, dtype=torch.uint8, device=dev))
+        self.register_buffer("scales", torch.zeros(s_shape, dtype=torch.float16, device=dev))
         self.requantize_()
 
     @torch.no_grad()

@@ -317,7 +317,7 @@ def test_runner_refreshes_w4_layers():
 # -- no GPU ------------------------------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("n,k,group", [(1, 2, 32), (16, 64, 64), (29, 130, 128), (40, 192, 32), (33, 100, 64)])
+@pytest.mark.parametrize("n,k,group", [(1, 2, 32), (16, 64, 64), (29, 130, 128), (140, 192, 32), (33, 100, 64)])
 def test_layout(n, k, group):
     """tiles and scales as include/glad_b200.h words them, element by element; the round trip."""
     q, packed, s = weight(n, k, group, 3, "cpu")
@@ -325,23 +325,22 @@ def test_layout(n, k, group):
     lib = N.load()
     assert w.tiles.numel() == lib.glad_w4_tiles_bytes(k, n, group)
     assert w.scales.numel() * 2 == lib.glad_w4_scales_bytes(k, n, group)
-    words = w.tiles.numpy().reshape(w.tiles.shape[0], w.tiles.shape[1], 128, 4).view(np.uint32).reshape(
-        w.tiles.shape[0], w.tiles.shape[1], 32, 4)
-    seen = np.zeros((w.tiles.shape[0] * 16, w.tiles.shape[1] * 64), np.int64)
-    for t in range(words.shape[0]):
-        for kb in range(words.shape[1]):
-            for lane in range(32):
-                r, c = lane >> 2, lane & 3
-                for j in range(4):
-                    for i in range(8):
-                        row = 16 * t + r + 8 * (i & 1)
-                        col = 64 * kb + 16 * j + 4 * c + 2 * ((i >> 1) & 1) + (i >> 2)
-                        v = (int(words[t, kb, lane, j]) >> (4 * i)) & 15
-                        seen[row, col] = v - 16 if v > 7 else v
+    T, U, G = w.tiles.shape[0], w.tiles.shape[1], 128 // group
+    words = w.tiles.numpy().view(np.uint32).reshape(T, U, 8, 2, 32, 4).astype(np.int64)
+    sc = w.scales.view(T, U, 8, G, 8, 2)
+    seen, scales = np.zeros((T * 128, U * 128), np.int64), torch.zeros(T * 128, U * G, dtype=torch.float16)
+    for t, u, b, lane in np.ndindex(T, U, 8, 32):
+        r, c = lane >> 2, lane & 3
+        for kb, j, i in np.ndindex(2, 4, 8):
+            row = 128 * t + 16 * b + r + 8 * (i & 1)
+            col = 128 * u + 64 * kb + 16 * j + 4 * c + 2 * ((i >> 1) & 1) + (i >> 2)
+            v = (words[t, u, b, kb, lane, j] >> (4 * i)) & 15
+            seen[row, col] = v - 16 if v > 7 else v
+        for gi, h in np.ndindex(G, 2):
+            scales[128 * t + 16 * b + r + 8 * h, u * G + gi] = sc[t, u, b, gi, r, h]
     assert np.array_equal(seen[:n, :k], q.numpy()) and not seen[n:].any() and not seen[:, k:].any()
     g = s.shape[1]
-    flat = torch.stack([w.scales[i // 16, :, 2 * (i % 8) + i % 16 // 8] for i in range(16 * w.scales.shape[0])])
-    assert torch.equal(flat[:n, :g], s) and not flat[n:].any() and not flat[:, g:].any()
+    assert torch.equal(scales[:n, :g], s) and not scales[n:].any() and not scales[:, g:].any()
     p2, s2 = unpack_w4(w)
     assert torch.equal(p2, packed) and torch.equal(s2, s)
 
@@ -370,8 +369,8 @@ def test_refusals():
                  (packed, s, 32), (packed[:, :0], s[:, :0], 64), (packed[0], s, 64)):
         with pytest.raises(ValueError):
             pack_w4(*args)
-    for args in ((w.tiles, w.scales, 127, 24, 64), (w.tiles, w.scales, 128, 24, 48), (w.tiles, w.scales, 128, 33, 64),
-                 (w.tiles[:, :1], w.scales, 128, 24, 64), (w.tiles, w.scales.float(), 128, 24, 64)):
+    for args in ((w.tiles, w.scales, 127, 24, 64), (w.tiles, w.scales, 128, 24, 48), (w.tiles, w.scales, 128, 133, 64),
+                 (w.tiles[..., :512], w.scales, 128, 24, 64), (w.tiles, w.scales.float(), 128, 24, 64)):
         with pytest.raises(ValueError):
             W4Weight(*args)
     with pytest.raises(ValueError):
