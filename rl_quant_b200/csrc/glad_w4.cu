@@ -57,6 +57,12 @@ __device__ __forceinline__ uint32_t b2_sub(uint32_t a, uint32_t b) {
   return d;
 }
 
+// (w & mask) ^ flip in one logic operation: with both constants as literals the compiler takes two.
+__device__ __forceinline__ uint32_t and_xor(uint32_t w, uint32_t mask, uint32_t flip) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(d) : "r"(w), "r"(mask), "r"(flip));
+  return d;
+}
 // Eight 4-bit weights -> the A registers of one 16x8x16 product. The two's-complement
 // nibble with its top bit flipped is q + 8.
 template <bool BF16>
@@ -64,13 +70,13 @@ __device__ __forceinline__ void unpack_w4(uint32_t w, uint32_t (&a)[4]) {
   if constexpr (BF16) {
     // 0x4300 | u is the bf16 128 + u (seven mantissa bits): each nibble is shifted to bit 0
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = b2_sub(((w >> (4 * i)) & 0x000f000fu) ^ 0x43084308u, 0x43084308u);
+    for (int i = 0; i < 4; ++i) a[i] = b2_sub(and_xor(w >> (4 * i), 0x000f000fu, 0x43084308u), 0x43084308u);
   } else {
-    a[0] = h2_sub((w & 0x000f000fu) ^ 0x64086408u, 0x64086408u);
-    a[1] = h2_fma((w & 0x00f000f0u) ^ 0x64806480u, 0x2c002c00u, 0xd480d480u);   // (1024 + 16 u) / 16 - 72
+    a[0] = h2_sub(and_xor(w, 0x000f000fu, 0x64086408u), 0x64086408u);
+    a[1] = h2_fma(and_xor(w, 0x00f000f0u, 0x64806480u), 0x2c002c00u, 0xd480d480u);   // (1024 + 16 u) / 16 - 72
     w >>= 8;
-    a[2] = h2_sub((w & 0x000f000fu) ^ 0x64086408u, 0x64086408u);
-    a[3] = h2_fma((w & 0x00f000f0u) ^ 0x64806480u, 0x2c002c00u, 0xd480d480u);
+    a[2] = h2_sub(and_xor(w, 0x000f000fu, 0x64086408u), 0x64086408u);
+    a[3] = h2_fma(and_xor(w, 0x00f000f0u, 0x64806480u), 0x2c002c00u, 0xd480d480u);
   }
 }
 
