@@ -31,6 +31,7 @@ struct W4Params {
   const float* xs;          // scales of 8-bit rows or null
   int xs_rows, xs_groups;   // 0/0: none or one value; 1/1: a row; 1/G: a row and group
   int x_fast;               // rows can be read 8 inputs at a time
+  int stream_warps;         // few rows: warps of a stream (4, 8, 16, 32)
   int splits;               // many rows: blocks that share a tile's inputs
   int x_tma;                // many rows: x is read by TMA
   const void* bias;
@@ -190,24 +191,24 @@ __device__ __forceinline__ void store_y4(const W4Params& p, int64_t m, int n, co
 }
 
 // ---- few rows (up to 8 NT): weight streaming ------------------------------------------------
-// One persistent block per SM walks 16-column tiles; its 16 warps split the inputs in units of
-// 128 and join their sums in warp order once a tile. Each warp streams its own units (1 KB of
-// weights and 128/GROUP * 32 bytes of scales) through a private shared-memory ring of
-// cp.async copies kRing - 1 units ahead, across tile borders, so about 48 KB are in flight on
-// an SM whatever the warps wait for. x is staged once in shared memory, in the form the products
-// take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
+// One persistent block per SM. Its warps form streams of W warps; each stream walks 16-column tiles,
+// its warps split the inputs in units of 128 and join their sums in warp order once a tile. Each warp
+// brings its own units (1 KB of weights and 128/GROUP * 32 bytes of scales) through a private
+// shared-memory ring of cp.async copies kRing - 1 units ahead, across tile borders, so 48 to 64 KB
+// are in flight on an SM whatever the warps wait for. x is staged once in shared memory, in the form
+// the products take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
 // a word's nibbles come apart). Rows past M read row M - 1: their sums are never stored.
-constexpr int kRowWarps = 16, kRing = 4;
-constexpr int kRowThreads = kRowWarps * 32;
-
+// Issue slots bound it: about 10 instructions unpack and multiply 256 weights of a warp.
 template <int NT, int GROUP>
 struct RowSmem {
+  static constexpr int kWarps = NT == 1 ? 32 : 16;
+  static constexpr int kRing = NT == 1 ? 3 : 4;
   static constexpr int kScales = 128 / GROUP;           // groups of a unit
   static constexpr int kWarpSlot = 1024 + kScales * 32;
-  static constexpr int kRingBytes = kRing * kRowWarps * kWarpSlot;
+  static constexpr int kRingBytes = kRing * kWarps * kWarpSlot;
   static constexpr int kBuffers = NT == 1 ? 2 : 1;      // of every warp's sums
-  static constexpr int kPart = kRowWarps * 8 * NT * 17;
-  static constexpr int kFixed = kRingBytes + kBuffers * kPart * 4;
+  static constexpr int kPart = 8 * NT * 17;             // floats of a warp's sums
+  static constexpr int kFixed = kRingBytes + kBuffers * kWarps * kPart * 4;
 };
 
 // D = A * B + 0 / D += A * B, m16n8k16 (f16, bf16 -> f32) and m16n8k32 (s8 -> s32).
@@ -250,20 +251,23 @@ __device__ __forceinline__ uint32_t w4_high16(uint32_t w) { return w & 0xf0f0f0f
 __device__ __forceinline__ uint32_t swap_mid(uint32_t v) { return __byte_perm(v, 0, 0x3120); }
 
 template <typename TX, int NT, int GROUP>
-__global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
+__global__ void __launch_bounds__(RowSmem<NT, GROUP>::kWarps * 32, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
   using L = RowSmem<NT, GROUP>;
   constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
   constexpr int SG = L::kScales, XP = I8 ? 8 : 16;       // bytes of eight staged inputs
+  constexpr int kRing = L::kRing, kThreads = L::kWarps * 32;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem + L::kRingBytes);
   uint8_t* xs = smem + L::kFixed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int T = (p.N + 15) / 16, U = p.U, M = (int)p.M;
-  const int u0 = (int)((int64_t)warp * U / kRowWarps), u1 = (int)((int64_t)(warp + 1) * U / kRowWarps);
+  const int T = (p.N + 15) / 16, U = p.U, M = (int)p.M, W = p.stream_warps;
+  const int stream = warp / W, ws = warp - stream * W;   // the stream's tiles are first, first + step, ...
+  const int first = stream * gridDim.x + blockIdx.x, step = gridDim.x * (L::kWarps / W);
+  const int u0 = (int)((int64_t)ws * U / W), u1 = (int)((int64_t)(ws + 1) * U / W);
   uint8_t* ring = smem + warp * (kRing * L::kWarpSlot);
+  float* part = reinterpret_cast<float*>(smem + L::kRingBytes) + stream * W * L::kPart;
 
   // the next unit to fetch: tile pt, unit pu
-  int pt = u0 < u1 ? blockIdx.x : T, pu = u0;
+  int pt = u0 < u1 ? first : T, pu = u0;
   const uint4* wsrc = nullptr;
   const uint8_t* ssrc = nullptr;
   auto seek = [&]() {
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
       ssrc += 8 * SG * 32;
       if (++pu == u1) {
         pu = u0;
-        pt += gridDim.x;
+        pt += step;
         seek();
       }
     }
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
   {
     // [32-input block][row][lane c of four][inputs 4c..4c+3, 16+4c..]: a warp's reads of eight rows are contiguous
     const int pieces = U * 16 * M;
-    for (int i = threadIdx.x; i < pieces; i += kRowThreads) {
+    for (int i = threadIdx.x; i < pieces; i += kThreads) {
       const int m = i / (U * 16), k8 = i - m * (U * 16);
       const uint4 v = staged(load_raw8<TX>(static_cast<const TX*>(p.x) + m * p.ldx, k8 * 8, p.K, p.x_fast));
       uint8_t* dst = xs + (((k8 >> 2) * M + m) * 4 + (k8 & 1) * 2) * XP + ((k8 >> 1) & 1) * (XP / 2);
@@ -323,7 +327,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
   const int xstep = M * 4 * XP;                          // bytes of 32 inputs of all rows
 
   int slot = 0, buffer = 0;
-  for (int t = blockIdx.x; t < T; t += gridDim.x) {
+  for (int t = first; t < T; t += step) {
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
       }
     }
     // with two buffers, the one written now was last read before the previous tile's barrier
-    float* mine = part + buffer * L::kPart + warp * (8 * NT * 17);
+    float* mine = part + (buffer * L::kWarps + ws) * L::kPart;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       mine[(8 * j + 2 * c) * 17 + r] = acc[j][0];
@@ -405,18 +409,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) w4_rows_kernel(const __grid_co
       mine[(8 * j + 2 * c) * 17 + r + 8] = acc[j][2];
       mine[(8 * j + 2 * c + 1) * 17 + r + 8] = acc[j][3];
     }
-    __syncthreads();
-    const int row = threadIdx.x >> 4, col = threadIdx.x & 15, n = 16 * t + col;
-    if (row < 8 * NT && row < M && n < p.N) {
-      const float* all = part + buffer * L::kPart + row * 17 + col;
+    named_bar_sync(1 + stream, W * 32);
+    for (int i = ws * 32 + lane; i < M * 16; i += W * 32) {
+      const int row = i >> 4, col = i & 15, n = 16 * t + col;
+      const float* all = part + buffer * L::kWarps * L::kPart + row * 17 + col;
       float v = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kRowWarps; ++k) v += all[k * (8 * NT * 17)];
+#pragma unroll 4
+      for (int k = 0; k < W; ++k) v += all[k * L::kPart];
       if (p.xs != nullptr && p.xs_groups <= 1) v *= p.xs[p.xs_rows ? row : 0];
-      store_y(p, row, n, v);
+      if (n < p.N) store_y(p, row, n, v);
     }
     if constexpr (L::kBuffers == 2) buffer ^= 1;
-    else __syncthreads();
+    else named_bar_sync(1 + stream, W * 32);
   }
 }
 
@@ -920,13 +924,25 @@ int w4_sms() {
 }
 
 template <typename TX, int NT, int GROUP>
-cudaError_t launch_rows(const W4Params& p, size_t x_bytes, cudaStream_t st) {
+cudaError_t launch_rows(W4Params p, size_t x_bytes, cudaStream_t st) {
+  using L = RowSmem<NT, GROUP>;
   static bool done[64] = {false};
   const cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP>, done);
   if (e != cudaSuccess) return e;
   const int tiles = (p.N + 15) / 16, sms = w4_sms();
-  return launch_k(w4_rows_kernel<TX, NT, GROUP>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowThreads),
-                  RowSmem<NT, GROUP>::kFixed + x_bytes, st, true, p);
+  // the stream width with the shortest longest stream: rounds of tiles x (units of a warp and half a unit's
+  // time to join the sums)
+  int64_t best = INT64_MAX;
+  for (int w = 4; w <= L::kWarps; w *= 2) {
+    const int64_t streams = (int64_t)sms * (L::kWarps / w);
+    const int64_t cost = ((tiles + streams - 1) / streams) * (2 * ((p.U + w - 1) / w) + 1);
+    if (cost <= best) {
+      best = cost;
+      p.stream_warps = w;
+    }
+  }
+  return launch_k(w4_rows_kernel<TX, NT, GROUP>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(L::kWarps * 32),
+                  L::kFixed + x_bytes, st, true, p);
 }
 
 // The driver's tensor-map encoder, looked up once.
