@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(RowSmem<NT, GROUP>::kWarps * 32, 1) w4_rows_ke
 
 // ---- many rows: tcgen05 -----------------------------------------------------------------------
 // A block computes 128 output columns x MT rows; D[n, m] lives in tensor memory, n its lanes. The
-// inputs go in stages of 128 bytes a row (64 of 16 bits, 128 of 8 bits: one swizzle atom). Roles by
+// inputs go in stages of 128 (one or two swizzle atoms of 128 bytes a row). Roles by
 // warp: one brings the packed weights (bulk copies, PD units of 128 inputs ahead), one the x tile
 // (TMA, NS stages ahead); teams of four unpack the weights of a unit each, in x's own type:
 // f16 or bf16, int8 times 16, or e4m3, all exact, and store them in tensor memory as the A operand (a
@@ -442,25 +442,26 @@ __device__ unsigned int g_w4_status;
 
 template <int XB, int MT, int GROUP>                     // XB: bytes of an input
 struct Tile {
-  static constexpr int SPU = XB;                         // stages of a unit (128 inputs)
-  static constexpr int NS = 8;                           // NS, PD, ND even: see the waits
-  static constexpr int PD = 4;
+  static constexpr int NS = 8 / XB;                      // stages: operands of a unit (128 inputs)
+  static constexpr int PD = MT < 128 ? 12 : XB == 2 ? 8 : 4;       // units of packed weights in flight
   static constexpr int ND = MT == 128 ? 2 : 4;
   static constexpr int SG = 128 / GROUP;                 // groups of a unit
   static constexpr int SPG = GROUP * XB / 32;            // products (32 bytes of inputs) of a group
+  static constexpr int ACOLS = 32 * XB;                  // tensor-memory columns of a stage's A
   static constexpr int MW = MT == 128 ? 2 : 4;           // warps that issue products
   static constexpr int SW = MT == 128 ? 16 : 8;          // warps that take the sums
   static constexpr int DW = 8;                           // warps that unpack
   static constexpr int kThreads = (SW + DW + MW + 2) * 32;
   static constexpr int NC = MT * 4 / SW;                 // columns of a sums thread
-  static constexpr int kStage = MT * 128;                // x of a stage
+  static constexpr int kBlock = MT * 128, kStage = XB * kBlock;    // x of a stage: 128 bytes a row and block
   static constexpr int kSlot = 8192;                     // packed weights of a unit
-  static constexpr int kXs = XB == 1 ? SW * SG * NC * 4 : 0;       // x scales of a unit, a copy a warp
-  static constexpr int kSmem = NS * kStage + PD * kSlot + kXs + 512 + 1024;
-  static constexpr int kACol = ND * MT;                  // first tensor-memory column of A: 32 a stage
-  static constexpr int kCols = ND * MT + NS * 32 <= 256 ? 256 : 512;
-  static_assert(ND * MT + NS * 32 <= kCols, "tensor memory");
-  static_assert(NS % (2 * MW) == 0 && ND % MW == 0 && PD % (DW / 4) == 0 && NS % (SPU * DW / 4) == 0, "phases");
+  static constexpr int SD = 4;                           // units of scales in flight, a copy a warp
+  static constexpr int kWs = SG * 64, kXs = XB == 1 ? SG * NC * 4 : 0;     // weight (32 rows), x scales of a unit
+  static constexpr int kSmem = NS * kStage + PD * kSlot + SW * SD * (kWs + kXs) + 512 + 1024;
+  static constexpr int kACol = ND * MT;                  // first tensor-memory column of A
+  static constexpr int kCols = ND * MT + NS * ACOLS <= 256 ? 256 : 512;
+  static_assert(ND * MT + NS * ACOLS <= kCols, "tensor memory");
+  static_assert(NS % MW == 0 && ND % MW == 0 && PD % (DW / 4) == 0 && NS % (DW / 4) == 0, "phases");
   static_assert(2 * MT * 512 <= NS * kStage, "the sums are sent and joined in the stage buffers");
   static_assert(kSmem <= 232448, "shared memory of one block");
   static_assert((2 * NS + 2 * PD + 2 * ND + 1) * 8 + 8 <= 512, "barrier area");
@@ -491,14 +492,20 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) |
          ((uint64_t)2 << 61);
 }
-// D (+)= A (tensor memory) * B^T from a converged warp: 32 bytes of inputs.
+// One lane of a converged warp, the same every time. With warp-uniform operands the single-thread
+// instructions then take them from uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// D (+)= A (tensor memory) * B^T, one thread issues: 32 bytes of inputs.
 #define W4_MMA_TS(name, kind)                                                                                \
   __device__ __forceinline__ void name(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) { \
     asm volatile(                                                                                            \
-        "{\n\t.reg .pred p, e;\n\t"                                                                           \
-        "elect.sync _|e, 0xffffffff;\n\t"                                                                      \
+        "{\n\t.reg .pred p;\n\t"                                                                              \
         "setp.ne.b32 p, %4, 0;\n\t"                                                                            \
-        "@e tcgen05.mma.cta_group::1.kind::" kind " [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),                        \
+        "tcgen05.mma.cta_group::1.kind::" kind " [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),                           \
         "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)                                                              \
         : "memory");                                                                                         \
   }
@@ -525,6 +532,9 @@ __device__ __forceinline__ void tma_x(uint32_t dst, const CUtensorMap* map, int 
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(map), "r"(k), "r"(m), "r"(smem_u32(bar))
       : "memory");
+}
+__device__ __forceinline__ void cp_async4_zfill(void* dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -573,13 +583,13 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   using L = Tile<(int)sizeof(TX), MT, GROUP>;
   constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
   constexpr bool E4M3 = std::is_same<TX, e4m3_t>::value;
-  constexpr int XB = (int)sizeof(TX), SG = L::SG, SPU = L::SPU, NC = L::NC, KS = 128 / XB;   // KS: inputs of a stage
+  constexpr int XB = (int)sizeof(TX), SG = L::SG, NC = L::NC;
   constexpr int SW = L::SW, DW = L::DW, CTL = SW + DW;   // first control warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* slots = smem + L::NS * L::kStage;
-  float* xsc = reinterpret_cast<float*>(slots + L::PD * L::kSlot);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xsc) + L::kXs);
+  uint8_t* scale_ring = slots + L::PD * L::kSlot;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale_ring + L::SW * L::SD * (L::kWs + L::kXs));
   uint64_t* empty = full + L::NS;                        // [NS] products done; full: operands written
   uint64_t* wfull = empty + L::NS;                       // [PD]
   uint64_t* wempty = wfull + L::PD;                      // [PD]
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // warp-uniform
   const int S = p.splits, rank = S > 1 ? (int)cluster_ctarank() : 0;
   const int nt = blockIdx.x / S;
   const int64_t m0 = (int64_t)blockIdx.y * MT;
@@ -600,7 +610,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < L::NS; ++i) {
       mbar_init(&full[i], 4 + (p.x_tma ? 1 : 0));
-      mbar_init(&empty[i], L::SPG >= 4 ? 1 : 4 / L::SPG < L::MW ? 4 / L::SPG : L::MW);
+      mbar_init(&empty[i], SG < L::MW ? SG : L::MW);
     }
     for (int i = 0; i < L::PD; ++i) {
       mbar_init(&wfull[i], 1);
@@ -617,14 +627,14 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   grid_dep_wait();
   grid_dep_launch();
 
   if (warp >= CTL) {
     if (warp == CTL + L::MW) {
       // ---- packed weights
-      if (lane == 0) {
+      if (elect_one()) {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(p.tiles) + ((int64_t)nt * U + un0) * 8192;
         int i = 0;
         for (; i < units; ++i, src += 8192) {
@@ -638,15 +648,16 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       }
     } else if (warp == CTL + L::MW + 1) {
       // ---- x tiles
-      if (lane == 0 && p.x_tma) {
+      if (p.x_tma && elect_one()) {
         const uint32_t base = smem_u32(smem);
-        const int stages = units * SPU;
         int i = 0;
-        for (; i < stages; ++i) {
+        for (; i < units; ++i) {
           const int st = i % L::NS;
           if (i >= L::NS && !w4_wait(&empty[st], (i / L::NS - 1) & 1, abort)) break;
           mbar_arrive_expect_tx(&full[st], L::kStage);
-          tma_x(base + st * L::kStage, &xmap, un0 * 128 + i * KS, (int)m0, &full[st]);
+#pragma unroll
+          for (int h = 0; h < XB; ++h)
+            tma_x(base + st * L::kStage + h * L::kBlock, &xmap, (un0 + i) * 128 + h * 64, (int)m0, &full[st]);
         }
         for (int k = max(0, i - L::NS); k < i && *abort; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1);
       }
@@ -656,32 +667,35 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       // the same warps'.
       constexpr uint32_t idesc = I8 ? idesc_i8(128, MT) : idesc_f16(128, MT) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t base = smem_u32(smem);
-      const int stages = units * SPU, me = warp - CTL;
+      const int me = warp - CTL;
       bool ok = true;
-      for (int i = 0; ok && i < stages; ++i) {
-        // the warps of a stage: its one group's, or those of its 4 / SPG groups
-        if (L::SPG >= 4 ? (i * 4 / L::SPG) % L::MW != me : (me - i * 4 / L::SPG % L::MW + L::MW) % L::MW >= 4 / L::SPG)
-          continue;
-        ok = __all_sync(0xffffffffu, w4_wait(&full[i % L::NS], (i / L::NS) & 1, abort));
-        tc_fence_after();
-        const uint32_t a = tmem + L::kACol + (i % L::NS) * 32;
-        const uint64_t b = desc_sw128(base + (i % L::NS) * L::kStage);
+      for (int u = 0; ok && u < units; ++u) {
+        const int st = u % L::NS;
+        if (SG < L::MW && (me - u * SG % L::MW + L::MW) % L::MW >= SG) continue;   // none of this unit's groups
+        ok = __all_sync(0xffffffffu, w4_wait(&full[st], (u / L::NS) & 1, abort));
+        const uint32_t a = tmem + L::kACol + st * L::ACOLS;
+        const uint64_t b = desc_sw128(base + st * L::kStage);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {                    // 32 bytes of inputs
-          const int in_group = (i * 4 + q) % L::SPG, gi = (i * 4 + q) / L::SPG, d = gi % L::ND;
-          if (L::SPG < 4 && gi % L::MW != me) continue;
-          if (in_group == 0 && gi >= L::ND) {
-            if (ok) ok = __all_sync(0xffffffffu, w4_wait(&dempty[d], (gi / L::ND - 1) & 1, abort));
-            tc_fence_after();
+        for (int j = 0; j < SG; ++j) {
+          const int gi = u * SG + j, d = gi % L::ND;
+          if (gi % L::MW != me) continue;
+          if (ok && gi >= L::ND) ok = __all_sync(0xffffffffu, w4_wait(&dempty[d], (gi / L::ND - 1) & 1, abort));
+          tc_fence_after();
+          if (ok && elect_one()) {
+#pragma unroll
+            for (int e = 0; e < L::SPG; ++e) {           // 32 bytes of inputs: 8 columns of A, 32 bytes of B's rows
+              const int q = j * L::SPG + e;
+              const uint64_t bq = b + (q >> 2) * (L::kBlock >> 4) + (q & 3) * 2;
+              if constexpr (I8) mma_ts_i8(tmem + d * MT, a + 8 * q, bq, idesc, e > 0 ? 1u : 0u);
+              else if constexpr (E4M3) mma_ts_f8(tmem + d * MT, a + 8 * q, bq, idesc, e > 0 ? 1u : 0u);
+              else mma_ts_f16(tmem + d * MT, a + 8 * q, bq, idesc, e > 0 ? 1u : 0u);
+            }
+            mma_commit(&dfull[d]);
           }
-          if (ok) {
-            if constexpr (I8) mma_ts_i8(tmem + d * MT, a + 8 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
-            else if constexpr (E4M3) mma_ts_f8(tmem + d * MT, a + 8 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
-            else mma_ts_f16(tmem + d * MT, a + 8 * q, b + 2 * q, idesc, in_group > 0 ? 1u : 0u);
-            if (in_group == L::SPG - 1) mma_commit_warp(&dfull[d]);
-          }
+          __syncwarp();
         }
-        if (ok) mma_commit_warp(&empty[i % L::NS]);
+        if (ok && elect_one()) mma_commit(&empty[st]);
+        __syncwarp();
       }
       // after a failure: products that were issued end before their operands go
       if (*abort)
@@ -693,13 +707,13 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     const uint32_t sbase = smem_u32(smem);
     bool ok = true;
 
-    // x that TMA cannot read (rows off 16 bytes): stage i by guarded loads
-    auto copy_x = [&](int i) {
-      const uint32_t b = sbase + (i % L::NS) * L::kStage;
+    // x that TMA cannot read (rows off 16 bytes): 128 bytes a row of unit u by guarded loads
+    auto copy_x = [&](int u, int h) {
+      const uint32_t b = sbase + (u % L::NS) * L::kStage + h * L::kBlock;
 #pragma unroll 1
       for (int id = dw * 32 + lane; id < MT * 8; id += 128) {
         const int row = id >> 3, piece = id & 7;
-        const int k = un0 * 128 + i * KS + piece * (16 / XB);
+        const int k = (un0 + u) * 128 + h * 64 + piece * (16 / XB);
         const int64_t m = m0 + row;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (m < p.M) {
@@ -716,11 +730,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     for (int u = (warp - SW) >> 2; u < units; u += DW / 4) {   // a team meets all phases of its slots
       const int slot = u % L::PD;
       if (ok) ok = w4_wait(&wfull[slot], (u / L::PD) & 1, abort);
-#pragma unroll
-      for (int h = 0; h < SPU; ++h) {
-        const int i = u * SPU + h;
-        if (ok && i >= L::NS) ok = w4_wait(&empty[i % L::NS], (i / L::NS - 1) & 1, abort);
-      }
+      if (ok && u >= L::NS) ok = w4_wait(&empty[u % L::NS], (u / L::NS - 1) & 1, abort);
       if (!ok) break;
       tc_fence_after();
       const uint8_t* in = slots + slot * L::kSlot;
@@ -742,17 +752,17 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
             unpack_w4<BF16>(word[j], a);
             v[4 * j] = a[0], v[4 * j + 1] = a[2], v[4 * j + 2] = a[1], v[4 * j + 3] = a[3];
           }
-          tmem_st_16x256b_x4(at + ((u * 2 + kb) % L::NS) * 32, v);
+          tmem_st_16x256b_x4(at + (u % L::NS) * L::ACOLS + kb * 32, v);
         } else {
           uint32_t v[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) unpack_w4_bytes<E4M3>(word[j], v[2 * j], v[2 * j + 1]);
-          tmem_st_16x128b_x4(at + (u % L::NS) * 32 + kb * 16, v);
+          tmem_st_16x128b_x4(at + (u % L::NS) * L::ACOLS + kb * 16, v);
         }
       }
       if (!p.x_tma) {
 #pragma unroll
-        for (int h = 0; h < SPU; ++h) copy_x(u * SPU + h);
+        for (int h = 0; h < XB; ++h) copy_x(u, h);
         fence_async_smem();
       }
       tmem_st_wait();
@@ -760,60 +770,51 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&wempty[slot]);
-#pragma unroll
-        for (int h = 0; h < SPU; ++h) mbar_arrive(&full[(u * SPU + h) % L::NS]);
+        mbar_arrive(&full[u % L::NS]);
       }
     }
   } else {
     // ---- sums
     const int q4 = warp & 3, col0 = (warp >> 2) * NC;
     const bool by_group = XB == 1 && p.xs_groups > 1;
-    // this thread's row of the weight scales
-    const __half* sp = p.scales + (((int64_t)nt * U + un0) * 8 + q4 * 2 + (lane >> 4)) * (SG * 16) + (lane & 7) * 2 +
-                       ((lane >> 3) & 1);
-    constexpr int XN = XB == 1 ? (SG * NC + 31) / 32 : 1;            // x scales of a unit a lane fetches
-    float* my_xs = xsc + warp * (SG * NC);
+    // the scales this warp multiplies by, fetched SD - 1 units ahead into a ring of its own
+    uint8_t* ring = scale_ring + warp * (L::SD * (L::kWs + L::kXs));
+    const uint8_t* wsrc = reinterpret_cast<const uint8_t*>(p.scales) + (((int64_t)nt * U + un0) * 8 + q4 * 2) * (SG * 32);
+    auto fetch = [&](int u) {
+      if (u < units) {
+        uint8_t* dst = ring + (u % L::SD) * (L::kWs + L::kXs);
+        if (lane < SG * 4) cp_async16(dst + lane * 16, wsrc + (int64_t)u * (8 * SG * 32) + lane * 16);
+        if constexpr (XB == 1) {
+          if (by_group) {
+#pragma unroll
+            for (int id = lane; id < SG * NC; id += 32) {
+              const int xg = (un0 + u) * SG + id / NC;
+              const int64_t m = m0 + col0 + id % NC;
+              const bool live = m < p.M && xg < p.xs_groups;
+              cp_async4_zfill(dst + L::kWs + id * 4, p.xs + (live ? m * p.xs_groups + xg : 0), live);
+            }
+          }
+        }
+      }
+      cp_async_commit();
+    };
     float acc[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
-    __half s_next[SG], s_after[SG];
-    float xs_next[XN];
     bool ok = true;
-    auto load_s = [&](int u, __half (&s)[SG]) {
 #pragma unroll
-      for (int j = 0; j < SG; ++j) s[j] = u < units ? sp[(u * 8 * SG + j) * 16] : __half(0.0f);
-    };
-    auto load_xs = [&](int u) {
-      if constexpr (XB == 1) {
-#pragma unroll
-        for (int e = 0; e < XN; ++e) {
-          const int id = e * 32 + lane, g = id / NC;
-          const int64_t m = m0 + col0 + id % NC;
-          const int xg = (un0 + u) * SG + g;
-          xs_next[e] = (by_group && u < units && g < SG && m < p.M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
-        }
-      }
-    };
-    load_s(0, s_next);
-    load_s(1, s_after);
-    load_xs(0);
+    for (int i = 0; i < L::SD - 1; ++i) fetch(i);
     for (int u = 0; ok && u < units; ++u) {
+      cp_async_wait_group<L::SD - 2>();
+      __syncwarp();
+      fetch(u + L::SD - 1);                              // the slot that every lane has just left
+      const uint8_t* in = ring + (u % L::SD) * (L::kWs + L::kXs);
+      const float* my_xs = reinterpret_cast<const float*>(in + L::kWs);
       float sc[SG];
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
-        sc[j] = __half2float(s_next[j]) * (I8 ? 0.0625f : 1.0f);   // the int8 operand is 16 q
-        s_next[j] = s_after[j];
-      }
-      load_s(u + 2, s_after);
-      if constexpr (XB == 1) {
-        if (by_group) {
-          __syncwarp();
-#pragma unroll
-          for (int e = 0; e < XN; ++e)
-            if (e * 32 + lane < SG * NC) my_xs[e * 32 + lane] = xs_next[e];
-          __syncwarp();
-          load_xs(u + 1);
-        }
+        sc[j] = __half2float(reinterpret_cast<const __half*>(in)[((lane >> 4) * SG + j) * 16 + (lane & 7) * 2 + ((lane >> 3) & 1)]);
+        if (I8) sc[j] *= 0.0625f;                        // the int8 operand is 16 q
       }
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
@@ -855,6 +856,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
         if (lane == 0) mbar_arrive(&dempty[d]);
       }
     }
+    cp_async_wait_all();
     // every product is done, so the stage buffers are free: [m][n]
     float* mine = reinterpret_cast<float*>(smem) + 32 * q4 + lane;
 #pragma unroll
