@@ -31,7 +31,7 @@ struct W4Params {
   const float* xs;          // scales of 8-bit rows or null
   int xs_rows, xs_groups;   // 0/0: none or one value; 1/1: a row; 1/G: a row and group
   int x_fast;               // rows can be read 8 inputs at a time
-  int stream_warps;         // few rows: warps of a stream (4, 8, 16, 32)
+  int stream_warps;         // few rows: warps of a stream (2, 4, 8, 16)
   int splits;               // many rows: blocks that share a tile's inputs
   int x_tma;                // many rows: x is read by TMA
   const void* bias;
@@ -191,23 +191,23 @@ __device__ __forceinline__ void store_y4(const W4Params& p, int64_t m, int n, co
 }
 
 // ---- few rows (up to 8 NT): weight streaming ------------------------------------------------
-// One persistent block per SM. Its warps form streams of W warps; each stream walks 16-column tiles,
+// One persistent block per SM. Its warps form streams of W warps; each stream walks tiles of 32 columns,
 // its warps split the inputs in units of 128 and join their sums in warp order once a tile. Each warp
-// brings its own units (1 KB of weights and 128/GROUP * 32 bytes of scales) through a private
-// shared-memory ring of cp.async copies kRing - 1 units ahead, across tile borders, so 48 to 64 KB
+// brings its own units (2 KB of weights and 128/GROUP * 64 bytes of scales) through a private
+// shared-memory ring of cp.async copies kRing - 1 units ahead, across tile borders, so about 64 KB
 // are in flight on an SM whatever the warps wait for. x is staged once in shared memory, in the form
 // the products take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
 // a word's nibbles come apart). Rows past M read row M - 1: their sums are never stored.
-// Issue slots bound it: about 10 instructions unpack and multiply 256 weights of a warp.
-template <int NT, int GROUP>
+// Issue slots bound it: a 32-bit word takes 9 instructions to unpack and one to multiply, so a unit is as
+// large as registers allow, which spreads the rest (copies, x, scales, addresses) over more words.
+template <int NT, int GROUP, int RING>
 struct RowSmem {
-  static constexpr int kWarps = NT == 1 ? 32 : 16;
-  static constexpr int kRing = NT == 1 ? 3 : 4;
+  static constexpr int kWarps = 16, kRing = RING;
   static constexpr int kScales = 128 / GROUP;           // groups of a unit
-  static constexpr int kWarpSlot = 1024 + kScales * 32;
+  static constexpr int kWarpSlot = 2048 + kScales * 64;
   static constexpr int kRingBytes = kRing * kWarps * kWarpSlot;
   static constexpr int kBuffers = NT == 1 ? 2 : 1;      // of every warp's sums
-  static constexpr int kPart = 8 * NT * 17;             // floats of a warp's sums
+  static constexpr int kPart = 8 * NT * 33;             // floats of a warp's sums
   static constexpr int kFixed = kRingBytes + kBuffers * kWarps * kPart * 4;
 };
 
@@ -250,16 +250,16 @@ __device__ __forceinline__ uint32_t w4_low16(uint32_t w) { return (w << 4) & 0xf
 __device__ __forceinline__ uint32_t w4_high16(uint32_t w) { return w & 0xf0f0f0f0u; }
 __device__ __forceinline__ uint32_t swap_mid(uint32_t v) { return __byte_perm(v, 0, 0x3120); }
 
-template <typename TX, int NT, int GROUP>
-__global__ void __launch_bounds__(RowSmem<NT, GROUP>::kWarps * 32, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
-  using L = RowSmem<NT, GROUP>;
+template <typename TX, int NT, int GROUP, int RING>
+__global__ void __launch_bounds__(512, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
+  using L = RowSmem<NT, GROUP, RING>;
   constexpr bool BF16 = std::is_same<TX, __nv_bfloat16>::value, I8 = std::is_same<TX, int8_t>::value;
   constexpr int SG = L::kScales, XP = I8 ? 8 : 16;       // bytes of eight staged inputs
   constexpr int kRing = L::kRing, kThreads = L::kWarps * 32;
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* xs = smem + L::kFixed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int T = (p.N + 15) / 16, U = p.U, M = (int)p.M, W = p.stream_warps;
+  const int T = (p.N + 31) / 32, U = p.U, M = (int)p.M, W = p.stream_warps;
   const int stream = warp / W, ws = warp - stream * W;   // the stream's tiles are first, first + step, ...
   const int first = stream * gridDim.x + blockIdx.x, step = gridDim.x * (L::kWarps / W);
   const int u0 = (int)((int64_t)ws * U / W), u1 = (int)((int64_t)(ws + 1) * U / W);
@@ -271,19 +271,19 @@ __global__ void __launch_bounds__(RowSmem<NT, GROUP>::kWarps * 32, 1) w4_rows_ke
   const uint4* wsrc = nullptr;
   const uint8_t* ssrc = nullptr;
   auto seek = [&]() {
-    const int64_t at = ((int64_t)(pt >> 3) * U + pu) * 8 + (pt & 7);   // 1 KB blocks
-    wsrc = p.tiles + at * 64 + lane;
-    ssrc = reinterpret_cast<const uint8_t*>(p.scales) + at * (SG * 32) + lane * 16;
+    const int64_t at = ((int64_t)(pt >> 2) * U + pu) * 4 + (pt & 3);   // 2 KB blocks
+    wsrc = p.tiles + at * 128 + lane;
+    ssrc = reinterpret_cast<const uint8_t*>(p.scales) + at * (SG * 64) + lane * 16;
   };
   seek();
   auto fetch = [&](int slot) {
     if (pt < T) {
       uint8_t* dst = ring + slot * L::kWarpSlot + lane * 16;
-      cp_async16(dst, wsrc);
-      cp_async16(dst + 512, wsrc + 32);
-      if (lane < SG * 2) cp_async16(dst + 1024, ssrc);
-      wsrc += 8 * 64;
-      ssrc += 8 * SG * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cp_async16(dst + i * 512, wsrc + i * 32);
+      if (lane < SG * 4) cp_async16(dst + 2048, ssrc);
+      wsrc += 4 * 128;
+      ssrc += 4 * SG * 64;
       if (++pu == u1) {
         pu = u0;
         pt += step;
@@ -328,74 +328,96 @@ __global__ void __launch_bounds__(RowSmem<NT, GROUP>::kWarps * 32, 1) w4_rows_ke
 
   int slot = 0, buffer = 0;
   for (int t = first; t < T; t += step) {
-    float acc[NT][4];
+    float acc[2][NT][4];                                 // [16 columns][8 rows]
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[h][j][e] = 0.0f;
+    const uint8_t* xat[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) xat[j] = xrow[j] + 4 * u0 * xstep;
     for (int u = u0; u < u1; ++u) {
       cp_async_wait_group<kRing - 2>();
       __syncwarp();
-      fetch((slot + kRing - 1) % kRing);                 // the slot that every lane has just left
+      fetch(slot == 0 ? kRing - 1 : slot - 1);           // the slot that every lane has just left
       const uint8_t* in = ring + slot * L::kWarpSlot;
-      slot = (slot + 1) % kRing;
-      uint4 w4[2] = {*reinterpret_cast<const uint4*>(in + lane * 16),
-                     *reinterpret_cast<const uint4*>(in + 512 + lane * 16)};
-      const uint32_t w[8] = {w4[0].x, w4[0].y, w4[0].z, w4[0].w, w4[1].x, w4[1].y, w4[1].z, w4[1].w};
-      float g[NT][4];
-      int gi8[NT][4];
+      slot = slot + 1 == kRing ? 0 : slot + 1;
+      float g[2][NT][4];
+      int gi8[2][NT][4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {                      // 32 inputs at a time
-        constexpr int QG = GROUP / 32;
-        uint4 x[NT];
+      for (int kb = 0; kb < 2; ++kb) {
+        uint4 w4[2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint8_t* src = xrow[j] + (4 * u + q) * xstep;
-          if constexpr (I8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(src);
-            x[j] = make_uint4(v.x, v.y, 0, 0);
-          } else {
-            x[j] = *reinterpret_cast<const uint4*>(src);
-          }
-        }
-        if constexpr (I8) {
-          const uint32_t a[4] = {w4_low16(w[2 * q]), w4_high16(w[2 * q]), w4_low16(w[2 * q + 1]), w4_high16(w[2 * q + 1])};
+        for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(in + h * 1024 + kb * 512 + lane * 16);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (q % QG == 0) mma_rows_i8<true>(gi8[j], a, x[j].x, x[j].y);
-            else mma_rows_i8<false>(gi8[j], a, x[j].x, x[j].y);
-          }
-        } else {
-          uint32_t a0[4], a1[4];
-          unpack_w4<BF16>(w[2 * q], a0);
-          unpack_w4<BF16>(w[2 * q + 1], a1);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (q % QG == 0) mma_rows<BF16, true>(g[j], a0, x[j].x, x[j].y);
-            else mma_rows<BF16, false>(g[j], a0, x[j].x, x[j].y);
-            mma_rows<BF16, false>(g[j], a1, x[j].z, x[j].w);
-          }
-        }
-        if ((q + 1) % QG == 0) {
-          const int gi = q / QG;
-          float2 s = __half22float2(*reinterpret_cast<const __half2*>(in + 1024 + gi * 32 + r * 4));
-          if constexpr (I8) s.x *= 0.0625f, s.y *= 0.0625f;   // the codes were multiplied by 16
+        for (int q2 = 0; q2 < 2; ++q2) {                 // 32 inputs at a time
+          constexpr int QG = GROUP / 32;
+          const int q = 2 * kb + q2;
+          uint4 x[NT];
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             if constexpr (I8) {
+              const uint2 v = *reinterpret_cast<const uint2*>(xat[j]);
+              x[j] = make_uint4(v.x, v.y, 0, 0);
+            } else {
+              x[j] = *reinterpret_cast<const uint4*>(xat[j]);
+            }
+            xat[j] += xstep;
+          }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) g[j][e] = i2f_small(gi8[j][e]);   // below 2^21
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w0 = q2 ? w4[h].z : w4[h].x, w1 = q2 ? w4[h].w : w4[h].y;
+            if constexpr (I8) {
+              const uint32_t a[4] = {w4_low16(w0), w4_high16(w0), w4_low16(w1), w4_high16(w1)};
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                if (q % QG == 0) mma_rows_i8<true>(gi8[h][j], a, x[j].x, x[j].y);
+                else mma_rows_i8<false>(gi8[h][j], a, x[j].x, x[j].y);
+              }
+            } else {
+              uint32_t a0[4], a1[4];
+              unpack_w4<BF16>(w0, a0);
+              unpack_w4<BF16>(w1, a1);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                if (q % QG == 0) mma_rows<BF16, true>(g[h][j], a0, x[j].x, x[j].y);
+                else mma_rows<BF16, false>(g[h][j], a0, x[j].x, x[j].y);
+                mma_rows<BF16, false>(g[h][j], a1, x[j].z, x[j].w);
+              }
             }
-            if (sizeof(TX) == 1 && p.xs_groups > 1) {
-              const int m = 8 * j + 2 * c, xg = u * SG + gi;
-              const float x0 = (m < M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
-              const float x1 = (m + 1 < M && xg < p.xs_groups) ? p.xs[(m + 1) * p.xs_groups + xg] : 0.0f;
-              g[j][0] *= x0, g[j][1] *= x1, g[j][2] *= x0, g[j][3] *= x1;
+          }
+          if ((q + 1) % QG == 0) {
+            const int gi = q / QG;
+            float2 s[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[h] = __half22float2(*reinterpret_cast<const __half2*>(in + 2048 + h * (SG * 32) + gi * 32 + r * 4));
+              if constexpr (I8) s[h].x *= 0.0625f, s[h].y *= 0.0625f;   // the codes were multiplied by 16
             }
-            acc[j][0] = fmaf(s.x, g[j][0], acc[j][0]);
-            acc[j][1] = fmaf(s.x, g[j][1], acc[j][1]);
-            acc[j][2] = fmaf(s.y, g[j][2], acc[j][2]);
-            acc[j][3] = fmaf(s.y, g[j][3], acc[j][3]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              float x0 = 1.0f, x1 = 1.0f;
+              const bool by_group = sizeof(TX) == 1 && p.xs_groups > 1;
+              if (by_group) {
+                const int m = 8 * j + 2 * c, xg = u * SG + gi;
+                x0 = (m < M && xg < p.xs_groups) ? p.xs[m * p.xs_groups + xg] : 0.0f;
+                x1 = (m + 1 < M && xg < p.xs_groups) ? p.xs[(m + 1) * p.xs_groups + xg] : 0.0f;
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if constexpr (I8) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) g[h][j][e] = i2f_small(gi8[h][j][e]);   // below 2^21
+                }
+                if (by_group) g[h][j][0] *= x0, g[h][j][1] *= x1, g[h][j][2] *= x0, g[h][j][3] *= x1;
+                acc[h][j][0] = fmaf(s[h].x, g[h][j][0], acc[h][j][0]);
+                acc[h][j][1] = fmaf(s[h].x, g[h][j][1], acc[h][j][1]);
+                acc[h][j][2] = fmaf(s[h].y, g[h][j][2], acc[h][j][2]);
+                acc[h][j][3] = fmaf(s[h].y, g[h][j][3], acc[h][j][3]);
+              }
+            }
           }
         }
       }
@@ -403,16 +425,16 @@ __global__ void __launch_bounds__(RowSmem<NT, GROUP>::kWarps * 32, 1) w4_rows_ke
     // with two buffers, the one written now was last read before the previous tile's barrier
     float* mine = part + (buffer * L::kWarps + ws) * L::kPart;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      mine[(8 * j + 2 * c) * 17 + r] = acc[j][0];
-      mine[(8 * j + 2 * c + 1) * 17 + r] = acc[j][1];
-      mine[(8 * j + 2 * c) * 17 + r + 8] = acc[j][2];
-      mine[(8 * j + 2 * c + 1) * 17 + r + 8] = acc[j][3];
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (8 * j + 2 * c + (e & 1) < M) mine[(8 * j + 2 * c + (e & 1)) * 33 + 16 * h + r + 8 * (e >> 1)] = acc[h][j][e];
     named_bar_sync(1 + stream, W * 32);
-    for (int i = ws * 32 + lane; i < M * 16; i += W * 32) {
-      const int row = i >> 4, col = i & 15, n = 16 * t + col;
-      const float* all = part + buffer * L::kWarps * L::kPart + row * 17 + col;
+    for (int i = ws * 32 + lane; i < M * 32; i += W * 32) {
+      const int row = i >> 5, col = i & 31, n = 32 * t + col;
+      const float* all = part + buffer * L::kWarps * L::kPart + row * 33 + col;
       float v = 0.0f;
 #pragma unroll 4
       for (int k = 0; k < W; ++k) v += all[k * L::kPart];
@@ -448,7 +470,7 @@ struct Tile {
   static constexpr int SG = 128 / GROUP;                 // groups of a unit
   static constexpr int SPG = GROUP * XB / 32;            // products (32 bytes of inputs) of a group
   static constexpr int ACOLS = 32 * XB;                  // tensor-memory columns of a stage's A
-  static constexpr int MW = MT == 128 ? 2 : 4;           // warps that issue products
+  static constexpr int MW = 2;                           // warps that issue products
   static constexpr int SW = MT == 128 ? 16 : 8;          // warps that take the sums
   static constexpr int DW = 8;                           // warps that unpack
   static constexpr int kThreads = (SW + DW + MW + 2) * 32;
@@ -468,7 +490,7 @@ struct Tile {
 };
 
 // Wait for a phase, 2 s at most. The timer is read only after many tries: a read costs more than most waits.
-__device__ __forceinline__ bool w4_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
+__device__ __noinline__ bool w4_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
   for (int i = 0; i < 1000; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
@@ -925,17 +947,17 @@ int w4_sms() {
   return cache[dev];
 }
 
-template <typename TX, int NT, int GROUP>
+template <typename TX, int NT, int GROUP, int RING>
 cudaError_t launch_rows(W4Params p, size_t x_bytes, cudaStream_t st) {
-  using L = RowSmem<NT, GROUP>;
+  using L = RowSmem<NT, GROUP, RING>;
   static bool done[64] = {false};
-  const cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP>, done);
+  const cudaError_t e = allow_max_smem((const void*)w4_rows_kernel<TX, NT, GROUP, RING>, done);
   if (e != cudaSuccess) return e;
-  const int tiles = (p.N + 15) / 16, sms = w4_sms();
+  const int tiles = (p.N + 31) / 32, sms = w4_sms();
   // the stream width with the shortest longest stream: rounds of tiles x (units of a warp and half a unit's
   // time to join the sums)
   int64_t best = INT64_MAX;
-  for (int w = 4; w <= L::kWarps; w *= 2) {
+  for (int w = 2; w <= L::kWarps; w *= 2) {
     const int64_t streams = (int64_t)sms * (L::kWarps / w);
     const int64_t cost = ((tiles + streams - 1) / streams) * (2 * ((p.U + w - 1) / w) + 1);
     if (cost <= best) {
@@ -943,7 +965,7 @@ cudaError_t launch_rows(W4Params p, size_t x_bytes, cudaStream_t st) {
       p.stream_warps = w;
     }
   }
-  return launch_k(w4_rows_kernel<TX, NT, GROUP>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(L::kWarps * 32),
+  return launch_k(w4_rows_kernel<TX, NT, GROUP, RING>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(L::kWarps * 32),
                   L::kFixed + x_bytes, st, true, p);
 }
 
@@ -1008,8 +1030,9 @@ template <typename TX, int GROUP>
 cudaError_t launch_group(const W4Params& p, cudaStream_t st) {
   // x in shared memory as the products take it
   const size_t x = (size_t)p.U * 128 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M, limit = 232448;
-  if (p.M <= 8 && RowSmem<1, GROUP>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP>(p, x, st);
-  if (p.M <= 16 && RowSmem<2, GROUP>::kFixed + x <= limit) return launch_rows<TX, 2, GROUP>(p, x, st);
+  if (p.M <= 8 && RowSmem<1, GROUP, 3>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP, 3>(p, x, st);
+  if (p.M <= 8 && RowSmem<1, GROUP, 2>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP, 2>(p, x, st);
+  if (p.M > 8 && p.M <= 16 && RowSmem<2, GROUP, 2>::kFixed + x <= limit) return launch_rows<TX, 2, GROUP, 2>(p, x, st);
   if (p.M <= 32) return launch_tile<TX, 32, GROUP>(p, st);
   if (p.M <= 64) return launch_tile<TX, 64, GROUP>(p, st);
   return launch_tile<TX, 128, GROUP>(p, st);
