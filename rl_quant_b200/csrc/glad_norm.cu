@@ -17,6 +17,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdio>
+#include <type_traits>
 
 #include "glad_common.cuh"
 
@@ -26,8 +27,7 @@ int set_last_error(int code, const char* msg);
 namespace {
 
 constexpr int kNormMaxCols = 32768;      // a row lives in the registers of one block
-constexpr int kNormMaxPartials = 1184;   // dw partial rows of the backward pass (8 per SM)
-constexpr int kNormRowsPerTeam = 4;      // rows a team sums before it may write a dw partial
+constexpr int kNormMaxPartials = 592;    // dw partial rows of the backward pass (4 per SM)
 
 struct NormParams {
   const void* x;        // forward: input rows; backward: dy
@@ -36,13 +36,13 @@ struct NormParams {
   const void* w;        // weight or null
   int64_t ldx, ldr, ldh;
   int64_t rows;
-  int cols, team;       // team: threads of one row
+  int cols, team, teams;   // team: threads of one row; teams of a block
   int w_f32;
-  float eps;
+  float eps, inv_cols;
   void* y;              // forward: output; backward: dx
   void* sum;            // forward: h out or null; backward: dr or null
   float* rstd;          // forward: out or null; backward: in
-  int q_e4m3, group;    // 8-bit form: group 0 = one scale a row
+  int group;            // 8-bit form: group 0 = one scale a row
   const float* given;   // given scale or null
   float* scales;
   float* partial;       // backward: dw partial rows [grid * teams, cols] or null
@@ -66,31 +66,83 @@ __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat
 template <>
 __device__ __forceinline__ float from_f(float v) { return v; }
 
-// VEC consecutive elements, VEC 1 or 8 (8: 16-byte aligned).
-template <int VEC, typename T>
-__device__ __forceinline__ void load_v(const T* p, float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    f[0] = to_f<T>(*p);
+// Two elements of a 32-bit word of a 16-bit type (paired conversions: single ones run at a quarter of the rate).
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   } else {
-    __align__(16) T v[VEC];
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// VEC consecutive elements as stored, VEC 1 or 8 (8: 16-byte aligned).
+template <int VEC, typename T>
+struct Raw {
+  uint32_t w[VEC == 1 ? 1 : VEC * (int)sizeof(T) / 4];
+};
+template <int VEC, typename T>
+__device__ __forceinline__ void load_raw(const T* p, Raw<VEC, T>& r) {
+  if constexpr (VEC == 1) {
+    if constexpr (sizeof(T) == 4) r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    else r.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
 #pragma unroll
-    for (int i = 0; i < (int)(VEC * sizeof(T) / 16); ++i)
-      reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = to_f<T>(v[i]);
+    for (int i = 0; i < (int)(VEC * sizeof(T) / 16); ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
+    }
   }
 }
 template <int VEC, typename T>
-__device__ __forceinline__ void store_v(T* p, const float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = from_f<T>(f[0]);
+__device__ __forceinline__ void to_floats(const Raw<VEC, T>& r, float (&f)[VEC]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = __uint_as_float(r.w[i]);
+  } else if constexpr (VEC == 1) {
+    f[0] = unpack2<T>(r.w[0]).x;
   } else {
-    __align__(16) T v[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = from_f<T>(f[i]);
+    for (int i = 0; i < VEC / 2; ++i) {
+      const float2 u = unpack2<T>(r.w[i]);
+      f[2 * i] = u.x, f[2 * i + 1] = u.y;
+    }
+  }
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void load_v(const T* p, float (&f)[VEC]) {
+  Raw<VEC, T> r;
+  load_raw<VEC, T>(p, r);
+  to_floats<VEC, T>(r, f);
+}
+// Stores f; with ROUND, f becomes what was stored.
+template <int VEC, typename T, bool ROUND = false>
+__device__ __forceinline__ void store_v(T* p, float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    const T v = from_f<T>(f[0]);
+    *p = v;
+    if (ROUND) f[0] = to_f<T>(v);
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < (int)(VEC * sizeof(T) / 16); ++i)
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  } else {
+    uint32_t w[VEC / 2];
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+      if (ROUND) {
+        const float2 u = unpack2<T>(w[i]);
+        f[2 * i] = u.x, f[2 * i + 1] = u.y;
+      }
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   }
 }
 // Weight elements [col, col + VEC): the input's type or fp32; ones without a weight.
@@ -107,12 +159,12 @@ __device__ __forceinline__ void load_w(const NormParams& p, int64_t col, float (
 }
 
 // Sum / unsigned maximum over the `team` threads that share a row; `red` holds one word a
-// warp. Every thread of the block calls it the same number of times.
+// warp and is used by one call between two barriers that follow it. Every thread of the block calls it
+// the same number of times.
 __device__ __forceinline__ float team_sum(float v, int team, float* red) {
   v = warp_sum(v);
   if (team == 32) return v;
-  const int warp = threadIdx.x >> 5, per = team >> 5, first = warp / per * per;
-  __syncthreads();
+  const int warp = threadIdx.x >> 5, per = team >> 5, first = team == (int)blockDim.x ? 0 : warp / per * per;
   if ((threadIdx.x & 31) == 0) red[warp] = v;
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -121,8 +173,7 @@ __device__ __forceinline__ float team_sum(float v, int team, float* red) {
 __device__ __forceinline__ uint32_t team_max(uint32_t v, int team, uint32_t* red) {
   v = __reduce_max_sync(0xffffffffu, v);
   if (team == 32) return v;
-  const int warp = threadIdx.x >> 5, per = team >> 5, first = warp / per * per;
-  __syncthreads();
+  const int warp = threadIdx.x >> 5, per = team >> 5, first = team == (int)blockDim.x ? 0 : warp / per * per;
   if ((threadIdx.x & 31) == 0) red[warp] = v;
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -130,78 +181,119 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, int team, uint32_t* red
 }
 
 // ---- 8-bit rounding ---------------------------------------------------------------------
-// The scale of a maximum held as the bits of |y| (a NaN has the largest bits and stays NaN).
-__device__ __forceinline__ float q_scale(uint32_t amax_bits, float qmax) {
-  return amax_bits == 0u ? 1.0f : __fdiv_rn(__uint_as_float(amax_bits), qmax);
+// A maximum that keeps a NaN.
+__device__ __forceinline__ float max_abs(float m, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(y)));
+  return r;
 }
-// Multiplying by RN(1/s) instead of dividing moves a code only where y/s lies within two
-// roundings of a border between two codes. Scales whose reciprocal may overflow divide.
-struct QuantStep {
-  float s, inv;
-  __device__ __forceinline__ float operator()(float y) const {
-    return fabsf(s) < 1e-36f ? __fdiv_rn(y, s) : __fmul_rn(y, inv);
+// The scale of a maximum held as the bits of |y| (a NaN has the largest bits and stays NaN).
+// Multiplying by RN(1/Q), and y by the approximate 1/s (one unit in the last place), instead of dividing
+// moves a scale by one rounding and a code only where y/s lies within three roundings of a border between
+// two codes; two divisions for each eight elements cost as much as the rest of the quantisation.
+template <bool E4M3>
+__device__ __forceinline__ float q_scale(uint32_t amax_bits) {
+  const float s = __fmul_rn(__uint_as_float(amax_bits), E4M3 ? (float)(1.0 / 448.0) : (float)(1.0 / 127.0));
+  return amax_bits == 0u ? 1.0f : s;
+}
+__device__ __forceinline__ float rcp_approx(float x) {   // x normal
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// y / s in place; where the reciprocal may overflow, both are first multiplied by 2^64 (exact there).
+template <int N>
+__device__ __forceinline__ void divide(float (&y)[N], float s) {
+  if (fabsf(s) < 1e-36f) {
+    const float inv = rcp_approx(__fmul_rn(s, 18446744073709551616.0f));
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], 18446744073709551616.0f), inv);
+  } else {
+    const float inv = rcp_approx(s);
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = __fmul_rn(y[e], inv);
   }
-};
-__device__ __forceinline__ QuantStep quant_step(float s) {
-  QuantStep q;
-  q.s = s;
-  q.inv = __frcp_rn(s);
-  return q;
 }
 __device__ __forceinline__ uint32_t code_i8(float t) {
   int q = __float2int_rn(t);                    // NaN -> 0, out of range saturates
   q = max(-127, min(127, q));
   return (uint32_t)q & 0xffu;
 }
-template <int VEC>
-__device__ __forceinline__ void store_q(uint8_t* p, const float (&t)[VEC], bool e4m3) {
+template <int VEC, bool E4M3>
+__device__ __forceinline__ void store_q(uint8_t* p, const float (&t)[VEC]) {
   if constexpr (VEC == 1) {
-    *p = e4m3 ? (uint8_t)__nv_cvt_float_to_fp8(t[0], __NV_SATFINITE, __NV_E4M3) : (uint8_t)code_i8(t[0]);
+    *p = E4M3 ? (uint8_t)__nv_cvt_float_to_fp8(t[0], __NV_SATFINITE, __NV_E4M3) : (uint8_t)code_i8(t[0]);
   } else {
-    uint32_t w[2] = {0, 0};
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) w[i] = 0;
 #pragma unroll
     for (int i = 0; i < VEC; i += 2) {
-      const uint32_t two = e4m3 ? (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[i], t[i + 1]), __NV_SATFINITE,
+      const uint32_t two = E4M3 ? (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[i], t[i + 1]), __NV_SATFINITE,
                                                                       __NV_E4M3)
                                 : (code_i8(t[i]) | (code_i8(t[i + 1]) << 8));
       w[i >> 2] |= two << (8 * (i & 3));
     }
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+}
+
+// A thread's place: its row's team in the block, its index there.
+__device__ __forceinline__ void place(int team, int& who, int& t) {
+  if (team == (int)blockDim.x) {
+    who = 0;
+    t = threadIdx.x;
+  } else {
+    who = threadIdx.x / team;
+    t = threadIdx.x - who * team;
   }
 }
 
 // ---- forward ------------------------------------------------------------------------------
-// One team of threads per row, up to E = VEC * NV elements a thread.
-template <typename TX, typename TH, int VEC, int NV, bool QUANT, int MAXT>
+// One team of threads per row, up to VEC * NV elements a thread. QUANT: 0 none, 1 int8, 2 e4m3.
+template <typename TX, typename TH, int VEC, int NV, int QUANT, int MAXT>
 __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ NormParams p) {
   __shared__ float red[32];
-  __shared__ uint32_t gmax[VEC == 1 && QUANT ? 1024 + 32 : 1];
-  const int t = threadIdx.x % p.team, teams = blockDim.x / p.team, who = threadIdx.x / p.team;
-  const int64_t row = (int64_t)blockIdx.x * teams + who;
-  const bool live = row < p.rows;
+  __shared__ uint32_t red_max[QUANT != 0 ? 32 : 1];
+  __shared__ uint32_t gmax[VEC == 1 && QUANT != 0 ? 1024 + 32 : 1];
+  constexpr bool E4M3 = QUANT == 2;
+  int who, t;
+  place(p.team, who, t);
   const int nvec = (p.cols + VEC - 1) / VEC;
-  float v[NV][VEC];
+  const int64_t row = (int64_t)blockIdx.x * p.teams + who;
+  const bool live = row < p.rows;
   grid_dep_wait();
   grid_dep_launch();
 
+  // every load of the row is issued before the first is used
+  Raw<VEC, TX> xn[NV];
+  Raw<VEC, TH> rn[NV];
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = i * p.team + t;
+      if (k < nvec) {
+        load_raw<VEC, TX>(static_cast<const TX*>(p.x) + row * p.ldx + (int64_t)k * VEC, xn[i]);
+        if (p.r != nullptr) load_raw<VEC, TH>(static_cast<const TH*>(p.r) + row * p.ldr + (int64_t)k * VEC, rn[i]);
+      }
+    }
+  }
+  float v[NV][VEC];
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = i * p.team + t;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
-    if (live && k < nvec) load_v<VEC, TX>(static_cast<const TX*>(p.x) + row * p.ldx + (int64_t)k * VEC, v[i]);
-  }
-  if (p.r != nullptr) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = i * p.team + t;
-      if (live && k < nvec) {
+    if (live && k < nvec) {
+      to_floats<VEC, TX>(xn[i], v[i]);
+      if (p.r != nullptr) {
         float r[VEC];
-        load_v<VEC, TH>(static_cast<const TH*>(p.r) + row * p.ldr + (int64_t)k * VEC, r);
+        to_floats<VEC, TH>(rn[i], r);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = to_f<TH>(from_f<TH>(__fadd_rn(v[i][e], r[e])));
-        store_v<VEC, TH>(static_cast<TH*>(p.sum) + row * p.cols + (int64_t)k * VEC, v[i]);
+        for (int e = 0; e < VEC; ++e) v[i][e] = __fadd_rn(v[i][e], r[e]);
+        store_v<VEC, TH, true>(static_cast<TH*>(p.sum) + row * p.cols + (int64_t)k * VEC, v[i]);
       }
     }
   }
@@ -210,10 +302,9 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) ss = fmaf(v[i][e], v[i][e], ss);
   ss = team_sum(ss, p.team, red);
-  const float rstd = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)p.cols), p.eps)));
+  const float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps));   // within 2 units in the last place
   if (p.rstd != nullptr && live && t == 0) p.rstd[row] = rstd;
 
-  uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = i * p.team + t;
@@ -221,54 +312,52 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
       float w[VEC];
       load_w<VEC, TX>(p, (int64_t)k * VEC, w);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rstd), w[e]);
-        if (QUANT) amax = max(amax, __float_as_uint(v[i][e]) & 0x7fffffffu);
-      }
-      if (!QUANT) store_v<VEC, TX>(static_cast<TX*>(p.y) + row * p.cols + (int64_t)k * VEC, v[i]);
+      for (int e = 0; e < VEC; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rstd), w[e]);
+      if (QUANT == 0) store_v<VEC, TX>(static_cast<TX*>(p.y) + row * p.cols + (int64_t)k * VEC, v[i]);
     }
   }
-  if constexpr (QUANT) {
-    const float qmax = p.q_e4m3 ? 448.0f : 127.0f;
+  if constexpr (QUANT != 0) {
     uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.cols;
     if (p.group == 0) {
       float s;
       if (p.given != nullptr) {
         s = *p.given;
       } else {
-        s = q_scale(team_max(amax, p.team, reinterpret_cast<uint32_t*>(red)), qmax);
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) amax = max_abs(amax, v[i][e]);
+        s = q_scale<E4M3>(team_max(__float_as_uint(amax), p.team, red_max));
         if (live && t == 0) p.scales[row] = s;
       }
-      const QuantStep step = quant_step(s);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int k = i * p.team + t;
         if (live && k < nvec) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) v[i][e] = step(v[i][e]);
-          store_q<VEC>(q + (int64_t)k * VEC, v[i], p.q_e4m3);
+          divide(v[i], s);
+          store_q<VEC, E4M3>(q + (int64_t)k * VEC, v[i]);
         }
       }
     } else {
       const int groups = (p.cols + p.group - 1) / p.group;
       float* scales = p.scales + row * groups;
       if constexpr (VEC > 1) {
-        // a group is 4, 8 or 16 neighbouring lanes
+        // a group is 4 to 32 neighbouring lanes
         const int lanes = p.group / VEC;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int k = i * p.team + t;
-          uint32_t m = 0;
+          float big = 0.0f;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
+          for (int e = 0; e < VEC; ++e) big = max_abs(big, v[i][e]);
+          uint32_t m = __float_as_uint(big);
           for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
           if (live && k < nvec) {
-            const float s = q_scale(m, qmax);
+            const float s = q_scale<E4M3>(m);
             if ((k & (lanes - 1)) == 0) scales[k / lanes] = s;
-            const QuantStep step = quant_step(s);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[i][e] = step(v[i][e]);
-            store_q<VEC>(q + (int64_t)k * VEC, v[i], p.q_e4m3);
+            divide(v[i], s);
+            store_q<VEC, E4M3>(q + (int64_t)k * VEC, v[i]);
           }
         }
       } else {
@@ -284,13 +373,13 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
         }
         __syncthreads();
         if (live)
-          for (int g = t; g < groups; g += p.team) scales[g] = q_scale(gm[g], qmax);
+          for (int g = t; g < groups; g += p.team) scales[g] = q_scale<E4M3>(gm[g]);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int k = i * p.team + t;
           if (live && k < nvec) {
-            const float one[1] = {quant_step(q_scale(gm[k / p.group], qmax))(v[i][0])};
-            store_q<1>(q + k, one, p.q_e4m3);
+            divide(v[i], q_scale<E4M3>(gm[k / p.group]));
+            store_q<1, E4M3>(q + k, v[i]);
           }
         }
       }
@@ -302,10 +391,14 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
 // A team walks rows team_id, team_id + teams, ...; its columns' share of dw stays in
 // registers and is written once as a partial row, which norm_dw_kernel sums in a fixed order.
 template <typename TX, typename TH, int VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float red[32];
-  const int t = threadIdx.x % p.team, teams = blockDim.x / p.team, who = threadIdx.x / p.team;
+__global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) norm_bwd_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float red[2][32];                           // rows use them in turn: one barrier a row
+  int who, t, parity = 0;
+  place(p.team, who, t);
+  const int teams = p.teams;
   const int nvec = (p.cols + VEC - 1) / VEC;
+  grid_dep_wait();
+  grid_dep_launch();
   float acc[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -341,8 +434,9 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const __grid_constant__ 
         }
       }
     }
-    dot = team_sum(dot, p.team, red);
-    const float c = __fmul_rn(__fmul_rn(rstd, rstd), __fdiv_rn(dot, (float)p.cols));
+    dot = team_sum(dot, p.team, red[parity]);
+    parity ^= 1;
+    const float c = __fmul_rn(__fmul_rn(rstd, rstd), __fmul_rn(dot, p.inv_cols));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int k = i * p.team + t;
@@ -378,8 +472,18 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* partial, int
   __shared__ float s[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float v = 0.0f;
-  if (c < cols)
-    for (int i = threadIdx.y; i < n; i += 32) v += partial[(int64_t)i * cols + c];
+  grid_dep_wait();
+  if (c < cols) {
+    int i = threadIdx.y;
+    for (; i + 7 * 32 < n; i += 8 * 32) {                // eight loads in flight
+      float u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = partial[(int64_t)(i + k * 32) * cols + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += u[k];
+    }
+    for (; i < n; i += 32) v += partial[(int64_t)i * cols + c];
+  }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   v = warp_sum(s[threadIdx.x][threadIdx.y]);
@@ -401,65 +505,70 @@ int num_sms() {
 }
 
 struct Shape {
-  int team, threads;
-  bool wide;            // 32 elements a thread instead of 8
+  int team, teams;      // threads of a row, rows of a block
+  int elems;            // elements a thread holds: 8, 16 or 32
 };
 Shape shape_of(int64_t rows, int cols) {
   Shape s;
-  // few rows: as many threads a row as there are 8-element pieces (latency); many rows: 32
-  // elements a thread, so that a thread has several loads in flight and a row fewer warps
-  s.wide = rows > 2 * num_sms() || cols > 8192;
-  const int e = s.wide ? 32 : 8;
-  s.team = ((cols + e - 1) / e + 31) / 32 * 32;
-  s.threads = s.team >= 256 ? s.team : 256 / s.team * s.team;
-  if (!s.wide) s.threads = s.team;
+  // Up to one 8-element piece for each thread the GPU holds: as many threads a row as it has pieces
+  // (latency). More: 16 elements a thread, so that a thread has several loads in flight and a row fewer
+  // warps (8192 x 4096 forward, bf16 with an f32 sum: 69 us with 32, 63 us with 16 = the copy bandwidth;
+  // 1003 x 1111 f16 forward + backward: 85 us with 32, 21 us with 8). 32 where a block could not hold the row.
+  s.elems = cols > 16384 ? 32 : rows * cols > (int64_t)num_sms() * 2048 * 8 || cols > 8192 ? 16 : 8;
+  s.team = ((cols + s.elems - 1) / s.elems + 31) / 32 * 32;
+  s.teams = s.elems == 8 || s.team >= 256 ? 1 : 256 / s.team;
   return s;
 }
 
-template <typename TX, typename TH, bool QUANT>
+template <typename TX, typename TH, int QUANT>
 cudaError_t launch_fwd(NormParams p, bool vec, cudaStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   p.team = s.team;
-  const int teams = s.threads / s.team;
-  const dim3 grid((unsigned)((p.rows + teams - 1) / teams)), block((unsigned)s.threads);
-  if (!s.wide)
+  p.teams = s.teams;
+  const int threads = s.team * s.teams;
+  const dim3 grid((unsigned)((p.rows + s.teams - 1) / s.teams)), block((unsigned)threads);
+  if (s.elems == 8)
     return vec ? launch_k(norm_fwd_kernel<TX, TH, 8, 1, QUANT, 1024>, grid, block, 0, st, true, p)
                : launch_k(norm_fwd_kernel<TX, TH, 1, 8, QUANT, 1024>, grid, block, 0, st, true, p);
-  if (s.threads <= 512)
-    return vec ? launch_k(norm_fwd_kernel<TX, TH, 8, 4, QUANT, 512>, grid, block, 0, st, true, p)
-               : launch_k(norm_fwd_kernel<TX, TH, 1, 32, QUANT, 512>, grid, block, 0, st, true, p);
+  if (s.elems == 16 && threads <= 512)
+    return vec ? launch_k(norm_fwd_kernel<TX, TH, 8, 2, QUANT, 512>, grid, block, 0, st, true, p)
+               : launch_k(norm_fwd_kernel<TX, TH, 1, 16, QUANT, 512>, grid, block, 0, st, true, p);
+  if (s.elems == 16)
+    return vec ? launch_k(norm_fwd_kernel<TX, TH, 8, 2, QUANT, 1024>, grid, block, 0, st, true, p)
+               : launch_k(norm_fwd_kernel<TX, TH, 1, 16, QUANT, 1024>, grid, block, 0, st, true, p);
   return vec ? launch_k(norm_fwd_kernel<TX, TH, 8, 4, QUANT, 1024>, grid, block, 0, st, true, p)
              : launch_k(norm_fwd_kernel<TX, TH, 1, 32, QUANT, 1024>, grid, block, 0, st, true, p);
 }
 
-int64_t bwd_teams(int64_t rows) {
-  const int64_t t = (rows + kNormRowsPerTeam - 1) / kNormRowsPerTeam;
-  return t < kNormMaxPartials ? t : kNormMaxPartials;
-}
+int64_t bwd_teams(int64_t rows) { return rows < kNormMaxPartials ? rows : kNormMaxPartials; }
 
 template <typename TX, typename TH>
 cudaError_t launch_bwd(NormParams p, bool vec, void* dw, int dw_f32, cudaStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   p.team = s.team;
-  const int teams = s.threads / s.team;
-  int64_t blocks = bwd_teams(p.rows) / teams;
+  p.teams = s.teams;
+  const int threads = s.team * s.teams;
+  int64_t blocks = bwd_teams(p.rows) / s.teams;
   if (blocks < 1) blocks = 1;
-  const dim3 grid((unsigned)blocks), block((unsigned)s.threads);
+  const dim3 grid((unsigned)blocks), block((unsigned)threads);
   cudaError_t e;
-  if (!s.wide)
-    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 1, 1024>, grid, block, 0, st, false, p)
-            : launch_k(norm_bwd_kernel<TX, TH, 1, 8, 1024>, grid, block, 0, st, false, p);
-  else if (s.threads <= 512)
-    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 4, 512>, grid, block, 0, st, false, p)
-            : launch_k(norm_bwd_kernel<TX, TH, 1, 32, 512>, grid, block, 0, st, false, p);
+  if (s.elems == 8)
+    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 1, 1024>, grid, block, 0, st, true, p)
+            : launch_k(norm_bwd_kernel<TX, TH, 1, 8, 1024>, grid, block, 0, st, true, p);
+  else if (s.elems == 16 && threads <= 512)
+    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 2, 512>, grid, block, 0, st, true, p)
+            : launch_k(norm_bwd_kernel<TX, TH, 1, 16, 512>, grid, block, 0, st, true, p);
+  else if (s.elems == 16)
+    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 2, 1024>, grid, block, 0, st, true, p)
+            : launch_k(norm_bwd_kernel<TX, TH, 1, 16, 1024>, grid, block, 0, st, true, p);
   else
-    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 4, 1024>, grid, block, 0, st, false, p)
-            : launch_k(norm_bwd_kernel<TX, TH, 1, 32, 1024>, grid, block, 0, st, false, p);
+    e = vec ? launch_k(norm_bwd_kernel<TX, TH, 8, 4, 1024>, grid, block, 0, st, true, p)
+            : launch_k(norm_bwd_kernel<TX, TH, 1, 32, 1024>, grid, block, 0, st, true, p);
   if (e != cudaSuccess || dw == nullptr) return e;
   const dim3 g2((unsigned)((p.cols + 31) / 32)), b2(32, 32);
-  const int n = (int)(blocks * teams);
-  if (dw_f32) return launch_k(norm_dw_kernel<float>, g2, b2, 0, st, false, (const float*)p.partial, n, p.cols, (float*)dw);
-  return launch_k(norm_dw_kernel<TX>, g2, b2, 0, st, false, (const float*)p.partial, n, p.cols, (TX*)dw);
+  const int n = (int)(blocks * s.teams);
+  if (dw_f32) return launch_k(norm_dw_kernel<float>, g2, b2, 0, st, true, (const float*)p.partial, n, p.cols, (float*)dw);
+  return launch_k(norm_dw_kernel<TX>, g2, b2, 0, st, true, (const float*)p.partial, n, p.cols, (TX*)dw);
 }
 
 // ---- argument checks ------------------------------------------------------------------------
@@ -509,7 +618,7 @@ const char* common_wrong(int x_dtype, int h_dtype, const void* w, int w_dtype, i
 
 int forward_call(const char* who, const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype,
                  int64_t ldr, const void* weight, int w_dtype, int64_t rows, int cols, float eps, void* sum_out,
-                 NormParams p, bool quant, void* stream) {
+                 NormParams p, int quant, void* stream) {
   const int h_dtype = residual ? r_dtype : x_dtype;
   const char* why = common_wrong(x_dtype, h_dtype, weight, w_dtype, rows, cols);
   if (why) return bad(who, why);
@@ -530,6 +639,7 @@ int forward_call(const char* who, const void* x, int x_dtype, int64_t ldx, const
   p.cols = cols;
   p.w_f32 = w_dtype == GLAD_DTYPE_F32;
   p.eps = eps;
+  p.inv_cols = 1.0f / (float)cols;
   p.sum = sum_out;
   const bool vec = cols % 8 == 0 && vec_ok(x, x_dtype, ldx, rows) && vec_ok(residual, h_dtype, ldr, rows) &&
                    on(weight, 16) && on(sum_out, 16) && on(p.y, quant ? 8 : 16);
@@ -537,7 +647,9 @@ int forward_call(const char* who, const void* x, int x_dtype, int64_t ldx, const
   return for_types(x_dtype, h_dtype, [&](auto tx, auto th) {
     using TX = decltype(tx);
     using TH = decltype(th);
-    const cudaError_t e = quant ? launch_fwd<TX, TH, true>(p, vec, st) : launch_fwd<TX, TH, false>(p, vec, st);
+    const cudaError_t e = quant == 0   ? launch_fwd<TX, TH, 0>(p, vec, st)
+                          : quant == 1 ? launch_fwd<TX, TH, 1>(p, vec, st)
+                                       : launch_fwd<TX, TH, 2>(p, vec, st);
     return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
   });
 }
@@ -556,7 +668,7 @@ int glad_rms_norm_forward(const void* x, int x_dtype, int64_t ldx, const void* r
   p.y = y;
   p.rstd = rstd_out;
   return forward_call("glad_rms_norm_forward", x, x_dtype, ldx, residual, r_dtype, ldr, weight, w_dtype, rows, cols,
-                      eps, sum_out, p, false, stream);
+                      eps, sum_out, p, 0, stream);
 }
 
 int glad_rms_norm_quant(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr,
@@ -570,12 +682,11 @@ int glad_rms_norm_quant(const void* x, int x_dtype, int64_t ldx, const void* res
   if (!on(given_scale, 4) || !on(scales, 4)) return bad(who, "scales must be 4-byte aligned");
   NormParams p{};
   p.y = q;
-  p.q_e4m3 = q_dtype == GLAD_DTYPE_E4M3;
   p.group = group;
   p.given = given_scale;
   p.scales = scales;
-  return forward_call(who, x, x_dtype, ldx, residual, r_dtype, ldr, weight, w_dtype, rows, cols, eps, sum_out, p, true,
-                      stream);
+  return forward_call(who, x, x_dtype, ldx, residual, r_dtype, ldr, weight, w_dtype, rows, cols, eps, sum_out, p,
+                      q_dtype == GLAD_DTYPE_E4M3 ? 2 : 1, stream);
 }
 
 size_t glad_rms_norm_backward_workspace_size(int64_t rows, int cols) {
@@ -622,6 +733,7 @@ int glad_rms_norm_backward(const void* dy, int x_dtype, int64_t lddy, const void
   p.w_f32 = w_dtype == GLAD_DTYPE_F32;
   p.rows = rows;
   p.cols = cols;
+  p.inv_cols = 1.0f / (float)cols;
   p.y = dx;
   p.sum = dresidual;
   p.rstd = const_cast<float*>(rstd);
