@@ -11,7 +11,7 @@ The public API mirrors qrt (qrt/__init__.py:18-34):
 
 Beside them, for the blocks around quantised layers (no qrt counterpart):
     rms_norm, rms_norm_quant, RMSNorm     add + RMS norm, 16/32-bit (trains) or 8-bit output
-    w4_linear, W4Linear, W4Weight, pack_w4, unpack_w4   4-bit linear of any shape
+    w4_linear, W4Linear, W4Weight, pack_w4, unpack_w4, w4_status   4-bit linear of any shape
 
 Names are resolved lazily, so importing a light submodule (``synthetic``,
 ``glad_model``) neither loads the CUDA library nor registers the qrt
@@ -32,7 +32,7 @@ _EXPORTS = {
     "FusedActor": "fused", "DeviceStatusError": "fused",
     "rms_norm": "norm", "rms_norm_quant": "norm", "RMSNorm": "norm",
     "w4_linear": "w4linear", "W4Linear": "w4linear", "W4Weight": "w4linear", "pack_w4": "w4linear",
-    "unpack_w4": "w4linear",
+    "unpack_w4": "w4linear", "w4_status": "w4linear",
     "GladActorCritic": "glad_model", "build_glad": "glad_model",
 }
 _SUBMODULES = ("swap", "calib", "_native", "synthetic", "glad_model", "qconv", "qlinear", "encoder_opt",

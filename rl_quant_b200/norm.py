@@ -54,32 +54,27 @@ def _rows(t):
 
 def _like(t, dtype=None):
     """Contiguous and uninitialised, of t's shape (empty_like is the cheaper call)."""
-    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+    if not t.is_contiguous():
+        return t.new_empty(t.shape, dtype=dtype)
+    return torch.empty_like(t) if dtype is None else torch.empty_like(t, dtype=dtype)
 
 
-def _inputs(x, weight, residual):
-    """The first arguments of both forward entry points, the tensors they point into and the sum's buffer."""
-    x2 = _rows(x)
+def _forward(x, weight, residual, eps, rstd):
+    """(y, h or None); ``rstd`` None or f32 [rows] to fill."""
+    x2 = x if x.dim() == 2 and x.stride(1) == 1 else _rows(x)
     rows, cols = x2.shape
-    wp, wt, rp, rt, ldr, h, r2 = None, 0, None, 0, 0, None, None
+    y = _like(x)
+    wp, wt, rp, rt, ldr, h, hp = None, 0, None, 0, 0, None, None
     if weight is not None:
         if not weight.is_contiguous():
             weight = weight.contiguous()
         wp, wt = weight.data_ptr(), _CODE[weight.dtype]
     if residual is not None:
         r2 = _rows(residual)
-        rp, rt, ldr = r2.data_ptr(), _CODE[residual.dtype], r2.stride(0)
         h = _like(residual)
-    args = (x2.data_ptr(), _CODE[x.dtype], x2.stride(0), rp, rt, ldr, wp, wt, rows, cols)
-    return args, (x2, weight, r2), h
-
-
-def _forward(x, weight, residual, eps, rstd):
-    """(y, h or None); ``rstd`` None or f32 [rows] to fill."""
-    args, keep, h = _inputs(x, weight, residual)
-    y = _like(x)
-    rc = N.on_device(N.load().glad_rms_norm_forward, x.device.index, *args, eps, y.data_ptr(),
-                     None if h is None else h.data_ptr(), None if rstd is None else rstd.data_ptr())
+        rp, rt, ldr, hp = r2.data_ptr(), _CODE[residual.dtype], r2.stride(0), h.data_ptr()
+    rc = N.on_device(N.load().glad_rms_norm_forward, x.device.index, x2.data_ptr(), _CODE[x.dtype], x2.stride(0), rp, rt,
+                     ldr, wp, wt, rows, cols, eps, y.data_ptr(), hp, None if rstd is None else rstd.data_ptr())
     if rc:
         N.check(rc, "rms_norm")
     return y, h
@@ -167,15 +162,27 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_quant has no gradient; use rms_norm, or torch.no_grad()")
     _check(x, weight, residual, eps)
-    args, keep, h = _inputs(x, weight, residual)
+    x2 = x if x.dim() == 2 and x.stride(1) == 1 else _rows(x)
+    rows, cols = x2.shape
     q = _like(x, out_dtype)
-    s = scale
+    s, sp, gp = scale, None, None
     if s is None:
-        s = x.new_empty(x.shape[:-1] + (-(-x.shape[-1] // group) if group else 1,), dtype=torch.float32)
-    rc = N.on_device(N.load().glad_rms_norm_quant, x.device.index, *args, eps,
-                     N.DTYPE_I8 if out_dtype == torch.int8 else N.DTYPE_E4M3, group,
-                     None if scale is None else scale.data_ptr(), q.data_ptr(), None if scale is not None else s.data_ptr(),
-                     None if h is None else h.data_ptr())
+        s = x.new_empty(x.shape[:-1] + (-(-cols // group) if group else 1,), dtype=torch.float32)
+        sp = s.data_ptr()
+    else:
+        gp = s.data_ptr()
+    wp, wt, rp, rt, ldr, h, hp = None, 0, None, 0, 0, None, None
+    if weight is not None:
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        wp, wt = weight.data_ptr(), _CODE[weight.dtype]
+    if residual is not None:
+        r2 = _rows(residual)
+        h = _like(residual)
+        rp, rt, ldr, hp = r2.data_ptr(), _CODE[residual.dtype], r2.stride(0), h.data_ptr()
+    rc = N.on_device(N.load().glad_rms_norm_quant, x.device.index, x2.data_ptr(), _CODE[x.dtype], x2.stride(0), rp, rt, ldr,
+                     wp, wt, rows, cols, eps, N.DTYPE_I8 if out_dtype == torch.int8 else N.DTYPE_E4M3, group, gp,
+                     q.data_ptr(), sp, hp)
     if rc:
         N.check(rc, "rms_norm_quant")
     return (q, s) if h is None else (q, s, h)

@@ -7,6 +7,8 @@ the group's scale multiplies the group's sum: y = sum_g s[n,g] * (sum_k x[m,k] q
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -27,7 +29,7 @@ def _shapes(in_features: int, out_features: int, group: int):
 class W4Weight:
     """A laid-out 4-bit weight [out_features, in_features]: ``tiles`` (uint8) and ``scales`` (fp16) on one device."""
 
-    __slots__ = ("tiles", "scales", "in_features", "out_features", "group")
+    __slots__ = ("_tiles", "_scales", "_shape")
 
     def __init__(self, tiles, scales, in_features, out_features, group):
         if group not in GROUPS:
@@ -41,8 +43,13 @@ class W4Weight:
             raise ValueError(f"scales must be contiguous float16 {s_shape}")
         if tiles.device != scales.device:
             raise ValueError(f"tiles on {tiles.device}, scales on {scales.device}")
-        self.tiles, self.scales = tiles, scales
-        self.in_features, self.out_features, self.group = in_features, out_features, group
+        self._tiles, self._scales, self._shape = tiles, scales, (in_features, out_features, group)
+
+    tiles = property(lambda self: self._tiles)
+    scales = property(lambda self: self._scales)
+    in_features = property(lambda self: self._shape[0])
+    out_features = property(lambda self: self._shape[1])
+    group = property(lambda self: self._shape[2])
 
 
 @torch.no_grad()
@@ -88,58 +95,77 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
     x float16 or bfloat16 (``x_scale`` None, ``out_dtype`` x's by default), or int8 / float8_e4m3fn codes with a float32
     ``x_scale`` of one value, [..., 1] (one a row) or [..., ceil(K / group)] (one a row and group of the weight) and
     ``out_dtype`` named. out_dtype float16, bfloat16 or float32; bias [N] has it. Inference only."""
-    K, n = weight.in_features, weight.out_features
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"x {tuple(x.shape)} does not match in_features {K}")
-    eight = x.dtype in (torch.int8, torch.float8_e4m3fn)
-    if not eight and x.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"x is {x.dtype}; expected float16, bfloat16, int8 or float8_e4m3fn")
+    K, n, group = weight._shape
+    shape, dt = x.shape, x.dtype
+    if not shape or shape[-1] != K:
+        raise ValueError(f"x {tuple(shape)} does not match in_features {K}")
+    eight = dt == torch.int8 or dt == torch.float8_e4m3fn
+    if not eight and dt != torch.float16 and dt != torch.bfloat16:
+        raise TypeError(f"x is {dt}; expected float16, bfloat16, int8 or float8_e4m3fn")
     if out_dtype is None:
         if eight:
             raise ValueError("8-bit rows need out_dtype")
-        out_dtype = x.dtype
+        out_dtype = dt
     if out_dtype not in _OUT:
         raise TypeError(f"out_dtype is {out_dtype}; expected float16, bfloat16 or float32")
+    dev = x.device
     per_row = groups = 0
+    xp = bp = None
     if eight:
         if x_scale is None:
             raise ValueError("8-bit rows need x_scale")
         if x_scale.dtype != torch.float32:
             raise TypeError(f"x_scale is {x_scale.dtype}; expected float32")
-        if x_scale.numel() != 1 or x_scale.shape == x.shape[:-1] + (1,):
-            g = -(-K // weight.group)
-            if x_scale.shape == x.shape[:-1] + (1,):
-                per_row, groups = 1, 1
-            elif x_scale.shape == x.shape[:-1] + (g,):
-                per_row, groups = 1, g
-            else:
-                raise ValueError(f"x_scale {tuple(x_scale.shape)}: one value, {tuple(x.shape[:-1]) + (1,)} or "
-                                 f"{tuple(x.shape[:-1]) + (g,)}")
-            if not x_scale.is_contiguous():
-                x_scale = x_scale.contiguous()
+        if x_scale.shape == shape[:-1] + (1,):
+            per_row, groups = 1, 1
+        elif x_scale.numel() != 1:
+            per_row, groups = 1, -(-K // group)
+            if x_scale.shape != shape[:-1] + (groups,):
+                raise ValueError(f"x_scale {tuple(x_scale.shape)}: one value, {tuple(shape[:-1]) + (1,)} or "
+                                 f"{tuple(shape[:-1]) + (groups,)}")
+        if x_scale.device != dev:
+            raise ValueError(f"tensors on {dev} and {x_scale.device}")
+        if not x_scale.is_contiguous():
+            x_scale = x_scale.contiguous()
+        xp = x_scale.data_ptr()
     elif x_scale is not None:
         raise ValueError("x_scale is for 8-bit rows")
-    if bias is not None and (bias.shape != (n,) or bias.dtype != out_dtype):
-        raise ValueError(f"bias must be {out_dtype} [{n}]")
-    for t in (weight.tiles, bias, x_scale):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"tensors on {x.device} and {t.device}")
+    if weight._tiles.device != dev:
+        raise ValueError(f"tensors on {dev} and {weight._tiles.device}")
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != out_dtype:
+            raise ValueError(f"bias must be {out_dtype} [{n}]")
+        if bias.device != dev:
+            raise ValueError(f"tensors on {dev} and {bias.device}")
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+        bp = bias.data_ptr()
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("w4_linear has no gradient; use torch.no_grad()")
     N.require_cuda(x)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    y = x.new_empty(x.shape[:-1] + (n,), dtype=out_dtype)
-    w = N.GladW4Weight(weight.tiles.data_ptr(), weight.scales.data_ptr(), K, n, weight.group)
-    rc = N.on_device(N.load().glad_w4_linear_forward, x.device.index, w, x2.data_ptr(), N.DTYPES[x.dtype], x2.shape[0],
-                     x2.stride(0), None if x_scale is None else x_scale.data_ptr(), per_row, groups,
-                     None if bias is None else bias.data_ptr(), y.data_ptr(), N.DTYPES[out_dtype])
+    y = x.new_empty(shape[:-1] + (n,), dtype=out_dtype)
+    w = N.GladW4Weight(weight._tiles.data_ptr(), weight._scales.data_ptr(), K, n, group)
+    rc = N.on_device(N.load().glad_w4_linear_forward, dev.index, w, x2.data_ptr(), N.DTYPES[dt], x2.shape[0],
+                     x2.stride(0), xp, per_row, groups, bp, y.data_ptr(), N.DTYPES[out_dtype])
     if rc:
         N.check(rc, "w4_linear")
     return y
+
+
+def w4_status(device=None) -> int:
+    """Device status bits of the w4_linear calls on ``device`` since the last call (0: fine); reads, clears and, where a
+    bounded wait inside a kernel ran out, raises ``DeviceStatusError``. Synchronises the current stream."""
+    from .fused import DeviceStatusError
+    word = ctypes.c_uint32(0)
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        rc = N.load().glad_w4_linear_status(word, N.stream_handle())
+    if rc == N.GLAD_ERR_DEVICE:
+        raise DeviceStatusError(f"w4_linear: device status {word.value:#x}")
+    N.check(rc, "w4_status")
+    return word.value
 
 
 class W4Linear(nn.Module):
