@@ -4,7 +4,7 @@
 //   h = x + r, rounded to r's type (h = x without a residual)
 //   rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * w
 //   8 bits: s = max|y| / Q over a row or a group of columns (Q = 127 int8, 448 e4m3;
-//           1 where the maximum is 0), q = round_half_even(y * (1/s)); or s is given.
+//           1 where that is 0 in fp32), q = round_half_even(y * (1/s)); or s is given.
 //   backward, g = dy * w:  dh' = dh + rstd * (g - h * rstd^2 * mean(g * h)),
 //           dx = dr = dh',  dw = sum over rows of dy * h * rstd
 //
@@ -194,7 +194,7 @@ __device__ __forceinline__ float max_abs(float m, float y) {
 template <bool E4M3>
 __device__ __forceinline__ float q_scale(uint32_t amax_bits) {
   const float s = __fmul_rn(__uint_as_float(amax_bits), E4M3 ? (float)(1.0 / 448.0) : (float)(1.0 / 127.0));
-  return amax_bits == 0u ? 1.0f : s;
+  return s == 0.0f ? 1.0f : s;                  // a row of zeros, or of values whose scale rounds to zero
 }
 __device__ __forceinline__ float rcp_approx(float x) {   // x normal
   float r;

@@ -147,7 +147,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
     """``(q, s)``, or ``(q, s, h)`` with a residual: the norm rounded to int8 or float8_e4m3fn codes, q * s ~ y.
 
     ``scale`` None: s = max|y| / 127 (448) of each row (``group`` 0, s [..., 1]) or of each ``group`` (32, 64, 128)
-    columns of a row (s [..., ceil(C / group)]), 1 where the maximum is 0. ``scale`` a float32 tensor of one value: that
+    columns of a row (s [..., ceil(C / group)]), 1 where that is 0. ``scale`` a float32 tensor of one value: that
     scale for all (static calibration), returned as s. Inference only: inputs that require a gradient are refused
     while gradients are enabled (``rms_norm`` is the form that trains)."""
     if out_dtype != torch.int8 and out_dtype != torch.float8_e4m3fn:

@@ -322,6 +322,19 @@ def test_module():
     with torch.no_grad():
         q, s = m.quant(x, out_dtype=torch.float8_e4m3fn, group=64)
     assert q.shape == x.shape and s.shape == (9, 5)
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+def test_quant_scale_that_rounds_to_zero(out):
+    """A largest value below half the smallest subnormal times Q has a scale of zero: the scale is 1, all codes are 0."""
+    x = torch.zeros(2, 64, device="cuda")
+    x[:, 3] = 1.0
+    w = torch.full((64,), 2.0 ** -149 * 5, device="cuda")       # y[:, 3] is about 8 * 5 * 2^-149
+    for group in (0, 32):
+        for wide in (x, torch.cat((x, x), 1)[:, 1:64]):
+            q, s = rms_norm_quant(wide, w[:wide.shape[1]], out_dtype=out, group=group)
+            assert torch.equal(s, torch.ones_like(s)) and not q.float().any()
+
+
 
 
 # -- refusals (no GPU) -----------------------------------------------------------------------------
