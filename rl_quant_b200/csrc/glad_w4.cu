@@ -116,12 +116,12 @@ __device__ __forceinline__ uint4 load_raw8(const T* row, int k, int K, bool fast
   }
   return v;
 }
-// ... as the four half2 (bf16x2) the products take; 8-bit inputs are exact in fp16.
+// ... as the four half2 (bf16x2) the products take; e4m3 is exact in fp16.
 template <typename T>
 __device__ __forceinline__ uint4 to_halves(uint4 v) {
   if constexpr (sizeof(T) == 2) {
     return v;
-  } else if constexpr (std::is_same<T, e4m3_t>::value) {
+  } else {
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -131,13 +131,6 @@ __device__ __forceinline__ uint4 to_halves(uint4 v) {
       r[i] = (uint32_t)h.x | ((uint32_t)h.y << 16);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
-  } else {
-    // x + 128 in a byte; 0x6400 | u is the half 1024 + u = 1152 + x
-    const uint32_t a = v.x ^ 0x80808080u, b = v.y ^ 0x80808080u;
-    return make_uint4(h2_sub(__byte_perm(a, 0x64646464u, 0x4140), 0x64806480u),
-                      h2_sub(__byte_perm(a, 0x64646464u, 0x4342), 0x64806480u),
-                      h2_sub(__byte_perm(b, 0x64646464u, 0x4140), 0x64806480u),
-                      h2_sub(__byte_perm(b, 0x64646464u, 0x4342), 0x64806480u));
   }
 }
 
@@ -409,7 +402,7 @@ __global__ void __launch_bounds__(512, 1) w4_rows_kernel(const __grid_constant__
               for (int h = 0; h < 2; ++h) {
                 if constexpr (I8) {
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) g[h][j][e] = i2f_small(gi8[h][j][e]);   // below 2^21
+                  for (int e = 0; e < 4; ++e) g[h][j][e] = i2f_small(gi8[h][j][e]);   // at most 2^21
                 }
                 if (by_group) g[h][j][0] *= x0, g[h][j][1] *= x1, g[h][j][2] *= x0, g[h][j][3] *= x1;
                 acc[h][j][0] = fmaf(s[h].x, g[h][j][0], acc[h][j][0]);
@@ -857,7 +850,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
           if constexpr (XB == 1) {
 #pragma unroll
             for (int e = 0; e < CH; ++e)
-              if (I8) w[e] = __float_as_uint(i2f_small((int)w[e]));      // |int| < 2^22
+              if (I8) w[e] = __float_as_uint(i2f_small((int)w[e]));      // |int| <= 2^21
             if (by_group) {
               const float4* xv = reinterpret_cast<const float4*>(my_xs + j * NC + k * CH);
 #pragma unroll

@@ -144,12 +144,14 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
         raise RuntimeError("w4_linear has no gradient; use torch.no_grad()")
     N.require_cuda(x)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if x2.stride(1) != 1:
+    ld, step = x2.stride()
+    if step != 1 or (ld < K and x2.shape[0] > 1):       # broadcast (overlapping) rows are copied
         x2 = x2.contiguous()
+        ld = K
     y = x.new_empty(shape[:-1] + (n,), dtype=out_dtype)
     w = N.GladW4Weight(weight._tiles.data_ptr(), weight._scales.data_ptr(), K, n, group)
     rc = N.on_device(N.load().glad_w4_linear_forward, dev.index, w, x2.data_ptr(), N.DTYPES[dt], x2.shape[0],
-                     x2.stride(0), xp, per_row, groups, bp, y.data_ptr(), N.DTYPES[out_dtype])
+                     ld, xp, per_row, groups, bp, y.data_ptr(), N.DTYPES[out_dtype])
     if rc:
         N.check(rc, "w4_linear")
     return y

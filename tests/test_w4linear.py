@@ -3,6 +3,8 @@
 Tolerance, fixed before the first run: the products x * q are exact; a tensor-core sum keeps at least 24 bits of its
 largest term, so each of at most K/16 steps, 64 joins and scale products is off by at most 2^-23 of the sum of
 magnitudes S = sum |x q| s xs seen so far, in all (K/16 + 64) * 2^-23 * S; the result is rounded once (half a step)."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -12,7 +14,7 @@ from rl_quant_b200 import _native as N
 from rl_quant_b200 import swap
 from rl_quant_b200.norm import RMSNorm, rms_norm_quant
 from rl_quant_b200.w4a16 import quantize_w4
-from rl_quant_b200.w4linear import W4Linear, W4Weight, pack_w4, unpack_w4, w4_linear
+from rl_quant_b200.w4linear import W4Linear, W4Weight, pack_w4, unpack_w4, w4_linear, w4_status
 
 gpu = pytest.mark.gpu
 F16, BF16, I8, E4M3 = torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn
@@ -178,6 +180,32 @@ def test_strides_alignment_and_shapes(t):
         g = torch.rand(70, 6, device="cuda")[:, ::2]
         assert torch.equal(w4_linear(base[:, :192], w, x_scale=g, out_dtype=F16),
                            w4_linear(base[:, :192], w, x_scale=g.contiguous(), out_dtype=F16))
+
+
+@gpu
+def test_status():
+    q, packed, s = weight(512, 2048, 128, 1)
+    w = pack_w4(packed, s, 128)
+    for m in (1, 24, 200):
+        w4_linear(rows(m, 2048, F16, 2), w)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert w4_status() == 0
+    assert w4_status("cuda:0") == 0
+
+
+@gpu
+@pytest.mark.parametrize("m", [5, 40])
+def test_broadcast_rows(m):
+    q, packed, s = weight(100, 192, 64, 1)
+    w = pack_w4(packed, s, 64)
+    for t in (F16, I8):
+        kw = dict(x_scale=torch.ones(1, 1, device="cuda").expand(m, 1), out_dtype=F16) if t == I8 else {}
+        x = rows(1, 192, t, 2).expand(m, 192)
+        want = w4_linear(x.contiguous(), w, **kw)
+        assert torch.equal(w4_linear(x, w, **kw), want) and torch.equal(want[0], want[-1])
+        k3 = dict(kw, x_scale=kw["x_scale"].unsqueeze(0)) if kw else kw
+        assert torch.equal(w4_linear(x.unsqueeze(0), w, **k3)[0], want)
 
 
 @gpu
@@ -420,3 +448,20 @@ def test_abi_refusals():
         assert call(**kw) == N.GLAD_ERR_INVALID_ARG, kw
         assert lib.glad_last_error()
     assert lib.glad_w4_tiles_bytes(127, 8, 64) == 0 and lib.glad_w4_scales_bytes(128, 8, 48) == 0
+    assert lib.glad_w4_linear_status(None, None) == N.GLAD_ERR_INVALID_ARG
+
+
+def test_status_raises(monkeypatch):
+    """A status word with a bit set, as a fake of the library reports it."""
+    from rl_quant_b200.fused import DeviceStatusError
+
+    class Fake:
+        def glad_w4_linear_status(self, word, stream):
+            word.value = 1
+            return N.GLAD_ERR_DEVICE
+
+    monkeypatch.setattr(N, "load", Fake)
+    monkeypatch.setattr(N, "stream_handle", lambda device=None: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    with pytest.raises(DeviceStatusError):
+        w4_status(0)
