@@ -47,9 +47,11 @@ def _check(x, weight, residual, eps):
 
 
 def _rows(t):
-    """[..., C] as rows of adjacent columns (a view where the strides allow one)."""
+    """[..., C] as rows of adjacent columns: a view where the strides allow one, a copy of broadcast (overlapping) rows."""
     t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
+    rows, cols = t2.shape
+    ld, step = t2.stride()
+    return t2 if (step == 1 or cols == 1) and (ld >= cols or rows <= 1) else t2.contiguous()
 
 
 def _like(t, dtype=None):
@@ -61,7 +63,7 @@ def _like(t, dtype=None):
 
 def _forward(x, weight, residual, eps, rstd):
     """(y, h or None); ``rstd`` None or f32 [rows] to fill."""
-    x2 = x if x.dim() == 2 and x.stride(1) == 1 else _rows(x)
+    x2 = _rows(x)
     rows, cols = x2.shape
     y = _like(x)
     wp, wt, rp, rt, ldr, h, hp = None, 0, None, 0, 0, None, None
@@ -162,7 +164,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_quant has no gradient; use rms_norm, or torch.no_grad()")
     _check(x, weight, residual, eps)
-    x2 = x if x.dim() == 2 and x.stride(1) == 1 else _rows(x)
+    x2 = _rows(x)
     rows, cols = x2.shape
     q = _like(x, out_dtype)
     s, sp, gp = scale, None, None

@@ -206,6 +206,60 @@ def test_strides_and_alignment(x_t):
     assert ((dx.double() - d).abs() <= half_step(x_t) * d.abs() + 2 * F32 * mag + tiny(x_t)).all()
 
 
+@gpu
+def test_gradients_of_leaves_are_their_own():
+    """x and a residual of its type have the same gradient: each leaf's is a tensor of its own, the same leaf in both
+    places gets the sum, and one set of leaves serves two graphs that live at once."""
+    x, r = rows((40, 96), torch.bfloat16, 1).requires_grad_(), rows((40, 96), torch.bfloat16, 2).requires_grad_()
+    w, g = rows((96,), torch.bfloat16, 3).requires_grad_(), rows((40, 96), torch.bfloat16, 4)
+    want = torch.autograd.grad(rms_norm(x, w, residual=r)[0], (x, w), g)
+    y, h = rms_norm(x, w, residual=r)
+    y2, _ = rms_norm(x, w, residual=r)
+    y.backward(g)
+    assert torch.equal(x.grad, want[0]) and torch.equal(r.grad, want[0]) and torch.equal(w.grad, want[1])
+    assert x.grad.data_ptr() != r.grad.data_ptr()
+    x.grad.zero_()
+    assert torch.equal(r.grad, want[0])
+    r.grad = None
+    y2.backward(g)
+    assert torch.equal(x.grad, want[0]) and torch.equal(r.grad, want[0])
+    y, h = rms_norm(x, w, residual=r)      # the sum alone: the gradient that arrives is passed on
+    x.grad = r.grad = None
+    h.backward(g)
+    x.grad.zero_()
+    assert torch.equal(r.grad, g) and bool(g.any())
+    both = torch.autograd.grad(rms_norm(x, w, residual=x)[0], x, g)[0]
+    one = torch.autograd.grad(rms_norm(x, w, residual=x.detach())[0], x, g)[0]
+    assert torch.equal(both, one * 2)
+    y, h = rms_norm(x, w, residual=r)
+    with torch.no_grad():
+        h.add_(1.0)                         # the backward pass reads the sum
+    with pytest.raises(RuntimeError):
+        y.backward(g)
+
+
+@gpu
+def test_broadcast_rows():
+    """Rows that share memory: expanded inputs, and the expanded gradient that a mean over the rows sends back."""
+    x, r, w = rows((1, 96), torch.float16, 1), rows((1, 96), torch.float16, 2), rows((96,), torch.float16, 3)
+    xe, re = x.expand(40, 96), r.expand(40, 96)
+    for a, b in ((rms_norm(xe, w), rms_norm(xe.contiguous(), w)),
+                 (rms_norm(xe.unsqueeze(0), w)[0], rms_norm(xe.contiguous(), w)),
+                 (rms_norm(xe, w, residual=re)[0], rms_norm(xe.contiguous(), w, residual=re.contiguous())[0]),
+                 (rms_norm_quant(xe, w, residual=re)[0], rms_norm_quant(xe.contiguous(), w, residual=re.contiguous())[0])):
+        assert torch.equal(a, b)
+    leaf, wl = rows((40, 96), torch.float16, 4).requires_grad_(), w.clone().requires_grad_()
+    dy = rows((96,), torch.float16, 5)
+    for shape in ((40, 96), (4, 10, 96)):
+        got = torch.autograd.grad(rms_norm(leaf.view(shape), wl), (leaf, wl), dy.expand(shape))
+        want = torch.autograd.grad(rms_norm(leaf, wl), (leaf, wl), dy.expand(40, 96).contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y, h = rms_norm(leaf, wl, residual=xe.contiguous())
+    got = torch.autograd.grad((y, h), (leaf,), (dy.expand(40, 96), dy.expand(40, 96)), retain_graph=True)
+    want = torch.autograd.grad((y, h), (leaf,), (dy.expand(40, 96).contiguous(), dy.expand(40, 96).contiguous()))
+    assert torch.equal(got[0], want[0])
+
+
 QMAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 
 
@@ -269,6 +323,19 @@ def test_quant_zero_and_nonfinite_rows():
 
 
 @gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+def test_quant_scale_that_rounds_to_zero(out):
+    """A largest value below half the smallest subnormal times Q has a scale of zero: the scale is 1, all codes are 0."""
+    x = torch.zeros(2, 64, device="cuda")
+    x[:, 3] = 1.0
+    w = torch.full((64,), 2.0 ** -149 * 5, device="cuda")       # y[:, 3] is about 8 * 5 * 2^-149
+    for group in (0, 32):
+        for wide in (x, torch.cat((x, x), 1)[:, 1:64]):
+            q, s = rms_norm_quant(wide, w[:wide.shape[1]], out_dtype=out, group=group)
+            assert torch.equal(s, torch.ones_like(s)) and not q.float().any()
+
+
+@gpu
 def test_streams_graph_and_64_bit_offsets():
     x, w = rows((50, 1000), torch.float16, 1), rows((1000,), torch.float16, 2)
     want = rms_norm(x, w)
@@ -322,19 +389,6 @@ def test_module():
     with torch.no_grad():
         q, s = m.quant(x, out_dtype=torch.float8_e4m3fn, group=64)
     assert q.shape == x.shape and s.shape == (9, 5)
-@gpu
-@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
-def test_quant_scale_that_rounds_to_zero(out):
-    """A largest value below half the smallest subnormal times Q has a scale of zero: the scale is 1, all codes are 0."""
-    x = torch.zeros(2, 64, device="cuda")
-    x[:, 3] = 1.0
-    w = torch.full((64,), 2.0 ** -149 * 5, device="cuda")       # y[:, 3] is about 8 * 5 * 2^-149
-    for group in (0, 32):
-        for wide in (x, torch.cat((x, x), 1)[:, 1:64]):
-            q, s = rms_norm_quant(wide, w[:wide.shape[1]], out_dtype=out, group=group)
-            assert torch.equal(s, torch.ones_like(s)) and not q.float().any()
-
-
 
 
 # -- refusals (no GPU) -----------------------------------------------------------------------------
