@@ -470,9 +470,12 @@ struct Tile {
   static constexpr int NC = MT * 4 / SW;                 // columns of a sums thread
   static constexpr int kBlock = MT * 128, kStage = XB * kBlock;    // x of a stage: 128 bytes a row and block
   static constexpr int kSlot = 8192;                     // packed weights of a unit
-  static constexpr int SD = 4;                           // units of scales in flight, a copy a warp
-  static constexpr int kWs = SG * 64, kXs = XB == 1 ? SG * NC * 4 : 0;     // weight (32 rows), x scales of a unit
-  static constexpr int kSmem = NS * kStage + PD * kSlot + SW * SD * (kWs + kXs) + 512 + 1024;
+  static constexpr int SD = 4;                           // units of weight scales in flight, a copy a warp
+  static constexpr int kWs = SG * 64;                    // weight scales of a unit and 32 rows
+  // x scales: two blocks of eight groups (XF units), [group][NC + 4 columns] (no bank conflicts of the copies)
+  static constexpr int XF = 8 / SG, XPITCH = NC + 4, kXs = XB == 1 ? 2 * 8 * XPITCH * 4 : 0;
+  static constexpr int kSums = SD * kWs + kXs;           // scales of a sums warp
+  static constexpr int kSmem = NS * kStage + PD * kSlot + SW * kSums + 512 + 1024;
   static constexpr int kACol = ND * MT;                  // first tensor-memory column of A
   static constexpr int kCols = ND * MT + NS * ACOLS <= 256 ? 256 : 512;
   static_assert(ND * MT + NS * ACOLS <= kCols, "tensor memory");
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* slots = smem + L::NS * L::kStage;
   uint8_t* scale_ring = slots + L::PD * L::kSlot;
-  uint64_t* full = reinterpret_cast<uint64_t*>(scale_ring + L::SW * L::SD * (L::kWs + L::kXs));
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale_ring + L::SW * L::kSums);
   uint64_t* empty = full + L::NS;                        // [NS] products done; full: operands written
   uint64_t* wfull = empty + L::NS;                       // [PD]
   uint64_t* wempty = wfull + L::PD;                      // [PD]
@@ -792,39 +795,42 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     // ---- sums
     const int q4 = warp & 3, col0 = (warp >> 2) * NC;
     const bool by_group = XB == 1 && p.xs_groups > 1;
-    // the scales this warp multiplies by, fetched SD - 1 units ahead into a ring of its own
-    uint8_t* ring = scale_ring + warp * (L::SD * (L::kWs + L::kXs));
+    // the scales this warp multiplies by, in a ring of its own: the weights' are fetched SD - 1 units ahead, x's
+    // in blocks of eight groups (one 32-byte sector a row: a group at a time, each copy was a sector of its own, which
+    // bound the kernel: 512 x 4096 x 4096 int8 rows, groups of 64: 75 us) one block ahead
+    uint8_t* ring = scale_ring + warp * L::kSums;
+    float* xring = reinterpret_cast<float*>(ring + L::SD * L::kWs);
     const uint8_t* wsrc = reinterpret_cast<const uint8_t*>(p.scales) + (((int64_t)nt * U + un0) * 8 + q4 * 2) * (SG * 32);
-    auto fetch = [&](int u) {
-      if (u < units) {
-        uint8_t* dst = ring + (u % L::SD) * (L::kWs + L::kXs);
-        if (lane < SG * 4) cp_async16(dst + lane * 16, wsrc + (int64_t)u * (8 * SG * 32) + lane * 16);
-        if constexpr (XB == 1) {
-          if (by_group) {
+    auto fetch_x = [&](int block) {
+      if (by_group && block * L::XF < units) {
 #pragma unroll
-            for (int id = lane; id < SG * NC; id += 32) {
-              const int xg = (un0 + u) * SG + id / NC;
-              const int64_t m = m0 + col0 + id % NC;
-              const bool live = m < p.M && xg < p.xs_groups;
-              cp_async4_zfill(dst + L::kWs + id * 4, p.xs + (live ? m * p.xs_groups + xg : 0), live);
-            }
-          }
+        for (int id = lane; id < 8 * NC; id += 32) {
+          const int g = id & 7, xg = un0 * SG + block * 8 + g;
+          const int64_t m = m0 + col0 + (id >> 3);
+          const bool live = m < p.M && xg < p.xs_groups;
+          cp_async4_zfill(xring + ((block & 1) * 8 + g) * L::XPITCH + (id >> 3), p.xs + (live ? m * p.xs_groups + xg : 0), live);
         }
       }
+    };
+    auto fetch = [&](int u) {
+      if (u < units && lane < SG * 4)
+        cp_async16(ring + (u % L::SD) * L::kWs + lane * 16, wsrc + (int64_t)u * (8 * SG * 32) + lane * 16);
       cp_async_commit();
     };
     float acc[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
     bool ok = true;
+    if (XB == 1) fetch_x(0);
 #pragma unroll
     for (int i = 0; i < L::SD - 1; ++i) fetch(i);
     for (int u = 0; ok && u < units; ++u) {
-      cp_async_wait_group<L::SD - 2>();
+      // copies are committed with the unit SD - 1 ahead; a block of x scales is needed XF units after its commit
+      cp_async_wait_group<XB == 1 && L::XF < L::SD - 1 ? L::XF - 1 : L::SD - 2>();
       __syncwarp();
-      fetch(u + L::SD - 1);                              // the slot that every lane has just left
-      const uint8_t* in = ring + (u % L::SD) * (L::kWs + L::kXs);
-      const float* my_xs = reinterpret_cast<const float*>(in + L::kWs);
+      if (XB == 1 && u % L::XF == 0) fetch_x(u / L::XF + 1);   // the slots that every lane has just left
+      fetch(u + L::SD - 1);
+      const uint8_t* in = ring + (u % L::SD) * L::kWs;
       float sc[SG];
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
@@ -852,7 +858,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
             for (int e = 0; e < CH; ++e)
               if (I8) w[e] = __float_as_uint(i2f_small((int)w[e]));      // |int| <= 2^21
             if (by_group) {
-              const float4* xv = reinterpret_cast<const float4*>(my_xs + j * NC + k * CH);
+              const float4* xv = reinterpret_cast<const float4*>(xring + (gi & 15) * L::XPITCH + k * CH);
 #pragma unroll
               for (int e = 0; e < CH; e += 4) {
                 const float4 x = xv[e / 4];
