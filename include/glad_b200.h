@@ -385,7 +385,7 @@ int glad_actor_forward_w4a16(const GladActorWeights* w, const GladW4Linear* mlp,
                              void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- root-mean-square norm (no counterpart in the reference) -----------------
- * Rows x [rows, cols] (f32, f16 or bf16, row stride ldx elements), optionally
+ * Rows x [rows, cols] (f32, f16 or bf16, row stride ldx >= cols elements), optionally
  * plus a residual of x's type or f32:
  *   h = x + residual, rounded to the residual's type    (h = x without one)
  *   rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight
@@ -401,7 +401,7 @@ int glad_rms_norm_forward(const void* x, int x_dtype, int64_t ldx, const void* r
  * GLAD_DTYPE_E4M3) of the unrounded y: q = round_half_even(y * (1/s)), |q| at
  * most Q = 127 (i8) or 448 (e4m3).
  *   given_scale (device f32 [1]): s is that scale for the whole tensor;
- *   group 0: one scale a row, s = max|y| / Q, 1 for a row of zeros; scales [rows];
+ *   group 0: one scale a row, s = max|y| / Q, 1 where that is 0; scales [rows];
  *   group 32, 64, 128: one scale for that many columns, the last group of a row
  *     may be shorter; scales [rows, ceil(cols / group)].
  * A NaN in a row (group) makes its scale NaN; its i8 code is 0.              */
@@ -433,7 +433,7 @@ int glad_rms_norm_backward(const void* dy, int x_dtype, int64_t lddy, const void
  *          n + 8 (i & 1), input k + 2 ((i >> 1) & 1) + (i >> 2); zero past N and K
  *   scales [ceil(N/128)][ceil(K/128)][8][128 / group][8][2] f16: rows 128t + 16b + r and
  *          the same + 8 of a group side by side; zero past N and K
- * x [M, K] (row stride ldx elements): f16 or bf16 with x_scale NULL; i8 or e4m3
+ * x [M, K] (row stride ldx >= K elements): f16 or bf16 with x_scale NULL; i8 or e4m3
  * with x_scale f32: one for all rows (x_scale_rows 0), one a row (x_scale_groups
  * 1) or one a row and group (x_scale_groups = ceil(K / group), rows contiguous).
  * y [M, N] contiguous, f16, bf16 or f32; bias [N] of y's type or NULL. The inner

@@ -252,6 +252,11 @@ __device__ __forceinline__ void place(int team, int& who, int& t) {
 
 // ---- forward ------------------------------------------------------------------------------
 // One team of threads per row, up to VEC * NV elements a thread. QUANT: 0 none, 1 int8, 2 e4m3.
+// 8192 x 4096, bf16 with an fp32 residual: 403 MB in 63 us, 6.4 TB/s, what a plain copy reaches here. 8192 x 8192 bf16 to
+// e4m3 with groups of 128: 472 MB in 87 us, 5.4 TB/s; there the instruction issue is busy for 75% of the time (a
+// maximum, a scale and a conversion an element on top). 1 x 4096 f16: 1.6 us, a launch.
+// A persistent block that fetches its next row ahead gained nothing: with one row a block the
+// scheduler already has five blocks' loads in flight on an SM.
 template <typename TX, typename TH, int VEC, int NV, int QUANT, int MAXT>
 __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ NormParams p) {
   __shared__ float red[32];
@@ -390,6 +395,9 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
 // ---- backward -----------------------------------------------------------------------------
 // A team walks rows team_id, team_id + teams, ...; its columns' share of dw stays in
 // registers and is written once as a partial row, which norm_dw_kernel sums in a fixed order.
+// 8192 x 4096, bf16 with an fp32 sum, gradients of both and of the weight: 537 MB in 98 us, 5.5 TB/s, 86% of a copy's
+// rate: 64 registers a thread for the row, its gradient and dw's share leave 32 warps an SM to hide the row's one
+// barrier. A ring of asynchronous copies ahead of the row and three blocks an SM (40 registers, spills) were slower.
 template <typename TX, typename TH, int VEC, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) norm_bwd_kernel(const __grid_constant__ NormParams p) {
   __shared__ float red[2][32];                           // rows use them in turn: one barrier a row
@@ -466,7 +474,8 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) norm_bwd_kernel(con
   }
 }
 
-// dw[c] = sum of the partial rows: 32 columns x 32 row slices a block, slices joined in order.
+// dw[c] = sum of the partial rows: 32 columns x 32 row slices a block, slices joined in order. 592 x 4096: 9.7 MB from
+// L2, 4 us behind the backward kernel.
 template <typename TW>
 __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* partial, int n, int cols, TW* dw) {
   __shared__ float s[32][33];

@@ -193,6 +193,10 @@ __device__ __forceinline__ void store_y4(const W4Params& p, int64_t m, int n, co
 // a word's nibbles come apart). Rows past M read row M - 1: their sums are never stored.
 // Issue slots bound it: a 32-bit word takes 9 instructions to unpack and one to multiply, so a unit is as
 // large as registers allow, which spreads the rest (copies, x, scales, addresses) over more words.
+// 1 x 28672 x 8192 bf16, groups of 128: 121 MB in 29.7 us, 4.1 TB/s, 64% of a copy's rate (f16, one operation less a
+// pair: 8 rows 31.5 us; int8, whose words take 4 to unpack: 8 rows 25.8 us, 4.7 TB/s). 1 x 4096 x 4096 f16, groups of
+// 64: 8.9 MB in 3.9 us, of which 1.6 us are a launch. 16 columns a step: 30.4 and 4.4 us; registers instead
+// of the rings of copies: 76.8 and 7 us (the newest load held up the oldest).
 template <int NT, int GROUP, int RING>
 struct RowSmem {
   static constexpr int kWarps = 16, kRing = RING;
@@ -453,6 +457,12 @@ __global__ void __launch_bounds__(512, 1) w4_rows_kernel(const __grid_constant__
 // groups of 64 half of the tensor core's time for them at fp16 rate. Blocks of a cluster split the
 // inputs when there are fewer tiles than SMs, send their sums to the rows' owners through
 // distributed shared memory and add them in rank order.
+// 1024 x 4096 x 4096 f16, groups of 64: 48.9 us, 0.70 PFLOP/s, 42% of a library product's rate (two rounds of tiles on 148
+// SMs: 512 rows, one round, 25.0 us); groups of 128, 512 rows: 20.8 us, 0.82 PFLOP/s. 64 rows of e4m3 x 4096 x 14336,
+// groups of 128 with scales of both: 30.8 MB in 22.5 us. Neither HBM (14% busy there) nor the tensor core (524 of
+// 1250 clocks a unit at groups of 128) is the bound but the issue slots (57 to 71% busy) of unpacking and sums
+// and the hand-offs between them. A deeper ring of x (54 us where four stages took 47.5), 16 unpacking warps, one or four
+// product warps and tiles of 256 rows were slower or no faster.
 __device__ unsigned int g_w4_status;
 
 template <int XB, int MT, int GROUP>                     // XB: bytes of an input
@@ -468,6 +478,10 @@ struct Tile {
   static constexpr int DW = 8;                           // warps that unpack
   static constexpr int kThreads = (SW + DW + MW + 2) * 32;
   static constexpr int NC = MT * 4 / SW;                 // columns of a sums thread
+  // Paired multiply-adds of the sums: 1024 x 4096 x 4096 f16, groups of 64: 53.9 -> 48.9 us. With one group a unit
+  // they gain nothing (512 rows: 20.8 us alone, 22.3 us paired), and 8-bit rows spill (512 rows of e4m3,
+  // groups of 32: 97 -> 119 us).
+  static constexpr bool kPacked = XB == 2 && SG > 1;
   static constexpr int kBlock = MT * 128, kStage = XB * kBlock;    // x of a stage: 128 bytes a row and block
   static constexpr int kSlot = 8192;                     // packed weights of a unit
   static constexpr int SD = 4;                           // units of weight scales in flight, a copy a warp
@@ -556,6 +570,20 @@ __device__ __forceinline__ void cp_async4_zfill(void* dst, const void* src, bool
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// acc += s * f, four values; PACKED: two multiply-adds an instruction (a pair of neighbouring registers).
+template <bool PACKED>
+__device__ __forceinline__ void add_scaled(float* acc, float s, const float (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    if constexpr (PACKED)
+      asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %2};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 c, {%0, %1};\n\t"
+          "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+          : "+f"(acc[i]), "+f"(acc[i + 1])
+          : "f"(s), "f"(f[i]), "f"(f[i + 1]));
+    else
+      acc[i] = fmaf(s, f[i], acc[i]), acc[i + 1] = fmaf(s, f[i + 1], acc[i + 1]);
+  }
 }
 // Cluster barrier in two halves, without ordering of memory accesses.
 __device__ __forceinline__ void cluster_arrive_relaxed() {
@@ -808,7 +836,8 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
           const int g = id & 7, xg = un0 * SG + block * 8 + g;
           const int64_t m = m0 + col0 + (id >> 3);
           const bool live = m < p.M && xg < p.xs_groups;
-          cp_async4_zfill(xring + ((block & 1) * 8 + g) * L::XPITCH + (id >> 3), p.xs + (live ? m * p.xs_groups + xg : 0), live);
+          cp_async4_zfill(xring + ((block & 1) * 8 + g) * L::XPITCH + (id >> 3),
+                          p.xs + (live ? m * p.xs_groups + xg : 0), live);
         }
       }
     };
@@ -853,24 +882,17 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
           tmem_ld_wait();
           if (AHEAD && k + 1 < PIECES) tmem_ld16(at + (k + 1) * CH, v[(k + 1) & AHEAD]);
           uint32_t (&w)[CH] = v[k & AHEAD];
-          if constexpr (XB == 1) {
 #pragma unroll
-            for (int e = 0; e < CH; ++e)
-              if (I8) w[e] = __float_as_uint(i2f_small((int)w[e]));      // |int| <= 2^21
+          for (int e = 0; e < CH; e += 4) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = I8 ? i2f_small((int)w[e + i]) : __uint_as_float(w[e + i]);   // |int| <= 2^21
             if (by_group) {
-              const float4* xv = reinterpret_cast<const float4*>(xring + (gi & 15) * L::XPITCH + k * CH);
-#pragma unroll
-              for (int e = 0; e < CH; e += 4) {
-                const float4 x = xv[e / 4];
-                w[e] = __float_as_uint(__uint_as_float(w[e]) * x.x);
-                w[e + 1] = __float_as_uint(__uint_as_float(w[e + 1]) * x.y);
-                w[e + 2] = __float_as_uint(__uint_as_float(w[e + 2]) * x.z);
-                w[e + 3] = __float_as_uint(__uint_as_float(w[e + 3]) * x.w);
-              }
+              const float4 x = *reinterpret_cast<const float4*>(xring + (gi & 15) * L::XPITCH + k * CH + e);
+              f[0] *= x.x, f[1] *= x.y, f[2] *= x.z, f[3] *= x.w;
             }
+            add_scaled<L::kPacked>(&acc[k * CH + e], sc[j], f);
           }
-#pragma unroll
-          for (int e = 0; e < CH; ++e) acc[k * CH + e] = fmaf(sc[j], __uint_as_float(w[e]), acc[k * CH + e]);
         }
         tc_fence_before();
         __syncwarp();
@@ -934,10 +956,14 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
 }
 
 // ---- launch -------------------------------------------------------------------------------------
+int current_device() {                                   // -1: none, or past the caches below
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : -1;
+}
 int w4_sms() {
   static int cache[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  const int dev = current_device();
+  if (dev < 0) return 148;
   if (cache[dev] == 0) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
@@ -1002,36 +1028,64 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
   cudaError_t e = allow_max_smem((const void*)w4_tile_kernel<TX, MT, GROUP>, done);
   if (e != cudaSuccess) return e;
   const int nt = (p.N + 127) / 128, mt = (int)((p.M + MT - 1) / MT), units = p.U, sms = w4_sms();
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(L::kThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  // As many blocks a tile as the GPU holds at once, four units of inputs each or more. Clusters are placed
+  // within groups of SMs, so fewer blocks fit in large ones (16 clusters of 8 took two rounds, 17 x 2048 x 4096:
+  // 9.7 us; 16 of 4: 6.3 us): the runtime tells how many do.
+  auto fits = [&](int n) {
+    static int cache[64][4] = {};                        // [device][log2 n]: clusters of n at once, plus one
+    const int dev = current_device(), i = n == 2 ? 1 : n == 4 ? 2 : 3;
+    if (dev < 0) return false;
+    if (cache[dev][i] == 0) {
+      int most = 0;
+      attr[0].val.clusterDim = {(unsigned)n, 1, 1};
+      cfg.gridDim = dim3((unsigned)n);
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&most, w4_tile_kernel<TX, MT, GROUP>, &cfg) != cudaSuccess) most = 0;
+      cache[dev][i] = most + 1;
+    }
+    return (int64_t)nt * mt <= cache[dev][i] - 1;
+  };
   int s = 1;
-  while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 4 * s) s *= 2;
+  while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 4 * s && fits(2 * s)) s *= 2;
   p.splits = s;
   CUtensorMap map{};
   const CUtensorMapDataType type = sizeof(TX) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : std::is_same<TX, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   p.x_tma = x_tensor_map(&map, p, sizeof(TX), type, MT);
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(nt * s), (unsigned)mt);
-  cfg.blockDim = dim3(L::kThreads);
-  cfg.dynamicSmemBytes = L::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {(unsigned)s, 1, 1};
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, w4_tile_kernel<TX, MT, GROUP>, p, map);
 }
 
 template <typename TX, int GROUP>
 cudaError_t launch_group(const W4Params& p, cudaStream_t st) {
-  // x in shared memory as the products take it
-  const size_t x = (size_t)p.U * 128 * (std::is_same<TX, int8_t>::value ? 1 : 2) * (size_t)p.M, limit = 232448;
+  constexpr bool I8 = std::is_same<TX, int8_t>::value;
+  // Rows of up to 16 are staged by every block, in shared memory as the products take them; the limit is the memory's
+  // (16 rows of 4096 f16 inputs, groups of 64, take the tile kernel). At 16 | 17 rows, where the kernels change:
+  // 28672 x 8192 f16 49.1 | 49.2 us, int8 35.8 | 49.7 us; 16384 x 1024 f16 5.9 | 6.1 us, groups of 32 6.1 | 8.7 us.
+  const size_t x = (size_t)p.U * 128 * (I8 ? 1 : 2) * (size_t)p.M, limit = 232448;
+  // Where four blocks can share a tile's inputs, staging 12 rows or more of 16-bit inputs costs more than the tile kernel
+  // (4096 x 4096: 11 rows 6.7 us, 12 rows 7.2 us, 16 rows 8.1 us against 6.9 us; 1024 x 4096: 16 rows 8.0 | 5.0 us).
+  // Not with smaller groups (4096 x 4096, groups of 32: 14 rows 8.1 | 9.1 us), 8-bit rows (e4m3, 12 rows 7.2 | 8.0 us)
+  // or few inputs (777 x 1002: 5.0 | 5.2 us).
+  const bool split =
+      GROUP == 128 && sizeof(TX) == 2 && p.M > 11 && p.U >= 16 && (int64_t)((p.N + 127) / 128) * 4 <= w4_sms();
   if (p.M <= 8 && RowSmem<1, GROUP, 3>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP, 3>(p, x, st);
   if (p.M <= 8 && RowSmem<1, GROUP, 2>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP, 2>(p, x, st);
-  if (p.M > 8 && p.M <= 16 && RowSmem<2, GROUP, 2>::kFixed + x <= limit) return launch_rows<TX, 2, GROUP, 2>(p, x, st);
+  if (p.M > 8 && p.M <= 16 && !split && RowSmem<2, GROUP, 2>::kFixed + x <= limit)
+    return launch_rows<TX, 2, GROUP, 2>(p, x, st);
+  // the smallest tile that holds all rows: 4096 x 4096 f16 at 32 | 33 rows 7.0 | 8.3 us, at 64 | 65 rows 8.6 | 12.1 us
   if (p.M <= 32) return launch_tile<TX, 32, GROUP>(p, st);
   if (p.M <= 64) return launch_tile<TX, 64, GROUP>(p, st);
   return launch_tile<TX, 128, GROUP>(p, st);
