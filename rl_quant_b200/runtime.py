@@ -22,7 +22,7 @@ import warnings
 import torch
 import torch.nn as nn
 
-from . import _native as N
+from . import _native as N, w4linear
 from .fused import FusedActor, FusedActorCritic, FusedCritic, FusedUnsupported, ppo_epilogue
 from .qconv import QuantCNN
 from .qlinear import QuantLinear
@@ -286,7 +286,7 @@ class InferenceRunner:
         return pipe(host_obs, out)
 
     def check_status(self) -> None:
-        """Raise ``DeviceStatusError`` if any fused forward launched since the previous
+        """Raise ``DeviceStatusError`` if any fused forward or 4-bit layer launched since the previous
         check (directly or by a captured graph's replay) reported that a bounded
         device-side wait ran out; its outputs are then not valid. Reads and clears the
         status word of every workspace (one host synchronisation): call it once per PPO
@@ -294,6 +294,8 @@ class InferenceRunner:
         for f in (self._fused, self._fused_critic, self._fused_ac):
             if f is not None:
                 f.check_status()
+        if any(isinstance(m, w4linear.W4Linear) for m in self.model.modules()):
+            w4linear.w4_status(self._device())
 
     def _device(self):
         for t in self.model.parameters():

@@ -94,7 +94,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
 
     x float16 or bfloat16 (``x_scale`` None, ``out_dtype`` x's by default), or int8 / float8_e4m3fn codes with a float32
     ``x_scale`` of one value, [..., 1] (one a row) or [..., ceil(K / group)] (one a row and group of the weight) and
-    ``out_dtype`` named. out_dtype float16, bfloat16 or float32; bias [N] has it. Inference only."""
+    ``out_dtype`` named. out_dtype float16, bfloat16 or float32; bias [N] has it. Up to 2^20 rows, inputs (an even number)
+    and outputs. Inference only."""
     K, n, group = weight._shape
     shape, dt = x.shape, x.dtype
     if not shape or shape[-1] != K:
@@ -198,6 +199,14 @@ class W4Linear(nn.Module):
         w = pack_w4(*quantize_w4(self.weight, self.group), self.group)
         self.tiles.copy_(w.tiles)
         self.scales.copy_(w.scales)
+        return self
+
+    def _apply(self, fn, recurse=True):
+        """A cast of the module (``.bfloat16()``) leaves the scales fp16, made anew from the cast weight."""
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float16:
+            self.scales = torch.zeros_like(self.scales, dtype=torch.float16)
+            self.requantize_()
         return self
 
     def w4(self) -> W4Weight:

@@ -465,3 +465,27 @@ def test_status_raises(monkeypatch):
     monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
     with pytest.raises(DeviceStatusError):
         w4_status(0)
+
+
+def test_runner_checks_w4_status(monkeypatch):
+    from rl_quant_b200 import w4linear
+    from rl_quant_b200.runtime import InferenceRunner
+    asked = []
+    monkeypatch.setattr(w4linear, "w4_status", asked.append)
+    run = InferenceRunner.__new__(InferenceRunner)
+    run._fused = run._fused_critic = run._fused_ac = None
+    run.model = nn.Sequential(nn.Linear(64, 8))
+    run.check_status()
+    assert not asked
+    swap.apply(run.model, {"0": {"bits": 4}})
+    run.check_status()
+    assert asked == [torch.device("cpu")]
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16, torch.float32, torch.float64])
+def test_module_casts(t):
+    m = W4Linear(nn.Linear(64, 40)).bfloat16().to(t)
+    assert m.weight.dtype == t and m.scales.dtype == F16
+    packed, s = unpack_w4(m.w4())
+    want, s2 = quantize_w4(m.weight, 64)
+    assert torch.equal(packed, want) and torch.equal(s, s2)
