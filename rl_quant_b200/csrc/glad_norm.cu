@@ -254,7 +254,7 @@ __device__ __forceinline__ void place(int team, int& who, int& t) {
 // One team of threads per row, up to VEC * NV elements a thread. QUANT: 0 none, 1 int8, 2 e4m3.
 // 8192 x 4096, bf16 with an fp32 residual: 403 MB in 63 us, 6.4 TB/s, what a plain copy reaches here. 8192 x 8192 bf16 to
 // e4m3 with groups of 128: 472 MB in 87 us, 5.4 TB/s; there the instruction issue is busy for 75% of the time (a
-// maximum, a scale and a conversion an element on top). 1 x 4096 f16: 1.6 us, a launch.
+// maximum, a scale and a conversion an element on top). 1 x 2048 f16: 1.6 us, a launch.
 // A persistent block that fetches its next row ahead gained nothing: with one row a block the
 // scheduler already has five blocks' loads in flight on an SM.
 template <typename TX, typename TH, int VEC, int NV, int QUANT, int MAXT>
