@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(512, 1) w4_rows_kernel(const __grid_constant__
 // inputs go in stages of 128 (one or two swizzle atoms of 128 bytes a row). Roles by
 // warp: one brings the packed weights (bulk copies, PD units of 128 inputs ahead), one the x tile
 // (TMA, NS stages ahead); teams of four unpack the weights of a unit each, in x's own type:
-// f16 or bf16, int8 times 16, or e4m3, all exact, and store them in tensor memory as the A operand (a
+// f16 or bf16, int8 times 16, or e4m3 times 2^-9, all exact, and store them in tensor memory as the A operand (a
 // warp's fragment order is the order of its 16x256b / 16x128b stores), so shared memory, whose
 // bandwidth bounded the same kernel with A in it, carries only x; MW issue the products of
 // groups in turn. Every group of inputs has an accumulator of its own (ND in rotation): SW warps
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(512, 1) w4_rows_kernel(const __grid_constant__
 // distributed shared memory and add them in rank order.
 // 1024 x 4096 x 4096 f16, groups of 64: 48.9 us, 0.70 PFLOP/s, 42% of a library product's rate (two rounds of tiles on 148
 // SMs: 512 rows, one round, 25.0 us); groups of 128, 512 rows: 20.8 us, 0.82 PFLOP/s. 64 rows of e4m3 x 4096 x 14336,
-// groups of 128 with scales of both: 30.8 MB in 22.5 us. Neither HBM (14% busy there) nor the tensor core (524 of
+// groups of 128 with scales of both: 30.8 MB in 20.5 us. Neither HBM (14% busy there) nor the tensor core (524 of
 // 1250 clocks a unit at groups of 128) is the bound but the issue slots (57 to 71% busy) of unpacking and sums
 // and the hand-offs between them. A deeper ring of x (54 us where four stages took 47.5), 16 unpacking warps, one or four
 // product warps and tiles of 256 rows were slower or no faster.
@@ -598,6 +598,12 @@ __device__ __forceinline__ void bulk_copy_s2c(uint32_t dst_cluster, uint32_t src
       : "memory");
 }
 
+// Every byte's top bit in all eight of its bits.
+__device__ __forceinline__ uint32_t byte_signs(uint32_t w) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, 0, 0xba98;" : "=r"(d) : "r"(w));
+  return d;
+}
 // The eight weights of a word as bytes in the operand's type: lo = row r, hi = row r + 8, inputs
 // k .. k + 3 in order.
 template <bool E4M3>
@@ -606,20 +612,12 @@ __device__ __forceinline__ void unpack_w4_bytes(uint32_t w, uint32_t& lo, uint32
     lo = swap_mid(w4_low16(w));
     hi = swap_mid(w4_high16(w));
   } else {
-    // e4m3 of 0..7 and of -8..-1, picked by the low three bits, chosen by the top bit
-    const uint32_t idx = w & 0x77777777u, neg = (w >> 3) & 0x11111111u;
-    uint32_t v[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t i = idx >> (16 * h), n = neg >> (16 * h);
-      const uint32_t pos = __byte_perm(0x44403800u, 0x4e4c4a48u, i);
-      const uint32_t ng = __byte_perm(0xcaccced0u, 0xb8c0c4c8u, i);
-      const uint32_t m = __byte_perm(0x0000ff00u, 0, n);
-      v[h] = (ng & m) | (pos & ~m);
-    }
-    // v[0]: (r, k) (r+8, k) (r, k+2) (r+8, k+2); v[1]: the same for k+1, k+3
-    lo = __byte_perm(v[0], v[1], 0x6240);
-    hi = __byte_perm(v[0], v[1], 0x7351);
+    // sign and magnitude: the codes 0 to 8 are the magnitude times 2^-9 (subnormals and the first normal number), and
+    // a negative nibble n has the magnitude 16 - n = (n ^ 15) + 1. Picking q's own codes from tables took a
+    // quarter more instructions (17 x 4096 x 14336, groups of 128: 18.7 against 14.7 us).
+    const uint32_t ml = byte_signs(w << 4), mh = byte_signs(w);
+    lo = swap_mid(((w ^ ml) & 0x0f0f0f0fu) + (ml & 0x81818181u));
+    hi = swap_mid((((w >> 4) ^ mh) & 0x0f0f0f0fu) + (mh & 0x81818181u));
   }
 }
 
@@ -865,6 +863,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       for (int j = 0; j < SG; ++j) {
         sc[j] = __half2float(reinterpret_cast<const __half*>(in)[((lane >> 4) * SG + j) * 16 + (lane & 7) * 2 + ((lane >> 3) & 1)]);
         if (I8) sc[j] *= 0.0625f;                        // the int8 operand is 16 q
+        if (E4M3) sc[j] *= 512.0f;                       // the e4m3 operand is 2^-9 q
       }
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
@@ -1075,12 +1074,11 @@ cudaError_t launch_group(const W4Params& p, cudaStream_t st) {
   // (16 rows of 4096 f16 inputs, groups of 64, take the tile kernel). At 16 | 17 rows, where the kernels change:
   // 28672 x 8192 f16 49.1 | 49.2 us, int8 35.8 | 49.7 us; 16384 x 1024 f16 5.9 | 6.1 us, groups of 32 6.1 | 8.7 us.
   const size_t x = (size_t)p.U * 128 * (I8 ? 1 : 2) * (size_t)p.M, limit = 232448;
-  // Where four blocks can share a tile's inputs, staging 12 rows or more of 16-bit inputs costs more than the tile kernel
-  // (4096 x 4096: 11 rows 6.7 us, 12 rows 7.2 us, 16 rows 8.1 us against 6.9 us; 1024 x 4096: 16 rows 8.0 | 5.0 us).
-  // Not with smaller groups (4096 x 4096, groups of 32: 14 rows 8.1 | 9.1 us), 8-bit rows (e4m3, 12 rows 7.2 | 8.0 us)
-  // or few inputs (777 x 1002: 5.0 | 5.2 us).
-  const bool split =
-      GROUP == 128 && sizeof(TX) == 2 && p.M > 11 && p.U >= 16 && (int64_t)((p.N + 127) / 128) * 4 <= w4_sms();
+  // Where four blocks can share a tile's inputs, staging 12 rows or more of 16 bits (e4m3 is staged as fp16) costs
+  // more than the tile kernel (4096 x 4096 f16: 11 rows 6.7 us, 12 rows 7.2 | 6.8 us, 16 rows 8.1 | 6.9 us;
+  // e4m3: 12 rows 7.4 | 6.8 us; 1024 x 4096 f16: 16 rows 8.0 | 5.0 us). Not with smaller groups (4096 x 4096, groups of 32: 14 rows 8.1 | 9.1 us), int8
+  // (12 rows 6.0 | 6.5 us) or few inputs (777 x 1002: 5.0 | 5.2 us).
+  const bool split = GROUP == 128 && !I8 && p.M > 11 && p.U >= 16 && (int64_t)((p.N + 127) / 128) * 4 <= w4_sms();
   if (p.M <= 8 && RowSmem<1, GROUP, 3>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP, 3>(p, x, st);
   if (p.M <= 8 && RowSmem<1, GROUP, 2>::kFixed + x <= limit) return launch_rows<TX, 1, GROUP, 2>(p, x, st);
   if (p.M > 8 && p.M <= 16 && !split && RowSmem<2, GROUP, 2>::kFixed + x <= limit)
