@@ -398,7 +398,7 @@ int glad_rms_norm_forward(const void* x, int x_dtype, int64_t ldx, const void* r
                           float* rstd_out, void* stream);
 
 /* The same norm with an 8-bit output q [rows, cols] (GLAD_DTYPE_I8 or
- * GLAD_DTYPE_E4M3) of the unrounded y: q = round_half_even(y * (1/s)), |q| at
+ * GLAD_DTYPE_E4M3) of the unrounded y: q = round_half_even(y / s), |q| at
  * most Q = 127 (i8) or 448 (e4m3).
  *   given_scale (device f32 [1]): s is that scale for the whole tensor;
  *   group 0: one scale a row, s = max|y| / Q, 1 where that is 0; scales [rows];

@@ -4,7 +4,7 @@
 //   h = x + r, rounded to r's type (h = x without a residual)
 //   rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * w
 //   8 bits: s = max|y| / Q over a row or a group of columns (Q = 127 int8, 448 e4m3;
-//           1 where that is 0 in fp32), q = round_half_even(y * (1/s)); or s is given.
+//           1 where that is 0 in fp32), q = round_half_even(y / s); or s is given.
 //   backward, g = dy * w:  dh' = dh + rstd * (g - h * rstd^2 * mean(g * h)),
 //           dx = dr = dh',  dw = sum over rows of dy * h * rstd
 //
@@ -181,38 +181,92 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, int team, uint32_t* red
 }
 
 // ---- 8-bit rounding ---------------------------------------------------------------------
-// A maximum that keeps a NaN.
-__device__ __forceinline__ float max_abs(float m, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(y)));
-  return r;
+// The largest of m and the |v|; a NaN stays.
+template <int N>
+__device__ __forceinline__ float max_abs(float m, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[0])));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[e]), "f"(v[e + 1]));
+  }
+  return m;
 }
-// The scale of a maximum held as the bits of |y| (a NaN has the largest bits and stays NaN).
-// Multiplying by RN(1/Q), and y by the approximate 1/s (one unit in the last place), instead of dividing
-// moves a scale by one rounding and a code only where y/s lies within three roundings of a border between
-// two codes; two divisions for each eight elements cost as much as the rest of the quantisation.
+// The 8-bit form finds its own scales with z = h * (Qz * 2^k) * w instead of y: 2^k is rstd without its mantissa m = rstd / 2^k,
+// and Qz = Q / kUp, below 1 with few bits, so y = z / Qz * m. The scale is s = max|y| / Q and a code rounds y / s = z / d,
+// d = max|z| / Q: rstd's own rounding cancels, and where h and w have 16 bits and z fits the 24 of fp32 (bf16 always), z
+// and d are exact, so a quotient on a border between two codes is found there.
 template <bool E4M3>
-__device__ __forceinline__ float q_scale(uint32_t amax_bits) {
-  const float s = __fmul_rn(__uint_as_float(amax_bits), E4M3 ? (float)(1.0 / 448.0) : (float)(1.0 / 127.0));
-  return s == 0.0f ? 1.0f : s;                  // a row of zeros, or of values whose scale rounds to zero
-}
-__device__ __forceinline__ float rcp_approx(float x) {   // x normal
+struct Q8 {
+  static constexpr float kMax = E4M3 ? 448.0f : 127.0f;        // Q
+  static constexpr float kUp = E4M3 ? 512.0f : 128.0f;
+  static constexpr float kZ = kMax / kUp;                      // Qz
+};
+__device__ __forceinline__ float rcp_approx(float x) {   // x normal; within one unit in the last place
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// y / s in place; where the reciprocal may overflow, both are first multiplied by 2^64 (exact there).
-template <int N>
-__device__ __forceinline__ void divide(float (&y)[N], float s) {
-  if (fabsf(s) < 1e-36f) {
-    const float inv = rcp_approx(__fmul_rn(s, 18446744073709551616.0f));
+// Two neighbouring elements in one instruction, the second operand (and the addend's) the same or a pair.
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y, float u, float v) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(a), "=f"(b) : "f"(x), "f"(y), "f"(u), "f"(v));
+}
+__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float u, float v, float s, float t) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%6, %7};\n\t"
+      "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(a), "=f"(b) : "f"(x), "f"(y), "f"(u), "f"(v), "f"(s), "f"(t));
+}
+// y / s by a product with the reciprocal and STEPS correction steps (Markstein, "Computation of elementary functions on
+// the IBM RISC System/6000 processor", 1990): a step takes the remainder, one fused multiply-add, times the reciprocal. The
+// product is off by at most 1.5 * 2^-23 of the quotient; after one step with a reciprocal good to 2^-23 what is rounded
+// is off by 2^-44, after a second one with the rounded reciprocal the result is the rounded quotient, always. `y` is
+// given negated: the remainder q * s - y then needs no sign of its own, and a zero keeps its sign.
+template <int STEPS>
+__device__ __forceinline__ float corrected(float minus_y, float s, float inv) {
+  float q = __fmul_rn(minus_y, -inv);
 #pragma unroll
-    for (int e = 0; e < N; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], 18446744073709551616.0f), inv);
+  for (int i = 0; i < STEPS; ++i) q = fmaf(fmaf(q, s, minus_y), -inv, q);
+  return q;
+}
+template <int STEPS, int N>
+__device__ __forceinline__ void corrected_v(float (&v)[N], float s, float inv) {
+  if constexpr (N == 1) {
+    v[0] = corrected<STEPS>(v[0], s, inv);
   } else {
-    const float inv = rcp_approx(s);
 #pragma unroll
-    for (int e = 0; e < N; ++e) y[e] = __fmul_rn(y[e], inv);
+    for (int e = 0; e < N; e += 2) {
+      float q0, q1, r0, r1;
+      mul2(q0, q1, v[e], v[e + 1], -inv, -inv);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        fma2(r0, r1, q0, q1, s, s, v[e], v[e + 1]);
+        fma2(q0, q1, r0, r1, -inv, -inv, q0, q1);
+      }
+      v[e] = q0, v[e + 1] = q1;
+    }
   }
+}
+// rstd = 2^k * m, returns Qz * 2^k. A finite rstd other than 0 lies between 2^-65 and 2^75; 0, infinity and NaN go into
+// z as they are.
+template <bool E4M3>
+__device__ __forceinline__ float split_rstd(float rstd, float& m) {
+  m = 1.0f;
+  if (!(rstd >= 0x1p-70f && rstd <= 0x1p80f)) return rstd;
+  const uint32_t e = __float_as_uint(rstd) & 0x7f800000u;
+  m = __fmul_rn(rstd, __uint_as_float(0x7f000000u - e));
+  return __fmul_rn(__uint_as_float(e), Q8<E4M3>::kZ);
+}
+// Whether a maximum of |z| keeps d, s and every remainder that a code depends on among the normal numbers.
+__device__ __forceinline__ bool plain_max(float top) { return top >= 0x1p-50f && top <= 0x1p90f; }
+// max|z| / Q, and the scale, where plain_max holds.
+template <bool E4M3>
+__device__ __forceinline__ float plain_over_q(float v) {
+  return corrected<1>(-v, Q8<E4M3>::kMax, (float)(1.0 / Q8<E4M3>::kMax));
+}
+template <bool E4M3>
+__device__ __forceinline__ float plain_scale(float d, float m) {
+  return plain_over_q<E4M3>(__fmul_rn(d, __fmul_rn(m, Q8<E4M3>::kUp)));
 }
 __device__ __forceinline__ uint32_t code_i8(float t) {
   int q = __float2int_rn(t);                    // NaN -> 0, out of range saturates
@@ -250,17 +304,72 @@ __device__ __forceinline__ void place(int team, int& who, int& t) {
   }
 }
 
+// Codes and scales where those of the fast form do not hold (a maximum or a given scale out of its range, an infinite
+// quotient), which is rare: the pieces `slow` (bit i: piece i) of a thread, one element at a time, from memory and by division.
+// row_top: the row's maximum of |z|.
+template <typename TX, typename TH, int VEC, int NV, bool E4M3>
+__device__ __noinline__ void quant_slow(const NormParams& p, uint32_t slow, float rstd, float row_top) {
+  int who, t;
+  place(p.team, who, t);
+  const int64_t row = (int64_t)blockIdx.x * p.teams + who;
+  const int groups = p.group != 0 ? (p.cols + p.group - 1) / p.group : 1;
+  auto y_of = [&](int c) {
+    const float h = p.r != nullptr ? to_f<TH>(static_cast<const TH*>(p.sum)[row * p.cols + c])
+                                   : to_f<TX>(static_cast<const TX*>(p.x)[row * p.ldx + c]);
+    float w[1];
+    load_w<1, TX>(p, c, w);
+    return __fmul_rn(__fmul_rn(h, rstd), w[0]);
+  };
+  float s = 1.0f, m;
+  if (p.given != nullptr) {
+    s = *p.given;
+  } else if (p.group == 0) {
+    split_rstd<E4M3>(rstd, m);
+    s = __fdiv_rn(__fmul_rn(__fdiv_rn(row_top, Q8<E4M3>::kZ), m), Q8<E4M3>::kMax);
+    if (s == 0.0f) s = 1.0f;                     // a scale that rounds to zero; a NaN stays
+    if (t == 0) p.scales[row] = s;
+  }
+#pragma unroll 1
+  for (int i = 0; i < NV; ++i) {
+    const int c0 = (i * p.team + t) * VEC;
+    if (!(slow >> i & 1) || c0 >= p.cols) continue;
+    if (p.group != 0) {
+      const int g0 = c0 / p.group * p.group;
+      float top[1] = {0.0f}, y[1];
+#pragma unroll 1
+      for (int c = g0; c < min(g0 + p.group, p.cols); ++c) {
+        y[0] = y_of(c);
+        top[0] = max_abs<1>(top[0], y);
+      }
+      s = __fdiv_rn(top[0], Q8<E4M3>::kMax);
+      if (s == 0.0f) s = 1.0f;
+      if (c0 == g0) p.scales[row * groups + c0 / p.group] = s;
+    }
+#pragma unroll 1
+    for (int c = c0; c < min(c0 + VEC, p.cols); ++c) {
+      const float q[1] = {__fdiv_rn(y_of(c), s)};
+      store_q<1, E4M3>(static_cast<uint8_t*>(p.y) + row * p.cols + c, q);
+    }
+  }
+}
+
 // ---- forward ------------------------------------------------------------------------------
 // One team of threads per row, up to VEC * NV elements a thread. QUANT: 0 none, 1 int8, 2 e4m3.
 // 8192 x 4096, bf16 with an fp32 residual: 403 MB in 63 us, 6.4 TB/s, what a plain copy reaches here. 8192 x 8192 bf16 to
-// e4m3 with groups of 128: 472 MB in 87 us, 5.4 TB/s; there the instruction issue is busy for 75% of the time (a
-// maximum, a scale and a conversion an element on top). 1 x 2048 f16: 1.6 us, a launch.
+// e4m3 with groups of 128: 472 MB in 91.6 us, 5.2 TB/s; there the instruction issue is busy for about 70% of the time (a
+// maximum, a scale, a quotient and a conversion an element on top; with a product by the reciprocal in place of the quotient
+// 87.4 us, but other codes on borders). 1 x 2048 f16: 1.6 us, a launch.
 // A persistent block that fetches its next row ahead gained nothing: with one row a block the
 // scheduler already has five blocks' loads in flight on an SM.
+// Blocks an SM of the 8-bit forms: three where a thread's elements fit 40 registers (8192 x 8192 e4m3, groups of 128: 91.6
+// against 105 us with two).
+template <typename TH, int VEC, int QUANT, int MAXT>
+constexpr int kFwdBlocks = QUANT == 0 || VEC == 1 ? 0 : MAXT == 512 && sizeof(TH) == 2 ? 3 : 1;
 template <typename TX, typename TH, int VEC, int NV, int QUANT, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(MAXT, kFwdBlocks<TH, VEC, QUANT, MAXT>) norm_fwd_kernel(const __grid_constant__ NormParams p) {
   __shared__ float red[32];
   __shared__ uint32_t red_max[QUANT != 0 ? 32 : 1];
+  __shared__ float red_rstd[QUANT != 0 ? 32 : 1];
   __shared__ uint32_t gmax[VEC == 1 && QUANT != 0 ? 1024 + 32 : 1];
   constexpr bool E4M3 = QUANT == 2;
   int who, t;
@@ -309,6 +418,8 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
   ss = team_sum(ss, p.team, red);
   const float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps));   // within 2 units in the last place
   if (p.rstd != nullptr && live && t == 0) p.rstd[row] = rstd;
+  float unit = rstd, m = 1.0f;                   // v becomes y; 8 bits: -y, or -z where the scale is found here
+  if (QUANT != 0) unit = -(p.given == nullptr ? split_rstd<E4M3>(rstd, m) : rstd);
 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -317,51 +428,61 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
       float w[VEC];
       load_w<VEC, TX>(p, (int64_t)k * VEC, w);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rstd), w[e]);
+      for (int e = 0; e < VEC; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], unit), w[e]);
       if (QUANT == 0) store_v<VEC, TX>(static_cast<TX*>(p.y) + row * p.cols + (int64_t)k * VEC, v[i]);
     }
   }
   if constexpr (QUANT != 0) {
     uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.cols;
+    // The fast form everywhere, without branches that would keep the pieces from overlapping; what it does not hold
+    // for is written again at the end. A maximum of zero gives zeros by any divisor, and the scale 1.
+    if ((threadIdx.x & 31) == 0) red_rstd[threadIdx.x >> 5] = rstd;      // for then, in no register
+    float row_top = 0.0f;
+    uint32_t slow = 0;
     if (p.group == 0) {
-      float s;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) row_top = max_abs<VEC>(row_top, v[i]);
       if (p.given != nullptr) {
-        s = *p.given;
+        const float s = *p.given, inv = __frcp_rn(s);
+        slow = s >= 0x1p-60f && s <= 0x1p60f && row_top <= s * 0x1p30f ? 0u : ~0u;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int k = i * p.team + t;
+          if (live && k < nvec) {
+            corrected_v<2>(v[i], s, inv);
+            store_q<VEC, E4M3>(q + (int64_t)k * VEC, v[i]);
+          }
+        }
       } else {
-        float amax = 0.0f;
+        row_top = __uint_as_float(team_max(__float_as_uint(row_top), p.team, red_max));
+        slow = plain_max(row_top) || row_top == 0.0f ? 0u : ~0u;
+        const float d = row_top == 0.0f ? 1.0f : plain_over_q<E4M3>(row_top), inv = rcp_approx(d);
+        if (live && t == 0) p.scales[row] = row_top == 0.0f ? 1.0f : plain_scale<E4M3>(d, m);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) amax = max_abs(amax, v[i][e]);
-        s = q_scale<E4M3>(team_max(__float_as_uint(amax), p.team, red_max));
-        if (live && t == 0) p.scales[row] = s;
-      }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int k = i * p.team + t;
-        if (live && k < nvec) {
-          divide(v[i], s);
-          store_q<VEC, E4M3>(q + (int64_t)k * VEC, v[i]);
+        for (int i = 0; i < NV; ++i) {
+          const int k = i * p.team + t;
+          if (live && k < nvec) {
+            corrected_v<1>(v[i], d, inv);
+            store_q<VEC, E4M3>(q + (int64_t)k * VEC, v[i]);
+          }
         }
       }
     } else {
       const int groups = (p.cols + p.group - 1) / p.group;
       float* scales = p.scales + row * groups;
       if constexpr (VEC > 1) {
-        // a group is 4 to 32 neighbouring lanes
+        // a group is 4 to 16 neighbouring lanes
         const int lanes = p.group / VEC;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int k = i * p.team + t;
-          float big = 0.0f;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) big = max_abs(big, v[i][e]);
-          uint32_t m = __float_as_uint(big);
-          for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          uint32_t u = __float_as_uint(max_abs<VEC>(0.0f, v[i]));
+          for (int o = lanes >> 1; o > 0; o >>= 1) u = max(u, __shfl_xor_sync(0xffffffffu, u, o));
           if (live && k < nvec) {
-            const float s = q_scale<E4M3>(m);
-            if ((k & (lanes - 1)) == 0) scales[k / lanes] = s;
-            divide(v[i], s);
+            const float top = __uint_as_float(u), d = u == 0 ? 1.0f : plain_over_q<E4M3>(top);
+            if (!plain_max(top) && u != 0) slow |= 1u << i;
+            if ((k & (lanes - 1)) == 0) scales[k / lanes] = u == 0 ? 1.0f : plain_scale<E4M3>(d, m);
+            corrected_v<1>(v[i], d, rcp_approx(d));
             store_q<VEC, E4M3>(q + (int64_t)k * VEC, v[i]);
           }
         }
@@ -373,22 +494,32 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int k = i * p.team + t;
-          const uint32_t m = __reduce_max_sync(0xffffffffu, k < nvec ? __float_as_uint(v[i][0]) & 0x7fffffffu : 0u);
-          if ((threadIdx.x & 31) == 0 && k < nvec) atomicMax(&gm[k / p.group], m);
+          const uint32_t u = __reduce_max_sync(0xffffffffu, k < nvec ? __float_as_uint(v[i][0]) & 0x7fffffffu : 0u);
+          if ((threadIdx.x & 31) == 0 && k < nvec) atomicMax(&gm[k / p.group], u);
         }
         __syncthreads();
-        if (live)
-          for (int g = t; g < groups; g += p.team) scales[g] = q_scale<E4M3>(gm[g]);
+        if (live) {
+          for (int g = t; g < groups; g += p.team) {
+            const float top = __uint_as_float(gm[g]);
+            if (top == 0.0f) scales[g] = 1.0f;
+            else if (plain_max(top)) scales[g] = plain_scale<E4M3>(plain_over_q<E4M3>(top), m);
+          }                                      // the others by the thread of the group's first column
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int k = i * p.team + t;
           if (live && k < nvec) {
-            divide(v[i], q_scale<E4M3>(gm[k / p.group]));
+            const uint32_t u = gm[k / p.group];
+            const float top = __uint_as_float(u), d = u == 0 ? 1.0f : plain_over_q<E4M3>(top);
+            if (!plain_max(top) && u != 0) slow |= 1u << i;
+            corrected_v<1>(v[i], d, rcp_approx(d));
             store_q<1, E4M3>(q + k, v[i]);
           }
         }
       }
     }
+    __syncwarp();
+    if (live && slow != 0) quant_slow<TX, TH, VEC, NV, E4M3>(p, slow, red_rstd[threadIdx.x >> 5], row_top);
   }
 }
 

@@ -301,6 +301,130 @@ def test_quant(shape, x_t, r_t, out):
     check_codes(q, given.double(), ref_norm(x, w)[0], out)
 
 
+def as_code(t, out):
+    """t (float32 or float64) to the nearest code, ties to even; NaN to 0 in int8."""
+    Q = QMAX[out]
+    t = t.clamp(-Q, Q)
+    return t.round().nan_to_num(0.0).to(torch.int8) if out == torch.int8 else t.to(out)
+
+
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("shape", [(200, 1024), (40, 8192), (65, 1001)])
+def test_quant_codes_on_borders(shape, out):
+    """bf16 values of few bits, so that y / s = h w Q / max|h w| often lies on a border between two codes. h w Q has at most
+    24 bits and the quotient in 64 bits is exact there; elsewhere it is 2^-24 or more away, relatively. So every code
+    is known."""
+    g = torch.Generator().manual_seed(shape[1])
+    x = (torch.randint(-127, 128, shape, generator=g) / 16).to(torch.bfloat16).cuda()
+    r = torch.randint(-8, 9, shape, generator=g).to(torch.bfloat16).cuda()
+    w = (torch.randint(1, 65, shape[1:], generator=g) / 32).to(torch.bfloat16).cuda()
+    for group in (0, 32, 128):
+        q, s, h = rms_norm_quant(x, w, residual=r, out_dtype=out, group=group)
+        p = h.double() * w.double()
+        width = group or shape[1]
+        top = torch.stack([c.abs().amax(1) for c in p.split(width, dim=1)], dim=1)
+        top = top.masked_fill(top == 0, 1.0).repeat_interleave(width, 1)[:, :shape[1]]
+        assert torch.equal(q.float(), as_code(p * QMAX[out] / top, out).float())
+
+
+def unit_rows(w, **kw):
+    """rms_norm_quant of one row of ones without eps: the norm is 1 exactly, so y is the weight w."""
+    w = torch.as_tensor(w, dtype=torch.float32)
+    pad = torch.zeros(1 << max(w.numel() - 1, 1).bit_length())           # a mean of 1 needs no power of two, but this is one
+    pad[:w.numel()] = w
+    q, s = rms_norm_quant(torch.ones(1, pad.numel(), device="cuda"), pad.cuda(), eps=0.0, **kw)
+    return q[0].cpu()[:w.numel()], s.cpu()
+
+
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+def test_quant_scale_is_the_quotient(out):
+    """s = max|y| / Q rounded once, for every significand of 17 bits (Qz y is exact then) and for sizes far from 1."""
+    v = torch.arange(1 << 16, 1 << 17).float() * 2.0 ** -16
+    for part in v.split(1024):
+        w = torch.zeros(1024, 32)
+        w[torch.arange(1024), torch.arange(1024) % 32] = part
+        _, s = unit_rows(w.flatten(), group=32, out_dtype=out)
+        assert np.array_equal(s[0].numpy(), part.numpy() / np.float32(QMAX[out]))
+    for e in (-115, -100, -61, -60, -30, 60, 99, 101, 126):
+        y = np.float32(2.0 ** e) * np.float32(1.25)
+        assert float(unit_rows([0.0, y, 0.0], out_dtype=out)[1]) == float(y / np.float32(QMAX[out]))
+
+
+def codes_near_borders(out):
+    """(s, y) with y / s next to a border: a product with a reciprocal good to 2^-23 and one correction is off by at most
+    2^-44.8 before it is rounded ((1.5 * 2^-23)^2), so it can round otherwise than
+    the exact quotient only where that lies this close to the middle between two fp32 numbers, one of which is a border: a
+    number M 2^i of b = 5 (e4m3) or 8 (int8) bits. In integers, 2 Y 2^k = S (M 2^(25 - b) +- 1) + c with |c| < 2^-44.8 2^49 < 19,
+    so S is within 19 of a multiple of 2^(25 - b). All such S, and for each the y around every border's neighbours."""
+    if out == torch.int8:
+        ties, step = np.arange(0.5, 127.0, 1.0), 1 << 17
+    else:
+        codes = torch.arange(127, dtype=torch.uint8).view(out).double().numpy()
+        ties, step = (codes[1:] + codes[:-1]) / 2, 1 << 20
+    f = ties.astype(np.float32)
+    assert (f == ties).all()
+    middles = np.concatenate([(f.astype(np.float64) + np.nextafter(f, np.float32(t))) / 2 for t in (0.0, 1e9)] + [ties])
+    for base in range(1 << 23, (1 << 24) + 1, step):
+        for S in range(max(base - 19, 1 << 23), min(base + 20, 1 << 24)):
+            y = (middles * S).astype(np.float32)                         # the product has at most 49 bits: exact in 64
+            y = np.concatenate([y, np.nextafter(y, np.float32(0)), np.nextafter(y, np.float32(3e38))])
+            yield np.float32(S * 2.0 ** -24), np.float32(2.0 ** -24) * np.concatenate([y, -y])
+
+
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+def test_quant_given_scale_next_to_every_border(out):
+    for s, y in codes_near_borders(out):
+        q, _ = unit_rows(y, scale=torch.tensor(s, device="cuda"), out_dtype=out)
+        assert torch.equal(q.view(torch.uint8), as_code(torch.from_numpy(y / s), out).view(torch.uint8)), float(s)
+
+
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+def test_quant_given_scale_of_any_size(out):
+    y = np.float32([0.0, -0.0, 1.0, -2.5, 1e-45, -1e-38, 3e38, -3.3e38, 1e30, 7e-30, np.inf, -np.inf, np.nan])
+    with np.errstate(all="ignore"):
+        for s in np.float32([2.0 ** 127, 1.5e38, 3e38, 2.0 ** 100, 1e25, 1e-30, 1e-38, 1e-45, 5e-40, 0.0, np.inf, np.nan, -1.0,
+                             -1e-40, -2e38, 1.0]):
+            q, _ = unit_rows(y, scale=torch.tensor(s, device="cuda"), out_dtype=out)
+            want = as_code(torch.from_numpy(y / s), out)
+            assert torch.equal(q.float().nan_to_num(1e3), want.float().nan_to_num(1e3)), float(s)
+
+
+@gpu
+@pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("shape", [(64, 512), (3, 4096), (40, 333), (2, 20000), (2, 20001)])
+def test_quant_rows_of_every_size(shape, out):
+    """Rows and groups whose maximum leaves the range of fast quotients stand beside ordinary ones, zeros and NaN: each has its
+    own scale and codes."""
+    R, C = shape
+    x = torch.ones(R, C, device="cuda")
+    g = torch.Generator().manual_seed(C)
+    w = torch.randn(C, generator=g)
+    size = torch.tensor([1.0, 0.0, 1e-20, 1e25, 1e-36, 3e36, 1e-44])
+    w *= size.repeat_interleave(32).repeat(-(-C // 224))[:C]
+    w[C // 2] = float("nan")
+    for group in (32, 64):
+        q, s = rms_norm_quant(x, w.cuda(), eps=0.0, out_dtype=out, group=group)
+        y = w.double()
+        top = torch.stack([c.abs().amax() for c in y.split(group)])
+        ref = top / QMAX[out]
+        ref32 = ref.float()                                # what underflows to 0 has the scale 1
+        ref = torch.where(ref32 == 0, torch.ones_like(ref), ref)
+        nan = torch.isnan(ref)
+        for r in range(R):
+            got = s[r].cpu().double()
+            assert torch.equal(torch.isnan(got), nan)
+            # the norm of ones is 1 to within F32; near the smallest number a rounding is half of 2^-149
+            assert ((got - ref).abs() <= 2 * F32 * ref + 2.0 ** -149)[~nan].all()
+            per = s[r].cpu().double().repeat_interleave(group)[:C]
+            live = ~torch.isnan(per)
+            check_codes(q[r].cpu()[live], per[live], y[live], out)
+            assert not q[r].cpu()[~live].float().nan_to_num(0.0).any()
+
+
 @gpu
 def test_quant_zero_and_nonfinite_rows():
     x = rows((6, 256), torch.float32, 1)
