@@ -204,15 +204,16 @@ class RMSNorm(nn.Module):
 
     @classmethod
     def from_torch(cls, norm: nn.RMSNorm) -> "RMSNorm":
-        """The same norm over the source module's own Parameter (optimiser references stay valid)."""
+        """The same norm over the source module's own Parameter (optimiser references stay valid). An eps of None is, as
+        in torch, that of the type the norm is computed in: float32's for 16-bit layers too."""
         if len(norm.normalized_shape) != 1:
             raise ValueError(f"normalized_shape {tuple(norm.normalized_shape)}: the last dimension only")
-        if norm.weight is not None:
-            eps = norm.eps if norm.eps is not None else torch.finfo(norm.weight.dtype).eps
-        elif norm.eps is None:
-            raise ValueError("a norm without weight and eps takes its eps from each input's type; set eps")
-        else:
-            eps = norm.eps
+        eps = norm.eps
+        if eps is None:
+            if norm.weight is None:
+                raise ValueError("a norm without weight and eps takes its eps from each input's type (float64's, or float32's "
+                                 "for the others); set eps")
+            eps = torch.finfo(torch.float64 if norm.weight.dtype == torch.float64 else torch.float32).eps
         m = cls(norm.normalized_shape[0], eps=eps, elementwise_affine=False)
         m.weight = norm.weight
         m.train(norm.training)

@@ -515,6 +515,41 @@ def test_module():
     assert q.shape == x.shape and s.shape == (9, 5)
 
 
+def default_eps_layer(t, device):
+    src = torch.nn.RMSNorm(192, device=device, dtype=t)
+    with torch.no_grad():
+        src.weight.copy_(torch.randn(192, generator=torch.Generator().manual_seed(1)))
+    x = (torch.randn(40, 192, generator=torch.Generator().manual_seed(2))
+         * torch.logspace(-4, 1, 40)[:, None]).to(t).to(device)
+    return src, x
+
+
+def check_default_eps(y, src, x):
+    """torch's own layer and y are each off the formula with float32's eps by F32 and one rounding, so by twice that from one
+    another; with another type's eps rows of 1e-2 are off by more than 10%."""
+    ref, _ = ref_norm(x, src.weight.detach(), torch.finfo(torch.float32).eps)
+    check_y(src(x).detach(), ref)
+    check_y(y, ref)
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16, torch.float32])
+def test_default_eps_is_torchs(t):
+    src, x = default_eps_layer(t, "cpu")
+    m = RMSNorm.from_torch(src)
+    check_default_eps(ref_norm(x, src.weight.detach(), m.eps)[0].to(t), src, x)
+
+
+@gpu
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16, torch.float32])
+def test_swapped_layer_with_default_eps(t):
+    from rl_quant_b200 import swap
+    src, x = default_eps_layer(t, "cuda")
+    model = torch.nn.Sequential(src)
+    swap.apply_norm(model)
+    assert isinstance(model[0], RMSNorm)
+    check_default_eps(model(x).detach(), src, x)
+
+
 # -- refusals (no GPU) -----------------------------------------------------------------------------
 
 
