@@ -456,6 +456,13 @@ int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, in
  * `stream`.                                                                 */
 int glad_w4_linear_status(uint32_t* status, void* stream);
 
+/* Test hook of that failure path: in the many-row kernels launched after this call the
+ * barriers named by the bits of `hold` wait for an arrival that never comes (1: a stage's
+ * operands, 2: a free accumulator, 4: a free weight slot, 8: the sums of a cluster's
+ * other blocks), and a wait gives up after `limit_ns` nanoseconds (at most, and 0 for, the
+ * normal 2 s). (0, 0) restores normal operation. Process-wide.                */
+int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
+
 /* ---- weight refresh (qrt/runtime.py:195-271) ------------------------------- */
 
 /* QuantLinear.requantize_ (qrt/qlinear.py:84-102) in place, for `n` layers in

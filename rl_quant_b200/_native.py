@@ -162,6 +162,7 @@ SIGNATURES = {
     "glad_w4_linear_forward": (c_int, [POINTER(GladW4Weight), c_void_p, c_int, c_int64, c_int64, c_void_p, c_int,
                                        c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "glad_w4_linear_status": (c_int, [POINTER(c_uint32), c_void_p]),
+    "glad_debug_w4_wait": (c_int, [c_uint32, c_uint64]),
     "glad_requant_qlinear": (c_int, [POINTER(GladQLinearSrc), c_int, c_void_p]),
     "glad_requant_qcnn": (c_int, [POINTER(GladQCNNSrc), c_void_p]),
     "glad_cast_copy": (c_int, [POINTER(GladCastCopy), c_int, c_void_p]),

@@ -38,6 +38,8 @@ struct W4Params {
   void* y;
   int y_dtype;
   int y_vec;                // four columns of y can be stored at once
+  uint32_t wait_ns;         // many rows: limit of a wait
+  uint32_t hold;            // many rows: barriers that wait for an arrival that never comes (glad_debug_w4_wait; 0)
 };
 
 struct e4m3_t { uint8_t v; };
@@ -496,10 +498,11 @@ struct Tile {
   static_assert(NS % MW == 0 && ND % MW == 0 && PD % (DW / 4) == 0 && NS % (DW / 4) == 0, "phases");
   static_assert(2 * MT * 512 <= NS * kStage, "the sums are sent and joined in the stage buffers");
   static_assert(kSmem <= 232448, "shared memory of one block");
-  static_assert((2 * NS + 2 * PD + 2 * ND + 1) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 * NS + 2 * PD + 2 * ND + 1 + MW) * 8 + 12 <= 512, "barrier area");
 };
 
-// Wait for a phase, 2 s at most. The timer is read only after many tries: a read costs more than most waits.
+// Wait for a phase, abort[1] nanoseconds at most; then abort[0] is set, which ends every wait of the block. The timer
+// is read only after many tries: a read costs more than most waits.
 __device__ __noinline__ bool w4_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
   for (int i = 0; i < 1000; ++i)
     if (mbar_try_wait(bar, parity)) return true;
@@ -507,7 +510,7 @@ __device__ __noinline__ bool w4_wait_slow(uint64_t* bar, uint32_t parity, volati
   while (!*abort) {
     for (int i = 0; i < 64; ++i)
       if (mbar_try_wait(bar, parity)) return true;
-    if (global_timer_ns() - t0 > 2000000000ull) {
+    if (global_timer_ns() - t0 > (uint32_t)abort[1]) {
       *abort = 1;
       atomicOr(&g_w4_status, kDevErrMmaTimeout);
     }
@@ -517,6 +520,15 @@ __device__ __noinline__ bool w4_wait_slow(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ bool w4_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return mbar_try_wait(bar, parity) || w4_wait_slow(bar, parity, abort);
 }
+// The same by a whole warp: lanes may see a phase end, or the block give up, at different tries, and what follows
+// (tensor-memory accesses, elections) takes all of them or none.
+__device__ __forceinline__ bool w4_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) ||
+         __all_sync(0xffffffffu, w4_wait_slow(bar, parity, abort));
+}
+// How long a warp waits at its end for copies and products that it issued: they take microseconds, but the barrier
+// may also count arrivals of others, which do not come after a wait has run out.
+constexpr uint64_t kDrainNs = 10000000;
 
 // K-major operand with 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart, the 16-byte
 // piece i of row r at i ^ (r & 7).
@@ -640,8 +652,9 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   uint64_t* dfull = wempty + L::PD;                      // [ND]
   uint64_t* dempty = dfull + L::ND;                      // [ND]
   uint64_t* joined = dempty + L::ND;                     // sums of the cluster's other blocks are here
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined + 1);
-  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint64_t* drain = joined + 1;                          // [MW] all products of a warp are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + L::MW);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);   // {a wait ran out, the limit in ns}
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // warp-uniform
   const int S = p.splits, rank = S > 1 ? (int)cluster_ctarank() : 0;
@@ -653,20 +666,22 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
   if (warp == CTL) tmem_alloc(tmem_slot, L::kCols);
   if (tid == 0) {
     for (int i = 0; i < L::NS; ++i) {
-      mbar_init(&full[i], 4 + (p.x_tma ? 1 : 0));
+      mbar_init(&full[i], 4 + (p.x_tma ? 1 : 0) + (p.hold & 1));
       mbar_init(&empty[i], SG < L::MW ? SG : L::MW);
     }
     for (int i = 0; i < L::PD; ++i) {
       mbar_init(&wfull[i], 1);
-      mbar_init(&wempty[i], 4);
+      mbar_init(&wempty[i], 4 + (p.hold >> 2 & 1));
     }
     for (int i = 0; i < L::ND; ++i) {
       mbar_init(&dfull[i], 1);
-      mbar_init(&dempty[i], SW);
+      mbar_init(&dempty[i], SW + (p.hold >> 1 & 1));
     }
-    mbar_init(joined, 1);
+    mbar_init(joined, 1 + (p.hold >> 3 & 1));
+    for (int i = 0; i < L::MW; ++i) mbar_init(&drain[i], 1);
     fence_mbar_init();
-    *abort = 0;
+    abort[0] = 0;
+    abort[1] = (int)p.wait_ns;
   }
   tc_fence_before();
   __syncthreads();
@@ -687,8 +702,8 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
           mbar_arrive_expect_tx(&wfull[slot], 8192);
           bulk_copy_g2s(slots + slot * L::kSlot, src, 8192, &wfull[slot]);
         }
-        // after a failure: copies that were issued land before the block leaves
-        for (int k = max(0, i - L::PD); k < i && *abort; ++k) mbar_wait_bounded(&wfull[k % L::PD], (k / L::PD) & 1);
+        // copies that were issued land before the block leaves, also where nobody waits for them any more
+        for (int k = max(0, i - L::PD); k < i; ++k) mbar_wait_bounded(&wfull[k % L::PD], (k / L::PD) & 1, kDrainNs);
       }
     } else if (warp == CTL + L::MW + 1) {
       // ---- x tiles
@@ -703,7 +718,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
           for (int h = 0; h < XB; ++h)
             tma_x(base + st * L::kStage + h * L::kBlock, &xmap, (un0 + i) * 128 + h * 64, (int)m0, &full[st]);
         }
-        for (int k = max(0, i - L::NS); k < i && *abort; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1);
+        for (int k = max(0, i - L::NS); k < i; ++k) mbar_wait_bounded(&full[k % L::NS], (k / L::NS) & 1, kDrainNs);
       }
     } else {
       // ---- products of every MW-th group. A wait must meet every phase of its barrier (phases are told apart
@@ -716,14 +731,14 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
       for (int u = 0; ok && u < units; ++u) {
         const int st = u % L::NS;
         if (SG < L::MW && (me - u * SG % L::MW + L::MW) % L::MW >= SG) continue;   // none of this unit's groups
-        ok = __all_sync(0xffffffffu, w4_wait(&full[st], (u / L::NS) & 1, abort));
+        ok = w4_wait_warp(&full[st], (u / L::NS) & 1, abort);
         const uint32_t a = tmem + L::kACol + st * L::ACOLS;
         const uint64_t b = desc_sw128(base + st * L::kStage);
 #pragma unroll
         for (int j = 0; j < SG; ++j) {
           const int gi = u * SG + j, d = gi % L::ND;
           if (gi % L::MW != me) continue;
-          if (ok && gi >= L::ND) ok = __all_sync(0xffffffffu, w4_wait(&dempty[d], (gi / L::ND - 1) & 1, abort));
+          if (ok && gi >= L::ND) ok = w4_wait_warp(&dempty[d], (gi / L::ND - 1) & 1, abort);
           tc_fence_after();
           if (ok && elect_one()) {
 #pragma unroll
@@ -741,9 +756,11 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
         if (ok && elect_one()) mma_commit(&empty[st]);
         __syncwarp();
       }
-      // after a failure: products that were issued end before their operands go
-      if (*abort)
-        for (int d = 0; d < L::ND; ++d) mbar_wait_bounded(&dfull[d], 0, 10000000ull);
+      // products that were issued end before their operands and accumulators go, also where nobody waits for them any
+      // more. A barrier of its own: the phases of dfull do not tell which use of an accumulator was the last.
+      if (elect_one()) mma_commit(&drain[me]);
+      __syncwarp();
+      mbar_wait_bounded(&drain[me], 0, kDrainNs);
     }
   } else if (warp >= SW) {
     // ---- A operand
@@ -773,8 +790,8 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     };
     for (int u = (warp - SW) >> 2; u < units; u += DW / 4) {   // a team meets all phases of its slots
       const int slot = u % L::PD;
-      if (ok) ok = w4_wait(&wfull[slot], (u / L::PD) & 1, abort);
-      if (ok && u >= L::NS) ok = w4_wait(&empty[u % L::NS], (u / L::NS - 1) & 1, abort);
+      if (ok) ok = w4_wait_warp(&wfull[slot], (u / L::PD) & 1, abort);
+      if (ok && u >= L::NS) ok = w4_wait_warp(&empty[u % L::NS], (u / L::NS - 1) & 1, abort);
       if (!ok) break;
       tc_fence_after();
       const uint8_t* in = slots + slot * L::kSlot;
@@ -868,7 +885,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
         const int gi = u * SG + j, d = gi % L::ND;
-        if (ok) ok = w4_wait(&dfull[d], (gi / L::ND) & 1, abort);
+        if (ok) ok = w4_wait_warp(&dfull[d], (gi / L::ND) & 1, abort);
         tc_fence_after();
         // one piece of 16 columns is read while the one before is added, where registers allow it
         constexpr int CH = 16, PIECES = NC / CH, AHEAD = MT == 128 ? 0 : 1;
@@ -917,7 +934,7 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
     if (tid < S)
       bulk_copy_s2c(mapa_shared(smem_u32(smem) + (MT + rank * own) * 512, tid), smem_u32(smem) + tid * own * 512, own * 512,
                     mapa_shared(smem_u32(joined), tid));
-    if (!w4_wait(joined, 0, abort)) mbar_wait_bounded(joined, 0);
+    if (!w4_wait_warp(joined, 0, abort)) mbar_wait_bounded(joined, 0, kDrainNs);
     __syncwarp();
     cluster_arrive_relaxed();                            // this block has received all that is sent to it
   } else {
@@ -955,6 +972,10 @@ __global__ void __launch_bounds__(Tile<(int)sizeof(TX), MT, GROUP>::kThreads, 1)
 }
 
 // ---- launch -------------------------------------------------------------------------------------
+// Failure-path test hook (glad_debug_w4_wait): process-wide, read at launch.
+uint32_t g_w4_hold = 0;
+uint32_t g_w4_wait_ns = 2000000000u;
+
 int current_device() {                                   // -1: none, or past the caches below
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : -1;
@@ -1056,6 +1077,8 @@ cudaError_t launch_tile(W4Params p, cudaStream_t st) {
   int s = 1;
   while (s < 8 && (int64_t)nt * mt * s * 2 <= sms && units >= 4 * s && fits(2 * s)) s *= 2;
   p.splits = s;
+  p.wait_ns = g_w4_wait_ns;
+  p.hold = g_w4_hold;
   CUtensorMap map{};
   const CUtensorMapDataType type = sizeof(TX) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : std::is_same<TX, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
@@ -1142,6 +1165,14 @@ int glad_w4_linear_status(uint32_t* status, void* stream) {
   }
   *status = word;
   if (word != 0) return set_last_error(GLAD_ERR_DEVICE, "glad_w4_linear_status: a bounded wait inside a kernel ran out");
+  return GLAD_OK;
+}
+
+int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns) {
+  if (hold > 15 || limit_ns > 2000000000ull)
+    return set_last_error(GLAD_ERR_INVALID_ARG, "glad_debug_w4_wait: hold above 15 or limit_ns above 2 s");
+  g_w4_hold = hold;
+  g_w4_wait_ns = limit_ns ? (uint32_t)limit_ns : 2000000000u;
   return GLAD_OK;
 }
 

@@ -12,6 +12,7 @@ import torch.nn as nn
 
 from rl_quant_b200 import _native as N
 from rl_quant_b200 import swap
+from rl_quant_b200.fused import DeviceStatusError
 from rl_quant_b200.norm import RMSNorm, rms_norm_quant
 from rl_quant_b200.w4a16 import quantize_w4
 from rl_quant_b200.w4linear import W4Linear, W4Weight, pack_w4, unpack_w4, w4_linear, w4_status
@@ -192,6 +193,36 @@ def test_status():
     with torch.cuda.stream(side):
         assert w4_status() == 0
     assert w4_status("cuda:0") == 0
+
+
+@gpu
+@pytest.mark.parametrize("t", [F16, I8, E4M3])
+@pytest.mark.parametrize("m", [20, 40, 100])
+@pytest.mark.parametrize("n,k,hold", [(256, 16384, 1), (256, 16384, 2), (256, 16384, 4), (256, 16384, 8), (19200, 2048, 1),
+                                      (19200, 2048, 2), (19200, 2048, 4), (100, 250, 1), (256, 2050, 1)])
+def test_waits_that_run_out(n, k, hold, m, t):
+    """One arrival that never comes (a host switch) and a limit of a millisecond: the kernel gives up, says so in the
+    status word, and the next calls are what they were. With blocks that share a tile's inputs (few columns) and
+    without, rows that are copied by TMA and rows that are not, and a single unit of inputs."""
+    lib = N.load()
+    q, packed, s = weight(n, k, 64, 1)
+    w = pack_w4(packed, s, 64)
+    x = rows(m, k, t, 2)
+    kw = {} if t == F16 else dict(x_scale=torch.full((m, -(-k // 64)), 0.01, device="cuda"), out_dtype=F16)
+    want = w4_linear(x, w, **kw)
+    assert w4_status() == 0
+    N.check(lib.glad_debug_w4_wait(hold, 1_000_000))
+    try:
+        w4_linear(x, w, **kw)
+        torch.cuda.synchronize()
+    finally:
+        N.check(lib.glad_debug_w4_wait(0, 0))
+    with pytest.raises(DeviceStatusError):
+        w4_status()
+    assert w4_status() == 0
+    for _ in range(2):
+        assert torch.equal(w4_linear(x, w, **kw), want)
+    assert w4_status() == 0
 
 
 @gpu
@@ -449,6 +480,7 @@ def test_abi_refusals():
         assert lib.glad_last_error()
     assert lib.glad_w4_tiles_bytes(127, 8, 64) == 0 and lib.glad_w4_scales_bytes(128, 8, 48) == 0
     assert lib.glad_w4_linear_status(None, None) == N.GLAD_ERR_INVALID_ARG
+    assert lib.glad_debug_w4_wait(16, 0) == lib.glad_debug_w4_wait(1, 2_000_000_001) == N.GLAD_ERR_INVALID_ARG
 
 
 def test_status_raises(monkeypatch):
