@@ -452,8 +452,9 @@ int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, in
 /* Device-side status word of glad_w4_linear_forward on the current device: 0, or
  * GLAD_DEVERR_* bits when a bounded wait inside a kernel ran out since the last
  * call of this function, in which case that call's outputs are not valid; reads
- * and clears it and returns GLAD_ERR_DEVICE when it was not 0. Synchronises
- * `stream`.                                                                 */
+ * and clears it in one step and returns GLAD_ERR_DEVICE when it was not 0. One word for the
+ * whole device: it tells of every caller's kernels, and to whoever asks first. It covers
+ * the work ordered before it in `stream`, which it synchronises.            */
 int glad_w4_linear_status(uint32_t* status, void* stream);
 
 /* Test hook of that failure path: in the many-row kernels launched after this call the

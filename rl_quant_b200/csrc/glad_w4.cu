@@ -12,6 +12,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdio>
 #include <type_traits>
 
@@ -466,6 +467,11 @@ __global__ void __launch_bounds__(512, 1) w4_rows_kernel(const __grid_constant__
 // and the hand-offs between them. A deeper ring of x (54 us where four stages took 47.5), 16 unpacking warps, one or four
 // product warps and tiles of 256 rows were slower or no faster.
 __device__ unsigned int g_w4_status;
+// Reads and clears the status word in one step, so that a bit set meanwhile is either returned or stays; the copies that
+// calls at the same time bring to the host have words of their own.
+constexpr int kStatusCalls = 64;
+__device__ unsigned int g_w4_taken[kStatusCalls];
+__global__ void w4_take_status_kernel(int slot) { g_w4_taken[slot] = atomicExch(&g_w4_status, 0u); }
 
 template <int XB, int MT, int GROUP>                     // XB: bytes of an input
 struct Tile {
@@ -1150,14 +1156,14 @@ size_t glad_w4_scales_bytes(int in_features, int out_features, int group) {
 int glad_w4_linear_status(uint32_t* status, void* stream) {
   if (!status) return set_last_error(GLAD_ERR_INVALID_ARG, "glad_w4_linear_status: status is NULL");
   const cudaStream_t st = (cudaStream_t)stream;
-  const unsigned int zero = 0;
+  static std::atomic<unsigned int> calls{0};
+  const int slot = (int)(calls.fetch_add(1) % kStatusCalls);
   unsigned int word = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(&word, g_w4_status, sizeof(word), 0, cudaMemcpyDeviceToHost, st);
+  w4_take_status_kernel<<<1, 1, 0, st>>>(slot);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = cudaMemcpyFromSymbolAsync(&word, g_w4_taken, sizeof(word), slot * sizeof(word), cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && word != 0) {
-    e = cudaMemcpyToSymbolAsync(g_w4_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  }
   if (e != cudaSuccess) {
     char msg[200];
     snprintf(msg, sizeof(msg), "glad_w4_linear_status: %s", cudaGetErrorString(e));

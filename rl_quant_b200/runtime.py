@@ -142,6 +142,7 @@ class InferenceRunner:
         self._ppo_rng = None
         self._fused_ac = None
         self._fused_ac_err = None
+        self._w4_told = w4linear.w4_failures()
         self._g_refresh = None
         self._g_sync = None
         self._sync_items = None
@@ -290,12 +291,14 @@ class InferenceRunner:
         check (directly or by a captured graph's replay) reported that a bounded
         device-side wait ran out; its outputs are then not valid. Reads and clears the
         status word of every workspace (one host synchronisation): call it once per PPO
-        iteration, as ``accelerate_runner`` does before each update."""
+        iteration, as ``accelerate_runner`` does before each update. 4-bit layers share one
+        word a device: every runner with such layers is told of each failure there once."""
         for f in (self._fused, self._fused_critic, self._fused_ac):
             if f is not None:
                 f.check_status()
         if any(isinstance(m, w4linear.W4Linear) for m in self.model.modules()):
-            w4linear.w4_status(self._device())
+            with w4linear.w4_status_reader(self.__dict__.setdefault("_w4_told", {})):
+                w4linear.w4_status(self._device())
 
     def _device(self):
         for t in self.model.parameters():

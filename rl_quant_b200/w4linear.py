@@ -7,7 +7,9 @@ the group's scale multiplies the group's sum: y = sum_g s[n,g] * (sum_k x[m,k] q
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import threading
 
 import torch
 import torch.nn as nn
@@ -158,17 +160,54 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
     return y
 
 
+# The kernels' status word is one a device and is cleared by reading. So that no reader loses what another one read
+# first, each failure found is counted here, and a reader (every InferenceRunner; the direct callers together) keeps the
+# counts that it has been told of.
+_status_lock = threading.Lock()
+_failures: dict[int, tuple[int, int]] = {}      # device index -> (failures found, bits of the last one)
+_told: dict[int, int] = {}
+_reader = threading.local()
+
+
+def w4_failures() -> dict[int, int]:
+    """Failures found so far by device index: where a new reader starts."""
+    with _status_lock:
+        return {k: n for k, (n, _) in _failures.items()}
+
+
+@contextlib.contextmanager
+def w4_status_reader(told: dict[int, int]):
+    """``w4_status`` calls of this thread inside are those of the reader that keeps ``told``."""
+    old, _reader.told = getattr(_reader, "told", None), told
+    try:
+        yield
+    finally:
+        _reader.told = old
+
+
 def w4_status(device=None) -> int:
-    """Device status bits of the w4_linear calls on ``device`` since the last call (0: fine); reads, clears and, where a
-    bounded wait inside a kernel ran out, raises ``DeviceStatusError``. Synchronises the current stream."""
+    """Device status bits of the w4_linear calls on ``device`` since this reader's last call (0: fine); where a bounded
+    wait inside a kernel ran out, raises ``DeviceStatusError``. The word is the device's: a failure of anyone's kernels
+    is told to every reader once. Covers the work before it in the current stream, which it synchronises."""
     from .fused import DeviceStatusError
+    index = device if isinstance(device, int) or device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
     word = ctypes.c_uint32(0)
-    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
-        rc = N.load().glad_w4_linear_status(word, N.stream_handle())
-    if rc == N.GLAD_ERR_DEVICE:
-        raise DeviceStatusError(f"w4_linear: device status {word.value:#x}")
-    N.check(rc, "w4_status")
-    return word.value
+    with _status_lock:                  # reading the word and counting are one step
+        with torch.cuda.device(index):
+            rc = N.load().glad_w4_linear_status(word, N.stream_handle())
+        if rc != N.GLAD_ERR_DEVICE:
+            N.check(rc, "w4_status")
+        count, bits = _failures.get(index, (0, 0))
+        if rc == N.GLAD_ERR_DEVICE:
+            count, bits = _failures[index] = (count + 1, word.value)
+        told = getattr(_reader, "told", None)
+        told = _told if told is None else told
+        known, told[index] = told.get(index, 0), count
+    if known != count:
+        raise DeviceStatusError(f"w4_linear: device status {bits:#x}")
+    return 0
 
 
 class W4Linear(nn.Module):

@@ -4,6 +4,7 @@ Tolerance, fixed before the first run: the products x * q are exact; a tensor-co
 largest term, so each of at most K/16 steps, 64 joins and scale products is off by at most 2^-23 of the sum of
 magnitudes S = sum |x q| s xs seen so far, in all (K/16 + 64) * 2^-23 * S; the result is rounded once (half a step)."""
 import contextlib
+import threading
 
 import numpy as np
 import pytest
@@ -512,6 +513,100 @@ def test_runner_checks_w4_status(monkeypatch):
     swap.apply(run.model, {"0": {"bits": 4}})
     run.check_status()
     assert asked == [torch.device("cpu")]
+
+
+def bare_runner():
+    from rl_quant_b200.runtime import InferenceRunner
+    run = InferenceRunner.__new__(InferenceRunner)
+    run._fused = run._fused_critic = run._fused_ac = None
+    run.model = nn.Sequential(W4Linear(nn.Linear(64, 8)))
+    run._device = lambda: 0
+    return run
+
+
+def test_every_reader_learns_of_a_failure(monkeypatch):
+    """Two runners and a direct caller on one device: the first to ask clears the device's word, and still all three are
+    told, once each, of each failure; another device's readers are not."""
+    class Fake:
+        bits = {0: 0, 1: 0}
+
+        def glad_w4_linear_status(self, word, stream):
+            word.value, self.bits[device[0]] = self.bits[device[0]], 0
+            return N.GLAD_ERR_DEVICE if word.value else N.GLAD_OK
+
+    device = [0]
+
+    def select(index):
+        device[0] = index
+        return contextlib.nullcontext()
+
+    monkeypatch.setattr(N, "load", Fake)
+    monkeypatch.setattr(N, "stream_handle", lambda d=None: 0)
+    monkeypatch.setattr(torch.cuda, "device", select)
+    a, b = bare_runner(), bare_runner()
+    for _ in range(2):                       # whatever was found before
+        for ask in (a.check_status, b.check_status, lambda: w4_status(0)):
+            with contextlib.suppress(DeviceStatusError):
+                ask()
+    for first in range(3):
+        asks = [a.check_status, b.check_status, lambda: w4_status(0)]
+        Fake.bits[0] = 1
+        assert w4_status(1) == 0
+        for ask in asks[first:] + asks[:first]:
+            with pytest.raises(DeviceStatusError):
+                ask()
+        for ask in asks:
+            ask()
+    a.check_status()
+    Fake.bits[0] = 1
+    with pytest.raises(DeviceStatusError):
+        b.check_status()
+    Fake.bits[0] = 1
+    with pytest.raises(DeviceStatusError):
+        a.check_status()
+    with pytest.raises(DeviceStatusError):
+        b.check_status()
+    with pytest.raises(DeviceStatusError):
+        w4_status(0)
+
+
+@gpu
+def test_readers_on_the_device():
+    """The same with kernels: one whose wait runs out on a side stream, two runners, a direct caller; calls in other streams
+    and threads at the same time get words of their own."""
+    lib = N.load()
+    q, packed, s = weight(256, 2048, 64, 1)
+    w, x = pack_w4(packed, s, 64), rows(40, 2048, F16, 2)
+    a, b = bare_runner(), bare_runner()
+    for ask in (a.check_status, b.check_status, w4_status):
+        with contextlib.suppress(DeviceStatusError):
+            ask()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    N.check(lib.glad_debug_w4_wait(1, 1_000_000))
+    try:
+        with torch.cuda.stream(side):
+            w4_linear(x, w)
+        side.synchronize()
+    finally:
+        N.check(lib.glad_debug_w4_wait(0, 0))
+    for ask in (b.check_status, a.check_status, w4_status):
+        with pytest.raises(DeviceStatusError):
+            ask()
+    found = []
+
+    def many():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                found.append(w4_status())
+
+    threads = [threading.Thread(target=many) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    a.check_status()
+    assert found == [0] * 200
 
 
 @pytest.mark.parametrize("t", [torch.float16, torch.bfloat16, torch.float32, torch.float64])
