@@ -214,7 +214,7 @@ class W4Linear(nn.Module):
     """``nn.Linear`` with 4-bit weights at inference and its own Parameters in training, like ``QuantLinear``:
     with gradients enabled the forward is ``F.linear`` on the source layer's weight and bias; without, ``w4_linear`` on
     the laid-out copy, which ``requantize_`` rewrites in place (captured CUDA graphs stay valid).
-    ``forward(q, x_scale)`` takes 8-bit rows."""
+    ``forward(q, x_scale)`` takes 8-bit rows, for inference only: refused while a gradient of its weight is asked for."""
 
     def __init__(self, linear: nn.Linear, group: int = 64):
         super().__init__()
@@ -252,8 +252,11 @@ class W4Linear(nn.Module):
         return W4Weight(self.tiles, self.scales, self.in_features, self.out_features, self.group)
 
     def forward(self, x, x_scale=None, out_dtype=None):
-        if torch.is_grad_enabled() and x_scale is None:
-            return F.linear(x, self.weight, self.bias)
+        if torch.is_grad_enabled():
+            if x_scale is None:
+                return F.linear(x, self.weight, self.bias)
+            if any(t is not None and t.requires_grad for t in (x, x_scale, self.weight, self.bias)):
+                raise RuntimeError("W4Linear on 8-bit rows has no gradient; use torch.no_grad()")
         if out_dtype is None and x_scale is not None:
             out_dtype = self.weight.dtype
         bias = self.bias

@@ -515,6 +515,24 @@ def test_runner_checks_w4_status(monkeypatch):
     assert asked == [torch.device("cpu")]
 
 
+def test_8_bit_rows_refuse_a_gradient():
+    """8-bit rows have no training form: with gradients enabled they are refused, not served without one."""
+    q, one = torch.zeros(3, 64, dtype=I8), torch.ones(())
+    m = W4Linear(nn.Linear(64, 8))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(q, x_scale=one)
+    m.weight.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(q, x_scale=one)                     # the bias
+    m.bias.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(q, x_scale=one.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        m(q, x_scale=one)                     # nothing asks for one: served (by the kernels only)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        W4Linear(nn.Linear(64, 8))(q, x_scale=one)
+
+
 def bare_runner():
     from rl_quant_b200.runtime import InferenceRunner
     run = InferenceRunner.__new__(InferenceRunner)
