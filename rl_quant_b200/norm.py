@@ -161,7 +161,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
             raise ValueError("a given scale is one for the whole tensor (group 0)")
         if scale.numel() != 1 or scale.dtype != torch.float32 or scale.device != x.device:
             raise ValueError("scale must be one float32 value on x's device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual, scale)):
         raise RuntimeError("rms_norm_quant has no gradient; use rms_norm, or torch.no_grad()")
     _check(x, weight, residual, eps)
     x2 = _rows(x)

@@ -143,7 +143,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
         if not bias.is_contiguous():
             bias = bias.contiguous()
         bp = bias.data_ptr()
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (x_scale is not None and x_scale.requires_grad)):
         raise RuntimeError("w4_linear has no gradient; use torch.no_grad()")
     N.require_cuda(x)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)

@@ -533,6 +533,20 @@ def test_8_bit_rows_refuse_a_gradient():
         W4Linear(nn.Linear(64, 8))(q, x_scale=one)
 
 
+def test_scales_refuse_a_gradient():
+    q, packed, s = weight(24, 128, 64, 1, "cpu")
+    w, x = pack_w4(packed, s, 64), torch.zeros(3, 128, dtype=I8)
+    for shape in ((), (3, 1), (3, 2)):
+        xs = torch.ones(shape, requires_grad=True)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            w4_linear(x, w, x_scale=xs, out_dtype=F16)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            w4_linear(x, w, x_scale=xs, out_dtype=F16)
+    given = torch.ones((), requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rms_norm_quant(torch.zeros(3, 64), scale=given)
+
+
 def bare_runner():
     from rl_quant_b200.runtime import InferenceRunner
     run = InferenceRunner.__new__(InferenceRunner)
