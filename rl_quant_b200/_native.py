@@ -10,6 +10,7 @@ import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_NAME = "libglad_b200.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
@@ -225,6 +226,14 @@ def require_cuda(*tensors: torch.Tensor) -> None:
         if t is not None and not t.is_cuda:
             raise RuntimeError("rl_quant_b200 kernels need CUDA tensors on an sm_100 device "
                                "(there is no CPU implementation)")
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """The kernels have no forward-mode derivative: a dual tensor is an error, not a zero derivative."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def conv_weights(w1p, b1f, qa, qc, w8, dq, b2f, a2, c2) -> GladConvWeights:

@@ -133,8 +133,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     """y in x's type, or ``(y, h)`` with a residual; h has the residual's type.
 
     x [..., C] float32, float16 or bfloat16, rows of any stride; weight [C] (None: ones) and residual
-    (x's shape) have x's type or float32; C up to 32768. Differentiable in x, weight and residual.
+    (x's shape) have x's type or float32; C up to 32768. Differentiable in x, weight and residual (backward mode).
     The sum is rounded to the residual's type first and the norm is of that value."""
+    N.refuse_tangents("rms_norm", x, weight, residual)
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
@@ -163,6 +164,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, residual
             raise ValueError("scale must be one float32 value on x's device")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual, scale)):
         raise RuntimeError("rms_norm_quant has no gradient; use rms_norm, or torch.no_grad()")
+    N.refuse_tangents("rms_norm_quant", x, weight, residual, scale)
     _check(x, weight, residual, eps)
     x2 = _rows(x)
     rows, cols = x2.shape

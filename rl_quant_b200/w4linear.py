@@ -98,6 +98,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: torch.Tensor | None = Non
     ``x_scale`` of one value, [..., 1] (one a row) or [..., ceil(K / group)] (one a row and group of the weight) and
     ``out_dtype`` named. out_dtype float16, bfloat16 or float32; bias [N] has it. Up to 2^20 rows, inputs (an even number)
     and outputs. Inference only."""
+    N.refuse_tangents("w4_linear", x, bias, x_scale)
     K, n, group = weight._shape
     shape, dt = x.shape, x.dtype
     if not shape or shape[-1] != K:

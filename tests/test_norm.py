@@ -550,6 +550,27 @@ def test_swapped_layer_with_default_eps(t):
     check_default_eps(model(x).detach(), src, x)
 
 
+def forward_mode(call, *inputs):
+    """``call`` with one input after another as a dual tensor, with gradients enabled and not, and once by torch.func."""
+    from torch.autograd import forward_ad
+    for i in range(len(inputs)):
+        for grad in (True, False):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                args = list(inputs)
+                args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                call(*args)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda a: call(a, *inputs[1:]), (inputs[0],), (torch.ones_like(inputs[0]),))
+
+
+def test_forward_mode_is_refused():
+    x, w, r = torch.ones(4, 64), torch.ones(64), torch.ones(4, 64)
+    forward_mode(lambda x, w, r: rms_norm(x, w, residual=r), x, w, r)
+    forward_mode(lambda x, w, r: rms_norm_quant(x, w, residual=r), x, w, r)
+    forward_mode(lambda s: rms_norm_quant(x, w, scale=s), torch.ones(()))
+    forward_mode(RMSNorm(64), x, r)
+
+
 # -- refusals (no GPU) -----------------------------------------------------------------------------
 
 

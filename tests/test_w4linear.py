@@ -547,6 +547,21 @@ def test_scales_refuse_a_gradient():
         rms_norm_quant(torch.zeros(3, 64), scale=given)
 
 
+def test_forward_mode_is_refused():
+    from test_norm import forward_mode
+    q, packed, s = weight(24, 128, 64, 1, "cpu")
+    w = pack_w4(packed, s, 64)
+    forward_mode(lambda x, b: w4_linear(x, w, b), torch.ones(3, 128, dtype=F16), torch.ones(24, dtype=F16))
+    forward_mode(lambda xs: w4_linear(torch.ones(3, 128, dtype=I8), w, x_scale=xs, out_dtype=F16), torch.ones(3, 1))
+    m, x = W4Linear(nn.Linear(64, 8).half()), torch.ones(3, 64, dtype=F16)
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+        m(forward_ad.make_dual(x, x))
+    with forward_ad.dual_level():             # with gradients enabled it is F.linear
+        y = m(forward_ad.make_dual(x, x))
+        assert torch.equal(forward_ad.unpack_dual(y).tangent, torch.nn.functional.linear(x, m.weight))
+
+
 def bare_runner():
     from rl_quant_b200.runtime import InferenceRunner
     run = InferenceRunner.__new__(InferenceRunner)
