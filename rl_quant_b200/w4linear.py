@@ -212,10 +212,33 @@ def w4_status(device=None) -> int:
     return 0
 
 
+def _top(x):
+    """float32 x without the lower 16 bits of its significand's 24: a bfloat16 number, x's sign, the rest exact in float32."""
+    return (x.view(torch.int32) & -65536).view(torch.float32)
+
+
+def _linear_f32(x, weight: W4Weight, bias, out_dtype):
+    """float32 rows as the sum of three bfloat16 rows of 8 bits each, which is exact (down to bfloat16's smallest numbers),
+    so x is not rounded: three times the rows in one ``w4_linear``, its float32 results added from the smallest up."""
+    hi = _top(x)
+    rest = torch.where(x == hi, 0.0, x - hi)            # 0 and not NaN behind an infinite part
+    mid = _top(rest)
+    parts = torch.stack((rest - mid, mid, hi)).bfloat16()
+    if 3 * (x.numel() // x.shape[-1]) <= 1 << 20:
+        lo, mid, hi = w4_linear(parts, weight, out_dtype=torch.float32)
+    else:
+        lo, mid, hi = (w4_linear(p, weight, out_dtype=torch.float32) for p in parts)
+    y = lo + mid + hi
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(out_dtype)
+
+
 class W4Linear(nn.Module):
     """``nn.Linear`` with 4-bit weights at inference and its own Parameters in training, like ``QuantLinear``:
     with gradients enabled the forward is ``F.linear`` on the source layer's weight and bias; without, ``w4_linear`` on
-    the laid-out copy, which ``requantize_`` rewrites in place (captured CUDA graphs stay valid).
+    the laid-out copy, which ``requantize_`` rewrites in place (captured CUDA graphs stay valid). Rows are float16, bfloat16 or
+    float32 (as three bfloat16 rows, not rounded).
     ``forward(q, x_scale)`` takes 8-bit rows, for inference only: refused while a gradient of its weight is asked for."""
 
     def __init__(self, linear: nn.Linear, group: int = 64):
@@ -259,6 +282,13 @@ class W4Linear(nn.Module):
                 return F.linear(x, self.weight, self.bias)
             if any(t is not None and t.requires_grad for t in (x, x_scale, self.weight, self.bias)):
                 raise RuntimeError("W4Linear on 8-bit rows has no gradient; use torch.no_grad()")
+        if x.dtype == torch.float32 and x_scale is None:
+            N.refuse_tangents("W4Linear", x, self.bias)
+            N.require_cuda(x)
+            if not x.dim() or x.shape[-1] != self.in_features:
+                raise ValueError(f"x {tuple(x.shape)} does not match in_features {self.in_features}")
+            with torch.no_grad():
+                return _linear_f32(x, self.w4(), self.bias, out_dtype or x.dtype)
         if out_dtype is None and x_scale is not None:
             out_dtype = self.weight.dtype
         bias = self.bias

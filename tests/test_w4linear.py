@@ -352,6 +352,93 @@ def test_block_serves_and_trains():
 
 
 @gpu
+@pytest.mark.parametrize("bias", [False, True])
+def test_float32_rows(bias):
+    """W4Linear serves what it trains on. x is split exactly, so the tolerance is that of the sums (module docstring): three
+    of them over parts whose magnitudes add up to less than 1.01 |x|, two additions and the bias; what a third part loses below
+    bfloat16's smallest number is 2^-134 of each input."""
+    torch.manual_seed(0)
+    for n, k, group in ((40, 64, 32), (777, 1002, 64), (130, 4096, 128)):
+        m = W4Linear(nn.Linear(k, n, bias=bias), group=group).cuda()
+        packed, s = quantize_w4(m.weight, group)
+        q = torch.stack((packed & 15, packed >> 4), -1).view(n, k).double()
+        W = (q - 16 * (q > 7)) * s.double()[:, torch.arange(k, device="cuda") // group]
+        b = m.bias.detach().double() if bias else torch.zeros(n, dtype=torch.float64, device="cuda")
+        for shape in ((1, k), (7, k), (3, 11, k), (300, k), (k,), (0, k)):
+            x = torch.randn(shape, device="cuda") * torch.logspace(-30, 30, k, device="cuda")[torch.randperm(k)].pow(
+                torch.rand((), device="cuda") < 0.5)
+            with torch.no_grad():
+                y = m(x)
+                assert y.dtype == torch.float32 and y.shape == shape[:-1] + (n,)
+                ref, S = x.double() @ W.T + b, x.double().abs() @ W.abs().T + b.abs()
+                tol = 1.01 * (k / 16 + 68) * 2.0 ** -23 * S + 2.0 ** -134 * W.abs().sum(1)
+                assert ((y.double() - ref).abs() <= tol).all()
+                y16 = m(x, out_dtype=F16)
+                assert y16.dtype == F16 and torch.equal(y16, y.half())
+        x = torch.randn(9, k, device="cuda")
+        with torch.no_grad():
+            clean = m(x)
+            x[1, 3], x[2, 5], x[3, 5] = float("nan"), float("inf"), -float("inf")
+            y = m(x)
+            assert torch.isnan(y[1]).all() and torch.equal(y[4:], clean[4:]) and torch.equal(y[0], clean[0])
+            nz = W[:, 5] != 0
+            for i, sign in ((2, 1.0), (3, -1.0)):
+                assert torch.equal(y[i][nz], sign * torch.sign(W[nz, 5]).float() * float("inf")) and torch.isnan(y[i][~nz]).all()
+            wide = torch.randn(5, 2 * k, device="cuda")
+            assert torch.equal(m(wide[:, ::2]), m(wide[:, ::2].contiguous()))
+            same = wide[:1, :k].expand(6, k)
+            assert torch.equal(m(same), m(same.contiguous()))
+            with pytest.raises(ValueError):
+                m(wide)
+
+
+@gpu
+def test_float32_rows_past_a_third_of_the_limit():
+    m = W4Linear(nn.Linear(64, 8)).cuda()
+    x = torch.randn(400000, 64, device="cuda")
+    with torch.no_grad():
+        y = m(x)
+        assert torch.equal(y[-1000:], m(x[-1000:])) and torch.equal(y[:1000], m(x[:1000]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("mode", ["eager", "manual-graph"])
+def test_runner_acts_through_w4_layers(dtype, mode):
+    """InferenceRunner over a policy with 4-bit layers: built, acted with, synchronised with its master and checked. The
+    reference is the same policy with the weights that the 4-bit copies stand for: four layers, each off by the tolerance of
+    its sums (fp16: and a rounding of 2^-11), of which 1e-3 (fp16: 2^-6) of the largest mean leaves a factor of ten for
+    cancellation."""
+    from rl_quant_b200 import InferenceRunner, build_glad
+    from rl_quant_b200.synthetic import glad_obs
+
+    def policy(seed):
+        torch.manual_seed(seed)
+        return build_glad().cuda().to(dtype).eval()
+
+    paths = ("actor.0", "actor.2", "actor.4")
+    model = policy(0)
+    swap.apply(model, {p: {"bits": 4, "group": 32} for p in paths})
+    with pytest.warns(UserWarning, match="op by op"):
+        run = InferenceRunner(model, mode=mode)
+    obs = glad_obs(33, seed=1).cuda().to(dtype)
+    for seed in (0, 1):
+        master = policy(seed)
+        run.sync_weights_from(master)
+        with torch.no_grad():
+            for p in paths:
+                lin = master.get_submodule(p)
+                packed, s = quantize_w4(lin.weight, 32)
+                q = torch.stack((packed & 15, packed >> 4), -1).view(lin.weight.shape).float()
+                lin.weight.copy_((q - 16 * (q > 7)) * s.float().repeat_interleave(32, 1)[:, :lin.in_features])
+            want = master.act_inference({"policy_obs": obs})[0].float()
+        got = run.act(obs)
+        assert got.dtype == dtype
+        assert (got.float() - want).abs().max() <= (1e-3 if dtype == torch.float32 else 2.0 ** -6) * want.abs().max()
+    run.check_status()
+
+
+@gpu
 def test_runner_refreshes_w4_layers():
     """InferenceRunner's weight hand-over reaches W4Linear layers (refresh_quant, eager and graphed)."""
     from rl_quant_b200 import InferenceRunner
