@@ -30,7 +30,7 @@ extern "C" {
 
 #define GLAD_DTYPE_F32 0
 #define GLAD_DTYPE_F16 1
-#define GLAD_DTYPE_BF16 2   /* rms_norm and w4_linear only */
+#define GLAD_DTYPE_BF16 2   /* rms_norm, w4_linear and cast-copy only */
 #define GLAD_DTYPE_I8 3     /* 8-bit activations: two's complement */
 #define GLAD_DTYPE_E4M3 4   /* 8-bit activations: 4 exponent, 3 mantissa bits, no infinities */
 
@@ -522,7 +522,7 @@ int glad_pack_weights(const GladPackItem* items, int n, void* blob, size_t blob_
 int glad_unpack_weights(const GladPackItem* items, int n, const void* blob, size_t blob_bytes, void* stream);
 
 /* The cast-copy half of sync_weights_from (qrt/runtime.py:251-253): n
- * element-wise copies with dtype conversion in one launch.                  */
+ * element-wise copies with dtype conversion (f32, f16, bf16) in one launch.  */
 typedef struct GladCastCopy {
   const void* src; void* dst; int64_t n; int32_t src_dtype; int32_t dst_dtype;
 } GladCastCopy;

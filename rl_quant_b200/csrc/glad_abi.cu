@@ -1025,8 +1025,8 @@ int glad_cast_copy(const GladCastCopy* items, int n, void* stream) {
   for (int i = 0; i < n; ++i) {
     const GladCastCopy& c = items[i];
     if ((!c.src || !c.dst) && c.n > 0) return fail(GLAD_ERR_INVALID_ARG, "item %d: NULL pointer", i);
-    if ((c.src_dtype != GLAD_DTYPE_F16 && c.src_dtype != GLAD_DTYPE_F32) ||
-        (c.dst_dtype != GLAD_DTYPE_F16 && c.dst_dtype != GLAD_DTYPE_F32))
+    if (c.src_dtype < GLAD_DTYPE_F32 || c.src_dtype > GLAD_DTYPE_BF16 || c.dst_dtype < GLAD_DTYPE_F32 ||
+        c.dst_dtype > GLAD_DTYPE_BF16)
       return fail(GLAD_ERR_INVALID_ARG, "item %d: unknown dtype", i);
   }
   GLAD_CHECK_CUDA(launch_cast_copy(items, n, (cudaStream_t)stream), "cast-copy launch");

@@ -4,6 +4,7 @@
 //
 // Reference: qrt/qlinear.py:84-138 (QuantLinear), qrt/qconv.py:247-284
 // (QuantCNN.requantize_), qrt/runtime.py:224-271 (sync_weights_from).
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include "glad_common.cuh"
@@ -451,12 +452,15 @@ __global__ void cast_copy_kernel(const __grid_constant__ CastTable t) {
   const GladCastCopy& c = t.it[blockIdx.y];
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < c.n;
        i += (int64_t)gridDim.x * blockDim.x) {
-    const float v = c.src_dtype == GLAD_DTYPE_F32 ? reinterpret_cast<const float*>(c.src)[i]
-                                                  : __half2float(reinterpret_cast<const __half*>(c.src)[i]);
+    const float v = c.src_dtype == GLAD_DTYPE_F32    ? reinterpret_cast<const float*>(c.src)[i]
+                    : c.src_dtype == GLAD_DTYPE_F16 ? __half2float(reinterpret_cast<const __half*>(c.src)[i])
+                                                    : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(c.src)[i]);
     if (c.dst_dtype == GLAD_DTYPE_F32)
       reinterpret_cast<float*>(c.dst)[i] = v;
-    else
+    else if (c.dst_dtype == GLAD_DTYPE_F16)
       reinterpret_cast<__half*>(c.dst)[i] = __float2half_rn(v);
+    else
+      reinterpret_cast<__nv_bfloat16*>(c.dst)[i] = __float2bfloat16_rn(v);
   }
 }
 

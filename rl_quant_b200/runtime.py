@@ -35,6 +35,8 @@ def _dt(t: torch.Tensor) -> int:
         return N.DTYPE_F16
     if t.dtype == torch.float32:
         return N.DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return N.DTYPE_BF16
     raise TypeError(f"unsupported dtype {t.dtype}")
 
 

@@ -439,6 +439,41 @@ def test_runner_acts_through_w4_layers(dtype, mode):
 
 
 @gpu
+@pytest.mark.parametrize("src_t", [torch.float32, F16, BF16])
+@pytest.mark.parametrize("dst_t", [torch.float32, F16, BF16])
+def test_runner_syncs_every_type(src_t, dst_t):
+    """sync_weights_from between a master and a copy of any two of the types that the layers take: each value is the master's,
+    rounded once; 4-bit copies are those of the new weights. Odd and empty sizes, infinities and NaN among them."""
+    from rl_quant_b200 import InferenceRunner
+
+    def model(t):
+        m = nn.Sequential(nn.RMSNorm(64, eps=1e-6), nn.Linear(64, 33), nn.ELU(), nn.Linear(33, 7)).cuda().to(t)
+        m.register_buffer("extra", torch.zeros(5, device="cuda").to(t))
+        m.register_buffer("none", torch.zeros(0, device="cuda").to(t))
+        return m
+
+    src, dst = model(src_t), model(dst_t)
+    swap.apply(dst, {"1": {"bits": 4, "group": 32}})
+    swap.apply_norm(dst)
+    src.extra.copy_(torch.tensor([float("inf"), -float("inf"), float("nan"), 6e4, 2.0 ** -20]))
+    run = InferenceRunner.__new__(InferenceRunner)
+    run.model, run._g_sync, run._sync_items = dst, None, None
+    run._quant_layers = [m for m in dst.modules() if m is not dst and hasattr(m, "requantize_")]
+    for graph in (False, True, True):
+        with torch.no_grad():
+            for p in src.parameters():
+                p.normal_()
+        run.sync_weights_from(src, use_graph=graph)
+        want = dict(src.named_parameters()) | dict(src.named_buffers())
+        have = dict(dst.named_parameters()) | dict(dst.named_buffers())
+        for name, t in want.items():
+            assert have[name].dtype == dst_t
+            assert torch.equal(have[name].detach().nan_to_num(1.5, 1e3, -1e3), t.detach().to(dst_t).nan_to_num(1.5, 1e3, -1e3)), name
+        w = pack_w4(*quantize_w4(dst[1].weight, 32), 32)
+        assert torch.equal(dst[1].tiles, w.tiles) and torch.equal(dst[1].scales, w.scales)
+
+
+@gpu
 def test_runner_refreshes_w4_layers():
     """InferenceRunner's weight hand-over reaches W4Linear layers (refresh_quant, eager and graphed)."""
     from rl_quant_b200 import InferenceRunner
@@ -647,6 +682,13 @@ def test_forward_mode_is_refused():
     with forward_ad.dual_level():             # with gradients enabled it is F.linear
         y = m(forward_ad.make_dual(x, x))
         assert torch.equal(forward_ad.unpack_dual(y).tangent, torch.nn.functional.linear(x, m.weight))
+
+
+def test_cast_copy_refuses_other_types():
+    lib = N.load()
+    a = np.zeros(64, np.float32).ctypes.data
+    for src, dst in ((N.DTYPE_I8, 0), (0, N.DTYPE_E4M3), (-1, 0), (0, 9)):
+        assert lib.glad_cast_copy(N.GladCastCopy(a, a, 0, src, dst), 1, None) == N.GLAD_ERR_INVALID_ARG
 
 
 def bare_runner():
