@@ -42,28 +42,28 @@ def _quantised(path: str, lin: nn.Linear, cfg: dict) -> nn.Module:
 def apply(model: nn.Module, plan: dict[str, dict]) -> dict[str, nn.Module]:
     """Swap every ``plan`` path to a QuantLinear, or to a W4Linear where the entry says ``"bits": 4``.
     ``plan = {path: {"s_z": float|None, "alpha": Tensor|None, "beta": Tensor|None, "act_mode": str}}`` or
-    ``{path: {"bits": 4, "group": 32|64|128}}``."""
+    ``{path: {"bits": 4, "group": 32|64|128}}``. All or none: the model stays as it was where a layer is refused."""
     swapped: dict[str, nn.Module] = {}
     for path, cfg in plan.items():
         lin = get_module(model, path)
         assert isinstance(lin, nn.Linear), f"{path} is not an nn.Linear: {type(lin)}"
-        q = _quantised(path, lin, cfg)
-        q.train(lin.training)
+        swapped[path] = _quantised(path, lin, cfg).train(lin.training)
+    for path, q in swapped.items():
         set_module(model, path, q)
-        swapped[path] = q
     return swapped
 
 
 def apply_norm(model: nn.Module, paths: list[str] | None = None) -> dict[str, nn.RMSNorm]:
-    """Swap the named ``nn.RMSNorm`` layers (None: every one) to ``RMSNorm``; returns the originals by path."""
+    """Swap the named ``nn.RMSNorm`` layers (None: every one) to ``RMSNorm``; returns the originals by path. All or none."""
     if paths is None:
         paths = [n for n, m in model.named_modules() if type(m) is nn.RMSNorm and n]
-    originals = {}
+    originals, swapped = {}, {}
     for path in paths:
         norm = get_module(model, path)
         assert isinstance(norm, nn.RMSNorm), f"{path} is not an nn.RMSNorm: {type(norm)}"
-        set_module(model, path, RMSNorm.from_torch(norm))
-        originals[path] = norm
+        originals[path], swapped[path] = norm, RMSNorm.from_torch(norm)
+    for path, norm in swapped.items():
+        set_module(model, path, norm)
     return originals
 
 

@@ -691,6 +691,25 @@ def test_cast_copy_refuses_other_types():
         assert lib.glad_cast_copy(N.GladCastCopy(a, a, 0, src, dst), 1, None) == N.GLAD_ERR_INVALID_ARG
 
 
+def test_a_refused_layer_leaves_the_model_as_it_was():
+    """A refusal in the middle of a plan: nothing of it is applied, so nothing has to be put back."""
+    m = nn.Sequential(nn.RMSNorm(64, eps=1e-6), nn.Linear(64, 7), nn.Linear(7, 5), nn.RMSNorm((1, 5), eps=1e-6),
+                      nn.RMSNorm(5, elementwise_affine=False))
+    before = list(m)
+    for plan, error in (({"1": {"bits": 4}, "2": {"bits": 4}}, ValueError), ({"1": {"bits": 4}, "2": {"bits": 5}}, ValueError),
+                        ({"1": {"bits": 4}, "0": {"bits": 4}}, AssertionError), ({"1": {"bits": 4}, "9": {"bits": 4}}, AttributeError)):
+        with pytest.raises(error):
+            swap.apply(m, plan)
+        assert all(a is b for a, b in zip(m, before))
+    for paths in (None, ["0", "3"], ["0", "4"]):
+        with pytest.raises(ValueError):
+            swap.apply_norm(m, paths)
+        assert all(a is b for a, b in zip(m, before))
+    with pytest.raises(AssertionError):
+        swap.apply_norm(m, ["0", "1"])
+    assert all(a is b for a, b in zip(m, before))
+
+
 def bare_runner():
     from rl_quant_b200.runtime import InferenceRunner
     run = InferenceRunner.__new__(InferenceRunner)
