@@ -141,8 +141,7 @@ __device__ __forceinline__ void store_v(T* p, float (&f)[VEC]) {
         f[2 * i] = u.x, f[2 * i + 1] = u.y;
       }
     }
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 // Weight elements [col, col + VEC): the input's type or fp32; ones without a weight.
@@ -288,8 +287,7 @@ __device__ __forceinline__ void store_q(uint8_t* p, const float (&t)[VEC]) {
                                 : (code_i8(t[i]) | (code_i8(t[i + 1]) << 8));
       w[i >> 2] |= two << (8 * (i & 3));
     }
-    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(p) = w[0];
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   }
 }
 
