@@ -395,7 +395,7 @@ def test_quant_given_scale_of_any_size(out):
 
 @gpu
 @pytest.mark.parametrize("out", [torch.int8, torch.float8_e4m3fn])
-@pytest.mark.parametrize("shape", [(64, 512), (3, 4096), (40, 333), (2, 20000), (2, 20001)])
+@pytest.mark.parametrize("shape", [(64, 512), (3, 4096), (40, 333), (2, 20000), (2, 20001), (9000, 288), (2500, 1001)])
 def test_quant_rows_of_every_size(shape, out):
     """Rows and groups whose maximum leaves the range of fast quotients stand beside ordinary ones, zeros and NaN: each has its
     own scale and codes."""
@@ -414,7 +414,15 @@ def test_quant_rows_of_every_size(shape, out):
         ref32 = ref.float()                                # what underflows to 0 has the scale 1
         ref = torch.where(ref32 == 0, torch.ones_like(ref), ref)
         nan = torch.isnan(ref)
-        for r in range(R):
+        same = lambda a, b: torch.equal(a.float().nan_to_num(1e3), b.float().nan_to_num(1e3))  # noqa: E731
+        assert same(q, q[:1].expand_as(q)) and same(s, s[:1].expand_as(s))
+        wide = torch.ones(R, C + 3, device="cuda", dtype=torch.float16)[:, 3:]     # rows off every word, other types
+        for x2, r2 in ((x, torch.zeros_like(x)), (wide, torch.zeros_like(x)), (wide, wide * 0)):
+            q2, s2, _ = rms_norm_quant(x2, w.cuda(), residual=r2, eps=0.0, out_dtype=out, group=group)
+            assert same(q2[0], q2[R - 1]) and same(s2, s2[:1].expand_as(s2))
+            assert (s2[0] - s[0]).abs().nan_to_num(0.0).le(4 * F32 * s[0].nan_to_num(1.0) + 2.0 ** -148).all()
+            assert torch.equal(torch.isnan(s2[0]), torch.isnan(s[0]))
+        for r in {0, R - 1}:
             got = s[r].cpu().double()
             assert torch.equal(torch.isnan(got), nan)
             # the norm of ones is 1 to within F32; near the smallest number a rounding is half of 2^-149
