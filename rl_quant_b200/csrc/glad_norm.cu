@@ -27,7 +27,9 @@ int set_last_error(int code, const char* msg);
 namespace {
 
 constexpr int kNormMaxCols = 32768;      // a row lives in the registers of one block
-constexpr int kNormMaxPartials = 592;    // dw partial rows of the backward pass (4 per SM)
+// dw partial rows of the backward pass: rows in work at once, in teams of threads. Four blocks an SM where a block is one
+// team (more than 2048 columns); narrow rows go up to eight teams a block, and the grid is as much smaller.
+constexpr int kNormMaxPartials = 592;
 
 struct NormParams {
   const void* x;        // forward: input rows; backward: dy
@@ -354,7 +356,7 @@ __device__ __noinline__ void quant_slow(const NormParams& p, uint32_t slow, floa
 // ---- forward ------------------------------------------------------------------------------
 // One team of threads per row, up to VEC * NV elements a thread. QUANT: 0 none, 1 int8, 2 e4m3.
 // 8192 x 4096, bf16 with an fp32 residual: 403 MB in 63 us, 6.4 TB/s, what a plain copy reaches here. 8192 x 8192 bf16 to
-// e4m3 with groups of 128: 472 MB in 91.6 us, 5.2 TB/s; there the instruction issue is busy for about 70% of the time (a
+// e4m3 with groups of 128: 472 MB in 91.6 us, 5.2 TB/s; there the instruction issue is busy for 77% of the time (a
 // maximum, a scale, a quotient and a conversion an element on top; with a product by the reciprocal in place of the quotient
 // 87.4 us, but other codes on borders). 1 x 2048 f16: 1.6 us, a launch.
 // A persistent block that fetches its next row ahead gained nothing: with one row a block the
@@ -526,7 +528,9 @@ __global__ void __launch_bounds__(MAXT, kFwdBlocks<TH, VEC, QUANT, MAXT>) norm_f
 // registers and is written once as a partial row, which norm_dw_kernel sums in a fixed order.
 // 8192 x 4096, bf16 with an fp32 sum, gradients of both and of the weight: 537 MB in 98 us, 5.5 TB/s, 86% of a copy's
 // rate: 64 registers a thread for the row, its gradient and dw's share leave 32 warps an SM to hide the row's one
-// barrier. A ring of asynchronous copies ahead of the row and three blocks an SM (40 registers, spills) were slower.
+// barrier, and are not quite enough: this instance spills 29 words a thread. A ring of asynchronous copies ahead of the row
+// and three blocks an SM (40 registers, more spills) were slower. Not timed: rows of more than 16384 columns (32 elements a
+// thread, since a block could not hold the row otherwise: 150 to 900 words spilled) and many rows of few columns.
 template <typename TX, typename TH, int VEC, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) norm_bwd_kernel(const __grid_constant__ NormParams p) {
   __shared__ float red[2][32];                           // rows use them in turn: one barrier a row

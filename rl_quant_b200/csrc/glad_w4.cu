@@ -190,12 +190,14 @@ __device__ __forceinline__ void store_y4(const W4Params& p, int64_t m, int n, co
 // One persistent block per SM. Its warps form streams of W warps; each stream walks tiles of 32 columns,
 // its warps split the inputs in units of 128 and join their sums in warp order once a tile. Each warp
 // brings its own units (2 KB of weights and 128/GROUP * 64 bytes of scales) through a private
-// shared-memory ring of cp.async copies kRing - 1 units ahead, across tile borders, so about 64 KB
-// are in flight on an SM whatever the warps wait for. x is staged once in shared memory, in the form
+// shared-memory ring of cp.async copies kRing - 1 units ahead, across tile borders, so about
+// 70 KB are in flight on an SM with rings of three units (up to 8 rows, where x fits beside them) and half of that with two. x is staged once in shared memory, in the form
 // the products take (e4m3 as fp16; int8 with the middle two of four inputs swapped, the order in which
 // a word's nibbles come apart). Rows past M read row M - 1: their sums are never stored.
-// Issue slots bound it: a 32-bit word takes 9 instructions to unpack and one to multiply, so a unit is as
-// large as registers allow, which spreads the rest (copies, x, scales, addresses) over more words.
+// A 32-bit word takes 9 instructions to unpack and one to multiply, so a unit is as
+// large as registers allow, which spreads the rest (copies, x, scales, addresses) over more words. Instruction issue is the
+// busiest part that a profile shows (59% of the slots at 1 x 28672 x 8192, 43% at 16 x 14336 x 4096 int8; HBM 45% and 22%), but
+// not full: 16 warps an SM do not cover the waits between a unit's loads, products and scales.
 // 1 x 28672 x 8192 bf16, groups of 128: 121 MB in 29.7 us, 4.1 TB/s, 64% of a copy's rate (f16, one operation less a
 // pair: 8 rows 31.5 us; int8, whose words take 4 to unpack: 8 rows 25.8 us, 4.7 TB/s). 1 x 4096 x 4096 f16, groups of
 // 64: 8.9 MB in 3.9 us, of which 1.6 us are a launch. 16 columns a step: 30.4 and 4.4 us; registers instead
