@@ -284,6 +284,8 @@ class W4Linear(nn.Module):
                 raise RuntimeError("W4Linear on 8-bit rows has no gradient; use torch.no_grad()")
         if x.dtype == torch.float32 and x_scale is None:
             N.refuse_tangents("W4Linear", x, self.bias)
+            if out_dtype is not None and out_dtype not in _OUT:
+                raise TypeError(f"out_dtype is {out_dtype}; expected float16, bfloat16 or float32")
             N.require_cuda(x)
             if not x.dim() or x.shape[-1] != self.in_features:
                 raise ValueError(f"x {tuple(x.shape)} does not match in_features {self.in_features}")

@@ -655,6 +655,19 @@ def test_8_bit_rows_refuse_a_gradient():
         W4Linear(nn.Linear(64, 8))(q, x_scale=one)
 
 
+def test_rows_of_every_type_refuse_other_outputs():
+    m = W4Linear(nn.Linear(64, 8))
+    with torch.no_grad():
+        for x in (torch.zeros(3, 64), torch.zeros(3, 64, dtype=F16)):
+            for out in (torch.float64, torch.int8):
+                with pytest.raises(TypeError):
+                    m(x, out_dtype=out)
+        with pytest.raises(TypeError):
+            m(torch.zeros(3, 64, dtype=torch.float64))
+        with pytest.raises(RuntimeError, match="CUDA"):
+            m(torch.zeros(3, 64))
+
+
 def test_scales_refuse_a_gradient():
     q, packed, s = weight(24, 128, 64, 1, "cpu")
     w, x = pack_w4(packed, s, 64), torch.zeros(3, 128, dtype=I8)
