@@ -285,11 +285,11 @@ def run(s):
         return outs + ([got.top_log_prob, got.top_index] if case["top"] else [])
     if not own:
         return _plain_clip(s)
-    from rl_quant_b200.gradnorm import clip_grad_norm_, clip_grads
+    from rl_quant_b200.gradnorm import clip_grads, clip_grads_
 
     kind = float(case["norm"])
     if s["out"] is None:            # in place; below the limit, so the gradients stay as they are
-        return [clip_grad_norm_(s["grads"], s["max_norm"], norm_type=kind), s["flat"]]
+        return [clip_grads_(s["grads"], s["max_norm"], norm_type=kind), s["flat"]]
     _, norm = clip_grads(s["grads"], s["max_norm"], norm_type=kind, out=s["out"])
     return [norm, s["out_flat"]]
 
