@@ -30,7 +30,7 @@ extern "C" {
 
 #define GLAD_DTYPE_F32 0
 #define GLAD_DTYPE_F16 1
-#define GLAD_DTYPE_BF16 2   /* rms_norm, w4_linear and cast-copy only */
+#define GLAD_DTYPE_BF16 2   /* not in the GLAD forwards */
 #define GLAD_DTYPE_I8 3     /* 8-bit activations: two's complement */
 #define GLAD_DTYPE_E4M3 4   /* 8-bit activations: 4 exponent, 3 mantissa bits, no infinities */
 
@@ -463,6 +463,43 @@ int glad_w4_linear_status(uint32_t* status, void* stream);
  * other blocks), and a wait gives up after `limit_ns` nanoseconds (at most, and 0 for, the
  * normal 2 s). (0, 0) restores normal operation. Process-wide.                */
 int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
+
+/* ---- log probabilities of given tokens (no counterpart in the reference) -------
+ * Rows of logits x [rows, cols] (f32, f16 or bf16, row stride ldx >= cols elements), a token
+ * (i32 or i64, token_bytes 4 or 8) a row, z = (x - max x) / temperature:
+ *   log_prob [rows] = z_token - ln sum e^z
+ *   entropy [rows]  = -sum p ln p, p = e^z / sum e^z               (NULL: not wanted)
+ *   top_index, top_log_prob [rows, top]: the `top` (0..32, at most cols) largest logits'
+ *     columns and log probabilities, largest first, the lower column first among equals
+ *   stats [rows, 2]: what the backward pass reads                   (NULL: not wanted)
+ * Logits of -inf have probability 0 and add nothing to the entropy; a row of nothing else has log probability
+ * -inf, entropy 0 and no gradient. A row whose token is ignore_index is not read: its
+ * outputs are 0 (top_index -1), its gradient 0. Any other token outside [0, cols) gives NaN,
+ * as does a NaN or +inf in the row. All f32 but top_index (i64).               */
+int glad_token_log_probs(const void* logits, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, const void* tokens,
+                         int token_bytes, int64_t ignore_index, float temperature, int top, float* log_prob,
+                         float* entropy, float* top_log_prob, int64_t* top_index, float* stats, void* stream);
+
+/* Its backward pass: d_logits [rows, cols] (x's type, contiguous) from the gradients of the
+ * three outputs (each NULL: none; d_entropy needs entropy, d_top needs top_index). */
+int glad_token_log_probs_backward(const void* logits, int x_dtype, int64_t ldx, int64_t rows, int64_t cols,
+                                  const void* tokens, int token_bytes, int64_t ignore_index, float temperature, int top,
+                                  const float* stats, const float* entropy, const int64_t* top_index, const float* d_log_prob,
+                                  const float* d_entropy, const float* d_top, void* d_logits, void* stream);
+
+/* ---- global norm over many tensors, and clipping by it -------------------------
+ * norm (device f32 [1]) of all elements of n tensors (f32, f16 or bf16 each: dtypes[i], sizes[i]
+ * elements one after the other): norm_type 2: square root of the sum of squares, 1: sum of the magnitudes,
+ * 0: largest magnitude. glad_clip_grads also writes outs[i] = c * grads[i] in the same
+ * type, c = min(1, max_norm / (norm + 1e-6)) as torch.nn.utils.clip_grad_norm_; outs[i] may
+ * be grads[i] (left alone where c is 1) and must overlap with no other tensor. Sums do not
+ * overflow or lose small gradients, and have a fixed order: the same call gives the same bits.
+ * The tables are host memory, read before the call returns.                    */
+size_t glad_grad_norm_workspace_size(int n);
+int glad_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int n, int norm_type,
+                   float* norm, void* workspace, size_t workspace_bytes, void* stream);
+int glad_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes, int n,
+                    int norm_type, float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- weight refresh (qrt/runtime.py:195-271) ------------------------------- */
 

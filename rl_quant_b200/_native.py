@@ -164,6 +164,15 @@ SIGNATURES = {
                                        c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "glad_w4_linear_status": (c_int, [POINTER(c_uint32), c_void_p]),
     "glad_debug_w4_wait": (c_int, [c_uint32, c_uint64]),
+    "glad_token_log_probs": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_float, c_int,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "glad_token_log_probs_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_float,
+                                              c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                              c_void_p]),
+    "glad_grad_norm_workspace_size": (c_size_t, [c_int]),
+    "glad_grad_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "glad_clip_grads": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_size_t,
+                                c_void_p]),
     "glad_requant_qlinear": (c_int, [POINTER(GladQLinearSrc), c_int, c_void_p]),
     "glad_requant_qcnn": (c_int, [POINTER(GladQCNNSrc), c_void_p]),
     "glad_cast_copy": (c_int, [POINTER(GladCastCopy), c_int, c_void_p]),
