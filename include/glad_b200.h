@@ -464,6 +464,31 @@ int glad_w4_linear_status(uint32_t* status, void* stream);
  * normal 2 s). (0, 0) restores normal operation. Process-wide.                */
 int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
 
+/* ---- low-rank adapters of many requests (no counterpart in the reference) ------
+ * Rows x [M, K] (f32, f16 or bf16, row stride ldx >= K elements); adapter i of L has a [r, K] and b [N, r]
+ * of x's type, one after the other, and a factor scale[i] (device f32, NULL: scale_value):
+ *   u[m] = scale[i] * a[i] x[m],   y[m] = base[m] + b[i] u[m],   i = index[m]
+ * index (i32 or i64, index_bytes 4 or 8; NULL: adapter 0 for all, L = 1) outside [0, L): no adapter, y = base.
+ * base [M, N] (row stride ldb, NULL: zeros) and y (contiguous) have x's type; u [M, r] f32 or NULL is what the
+ * backward pass reads. r 1..128, L up to 16384, M, K and N up to 2^24. u and the sums are f32, y is rounded once.
+ * Infinite inputs give infinite or NaN outputs in their rows.
+ * More than 256 rows with an index, and every backward pass with one, need glad_lora_plan's order of the rows: a plan
+ * of glad_lora_plan_size(M, L) bytes for this M, L, r and index.                  */
+size_t glad_lora_plan_size(int64_t M, int L);
+int glad_lora_plan(const void* index, int index_bytes, int64_t M, int L, int r, void* plan, size_t plan_bytes, void* stream);
+int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const void* a, const void* b, int64_t N,
+                      int L, int r, const void* index, int index_bytes, const void* plan, const float* scale, float scale_value,
+                      const void* base, int64_t ldb, void* y, float* u, void* stream);
+
+/* Its backward pass: du[m] = scale[i] * b[i]^T dy[m], dx[m] = a[i]^T du[m] (contiguous),
+ * da[i] = sum over i's rows of du[m] x[m]^T, db[i] = the same of dy[m] u[m]^T; the gradient of base is dy. dx, da, db of x's type,
+ * each NULL: not wanted; da needs x and du (f32 [M, r] of workspace), db needs u. Sums have a fixed
+ * order: the same call gives the same bits. Adapters without rows get zeros.    */
+int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, int64_t M, int64_t K, const void* a,
+                       const void* b, int64_t N, int L, int r, const void* index, int index_bytes, const void* plan,
+                       const float* scale, float scale_value, const float* u, float* du, void* dx, void* da, void* db,
+                       void* stream);
+
 /* ---- log probabilities of given tokens (no counterpart in the reference) -------
  * Rows of logits x [rows, cols] (f32, f16 or bf16, row stride ldx >= cols elements), a token
  * (i32 or i64, token_bytes 4 or 8) a row, z = (x - max x) / temperature:

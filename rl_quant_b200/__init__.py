@@ -12,6 +12,7 @@ The public API mirrors qrt (qrt/__init__.py:18-34):
 Beside them, for the blocks around quantised layers (no qrt counterpart):
     rms_norm, rms_norm_quant, RMSNorm     add + RMS norm, 16/32-bit (trains) or 8-bit output
     w4_linear, W4Linear, W4Weight, pack_w4, unpack_w4, w4_status   4-bit linear of any shape
+    lora_linear, LoRALinear               low-rank adapters of many requests beside a shared linear (train)
     token_log_probs                       log probabilities, entropy, top alternatives of logits (trains)
     grad_norm, clip_grads, clip_grads_, clip_grad_norm_   global norm over many tensors, and clipping
 
@@ -35,13 +36,14 @@ _EXPORTS = {
     "rms_norm": "norm", "rms_norm_quant": "norm", "RMSNorm": "norm",
     "w4_linear": "w4linear", "W4Linear": "w4linear", "W4Weight": "w4linear", "pack_w4": "w4linear",
     "unpack_w4": "w4linear", "w4_status": "w4linear",
+    "lora_linear": "lora", "LoRALinear": "lora",
     "token_log_probs": "logprob", "TokenLogProbs": "logprob",
     "grad_norm": "gradnorm", "clip_grads": "gradnorm", "clip_grads_": "gradnorm", "clip_grad_norm_": "gradnorm",
     "GladActorCritic": "glad_model", "build_glad": "glad_model",
 }
 _SUBMODULES = ("swap", "calib", "_native", "synthetic", "glad_model", "qconv", "qlinear", "encoder_opt",
                "runtime", "integration", "let", "fused", "build", "norm", "w4linear", "w4a16",
-               "logprob", "gradnorm")
+               "lora", "logprob", "gradnorm")
 
 __all__ = sorted(_EXPORTS) + ["swap", "calib"]
 

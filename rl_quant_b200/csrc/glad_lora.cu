@@ -1,0 +1,229 @@
+// C entries of the low-rank adapters (glad_lora.cuh), and the order of rows by adapter that larger calls need.
+#include "glad_lora.cuh"
+
+namespace glad {
+namespace lora {
+
+extern template cudaError_t run<__half>(Params, bool, cudaStream_t);
+extern template cudaError_t run<__nv_bfloat16>(Params, bool, cudaStream_t);
+extern template cudaError_t run<float>(Params, bool, cudaStream_t);
+extern template cudaError_t run_outer<__half>(OuterParams, cudaStream_t);
+extern template cudaError_t run_outer<__nv_bfloat16>(OuterParams, cudaStream_t);
+extern template cudaError_t run_outer<float>(OuterParams, cudaStream_t);
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+struct PlanParams {
+  const void* index;
+  int32_t* plan;
+  int M, L, index64, warps, tile_rows;
+};
+
+// A stable counting sort by one block: the first `warps` warps count the adapters of a run of rows each, the counts are added up by
+// adapter, then by warp, and the warps place their rows. Rows of an adapter stay in order, so sums over them repeat.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
+  extern __shared__ int32_t sh[];
+  const int G = p.L + 1;                                // groups: adapters, then the rows without one
+  int32_t* cnt = sh;                                    // [warps][G]
+  int32_t* tile0 = sh + p.warps * G;                    // [G + 1]
+  __shared__ int32_t sums[2][kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < p.warps * G; i += kPlanThreads) cnt[i] = 0;
+  grid_dep_wait();
+  __syncthreads();
+  const int run = ((p.M + p.warps - 1) / p.warps + 31) / 32 * 32;
+  const int64_t lo = (int64_t)warp * run;
+  const int64_t hi = lo + run < p.M ? lo + run : p.M;
+  auto group_of = [&](int64_t m) -> int {
+    const int64_t a = p.index64 ? static_cast<const int64_t*>(p.index)[m] : (int64_t)static_cast<const int32_t*>(p.index)[m];
+    return a >= 0 && a < p.L ? (int)a : p.L;
+  };
+  if (warp < p.warps) {
+    for (int64_t m0 = lo; m0 < hi; m0 += 32) {
+      const int a = m0 + lane < hi ? group_of(m0 + lane) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, a);
+      if (a >= 0 && lane == __ffs(same) - 1) cnt[warp * G + a] += __popc(same);
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  int row_carry = 0, tile_carry = 0;
+  for (int a0 = 0; a0 < G; a0 += kPlanThreads) {        // exclusive sums over the groups, of rows and of tiles
+    const int a = a0 + tid;
+    int rows = 0;
+    if (a < G)
+      for (int w = 0; w < p.warps; ++w) rows += cnt[w * G + a];
+    const int tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    int r = rows, t = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int ur = __shfl_up_sync(0xffffffffu, r, o), ut = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) r += ur, t += ut;
+    }
+    if (lane == 31) sums[0][warp] = r, sums[1][warp] = t;
+    __syncthreads();
+    int before_r = row_carry, before_t = tile_carry;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) before_r += sums[0][w], before_t += sums[1][w];
+      row_carry += sums[0][w];
+      tile_carry += sums[1][w];
+    }
+    if (a < G) {
+      int at = before_r + r - rows;
+      p.plan[1 + a] = at;
+      tile0[a] = before_t + t - tiles;
+      for (int w = 0; w < p.warps; ++w) {
+        const int c = cnt[w * G + a];
+        cnt[w * G + a] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0) p.plan[0] = tile_carry, p.plan[1 + G] = p.M, tile0[G] = tile_carry;
+  __syncthreads();
+  int32_t* order = p.plan + 3 + p.L;
+  if (warp < p.warps) {
+    for (int64_t m0 = lo; m0 < hi; m0 += 32) {
+      const int a = m0 + lane < hi ? group_of(m0 + lane) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, a);
+      if (a >= 0) order[cnt[warp * G + a] + __popc(same & ((1u << lane) - 1))] = (int32_t)(m0 + lane);
+      __syncwarp();
+      if (a >= 0 && lane == __ffs(same) - 1) cnt[warp * G + a] += __popc(same);
+      __syncwarp();
+    }
+  }
+  int32_t* tiles = order + p.M;
+  for (int t = tid; t < tile_carry; t += kPlanThreads) {
+    int a = 0, b = G;                                   // the last group whose first tile is at or before t
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (tile0[mid] <= t) a = mid;
+      else b = mid;
+    }
+    tiles[2 * t] = a == p.L ? -1 : a;
+    tiles[2 * t + 1] = p.plan[1 + a] + (t - tile0[a]) * p.tile_rows;
+  }
+}
+
+template <typename F>
+cudaError_t for_type(int dtype, F&& f) {
+  if (dtype == GLAD_DTYPE_F16) return f(__half());
+  if (dtype == GLAD_DTYPE_BF16) return f(__nv_bfloat16());
+  return f(float());
+}
+
+const char* shape_wrong(int dtype, int64_t M, int64_t K, int64_t N, int L, int r, const void* index, int index_bytes) {
+  if (!is_float(dtype)) return "x must be f32, f16 or bf16";
+  if (M < 0 || M > 1 << 24) return "rows must be in [0, 2^24]";
+  if (K < 1 || K > 1 << 24 || N < 1 || N > 1 << 24) return "inputs and outputs must be in [1, 2^24]";
+  if (L < 1 || L > kMaxAdapters) return "the number of adapters must be in [1, 16384]";
+  if (r < 1 || r > kMaxRank) return "the rank must be in [1, 128]";
+  if (!index && L != 1 && M > 0) return "several adapters need an index";
+  if (index && index_bytes != 4 && index_bytes != 8) return "the index must have 4 or 8 bytes";
+  if (!on(index, index_bytes ? index_bytes : 4)) return "the index is not element-aligned";
+  return nullptr;
+}
+
+int64_t plan_words(int64_t M, int L) { return 3 + L + M + 2 * max_tiles(M, L, kMaxRank, true, true); }
+
+}  // namespace
+}  // namespace lora
+}  // namespace glad
+
+using namespace glad;
+using namespace glad::lora;
+
+extern "C" {
+
+size_t glad_lora_plan_size(int64_t M, int L) {
+  if (M < 0 || M > 1 << 24 || L < 1 || L > kMaxAdapters) return 0;
+  return (size_t)plan_words(M, L) * 4;
+}
+
+int glad_lora_plan(const void* index, int index_bytes, int64_t M, int L, int r, void* plan, size_t plan_bytes, void* stream) {
+  const char* who = "glad_lora_plan";
+  const char* why = shape_wrong(GLAD_DTYPE_F32, M, 1, 1, L, r, index, index_bytes);
+  if (why) return bad(who, why);
+  if (M == 0) return GLAD_OK;
+  if (!index) return bad(who, "index must be set");
+  if (!plan || plan_bytes < glad_lora_plan_size(M, L) || !on(plan, 16))
+    return set_last_error(GLAD_ERR_WORKSPACE, "glad_lora_plan: a plan of glad_lora_plan_size bytes is required");
+  const int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
+  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true)};
+  const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
+  cudaError_t e = cudaSuccess;
+  if (smem > 40 * 1024) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = launch_k(plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, true, p);
+  return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
+}
+
+int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const void* a, const void* b, int64_t N,
+                      int L, int r, const void* index, int index_bytes, const void* plan, const float* scale, float scale_value,
+                      const void* base, int64_t ldb, void* y, float* u, void* stream) {
+  const char* who = "glad_lora_forward";
+  const char* why = shape_wrong(dtype, M, K, N, L, r, index, index_bytes);
+  if (why) return bad(who, why);
+  if (M == 0) return GLAD_OK;
+  if (!x || !a || !b || !y) return bad(who, "x, a, b and y must be set");
+  if ((why = rows_wrong(x, dtype, ldx, M, (int)K))) return bad(who, why);
+  if (base && (why = rows_wrong(base, dtype, ldb, M, (int)N))) return bad(who, why);
+  if (!on(a, width_of(dtype)) || !on(b, width_of(dtype)) || !on(y, width_of(dtype)) || !on(u, 4) || !on(scale, 4) ||
+      !on(plan, 16))
+    return bad(who, "a tensor is not element-aligned");
+  if (index && !plan && M > kSelfRows) return bad(who, "more than 256 rows with an index need a plan");
+  Params p{};
+  p.x = x, p.ldx = ldx, p.M = (int)M, p.K = (int)K, p.N = (int)N, p.w1 = a, p.w2 = b, p.L = L, p.r = r;
+  p.index = index, p.index64 = index_bytes == 8, p.plan = static_cast<const int32_t*>(plan);
+  p.scale = scale, p.scale_value = scale_value, p.base = base, p.ldb = base ? ldb : 0, p.y = y, p.u = u;
+  const cudaError_t e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, false, (cudaStream_t)stream); });
+  return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
+}
+
+int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, int64_t M, int64_t K, const void* a,
+                       const void* b, int64_t N, int L, int r, const void* index, int index_bytes, const void* plan,
+                       const float* scale, float scale_value, const float* u, float* du, void* dx, void* da, void* db,
+                       void* stream) {
+  const char* who = "glad_lora_backward";
+  const char* why = shape_wrong(dtype, M, K, N, L, r, index, index_bytes);
+  if (why) return bad(who, why);
+  const size_t e_bytes = width_of(dtype);
+  if (!on(a, e_bytes) || !on(b, e_bytes) || !on(dx, e_bytes) || !on(da, e_bytes) || !on(db, e_bytes) || !on(u, 4) ||
+      !on(du, 4) || !on(scale, 4) || !on(plan, 16))
+    return bad(who, "a tensor is not element-aligned");
+  const cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e = cudaSuccess;
+  if (M == 0) {
+    if (da) e = cudaMemsetAsync(da, 0, (size_t)L * r * K * e_bytes, st);
+    if (db && e == cudaSuccess) e = cudaMemsetAsync(db, 0, (size_t)L * r * N * e_bytes, st);
+    return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
+  }
+  if (!dy || !a || !b) return bad(who, "dy, a and b must be set");
+  if (index && !plan) return bad(who, "an index needs a plan");
+  if ((why = rows_wrong(dy, dtype, lddy, M, (int)N))) return bad(who, why);
+  if (da && (!x || !du)) return bad(who, "da needs x and du");
+  if (db && !u) return bad(who, "db needs u");
+  if (da && (why = rows_wrong(x, dtype, ldx, M, (int)K))) return bad(who, why);
+  if (dx || da) {
+    Params p{};
+    p.x = dy, p.ldx = lddy, p.M = (int)M, p.K = (int)N, p.N = (int)K, p.w1 = b, p.w2 = a, p.L = L, p.r = r;
+    p.index = index, p.index64 = index_bytes == 8, p.plan = static_cast<const int32_t*>(plan);
+    p.scale = scale, p.scale_value = scale_value, p.y = dx, p.u = da ? du : nullptr;
+    e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, true, st); });
+  }
+  OuterParams o{};
+  o.plan = static_cast<const int32_t*>(plan), o.M = (int)M, o.r = r, o.L = L;
+  if (da && e == cudaSuccess) {
+    o.x = x, o.ldx = ldx, o.v = du, o.out = da, o.K = (int)K, o.step_r = K, o.step_k = 1;
+    e = for_type(dtype, [&](auto t) { return run_outer<decltype(t)>(o, st); });
+  }
+  if (db && e == cudaSuccess) {
+    o.x = dy, o.ldx = lddy, o.v = u, o.out = db, o.K = (int)N, o.step_r = 1, o.step_k = r;
+    e = for_type(dtype, [&](auto t) { return run_outer<decltype(t)>(o, st); });
+  }
+  return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
+}
+
+}  // extern "C"

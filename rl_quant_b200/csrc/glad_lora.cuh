@@ -1,0 +1,612 @@
+// Low-rank adapters of many requests beside a shared projection:
+//   forward   u[m] = s[i] A[i] x[m],  y[m] = base[m] + B[i] u[m]          (i: row m's adapter; none: y = base or 0)
+//   backward  du[m] = s[i] B[i]^T dy[m],  dx[m] = A[i]^T du[m]            (the same kernel on transposed weights)
+//             dA[i] = sum over i's rows of du[m] x[m]^T,  dB[i] = the same of dy[m] u[m]^T
+//
+// Few operations a byte (2 r of them), so the bytes of x, base, y and the adapters in use are the bound. Rows of an adapter are
+// taken in tiles; a cluster of blocks shares a tile: its warps split K for u, the parts are added through distributed
+// shared memory in a fixed order, and the warps split N for y. Operands go from global memory straight into
+// the fragments of mma.sync: a product's order of k is free as long as both operands share it, so a lane takes
+// 16 adjacent bytes of a row as its k of several instructions, and likewise 32 adjacent bytes of an output row.
+//
+// u is fp32 and stays so: as an operand it is split into two tf32 numbers (22 bits). Inputs of 16 bits are exact in tf32;
+// fp32 inputs are split the same way, three products each.
+#pragma once
+#include "glad_elem.cuh"
+#include "tc05.cuh"
+
+namespace glad {
+namespace lora {
+
+constexpr int kThreads = 256, kWarps = 8;
+constexpr int kSelfRows = 256;        // up to so many rows the kernel finds the rows of an adapter itself
+constexpr int kMaxAdapters = 16384, kMaxRank = 128;
+
+// What glad_lora_plan leaves: rows in the order of their adapters, and tiles of them. In 32-bit words:
+//   [0] tiles, [1 .. L+2] first place of each adapter's rows in the order (L: of the rows without one; L+1: M),
+//   then the order [M], then the tiles (adapter or -1, first place) [2 * max]
+struct Plan {
+  const int32_t* w;
+  int L, M;
+  __device__ int tiles() const { return w[0]; }
+  __device__ int first(int a) const { return w[1 + a]; }
+  __device__ int row(int place) const { return w[3 + L + place]; }
+  __device__ int2 tile(int t) const { return make_int2(w[3 + L + M + 2 * t], w[3 + L + M + 2 * t + 1]); }
+};
+
+struct Params {
+  const void* x;        // [M, K]
+  const void* w1;       // A [L, r, K]; transposed: B [L, K, r]
+  const void* w2;       // B [L, N, r]; transposed: A [L, r, N]
+  const void* base;     // [M, N] or null
+  void* y;              // [M, N]
+  float* u;             // [M, r] or null
+  const float* scale;   // [L] or null: scale_value
+  const void* index;    // null: adapter 0 for every row
+  const int32_t* plan;  // null: the kernel looks at index itself
+  int64_t ldx, ldb;
+  float scale_value;
+  int M, K, N, r, L, index64, cluster;
+};
+
+struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
+  const void* x;        // [M, K]
+  const float* v;       // [M, r]
+  void* out;            // element (rank, k) of adapter a at a * r * K + rank * step_r + k * step_k
+  const int32_t* plan;  // null: all rows are adapter 0's
+  int64_t ldx, step_r, step_k;
+  int M, K, r, L, cluster;
+};
+
+__device__ __forceinline__ float tf32(float v) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return __uint_as_float(r);
+}
+// v = hi + lo, 11 bits each. Where v or hi is not finite, lo is 0.
+__device__ __forceinline__ void split(float v, float& hi, float& lo) {
+  hi = tf32(v);
+  lo = fabsf(hi) < INFINITY ? tf32(v - hi) : 0.0f;
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const float4& a, float b0, float b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(a.z)), "r"(__float_as_uint(a.w)),
+        "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// a and b of the product with (hi, lo) parts each.
+__device__ __forceinline__ void mma_split(float (&c)[4], const float4& ah, const float4& al, float b0, float b1) {
+  float h0, l0, h1, l1;
+  split(b0, h0, l0);
+  split(b1, h1, l1);
+  mma_tf32(c, al, h0, h1);
+  mma_tf32(c, ah, l0, l1);
+  mma_tf32(c, ah, h0, h1);
+}
+__device__ __forceinline__ void split4(const float4& v, float4& hi, float4& lo) {
+  split(v.x, hi.x, lo.x);
+  split(v.y, hi.y, lo.y);
+  split(v.z, hi.z, lo.z);
+  split(v.w, hi.w, lo.w);
+}
+
+// n adjacent elements as 32-bit words (16-bit types: two a word), those at or past `live` zero. VEC: live is 0 or at least n, and
+// the address on the boundary of the access.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_n(const T* p, int live, uint32_t (&w)[N * (int)sizeof(T) / 4]) {
+  constexpr int W = N * (int)sizeof(T) / 4;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = 0;
+    if (live > 0) {
+      if constexpr (W == 1) w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      else if constexpr (W == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x, w[1] = v.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+          w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = i < live ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+      } else {
+        const uint32_t lo = 2 * i < live ? reinterpret_cast<const uint16_t*>(p)[2 * i] : 0u;
+        const uint32_t hi = 2 * i + 1 < live ? reinterpret_cast<const uint16_t*>(p)[2 * i + 1] : 0u;
+        w[i] = lo | hi << 16;
+      }
+    }
+  }
+}
+// Element e of such words as fp32.
+template <typename T, int W>
+__device__ __forceinline__ float elem(const uint32_t (&w)[W], int e) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w[e]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[e >> 1]);
+    return e & 1 ? __high2float(h) : __low2float(h);
+  } else {
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+}
+// The 16-bit elements number e of words a and b as a pair.
+__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, int e) {
+  return __byte_perm(a, b, e & 1 ? 0x7632 : 0x5410);
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ int adapter_of(const Params& p, int m) {
+  const int64_t a = p.index64 ? static_cast<const int64_t*>(p.index)[m] : (int64_t)static_cast<const int32_t*>(p.index)[m];
+  return a >= 0 && a < p.L ? (int)a : -1;
+}
+
+// The rows of this cluster's tile into rows[0 .. n); returns n (0: nothing to do) and the adapter.
+template <int R>
+__device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, int& adapter) {
+  const int tid = threadIdx.x;
+  int n;
+  if (p.index == nullptr) {
+    adapter = 0;
+    n = min(R, p.M - tile * R);
+    if (tid < n) rows[tid] = tile * R + tid;
+  } else if (p.plan != nullptr) {
+    const Plan plan{p.plan, p.L, p.M};
+    if (tile >= plan.tiles()) return 0;
+    const int2 t = plan.tile(tile);
+    adapter = t.x;
+    n = min(R, plan.first((adapter < 0 ? p.L : adapter) + 1) - t.y);
+    if (tid < n) rows[tid] = plan.row(t.y + tid);
+  } else {
+    // One cluster a row: it is the tile's where R, 2 R, ... rows of the same adapter (none) come before it.
+    __shared__ int of[kSelfRows], counts[kWarps];
+    if (tid < p.M) of[tid] = adapter_of(p, tid);
+    __syncthreads();
+    adapter = of[tile];
+    const bool same = tid < p.M && of[tid] == adapter;
+    if (__syncthreads_count(same && tid < tile) % R != 0) return 0;
+    const bool mine = same && tid >= tile;
+    const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+    if ((tid & 31) == 0) counts[tid >> 5] = __popc(votes);
+    __syncthreads();
+    int at = __popc(votes & ((1u << (tid & 31)) - 1)), all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < tid >> 5) at += counts[w];
+      all += counts[w];
+    }
+    if (mine && at < R) rows[at] = tid;
+    n = min(R, all);
+  }
+  __syncthreads();
+  if (tid >= n && tid < R) rows[tid] = rows[0];       // read, not used
+  __syncthreads();
+  return n;
+}
+
+template <int RT, int MT>
+constexpr size_t smem_bytes() {
+  return (size_t)(kWarps + 1) * 16 * MT * RT * sizeof(float);
+}
+
+// RT: the rank, rounded up to 16, 32, 64 or 128; MT * 16 rows a tile.
+template <typename T, int RT, int MT, bool TRANS, bool VEC>
+__global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_kernel(const Params p) {
+  constexpr int R = 16 * MT, NT = RT / 8, EL = 16 / (int)sizeof(T), CH = 4 * EL;
+  constexpr int E = RT / 4, ST = E / 2;               // ranks of a lane as an operand of y, and their instructions
+  extern __shared__ __align__(16) float sm[];
+  float* part = sm;                                   // this block's part of u, [R][RT]
+  float* red = sm + R * RT;                           // [warps][R][RT]; then u as split operands
+  __shared__ int rows[R];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
+  grid_dep_wait();
+  int adapter;
+  const int n = find_rows<R>(p, tile, rows, adapter);
+  if (n == 0) return;                                 // the whole cluster
+
+  if (adapter >= 0) {
+    const T* xr[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) xr[i] = static_cast<const T*>(p.x) + (int64_t)rows[g + 8 * i] * p.ldx;
+    const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
+    float acc[MT][NT][4] = {};
+    for (int k0 = (rank * kWarps + warp) * CH; k0 < p.K; k0 += C * kWarps * CH) {
+      const int k = k0 + q * EL, live = p.K - k;
+      uint32_t xa[2 * MT][4];
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) load_n<T, EL, VEC>(xr[i] + k, live, xa[i]);
+      uint32_t wb[NT][4];
+      if constexpr (!TRANS) {
+        // instruction column g of tile t: rank 8 t + g
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          load_n<T, EL, VEC>(w1 + (int64_t)(8 * t + g) * p.K + k, 8 * t + g < p.r ? live : 0, wb[t]);
+      } else {
+        // instruction column g of tile t: rank NT g + t, adjacent in a row of B
+        constexpr int W = NT * (int)sizeof(T) / 4;
+        uint32_t raw[EL][W];
+#pragma unroll
+        for (int e = 0; e < EL; ++e)
+          load_n<T, NT, VEC>(w1 + (int64_t)(k + e) * p.r + g * NT, e < live ? p.r - g * NT : 0, raw[e]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (sizeof(T) == 4) wb[t][w] = raw[w][t];
+            else wb[t][w] = pair_of(raw[2 * w][t >> 1], raw[2 * w + 1][t >> 1], t);
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if constexpr (sizeof(T) == 4) {
+            float4 ah, al;
+            split4(make_float4(__uint_as_float(xa[2 * i][2 * j]), __uint_as_float(xa[2 * i + 1][2 * j]),
+                               __uint_as_float(xa[2 * i][2 * j + 1]), __uint_as_float(xa[2 * i + 1][2 * j + 1])), ah, al);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              mma_split(acc[i][t], ah, al, __uint_as_float(wb[t][2 * j]), __uint_as_float(wb[t][2 * j + 1]));
+          } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              mma_16<T>(acc[i][t], xa[2 * i][2 * j], xa[2 * i + 1][2 * j], xa[2 * i][2 * j + 1], xa[2 * i + 1][2 * j + 1],
+                        wb[t][2 * j], wb[t][2 * j + 1]);
+          }
+        }
+      }
+    }
+    float* mine = red + warp * R * RT;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int col = 2 * q + (c & 1), at = TRANS ? col * NT + t : 8 * t + col;
+          mine[(16 * i + g + 8 * (c >> 1)) * RT + at] = acc[i][t][c];
+        }
+    __syncthreads();
+    for (int i = tid; i < R * RT; i += kThreads) {
+      float s = red[i];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) s += red[w * R * RT + i];
+      part[i] = s;
+    }
+  }
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  if (adapter >= 0) {
+    const float s = p.scale ? p.scale[adapter] : p.scale_value;
+    const uint32_t here = smem_u32(part);
+    float* whole = red;                                // [R][RT]
+    for (int i = tid; i < R * RT; i += kThreads) {
+      float v;
+      if (C > 1) {
+        v = ld_cluster(mapa_shared(here + 4 * i, 0));
+        for (int c = 1; c < C; ++c) v += ld_cluster(mapa_shared(here + 4 * i, c));
+      } else {
+        v = part[i];
+      }
+      v *= s;
+      whole[i] = v;
+      const int row = i / RT, at = i % RT;
+      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = v;
+    }
+  }
+  if (C > 1) cluster_sync_all();                       // nobody reads another block's part any more
+  else __syncthreads();
+  if (p.y == nullptr) return;
+  // u as the operand of instruction j: ranks E q + 2 j and E q + 2 j + 1 of rows g and g + 8, in two parts
+  float4* frag = reinterpret_cast<float4*>(red + R * RT);   // [MT][ST][32][2]
+  if (adapter >= 0) {
+    for (int i = tid; i < MT * ST * 32; i += kThreads) {
+      const int l = i & 31, j = (i >> 5) % ST, m = (i >> 5) / ST;
+      const float* v = red + (16 * m + (l >> 2)) * RT + (l & 3) * E + 2 * j;
+      split4(make_float4(v[0], v[8 * RT], v[1], v[8 * RT + 1]), frag[2 * i], frag[2 * i + 1]);
+    }
+  }
+  __syncthreads();
+
+  constexpr int TL = EL, CW = 2 * TL, BW = 8 * TL;     // tiles, a lane's adjacent columns, columns of a step
+  const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(adapter < 0 ? 0 : adapter) * p.N * p.r;
+  for (int n0 = (rank * kWarps + warp) * BW; n0 < p.N; n0 += C * kWarps * BW) {
+    const int col = n0 + q * CW;
+    uint32_t bw[2 * MT][2][4];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool on = p.base != nullptr && g + 8 * i < n;
+        load_n<T, EL, VEC>(static_cast<const T*>(p.base) + (on ? (int64_t)rows[g + 8 * i] * p.ldb + col + h * EL : 0),
+                           on ? p.N - col - h * EL : 0, bw[i][h]);
+      }
+    float c[MT][TL][4] = {};
+    if (adapter >= 0) {
+      if constexpr (!TRANS) {
+        // instruction column g of tile t: output column CW (g / 2) + 2 t + g % 2
+        constexpr int PE = E < EL ? E : EL, PIECES = E / PE;
+#pragma unroll 1
+        for (int pi = 0; pi < PIECES; ++pi) {
+          uint32_t wv[TL][PE * sizeof(T) / 4];
+          const int from = q * E + pi * PE;
+#pragma unroll
+          for (int t = 0; t < TL; ++t) {
+            const int o = n0 + (g >> 1) * CW + 2 * t + (g & 1);
+            load_n<T, PE, VEC>(w2 + (int64_t)(o < p.N ? o : 0) * p.r + from, o < p.N ? p.r - from : 0, wv[t]);
+          }
+#pragma unroll
+          for (int s = 0; s < PE / 2; ++s) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const float4* f = frag + 2 * ((i * ST + pi * (PE / 2) + s) * 32 + lane);
+              const float4 ah = f[0], al = f[1];
+#pragma unroll
+              for (int t = 0; t < TL; ++t) {
+                const float b0 = elem<T>(wv[t], 2 * s), b1 = elem<T>(wv[t], 2 * s + 1);
+                if constexpr (sizeof(T) == 4) {
+                  mma_split(c[i][t], ah, al, b0, b1);
+                } else {
+                  mma_tf32(c[i][t], al, b0, b1);
+                  mma_tf32(c[i][t], ah, b0, b1);
+                }
+              }
+            }
+          }
+        }
+      } else {
+        // instruction column g of tile t: output column TL g + t, adjacent in a row of A
+        const int at = n0 + g * TL;
+#pragma unroll 2
+        for (int s = 0; s < ST; ++s) {
+          const int from = q * E + 2 * s;
+          uint32_t w0[4], w1v[4];
+          load_n<T, EL, VEC>(w2 + (int64_t)(from < p.r ? from : 0) * p.N + at, from < p.r ? p.N - at : 0, w0);
+          load_n<T, EL, VEC>(w2 + (int64_t)(from + 1 < p.r ? from + 1 : 0) * p.N + at, from + 1 < p.r ? p.N - at : 0, w1v);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const float4* f = frag + 2 * ((i * ST + s) * 32 + lane);
+            const float4 ah = f[0], al = f[1];
+#pragma unroll
+            for (int t = 0; t < TL; ++t) {
+              const float b0 = elem<T>(w0, t), b1 = elem<T>(w1v, t);
+              if constexpr (sizeof(T) == 4) {
+                mma_split(c[i][t], ah, al, b0, b1);
+              } else {
+                mma_tf32(c[i][t], al, b0, b1);
+                mma_tf32(c[i][t], ah, b0, b1);
+              }
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      if (g + 8 * i >= n) continue;
+      T* y = static_cast<T*>(p.y) + (int64_t)rows[g + 8 * i] * p.N + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float o[EL];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+          const int l = h * EL + e;                    // the lane's column
+          const int t = TRANS ? l % TL : l >> 1, odd = TRANS ? l / TL : l & 1;
+          o[e] = c[i >> 1][t][2 * (i & 1) + odd] + elem<T>(bw[i][h], e);
+        }
+        if constexpr (VEC) {
+          if (col + h * EL < p.N) {
+            if constexpr (sizeof(T) == 4)
+              *reinterpret_cast<float4*>(y + h * EL) = make_float4(o[0], o[1], o[2], o[3]);
+            else
+              *reinterpret_cast<uint4*>(y + h * EL) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
+                                                                 pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < EL; ++e)
+            if (col + h * EL + e < p.N) y[h * EL + e] = from_f<T>(o[e]);
+        }
+      }
+    }
+  }
+}
+
+// RT: ranks of a block, 16 or 32 (blockIdx.z: which). A cluster shares 8 EL columns of one adapter's gradient; its warps split
+// the rows, and the parts are added in a fixed order.
+template <typename T, int RT, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p) {
+  constexpr int EL = 16 / (int)sizeof(T), TL = EL, BW = 8 * TL, RM = RT / 16;
+  extern __shared__ __align__(16) float sm[];
+  float* part = sm;                                    // [RT][BW]
+  float* red = sm + RT * BW;                           // [warps][RT][BW]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int C = p.cluster, rank = (int)blockIdx.x % C, n0 = (int)blockIdx.x / C * BW;
+  const int a = blockIdx.y, r0 = blockIdx.z * RT;
+  grid_dep_wait();
+  const Plan plan{p.plan, p.L, p.M};
+  const int from = p.plan ? plan.first(a) : 0, rows = p.plan ? plan.first(a + 1) - from : p.M;
+  const int at = n0 + g * EL, live = p.K - at;
+  float acc[RM][TL][4] = {};
+#pragma unroll 2
+  for (int i0 = (rank * kWarps + warp) * 8; i0 < rows; i0 += C * kWarps * 8) {
+    uint32_t xw[2][4];
+    float4 v[RM];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = i0 + q + 4 * h;
+      const bool on = i < rows;
+      const int m = !on ? 0 : p.plan ? plan.row(from + i) : i;
+      load_n<T, EL, VEC>(static_cast<const T*>(p.x) + (int64_t)m * p.ldx + at, on ? live : 0, xw[h]);
+      const float* vr = p.v + (int64_t)m * p.r;
+#pragma unroll
+      for (int k = 0; k < RM; ++k) {
+        const int lo = r0 + 16 * k + g, hi = lo + 8;
+        const float v0 = on && lo < p.r ? vr[lo] : 0.0f, v1 = on && hi < p.r ? vr[hi] : 0.0f;
+        if (h == 0) v[k].x = v0, v[k].y = v1;
+        else v[k].z = v0, v[k].w = v1;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < RM; ++k) {
+      float4 ah, al;
+      split4(v[k], ah, al);
+#pragma unroll
+      for (int t = 0; t < TL; ++t) {
+        const float b0 = elem<T>(xw[0], t), b1 = elem<T>(xw[1], t);
+        if constexpr (sizeof(T) == 4) {
+          mma_split(acc[k][t], ah, al, b0, b1);
+        } else {
+          mma_tf32(acc[k][t], al, b0, b1);
+          mma_tf32(acc[k][t], ah, b0, b1);
+        }
+      }
+    }
+  }
+  float* mine = red + warp * RT * BW;
+#pragma unroll
+  for (int k = 0; k < RM; ++k)
+#pragma unroll
+    for (int t = 0; t < TL; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        mine[(16 * k + g + 8 * (c >> 1)) * BW + (2 * q + (c & 1)) * TL + t] = acc[k][t][c];
+  __syncthreads();
+  for (int i = tid; i < RT * BW; i += kThreads) {
+    float s = red[i];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) s += red[w * RT * BW + i];
+    part[i] = s;
+  }
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  T* out = static_cast<T*>(p.out) + (int64_t)a * p.r * p.K;
+  const uint32_t here = smem_u32(part);
+  const bool by_rank = p.step_r == 1;                  // adjacent threads write adjacent elements
+  for (int i = rank * kThreads + tid; i < RT * BW; i += C * kThreads) {
+    const int k = by_rank ? i % RT : i / BW, col = by_rank ? i / RT : i % BW;
+    const uint32_t src = here + 4 * (k * BW + col);
+    float v;
+    if (C > 1) {
+      v = ld_cluster(mapa_shared(src, 0));
+      for (int c = 1; c < C; ++c) v += ld_cluster(mapa_shared(src, c));
+    } else {
+      v = part[k * BW + col];
+    }
+    if (r0 + k < p.r && n0 + col < p.K) out[(r0 + k) * p.step_r + (int64_t)(n0 + col) * p.step_k] = from_f<T>(v);
+  }
+  if (C > 1) cluster_sync_all();
+}
+
+template <typename F, typename P>
+cudaError_t launch_clusters(F* kernel, const P& p, dim3 grid, size_t smem, cudaStream_t st) {
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// Rows of a tile: 16 where an adapter has no more on average, or where 32 need too many registers.
+inline int tile_rows(int64_t M, int L, int r, bool indexed) {
+  if (r > 64) return 16;
+  return M > 16 * (int64_t)(indexed ? L : 1) ? 32 : 16;
+}
+inline int64_t max_tiles(int64_t M, int L, int r, bool indexed, bool planned) {
+  const int R = tile_rows(M, L, r, indexed);
+  if (!indexed) return (M + R - 1) / R;
+  if (!planned) return M;
+  const int64_t all = (M + R - 1) / R + L + 1;
+  return all < M ? all : M;
+}
+
+template <typename T, int RT, int MT, bool TRANS>
+cudaError_t launch_rt(const Params& p, int64_t tiles, bool vec, cudaStream_t st) {
+  const dim3 grid((unsigned)(tiles * p.cluster));
+  if (vec) return launch_clusters(lora_kernel<T, RT, MT, TRANS, true>, p, grid, smem_bytes<RT, MT>(), st);
+  return launch_clusters(lora_kernel<T, RT, MT, TRANS, false>, p, grid, smem_bytes<RT, MT>(), st);
+}
+
+// The kernel for p's type, rank and rows; vec: every access on its boundary.
+template <typename T>
+cudaError_t run(Params p, bool trans, cudaStream_t st) {
+  const bool indexed = p.index != nullptr;
+  const int R = tile_rows(p.M, p.L, p.r, indexed);
+  const int64_t tiles = max_tiles(p.M, p.L, p.r, indexed, p.plan != nullptr);
+  const int64_t real = (p.M + R - 1) / R;
+  p.cluster = 1;
+  while (p.cluster < 8 && real * p.cluster * 2 <= 3 * num_sms()) p.cluster *= 2;
+  const int RT = p.r <= 16 ? 16 : p.r <= 32 ? 32 : p.r <= 64 ? 64 : 128, EL = 16 / (int)sizeof(T);
+  const bool vec = p.K % EL == 0 && p.N % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && on(p.w1, 16) &&
+                   on(p.w2, 16) && on(p.base, 16) && (p.M <= 1 || p.ldb % EL == 0) && on(p.y, 16) && p.r % (RT / 4) == 0;
+#define GLAD_LORA(RT_, MT_) \
+  return trans ? launch_rt<T, RT_, MT_, true>(p, tiles, vec, st) : launch_rt<T, RT_, MT_, false>(p, tiles, vec, st)
+  if (RT == 16) {
+    if (R == 32) GLAD_LORA(16, 2);
+    GLAD_LORA(16, 1);
+  }
+  if (RT == 32) {
+    if (R == 32) GLAD_LORA(32, 2);
+    GLAD_LORA(32, 1);
+  }
+  if (RT == 64) {
+    if (R == 32) GLAD_LORA(64, 2);
+    GLAD_LORA(64, 1);
+  }
+  GLAD_LORA(128, 1);
+#undef GLAD_LORA
+}
+
+template <typename T>
+cudaError_t run_outer(OuterParams p, cudaStream_t st) {
+  constexpr int EL = 16 / (int)sizeof(T), BW = 8 * EL;
+  const int RT = p.r <= 16 ? 16 : 32;
+  const int64_t rows = p.plan ? (p.M + p.L - 1) / p.L : p.M;       // of an adapter, on average
+  p.cluster = 1;
+  while (p.cluster < 8 && rows >= (int64_t)p.cluster * 2 * 64) p.cluster *= 2;
+  const bool vec = p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0);
+  const dim3 grid((unsigned)((p.K + BW - 1) / BW * p.cluster), (unsigned)p.L, (unsigned)((p.r + RT - 1) / RT));
+  const size_t smem = (size_t)(kWarps + 1) * RT * BW * sizeof(float);
+  if (RT == 16)
+    return vec ? launch_clusters(outer_kernel<T, 16, true>, p, grid, smem, st)
+               : launch_clusters(outer_kernel<T, 16, false>, p, grid, smem, st);
+  return vec ? launch_clusters(outer_kernel<T, 32, true>, p, grid, smem, st)
+             : launch_clusters(outer_kernel<T, 32, false>, p, grid, smem, st);
+}
+
+}  // namespace lora
+}  // namespace glad

@@ -1,0 +1,9 @@
+// The adapter kernels (glad_lora.cuh) for rows of f16.
+#include "glad_lora.cuh"
+
+namespace glad {
+namespace lora {
+template cudaError_t run<__half>(Params, bool, cudaStream_t);
+template cudaError_t run_outer<__half>(OuterParams, cudaStream_t);
+}  // namespace lora
+}  // namespace glad

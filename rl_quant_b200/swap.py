@@ -1,4 +1,4 @@
-"""Module surgery: nn.Linear <-> QuantLinear (qrt/swap.py:39-74) or W4Linear, nn.RMSNorm <-> RMSNorm.
+"""Module surgery: nn.Linear <-> QuantLinear (qrt/swap.py:39-74) or W4Linear, nn.RMSNorm <-> RMSNorm, adapters over any linear.
 
 The swap moves the source layer's Parameter objects into the QuantLinear
 (no copies), so optimisers created before or after stay valid, and both
@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch.nn as nn
 
+from .lora import LoRALinear
 from .norm import RMSNorm
 from .qlinear import QuantLinear
 from .w4linear import W4Linear
@@ -72,6 +73,35 @@ def restore_norm(model: nn.Module, originals: dict[str, nn.RMSNorm]) -> None:
     for path, norm in originals.items():
         norm.train(get_module(model, path).training)
         set_module(model, path, norm)
+
+
+def apply_lora(model: nn.Module, paths: list[str], rank: int = 16, adapters: int = 1, alpha: float | None = None,
+               freeze: bool = True) -> dict[str, LoRALinear]:
+    """Put ``adapters`` low-rank adapters over each of the named linear layers (nn.Linear, QuantLinear, W4Linear); returns the
+    new layers by path. All or none."""
+    swapped: dict[str, LoRALinear] = {}
+    for path in paths:
+        lin = get_module(model, path)
+        assert isinstance(lin, (nn.Linear, QuantLinear, W4Linear)), f"{path} is not a linear layer: {type(lin)}"
+        swapped[path] = LoRALinear(lin, rank, adapters, alpha, freeze=False)
+    for path, mod in swapped.items():
+        if freeze:
+            for p in mod.base.parameters():
+                p.requires_grad_(False)
+        set_module(model, path, mod)
+    return swapped
+
+
+def select_lora(swapped: dict[str, LoRALinear], index) -> None:
+    """Name the rows' adapters (``LoRALinear.select``) in every layer that ``apply_lora`` returned."""
+    for mod in swapped.values():
+        mod.select(index)
+
+
+def restore_lora(model: nn.Module, swapped: dict[str, LoRALinear]) -> None:
+    """Put the layers below the adapters back, with the swapped modules' train/eval flag."""
+    for path, mod in swapped.items():
+        set_module(model, path, mod.base.train(mod.training))
 
 
 def restore(model: nn.Module, swapped: dict[str, nn.Module]) -> None:

@@ -1,0 +1,387 @@
+"""lora_linear and its gradients against the formula in 64 bits.
+
+Tolerances, fixed before the first run. One matrix instruction adds up to 17 terms aligned to the largest, each off by at most
+2^-24 of it: 2^-20 of the running sum of magnitudes. A warp runs at most K / 64 + 2 of them for u (the 16-bit products are
+exact; split fp32 ones are off by 2^-20), and the joins of warps and blocks add at most 16 roundings: so u is off by (K / 64 + 20) 2^-20 sum |x| |A|.
+In y each term of u counts with its own error, splitting u is off by 2^-21, and at most 3 r / 8 + 2 instructions follow; the rounding to
+the type is half a step. The gradients are the same sums with other operands; rows of an adapter take the place of K.
+Inputs of one sign make the sums of magnitudes the sums themselves."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from rl_quant_b200 import LoRALinear, lora_linear, swap
+from rl_quant_b200 import lora as lora_mod
+
+gpu = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+S = 2.0 ** -20
+
+
+def half_step(t):
+    return 2.0 ** -24 if t == torch.float32 else torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def make(m, k, n, r, L, dtype, seed, sign=False, base=True, index="mixed"):
+    g = torch.Generator().manual_seed(seed)
+
+    def rnd(*s):
+        v = torch.randn(*s, generator=g)
+        return v.abs() if sign else v
+    x, a, b = rnd(m, k).to(dtype).cuda(), (rnd(L, r, k) / math.sqrt(k)).to(dtype).cuda(), (rnd(L, n, r) * 0.1).to(dtype).cuda()
+    base = rnd(m, n).to(dtype).cuda() if base else None
+    scale = (0.5 + torch.rand(L, generator=g)).cuda()
+    if index is None:
+        i = None
+    elif index == "one":
+        i = torch.full((m,), L - 1, dtype=torch.int64, device="cuda")
+    else:
+        i = torch.randint(-1, L, (m,), generator=g)
+        i = (i.sort().values if index == "runs" else i).cuda()
+    return x, a, b, i, scale, base, rnd(m, n).to(dtype).cuda()
+
+
+def ref(x, a, b, i, scale, base, dy):
+    """((y, bound), (dx, bound), (da, bound), (db, bound)); the bounds are of what precedes the last rounding."""
+    D = torch.float64
+    m, k = x.shape
+    L, r, _ = a.shape
+    n = b.shape[1]
+    new = lambda *s: torch.zeros(*s, dtype=D, device="cuda")  # noqa: E731
+    out = [[new(m, n), new(m, n)], [new(m, k), new(m, k)], [new(L, r, k), new(L, r, k)], [new(L, n, r), new(L, n, r)]]
+    if base is not None:
+        out[0][0] += base.to(D)
+        out[0][1] += base.to(D).abs() * S
+    for j in range(L):
+        rows = torch.arange(m, device="cuda") if i is None else (i == j).nonzero()[:, 0]
+        if not len(rows):
+            continue
+        X, A, B, G = x[rows].to(D), a[j].to(D), b[j].to(D), dy[rows].to(D)
+        s = float(scale[j]) if isinstance(scale, torch.Tensor) else scale
+        U, V = s * X @ A.T, s * G @ B
+        U1, V1 = s * X.abs() @ A.abs().T, s * G.abs() @ B.abs()
+        eU, eV = (k / 64 + 21) * S * U1, (n / 64 + 21) * S * V1
+        more, many = (3 * r / 8 + 3) * S, (3 * len(rows) / 8 + 20) * S
+        out[0][0][rows] += U @ B.T
+        out[0][1][rows] += (eU + more * U.abs()) @ B.abs().T
+        out[1][0][rows] = V @ A
+        out[1][1][rows] = (eV + more * V.abs()) @ A.abs()
+        out[2][0][j], out[2][1][j] = V.T @ X, (eV + many * V.abs()).T @ X.abs()
+        out[3][0][j], out[3][1][j] = G.T @ U, G.abs().T @ (eU + many * U.abs())
+    return out
+
+
+def close(got, want, dtype):
+    value, bound = want
+    assert got.dtype == dtype and got.shape == value.shape
+    tol = bound + half_step(dtype) * (value.abs() + bound) + tiny(dtype)
+    worst = ((got.double() - value).abs() - tol).max() if got.numel() else torch.tensor(0.0)
+    assert float(worst) <= 0.0, float(worst)
+
+
+def check(x, a, b, i, scale, base, dy, back=True):
+    want = ref(x, a, b, i, scale, base, dy)
+    y = lora_linear(x, a, b, i, scale, base)
+    close(y, want[0], x.dtype)
+    if i is not None and base is not None:
+        assert torch.equal(y[i < 0], base[i < 0])
+    if not back:
+        return y
+    leaves = [t.detach().clone().requires_grad_() for t in (x, a, b)]
+    bl = None if base is None else base.clone().requires_grad_()
+    y2 = lora_linear(*leaves, i, scale, bl)
+    close(y2.detach(), want[0], x.dtype)
+    grads = torch.autograd.grad(y2, leaves + ([] if bl is None else [bl]), dy)
+    for g, w in zip(grads, want[1:]):
+        close(g, w, x.dtype)
+    if bl is not None:
+        assert torch.equal(grads[3], dy)
+    return y
+
+
+# rows, inputs, outputs, rank, adapters: one token to many, ranks at and off the tile sizes, sizes off every vector
+SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65, 3, 2), (16, 256, 128, 8, 1), (17, 128, 256, 4, 4),
+         (64, 512, 1024, 16, 64), (33, 96, 64, 32, 2), (40, 1002, 777, 9, 5), (256, 264, 136, 24, 3), (257, 64, 72, 64, 3),
+         (300, 200, 320, 48, 1), (300, 72, 64, 100, 2), (130, 128, 128, 128, 2), (1000, 48, 40, 16, 130), (2050, 520, 264, 16, 2),
+         (600, 1024, 1024, 33, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_sizes(size, dtype):
+    m, k, n, r, L = size
+    for seed, (sign, base, index) in enumerate(((True, False, "mixed"), (False, True, "runs"), (False, True, "one"))):
+        if index == "one" and L == 1:
+            index = None
+        check(*make(m, k, n, r, L, dtype, seed, sign, base, index))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides(dtype):
+    x, a, b, i, scale, base, dy = make(50, 128, 96, 16, 3, dtype, 4)
+    want = lora_linear(x, a, b, i, scale, base)
+    wide = torch.zeros(50, 300, dtype=dtype, device="cuda")
+    wide[:, 8:136] = x
+    wide2 = torch.zeros(50, 201, dtype=dtype, device="cuda")
+    wide2[:, 3:99] = base
+    assert torch.equal(lora_linear(wide[:, 8:136], a, b, i, scale, base), want)
+    for xs, bs in ((x, wide2[:, 3:99]), (x.t().contiguous().t(), base.t().contiguous().t())):
+        close(lora_linear(xs, a, b, i, scale, bs), ref(x, a, b, i, scale, base, dy)[0], dtype)
+    wide[:, 3:131] = x
+    close(lora_linear(wide[:, 3:131], a, b, i, scale, base), ref(x, a, b, i, scale, base, dy)[0], dtype)
+    turned = a.transpose(1, 2).contiguous().transpose(1, 2)
+    spread = torch.zeros(50, 2, dtype=torch.int32, device="cuda")
+    spread[:, 1] = i
+    assert torch.equal(lora_linear(x, turned, b, spread[:, 1], scale, base), want)
+    cube = lora_linear(x.view(5, 10, 128), a, b, i.view(5, 10), scale, base.view(5, 10, 96))
+    assert cube.shape == (5, 10, 96) and torch.equal(cube.view(50, 96), want)
+    one = x[:1].expand(50, 128)
+    close(lora_linear(one, a, b, i, scale, base), ref(one, a, b, i, scale, base, dy)[0], dtype)
+    for leaf, args in ((x.clone().requires_grad_(), ()),):
+        y = lora_linear(leaf, a, b, i, scale, base)
+        g, = torch.autograd.grad(y, leaf, dy.t().contiguous().t())
+        close(g, ref(x, a, b, i, scale, base, dy)[1], dtype)
+        g, = torch.autograd.grad(lora_linear(leaf, a, b, i, scale, base).sum(), leaf)
+        close(g, ref(x, a, b, i, scale, base, torch.ones_like(dy))[1], dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [20, 400])
+def test_index(m, dtype):
+    """Outside 0..L-1: no adapter. Adapters without rows: zero gradients. A number as scale."""
+    x, a, b, i, scale, base, dy = make(m, 64, 48, 8, 6, dtype, 5)
+    i = i.clone()
+    i[i == 2] = 3
+    i[0], i[1], i[2] = 6, -7, 2 ** 40
+    clean = torch.where((i < 0) | (i > 5), -1, i)
+    y = check(x, a, b, clean, scale, base, dy)
+    assert torch.equal(lora_linear(x, a, b, i, scale, base), y)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    dx, da, db = torch.autograd.grad(lora_linear(*leaves, i, scale, base), leaves, dy)
+    assert not dx[:3].any() and not da[2].any() and not db[2].any()
+    none = torch.full_like(i, -1)
+    assert torch.equal(lora_linear(x, a, b, none, scale, base), base)
+    assert not lora_linear(x, a, b, none, scale).any()
+    close(lora_linear(x, a, b, clean, 0.75, base), ref(x, a, b, clean, 0.75, base, dy)[0], dtype)
+    # rows alone give what they give together, up to the order of the sums
+    for j in (3, m - 1):
+        close(lora_linear(x[j:j + 1], a, b, i[j:j + 1], scale, base[j:j + 1]),
+              [t[j:j + 1] for t in ref(x, a, b, clean, scale, base, dy)[0]], dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_some_gradients_only(dtype):
+    x, a, b, i, scale, base, dy = make(70, 64, 96, 16, 3, dtype, 6)
+    want = ref(x, a, b, i, scale, base, dy)[1:]
+    for use in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1)):
+        leaves = [t.clone().requires_grad_(bool(u)) for t, u in zip((x, a, b), use)]
+        y = lora_linear(*leaves, i, scale, base)
+        for g, w in zip(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy), [w for w, u in zip(want, use) if u]):
+            close(g, w, dtype)
+    bl = base.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(lora_linear(x, a, b, i, scale, bl), bl, dy)[0], dy)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_keep_to_themselves(dtype):
+    """A NaN or an infinity in a row of x or of base stays in that row; in an adapter, in its rows."""
+    x, a, b, i, scale, base, dy = make(90, 96, 80, 16, 4, dtype, 7)
+    want = lora_linear(x, a, b, i, scale, base)
+    i[5], i[9] = 1, -1
+    want = lora_linear(x, a, b, i, scale, base)
+    bad = x.clone()
+    bad[5, 3] = math.nan
+    bad[9] = math.inf                      # a row without an adapter
+    got = lora_linear(bad, a, b, i, scale, base)
+    keep = torch.ones(90, dtype=torch.bool)
+    keep[5] = False
+    assert torch.equal(got[keep], want[keep]) and got[5].isnan().all()
+    ab = a.clone()
+    ab[2] = math.nan
+    got = lora_linear(x, ab, b, i, scale, base)
+    assert torch.equal(got[i != 2], want[i != 2]) and got[i == 2].isnan().all()
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    g = dy.clone()
+    g[5] = math.nan
+    dx, da, db = torch.autograd.grad(lora_linear(*leaves, i, scale, base), leaves, g)
+    assert torch.isfinite(dx[keep]).all() and torch.isfinite(da[[0, 2, 3]]).all() and torch.isfinite(db[[0, 2, 3]]).all()
+    assert dx[5].isnan().all() and da[1].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_repeats_streams_and_graphs(dtype):
+    for m in (30, 700):
+        x, a, b, i, scale, base, dy = make(m, 256, 192, 16, 5, dtype, 8)
+        leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+
+        def once():
+            y = lora_linear(*leaves, i, scale, base)
+            return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+        first = once()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            again = once()
+        torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(u, v) for u, v in zip(first, again))
+        moving = i.clone()
+        with torch.no_grad():
+            lora_linear(x, a, b, moving, scale, base)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y1 = lora_linear(x, a, b, moving, scale, base)
+                y2 = lora_linear(x, a, b, moving, 2.0)
+            moving.copy_(i.flip(0))
+            for _ in range(2):
+                graph.replay()
+            assert torch.equal(y1, lora_linear(x, a, b, i.flip(0), scale, base))
+            assert torch.equal(y2, lora_linear(x, a, b, i.flip(0), 2.0))
+
+
+@gpu
+def test_gradients_against_differences():
+    x, a, b, i, scale, base, dy = make(9, 20, 12, 4, 2, torch.float32, 9)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    grads = torch.autograd.grad(lora_linear(*leaves, i, scale, base), leaves, dy)
+    data = [t.double() for t in (x, a, b)]
+
+    def f(x_, a_, b_):
+        total = 0.0
+        for m in range(9):
+            j = int(i[m])
+            if j >= 0:
+                total = total + (float(scale[j]) * (b_[j] @ (a_[j] @ x_[m])) * dy[m].double()).sum()
+        return total
+    for t in range(3):
+        for at in ((0,) * data[t].dim(), tuple(v - 1 for v in data[t].shape)):
+            hi, lo = [v.clone() for v in data], [v.clone() for v in data]
+            hi[t][at] += 1e-4
+            lo[t][at] -= 1e-4
+            d = float(f(*hi) - f(*lo)) / 2e-4 if not isinstance(f(*hi), float) else 0.0
+            assert abs(d - float(grads[t][at])) < 1e-4 * (1 + abs(d))
+
+
+@gpu
+def test_empty_and_large_offsets():
+    x, a, b, i, scale, base, dy = make(4, 64, 64, 16, 2, torch.bfloat16, 10)
+    assert lora_linear(x[:0], a, b, i[:0], scale, base[:0]).shape == (0, 64)
+    leaves = [t.clone().requires_grad_() for t in (x[:0], a, b)]
+    dx, da, db = torch.autograd.grad(lora_linear(*leaves, i[:0], scale).sum(), leaves)
+    assert dx.shape == (0, 64) and not da.any() and not db.any()
+    # rows whose offsets pass 2^31 elements
+    m = 70000
+    big = torch.zeros(m, 32768, dtype=torch.bfloat16, device="cuda")
+    big[m - 1] = 1.0
+    a, b = torch.full((1, 16, 32768), 2.0 ** -15, dtype=torch.bfloat16, device="cuda"), torch.ones(1, 64, 16, dtype=torch.bfloat16,
+                                                                                                   device="cuda")
+    y = lora_linear(big, a, b)
+    assert (y[m - 1] == 16.0).all() and not y[:m - 1].any()
+    leaf = a.clone().requires_grad_()
+    da, = torch.autograd.grad(lora_linear(big, leaf, b), leaf, torch.ones(m, 64, dtype=torch.bfloat16, device="cuda"))
+    assert (da == 64.0).all()
+
+
+def net(dtype, device):
+    torch.manual_seed(0)
+    return nn.Sequential(nn.Linear(96, 128), nn.ELU(), nn.Linear(128, 64)).to(device=device, dtype=dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_module_over_4_bit_layers(dtype):
+    m = net(dtype, "cuda")
+    plain = net(dtype, "cuda")
+    q = swap.apply(m, {"0": {"bits": 4, "group": 32}, "2": {"bits": 4, "group": 32}})
+    x = torch.randn(40, 96, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    with torch.no_grad():
+        before = m(x)
+    layers = swap.apply_lora(m, ["0", "2"], rank=8, adapters=3, alpha=16)
+    index = torch.arange(40, device="cuda") % 4 - 1
+    swap.select_lora(layers, index)
+    with torch.no_grad():
+        assert torch.equal(m(x), before)                 # new adapters change nothing
+        for mod in layers.values():
+            mod.lora_b.normal_(std=0.05)
+        y = m(x)
+        assert torch.equal(y[index < 0], before[index < 0]) and not torch.equal(y, before)
+        for j in range(3):
+            swap.select_lora(layers, j)
+            assert torch.allclose(m(x)[index == j].float(), y[index == j].float(), rtol=2 ** -6, atol=2 ** -6)
+        swap.select_lora(layers, None)
+        assert torch.equal(m(x), before)
+    swap.select_lora(layers, index)
+    out = m(x)                                           # training: the source layers' own weights below
+    out.float().square().sum().backward()
+    assert all(mod.lora_a.grad is not None and mod.lora_b.grad is not None for mod in layers.values())
+    assert all(mod.base.weight.grad is None for mod in layers.values())
+    swap.restore_lora(m, layers)
+    assert m[0] is q["0"]
+    swap.restore(m, q)
+    assert torch.equal(m[0].weight, plain[0].weight)
+
+
+def test_module_surgery():
+    m = net(torch.float32, "cpu")
+    m.eval()
+    lin = m[0]
+    with pytest.raises(AssertionError, match="not a linear"):
+        swap.apply_lora(m, ["0", "1"])
+    with pytest.raises(ValueError, match="rank"):
+        swap.apply_lora(m, ["0"], rank=129)
+    assert m[0] is lin and lin.weight.requires_grad       # all or none
+    layers = swap.apply_lora(m, ["0"], rank=4, adapters=2, alpha=8)
+    mod = layers["0"]
+    assert isinstance(m[0], LoRALinear) and not m[0].training and mod.scale == 2.0
+    assert mod.lora_a.shape == (2, 4, 96) and mod.lora_b.shape == (2, 128, 4) and not mod.lora_b.any()
+    assert not lin.weight.requires_grad and {n for n, p in m.named_parameters() if p.requires_grad} == {
+        "0.lora_a", "0.lora_b", "2.weight", "2.bias"}
+    for bad in (2, -2):
+        with pytest.raises(ValueError, match="adapter"):
+            mod.select(bad)
+    with pytest.raises(TypeError, match="int8"):
+        mod(torch.zeros(3, 96, dtype=torch.int8))
+    x = torch.randn(3, 96)
+    assert torch.equal(mod.select(None)(x), lin(x))
+    swap.restore_lora(m, layers)
+    assert m[0] is lin and not lin.training
+
+
+def test_refusals():
+    x, a, b = torch.zeros(3, 8), torch.zeros(2, 4, 8), torch.zeros(2, 5, 4)
+    i = torch.zeros(3, dtype=torch.int64)
+
+    def call(x=x, a=a, b=b, index=i, **kw):
+        return lora_linear(x, a, b, index, **kw)
+    for bad, kind, what in (
+            (dict(x=x.double()), TypeError, "x is"), (dict(a=a[0]), ValueError, "must be"), (dict(b=b[:1]), ValueError, "must be"),
+            (dict(b=torch.zeros(2, 5, 3)), ValueError, "must be"), (dict(x=torch.zeros(3, 7)), ValueError, "inputs"),
+            (dict(a=a.half()), TypeError, "expected x's"), (dict(index=None), ValueError, "need an index"),
+            (dict(index=i.float()), TypeError, "index is"), (dict(index=i[:2]), ValueError, "does not match"),
+            (dict(scale=torch.ones(3)), ValueError, "scale"), (dict(scale=torch.ones(2).half()), ValueError, "scale"),
+            (dict(scale=torch.ones(2, requires_grad=True)), RuntimeError, "no gradient of scale"),
+            (dict(base=torch.zeros(3, 4)), ValueError, "base"), (dict(base=torch.zeros(3, 5).half()), TypeError, "base"),
+            (dict(a=torch.zeros(2, 200, 8), b=torch.zeros(2, 5, 200)), ValueError, "up to"),
+            (dict(a=torch.zeros(2, 0, 8), b=torch.zeros(2, 5, 0)), ValueError, "up to"),
+            (dict(a=torch.zeros(2, 4, 8, device="meta")), ValueError, "tensors on"),
+            (dict(), RuntimeError, "CUDA")):
+        with pytest.raises(kind, match=what):
+            call(**bad)
+    big = torch.zeros(1, 8).expand(lora_mod.MAX_SIZE + 1, 8)
+    with pytest.raises(ValueError, match="rows"):
+        lora_linear(big, a[:1], b[:1])
+    import torch.autograd.forward_ad as fwAD
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(x=fwAD.make_dual(x, torch.ones_like(x)))
