@@ -491,7 +491,7 @@ int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, i
 
 /* ---- log probabilities of given tokens (no counterpart in the reference) -------
  * Rows of logits x [rows, cols] (f32, f16 or bf16, row stride ldx >= cols elements), a token
- * (i32 or i64, token_bytes 4 or 8) a row, z = (x - max x) / temperature:
+ * (i32 or i64, token_bytes 4 or 8) a row, z = (x - max x) / temperature (1e-6 to 1e6):
  *   log_prob [rows] = z_token - ln sum e^z
  *   entropy [rows]  = -sum p ln p, p = e^z / sum e^z               (NULL: not wanted)
  *   top_index, top_log_prob [rows, top]: the `top` (0..32, at most cols) largest logits'

@@ -110,8 +110,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, temperature: flo
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(shape)}")
     if tokens.device != logits.device:
         raise ValueError(f"tensors on {logits.device} and {tokens.device}")
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"temperature must be in [1e-30, 1e30], got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6], got {temperature}")
     if not 0 <= top <= MAX_TOP or top > shape[-1]:
         raise ValueError(f"top must be in 0..{MAX_TOP} and at most the {shape[-1]} columns, got {top}")
     N.require_cuda(logits)

@@ -184,9 +184,10 @@ def test_bad_rows(cols, dtype):
     d, = torch.autograd.grad(out.log_prob.nan_to_num().sum() + out.entropy.sum() * 0 + out.log_prob.sum(), g)
     assert (d[4] == 0).all() and d[[1, 2, 3, 5]].isnan().any(-1).all()
     good = [0, 6]
-    want = token_log_probs(clean[good], tok[good], entropy=True, top=4)
+    # the same rows at the same addresses (another alignment of a row adds in another order)
+    want = token_log_probs(clean, tok.clamp(0, cols - 1), entropy=True, top=4)
     for a, b in zip(out, want):
-        assert torch.equal(a[good], b)
+        assert torch.equal(a[good], b[good])
     assert torch.isfinite(d[good]).all()
     assert ((out.top_index >= -1) & (out.top_index < cols)).all()
     keep = token_log_probs(clean, tok.clamp(0, cols - 1), ignore_index=int(tok[6]))
