@@ -1,18 +1,25 @@
 // Global norm over many tensors, and the tensors scaled by it:
 //   n = (sum |g|^2)^(1/2), sum |g| or max |g| over all tensors,  c = min(1, max_norm / (n + 1e-6)),  g' = c g
 //
-// The tensors are cut into chunks; a persistent grid walks the chunks twice, in two kernels (the scalar c needs all
-// of them first). Partial results go to fixed places and are added in a fixed order: the same call gives the same bits.
-// DRAM bytes are the bound of large calls, launch latency of small ones.
+// The tensors are cut into units of 2048 elements, and a block takes a run of neighbouring units, twice, in two kernels (the
+// scalar c needs all of them first): forwards for the sums, backwards to scale, so that what it read last is still in the L2.
+// Partial results go to fixed places and are added in a fixed order: the same call gives the same bits. DRAM bytes are the
+// bound of large calls, launch latency of small ones.
 #include "glad_elem.cuh"
 #include "tc05.cuh"
+
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
 
 namespace glad {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxBlocks = 1280;         // partial results of one launch
-constexpr int kBig = 1024, kSmall = 128; // tensors of one launch; the table travels in the kernel's parameters
+constexpr int kThreads = 256, kPerSm = 4;
+constexpr int kMaxBlocks = 640;          // partial results of one launch
+constexpr int kUnit = 2048;              // elements; a call of few units has as many blocks, so small calls spread too
+constexpr int kMost = 1024;              // tensors of one launch; the table travels in the kernel's parameters
 
 enum Kind { kInf = 0, kOne = 1, kTwo = 2 };
 
@@ -21,71 +28,70 @@ struct Table {
   const void* src[CAP];
   void* dst[CAP];
   int64_t size[CAP];
-  int32_t first[CAP + 1];    // first chunk of each tensor; their number at the end
+  int32_t first[CAP + 1];    // first unit of each tensor; their number at the end
   uint8_t dtype[CAP];
   int32_t n;
-  int32_t chunk;             // elements
 };
-static_assert(sizeof(Table<kBig>) <= 32000, "kernel parameters end at 32764 bytes");
+static_assert(sizeof(Table<kMost>) <= 32000, "kernel parameters end at 32764 bytes");
 
-// The tensor that chunk c belongs to.
+// The tensor that unit u belongs to.
 template <int CAP>
-__device__ __forceinline__ int tensor_of(const Table<CAP>& t, int c) {
+__device__ __forceinline__ int tensor_of(const Table<CAP>& t, int u) {
   int lo = 0, hi = t.n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (t.first[mid] <= c) lo = mid;
+    if (t.first[mid] <= u) lo = mid;
     else hi = mid;
   }
   return lo;
 }
-
-// Calls f(value, slot) for the block's elements [p, p + n) that are this thread's: 16-byte loads between the first and the
-// last 16-byte boundary, several at once.
-template <typename T, typename F>
-__device__ __forceinline__ void visit(const T* p, int n, F&& f) {
-  constexpr int V = 16 / sizeof(T), U = 4;
-  const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-  const int head = off ? min(n, V - off) : 0, vecs = (n - head) / V;
-  const uint4* q = reinterpret_cast<const uint4*>(p + head);
-  for (int i = threadIdx.x; i < vecs; i += kThreads * U) {
-    uint4 w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * kThreads < vecs) w[u] = q[i + u * kThreads];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * kThreads < vecs) {
-        Raw<V, T> r = {{w[u].x, w[u].y, w[u].z, w[u].w}};
-        float v[V];
-        to_floats<V, T>(r, v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f(v[e], e);
-      }
-    }
-  }
-  const int rest = n - vecs * V;                         // head and tail: fewer than 2 V elements
-  if ((int)threadIdx.x < rest) {
-    const int i = (int)threadIdx.x < head ? (int)threadIdx.x : vecs * V + (int)threadIdx.x;
-    f(to_f<T>(p[i]), 0);
-  }
+// Where block b's run of units starts.
+template <int CAP>
+__device__ __forceinline__ int first_unit(const Table<CAP>& t, unsigned b) {
+  return (int)((int64_t)t.first[t.n] * b / gridDim.x);
 }
+// Calls f(pointer type, tensor, first element, elements) for the part of tensor i in units [lo, hi).
+template <int CAP, typename F>
+__device__ __forceinline__ void part_of(const Table<CAP>& t, int i, int lo, int hi, F&& f) {
+  const int u0 = max(lo, t.first[i]) - t.first[i], u1 = min(hi, t.first[i + 1]) - t.first[i];
+  const int64_t at = (int64_t)u0 * kUnit;
+  const int n = (int)(min((int64_t)u1 * kUnit, t.size[i]) - at);
+  if (t.dtype[i] == GLAD_DTYPE_F32) f(float(), at, n);
+  else if (t.dtype[i] == GLAD_DTYPE_F16) f(__half(), at, n);
+  else f(__nv_bfloat16(), at, n);
+}
+
+// Elements [p, p + n): head before the first 16-byte boundary, 16-byte pieces, and a tail.
+template <typename T>
+struct Cut {
+  static constexpr int V = 16 / (int)sizeof(T);
+  int head, vecs, rest;
+  __device__ Cut(const T* p, int n) {
+    const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+    head = off ? min(n, V - off) : 0;
+    vecs = (n - head) / V;
+    rest = n - vecs * V;
+  }
+  __device__ int single(int i) const { return i < head ? i : vecs * V + i; }
+};
+constexpr int kBatch = 4;                // pieces a thread loads at once
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
   return a;
 }
 
-// This thread's part of a chunk's sum (or maximum). A few dozen squares are added in fp32; where they leave its range or
-// its precise part, they are added again in 64 bits, so the norm is right for gradients of any magnitude.
-template <int KIND, typename T>
-__device__ __forceinline__ void add_chunk(const T* p, int n, double& total) {
+// N values more. Squares (and magnitudes) of a few dozen are added in fp32; where they leave its range or its precise part, they
+// are added again in 64 bits, so the norm is right for gradients of any magnitude. Between them the sums are 64-bit.
+template <int KIND, int N>
+__device__ __forceinline__ void add_values(const float (&v)[N], double& total) {
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  visit<T>(p, n, [&](float v, int e) {
-    if constexpr (KIND == kInf) s[e & 3] = max_nan(s[e & 3], fabsf(v));
-    else if constexpr (KIND == kOne) s[e & 3] += fabsf(v);
-    else s[e & 3] = fmaf(v, v, s[e & 3]);
-  });
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    if constexpr (KIND == kInf) s[e & 3] = max_nan(s[e & 3], fabsf(v[e]));
+    else if constexpr (KIND == kOne) s[e & 3] += fabsf(v[e]);
+    else s[e & 3] = fmaf(v[e], v[e], s[e & 3]);
+  }
   if constexpr (KIND == kInf) {
     total = max_nan((float)total, max_nan(max_nan(s[0], s[1]), max_nan(s[2], s[3])));
   } else {
@@ -93,10 +99,43 @@ __device__ __forceinline__ void add_chunk(const T* p, int n, double& total) {
     if (sum > 1e-25f && sum < 1e30f) {
       total += sum;
     } else {
-      double d = 0.0;
-      visit<T>(p, n, [&](float v, int) { d += KIND == kOne ? fabs((double)v) : (double)v * v; });
-      total += d;
+#pragma unroll 1
+      for (int e = 0; e < N; e += 4) {
+#pragma unroll
+        for (int i = 0; i < 4 && i < N; ++i) {
+          float x = v[i];
+#pragma unroll
+          for (int k = 4; k < N; k += 4) x = e == k ? v[k + i] : x;
+          total += KIND == kOne ? fabs((double)x) : (double)x * x;
+        }
+      }
     }
+  }
+}
+
+template <int KIND, typename T>
+__device__ __forceinline__ void add_part(const T* p, int n, double& total) {
+  constexpr int V = Cut<T>::V;
+  const Cut<T> cut(p, n);
+  const uint4* q = reinterpret_cast<const uint4*>(p + cut.head);
+  for (int i = threadIdx.x; i < cut.vecs; i += kThreads * kBatch) {
+    uint4 w[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) w[u] = i + u * kThreads < cut.vecs ? q[i + u * kThreads] : make_uint4(0, 0, 0, 0);
+    float v[kBatch * V];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const Raw<V, T> r = {{w[u].x, w[u].y, w[u].z, w[u].w}};
+      float f[V];
+      to_floats<V, T>(r, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[u * V + e] = f[e];
+    }
+    add_values<KIND>(v, total);
+  }
+  if ((int)threadIdx.x < cut.rest) {
+    const float v[1] = {to_f<T>(p[cut.single(threadIdx.x)])};
+    add_values<KIND>(v, total);
   }
 }
 
@@ -120,66 +159,55 @@ __device__ __forceinline__ double block_combine(double v, double* red) {
 }
 
 template <int KIND, int CAP>
-__global__ void __launch_bounds__(kThreads) grad_sum_kernel(const __grid_constant__ Table<CAP> t, double* partial) {
+__global__ void __launch_bounds__(kThreads, kPerSm) grad_sum_kernel(const __grid_constant__ Table<CAP> t, double* partial) {
   __shared__ double red[kThreads / 32];
   grid_dep_wait();
   double total = 0.0;
-  const int chunks = t.first[t.n];
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int i = tensor_of(t, c);
-    const int64_t at = (int64_t)(c - t.first[i]) * t.chunk;
-    const int n = (int)min((int64_t)t.chunk, t.size[i] - at);
-    if (t.dtype[i] == GLAD_DTYPE_F32) add_chunk<KIND>(static_cast<const float*>(t.src[i]) + at, n, total);
-    else if (t.dtype[i] == GLAD_DTYPE_F16) add_chunk<KIND>(static_cast<const __half*>(t.src[i]) + at, n, total);
-    else add_chunk<KIND>(static_cast<const __nv_bfloat16*>(t.src[i]) + at, n, total);
-  }
+  const int lo = first_unit(t, blockIdx.x), hi = first_unit(t, blockIdx.x + 1);
+  for (int i = tensor_of(t, lo); i < t.n && t.first[i] < hi; ++i)
+    part_of(t, i, lo, hi, [&](auto type, int64_t at, int n) {
+      add_part<KIND>(static_cast<const decltype(type)*>(t.src[i]) + at, n, total);
+    });
   total = block_combine<KIND>(total, red);
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
 }
 
-// dst = c src (both may be the same). Unlike alignments: elements one by one.
+// q = c p (both may be the same), the last pieces first. Unlike alignments: elements one by one.
 template <typename T>
-__device__ __forceinline__ void scale_chunk(const T* p, T* q, int n, float c) {
-  constexpr int V = 16 / sizeof(T), U = 4;
-  const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-  const bool alike = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15) == 0;
-  const int head = alike ? (off ? min(n, V - off) : 0) : n, vecs = (n - head) / V;
-  const uint4* pv = reinterpret_cast<const uint4*>(p + head);
-  uint4* qv = reinterpret_cast<uint4*>(q + head);
-  for (int i = threadIdx.x; i < vecs; i += kThreads * U) {
-    uint4 w[U];
+__device__ __forceinline__ void scale_part(const T* p, T* q, int n, float c) {
+  constexpr int V = Cut<T>::V;
+  Cut<T> cut(p, n);
+  if (((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15) != 0) cut.head = cut.rest = n, cut.vecs = 0;
+  const uint4* pv = reinterpret_cast<const uint4*>(p + cut.head);
+  uint4* qv = reinterpret_cast<uint4*>(q + cut.head);
+  for (int b = (cut.vecs - 1) / (kThreads * kBatch) * (kThreads * kBatch); b >= 0; b -= kThreads * kBatch) {
+    const int i = b + threadIdx.x;
+    uint4 w[kBatch];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * kThreads < vecs) w[u] = pv[i + u * kThreads];
+    for (int u = 0; u < kBatch; ++u)
+      if (i + u * kThreads < cut.vecs) w[u] = pv[i + u * kThreads];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * kThreads < vecs) {
-        Raw<V, T> r = {{w[u].x, w[u].y, w[u].z, w[u].w}};
-        float v[V];
-        to_floats<V, T>(r, v);
+    for (int u = 0; u < kBatch; ++u) {
+      if (i + u * kThreads >= cut.vecs) continue;
+      const Raw<V, T> r = {{w[u].x, w[u].y, w[u].z, w[u].w}};
+      float v[V];
+      to_floats<V, T>(r, v);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] *= c;
-        if constexpr (sizeof(T) == 4) {
-          qv[i + u * kThreads] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                                            __float_as_uint(v[3]));
-        } else {
-          qv[i + u * kThreads] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
-                                            pack2<T>(v[6], v[7]));
-        }
-      }
+      for (int e = 0; e < V; ++e) v[e] *= c;
+      if constexpr (sizeof(T) == 4)
+        qv[i + u * kThreads] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      else
+        qv[i + u * kThreads] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     }
   }
-  for (int i = threadIdx.x; i < n - vecs * V; i += kThreads) {
-    const int at = i < head ? i : vecs * V + i;
-    q[at] = from_f<T>(to_f<T>(p[at]) * c);
-  }
+  for (int i = threadIdx.x; i < cut.rest; i += kThreads) q[cut.single(i)] = from_f<T>(to_f<T>(p[cut.single(i)]) * c);
 }
 
 // The norm from the partial results, then every tensor times the coefficient. Tensors written in place are left alone
-// where the coefficient is 1. The chunks are walked from the last one: those are still in the L2.
+// where the coefficient is 1.
 template <int KIND, int CAP>
-__global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* partial,
-                                                              int parts, float max_norm, float* norm_out) {
+__global__ void __launch_bounds__(kThreads, kPerSm) grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* partial,
+                                                                      int parts, float max_norm, float* norm_out) {
   __shared__ double red[kThreads / 32];
   grid_dep_wait();
   double v = 0.0;
@@ -189,17 +217,14 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
   float c = max_norm / (norm + 1e-6f);
   c = c > 1.0f ? 1.0f : c;                               // a NaN stays
-  for (int k = t.first[t.n] - 1 - (int)blockIdx.x; k >= 0; k -= gridDim.x) {
-    const int i = tensor_of(t, k);
+  const int lo = first_unit(t, blockIdx.x), hi = first_unit(t, blockIdx.x + 1);
+  if (lo >= hi) return;
+  for (int i = tensor_of(t, hi - 1); i >= 0 && t.first[i + 1] > lo; --i) {
     if (c == 1.0f && t.src[i] == t.dst[i]) continue;
-    const int64_t at = (int64_t)(k - t.first[i]) * t.chunk;
-    const int n = (int)min((int64_t)t.chunk, t.size[i] - at);
-    if (t.dtype[i] == GLAD_DTYPE_F32)
-      scale_chunk(static_cast<const float*>(t.src[i]) + at, static_cast<float*>(t.dst[i]) + at, n, c);
-    else if (t.dtype[i] == GLAD_DTYPE_F16)
-      scale_chunk(static_cast<const __half*>(t.src[i]) + at, static_cast<__half*>(t.dst[i]) + at, n, c);
-    else
-      scale_chunk(static_cast<const __nv_bfloat16*>(t.src[i]) + at, static_cast<__nv_bfloat16*>(t.dst[i]) + at, n, c);
+    part_of(t, i, lo, hi, [&](auto type, int64_t at, int n) {
+      using T = decltype(type);
+      scale_part(static_cast<const T*>(t.src[i]) + at, static_cast<T*>(t.dst[i]) + at, n, c);
+    });
   }
 }
 
@@ -212,26 +237,22 @@ struct Call {
   float max_norm;
   float* norm;
   double* partial;
-  int chunk;
 };
 
 // Tensors [from, from + CAP) as a table; returns where the next one starts (empty tensors take no place).
 template <int CAP>
 int fill(Table<CAP>& t, const Call& c, int from) {
   int n = 0;
-  int64_t chunks = 0;
+  int64_t units = 0;
   t.first[0] = 0;
-  t.chunk = c.chunk;
   for (; from < c.n && n < CAP; ++from) {
     if (c.sizes[from] == 0) continue;
-    const int64_t more = (c.sizes[from] + c.chunk - 1) / c.chunk;
-    if (chunks + more > 0x7fffffff) break;
+    units += (c.sizes[from] + kUnit - 1) / kUnit;
     t.src[n] = c.src[from];
     t.dst[n] = c.dst ? c.dst[from] : nullptr;
     t.size[n] = c.sizes[from];
     t.dtype[n] = (uint8_t)c.dtypes[from];
-    chunks += more;
-    t.first[++n] = (int32_t)chunks;
+    t.first[++n] = (int32_t)units;
   }
   t.n = n;
   return from;
@@ -239,7 +260,7 @@ int fill(Table<CAP>& t, const Call& c, int from) {
 
 template <int KIND, int CAP>
 cudaError_t launch(const Call& c, cudaStream_t st) {
-  int limit = 8 * num_sms();
+  int limit = kPerSm * num_sms();
   if (limit > kMaxBlocks) limit = kMaxBlocks;
   Table<CAP> t;
   int parts = 0;
@@ -260,7 +281,7 @@ cudaError_t launch(const Call& c, cudaStream_t st) {
       t.first[0] = 0;
     }
     if (!first && t.n == 0) break;
-    const int chunks = t.first[t.n], blocks = chunks < 1 ? 1 : chunks < limit ? chunks : limit;
+    const int units = t.first[t.n], blocks = units < 1 ? 1 : units < limit ? units : limit;
     e = launch_k(grad_scale_kernel<KIND, CAP>, dim3(blocks), dim3(kThreads), 0, st, true, t, (const double*)c.partial,
                  parts, c.max_norm, first ? c.norm : (float*)nullptr);
     first = false;
@@ -270,7 +291,25 @@ cudaError_t launch(const Call& c, cudaStream_t st) {
 
 template <int KIND>
 cudaError_t launch(const Call& c, cudaStream_t st) {
-  return c.n <= kSmall ? launch<KIND, kSmall>(c, st) : launch<KIND, kBig>(c, st);
+  // a table no larger than needed: its bytes are part of a launch
+  return c.n <= 64 ? launch<KIND, 64>(c, st) : c.n <= 320 ? launch<KIND, 320>(c, st) : launch<KIND, kMost>(c, st);
+}
+
+// Whether a tensor that is written (or read) lies over another one; dst[i] may be src[i].
+bool shared(const void* const* src, void* const* dst, const int64_t* sizes, const int32_t* dtypes, int n) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> blocks;
+  blocks.reserve(2 * (size_t)n);
+  for (int i = 0; i < n; ++i) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(src[i]), b = reinterpret_cast<uintptr_t>(dst[i]);
+    const uintptr_t bytes = (uintptr_t)sizes[i] * width_of(dtypes[i]);
+    if (bytes == 0) continue;
+    blocks.emplace_back(a, a + bytes);
+    if (a != b) blocks.emplace_back(b, b + bytes);
+  }
+  std::sort(blocks.begin(), blocks.end());
+  for (size_t i = 1; i < blocks.size(); ++i)
+    if (blocks[i].first < blocks[i - 1].second) return true;
+  return false;
 }
 
 int call(const char* who, const void* const* src, void* const* dst, const int64_t* sizes, const int32_t* dtypes, int n,
@@ -282,19 +321,17 @@ int call(const char* who, const void* const* src, void* const* dst, const int64_
   int64_t total = 0;
   for (int i = 0; i < n; ++i) {
     if (!is_float(dtypes[i])) return bad(who, "a tensor is not f32, f16 or bf16");
-    if (sizes[i] < 0 || sizes[i] > (int64_t)1 << 40) return bad(who, "a tensor's size must be in [0, 2^40]");
+    if (sizes[i] < 0 || sizes[i] > (int64_t)1 << 38) return bad(who, "a tensor's size must be in [0, 2^38]");
     if (sizes[i] && (!src[i] || (dst && !dst[i]))) return bad(who, "a tensor is not set");
     if (!on(src[i], width_of(dtypes[i])) || (dst && !on(dst[i], width_of(dtypes[i]))))
       return bad(who, "a tensor is not element-aligned");
     total += sizes[i];
-    if (total > (int64_t)1 << 50) return bad(who, "more than 2^50 elements");
+    if (total > (int64_t)1 << 38) return bad(who, "more than 2^38 elements");
   }
+  if (dst && shared(src, dst, sizes, dtypes, n)) return bad(who, "two of the tensors share memory");
   if (!workspace || workspace_bytes < glad_grad_norm_workspace_size(n) || !on(workspace, 8))
     return set_last_error(GLAD_ERR_WORKSPACE, "a workspace of glad_grad_norm_workspace_size bytes is required");
-  Call c{src, dst, sizes, dtypes, n, max_norm, norm, static_cast<double*>(workspace), 2048};
-  // Chunks of 2048 elements spread small calls over the GPU; larger ones, up to 32768, have less to look up.
-  while (c.chunk < 32768 && total / c.chunk > 8 * 1184) c.chunk *= 2;
-  while (total / c.chunk > 0x40000000) c.chunk *= 2;
+  const Call c{src, dst, sizes, dtypes, n, max_norm, norm, static_cast<double*>(workspace)};
   const cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = norm_type == 0 ? launch<kInf>(c, st) : norm_type == 1 ? launch<kOne>(c, st) : launch<kTwo>(c, st);
   return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
@@ -308,7 +345,7 @@ using namespace glad;
 extern "C" {
 
 size_t glad_grad_norm_workspace_size(int n) {
-  const int launches = n <= kSmall ? 1 : (n + kBig - 1) / kBig;
+  const int launches = (n + kMost - 1) / kMost;
   return (size_t)(launches + 1) * kMaxBlocks * sizeof(double);
 }
 
@@ -322,8 +359,12 @@ int glad_clip_grads(const void* const* grads, void* const* outs, const int64_t* 
                     int norm_type, float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   if (n > 0 && !outs) return bad("glad_clip_grads", "outs must be set");
   static void* const none[1] = {nullptr};
-  return call("glad_clip_grads", grads, outs ? outs : none, sizes, dtypes, n, norm_type, max_norm, norm, workspace,
-              workspace_bytes, stream);
+  try {
+    return call("glad_clip_grads", grads, outs ? outs : none, sizes, dtypes, n, norm_type, max_norm, norm, workspace,
+                workspace_bytes, stream);
+  } catch (const std::bad_alloc&) {
+    return bad("glad_clip_grads", "out of host memory");
+  }
 }
 
 }  // extern "C"

@@ -10,13 +10,16 @@ the GPU. The coefficient stays on it, so a step with clipping can be captured in
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 
 import torch
+from torch import Tensor
 
 from . import _native as N
 
 _CODE = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 _KIND = {2.0: 2, 1.0: 1, float("inf"): 0}
+_dtype, _shape, _requires_grad = attrgetter("dtype"), attrgetter("shape"), attrgetter("requires_grad")
 
 
 def _kind(norm_type) -> int:
@@ -27,30 +30,34 @@ def _kind(norm_type) -> int:
 
 
 def _tensors(grads, what):
-    if isinstance(grads, torch.Tensor):
+    if isinstance(grads, Tensor):
         return [grads]
     grads = list(grads)
     for t in grads:
-        if not isinstance(t, torch.Tensor):
+        if not isinstance(t, Tensor):
             raise TypeError(f"{what} must be tensors, got {type(t).__name__}")
     return grads
 
 
 def _check(grads):
-    """One device and known types; the type codes."""
-    codes = array("i")
-    dev = grads[0].device
+    """One CUDA device and known types; the type codes. (Whole lists at a time: the host's share of a call with hundreds of
+    tensors is several times the kernels'.)"""
+    dtypes = set(map(_dtype, grads))
+    for dt in dtypes:
+        if dt not in _CODE:
+            raise TypeError(f"a gradient is {dt}; expected float32, float16 or bfloat16")
     for t in grads:
-        code = _CODE.get(t.dtype)
-        if code is None:
-            raise TypeError(f"a gradient is {t.dtype}; expected float32, float16 or bfloat16")
         if t.layout is not torch.strided:
             raise TypeError(f"a gradient is {t.layout}; expected a dense one")
-        if t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-        codes.append(code)
-    N.require_cuda(grads[0])
-    return codes
+    dev = grads[0].device
+    if len(set(map(Tensor.get_device, grads))) != 1 or dev.type != "cuda":
+        for t in grads:
+            if t.device != dev:
+                raise ValueError(f"tensors on {dev} and {t.device}")
+        N.require_cuda(grads[0])
+    if len(dtypes) == 1:
+        return array("i", (_CODE[grads[0].dtype],)) * len(grads)
+    return array("i", [_CODE[dt] for dt in map(_dtype, grads)])
 
 
 def _dense(t) -> bool:
@@ -65,6 +72,13 @@ def _dense(t) -> bool:
     return True
 
 
+def _all_dense(grads):
+    """The tensors as dense ones, and whether they all were contiguous."""
+    if all(map(Tensor.is_contiguous, grads)):
+        return grads, True
+    return [t if _dense(t) else t.contiguous() for t in grads], False
+
+
 def _overlapping(t) -> bool:
     return t.numel() > 1 and any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape))
 
@@ -73,19 +87,11 @@ def _address(table) -> int:
     return table.buffer_info()[0]
 
 
-def _refuse_shared(blocks):
-    """No two tensors of a call that writes may share memory."""
-    blocks.sort()
-    for (_, end), (start, _) in zip(blocks, blocks[1:]):
-        if start < end:
-            raise ValueError("two of the tensors share memory")
-
-
 def _run(grads, codes, outs, kind, max_norm):
     """The norm; ``outs`` None or where the clipped gradients go (dense, like the gradients)."""
     dev, n = grads[0].device, len(grads)
-    src = array("Q", [t.data_ptr() for t in grads])
-    sizes = array("q", [t.numel() for t in grads])
+    src = array("Q", map(Tensor.data_ptr, grads))
+    sizes = array("q", map(Tensor.numel, grads))
     lib = N.load()
     ws = torch.empty(lib.glad_grad_norm_workspace_size(n), dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
@@ -93,7 +99,7 @@ def _run(grads, codes, outs, kind, max_norm):
         rc = N.on_device(lib.glad_grad_norm, dev.index, _address(src), _address(sizes), _address(codes), n, kind,
                          norm.data_ptr(), ws.data_ptr(), ws.numel())
     else:
-        dst = src if outs is grads else array("Q", [t.data_ptr() for t in outs])
+        dst = src if outs is grads else array("Q", map(Tensor.data_ptr, outs))
         rc = N.on_device(lib.glad_clip_grads, dev.index, _address(src), _address(dst), _address(sizes), _address(codes), n,
                          kind, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel())
     if rc:
@@ -103,7 +109,9 @@ def _run(grads, codes, outs, kind, max_norm):
 
 def _written(tensors):
     """Tell autograd, as torch's in-place operators do (inference tensors have no version)."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    if any(map(Tensor.is_inference, tensors)):
+        tensors = [t for t in tensors if not t.is_inference()]
+    torch.autograd.graph.increment_version(tensors)
 
 
 def _max_norm(value) -> float:
@@ -115,7 +123,7 @@ def _max_norm(value) -> float:
 
 def _refuse_grad(what, tensors):
     N.refuse_tangents(what, *tensors)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(map(_requires_grad, tensors)):
         raise RuntimeError(f"{what} has no gradient; use torch.no_grad()")
 
 
@@ -128,7 +136,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
         return torch.tensor(0.0)
     _refuse_grad("grad_norm", grads)
     codes = _check(grads)
-    return _run([t if _dense(t) else t.contiguous() for t in grads], codes, None, kind, 0.0)
+    return _run(_all_dense(grads)[0], codes, None, kind, 0.0)
 
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
@@ -145,23 +153,20 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
     if given is not None:
         _refuse_grad("clip_grads", given)
     codes = _check(grads)
-    grads = [t if _dense(t) else t.contiguous() for t in grads]
+    grads, whole = _all_dense(grads)
     if given is None:
         given = [torch.empty_like(t) for t in grads]
         return given, _run(grads, codes, given, kind, max_norm)
-    blocks = []
-    for t, o in zip(grads, given):
-        if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.layout is not torch.strided:
-            raise ValueError(f"out {tuple(o.shape)} {o.dtype} on {o.device} does not match the gradient {tuple(t.shape)} "
-                             f"{t.dtype} on {t.device}")
-        if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
-            raise ValueError(f"out has strides {o.stride()}, the gradient {t.stride()}")
-        at, size = t.data_ptr(), t.numel() * t.element_size()
-        if size:
-            blocks.append((at, at + size))
-            if o.data_ptr() != at:
-                blocks.append((o.data_ptr(), o.data_ptr() + size))
-    _refuse_shared(blocks)
+    if list(map(_shape, given)) != list(map(_shape, grads)) or list(map(_dtype, given)) != list(map(_dtype, grads)) or \
+            set(map(Tensor.get_device, given)) != {grads[0].get_device()}:
+        for t, o in zip(grads, given):
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+                raise ValueError(f"out {tuple(o.shape)} {o.dtype} on {o.device} does not match the gradient {tuple(t.shape)} "
+                                 f"{t.dtype} on {t.device}")
+    if not (whole and all(map(Tensor.is_contiguous, given))):
+        for t, o in zip(grads, given):
+            if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
+                raise ValueError(f"out has strides {o.stride()}, the gradient {t.stride()}")
     norm = _run(grads, codes, given, kind, max_norm)
     _written(given)
     return given, norm
@@ -175,19 +180,17 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
         return torch.tensor(0.0)
     N.refuse_tangents("clip_grads_", *grads)
     codes = _check(grads)
-    blocks, whole, strided = [], [], []
-    for t in grads:
-        if _dense(t):
-            at = t.data_ptr()
-            if t.numel():
-                blocks.append((at, at + t.numel() * t.element_size()))
-            whole.append(t)
-        elif _overlapping(t):
-            raise ValueError(f"a gradient of strides {t.stride()} has elements that share memory")
-        else:
-            whole.append(t.contiguous())
-            strided.append((t, whole[-1]))
-    _refuse_shared(blocks)
+    whole, strided = grads, []
+    if not all(map(Tensor.is_contiguous, grads)):
+        whole = []
+        for t in grads:
+            if _dense(t):
+                whole.append(t)
+            elif _overlapping(t):
+                raise ValueError(f"a gradient of strides {t.stride()} has elements that share memory")
+            else:
+                whole.append(t.contiguous())
+                strided.append((t, whole[-1]))
     norm = _run(whole, codes, whole, kind, max_norm)
     for t, c in strided:
         t.copy_(c)

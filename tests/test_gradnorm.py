@@ -258,17 +258,44 @@ def test_refusals():
         grad_norm([leaf])
 
 
-def test_shared_memory_is_found(monkeypatch):
-    monkeypatch.setattr(gradnorm.N, "require_cuda", lambda *t: None)
-    x = torch.ones(10)
+@gpu
+def test_shared_memory_is_refused():
+    x = torch.ones(10, device="cuda")
     for ts in ([x, x], [x[:6], x[5:]]):
         with pytest.raises(ValueError, match="share memory"):
             clip_grads_(ts, 1.0)
     with pytest.raises(ValueError, match="share memory"):
-        clip_grads_([torch.ones(1).expand(4)], 1.0)
+        clip_grads_([torch.ones(1, device="cuda").expand(4)], 1.0)
+    five = torch.ones(5, device="cuda")
     with pytest.raises(ValueError, match="share memory"):
-        clip_grads([x[:5], torch.ones(5)], 1.0, out=[torch.ones(5), x[4:9]])
+        clip_grads([x[:5], five], 1.0, out=[five.clone(), x[4:9]])
+    assert (x == 1).all()
+    out, n = clip_grads([x[:5], x[5:]], 1.0, out=[x[:5], x[5:]])        # in place
+    assert torch.allclose(x, torch.full_like(x, 10 ** -0.5), rtol=1e-6)
     with pytest.raises(ValueError, match="does not match"):
-        clip_grads([x], 1.0, out=[torch.ones(9)])
+        clip_grads([x], 1.0, out=[x[:9]])
+    with pytest.raises(ValueError, match="does not match"):
+        clip_grads([x], 1.0, out=[torch.ones(10)])
     with pytest.raises(ValueError, match="strides"):
-        clip_grads([torch.ones(3, 4)], 1.0, out=[torch.ones(4, 3).t()])
+        clip_grads([torch.ones(3, 4, device="cuda")], 1.0, out=[torch.ones(4, 3, device="cuda").t()])
+
+
+def test_the_library_finds_shared_memory():
+    """The C entry's own check, on host addresses that nothing reads: it comes before any launch."""
+    import ctypes
+
+    from rl_quant_b200 import _native as N
+    buf = ctypes.create_string_buffer(4096)
+    at = (ctypes.addressof(buf) + 255) // 256 * 256
+    lib = N.load()
+
+    def call(src, dst, sizes):
+        n = len(src)
+        arr = lambda t, v: (t * n)(*v)  # noqa: E731
+        return lib.glad_clip_grads(arr(ctypes.c_uint64, src), arr(ctypes.c_uint64, dst), arr(ctypes.c_int64, sizes),
+                                   arr(ctypes.c_int32, [N.DTYPE_F32] * n), n, 2, 1.0, at + 2048, None, 0, None)
+    for src, dst, sizes in (([at, at], [at, at], [4, 4]), ([at, at + 12], [at, at + 12], [4, 4]),
+                            ([at, at + 64], [at + 128, at + 64], [40, 4]), ([at], [at + 8], [4])):
+        assert call(src, dst, sizes) == N.GLAD_ERR_INVALID_ARG and b"share" in lib.glad_last_error()
+    for src, dst, sizes in (([at, at + 16], [at, at + 16], [4, 4]), ([at, at], [at, at + 64], [0, 4])):
+        assert call(src, dst, sizes) == N.GLAD_ERR_WORKSPACE
