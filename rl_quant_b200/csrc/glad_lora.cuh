@@ -47,6 +47,7 @@ struct Params {
   int64_t ldx, ldb;
   float scale_value;
   int M, K, N, r, L, index64, cluster;
+  int halves;           // a tile of the plan (32 rows) is taken as two of 16
 };
 
 struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
@@ -173,11 +174,14 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
     if (tid < n) rows[tid] = tile * R + tid;
   } else if (p.plan != nullptr) {
     const Plan plan{p.plan, p.L, p.M};
-    if (tile >= plan.tiles()) return 0;
-    const int2 t = plan.tile(tile);
+    const int whole = p.halves ? tile >> 1 : tile;
+    if (whole >= plan.tiles()) return 0;
+    const int2 t = plan.tile(whole);
     adapter = t.x;
-    n = min(R, plan.first((adapter < 0 ? p.L : adapter) + 1) - t.y);
-    if (tid < n) rows[tid] = plan.row(t.y + tid);
+    const int from = t.y + (p.halves ? (tile & 1) * R : 0);
+    n = min(R, plan.first((adapter < 0 ? p.L : adapter) + 1) - from);
+    if (n <= 0) return 0;
+    if (tid < n) rows[tid] = plan.row(from + tid);
   } else {
     // One cluster a row: it is the tile's where R, 2 R, ... rows of the same adapter (none) come before it.
     __shared__ int of[kSelfRows], counts[kWarps];
@@ -209,9 +213,12 @@ constexpr size_t smem_bytes() {
   return (size_t)(kWarps + 1) * 16 * MT * RT * sizeof(float);
 }
 
-// RT: the rank, rounded up to 16, 32, 64 or 128; MT * 16 rows a tile.
-template <typename T, int RT, int MT, bool TRANS, bool VEC>
-__global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_kernel(const Params p) {
+// For tensors off the 16-byte boundaries: operands straight from memory, element by element.
+// RT: the rank, rounded up to 16, 32, 64 or 128; 16 rows a tile.
+template <typename T, int RT, bool TRANS>
+__global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_any_kernel(const Params p) {
+  constexpr int MT = 1;
+  constexpr bool VEC = false;
   constexpr int R = 16 * MT, NT = RT / 8, EL = 16 / (int)sizeof(T), CH = 4 * EL;
   constexpr int E = RT / 4, ST = E / 2;               // ranks of a lane as an operand of y, and their instructions
   extern __shared__ __align__(16) float sm[];
@@ -433,10 +440,42 @@ __global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_kernel(const
   }
 }
 
+// The warps' parts of a gradient tile, [RT][BW] each `step` floats apart, added up and, over the cluster, written.
+template <typename T, int RT, int BW>
+__device__ __forceinline__ void outer_end(const OuterParams& p, float* part, const float* red, int step, int a, int r0, int n0,
+                                          int rank, int C) {
+  const int tid = threadIdx.x;
+  for (int i = tid; i < RT * BW; i += kThreads) {
+    float s = red[i];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) s += red[w * step + i];
+    part[i] = s;
+  }
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  T* out = static_cast<T*>(p.out) + (int64_t)a * p.r * p.K;
+  const uint32_t here = smem_u32(part);
+  const bool by_rank = p.step_r == 1;                  // adjacent threads write adjacent elements
+  for (int i = rank * kThreads + tid; i < RT * BW; i += C * kThreads) {
+    const int k = by_rank ? i % RT : i / BW, col = by_rank ? i / RT : i % BW;
+    const uint32_t src = here + 4 * (k * BW + col);
+    float v;
+    if (C > 1) {
+      v = ld_cluster(mapa_shared(src, 0));
+      for (int c = 1; c < C; ++c) v += ld_cluster(mapa_shared(src, c));
+    } else {
+      v = part[k * BW + col];
+    }
+    if (r0 + k < p.r && n0 + col < p.K) out[(r0 + k) * p.step_r + (int64_t)(n0 + col) * p.step_k] = from_f<T>(v);
+  }
+  if (C > 1) cluster_sync_all();
+}
+
 // RT: ranks of a block, 16 or 32 (blockIdx.z: which). A cluster shares 8 EL columns of one adapter's gradient; its warps split
-// the rows, and the parts are added in a fixed order.
-template <typename T, int RT, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p) {
+// the rows, and the parts are added in a fixed order. For tensors off the 16-byte boundaries.
+template <typename T, int RT>
+__global__ void __launch_bounds__(kThreads, 2) outer_any_kernel(const OuterParams p) {
+  constexpr bool VEC = false;
   constexpr int EL = 16 / (int)sizeof(T), TL = EL, BW = 8 * TL, RM = RT / 16;
   extern __shared__ __align__(16) float sm[];
   float* part = sm;                                    // [RT][BW]
@@ -493,30 +532,526 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p)
       for (int c = 0; c < 4; ++c)
         mine[(16 * k + g + 8 * (c >> 1)) * BW + (2 * q + (c & 1)) * TL + t] = acc[k][t][c];
   __syncthreads();
-  for (int i = tid; i < RT * BW; i += kThreads) {
-    float s = red[i];
+  outer_end<T, RT, BW>(p, part, red, RT * BW, a, r0, n0, rank, C);
+}
+
+// ---- the same from asynchronously filled rings ---------------------------------------------------
+// Every warp copies what it needs next, by itself: 16-byte copies into a ring of its own while it works on the stage before, so
+// the bytes in flight (up to 100 KB an SM) do not depend on registers or on other warps. The pieces are placed so that a
+// fragment's reads touch every bank once.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {       // zeros where not live
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(live ? 8 : 0) : "memory");
+}
+// A row piece of the ranks' direction: `count` pieces of 16 bytes a row, of which those below rank r are copied; f(row, piece) gives
+// the row's address (null: zeros) and where it goes. Ranks off 16 bytes are copied in halves.
+template <typename T, int COUNT, int ROWS, typename F>
+__device__ __forceinline__ void copy_ranks(int lane, int r, int from, F&& f) {
+  constexpr int EL = 16 / (int)sizeof(T);
+  if (r % EL == 0) {
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) s += red[w * RT * BW + i];
-    part[i] = s;
+    for (int j = 0; j < COUNT * ROWS / 32; ++j) {
+      const int id = lane + 32 * j, row = id / COUNT, c = id % COUNT, at = from + c * EL;
+      uint32_t dst;
+      const T* src = f(row, dst);
+      const bool live = src != nullptr && at < r;
+      copy16(dst + 16 * c, live ? src + at : f.any, live);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2 * COUNT * ROWS / 32; ++j) {
+      const int id = lane + 32 * j, row = id / (2 * COUNT), c = id % (2 * COUNT), at = from + c * (EL / 2);
+      uint32_t dst;
+      const T* src = f(row, dst);
+      const bool live = src != nullptr && at < r;
+      copy8(dst + 8 * c, live ? src + at : f.any, live);
+    }
+  }
+}
+template <typename T, typename G>
+struct RankRow {                         // a row's address and place, and some address of the tensor
+  const T* any;
+  G g;
+  __device__ __forceinline__ const T* operator()(int row, uint32_t& dst) const { return g(row, dst); }
+};
+template <typename T, typename G>
+__device__ __forceinline__ RankRow<T, G> rank_row(const T* any, G g) {
+  return {any, g};
+}
+
+template <int N>
+__device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "r"(addr + 4 * i));
+  }
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint32_t w[4];
+  lds(addr, w);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// fp32 numbers as an operand beside rows of T: two bf16 numbers (16 bits) for bf16, whose products then run at the full rate,
+// else two tf32 numbers (22 bits; fp16 pairs would not hold the range of gradients).
+template <typename T>
+constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
+__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  const float2 f = __bfloat1622float2(h);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(fabsf(f.x) < INFINITY ? a - f.x : 0.0f, fabsf(f.y) < INFINITY ? b - f.y : 0.0f);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void mma_pair(float (&c)[4], const uint4& hi, const uint4& lo, uint32_t b0, uint32_t b1) {
+  mma_16<__nv_bfloat16>(c, lo.x, lo.y, lo.z, lo.w, b0, b1);
+  mma_16<__nv_bfloat16>(c, hi.x, hi.y, hi.z, hi.w, b0, b1);
+}
+__device__ __forceinline__ float4 as_f4(const uint4& v) {
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+// One step of a product whose A operand is split, B operand elements b0, b1 of T.
+template <typename T>
+__device__ __forceinline__ void mma_step(float (&c)[4], const uint4& hi, const uint4& lo, float b0, float b1) {
+  if constexpr (sizeof(T) == 4) {
+    mma_split(c, as_f4(hi), as_f4(lo), b0, b1);
+  } else {
+    mma_tf32(c, as_f4(lo), b0, b1);
+    mma_tf32(c, as_f4(hi), b0, b1);
+  }
+}
+
+template <typename T, int RT, int MT>
+struct Ring {
+  static constexpr int SZ = (int)sizeof(T), R = 16 * MT;
+  static constexpr int kStage1 = R * 64 + RT * 64;                    // 64 bytes of every row of x, and as much of A
+  static constexpr int kStages = RT <= 32 ? 4 : RT == 64 ? 3 : 2;
+  static constexpr int PB = RT * SZ < 64 ? RT * SZ : 64, PR = PB / SZ; // bytes and ranks of a piece of a row of B
+  static constexpr int kW2 = 128 / SZ * PB, kBase = R * 128, kSlot = kW2 + kBase;
+  static constexpr int kBytes = kStages * kStage1 > 2 * kSlot ? kStages * kStage1 : 2 * kSlot;     // of a warp
+  static constexpr int kSmem = kWarps * kBytes + R * RT * 4 + R * RT * 8;
+  static_assert(kSlot + R * RT * 4 <= kBytes, "a warp's part of u fits behind the first slot");
+};
+
+template <typename T, int RT, int MT, bool TRANS>
+__global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const Params p) {
+  using L = Ring<T, RT, MT>;
+  constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 4 * EL, S1 = L::kStages;
+  constexpr int PR = L::PR, PB = L::PB, PIECES = RT / PR, E = PR / 4;           // E: a lane's ranks of a piece
+  constexpr int SE = kPairs<T> ? 4 : 2, PS = E / SE, ST = PIECES * PS;          // ranks of a lane, and instructions, a step
+  constexpr int TL = EL, CW = 2 * TL, BW = 8 * TL;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int rows[R];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
+  const uint32_t ring = smem_u32(smem) + warp * L::kBytes;
+  float* part = reinterpret_cast<float*>(smem + kWarps * L::kBytes);            // this block's part of u, [R][RT]
+  uint4* frag = reinterpret_cast<uint4*>(part + R * RT);                        // u as split operands, [MT][ST][32][2]
+  auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * L::kBytes + L::kSlot); };   // warp w's part, [R][RT]
+  grid_dep_wait();
+  int adapter;
+  const int n = find_rows<R>(p, tile, rows, adapter);
+  if (n == 0) return;                                 // the whole cluster
+  const int W = C * kWarps, w0 = rank * kWarps + warp;
+
+  if (adapter >= 0) {
+    const T* xr[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) xr[i] = static_cast<const T*>(p.x) + (int64_t)rows[g + 8 * i] * p.ldx;
+    const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
+    auto fetch = [&](int i) {                          // the warp's chunk number i
+      const int k0 = (w0 + i * W) * CH;
+      if (k0 < p.K) {
+        const uint32_t at = ring + i % S1 * L::kStage1;
+        const int k = k0 + q * EL;
+        const bool live = k < p.K;
+#pragma unroll
+        for (int j = 0; j < 2 * MT; ++j) copy16(at + (g + 8 * j) * 64 + q * 16, live ? xr[j] + k : xr[j], live);
+        const uint32_t wat = at + R * 64;
+        if constexpr (!TRANS) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const bool in = live && 8 * t + g < p.r;
+            copy16(wat + (8 * t + g) * 64 + q * 16, in ? w1 + (int64_t)(8 * t + g) * p.K + k : w1, in);
+          }
+        } else {
+          copy_ranks<T, RT * SZ / 16, CH>(lane, p.r, 0, rank_row(w1, [&](int row, uint32_t& dst) -> const T* {
+            dst = wat + (row % EL * 4 + row / EL) * (RT * SZ);
+            return k0 + row < p.K ? w1 + (int64_t)(k0 + row) * p.r : nullptr;
+          }));
+        }
+      }
+      cp_async_commit();
+    };
+    float acc[MT][NT][4] = {};
+#pragma unroll
+    for (int i = 0; i < S1 - 1; ++i) fetch(i);
+    for (int i = 0; (w0 + i * W) * CH < p.K; ++i) {
+      cp_async_wait_group<S1 - 2>();
+      __syncwarp();
+      const uint32_t at = ring + i % S1 * L::kStage1, wat = at + R * 64;
+      uint32_t xa[2 * MT][4];
+#pragma unroll
+      for (int j = 0; j < 2 * MT; ++j) lds(at + (g + 8 * j) * 64 + q * 16, xa[j]);
+      auto products = [&](int t, const uint32_t (&wb)[4]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            if constexpr (SZ == 4) {
+              float4 ah, al;
+              split4(make_float4(__uint_as_float(xa[2 * m][2 * j]), __uint_as_float(xa[2 * m + 1][2 * j]),
+                                 __uint_as_float(xa[2 * m][2 * j + 1]), __uint_as_float(xa[2 * m + 1][2 * j + 1])), ah, al);
+              mma_split(acc[m][t], ah, al, __uint_as_float(wb[2 * j]), __uint_as_float(wb[2 * j + 1]));
+            } else {
+              mma_16<T>(acc[m][t], xa[2 * m][2 * j], xa[2 * m + 1][2 * j], xa[2 * m][2 * j + 1], xa[2 * m + 1][2 * j + 1],
+                        wb[2 * j], wb[2 * j + 1]);
+            }
+          }
+      };
+      if constexpr (!TRANS) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          uint32_t wb[4];
+          lds(wat + (8 * t + g) * 64 + q * 16, wb);
+          products(t, wb);
+        }
+      } else {
+        constexpr int WN = NT * SZ / 4;                // words of a lane's ranks
+        uint32_t raw[EL][WN];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) lds(wat + (e * 4 + q) * (RT * SZ) + g * NT * SZ, raw[e]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          uint32_t wb[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (SZ == 4) wb[w] = raw[w][t];
+            else wb[w] = pair_of(raw[2 * w][t >> 1], raw[2 * w + 1][t >> 1], t);
+          }
+          products(t, wb);
+        }
+      }
+      __syncwarp();
+      fetch(i + S1 - 1);
+    }
+    cp_async_wait_all();
+    __syncwarp();
+    float* mine = red(warp);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int col = 2 * q + (c & 1), at = TRANS ? col * NT + t : 8 * t + col;
+          mine[(16 * i + g + 8 * (c >> 1)) * RT + at] = acc[i][t][c];
+        }
+  }
+
+  // The second product's operands: base and B of a step (a piece of the ranks of a block of columns).
+  const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(adapter < 0 ? 0 : adapter) * p.N * p.r;
+  const int pieces = adapter < 0 ? 1 : PIECES;
+  const int blocks = p.y == nullptr ? 0 : max(0, ((p.N + BW - 1) / BW - w0 + W - 1) / W), steps = blocks * pieces;
+  auto fetch2 = [&](int s) {
+    if (s < steps) {
+      const int b = s / pieces, pi = s % pieces, n0 = (w0 + b * W) * BW;
+      if (pi == 0 && p.base != nullptr) {
+        const uint32_t at = ring + (b & 1) * L::kSlot + L::kW2;
+#pragma unroll
+        for (int j = 0; j < 4 * MT; ++j) {
+          const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL;
+          const bool live = row < n && col < p.N;
+          const T* src = static_cast<const T*>(p.base);
+          copy16(at + row * 128 + ((c ^ (row & 1)) * 16), live ? src + (int64_t)rows[row] * p.ldb + col : src, live);
+        }
+      }
+      if (adapter >= 0) {
+        const uint32_t at = ring + (s & 1) * L::kSlot;
+        if constexpr (!TRANS) {
+          // column CW (g / 2) + 2 t + g % 2 of the block is tile t's instruction column g: placed at 8 t + g
+          copy_ranks<T, PB / 16, BW>(lane, p.r, pi * PR, rank_row(w2, [&](int row, uint32_t& dst) -> const T* {
+            dst = at + (row % CW / 2 * 8 + row / CW * 2 + (row & 1)) * PB;
+            return n0 + row < p.N ? w2 + (int64_t)(n0 + row) * p.r : nullptr;
+          }));
+        } else {
+#pragma unroll
+          for (int j = 0; j < PR / 4; ++j) {
+            const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL, rk = pi * PR + row;
+            const bool live = rk < p.r && col < p.N;
+            copy16(at + row * 128 + ((c ^ (2 * (row / E))) * 16), live ? w2 + (int64_t)rk * p.N + col : w2, live);
+          }
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  fetch2(0);
+  if (adapter >= 0) {
+    __syncthreads();
+    for (int i = tid; i < R * RT; i += kThreads) {
+      float s = red(0)[i];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) s += red(w)[i];
+      part[i] = s;
+    }
   }
   if (C > 1) cluster_sync_all();
   else __syncthreads();
-  T* out = static_cast<T*>(p.out) + (int64_t)a * p.r * p.K;
-  const uint32_t here = smem_u32(part);
-  const bool by_rank = p.step_r == 1;                  // adjacent threads write adjacent elements
-  for (int i = rank * kThreads + tid; i < RT * BW; i += C * kThreads) {
-    const int k = by_rank ? i % RT : i / BW, col = by_rank ? i / RT : i % BW;
-    const uint32_t src = here + 4 * (k * BW + col);
-    float v;
-    if (C > 1) {
-      v = ld_cluster(mapa_shared(src, 0));
-      for (int c = 1; c < C; ++c) v += ld_cluster(mapa_shared(src, c));
-    } else {
-      v = part[k * BW + col];
+  if (adapter >= 0) {
+    const float s = p.scale ? p.scale[adapter] : p.scale_value;
+    const uint32_t here = smem_u32(part);
+    float* whole = red(0);                             // [R][RT]
+    for (int i = tid; i < R * RT; i += kThreads) {
+      float v;
+      if (C > 1) {
+        v = ld_cluster(mapa_shared(here + 4 * i, 0));
+        for (int c = 1; c < C; ++c) v += ld_cluster(mapa_shared(here + 4 * i, c));
+      } else {
+        v = part[i];
+      }
+      v *= s;
+      whole[i] = v;
+      const int row = i / RT, at = i % RT;
+      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = v;
     }
-    if (r0 + k < p.r && n0 + col < p.K) out[(r0 + k) * p.step_r + (int64_t)(n0 + col) * p.step_k] = from_f<T>(v);
+    __syncthreads();
+    for (int i = tid; i < MT * ST * 32; i += kThreads) {
+      const int l = i & 31, st = (i >> 5) % ST, m = (i >> 5) / ST;
+      const float* v = whole + (16 * m + (l >> 2)) * RT + st / PS * PR + (l & 3) * E + st % PS * SE;
+      uint4 hi, lo;
+      if constexpr (kPairs<T>) {
+        split_bf16(v[0], v[1], hi.x, lo.x);
+        split_bf16(v[8 * RT], v[8 * RT + 1], hi.y, lo.y);
+        split_bf16(v[2], v[3], hi.z, lo.z);
+        split_bf16(v[8 * RT + 2], v[8 * RT + 3], hi.w, lo.w);
+      } else {
+        float4 h, o;
+        split4(make_float4(v[0], v[8 * RT], v[1], v[8 * RT + 1]), h, o);
+        hi = make_uint4(__float_as_uint(h.x), __float_as_uint(h.y), __float_as_uint(h.z), __float_as_uint(h.w));
+        lo = make_uint4(__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w));
+      }
+      frag[2 * i] = hi, frag[2 * i + 1] = lo;
+    }
   }
-  if (C > 1) cluster_sync_all();
+  if (C > 1) cluster_sync_all();                       // nobody reads another block's part any more
+  else __syncthreads();
+
+  const uint32_t fr = smem_u32(frag);
+  float c[MT][TL][4];
+  for (int s = 0; s < steps; ++s) {
+    fetch2(s + 1);
+    cp_async_wait_group<1>();
+    __syncwarp();
+    const int b = s / pieces, pi = s % pieces;
+    if (pi == 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < TL; ++t) c[m][t][0] = c[m][t][1] = c[m][t][2] = c[m][t][3] = 0.0f;
+    }
+    if (adapter >= 0) {
+      const uint32_t at = ring + (s & 1) * L::kSlot;
+      if constexpr (!TRANS) {
+        uint32_t wv[TL][PB / 16];
+#pragma unroll
+        for (int t = 0; t < TL; ++t) lds(at + (t * 8 + g) * PB + q * (PB / 4), wv[t]);
+#pragma unroll
+        for (int j = 0; j < PS; ++j)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint32_t f = fr + 32 * ((m * ST + pi * PS + j) * 32 + lane);
+            const uint4 hi = lds128(f), lo = lds128(f + 16);
+#pragma unroll
+            for (int t = 0; t < TL; ++t) {
+              if constexpr (kPairs<T>) mma_pair(c[m][t], hi, lo, wv[t][2 * j], wv[t][2 * j + 1]);
+              else mma_step<T>(c[m][t], hi, lo, elem<T>(wv[t], 2 * j), elem<T>(wv[t], 2 * j + 1));
+            }
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < PS; ++j) {
+          uint32_t wr[SE][4];
+#pragma unroll
+          for (int e = 0; e < SE; ++e) lds(at + (q * E + SE * j + e) * 128 + ((g ^ (2 * q)) * 16), wr[e]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint32_t f = fr + 32 * ((m * ST + pi * PS + j) * 32 + lane);
+            const uint4 hi = lds128(f), lo = lds128(f + 16);
+#pragma unroll
+            for (int t = 0; t < TL; ++t) {
+              if constexpr (kPairs<T>)
+                mma_pair(c[m][t], hi, lo, pair_of(wr[0][t >> 1], wr[1][t >> 1], t), pair_of(wr[2][t >> 1], wr[3][t >> 1], t));
+              else
+                mma_step<T>(c[m][t], hi, lo, elem<T>(wr[0], t), elem<T>(wr[1], t));
+            }
+          }
+        }
+      }
+    }
+    if (pi == pieces - 1) {
+      const int col = (w0 + b * W) * BW + q * CW;
+      const uint32_t at = ring + (b & 1) * L::kSlot + L::kW2;
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) {
+        const int row = g + 8 * i;
+        if (row >= n) continue;
+        T* y = static_cast<T*>(p.y) + (int64_t)rows[row] * p.N + col;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (col + h * EL >= p.N) continue;
+          uint32_t bw[4] = {0, 0, 0, 0};
+          if (p.base != nullptr) lds(at + row * 128 + (((2 * q + h) ^ (row & 1)) * 16), bw);
+          float o[EL];
+#pragma unroll
+          for (int e = 0; e < EL; ++e) {
+            const int l = h * EL + e;                  // the lane's column
+            const int t = TRANS ? l % TL : l >> 1, odd = TRANS ? l / TL : l & 1;
+            o[e] = c[i >> 1][t][2 * (i & 1) + odd] + elem<T>(bw, e);
+          }
+          if constexpr (SZ == 4)
+            *reinterpret_cast<float4*>(y + h * EL) = make_float4(o[0], o[1], o[2], o[3]);
+          else
+            *reinterpret_cast<uint4*>(y + h * EL) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
+                                                               pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+        }
+      }
+    }
+    __syncwarp();
+  }
+  cp_async_wait_all();
+}
+
+template <typename T, int RT>
+struct OuterRing {
+  static constexpr int kPitch = RT * 4 + (kPairs<T> ? 16 : 32);        // of a row of v: a fragment's reads touch every bank once
+  static constexpr int kStage = 16 * 128 + 16 * kPitch, kStages = RT == 16 ? 3 : 2;
+  static constexpr int kBytes = kStages * kStage;                      // of a warp
+  static constexpr int BW = 128 / (int)sizeof(T);
+  static constexpr int kSmem = kWarps * kBytes + RT * BW * 4;
+  static_assert(RT * BW * 4 <= kBytes, "a warp's part of the gradient fits into its ring");
+};
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p) {
+  using L = OuterRing<T, RT>;
+  constexpr int EL = 16 / (int)sizeof(T), TL = EL, BW = 8 * TL, RM = RT / 16, S = L::kStages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int C = p.cluster, rank = (int)blockIdx.x % C, n0 = (int)blockIdx.x / C * BW;
+  const int a = blockIdx.y, r0 = blockIdx.z * RT;
+  const uint32_t ring = smem_u32(smem) + warp * L::kBytes;
+  grid_dep_wait();
+  const Plan plan{p.plan, p.L, p.M};
+  const int from = p.plan ? plan.first(a) : 0, rows = p.plan ? plan.first(a + 1) - from : p.M;
+  const int W = C * kWarps, w0 = rank * kWarps + warp;
+  // lanes 0 .. 15: the rows of the warp's group number i of 16 (-1: none)
+  auto index_of = [&](int i) {
+    const int at = (w0 + i * W) * 16 + lane;
+    return lane < 16 && at < rows ? p.plan ? plan.row(from + at) : at : -1;
+  };
+  int next = index_of(0);
+  auto fetch = [&](int i) {
+    const int mine = next;
+    next = index_of(i + 1);
+    if ((w0 + i * W) * 16 < rows) {
+      const uint32_t at = ring + i % S * L::kStage;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL;
+        const int m = __shfl_sync(0xffffffffu, mine, row);
+        const bool live = m >= 0 && col < p.K;
+        const T* x = static_cast<const T*>(p.x);
+        const int turn = kPairs<T> ? row >> 1 & 3 : row & 3;           // a fragment's four rows at four places
+        copy16(at + row * 128 + ((c ^ (2 * turn)) * 16), live ? x + (int64_t)m * p.ldx + col : x, live);
+      }
+#pragma unroll
+      for (int j = 0; j < RT / 8; ++j) {
+        const int id = lane + 32 * j, row = id / (RT / 4), c = id % (RT / 4), rk = r0 + 4 * c;
+        const int m = __shfl_sync(0xffffffffu, mine, row);
+        const bool live = m >= 0 && rk < p.r;
+        copy16(at + 2048 + row * L::kPitch + 16 * c, live ? p.v + (int64_t)m * p.r + rk : p.v, live);
+      }
+    }
+    cp_async_commit();
+  };
+  float acc[RM][TL][4] = {};
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i);
+  for (int i = 0; (w0 + i * W) * 16 < rows; ++i) {
+    cp_async_wait_group<S - 2>();
+    __syncwarp();
+    const uint32_t at = ring + i % S * L::kStage, vat = at + 2048;
+    auto v_at = [&](int m, int rk) {
+      uint32_t w[1];
+      lds(vat + m * L::kPitch + 4 * rk, w);
+      return __uint_as_float(w[0]);
+    };
+    if constexpr (kPairs<T>) {
+      uint32_t xw[4][4];                               // rows 2 q, 2 q + 1, 2 q + 8, 2 q + 9
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lds(at + (2 * q + (e & 1) + 8 * (e >> 1)) * 128 + ((g ^ (2 * q)) * 16), xw[e]);
+#pragma unroll
+      for (int k = 0; k < RM; ++k) {
+        uint4 hi, lo;
+        const int rk = 16 * k + g;
+        split_bf16(v_at(2 * q, rk), v_at(2 * q + 1, rk), hi.x, lo.x);
+        split_bf16(v_at(2 * q, rk + 8), v_at(2 * q + 1, rk + 8), hi.y, lo.y);
+        split_bf16(v_at(2 * q + 8, rk), v_at(2 * q + 9, rk), hi.z, lo.z);
+        split_bf16(v_at(2 * q + 8, rk + 8), v_at(2 * q + 9, rk + 8), hi.w, lo.w);
+#pragma unroll
+        for (int t = 0; t < TL; ++t)
+          mma_pair(acc[k][t], hi, lo, pair_of(xw[0][t >> 1], xw[1][t >> 1], t), pair_of(xw[2][t >> 1], xw[3][t >> 1], t));
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                    // rows 8 h + q and 8 h + q + 4
+        uint32_t x0[4], x1[4];
+        lds(at + (8 * h + q) * 128 + ((g ^ (2 * q)) * 16), x0);
+        lds(at + (8 * h + q + 4) * 128 + ((g ^ (2 * q)) * 16), x1);
+#pragma unroll
+        for (int k = 0; k < RM; ++k) {
+          const int rk = 16 * k + g, m = 8 * h + q;
+          float4 ah, al;
+          split4(make_float4(v_at(m, rk), v_at(m, rk + 8), v_at(m + 4, rk), v_at(m + 4, rk + 8)), ah, al);
+#pragma unroll
+          for (int t = 0; t < TL; ++t) {
+            const float b0 = elem<T>(x0, t), b1 = elem<T>(x1, t);
+            if constexpr (sizeof(T) == 4) {
+              mma_split(acc[k][t], ah, al, b0, b1);
+            } else {
+              mma_tf32(acc[k][t], al, b0, b1);
+              mma_tf32(acc[k][t], ah, b0, b1);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    fetch(i + S - 1);
+  }
+  cp_async_wait_all();
+  __syncwarp();
+  float* mine = reinterpret_cast<float*>(smem + warp * L::kBytes);
+#pragma unroll
+  for (int k = 0; k < RM; ++k)
+#pragma unroll
+    for (int t = 0; t < TL; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        mine[(16 * k + g + 8 * (c >> 1)) * BW + (2 * q + (c & 1)) * TL + t] = acc[k][t][c];
+  __syncthreads();
+  outer_end<T, RT, BW>(p, reinterpret_cast<float*>(smem + kWarps * L::kBytes), reinterpret_cast<const float*>(smem),
+                       L::kBytes / 4, a, r0, n0, rank, C);
 }
 
 template <typename F, typename P>
@@ -541,7 +1076,7 @@ cudaError_t launch_clusters(F* kernel, const P& p, dim3 grid, size_t smem, cudaS
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-// Rows of a tile: 16 where an adapter has no more on average, or where 32 need too many registers.
+// Rows of a tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
 inline int tile_rows(int64_t M, int L, int r, bool indexed) {
   if (r > 64) return 16;
   return M > 16 * (int64_t)(indexed ? L : 1) ? 32 : 16;
@@ -555,40 +1090,53 @@ inline int64_t max_tiles(int64_t M, int L, int r, bool indexed, bool planned) {
 }
 
 template <typename T, int RT, int MT, bool TRANS>
-cudaError_t launch_rt(const Params& p, int64_t tiles, bool vec, cudaStream_t st) {
-  const dim3 grid((unsigned)(tiles * p.cluster));
-  if (vec) return launch_clusters(lora_kernel<T, RT, MT, TRANS, true>, p, grid, smem_bytes<RT, MT>(), st);
-  return launch_clusters(lora_kernel<T, RT, MT, TRANS, false>, p, grid, smem_bytes<RT, MT>(), st);
+cudaError_t launch_ring(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
+  // blocks of a tile: while the tiles alone do not fill the GPU's places
+  const int places = (RT == 16 ? 2 : 1) * num_sms();
+  p.cluster = 1;
+  while (p.cluster < 8 && likely * p.cluster * 2 <= places) p.cluster *= 2;
+  return launch_clusters(lora_kernel<T, RT, MT, TRANS>, p, dim3((unsigned)(tiles * p.cluster)), Ring<T, RT, MT>::kSmem, st);
+}
+template <typename T, int RT, bool TRANS>
+cudaError_t launch_any(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
+  p.cluster = 1;
+  while (p.cluster < 8 && likely * p.cluster * 2 <= 2 * num_sms()) p.cluster *= 2;
+  return launch_clusters(lora_any_kernel<T, RT, TRANS>, p, dim3((unsigned)(tiles * p.cluster)), smem_bytes<RT, 1>(), st);
 }
 
-// The kernel for p's type, rank and rows; vec: every access on its boundary.
+// Whether every access of the ring kernels is on its boundary.
 template <typename T>
-cudaError_t run(Params p, bool trans, cudaStream_t st) {
+bool aligned(const Params& p) {
+  constexpr int EL = 16 / (int)sizeof(T);
+  return p.K % EL == 0 && p.N % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && on(p.w1, 16) && on(p.w2, 16) &&
+         on(p.base, 16) && (p.M <= 1 || p.ldb % EL == 0) && on(p.y, 16) && p.r % (EL / 2) == 0;
+}
+
+template <typename T, bool TRANS>
+cudaError_t run_as(const Params& p, cudaStream_t st) {
   const bool indexed = p.index != nullptr;
   const int R = tile_rows(p.M, p.L, p.r, indexed);
   const int64_t tiles = max_tiles(p.M, p.L, p.r, indexed, p.plan != nullptr);
-  const int64_t real = (p.M + R - 1) / R;
-  p.cluster = 1;
-  while (p.cluster < 8 && real * p.cluster * 2 <= 3 * num_sms()) p.cluster *= 2;
-  const int RT = p.r <= 16 ? 16 : p.r <= 32 ? 32 : p.r <= 64 ? 64 : 128, EL = 16 / (int)sizeof(T);
-  const bool vec = p.K % EL == 0 && p.N % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && on(p.w1, 16) &&
-                   on(p.w2, 16) && on(p.base, 16) && (p.M <= 1 || p.ldb % EL == 0) && on(p.y, 16) && p.r % (RT / 4) == 0;
-#define GLAD_LORA(RT_, MT_) \
-  return trans ? launch_rt<T, RT_, MT_, true>(p, tiles, vec, st) : launch_rt<T, RT_, MT_, false>(p, tiles, vec, st)
-  if (RT == 16) {
-    if (R == 32) GLAD_LORA(16, 2);
-    GLAD_LORA(16, 1);
+  int64_t likely = (p.M + R - 1) / R + (indexed ? p.L - 1 : 0);
+  if (likely > p.M) likely = p.M;
+  if (aligned<T>(p)) {
+    if (p.r <= 16) return R == 32 ? launch_ring<T, 16, 2, TRANS>(p, tiles, likely, st) : launch_ring<T, 16, 1, TRANS>(p, tiles, likely, st);
+    if (p.r <= 32) return R == 32 ? launch_ring<T, 32, 2, TRANS>(p, tiles, likely, st) : launch_ring<T, 32, 1, TRANS>(p, tiles, likely, st);
+    if (p.r <= 64) return R == 32 ? launch_ring<T, 64, 2, TRANS>(p, tiles, likely, st) : launch_ring<T, 64, 1, TRANS>(p, tiles, likely, st);
+    return launch_ring<T, 128, 1, TRANS>(p, tiles, likely, st);
   }
-  if (RT == 32) {
-    if (R == 32) GLAD_LORA(32, 2);
-    GLAD_LORA(32, 1);
-  }
-  if (RT == 64) {
-    if (R == 32) GLAD_LORA(64, 2);
-    GLAD_LORA(64, 1);
-  }
-  GLAD_LORA(128, 1);
-#undef GLAD_LORA
+  // 16 rows a tile: the plan's tiles of 32 in two
+  Params h = p;
+  h.halves = R == 32 && p.plan != nullptr;
+  const int64_t all = h.halves ? 2 * tiles : indexed ? tiles : (p.M + 15) / 16;
+  if (p.r <= 16) return launch_any<T, 16, TRANS>(h, all, likely, st);
+  if (p.r <= 32) return launch_any<T, 32, TRANS>(h, all, likely, st);
+  if (p.r <= 64) return launch_any<T, 64, TRANS>(h, all, likely, st);
+  return launch_any<T, 128, TRANS>(h, all, likely, st);
+}
+template <typename T>
+cudaError_t run(Params p, bool trans, cudaStream_t st) {
+  return trans ? run_as<T, true>(p, st) : run_as<T, false>(p, st);
 }
 
 template <typename T>
@@ -596,16 +1144,16 @@ cudaError_t run_outer(OuterParams p, cudaStream_t st) {
   constexpr int EL = 16 / (int)sizeof(T), BW = 8 * EL;
   const int RT = p.r <= 16 ? 16 : 32;
   const int64_t rows = p.plan ? (p.M + p.L - 1) / p.L : p.M;       // of an adapter, on average
+  const int64_t tiles = (int64_t)((p.K + BW - 1) / BW) * p.L * ((p.r + RT - 1) / RT);
   p.cluster = 1;
-  while (p.cluster < 8 && rows >= (int64_t)p.cluster * 2 * 64) p.cluster *= 2;
-  const bool vec = p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0);
+  while (p.cluster < 8 && rows >= (int64_t)p.cluster * 2 * kWarps * 16 && tiles * p.cluster * 2 <= 2 * num_sms()) p.cluster *= 2;
   const dim3 grid((unsigned)((p.K + BW - 1) / BW * p.cluster), (unsigned)p.L, (unsigned)((p.r + RT - 1) / RT));
+  if (p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && on(p.v, 16) && p.r % 4 == 0)
+    return RT == 16 ? launch_clusters(outer_kernel<T, 16>, p, grid, OuterRing<T, 16>::kSmem, st)
+                    : launch_clusters(outer_kernel<T, 32>, p, grid, OuterRing<T, 32>::kSmem, st);
   const size_t smem = (size_t)(kWarps + 1) * RT * BW * sizeof(float);
-  if (RT == 16)
-    return vec ? launch_clusters(outer_kernel<T, 16, true>, p, grid, smem, st)
-               : launch_clusters(outer_kernel<T, 16, false>, p, grid, smem, st);
-  return vec ? launch_clusters(outer_kernel<T, 32, true>, p, grid, smem, st)
-             : launch_clusters(outer_kernel<T, 32, false>, p, grid, smem, st);
+  return RT == 16 ? launch_clusters(outer_any_kernel<T, 16>, p, grid, smem, st)
+                  : launch_clusters(outer_any_kernel<T, 32>, p, grid, smem, st);
 }
 
 }  // namespace lora

@@ -3,8 +3,8 @@
 Tolerances, fixed before the first run. One matrix instruction adds up to 17 terms aligned to the largest, each off by at most
 2^-24 of it: 2^-20 of the running sum of magnitudes. A warp runs at most K / 64 + 2 of them for u (the 16-bit products are
 exact; split fp32 ones are off by 2^-20), and the joins of warps and blocks add at most 16 roundings: so u is off by (K / 64 + 20) 2^-20 sum |x| |A|.
-In y each term of u counts with its own error, splitting u is off by 2^-21, and at most 3 r / 8 + 2 instructions follow; the rounding to
-the type is half a step. The gradients are the same sums with other operands; rows of an adapter take the place of K.
+In y each term of u counts with its own error, splitting u is off by 2^-21 (two tf32 numbers) or 2^-17 (two bf16 ones beside
+bf16 rows), and at most 3 r / 8 + 2 instructions follow; the rounding to the type is half a step. The gradients are the same sums with other operands; rows of an adapter take the place of K.
 Inputs of one sign make the sums of magnitudes the sums themselves."""
 import math
 
@@ -67,7 +67,8 @@ def ref(x, a, b, i, scale, base, dy):
         U, V = s * X @ A.T, s * G @ B
         U1, V1 = s * X.abs() @ A.abs().T, s * G.abs() @ B.abs()
         eU, eV = (k / 64 + 21) * S * U1, (n / 64 + 21) * S * V1
-        more, many = (3 * r / 8 + 3) * S, (3 * len(rows) / 8 + 20) * S
+        split = 8 if x.dtype == torch.bfloat16 else 1
+        more, many = (3 * r / 8 + 2 + split) * S, (3 * len(rows) / 8 + 19 + split) * S
         out[0][0][rows] += U @ B.T
         out[0][1][rows] += (eU + more * U.abs()) @ B.abs().T
         out[1][0][rows] = V @ A
@@ -132,9 +133,12 @@ def test_strides(dtype):
     wide[:, 8:136] = x
     wide2 = torch.zeros(50, 201, dtype=dtype, device="cuda")
     wide2[:, 3:99] = base
-    assert torch.equal(lora_linear(wide[:, 8:136], a, b, i, scale, base), want)
-    for xs, bs in ((x, wide2[:, 3:99]), (x.t().contiguous().t(), base.t().contiguous().t())):
+    # rows off the 16-byte boundaries are added up by another kernel, in another order
+    for xs, bs in ((wide[:, 8:136], base), (x, wide2[:, 3:99]), (x.t().contiguous().t(), base.t().contiguous().t())):
         close(lora_linear(xs, a, b, i, scale, bs), ref(x, a, b, i, scale, base, dy)[0], dtype)
+    more = torch.zeros(50, 304, dtype=dtype, device="cuda")
+    more[:, 8:136] = x
+    assert torch.equal(lora_linear(more[:, 8:136], a, b, i, scale, base), want)      # on them: the same
     wide[:, 3:131] = x
     close(lora_linear(wide[:, 3:131], a, b, i, scale, base), ref(x, a, b, i, scale, base, dy)[0], dtype)
     turned = a.transpose(1, 2).contiguous().transpose(1, 2)
