@@ -633,8 +633,8 @@ __device__ __forceinline__ void mma_step(float (&c)[4], const uint4& hi, const u
 template <typename T, int RT, int MT>
 struct Ring {
   static constexpr int SZ = (int)sizeof(T), R = 16 * MT;
-  static constexpr int kStage1 = R * 64 + RT * 64;                    // 64 bytes of every row of x, and as much of A
-  static constexpr int kStages = RT <= 32 ? 4 : RT == 64 ? 3 : 2;
+  static constexpr int kStage1 = R * 128 + RT * 128;                  // 128 bytes of every row of x, and as much of A
+  static constexpr int kStages = RT == 128 ? 1 : 2;
   static constexpr int PB = RT * SZ < 64 ? RT * SZ : 64, PR = PB / SZ; // bytes and ranks of a piece of a row of B
   static constexpr int kW2 = 128 / SZ * PB, kBase = R * 128, kSlot = kW2 + kBase;
   static constexpr int kBytes = kStages * kStage1 > 2 * kSlot ? kStages * kStage1 : 2 * kSlot;     // of a warp
@@ -642,14 +642,17 @@ struct Ring {
   static_assert(kSlot + R * RT * 4 <= kBytes, "a warp's part of u fits behind the first slot");
 };
 
+// Where 16-byte piece c of a 128-byte row lies: halves swapped in odd rows, so that eight lanes on half a row of two touch all banks.
+__device__ __forceinline__ int swap(int c, int row) { return (c ^ ((row & 1) * 4)) * 16; }
+
 template <typename T, int RT, int MT, bool TRANS>
 __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const Params p) {
   using L = Ring<T, RT, MT>;
-  constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 4 * EL, S1 = L::kStages;
+  constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 8 * EL, S1 = L::kStages;
   constexpr int PR = L::PR, PB = L::PB, PIECES = RT / PR, E = PR / 4;           // E: a lane's ranks of a piece
   constexpr int SE = kPairs<T> ? 4 : 2, PS = E / SE, ST = PIECES * PS;          // ranks of a lane, and instructions, a step
-  constexpr int TL = EL, CW = 2 * TL, BW = 8 * TL;
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int TL = EL, BW = 8 * TL;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int rows[R];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
@@ -664,28 +667,31 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   const int W = C * kWarps, w0 = rank * kWarps + warp;
 
   if (adapter >= 0) {
-    const T* xr[2 * MT];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) xr[i] = static_cast<const T*>(p.x) + (int64_t)rows[g + 8 * i] * p.ldx;
     const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
     auto fetch = [&](int i) {                          // the warp's chunk number i
       const int k0 = (w0 + i * W) * CH;
       if (k0 < p.K) {
         const uint32_t at = ring + i % S1 * L::kStage1;
-        const int k = k0 + q * EL;
+        const int k = k0 + (lane & 7) * EL;
         const bool live = k < p.K;
 #pragma unroll
-        for (int j = 0; j < 2 * MT; ++j) copy16(at + (g + 8 * j) * 64 + q * 16, live ? xr[j] + k : xr[j], live);
-        const uint32_t wat = at + R * 64;
+        for (int j = 0; j < 4 * MT; ++j) {
+          const int row = (lane >> 3) + 4 * j;
+          const T* src = static_cast<const T*>(p.x);
+          copy16(at + row * 128 + swap(lane & 7, row), live ? src + (int64_t)rows[row] * p.ldx + k : src, live);
+        }
+        const uint32_t wat = at + R * 128;
         if constexpr (!TRANS) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const bool in = live && 8 * t + g < p.r;
-            copy16(wat + (8 * t + g) * 64 + q * 16, in ? w1 + (int64_t)(8 * t + g) * p.K + k : w1, in);
+          for (int j = 0; j < RT / 4; ++j) {
+            const int row = (lane >> 3) + 4 * j;
+            const bool in = live && row < p.r;
+            copy16(wat + row * 128 + swap(lane & 7, row), in ? w1 + (int64_t)row * p.K + k : w1, in);
           }
         } else {
+          // the four lanes of a column read rows EL q + e of each half at once: those lie side by side
           copy_ranks<T, RT * SZ / 16, CH>(lane, p.r, 0, rank_row(w1, [&](int row, uint32_t& dst) -> const T* {
-            dst = wat + (row % EL * 4 + row / EL) * (RT * SZ);
+            dst = wat + (row / (4 * EL) * (4 * EL) + row % EL * 4 + row / EL % 4) * (RT * SZ);
             return k0 + row < p.K ? w1 + (int64_t)(k0 + row) * p.r : nullptr;
           }));
         }
@@ -696,53 +702,61 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
 #pragma unroll
     for (int i = 0; i < S1 - 1; ++i) fetch(i);
     for (int i = 0; (w0 + i * W) * CH < p.K; ++i) {
-      cp_async_wait_group<S1 - 2>();
-      __syncwarp();
-      const uint32_t at = ring + i % S1 * L::kStage1, wat = at + R * 64;
-      uint32_t xa[2 * MT][4];
-#pragma unroll
-      for (int j = 0; j < 2 * MT; ++j) lds(at + (g + 8 * j) * 64 + q * 16, xa[j]);
-      auto products = [&](int t, const uint32_t (&wb)[4]) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            if constexpr (SZ == 4) {
-              float4 ah, al;
-              split4(make_float4(__uint_as_float(xa[2 * m][2 * j]), __uint_as_float(xa[2 * m + 1][2 * j]),
-                                 __uint_as_float(xa[2 * m][2 * j + 1]), __uint_as_float(xa[2 * m + 1][2 * j + 1])), ah, al);
-              mma_split(acc[m][t], ah, al, __uint_as_float(wb[2 * j]), __uint_as_float(wb[2 * j + 1]));
-            } else {
-              mma_16<T>(acc[m][t], xa[2 * m][2 * j], xa[2 * m + 1][2 * j], xa[2 * m][2 * j + 1], xa[2 * m + 1][2 * j + 1],
-                        wb[2 * j], wb[2 * j + 1]);
-            }
-          }
-      };
-      if constexpr (!TRANS) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          uint32_t wb[4];
-          lds(wat + (8 * t + g) * 64 + q * 16, wb);
-          products(t, wb);
-        }
+      if constexpr (S1 == 1) {
+        fetch(i);
+        cp_async_wait_all();
       } else {
-        constexpr int WN = NT * SZ / 4;                // words of a lane's ranks
-        uint32_t raw[EL][WN];
+        fetch(i + S1 - 1);
+        cp_async_wait_group<S1 - 1>();
+      }
+      __syncwarp();
+      const uint32_t at = ring + i % S1 * L::kStage1, wat = at + R * 128;
 #pragma unroll
-        for (int e = 0; e < EL; ++e) lds(wat + (e * 4 + q) * (RT * SZ) + g * NT * SZ, raw[e]);
+      for (int h = 0; h < 2; ++h) {                    // a lane's k: pieces q and q + 4 of the row
+        uint32_t xa[2 * MT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          uint32_t wb[4];
+        for (int j = 0; j < 2 * MT; ++j) lds(at + (g + 8 * j) * 128 + swap(q + 4 * h, g), xa[j]);
+        auto products = [&](int t, const uint32_t (&wb)[4]) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if constexpr (SZ == 4) wb[w] = raw[w][t];
-            else wb[w] = pair_of(raw[2 * w][t >> 1], raw[2 * w + 1][t >> 1], t);
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              if constexpr (SZ == 4) {
+                float4 ah, al;
+                split4(make_float4(__uint_as_float(xa[2 * m][2 * j]), __uint_as_float(xa[2 * m + 1][2 * j]),
+                                   __uint_as_float(xa[2 * m][2 * j + 1]), __uint_as_float(xa[2 * m + 1][2 * j + 1])), ah, al);
+                mma_split(acc[m][t], ah, al, __uint_as_float(wb[2 * j]), __uint_as_float(wb[2 * j + 1]));
+              } else {
+                mma_16<T>(acc[m][t], xa[2 * m][2 * j], xa[2 * m + 1][2 * j], xa[2 * m][2 * j + 1], xa[2 * m + 1][2 * j + 1],
+                          wb[2 * j], wb[2 * j + 1]);
+              }
+            }
+        };
+        if constexpr (!TRANS) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            uint32_t wb[4];
+            lds(wat + (8 * t + g) * 128 + swap(q + 4 * h, g), wb);
+            products(t, wb);
           }
-          products(t, wb);
+        } else {
+          constexpr int WN = NT * SZ / 4;              // words of a lane's ranks
+          uint32_t raw[EL][WN];
+#pragma unroll
+          for (int e = 0; e < EL; ++e) lds(wat + (h * 4 * EL + e * 4 + q) * (RT * SZ) + g * NT * SZ, raw[e]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            uint32_t wb[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if constexpr (SZ == 4) wb[w] = raw[w][t];
+              else wb[w] = pair_of(raw[2 * w][t >> 1], raw[2 * w + 1][t >> 1], t);
+            }
+            products(t, wb);
+          }
         }
       }
       __syncwarp();
-      fetch(i + S1 - 1);
     }
     cp_async_wait_all();
     __syncwarp();
@@ -772,15 +786,17 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
           const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL;
           const bool live = row < n && col < p.N;
           const T* src = static_cast<const T*>(p.base);
-          copy16(at + row * 128 + ((c ^ (row & 1)) * 16), live ? src + (int64_t)rows[row] * p.ldb + col : src, live);
+          copy16(at + row * 128 + swap(c, row), live ? src + (int64_t)rows[row] * p.ldb + col : src, live);
         }
       }
       if (adapter >= 0) {
         const uint32_t at = ring + (s & 1) * L::kSlot;
         if constexpr (!TRANS) {
-          // column CW (g / 2) + 2 t + g % 2 of the block is tile t's instruction column g: placed at 8 t + g
+          // column 4 EL h + EL (g / 2) + 2 t + g % 2 of the block is column g of the instruction of tile TL / 2 h + t: row 8 tile + g
+          // of the ring
           copy_ranks<T, PB / 16, BW>(lane, p.r, pi * PR, rank_row(w2, [&](int row, uint32_t& dst) -> const T* {
-            dst = at + (row % CW / 2 * 8 + row / CW * 2 + (row & 1)) * PB;
+            const int t = row / (4 * EL) * (TL / 2) + row % EL / 2, at_row = row % (4 * EL) / EL * 2 + (row & 1);
+            dst = at + (t * 8 + at_row) * PB;
             return n0 + row < p.N ? w2 + (int64_t)(n0 + row) * p.r : nullptr;
           }));
         } else {
@@ -788,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
           for (int j = 0; j < PR / 4; ++j) {
             const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL, rk = pi * PR + row;
             const bool live = rk < p.r && col < p.N;
-            copy16(at + row * 128 + ((c ^ (2 * (row / E))) * 16), live ? w2 + (int64_t)rk * p.N + col : w2, live);
+            copy16(at + row * 128 + ((c ^ (row / E)) * 16), live ? w2 + (int64_t)rk * p.N + col : w2, live);
           }
         }
       }
@@ -882,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
         for (int j = 0; j < PS; ++j) {
           uint32_t wr[SE][4];
 #pragma unroll
-          for (int e = 0; e < SE; ++e) lds(at + (q * E + SE * j + e) * 128 + ((g ^ (2 * q)) * 16), wr[e]);
+          for (int e = 0; e < SE; ++e) lds(at + (q * E + SE * j + e) * 128 + (((g / 2 + g % 2 * 4) ^ q) * 16), wr[e]);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             const uint32_t f = fr + 32 * ((m * ST + pi * PS + j) * 32 + lane);
@@ -899,30 +915,30 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
       }
     }
     if (pi == pieces - 1) {
-      const int col = (w0 + b * W) * BW + q * CW;
+      const int n0 = (w0 + b * W) * BW;
       const uint32_t at = ring + (b & 1) * L::kSlot + L::kW2;
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i) {
         const int row = g + 8 * i;
         if (row >= n) continue;
-        T* y = static_cast<T*>(p.y) + (int64_t)rows[row] * p.N + col;
+        T* y = static_cast<T*>(p.y) + (int64_t)rows[row] * p.N;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (col + h * EL >= p.N) continue;
+        for (int h = 0; h < 2; ++h) {                  // a lane's columns: pieces q and q + 4
+          const int col = n0 + (q + 4 * h) * EL;
+          if (col >= p.N) continue;
           uint32_t bw[4] = {0, 0, 0, 0};
-          if (p.base != nullptr) lds(at + row * 128 + (((2 * q + h) ^ (row & 1)) * 16), bw);
+          if (p.base != nullptr) lds(at + row * 128 + swap(q + 4 * h, row), bw);
           float o[EL];
 #pragma unroll
           for (int e = 0; e < EL; ++e) {
-            const int l = h * EL + e;                  // the lane's column
-            const int t = TRANS ? l % TL : l >> 1, odd = TRANS ? l / TL : l & 1;
+            const int t = TRANS ? e : h * (TL / 2) + (e >> 1), odd = TRANS ? h : e & 1;
             o[e] = c[i >> 1][t][2 * (i & 1) + odd] + elem<T>(bw, e);
           }
           if constexpr (SZ == 4)
-            *reinterpret_cast<float4*>(y + h * EL) = make_float4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<float4*>(y + col) = make_float4(o[0], o[1], o[2], o[3]);
           else
-            *reinterpret_cast<uint4*>(y + h * EL) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
-                                                               pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+            *reinterpret_cast<uint4*>(y + col) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
+                                                            pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
         }
       }
     }
@@ -945,7 +961,7 @@ template <typename T, int RT>
 __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p) {
   using L = OuterRing<T, RT>;
   constexpr int EL = 16 / (int)sizeof(T), TL = EL, BW = 8 * TL, RM = RT / 16, S = L::kStages;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int C = p.cluster, rank = (int)blockIdx.x % C, n0 = (int)blockIdx.x / C * BW;
   const int a = blockIdx.y, r0 = blockIdx.z * RT;
