@@ -469,8 +469,8 @@ int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
  * of x's type, one after the other, and a factor scale[i] (device f32, NULL: scale_value):
  *   u[m] = scale[i] * a[i] x[m],   y[m] = base[m] + b[i] u[m],   i = index[m]
  * index (i32 or i64, index_bytes 4 or 8; NULL: adapter 0 for all, L = 1) outside [0, L): no adapter, y = base.
- * base [M, N] (row stride ldb, NULL: zeros) and y (contiguous) have x's type; u [M, r] f32 or NULL is what the
- * backward pass reads. r 1..128, L up to 16384, M, K and N up to 2^24. u and the sums are f32, y is rounded once.
+ * base [M, N] (row stride ldb, NULL: zeros) and y (contiguous) have x's type; u [M, r] (4 bytes each) or NULL is what the
+ * backward pass reads (bf16 rows: two bf16 numbers, u's sum). r 1..128, L up to 16384, M, K and N up to 2^24. u and the sums are f32, y is rounded once.
  * Infinite inputs give infinite or NaN outputs in their rows.
  * More than 256 rows with an index, and every backward pass with one, need glad_lora_plan's order of the rows: a plan
  * of glad_lora_plan_size(M, L) bytes for this M, L, r and index.                  */
@@ -482,7 +482,7 @@ int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t 
 
 /* Its backward pass: du[m] = scale[i] * b[i]^T dy[m], dx[m] = a[i]^T du[m] (contiguous),
  * da[i] = sum over i's rows of du[m] x[m]^T, db[i] = the same of dy[m] u[m]^T; the gradient of base is dy. dx, da, db of x's type,
- * each NULL: not wanted; da needs x and du (f32 [M, r] of workspace), db needs u. Sums have a fixed
+ * each NULL: not wanted; da needs x and du (4 bytes [M, r] of workspace), db needs u. Sums have a fixed
  * order: the same call gives the same bits. Adapters without rows get zeros.    */
 int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, int64_t M, int64_t K, const void* a,
                        const void* b, int64_t N, int L, int r, const void* index, int index_bytes, const void* plan,

@@ -40,7 +40,7 @@ struct Params {
   const void* w2;       // B [L, N, r]; transposed: A [L, r, N]
   const void* base;     // [M, N] or null
   void* y;              // [M, N]
-  float* u;             // [M, r] or null
+  float* u;             // [M, r] or null, as kept() gives it
   const float* scale;   // [L] or null: scale_value
   const void* index;    // null: adapter 0 for every row
   const int32_t* plan;  // null: the kernel looks at index itself
@@ -52,11 +52,12 @@ struct Params {
 
 struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
   const void* x;        // [M, K]
-  const float* v;       // [M, r]
+  const float* v;       // [M, r], as kept() gives it
   void* out;            // element (rank, k) of adapter a at a * r * K + rank * step_r + k * step_k
   const int32_t* plan;  // null: all rows are adapter 0's
   int64_t ldx, step_r, step_k;
   int M, K, r, L, cluster;
+  uint32_t pitch;       // of x in bytes, where it fits
 };
 
 __device__ __forceinline__ float tf32(float v) {
@@ -64,10 +65,10 @@ __device__ __forceinline__ float tf32(float v) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
   return __uint_as_float(r);
 }
-// v = hi + lo, 11 bits each. Where v or hi is not finite, lo is 0.
+// v = hi + lo, 11 bits each. Where hi is infinite, lo is finite (the difference would be a NaN).
 __device__ __forceinline__ void split(float v, float& hi, float& lo) {
   hi = tf32(v);
-  lo = fabsf(hi) < INFINITY ? tf32(v - hi) : 0.0f;
+  lo = tf32(fmaxf(v - hi, -3e38f));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const float4& a, float b0, float b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -208,6 +209,34 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
   return n;
 }
 
+// fp32 numbers as an operand beside rows of T: two bf16 numbers (16 bits) for bf16, whose products then run at the full rate,
+// else two tf32 numbers (22 bits; fp16 pairs would not hold the range of gradients).
+template <typename T>
+constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
+__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  const float2 f = __bfloat1622float2(h);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(fmaxf(a - f.x, -3e38f), fmaxf(b - f.y, -3e38f));    // as in split()
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// u and du as they are kept: the two bf16 numbers side by side, or fp32.
+template <typename T>
+__device__ __forceinline__ float kept(float v) {
+  if constexpr (kPairs<T>) {
+    uint32_t hi, lo;
+    split_bf16(v, 0.0f, hi, lo);
+    return __uint_as_float(__byte_perm(hi, lo, 0x5410));
+  } else {
+    return v;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float value_kept(float k) {
+  if constexpr (kPairs<T>) return __uint_as_float(__float_as_uint(k) << 16) + __uint_as_float(__float_as_uint(k) & 0xffff0000u);
+  else return k;
+}
+
 template <int RT, int MT>
 constexpr size_t smem_bytes() {
   return (size_t)(kWarps + 1) * 16 * MT * RT * sizeof(float);
@@ -319,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_any_kernel(c
       v *= s;
       whole[i] = v;
       const int row = i / RT, at = i % RT;
-      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = v;
+      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = kept<T>(v);
     }
   }
   if (C > 1) cluster_sync_all();                       // nobody reads another block's part any more
@@ -502,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2) outer_any_kernel(const OuterParam
 #pragma unroll
       for (int k = 0; k < RM; ++k) {
         const int lo = r0 + 16 * k + g, hi = lo + 8;
-        const float v0 = on && lo < p.r ? vr[lo] : 0.0f, v1 = on && hi < p.r ? vr[hi] : 0.0f;
+        const float v0 = on && lo < p.r ? value_kept<T>(vr[lo]) : 0.0f, v1 = on && hi < p.r ? value_kept<T>(vr[hi]) : 0.0f;
         if (h == 0) v[k].x = v0, v[k].y = v1;
         else v[k].z = v0, v[k].w = v1;
       }
@@ -539,46 +568,50 @@ __global__ void __launch_bounds__(kThreads, 2) outer_any_kernel(const OuterParam
 // Every warp copies what it needs next, by itself: 16-byte copies into a ring of its own while it works on the stage before, so
 // the bytes in flight (up to 100 KB an SM) do not depend on registers or on other warps. The pieces are placed so that a
 // fragment's reads touch every bank once.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {       // zeros where not live
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(live ? 8 : 0) : "memory");
 }
-// A row piece of the ranks' direction: `count` pieces of 16 bytes a row, of which those below rank r are copied; f(row, piece) gives
-// the row's address (null: zeros) and where it goes. Ranks off 16 bytes are copied in halves.
-template <typename T, int COUNT, int ROWS, typename F>
-__device__ __forceinline__ void copy_ranks(int lane, int r, int from, F&& f) {
-  constexpr int EL = 16 / (int)sizeof(T);
+// ROWS rows of ranks, src on the first's: COUNT 16-byte pieces of each, of which `ranks` ranks are there and the rest is zeros, as
+// are rows from `there` on. Row i goes to place P::at(i), PITCH bytes each. P::at moves bits only, so a lane's places are its first
+// one plus constants. Rows off 16 bytes are copied in halves.
+template <typename T, int COUNT, int ROWS, int PITCH, typename P>
+__device__ __forceinline__ void copy_rows(int lane, uint32_t dst, const T* src, int r, int ranks, int there) {
+  constexpr int EL = 16 / (int)sizeof(T), STEP = 32 / COUNT;
+  static_assert(COUNT <= 32 && ROWS % STEP == 0, "a lane's pieces are of one column");
   if (r % EL == 0) {
+    const int row0 = lane / COUNT, c = lane % COUNT;
+    const bool in = c * EL < ranks;
+    const T* s = src + (in ? c * EL : 0);
+    const uint32_t d = dst + P::at(row0) * PITCH + 16 * c;
+    if (in && there >= ROWS) {
+      s += (int64_t)row0 * r;
 #pragma unroll
-    for (int j = 0; j < COUNT * ROWS / 32; ++j) {
-      const int id = lane + 32 * j, row = id / COUNT, c = id % COUNT, at = from + c * EL;
-      uint32_t dst;
-      const T* src = f(row, dst);
-      const bool live = src != nullptr && at < r;
-      copy16(dst + 16 * c, live ? src + at : f.any, live);
+      for (int j = 0; j < ROWS / STEP; ++j) {
+        copy16(d + P::at(STEP * j) * PITCH, s);
+        s += STEP * r;
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < ROWS / STEP; ++j) {
+        const int row = row0 + STEP * j;
+        const bool live = in && row < there;
+        copy16(dst + P::at(row) * PITCH + 16 * c, s + (live ? (int64_t)row * r : 0), live);
+      }
     }
   } else {
-#pragma unroll
-    for (int j = 0; j < 2 * COUNT * ROWS / 32; ++j) {
-      const int id = lane + 32 * j, row = id / (2 * COUNT), c = id % (2 * COUNT), at = from + c * (EL / 2);
-      uint32_t dst;
-      const T* src = f(row, dst);
-      const bool live = src != nullptr && at < r;
-      copy8(dst + 8 * c, live ? src + at : f.any, live);
+#pragma unroll 1
+    for (int id = lane; id < 2 * COUNT * ROWS; id += 32) {
+      const int row = id / (2 * COUNT), c = id % (2 * COUNT);
+      const bool live = row < there && c * (EL / 2) < ranks;
+      copy8(dst + P::at(row) * PITCH + 8 * c, src + (live ? (int64_t)row * r + c * (EL / 2) : 0), live);
     }
   }
-}
-template <typename T, typename G>
-struct RankRow {                         // a row's address and place, and some address of the tensor
-  const T* any;
-  G g;
-  __device__ __forceinline__ const T* operator()(int row, uint32_t& dst) const { return g(row, dst); }
-};
-template <typename T, typename G>
-__device__ __forceinline__ RankRow<T, G> rank_row(const T* any, G g) {
-  return {any, g};
 }
 
 template <int N>
@@ -601,17 +634,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// fp32 numbers as an operand beside rows of T: two bf16 numbers (16 bits) for bf16, whose products then run at the full rate,
-// else two tf32 numbers (22 bits; fp16 pairs would not hold the range of gradients).
-template <typename T>
-constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
-__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  const float2 f = __bfloat1622float2(h);
-  const __nv_bfloat162 l = __floats2bfloat162_rn(fabsf(f.x) < INFINITY ? a - f.x : 0.0f, fabsf(f.y) < INFINITY ? b - f.y : 0.0f);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 __device__ __forceinline__ void mma_pair(float (&c)[4], const uint4& hi, const uint4& lo, uint32_t b0, uint32_t b1) {
   mma_16<__nv_bfloat16>(c, lo.x, lo.y, lo.z, lo.w, b0, b1);
   mma_16<__nv_bfloat16>(c, hi.x, hi.y, hi.z, hi.w, b0, b1);
@@ -645,6 +667,20 @@ struct Ring {
 // Where 16-byte piece c of a 128-byte row lies: halves swapped in odd rows, so that eight lanes on half a row of two touch all banks.
 __device__ __forceinline__ int swap(int c, int row) { return (c ^ ((row & 1) * 4)) * 16; }
 
+// Places of a chunk's rows of B as k: the four lanes of a column read rows EL q + e of a half at once, which lie side by side.
+template <int EL>
+struct KPlace {
+  __host__ __device__ static constexpr int at(int row) { return row / (4 * EL) * (4 * EL) + row % EL * 4 + row / EL % 4; }
+};
+// Places of a block's rows of B as columns: column 4 EL h + EL (g / 2) + 2 t + g % 2 is column g of the instruction of tile EL / 2 h + t
+// and lies at 8 tile + g.
+template <int EL>
+struct NPlace {
+  __host__ __device__ static constexpr int at(int row) {
+    return (row / (4 * EL) * (EL / 2) + row % EL / 2) * 8 + row % (4 * EL) / EL * 2 + (row & 1);
+  }
+};
+
 template <typename T, int RT, int MT, bool TRANS>
 __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const Params p) {
   using L = Ring<T, RT, MT>;
@@ -654,6 +690,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   constexpr int TL = EL, BW = 8 * TL;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int rows[R];
+  __shared__ int64_t base_at[R];                       // their places in base
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
   const uint32_t ring = smem_u32(smem) + warp * L::kBytes;
@@ -665,52 +702,55 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   const int n = find_rows<R>(p, tile, rows, adapter);
   if (n == 0) return;                                 // the whole cluster
   const int W = C * kWarps, w0 = rank * kWarps + warp;
+  if (tid < R) base_at[tid] = (int64_t)rows[tid] * p.ldb;
+  __syncthreads();
 
   if (adapter >= 0) {
+    // the lane's piece lane % 8 of rows lane / 8 + 4 j, at its next chunk of K
     const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
-    auto fetch = [&](int i) {                          // the warp's chunk number i
-      const int k0 = (w0 + i * W) * CH;
-      if (k0 < p.K) {
-        const uint32_t at = ring + i % S1 * L::kStage1;
-        const int k = k0 + (lane & 7) * EL;
-        const bool live = k < p.K;
+    const T* xp[4 * MT];
+#pragma unroll
+    for (int j = 0; j < 4 * MT; ++j)
+      xp[j] = static_cast<const T*>(p.x) + (int64_t)rows[(lane >> 3) + 4 * j] * p.ldx + w0 * CH + (lane & 7) * EL;
+    const T* wp = TRANS ? w1 + (int64_t)w0 * CH * p.r : w1 + (int64_t)(lane >> 3) * p.K + w0 * CH + (lane & 7) * EL;
+    int from = w0 * CH, slot = 0;
+    auto fetch = [&]() {
+      if (from < p.K) {
+        const uint32_t at = ring + slot * L::kStage1, to = at + (lane >> 3) * 128 + swap(lane & 7, lane >> 3), wat = at + R * 128;
+        const bool whole = from + CH <= p.K, live = from + (lane & 7) * EL < p.K;
 #pragma unroll
         for (int j = 0; j < 4 * MT; ++j) {
-          const int row = (lane >> 3) + 4 * j;
-          const T* src = static_cast<const T*>(p.x);
-          copy16(at + row * 128 + swap(lane & 7, row), live ? src + (int64_t)rows[row] * p.ldx + k : src, live);
+          if (whole) copy16(to + j * 512, xp[j]);
+          else copy16(to + j * 512, live ? xp[j] : static_cast<const T*>(p.x), live);
+          xp[j] += W * CH;
         }
-        const uint32_t wat = at + R * 128;
         if constexpr (!TRANS) {
 #pragma unroll
           for (int j = 0; j < RT / 4; ++j) {
-            const int row = (lane >> 3) + 4 * j;
-            const bool in = live && row < p.r;
-            copy16(wat + row * 128 + swap(lane & 7, row), in ? w1 + (int64_t)row * p.K + k : w1, in);
+            const T* src = wp + (int64_t)(4 * j) * p.K;
+            const bool in = live && (lane >> 3) + 4 * j < p.r;
+            copy16(to + R * 128 + j * 512, in ? src : w1, in);
           }
+          wp += W * CH;
         } else {
-          // the four lanes of a column read rows EL q + e of each half at once: those lie side by side
-          copy_ranks<T, RT * SZ / 16, CH>(lane, p.r, 0, rank_row(w1, [&](int row, uint32_t& dst) -> const T* {
-            dst = wat + (row / (4 * EL) * (4 * EL) + row % EL * 4 + row / EL % 4) * (RT * SZ);
-            return k0 + row < p.K ? w1 + (int64_t)(k0 + row) * p.r : nullptr;
-          }));
+          copy_rows<T, RT * SZ / 16, CH, RT * SZ, KPlace<EL>>(lane, wat, wp, p.r, p.r, p.K - from);
+          wp += (int64_t)W * CH * p.r;
         }
+        from += W * CH;
       }
+      slot = slot + 1 == S1 ? 0 : slot + 1;
       cp_async_commit();
     };
     float acc[MT][NT][4] = {};
 #pragma unroll
-    for (int i = 0; i < S1 - 1; ++i) fetch(i);
-    for (int i = 0; (w0 + i * W) * CH < p.K; ++i) {
-      if constexpr (S1 == 1) {
-        fetch(i);
-        cp_async_wait_all();
-      } else {
-        fetch(i + S1 - 1);
-        cp_async_wait_group<S1 - 1>();
-      }
+    for (int i = 0; i < S1 - 1; ++i) fetch();
+    int stage = 0;
+    for (int k0 = w0 * CH; k0 < p.K; k0 += W * CH) {
+      fetch();
+      cp_async_wait_group<S1 - 1>();
       __syncwarp();
-      const uint32_t at = ring + i % S1 * L::kStage1, wat = at + R * 128;
+      const uint32_t at = ring + stage * L::kStage1, wat = at + R * 128;
+      stage = stage + 1 == S1 ? 0 : stage + 1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {                    // a lane's k: pieces q and q + 4 of the row
         uint32_t xa[2 * MT][4];
@@ -774,44 +814,52 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
 
   // The second product's operands: base and B of a step (a piece of the ranks of a block of columns).
   const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(adapter < 0 ? 0 : adapter) * p.N * p.r;
-  const int pieces = adapter < 0 ? 1 : PIECES;
-  const int blocks = p.y == nullptr ? 0 : max(0, ((p.N + BW - 1) / BW - w0 + W - 1) / W), steps = blocks * pieces;
-  auto fetch2 = [&](int s) {
-    if (s < steps) {
-      const int b = s / pieces, pi = s % pieces, n0 = (w0 + b * W) * BW;
-      if (pi == 0 && p.base != nullptr) {
-        const uint32_t at = ring + (b & 1) * L::kSlot + L::kW2;
-#pragma unroll
-        for (int j = 0; j < 4 * MT; ++j) {
-          const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL;
-          const bool live = row < n && col < p.N;
+  const bool any = adapter >= 0;
+  int next_n = p.y == nullptr ? p.N : w0 * BW, next_piece = 0, w_slot = 0, b_slot = 0;       // what is copied next
+  auto fetch2 = [&]() {
+    if (next_n < p.N) {
+      if (next_piece == 0) {
+        if (p.base != nullptr) {
+          const uint32_t at = ring + b_slot * L::kSlot + L::kW2 + (lane >> 3) * 128 + swap(lane & 7, lane >> 3);
+          const int col = next_n + (lane & 7) * EL;
           const T* src = static_cast<const T*>(p.base);
-          copy16(at + row * 128 + swap(c, row), live ? src + (int64_t)rows[row] * p.ldb + col : src, live);
-        }
-      }
-      if (adapter >= 0) {
-        const uint32_t at = ring + (s & 1) * L::kSlot;
-        if constexpr (!TRANS) {
-          // column 4 EL h + EL (g / 2) + 2 t + g % 2 of the block is column g of the instruction of tile TL / 2 h + t: row 8 tile + g
-          // of the ring
-          copy_ranks<T, PB / 16, BW>(lane, p.r, pi * PR, rank_row(w2, [&](int row, uint32_t& dst) -> const T* {
-            const int t = row / (4 * EL) * (TL / 2) + row % EL / 2, at_row = row % (4 * EL) / EL * 2 + (row & 1);
-            dst = at + (t * 8 + at_row) * PB;
-            return n0 + row < p.N ? w2 + (int64_t)(n0 + row) * p.r : nullptr;
-          }));
-        } else {
+          if (next_n + BW <= p.N && n == R) {
 #pragma unroll
-          for (int j = 0; j < PR / 4; ++j) {
-            const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL, rk = pi * PR + row;
-            const bool live = rk < p.r && col < p.N;
-            copy16(at + row * 128 + ((c ^ (row / E)) * 16), live ? w2 + (int64_t)rk * p.N + col : w2, live);
+            for (int j = 0; j < 4 * MT; ++j) copy16(at + j * 512, src + base_at[(lane >> 3) + 4 * j] + col);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4 * MT; ++j) {
+              const bool live = (lane >> 3) + 4 * j < n && col < p.N;
+              copy16(at + j * 512, live ? src + base_at[(lane >> 3) + 4 * j] + col : src, live);
+            }
           }
         }
+        b_slot ^= 1;
+      }
+      if (any) {
+        const uint32_t at = ring + w_slot * L::kSlot;
+        if constexpr (!TRANS) {
+          copy_rows<T, PB / 16, BW, PB, NPlace<EL>>(lane, at, w2 + (int64_t)next_n * p.r + (next_piece * PR < p.r ? next_piece * PR : 0),
+                                                    p.r, p.r - next_piece * PR, p.N - next_n);
+        } else {
+          const int col = next_n + (lane & 7) * EL;
+#pragma unroll
+          for (int j = 0; j < PR / 4; ++j) {
+            const int row = (lane >> 3) + 4 * j, rk = next_piece * PR + row;
+            const bool live = rk < p.r && col < p.N;
+            copy16(at + row * 128 + (((lane & 7) ^ (row / E)) * 16), live ? w2 + (int64_t)rk * p.N + col : w2, live);
+          }
+        }
+        w_slot ^= 1;
+      }
+      if (++next_piece >= (any ? PIECES : 1)) {
+        next_piece = 0;
+        next_n += W * BW;
       }
     }
     cp_async_commit();
   };
-  fetch2(0);
+  fetch2();
   if (adapter >= 0) {
     __syncthreads();
     for (int i = tid; i < R * RT; i += kThreads) {
@@ -838,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
       v *= s;
       whole[i] = v;
       const int row = i / RT, at = i % RT;
-      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = v;
+      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = kept<T>(v);
     }
     __syncthreads();
     for (int i = tid; i < MT * ST * 32; i += kThreads) {
@@ -864,19 +912,22 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
 
   const uint32_t fr = smem_u32(frag);
   float c[MT][TL][4];
-  for (int s = 0; s < steps; ++s) {
-    fetch2(s + 1);
+  T* yp[2 * MT];
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) yp[i] = static_cast<T*>(p.y) + (int64_t)rows[g + 8 * i] * p.N + q * EL;
+  int slot = 0, base_slot = 0, pi = 0;
+  for (int n0 = p.y == nullptr ? p.N : w0 * BW; n0 < p.N;) {
+    fetch2();
     cp_async_wait_group<1>();
     __syncwarp();
-    const int b = s / pieces, pi = s % pieces;
     if (pi == 0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < TL; ++t) c[m][t][0] = c[m][t][1] = c[m][t][2] = c[m][t][3] = 0.0f;
     }
-    if (adapter >= 0) {
-      const uint32_t at = ring + (s & 1) * L::kSlot;
+    if (any) {
+      const uint32_t at = ring + slot * L::kSlot;
       if constexpr (!TRANS) {
         uint32_t wv[TL][PB / 16];
 #pragma unroll
@@ -914,18 +965,17 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
         }
       }
     }
-    if (pi == pieces - 1) {
-      const int n0 = (w0 + b * W) * BW;
-      const uint32_t at = ring + (b & 1) * L::kSlot + L::kW2;
+    slot ^= 1;
+    if (++pi >= (any ? PIECES : 1)) {
+      const uint32_t at = ring + base_slot * L::kSlot + L::kW2;
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i) {
         const int row = g + 8 * i;
         if (row >= n) continue;
-        T* y = static_cast<T*>(p.y) + (int64_t)rows[row] * p.N;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                  // a lane's columns: pieces q and q + 4
-          const int col = n0 + (q + 4 * h) * EL;
-          if (col >= p.N) continue;
+          if (n0 + (q + 4 * h) * EL >= p.N) continue;
+          T* y = yp[i] + n0 + 4 * h * EL;
           uint32_t bw[4] = {0, 0, 0, 0};
           if (p.base != nullptr) lds(at + row * 128 + swap(q + 4 * h, row), bw);
           float o[EL];
@@ -935,12 +985,15 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
             o[e] = c[i >> 1][t][2 * (i & 1) + odd] + elem<T>(bw, e);
           }
           if constexpr (SZ == 4)
-            *reinterpret_cast<float4*>(y + col) = make_float4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
           else
-            *reinterpret_cast<uint4*>(y + col) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
-                                                            pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+            *reinterpret_cast<uint4*>(y) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
+                                                      pack2<T>(o[6], o[7]));
         }
       }
+      pi = 0;
+      base_slot ^= 1;
+      n0 += W * BW;
     }
     __syncwarp();
   }
@@ -970,47 +1023,56 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p)
   const Plan plan{p.plan, p.L, p.M};
   const int from = p.plan ? plan.first(a) : 0, rows = p.plan ? plan.first(a + 1) - from : p.M;
   const int W = C * kWarps, w0 = rank * kWarps + warp;
-  // lanes 0 .. 15: the rows of the warp's group number i of 16 (-1: none)
-  auto index_of = [&](int i) {
-    const int at = (w0 + i * W) * 16 + lane;
+  // lanes 0 .. 15: the rows of the warp's next group of 16 (-1: none)
+  int group = w0 * 16, slot = 0;
+  auto index_of = [&](int first) {
+    const int at = first + lane;
     return lane < 16 && at < rows ? p.plan ? plan.row(from + at) : at : -1;
   };
-  int next = index_of(0);
-  auto fetch = [&](int i) {
-    const int mine = next;
-    next = index_of(i + 1);
-    if ((w0 + i * W) * 16 < rows) {
-      const uint32_t at = ring + i % S * L::kStage;
+  int next = index_of(group);
+  const bool in = n0 + (lane & 7) * EL < p.K;
+  const char* xc = static_cast<const char*>(p.x) + (in ? (n0 + (lane & 7) * EL) * (int)sizeof(T) : 0);
+  constexpr int VC = RT / 4, VS = 32 / VC;             // pieces of a row of v, rows a step
+  const bool v_in = r0 + 4 * (lane % VC) < p.r;
+  const char* vc = reinterpret_cast<const char*>(p.v + (v_in ? r0 + 4 * (lane % VC) : 0));
+  auto fetch = [&]() {
+    if (group < rows) {
+      const int mine = next;
+      group += W * 16;
+      next = index_of(group);
+      const uint32_t at = ring + slot * L::kStage;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int row = (lane >> 3) + 4 * j, c = lane & 7, col = n0 + c * EL;
+        const int row = (lane >> 3) + 4 * j;
         const int m = __shfl_sync(0xffffffffu, mine, row);
-        const bool live = m >= 0 && col < p.K;
-        const T* x = static_cast<const T*>(p.x);
         const int turn = kPairs<T> ? row >> 1 & 3 : row & 3;           // a fragment's four rows at four places
-        copy16(at + row * 128 + ((c ^ (2 * turn)) * 16), live ? x + (int64_t)m * p.ldx + col : x, live);
+        copy16(at + row * 128 + (((lane & 7) ^ (2 * turn)) * 16), xc + (uint64_t)(uint32_t)max(m, 0) * p.pitch, in && m >= 0);
       }
 #pragma unroll
-      for (int j = 0; j < RT / 8; ++j) {
-        const int id = lane + 32 * j, row = id / (RT / 4), c = id % (RT / 4), rk = r0 + 4 * c;
+      for (int j = 0; j < 16 / VS; ++j) {
+        const int row = lane / VC + VS * j;
         const int m = __shfl_sync(0xffffffffu, mine, row);
-        const bool live = m >= 0 && rk < p.r;
-        copy16(at + 2048 + row * L::kPitch + 16 * c, live ? p.v + (int64_t)m * p.r + rk : p.v, live);
+        copy16(at + 2048 + row * L::kPitch + 16 * (lane % VC), vc + (uint64_t)(uint32_t)max(m, 0) * (uint32_t)(4 * p.r),
+               v_in && m >= 0);
       }
     }
+    slot = slot + 1 == S ? 0 : slot + 1;
     cp_async_commit();
   };
   float acc[RM][TL][4] = {};
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i) fetch(i);
-  for (int i = 0; (w0 + i * W) * 16 < rows; ++i) {
-    cp_async_wait_group<S - 2>();
+  for (int i = 0; i < S - 1; ++i) fetch();
+  int stage = 0;
+  for (int i0 = w0 * 16; i0 < rows; i0 += W * 16) {
+    fetch();
+    cp_async_wait_group<S - 1>();
     __syncwarp();
-    const uint32_t at = ring + i % S * L::kStage, vat = at + 2048;
-    auto v_at = [&](int m, int rk) {
+    const uint32_t at = ring + stage * L::kStage, vat = at + 2048;
+    stage = stage + 1 == S ? 0 : stage + 1;
+    auto word_at = [&](int m, int rk) {
       uint32_t w[1];
       lds(vat + m * L::kPitch + 4 * rk, w);
-      return __uint_as_float(w[0]);
+      return w[0];
     };
     if constexpr (kPairs<T>) {
       uint32_t xw[4][4];                               // rows 2 q, 2 q + 1, 2 q + 8, 2 q + 9
@@ -1020,10 +1082,14 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p)
       for (int k = 0; k < RM; ++k) {
         uint4 hi, lo;
         const int rk = 16 * k + g;
-        split_bf16(v_at(2 * q, rk), v_at(2 * q + 1, rk), hi.x, lo.x);
-        split_bf16(v_at(2 * q, rk + 8), v_at(2 * q + 1, rk + 8), hi.y, lo.y);
-        split_bf16(v_at(2 * q + 8, rk), v_at(2 * q + 9, rk), hi.z, lo.z);
-        split_bf16(v_at(2 * q + 8, rk + 8), v_at(2 * q + 9, rk + 8), hi.w, lo.w);
+        auto two_of = [&](int m, int rank_at, uint32_t& h, uint32_t& l) {
+          const uint32_t u = word_at(m, rank_at), v = word_at(m + 1, rank_at);
+          h = __byte_perm(u, v, 0x5410), l = __byte_perm(u, v, 0x7632);
+        };
+        two_of(2 * q, rk, hi.x, lo.x);
+        two_of(2 * q, rk + 8, hi.y, lo.y);
+        two_of(2 * q + 8, rk, hi.z, lo.z);
+        two_of(2 * q + 8, rk + 8, hi.w, lo.w);
 #pragma unroll
         for (int t = 0; t < TL; ++t)
           mma_pair(acc[k][t], hi, lo, pair_of(xw[0][t >> 1], xw[1][t >> 1], t), pair_of(xw[2][t >> 1], xw[3][t >> 1], t));
@@ -1038,6 +1104,7 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p)
         for (int k = 0; k < RM; ++k) {
           const int rk = 16 * k + g, m = 8 * h + q;
           float4 ah, al;
+          auto v_at = [&](int mm, int kk) { return __uint_as_float(word_at(mm, kk)); };
           split4(make_float4(v_at(m, rk), v_at(m, rk + 8), v_at(m + 4, rk), v_at(m + 4, rk + 8)), ah, al);
 #pragma unroll
           for (int t = 0; t < TL; ++t) {
@@ -1053,7 +1120,6 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p)
       }
     }
     __syncwarp();
-    fetch(i + S - 1);
   }
   cp_async_wait_all();
   __syncwarp();
@@ -1164,7 +1230,8 @@ cudaError_t run_outer(OuterParams p, cudaStream_t st) {
   p.cluster = 1;
   while (p.cluster < 8 && rows >= (int64_t)p.cluster * 2 * kWarps * 16 && tiles * p.cluster * 2 <= 2 * num_sms()) p.cluster *= 2;
   const dim3 grid((unsigned)((p.K + BW - 1) / BW * p.cluster), (unsigned)p.L, (unsigned)((p.r + RT - 1) / RT));
-  if (p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && on(p.v, 16) && p.r % 4 == 0)
+  p.pitch = (uint32_t)(p.ldx * (int64_t)sizeof(T));
+  if (p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && p.ldx < (int64_t)1 << 29 && on(p.v, 16) && p.r % 4 == 0)
     return RT == 16 ? launch_clusters(outer_kernel<T, 16>, p, grid, OuterRing<T, 16>::kSmem, st)
                     : launch_clusters(outer_kernel<T, 32>, p, grid, OuterRing<T, 32>::kSmem, st);
   const size_t smem = (size_t)(kWarps + 1) * RT * BW * sizeof(float);
