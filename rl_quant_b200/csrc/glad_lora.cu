@@ -7,9 +7,9 @@ namespace lora {
 extern template cudaError_t run<__half>(Params, bool, cudaStream_t);
 extern template cudaError_t run<__nv_bfloat16>(Params, bool, cudaStream_t);
 extern template cudaError_t run<float>(Params, bool, cudaStream_t);
-extern template cudaError_t run_outer<__half>(OuterParams, cudaStream_t);
-extern template cudaError_t run_outer<__nv_bfloat16>(OuterParams, cudaStream_t);
-extern template cudaError_t run_outer<float>(OuterParams, cudaStream_t);
+extern template cudaError_t run_outer<__half>(OuterPair, int, cudaStream_t);
+extern template cudaError_t run_outer<__nv_bfloat16>(OuterPair, int, cudaStream_t);
+extern template cudaError_t run_outer<float>(OuterPair, int, cudaStream_t);
 
 namespace {
 
@@ -35,19 +35,36 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   __syncthreads();
   const int run = ((p.M + p.warps - 1) / p.warps + 31) / 32 * 32;
   const int64_t lo = (int64_t)warp * run;
-  const int64_t hi = lo + run < p.M ? lo + run : p.M;
-  auto group_of = [&](int64_t m) -> int {
-    const int64_t a = p.index64 ? static_cast<const int64_t*>(p.index)[m] : (int64_t)static_cast<const int32_t*>(p.index)[m];
-    return a >= 0 && a < p.L ? (int)a : p.L;
-  };
-  if (warp < p.warps) {
-    for (int64_t m0 = lo; m0 < hi; m0 += 32) {
-      const int a = m0 + lane < hi ? group_of(m0 + lane) : -1;
-      const uint32_t same = __match_any_sync(0xffffffffu, a);
-      if (a >= 0 && lane == __ffs(same) - 1) cnt[warp * G + a] += __popc(same);
-      __syncwarp();
+  const int64_t hi = warp >= p.warps ? lo : lo + run < p.M ? lo + run : p.M;
+  // a lane's groups of the next kAhead steps of 32 rows (-1: past the end), loaded at once
+  constexpr int kAhead = 8;
+  int ahead[kAhead];
+  auto load = [&](int64_t m0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t m = m0 + 32 * j + lane;
+      int64_t a = -1;
+      if (m < hi) {
+        a = p.index64 ? static_cast<const int64_t*>(p.index)[m] : (int64_t)static_cast<const int32_t*>(p.index)[m];
+        a = a >= 0 && a < p.L ? a : p.L;
+      }
+      ahead[j] = (int)a;
     }
-  }
+  };
+  // calls f(first row of a step, this lane's group, the lanes of the same group), in order
+  auto steps = [&](auto&& f) {
+    for (int64_t m0 = lo; m0 < hi; m0 += 32 * kAhead) {
+      if (run > 32 * kAhead) load(m0);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (m0 + 32 * j < hi) f(m0 + 32 * j, ahead[j], __match_any_sync(0xffffffffu, ahead[j]));
+    }
+  };
+  load(lo);
+  steps([&](int64_t, int a, uint32_t same) {
+    if (a >= 0 && lane == __ffs(same) - 1) cnt[warp * G + a] += __popc(same);
+    __syncwarp();
+  });
   __syncthreads();
   int row_carry = 0, tile_carry = 0;
   for (int a0 = 0; a0 < G; a0 += kPlanThreads) {        // exclusive sums over the groups, of rows and of tiles
@@ -64,12 +81,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     }
     if (lane == 31) sums[0][warp] = r, sums[1][warp] = t;
     __syncthreads();
-    int before_r = row_carry, before_t = tile_carry;
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-      if (w < warp) before_r += sums[0][w], before_t += sums[1][w];
-      row_carry += sums[0][w];
-      tile_carry += sums[1][w];
+    static_assert(kPlanThreads == 1024, "a lane a warp");
+    int wr = sums[0][lane], wt = sums[1][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int ur = __shfl_up_sync(0xffffffffu, wr, o), ut = __shfl_up_sync(0xffffffffu, wt, o);
+      if (lane >= o) wr += ur, wt += ut;
     }
+    const int before_r = row_carry + (warp ? __shfl_sync(0xffffffffu, wr, warp ? warp - 1 : 0) : 0);
+    const int before_t = tile_carry + (warp ? __shfl_sync(0xffffffffu, wt, warp ? warp - 1 : 0) : 0);
+    row_carry += __shfl_sync(0xffffffffu, wr, 31);
+    tile_carry += __shfl_sync(0xffffffffu, wt, 31);
     if (a < G) {
       int at = before_r + r - rows;
       p.plan[1 + a] = at;
@@ -85,16 +107,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   if (tid == 0) p.plan[0] = tile_carry, p.plan[1 + G] = p.M, tile0[G] = tile_carry;
   __syncthreads();
   int32_t* order = p.plan + 3 + p.L;
-  if (warp < p.warps) {
-    for (int64_t m0 = lo; m0 < hi; m0 += 32) {
-      const int a = m0 + lane < hi ? group_of(m0 + lane) : -1;
-      const uint32_t same = __match_any_sync(0xffffffffu, a);
-      if (a >= 0) order[cnt[warp * G + a] + __popc(same & ((1u << lane) - 1))] = (int32_t)(m0 + lane);
-      __syncwarp();
-      if (a >= 0 && lane == __ffs(same) - 1) cnt[warp * G + a] += __popc(same);
-      __syncwarp();
-    }
-  }
+  steps([&](int64_t m0, int a, uint32_t same) {
+    if (a >= 0) order[cnt[warp * G + a] + __popc(same & ((1u << lane) - 1))] = (int32_t)(m0 + lane);
+    __syncwarp();
+    if (a >= 0 && lane == __ffs(same) - 1) cnt[warp * G + a] += __popc(same);
+    __syncwarp();
+  });
   int32_t* tiles = order + p.M;
   for (int t = tid; t < tile_carry; t += kPlanThreads) {
     int a = 0, b = G;                                   // the last group whose first tile is at or before t
@@ -151,7 +169,9 @@ int glad_lora_plan(const void* index, int index_bytes, int64_t M, int L, int r, 
   if (!index) return bad(who, "index must be set");
   if (!plan || plan_bytes < glad_lora_plan_size(M, L) || !on(plan, 16))
     return set_last_error(GLAD_ERR_WORKSPACE, "glad_lora_plan: a plan of glad_lora_plan_size bytes is required");
-  const int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
+  // counting warps: 256 rows each if possible, which they hold in registers; as many as shared memory has counters for
+  int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
+  if (M < 256 * warps) warps = (int)((M + 255) / 256);
   const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true)};
   const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
   cudaError_t e = cudaSuccess;
@@ -213,16 +233,18 @@ int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, i
     p.scale = scale, p.scale_value = scale_value, p.y = dx, p.u = da ? du : nullptr;
     e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, true, st); });
   }
-  OuterParams o{};
-  o.plan = static_cast<const int32_t*>(plan), o.M = (int)M, o.r = r, o.L = L;
-  if (da && e == cudaSuccess) {
-    o.x = x, o.ldx = ldx, o.v = du, o.out = da, o.K = (int)K, o.step_r = K, o.step_k = 1;
-    e = for_type(dtype, [&](auto t) { return run_outer<decltype(t)>(o, st); });
-  }
-  if (db && e == cudaSuccess) {
-    o.x = dy, o.ldx = lddy, o.v = u, o.out = db, o.K = (int)N, o.step_r = 1, o.step_k = r;
-    e = for_type(dtype, [&](auto t) { return run_outer<decltype(t)>(o, st); });
-  }
+  // db first: dy has just been read
+  OuterPair pair{};
+  int count = 0;
+  auto add = [&](const void* rows, int64_t ld, const float* v, void* out, int64_t cols, int64_t step_r, int64_t step_k) {
+    OuterParams& o = pair.of[count++];
+    o.plan = static_cast<const int32_t*>(plan), o.M = (int)M, o.r = r, o.L = L;
+    o.x = rows, o.ldx = ld, o.v = v, o.out = out, o.K = (int)cols, o.step_r = step_r, o.step_k = step_k;
+  };
+  if (db) add(dy, lddy, u, db, N, 1, r);
+  if (da) add(x, ldx, du, da, K, K, 1);
+  if (count && e == cudaSuccess)
+    e = for_type(dtype, [&](auto t) { return run_outer<decltype(t)>(pair, count, st); });
   return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
 }
 

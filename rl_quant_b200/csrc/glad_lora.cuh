@@ -58,6 +58,11 @@ struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
   int64_t ldx, step_r, step_k;
   int M, K, r, L, cluster;
   uint32_t pitch;       // of x in bytes, where it fits
+  int blocks;
+};
+struct OuterPair {
+  OuterParams of[2];
+  int cluster;
 };
 
 __device__ __forceinline__ float tf32(float v) {
@@ -209,15 +214,25 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
   return n;
 }
 
-// fp32 numbers as an operand beside rows of T: two bf16 numbers (16 bits) for bf16, whose products then run at the full rate,
-// else two tf32 numbers (22 bits; fp16 pairs would not hold the range of gradients).
+// fp32 numbers as an operand beside rows of T, whose products should run at the rate of T: two bf16 numbers (16 bits) for bf16;
+// two fp16 numbers (22 bits) for fp16 where a power of two can bring them into its range: u, by row (kHalves). Else two
+// tf32 numbers (22 bits), at half the rate: fp32, and fp16's sums over rows, which have no factor in common.
 template <typename T>
 constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
+template <typename T>
+constexpr bool kHalves = std::is_same<T, __half>::value;
 __device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   const float2 f = __bfloat1622float2(h);
   const __nv_bfloat162 l = __floats2bfloat162_rn(fmaxf(a - f.x, -3e38f), fmaxf(b - f.y, -3e38f));    // as in split()
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(fmaxf(a - f.x, -3e38f), fmaxf(b - f.y, -3e38f));
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // u and du as they are kept: the two bf16 numbers side by side, or fp32.
@@ -634,9 +649,10 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+template <typename T>
 __device__ __forceinline__ void mma_pair(float (&c)[4], const uint4& hi, const uint4& lo, uint32_t b0, uint32_t b1) {
-  mma_16<__nv_bfloat16>(c, lo.x, lo.y, lo.z, lo.w, b0, b1);
-  mma_16<__nv_bfloat16>(c, hi.x, hi.y, hi.z, hi.w, b0, b1);
+  mma_16<T>(c, lo.x, lo.y, lo.z, lo.w, b0, b1);
+  mma_16<T>(c, hi.x, hi.y, hi.z, hi.w, b0, b1);
 }
 __device__ __forceinline__ float4 as_f4(const uint4& v) {
   return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
@@ -686,11 +702,13 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   using L = Ring<T, RT, MT>;
   constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 8 * EL, S1 = L::kStages;
   constexpr int PR = L::PR, PB = L::PB, PIECES = RT / PR, E = PR / 4;           // E: a lane's ranks of a piece
-  constexpr int SE = kPairs<T> ? 4 : 2, PS = E / SE, ST = PIECES * PS;          // ranks of a lane, and instructions, a step
+  constexpr bool PAIRS = kPairs<T> || kHalves<T>;
+  constexpr int SE = PAIRS ? 4 : 2, PS = E / SE, ST = PIECES * PS;          // ranks of a lane, and instructions, a step
   constexpr int TL = EL, BW = 8 * TL;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int rows[R];
   __shared__ int64_t base_at[R];                       // their places in base
+  __shared__ float up[kHalves<T> ? R : 1], down[kHalves<T> ? R : 1];   // powers of two of the rows of u
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
   const uint32_t ring = smem_u32(smem) + warp * L::kBytes;
@@ -889,11 +907,30 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
       if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = kept<T>(v);
     }
     __syncthreads();
+    if constexpr (kHalves<T>) {
+      // a row's power of two: its largest number to 2^14, so that the lower halves reach 2^-38 of it
+      for (int row = warp; row < R; row += kWarps) {
+        float most = 0.0f;
+        for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(whole[row * RT + i]));
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        int e = 14 - ((int)(bits >> 23) - 127);
+        if (bits == 0 || bits >= 0x7f800000u) e = 0;
+        e = min(max(e, -126), 126);
+        if (lane == 0) up[row] = __uint_as_float((uint32_t)(127 + e) << 23), down[row] = __uint_as_float((uint32_t)(127 - e) << 23);
+      }
+      __syncthreads();
+    }
     for (int i = tid; i < MT * ST * 32; i += kThreads) {
       const int l = i & 31, st = (i >> 5) % ST, m = (i >> 5) / ST;
       const float* v = whole + (16 * m + (l >> 2)) * RT + st / PS * PR + (l & 3) * E + st % PS * SE;
       uint4 hi, lo;
-      if constexpr (kPairs<T>) {
+      if constexpr (kHalves<T>) {
+        const float s0 = up[16 * m + (l >> 2)], s1 = up[16 * m + (l >> 2) + 8];
+        split_f16(v[0] * s0, v[1] * s0, hi.x, lo.x);
+        split_f16(v[8 * RT] * s1, v[8 * RT + 1] * s1, hi.y, lo.y);
+        split_f16(v[2] * s0, v[3] * s0, hi.z, lo.z);
+        split_f16(v[8 * RT + 2] * s1, v[8 * RT + 3] * s1, hi.w, lo.w);
+      } else if constexpr (kPairs<T>) {
         split_bf16(v[0], v[1], hi.x, lo.x);
         split_bf16(v[8 * RT], v[8 * RT + 1], hi.y, lo.y);
         split_bf16(v[2], v[3], hi.z, lo.z);
@@ -940,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
             const uint4 hi = lds128(f), lo = lds128(f + 16);
 #pragma unroll
             for (int t = 0; t < TL; ++t) {
-              if constexpr (kPairs<T>) mma_pair(c[m][t], hi, lo, wv[t][2 * j], wv[t][2 * j + 1]);
+              if constexpr (PAIRS) mma_pair<T>(c[m][t], hi, lo, wv[t][2 * j], wv[t][2 * j + 1]);
               else mma_step<T>(c[m][t], hi, lo, elem<T>(wv[t], 2 * j), elem<T>(wv[t], 2 * j + 1));
             }
           }
@@ -956,8 +993,8 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
             const uint4 hi = lds128(f), lo = lds128(f + 16);
 #pragma unroll
             for (int t = 0; t < TL; ++t) {
-              if constexpr (kPairs<T>)
-                mma_pair(c[m][t], hi, lo, pair_of(wr[0][t >> 1], wr[1][t >> 1], t), pair_of(wr[2][t >> 1], wr[3][t >> 1], t));
+              if constexpr (PAIRS)
+                mma_pair<T>(c[m][t], hi, lo, pair_of(wr[0][t >> 1], wr[1][t >> 1], t), pair_of(wr[2][t >> 1], wr[3][t >> 1], t));
               else
                 mma_step<T>(c[m][t], hi, lo, elem<T>(wr[0], t), elem<T>(wr[1], t));
             }
@@ -972,6 +1009,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
       for (int i = 0; i < 2 * MT; ++i) {
         const int row = g + 8 * i;
         if (row >= n) continue;
+        const float factor = kHalves<T> ? (any ? down[row] : 0.0f) : 1.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                  // a lane's columns: pieces q and q + 4
           if (n0 + (q + 4 * h) * EL >= p.N) continue;
@@ -982,7 +1020,8 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
 #pragma unroll
           for (int e = 0; e < EL; ++e) {
             const int t = TRANS ? e : h * (TL / 2) + (e >> 1), odd = TRANS ? h : e & 1;
-            o[e] = c[i >> 1][t][2 * (i & 1) + odd] + elem<T>(bw, e);
+            const float v = c[i >> 1][t][2 * (i & 1) + odd], b = elem<T>(bw, e);
+            o[e] = kHalves<T> ? fmaf(v, factor, b) : v + b;
           }
           if constexpr (SZ == 4)
             *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
@@ -1010,13 +1049,17 @@ struct OuterRing {
   static_assert(RT * BW * 4 <= kBytes, "a warp's part of the gradient fits into its ring");
 };
 
+// Two gradients in one launch: the first blocks are of the first.
 template <typename T, int RT>
-__global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p) {
+__global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constant__ OuterPair pair) {
   using L = OuterRing<T, RT>;
+  const int second = (int)blockIdx.x >= pair.of[0].blocks;
+  const OuterParams& p = pair.of[second];
+  const int block = (int)blockIdx.x - (second ? pair.of[0].blocks : 0);
   constexpr int EL = 16 / (int)sizeof(T), TL = EL, BW = 8 * TL, RM = RT / 16, S = L::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-  const int C = p.cluster, rank = (int)blockIdx.x % C, n0 = (int)blockIdx.x / C * BW;
+  const int C = p.cluster, rank = block % C, n0 = block / C * BW;
   const int a = blockIdx.y, r0 = blockIdx.z * RT;
   const uint32_t ring = smem_u32(smem) + warp * L::kBytes;
   grid_dep_wait();
@@ -1092,7 +1135,7 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const OuterParams p)
         two_of(2 * q + 8, rk + 8, hi.w, lo.w);
 #pragma unroll
         for (int t = 0; t < TL; ++t)
-          mma_pair(acc[k][t], hi, lo, pair_of(xw[0][t >> 1], xw[1][t >> 1], t), pair_of(xw[2][t >> 1], xw[3][t >> 1], t));
+          mma_pair<T>(acc[k][t], hi, lo, pair_of(xw[0][t >> 1], xw[1][t >> 1], t), pair_of(xw[2][t >> 1], xw[3][t >> 1], t));
       }
     } else {
 #pragma unroll
@@ -1221,22 +1264,44 @@ cudaError_t run(Params p, bool trans, cudaStream_t st) {
   return trans ? run_as<T, true>(p, st) : run_as<T, false>(p, st);
 }
 
+// One or two gradients (count).
 template <typename T>
-cudaError_t run_outer(OuterParams p, cudaStream_t st) {
+cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
   constexpr int EL = 16 / (int)sizeof(T), BW = 8 * EL;
-  const int RT = p.r <= 16 ? 16 : 32;
-  const int64_t rows = p.plan ? (p.M + p.L - 1) / p.L : p.M;       // of an adapter, on average
-  const int64_t tiles = (int64_t)((p.K + BW - 1) / BW) * p.L * ((p.r + RT - 1) / RT);
-  p.cluster = 1;
-  while (p.cluster < 8 && rows >= (int64_t)p.cluster * 2 * kWarps * 16 && tiles * p.cluster * 2 <= 2 * num_sms()) p.cluster *= 2;
-  const dim3 grid((unsigned)((p.K + BW - 1) / BW * p.cluster), (unsigned)p.L, (unsigned)((p.r + RT - 1) / RT));
-  p.pitch = (uint32_t)(p.ldx * (int64_t)sizeof(T));
-  if (p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && p.ldx < (int64_t)1 << 29 && on(p.v, 16) && p.r % 4 == 0)
-    return RT == 16 ? launch_clusters(outer_kernel<T, 16>, p, grid, OuterRing<T, 16>::kSmem, st)
-                    : launch_clusters(outer_kernel<T, 32>, p, grid, OuterRing<T, 32>::kSmem, st);
+  const OuterParams& first = pair.of[0];
+  const int RT = first.r <= 16 ? 16 : 32, ranks = (first.r + RT - 1) / RT;
+  const int64_t rows = first.plan ? (first.M + first.L - 1) / first.L : first.M;       // of an adapter, on average
+  int64_t tiles = 0;
+  bool ring = first.r % 4 == 0;
+  for (int i = 0; i < count; ++i) {
+    OuterParams& p = pair.of[i];
+    tiles += (int64_t)((p.K + BW - 1) / BW) * p.L * ranks;
+    p.pitch = (uint32_t)(p.ldx * (int64_t)sizeof(T));
+    ring = ring && p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && p.ldx < (int64_t)1 << 29 && on(p.v, 16);
+  }
+  // blocks of a tile: while every warp keeps a few groups of 16 rows and the tiles alone do not fill the GPU
+  int C = 1;
+  while (C < 8 && rows >= (int64_t)C * 2 * kWarps * 16 && tiles * C * 2 <= 2 * num_sms()) C *= 2;
+  unsigned blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    pair.of[i].cluster = C;
+    pair.of[i].blocks = (pair.of[i].K + BW - 1) / BW * C;
+    blocks += (unsigned)pair.of[i].blocks;
+  }
+  pair.cluster = C;
+  if (ring) {
+    const dim3 grid(blocks, (unsigned)first.L, (unsigned)ranks);
+    return RT == 16 ? launch_clusters(outer_kernel<T, 16>, pair, grid, OuterRing<T, 16>::kSmem, st)
+                    : launch_clusters(outer_kernel<T, 32>, pair, grid, OuterRing<T, 32>::kSmem, st);
+  }
   const size_t smem = (size_t)(kWarps + 1) * RT * BW * sizeof(float);
-  return RT == 16 ? launch_clusters(outer_any_kernel<T, 16>, p, grid, smem, st)
-                  : launch_clusters(outer_any_kernel<T, 32>, p, grid, smem, st);
+  cudaError_t e = cudaSuccess;
+  for (int i = 0; i < count && e == cudaSuccess; ++i) {
+    const dim3 grid((unsigned)pair.of[i].blocks, (unsigned)first.L, (unsigned)ranks);
+    e = RT == 16 ? launch_clusters(outer_any_kernel<T, 16>, pair.of[i], grid, smem, st)
+                 : launch_clusters(outer_any_kernel<T, 32>, pair.of[i], grid, smem, st);
+  }
+  return e;
 }
 
 }  // namespace lora

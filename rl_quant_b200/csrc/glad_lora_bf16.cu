@@ -4,6 +4,6 @@
 namespace glad {
 namespace lora {
 template cudaError_t run<__nv_bfloat16>(Params, bool, cudaStream_t);
-template cudaError_t run_outer<__nv_bfloat16>(OuterParams, cudaStream_t);
+template cudaError_t run_outer<__nv_bfloat16>(OuterPair, int, cudaStream_t);
 }  // namespace lora
 }  // namespace glad

@@ -4,6 +4,6 @@
 namespace glad {
 namespace lora {
 template cudaError_t run<__half>(Params, bool, cudaStream_t);
-template cudaError_t run_outer<__half>(OuterParams, cudaStream_t);
+template cudaError_t run_outer<__half>(OuterPair, int, cudaStream_t);
 }  // namespace lora
 }  // namespace glad

@@ -4,6 +4,6 @@
 namespace glad {
 namespace lora {
 template cudaError_t run<float>(Params, bool, cudaStream_t);
-template cudaError_t run_outer<float>(OuterParams, cudaStream_t);
+template cudaError_t run_outer<float>(OuterPair, int, cudaStream_t);
 }  // namespace lora
 }  // namespace glad
