@@ -472,18 +472,17 @@ int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
  * base [M, N] (row stride ldb, NULL: zeros) and y (contiguous) have x's type; u [M, r] (4 bytes each) or NULL is what the
  * backward pass reads (bf16 rows: two bf16 numbers, u's sum). r 1..128, L up to 16384, M, K and N up to 2^24. u and the sums are f32, y is rounded once.
  * Infinite inputs give infinite or NaN outputs in their rows.
- * More than 256 rows with an index, and every backward pass with one, need glad_lora_plan's order of the rows: a plan
- * of glad_lora_plan_size(M, L) bytes for this M, L, r and index.                  */
+ * plan: glad_lora_plan_size(M, L) bytes (16-byte aligned) that the call fills with the order of the rows by adapter;
+ * needed with an index for more than 256 rows and where a backward pass follows, else NULL.  */
 size_t glad_lora_plan_size(int64_t M, int L);
-int glad_lora_plan(const void* index, int index_bytes, int64_t M, int L, int r, void* plan, size_t plan_bytes, void* stream);
 int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const void* a, const void* b, int64_t N,
-                      int L, int r, const void* index, int index_bytes, const void* plan, const float* scale, float scale_value,
-                      const void* base, int64_t ldb, void* y, float* u, void* stream);
+                      int L, int r, const void* index, int index_bytes, void* plan, size_t plan_bytes, const float* scale,
+                      float scale_value, const void* base, int64_t ldb, void* y, float* u, void* stream);
 
 /* Its backward pass: du[m] = scale[i] * b[i]^T dy[m], dx[m] = a[i]^T du[m] (contiguous),
  * da[i] = sum over i's rows of du[m] x[m]^T, db[i] = the same of dy[m] u[m]^T; the gradient of base is dy. dx, da, db of x's type,
- * each NULL: not wanted; da needs x and du (4 bytes [M, r] of workspace), db needs u. Sums have a fixed
- * order: the same call gives the same bits. Adapters without rows get zeros.    */
+ * each NULL: not wanted; da needs x and du (4 bytes [M, r] of workspace), db needs u; an index needs the
+ * forward pass's plan. Sums have a fixed order: the same call gives the same bits. Adapters without rows get zeros.    */
 int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, int64_t M, int64_t K, const void* a,
                        const void* b, int64_t N, int L, int r, const void* index, int index_bytes, const void* plan,
                        const float* scale, float scale_value, const float* u, float* du, void* dx, void* da, void* db,

@@ -165,10 +165,9 @@ SIGNATURES = {
     "glad_w4_linear_status": (c_int, [POINTER(c_uint32), c_void_p]),
     "glad_debug_w4_wait": (c_int, [c_uint32, c_uint64]),
     "glad_lora_plan_size": (c_size_t, [c_int64, c_int]),
-    "glad_lora_plan": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "glad_lora_forward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int,
-                                  c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p, c_void_p,
-                                  c_void_p]),
+                                  c_void_p, c_int, c_void_p, c_size_t, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                                  c_void_p, c_void_p]),
     "glad_lora_backward": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64,
                                    c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p]),

@@ -147,6 +147,18 @@ const char* shape_wrong(int dtype, int64_t M, int64_t K, int64_t N, int L, int r
 
 int64_t plan_words(int64_t M, int L) { return 3 + L + M + 2 * max_tiles(M, L, kMaxRank, true, true); }
 
+cudaError_t make_plan(const void* index, int index_bytes, int64_t M, int L, int r, void* plan, cudaStream_t st) {
+  static size_t limit[64] = {};
+  // counting warps: 256 rows each if possible, which they hold in registers; as many as shared memory has counters for
+  int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
+  if (M < 256 * warps) warps = (int)((M + 255) / 256);
+  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true)};
+  const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
+  const cudaError_t e = allow_smem(plan_kernel, smem, limit);
+  if (e != cudaSuccess) return e;
+  return launch_k(plan_kernel, dim3(1), dim3(kPlanThreads), smem, st, true, p);
+}
+
 }  // namespace
 }  // namespace lora
 }  // namespace glad
@@ -161,28 +173,9 @@ size_t glad_lora_plan_size(int64_t M, int L) {
   return (size_t)plan_words(M, L) * 4;
 }
 
-int glad_lora_plan(const void* index, int index_bytes, int64_t M, int L, int r, void* plan, size_t plan_bytes, void* stream) {
-  const char* who = "glad_lora_plan";
-  const char* why = shape_wrong(GLAD_DTYPE_F32, M, 1, 1, L, r, index, index_bytes);
-  if (why) return bad(who, why);
-  if (M == 0) return GLAD_OK;
-  if (!index) return bad(who, "index must be set");
-  if (!plan || plan_bytes < glad_lora_plan_size(M, L) || !on(plan, 16))
-    return set_last_error(GLAD_ERR_WORKSPACE, "glad_lora_plan: a plan of glad_lora_plan_size bytes is required");
-  // counting warps: 256 rows each if possible, which they hold in registers; as many as shared memory has counters for
-  int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
-  if (M < 256 * warps) warps = (int)((M + 255) / 256);
-  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true)};
-  const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
-  cudaError_t e = cudaSuccess;
-  if (smem > 40 * 1024) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess) e = launch_k(plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, true, p);
-  return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
-}
-
 int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const void* a, const void* b, int64_t N,
-                      int L, int r, const void* index, int index_bytes, const void* plan, const float* scale, float scale_value,
-                      const void* base, int64_t ldb, void* y, float* u, void* stream) {
+                      int L, int r, const void* index, int index_bytes, void* plan, size_t plan_bytes, const float* scale,
+                      float scale_value, const void* base, int64_t ldb, void* y, float* u, void* stream) {
   const char* who = "glad_lora_forward";
   const char* why = shape_wrong(dtype, M, K, N, L, r, index, index_bytes);
   if (why) return bad(who, why);
@@ -194,11 +187,15 @@ int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t 
       !on(plan, 16))
     return bad(who, "a tensor is not element-aligned");
   if (index && !plan && M > kSelfRows) return bad(who, "more than 256 rows with an index need a plan");
+  if (!index) plan = nullptr;
+  if (plan && plan_bytes < glad_lora_plan_size(M, L))
+    return set_last_error(GLAD_ERR_WORKSPACE, "glad_lora_forward: a plan of glad_lora_plan_size bytes is required");
   Params p{};
   p.x = x, p.ldx = ldx, p.M = (int)M, p.K = (int)K, p.N = (int)N, p.w1 = a, p.w2 = b, p.L = L, p.r = r;
   p.index = index, p.index64 = index_bytes == 8, p.plan = static_cast<const int32_t*>(plan);
   p.scale = scale, p.scale_value = scale_value, p.base = base, p.ldb = base ? ldb : 0, p.y = y, p.u = u;
-  const cudaError_t e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, false, (cudaStream_t)stream); });
+  cudaError_t e = plan ? make_plan(index, index_bytes, M, L, r, plan, (cudaStream_t)stream) : cudaSuccess;
+  if (e == cudaSuccess) e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, false, (cudaStream_t)stream); });
   return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
 }
 
@@ -221,7 +218,8 @@ int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, i
     return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
   }
   if (!dy || !a || !b) return bad(who, "dy, a and b must be set");
-  if (index && !plan) return bad(who, "an index needs a plan");
+  if (index && !plan) return bad(who, "an index needs the forward pass's plan");
+  if (!index) plan = nullptr;
   if ((why = rows_wrong(dy, dtype, lddy, M, (int)N))) return bad(who, why);
   if (da && (!x || !du)) return bad(who, "da needs x and du");
   if (db && !u) return bad(who, "db needs u");

@@ -22,7 +22,7 @@ constexpr int kThreads = 256, kWarps = 8;
 constexpr int kSelfRows = 256;        // up to so many rows the kernel finds the rows of an adapter itself
 constexpr int kMaxAdapters = 16384, kMaxRank = 128;
 
-// What glad_lora_plan leaves: rows in the order of their adapters, and tiles of them. In 32-bit words:
+// What plan_kernel leaves: rows in the order of their adapters, and tiles of them. In 32-bit words:
 //   [0] tiles, [1 .. L+2] first place of each adapter's rows in the order (L: of the rows without one; L+1: M),
 //   then the order [M], then the tiles (adapter or -1, first place) [2 * max]
 struct Plan {
@@ -1179,26 +1179,37 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
                        L::kBytes / 4, a, r0, n0, rank, C);
 }
 
-template <typename F, typename P>
-cudaError_t launch_clusters(F* kernel, const P& p, dim3 grid, size_t smem, cudaStream_t st) {
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+// Allows a kernel its dynamic shared memory, once a device (the call costs as much as a launch). `limit`: 0 or what was allowed.
+template <typename K>
+cudaError_t allow_smem(K* kernel, size_t smem, size_t (&limit)[64]) {
+  if (smem <= 40 * 1024) return cudaSuccess;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && limit[dev] >= smem)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && dev < 64) limit[dev] = smem;
+  return e;
+}
+
+template <auto Kernel, typename P>
+cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st) {
+  static size_t limit[64] = {};
+  const cudaError_t e = allow_smem(Kernel, smem, limit);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = pdl_enabled() ? attr : attr + 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (p.cluster > 1 ? 1 : 0);
+  return cudaLaunchKernelEx(&cfg, Kernel, p);
 }
 
 // Rows of a tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
@@ -1220,13 +1231,13 @@ cudaError_t launch_ring(Params p, int64_t tiles, int64_t likely, cudaStream_t st
   const int places = (RT == 16 ? 2 : 1) * num_sms();
   p.cluster = 1;
   while (p.cluster < 8 && likely * p.cluster * 2 <= places) p.cluster *= 2;
-  return launch_clusters(lora_kernel<T, RT, MT, TRANS>, p, dim3((unsigned)(tiles * p.cluster)), Ring<T, RT, MT>::kSmem, st);
+  return launch_clusters<lora_kernel<T, RT, MT, TRANS>>(p, dim3((unsigned)(tiles * p.cluster)), Ring<T, RT, MT>::kSmem, st);
 }
 template <typename T, int RT, bool TRANS>
 cudaError_t launch_any(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
   p.cluster = 1;
   while (p.cluster < 8 && likely * p.cluster * 2 <= 2 * num_sms()) p.cluster *= 2;
-  return launch_clusters(lora_any_kernel<T, RT, TRANS>, p, dim3((unsigned)(tiles * p.cluster)), smem_bytes<RT, 1>(), st);
+  return launch_clusters<lora_any_kernel<T, RT, TRANS>>(p, dim3((unsigned)(tiles * p.cluster)), smem_bytes<RT, 1>(), st);
 }
 
 // Whether every access of the ring kernels is on its boundary.
@@ -1291,15 +1302,15 @@ cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
   pair.cluster = C;
   if (ring) {
     const dim3 grid(blocks, (unsigned)first.L, (unsigned)ranks);
-    return RT == 16 ? launch_clusters(outer_kernel<T, 16>, pair, grid, OuterRing<T, 16>::kSmem, st)
-                    : launch_clusters(outer_kernel<T, 32>, pair, grid, OuterRing<T, 32>::kSmem, st);
+    return RT == 16 ? launch_clusters<outer_kernel<T, 16>>(pair, grid, OuterRing<T, 16>::kSmem, st)
+                    : launch_clusters<outer_kernel<T, 32>>(pair, grid, OuterRing<T, 32>::kSmem, st);
   }
   const size_t smem = (size_t)(kWarps + 1) * RT * BW * sizeof(float);
   cudaError_t e = cudaSuccess;
   for (int i = 0; i < count && e == cudaSuccess; ++i) {
     const dim3 grid((unsigned)pair.of[i].blocks, (unsigned)first.L, (unsigned)ranks);
-    e = RT == 16 ? launch_clusters(outer_any_kernel<T, 16>, pair.of[i], grid, smem, st)
-                 : launch_clusters(outer_any_kernel<T, 32>, pair.of[i], grid, smem, st);
+    e = RT == 16 ? launch_clusters<outer_any_kernel<T, 16>>(pair.of[i], grid, smem, st)
+                 : launch_clusters<outer_any_kernel<T, 32>>(pair.of[i], grid, smem, st);
   }
   return e;
 }

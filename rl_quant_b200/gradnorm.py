@@ -19,7 +19,8 @@ from . import _native as N
 
 _CODE = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 _KIND = {2.0: 2, 1.0: 1, float("inf"): 0}
-_dtype, _shape, _requires_grad = attrgetter("dtype"), attrgetter("shape"), attrgetter("requires_grad")
+_dtype, _shape, _layout = attrgetter("dtype"), attrgetter("shape"), attrgetter("layout")
+_requires_grad = attrgetter("requires_grad")
 
 
 def _kind(norm_type) -> int:
@@ -33,9 +34,9 @@ def _tensors(grads, what):
     if isinstance(grads, Tensor):
         return [grads]
     grads = list(grads)
-    for t in grads:
-        if not isinstance(t, Tensor):
-            raise TypeError(f"{what} must be tensors, got {type(t).__name__}")
+    for kind in set(map(type, grads)):
+        if not issubclass(kind, Tensor):
+            raise TypeError(f"{what} must be tensors, got {kind.__name__}")
     return grads
 
 
@@ -46,9 +47,9 @@ def _check(grads):
     for dt in dtypes:
         if dt not in _CODE:
             raise TypeError(f"a gradient is {dt}; expected float32, float16 or bfloat16")
-    for t in grads:
-        if t.layout is not torch.strided:
-            raise TypeError(f"a gradient is {t.layout}; expected a dense one")
+    for layout in set(map(_layout, grads)):
+        if layout is not torch.strided:
+            raise TypeError(f"a gradient is {layout}; expected a dense one")
     dev = grads[0].device
     if len(set(map(Tensor.get_device, grads))) != 1 or dev.type != "cuda":
         for t in grads:
@@ -107,13 +108,6 @@ def _run(grads, codes, outs, kind, max_norm):
     return norm
 
 
-def _written(tensors):
-    """Tell autograd, as torch's in-place operators do (inference tensors have no version)."""
-    if any(map(Tensor.is_inference, tensors)):
-        tensors = [t for t in tensors if not t.is_inference()]
-    torch.autograd.graph.increment_version(tensors)
-
-
 def _max_norm(value) -> float:
     value = float(value)
     if not value >= 0.0:
@@ -168,7 +162,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
             if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
                 raise ValueError(f"out has strides {o.stride()}, the gradient {t.stride()}")
     norm = _run(grads, codes, given, kind, max_norm)
-    _written(given)
+    torch.autograd.graph.increment_version(given)       # as torch's in-place operators do
     return given, norm
 
 
@@ -194,7 +188,7 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     norm = _run(whole, codes, whole, kind, max_norm)
     for t, c in strided:
         t.copy_(c)
-    _written(grads)
+    torch.autograd.graph.increment_version(grads)       # as torch's in-place operators do
     return norm
 
 

@@ -30,35 +30,25 @@ def _rows(t):
     return t2 if (step == 1 or cols == 1) and (ld >= cols or rows <= 1) else t2.contiguous()
 
 
-def _plan(index, M, L, r):
-    """The rows' order by adapter (None: not needed)."""
-    lib = N.load()
-    plan = torch.empty(lib.glad_lora_plan_size(M, L), dtype=torch.uint8, device=index.device)
-    rc = N.on_device(lib.glad_lora_plan, index.device.index, index.data_ptr(), index.element_size(), M, L, r,
-                     plan.data_ptr(), plan.numel())
-    if rc:
-        N.check(rc, "lora_linear")
-    return plan
-
-
-def _scale(scale):
-    return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
-
-
-def _forward(x, a, b, index, scale, base, plan, u):
+def _forward(x, a, b, index, scale, base, plan, plan_bytes, u):
+    """``plan`` and ``u`` are addresses of scratch memory, or None."""
     x2 = _rows(x)
     M, K = x2.shape
     L, r, _ = a.shape
     n = b.shape[1]
     y = x.new_empty(x.shape[:-1] + (n,))
-    bp, ldb = None, 0
+    bp, ldb, ip, ib, sp, sv = None, 0, None, 0, None, 0.0
     if base is not None:
         b2 = _rows(base)
         bp, ldb = b2.data_ptr(), b2.stride(0)
-    ip, ib = (None, 0) if index is None else (index.data_ptr(), index.element_size())
-    sp, sv = _scale(scale)
+    if index is not None:
+        ip, ib = index.data_ptr(), index.element_size()
+    if isinstance(scale, torch.Tensor):
+        sp = scale.data_ptr()
+    else:
+        sv = scale
     rc = N.on_device(N.load().glad_lora_forward, x.device.index, x2.data_ptr(), _CODE[x.dtype], x2.stride(0), M, K,
-                     a.data_ptr(), b.data_ptr(), n, L, r, ip, ib, N.ptr(plan), sp, sv, bp, ldb, y.data_ptr(), N.ptr(u))
+                     a.data_ptr(), b.data_ptr(), n, L, r, ip, ib, plan, plan_bytes, sp, sv, bp, ldb, y.data_ptr(), u)
     if rc:
         N.check(rc, "lora_linear")
     return y
@@ -67,34 +57,47 @@ def _forward(x, a, b, index, scale, base, plan, u):
 class _LoRA(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, index, scale, base):
-        M, (L, r, _) = x.numel() // x.shape[-1], a.shape
-        plan = _plan(index, M, L, r) if index is not None and M else None
-        u = x.new_empty((M, r), dtype=torch.float32) if ctx.needs_input_grad[2] else None
-        y = _forward(x, a, b, index, scale, base, plan, u)
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, a, b, index,
-                              scale if isinstance(scale, torch.Tensor) else None, plan, u)
-        ctx.scale, ctx.x_shape = scale if not isinstance(scale, torch.Tensor) else 0.0, x.shape
+        L, r, K = a.shape
+        M = x.numel() // K
+        # one buffer: the order of the rows, then u
+        plan_bytes = N.load().glad_lora_plan_size(M, L) + 15 & -16 if index is not None else 0
+        kept = torch.empty(plan_bytes + 4 * M * r, dtype=torch.uint8, device=x.device)
+        at = kept.data_ptr()
+        plan, u = at if plan_bytes else None, at + plan_bytes if ctx.needs_input_grad[2] else None
+        y = _forward(x, a, b, index, scale, base, plan, plan_bytes, u)
+        given = isinstance(scale, torch.Tensor)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, a, b, index, scale if given else None, kept)
+        ctx.scale, ctx.x_shape, ctx.plan_bytes = 0.0 if given else scale, x.shape, plan_bytes
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, a, b, index, scale, plan, u = ctx.saved_tensors
         need_x, need_a, need_b, _, _, need_base = ctx.needs_input_grad
+        x, a, b, index, scale, kept = ctx.saved_tensors
         dx = da = db = None
         if need_x or need_a or need_b:
             d2 = _rows(dy)
             M, n = d2.shape
             L, r, K = a.shape
-            x2 = None if x is None else _rows(x)
-            dx = dy.new_empty(ctx.x_shape) if need_x else None
-            da = torch.empty_like(a) if need_a else None
-            db = torch.empty_like(b) if need_b else None
-            du = dy.new_empty((M, r), dtype=torch.float32) if need_a else None
-            ip, ib = (None, 0) if index is None else (index.data_ptr(), index.element_size())
-            rc = N.on_device(N.load().glad_lora_backward, dy.device.index, d2.data_ptr(), _CODE[dy.dtype], d2.stride(0),
-                             N.ptr(x2), 0 if x2 is None else x2.stride(0), M, K, a.data_ptr(), b.data_ptr(), n, L, r, ip, ib,
-                             N.ptr(plan), N.ptr(scale), ctx.scale, N.ptr(u), N.ptr(du), N.ptr(dx), N.ptr(da), N.ptr(db))
+            xp = dxp = dap = dbp = up = dup = ip = plan = None
+            ldx = ib = 0
+            if need_x:
+                dx = dy.new_empty(ctx.x_shape)
+                dxp = dx.data_ptr()
+            if need_a:
+                x2 = _rows(x)
+                xp, ldx = x2.data_ptr(), x2.stride(0)
+                da, du = torch.empty_like(a), dy.new_empty((M, r), dtype=torch.float32)
+                dap, dup = da.data_ptr(), du.data_ptr()
+            if need_b:
+                db = torch.empty_like(b)
+                dbp, up = db.data_ptr(), kept.data_ptr() + ctx.plan_bytes
+            if index is not None:
+                ip, ib, plan = index.data_ptr(), index.element_size(), kept.data_ptr()
+            rc = N.on_device(N.load().glad_lora_backward, dy.device.index, d2.data_ptr(), _CODE[dy.dtype], d2.stride(0), xp,
+                             ldx, M, K, a.data_ptr(), b.data_ptr(), n, L, r, ip, ib, plan,
+                             None if scale is None else scale.data_ptr(), ctx.scale, up, dup, dxp, dap, dbp)
             if rc:
                 N.check(rc, "lora_linear backward")
         return dx, da, db, None, None, dy if need_base else None
@@ -108,60 +111,65 @@ def lora_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.
     stride. index [...] int64 or int32 names the adapter of each row of x; outside 0..L-1 (by custom -1) the row has none. None:
     adapter 0 for all (L = 1). scale a number, or float32 [L]. r up to 128, L up to 16384. Differentiable in x, a, b and
     base (backward mode). Sums are float32 and the result is rounded once."""
-    dt, shape = x.dtype, x.shape
+    dt, shape, dev, a_shape, b_shape = x.dtype, x.shape, x.device, a.shape, b.shape
     if dt not in _CODE:
         raise TypeError(f"x is {dt}; expected float32, float16 or bfloat16")
-    if a.dim() != 3 or b.dim() != 3:
-        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} must be [L, r, K] and [L, N, r]")
-    L, r, K = a.shape
-    n = b.shape[1]
-    if b.shape[0] != L or b.shape[2] != r:
-        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} must be [L, r, K] and [L, N, r]")
+    if len(a_shape) != 3 or len(b_shape) != 3 or b_shape[0] != a_shape[0] or b_shape[2] != a_shape[1]:
+        raise ValueError(f"a {tuple(a_shape)} and b {tuple(b_shape)} must be [L, r, K] and [L, N, r]")
+    (L, r, K), n = a_shape, b_shape[1]
     if not 1 <= r <= MAX_RANK or not 1 <= L <= MAX_ADAPTERS or not 1 <= K <= MAX_SIZE or not 1 <= n <= MAX_SIZE:
         raise ValueError(f"{L} adapters of rank {r}, {K} inputs and {n} outputs: up to {MAX_ADAPTERS}, {MAX_RANK} and {MAX_SIZE}")
     if not shape or shape[-1] != K:
         raise ValueError(f"x {tuple(shape)} does not match a's {K} inputs")
-    if x.numel() // K > MAX_SIZE:
-        raise ValueError(f"{x.numel() // K} rows: up to {MAX_SIZE}")
+    M = x.numel() // K
+    if M > MAX_SIZE:
+        raise ValueError(f"{M} rows: up to {MAX_SIZE}")
     if a.dtype != dt or b.dtype != dt:
         raise TypeError(f"a is {a.dtype} and b {b.dtype}; expected x's {dt}")
-    dev = x.device
-    given = [t for t in (a, b, index, base) if t is not None]
-    if index is None:
-        if L != 1:
-            raise ValueError(f"{L} adapters need an index")
-    else:
+    if a.device != dev or b.device != dev:
+        raise ValueError(f"tensors on {dev}, {a.device} and {b.device}")
+    grad = torch.is_grad_enabled()
+    if index is not None:
         if index.dtype != torch.int64 and index.dtype != torch.int32:
             raise TypeError(f"index is {index.dtype}; expected int64 or int32")
         if index.shape != shape[:-1]:
             raise ValueError(f"index {tuple(index.shape)} does not match x {tuple(shape)}")
+        if index.device != dev:
+            raise ValueError(f"tensors on {dev} and {index.device}")
+        if not index.is_contiguous():
+            index = index.contiguous()
+    elif L != 1:
+        raise ValueError(f"{L} adapters need an index")
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32 or scale.shape != (L,):
             raise ValueError(f"scale must be a number or float32 [{L}]")
-        if torch.is_grad_enabled() and scale.requires_grad:
+        if scale.device != dev:
+            raise ValueError(f"tensors on {dev} and {scale.device}")
+        if grad and scale.requires_grad:
             raise RuntimeError("lora_linear has no gradient of scale")
-        given.append(scale)
+        N.refuse_tangents("lora_linear", scale)
+        if not scale.is_contiguous():
+            scale = scale.contiguous()
     if base is not None:
         if base.shape != shape[:-1] + (n,):
             raise ValueError(f"base {tuple(base.shape)} does not match {tuple(shape[:-1]) + (n,)}")
         if base.dtype != dt:
             raise TypeError(f"base is {base.dtype}; expected x's {dt}")
-    for t in given:
-        if t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    N.refuse_tangents("lora_linear", x, a, b, base, scale if isinstance(scale, torch.Tensor) else None)
+        if base.device != dev:
+            raise ValueError(f"tensors on {dev} and {base.device}")
+    N.refuse_tangents("lora_linear", x, a, b, base)
     N.require_cuda(x)
-    a, b = a.contiguous(), b.contiguous()
-    if index is not None:
-        index = index.contiguous()
-    if isinstance(scale, torch.Tensor):
-        scale = scale.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad
-                                    or (base is not None and base.requires_grad)):
+    if not a.is_contiguous():
+        a = a.contiguous()
+    if not b.is_contiguous():
+        b = b.contiguous()
+    if grad and (x.requires_grad or a.requires_grad or b.requires_grad or (base is not None and base.requires_grad)):
         return _LoRA.apply(x, a, b, index, scale, base)
-    M = x.numel() // K
-    plan = _plan(index, M, L, r) if index is not None and M > SELF_ROWS else None
-    return _forward(x, a, b, index, scale, base, plan, None)
+    if index is None or M <= SELF_ROWS:
+        return _forward(x, a, b, index, scale, base, None, 0, None)
+    size = N.load().glad_lora_plan_size(M, L)
+    plan = torch.empty(size, dtype=torch.uint8, device=dev)
+    return _forward(x, a, b, index, scale, base, plan.data_ptr(), size, None)
 
 
 class LoRALinear(nn.Module):
