@@ -19,7 +19,8 @@ namespace glad {
 namespace lora {
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr int kSelfRows = 256;        // up to so many rows the kernel finds the rows of an adapter itself
+constexpr int kSelfRows = 256;        // up to so many rows the kernel finds the rows of an adapter itself, a cluster a row,
+constexpr int kScanRows = 8192, kScanAdapters = 512;   // or, with few adapters, by counting all of them
 constexpr int kMaxAdapters = 16384, kMaxRank = 128;
 
 // What plan_kernel leaves: rows in the order of their adapters, and tiles of them. In 32-bit words:
@@ -169,9 +170,10 @@ __device__ __forceinline__ int adapter_of(const Params& p, int m) {
   return a >= 0 && a < p.L ? (int)a : -1;
 }
 
-// The rows of this cluster's tile into rows[0 .. n); returns n (0: nothing to do) and the adapter.
+// The rows of this cluster's tile into rows[0 .. n); returns n (0: nothing to do) and the adapter. `scratch` is shared memory for
+// kScanRows short numbers.
 template <int R>
-__device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, int& adapter) {
+__device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, int& adapter, void* scratch) {
   const int tid = threadIdx.x;
   int n;
   if (p.index == nullptr) {
@@ -188,6 +190,69 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
     n = min(R, plan.first((adapter < 0 ? p.L : adapter) + 1) - from);
     if (n <= 0) return 0;
     if (tid < n) rows[tid] = plan.row(from + tid);
+  } else if (p.M > kSelfRows) {
+    // Count the rows of every adapter, look the tile up among their tiles, and collect the adapter's rows from the tile's first on.
+    __shared__ int cnt[kScanAdapters + 1], sums[kWarps], found[2];
+    uint16_t* of = static_cast<uint16_t*>(scratch);
+    const int lane = tid & 31, G = p.L + 1;
+    for (int i = tid; i < G; i += kThreads) cnt[i] = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < p.M; i0 += kThreads) {
+      const int i = i0 + tid;
+      int a = -1;
+      if (i < p.M) {
+        a = adapter_of(p, i);
+        a = a < 0 ? p.L : a;
+        of[i] = (uint16_t)a;
+      }
+      const uint32_t same = __match_any_sync(0xffffffffu, a);
+      if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(&cnt[a], __popc(same));
+    }
+    __syncthreads();
+    if (tid < 32) {
+      int carry = 0, a = -1, first = 0;
+      for (int a0 = 0; a0 < G && a < 0; a0 += 32) {
+        const int tiles = a0 + lane < G ? (cnt[a0 + lane] + R - 1) / R : 0;
+        int t = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const int u = __shfl_up_sync(0xffffffffu, t, o);
+          if (lane >= o) t += u;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, carry + t > tile);
+        if (past) {
+          const int l = __ffs(past) - 1;
+          a = a0 + l;
+          first = (tile - carry - __shfl_sync(0xffffffffu, t - tiles, l)) * R;
+        }
+        carry += __shfl_sync(0xffffffffu, t, 31);
+      }
+      if (lane == 0) found[0] = a, found[1] = first;
+    }
+    __syncthreads();
+    const int a = found[0], first = found[1];
+    if (a < 0) return 0;
+    adapter = a == p.L ? -1 : a;
+    n = min(R, cnt[a] - first);
+    const int run = (p.M + kThreads - 1) / kThreads, lo = tid * run, hi = min(p.M, lo + run);
+    int mine = 0;
+    for (int i = lo; i < hi; ++i) mine += of[i] == a;
+    int at = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int u = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += u;
+    }
+    if (lane == 31) sums[tid >> 5] = at;
+    __syncthreads();
+    at -= mine;
+    for (int w = 0; w < tid >> 5; ++w) at += sums[w];
+    if (at < first + R && at + mine > first)
+      for (int i = lo; i < hi; ++i)
+        if (of[i] == a) {
+          if (at >= first && at < first + R) rows[at - first] = i;
+          ++at;
+        }
   } else {
     // One cluster a row: it is the tile's where R, 2 R, ... rows of the same adapter (none) come before it.
     __shared__ int of[kSelfRows], counts[kWarps];
@@ -254,7 +319,8 @@ __device__ __forceinline__ float value_kept(float k) {
 
 template <int RT, int MT>
 constexpr size_t smem_bytes() {
-  return (size_t)(kWarps + 1) * 16 * MT * RT * sizeof(float);
+  constexpr size_t u = (size_t)(kWarps + 1) * 16 * MT * RT * sizeof(float);
+  return u > kScanRows * 2 ? u : kScanRows * 2;
 }
 
 // For tensors off the 16-byte boundaries: operands straight from memory, element by element.
@@ -273,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_any_kernel(c
   const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
   grid_dep_wait();
   int adapter;
-  const int n = find_rows<R>(p, tile, rows, adapter);
+  const int n = find_rows<R>(p, tile, rows, adapter, sm);
   if (n == 0) return;                                 // the whole cluster
 
   if (adapter >= 0) {
@@ -672,12 +738,16 @@ template <typename T, int RT, int MT>
 struct Ring {
   static constexpr int SZ = (int)sizeof(T), R = 16 * MT;
   static constexpr int kStage1 = R * 128 + RT * 128;                  // 128 bytes of every row of x, and as much of A
-  static constexpr int kStages = RT == 128 ? 1 : 2;
   static constexpr int PB = RT * SZ < 64 ? RT * SZ : 64, PR = PB / SZ; // bytes and ranks of a piece of a row of B
   static constexpr int kW2 = 128 / SZ * PB, kBase = R * 128, kSlot = kW2 + kBase;
-  static constexpr int kBytes = kStages * kStage1 > 2 * kSlot ? kStages * kStage1 : 2 * kSlot;     // of a warp
+  // As many as let two blocks live on an SM at rank 16, and one above: every one more covers more of a copy's latency where a warp
+  // has few steps (64 requests at rank 16: @B2@ -> @B3@ us with three slots; 2048 rows at rank 64: @P2@ -> @P3@).
+  static constexpr int kSlots = RT == 16 && MT == 2 ? 2 : RT == 32 && MT == 1 ? 2 : 3;
+  static constexpr int kStages = RT == 128 ? 1 : RT == 64 ? 2 : kSlots;
+  static constexpr int kRed = (kSlots - 1) * kSlot;                   // a warp's part of u lies behind the slots that are filled before it is read
+  static constexpr int kNeed = kRed + R * RT * 4 > kSlots * kSlot ? kRed + R * RT * 4 : kSlots * kSlot;
+  static constexpr int kBytes = kStages * kStage1 > kNeed ? kStages * kStage1 : kNeed;               // of a warp
   static constexpr int kSmem = kWarps * kBytes + R * RT * 4 + R * RT * 8;
-  static_assert(kSlot + R * RT * 4 <= kBytes, "a warp's part of u fits behind the first slot");
 };
 
 // Where 16-byte piece c of a 128-byte row lies: halves swapped in odd rows, so that eight lanes on half a row of two touch all banks.
@@ -700,7 +770,7 @@ struct NPlace {
 template <typename T, int RT, int MT, bool TRANS>
 __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const Params p) {
   using L = Ring<T, RT, MT>;
-  constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 8 * EL, S1 = L::kStages;
+  constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 8 * EL, S1 = L::kStages, S2 = L::kSlots;
   constexpr int PR = L::PR, PB = L::PB, PIECES = RT / PR, E = PR / 4;           // E: a lane's ranks of a piece
   constexpr bool PAIRS = kPairs<T> || kHalves<T>;
   constexpr int SE = PAIRS ? 4 : 2, PS = E / SE, ST = PIECES * PS;          // ranks of a lane, and instructions, a step
@@ -714,10 +784,10 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   const uint32_t ring = smem_u32(smem) + warp * L::kBytes;
   float* part = reinterpret_cast<float*>(smem + kWarps * L::kBytes);            // this block's part of u, [R][RT]
   uint4* frag = reinterpret_cast<uint4*>(part + R * RT);                        // u as split operands, [MT][ST][32][2]
-  auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * L::kBytes + L::kSlot); };   // warp w's part, [R][RT]
+  auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * L::kBytes + L::kRed); };   // warp w's part, [R][RT]
   grid_dep_wait();
   int adapter;
-  const int n = find_rows<R>(p, tile, rows, adapter);
+  const int n = find_rows<R>(p, tile, rows, adapter, smem);
   if (n == 0) return;                                 // the whole cluster
   const int W = C * kWarps, w0 = rank * kWarps + warp;
   if (tid < R) base_at[tid] = (int64_t)rows[tid] * p.ldb;
@@ -735,11 +805,15 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
     auto fetch = [&]() {
       if (from < p.K) {
         const uint32_t at = ring + slot * L::kStage1, to = at + (lane >> 3) * 128 + swap(lane & 7, lane >> 3), wat = at + R * 128;
-        const bool whole = from + CH <= p.K, live = from + (lane & 7) * EL < p.K;
+        const bool whole = from + CH <= p.K && n == R, live = from + (lane & 7) * EL < p.K;
 #pragma unroll
         for (int j = 0; j < 4 * MT; ++j) {
-          if (whole) copy16(to + j * 512, xp[j]);
-          else copy16(to + j * 512, live ? xp[j] : static_cast<const T*>(p.x), live);
+          if (whole) {
+            copy16(to + j * 512, xp[j]);
+          } else {
+            const bool in = live && (lane >> 3) + 4 * j < n;
+            copy16(to + j * 512, in ? xp[j] : static_cast<const T*>(p.x), in);
+          }
           xp[j] += W * CH;
         }
         if constexpr (!TRANS) {
@@ -852,7 +926,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
             }
           }
         }
-        b_slot ^= 1;
+        b_slot = b_slot + 1 == S2 ? 0 : b_slot + 1;
       }
       if (any) {
         const uint32_t at = ring + w_slot * L::kSlot;
@@ -868,7 +942,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
             copy16(at + row * 128 + (((lane & 7) ^ (row / E)) * 16), live ? w2 + (int64_t)rk * p.N + col : w2, live);
           }
         }
-        w_slot ^= 1;
+        w_slot = w_slot + 1 == S2 ? 0 : w_slot + 1;
       }
       if (++next_piece >= (any ? PIECES : 1)) {
         next_piece = 0;
@@ -877,7 +951,8 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
     }
     cp_async_commit();
   };
-  fetch2();
+#pragma unroll
+  for (int i = 0; i < S2 - 1; ++i) fetch2();           // on their way while u is added up
   if (adapter >= 0) {
     __syncthreads();
     for (int i = tid; i < R * RT; i += kThreads) {
@@ -955,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   int slot = 0, base_slot = 0, pi = 0;
   for (int n0 = p.y == nullptr ? p.N : w0 * BW; n0 < p.N;) {
     fetch2();
-    cp_async_wait_group<1>();
+    cp_async_wait_group<S2 - 1>();
     __syncwarp();
     if (pi == 0) {
 #pragma unroll
@@ -1002,7 +1077,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
         }
       }
     }
-    slot ^= 1;
+    slot = slot + 1 == S2 ? 0 : slot + 1;
     if (++pi >= (any ? PIECES : 1)) {
       const uint32_t at = ring + base_slot * L::kSlot + L::kW2;
 #pragma unroll
@@ -1031,7 +1106,7 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
         }
       }
       pi = 0;
-      base_slot ^= 1;
+      base_slot = base_slot + 1 == S2 ? 0 : base_slot + 1;
       n0 += W * BW;
     }
     __syncwarp();
@@ -1220,7 +1295,7 @@ inline int tile_rows(int64_t M, int L, int r, bool indexed) {
 inline int64_t max_tiles(int64_t M, int L, int r, bool indexed, bool planned) {
   const int R = tile_rows(M, L, r, indexed);
   if (!indexed) return (M + R - 1) / R;
-  if (!planned) return M;
+  if (!planned && M <= kSelfRows) return M;
   const int64_t all = (M + R - 1) / R + L + 1;
   return all < M ? all : M;
 }
@@ -1264,7 +1339,10 @@ cudaError_t run_as(const Params& p, cudaStream_t st) {
   // 16 rows a tile: the plan's tiles of 32 in two
   Params h = p;
   h.halves = R == 32 && p.plan != nullptr;
-  const int64_t all = h.halves ? 2 * tiles : indexed ? tiles : (p.M + 15) / 16;
+  int64_t all = tiles;
+  if (h.halves) all = 2 * tiles;
+  else if (!indexed) all = (p.M + 15) / 16;
+  else if (!p.plan && p.M > kSelfRows) all = (p.M + 15) / 16 + p.L;
   if (p.r <= 16) return launch_any<T, 16, TRANS>(h, all, likely, st);
   if (p.r <= 32) return launch_any<T, 32, TRANS>(h, all, likely, st);
   if (p.r <= 64) return launch_any<T, 64, TRANS>(h, all, likely, st);

@@ -19,7 +19,11 @@ _CODE = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16:
 MAX_RANK = 128
 MAX_ADAPTERS = 16384
 MAX_SIZE = 1 << 24           # rows, inputs, outputs
-SELF_ROWS = 256              # above, the forward needs the rows in the order of their adapters
+
+
+def _needs_plan(M, L):
+    """Whether a forward pass alone needs the order of the rows by adapter laid down first."""
+    return M > 8192 or (M > 256 and L > 512)
 
 
 def _rows(t):
@@ -165,7 +169,7 @@ def lora_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.
         b = b.contiguous()
     if grad and (x.requires_grad or a.requires_grad or b.requires_grad or (base is not None and base.requires_grad)):
         return _LoRA.apply(x, a, b, index, scale, base)
-    if index is None or M <= SELF_ROWS:
+    if index is None or not _needs_plan(M, L):
         return _forward(x, a, b, index, scale, base, None, 0, None)
     size = N.load().glad_lora_plan_size(M, L)
     plan = torch.empty(size, dtype=torch.uint8, device=dev)

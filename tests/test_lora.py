@@ -110,7 +110,8 @@ def check(x, a, b, i, scale, base, dy, back=True):
 SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65, 3, 2), (16, 256, 128, 8, 1), (17, 128, 256, 4, 4),
          (64, 512, 1024, 16, 64), (33, 96, 64, 32, 2), (40, 1002, 777, 9, 5), (256, 264, 136, 24, 3), (257, 64, 72, 64, 3),
          (300, 200, 320, 48, 1), (300, 72, 64, 100, 2), (130, 128, 128, 128, 2), (1000, 48, 40, 16, 130), (2050, 520, 264, 16, 2),
-         (600, 1024, 1024, 33, 1)]
+         (600, 1024, 1024, 33, 1),
+         (8192, 32, 24, 16, 512), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3)]
 
 
 @gpu
