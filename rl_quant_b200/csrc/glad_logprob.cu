@@ -581,8 +581,8 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// HELD: the block's slice is at most kHeld pieces a thread, all loaded at once and kept in registers for the alternatives
-// (61 x 128001 bf16 with 20 of them: 17.6 us -> @HELD@). Else four pieces at a time, and the alternatives read them again.
+// HELD: the block's slice is at most kHeld pieces a thread, all loaded at once (one latency instead of two or more) and kept
+// in registers for the alternatives. Else four pieces at a time, and the alternatives read them again.
 constexpr int kHeld = 8;
 template <typename T, bool ENT, bool HELD>
 __global__ void __launch_bounds__(kRowThreads) logp_row_kernel(const LogpParams p) {

@@ -740,10 +740,8 @@ struct Ring {
   static constexpr int kStage1 = R * 128 + RT * 128;                  // 128 bytes of every row of x, and as much of A
   static constexpr int PB = RT * SZ < 64 ? RT * SZ : 64, PR = PB / SZ; // bytes and ranks of a piece of a row of B
   static constexpr int kW2 = 128 / SZ * PB, kBase = R * 128, kSlot = kW2 + kBase;
-  // As many as let two blocks live on an SM at rank 16, and one above: every one more covers more of a copy's latency where a warp
-  // has few steps (64 requests at rank 16: @B2@ -> @B3@ us with three slots; 2048 rows at rank 64: @P2@ -> @P3@).
-  static constexpr int kSlots = RT == 16 && MT == 2 ? 2 : RT == 32 && MT == 1 ? 2 : 3;
-  static constexpr int kStages = RT == 128 ? 1 : RT == 64 ? 2 : kSlots;
+  // Two of each: a third changed nothing (64 requests at rank 16 13.4 us both ways, 2048 rows at rank 64 29.4 and 29.7).
+  static constexpr int kSlots = 2, kStages = RT == 128 ? 1 : 2;
   static constexpr int kRed = (kSlots - 1) * kSlot;                   // a warp's part of u lies behind the slots that are filled before it is read
   static constexpr int kNeed = kRed + R * RT * 4 > kSlots * kSlot ? kRed + R * RT * 4 : kSlots * kSlot;
   static constexpr int kBytes = kStages * kStage1 > kNeed ? kStages * kStage1 : kNeed;               // of a warp
