@@ -24,6 +24,7 @@ import torch.nn as nn
 
 from . import _native as N, w4linear
 from .fused import FusedActor, FusedActorCritic, FusedCritic, FusedUnsupported, ppo_epilogue
+from .lora import LoRALinear
 from .qconv import QuantCNN
 from .qlinear import QuantLinear
 
@@ -414,12 +415,21 @@ class InferenceRunner:
     @torch.inference_mode()
     def sync_weights_from(self, src_model, use_graph: bool = True):
         """Cast-copy every same-named parameter/buffer of ``src_model`` (the fp32
-        master) into this copy, then requantise (qrt/runtime.py:224-271)."""
+        master) into this copy, then requantise (qrt/runtime.py:224-271). A layer under
+        adapters here takes the weights of a master without them; a master's adapters that
+        this copy lacks are an error."""
         if self._sync_items is None:
             for p in self.model.parameters():
                 p.requires_grad_(False)
             dst = dict(self.model.named_parameters())
             dst.update(dict(self.model.named_buffers()))
+            for path, m in self.model.named_modules():
+                if isinstance(m, LoRALinear):       # the layer below under the name that it has without adapters
+                    for name, t in list(m.base.named_parameters()) + list(m.base.named_buffers()):
+                        dst.setdefault(f"{path}.{name}" if path else name, t)
+            for path, m in src_model.named_modules():
+                if isinstance(m, LoRALinear) and (f"{path}.lora_a" if path else "lora_a") not in dst:
+                    raise ValueError(f"{path}: the source has adapters, this copy has none")
             items, keep = [], []
             for name, s in list(src_model.named_parameters()) + list(src_model.named_buffers()):
                 d = dst.get(name)

@@ -337,6 +337,58 @@ def test_module_over_4_bit_layers(dtype):
     assert torch.equal(m[0].weight, plain[0].weight)
 
 
+@gpu
+@pytest.mark.parametrize("mode", ["eager", "manual-graph"])
+def test_runner_with_adapters(mode):
+    """InferenceRunner over a policy with adapters on a plain and on a 4-bit layer: sync_weights_from masters without and with
+    adapters, and the actions are those of the policy itself."""
+    from rl_quant_b200 import InferenceRunner, build_glad
+    from rl_quant_b200.synthetic import glad_obs
+    paths = ["actor.0", "actor.2"]
+
+    def policy(seed, dtype):
+        torch.manual_seed(seed)
+        return build_glad().cuda().to(dtype).eval()
+    copy = policy(0, torch.float16)
+    swap.apply(copy, {"actor.0": {"bits": 4, "group": 32}})
+    layers = swap.apply_lora(copy, paths, rank=8, adapters=3)
+    with pytest.warns(UserWarning, match="op by op"):
+        run = InferenceRunner(copy, mode=mode)
+    obs = glad_obs(33, seed=1).cuda().half()
+    task = torch.arange(33, device="cuda") % 4 - 1
+    swap.select_lora(layers, task)
+    for seed in (1, 2):
+        master = policy(seed, torch.float32)
+        run.sync_weights_from(master)
+        for p in paths:
+            mine, theirs = copy.get_submodule(p).base, master.get_submodule(p)
+            assert torch.equal(mine.weight, theirs.weight.half()) and torch.equal(mine.bias, theirs.bias.half())
+        lin = nn.Linear(224, 512).cuda().half()
+        lin.weight.data.copy_(master.actor[0].weight)
+        assert torch.equal(copy.actor[0].base.tiles, swap.W4Linear(lin, 32).tiles)
+        with torch.no_grad():
+            assert torch.equal(run.act(obs), copy.act_inference({"policy_obs": obs})[0])
+    master = policy(3, torch.float32)
+    for mod in swap.apply_lora(master, paths, rank=8, adapters=3).values():
+        nn.init.normal_(mod.lora_b, std=0.1)
+    with pytest.warns(UserWarning):
+        run = InferenceRunner(copy, mode=mode)
+    run.sync_weights_from(master)
+    assert torch.equal(copy.actor[0].lora_b, master.actor[0].lora_b.half())
+    assert torch.equal(copy.actor[2].base.weight, master.actor[2].base.weight.half())
+    with torch.no_grad():
+        first = run.act(obs).clone()
+        assert torch.equal(first, copy.act_inference({"policy_obs": obs})[0])
+        task.copy_(task.flip(0))                       # read at every call, a captured one too
+        second = run.act(obs).clone()
+        assert torch.equal(second, copy.act_inference({"policy_obs": obs})[0]) and not torch.equal(first, second)
+    run.check_status()
+    with pytest.warns(UserWarning):
+        bare = InferenceRunner(policy(0, torch.float16), mode=mode)
+    with pytest.raises(ValueError, match="adapters"):
+        bare.sync_weights_from(master)
+
+
 def test_module_surgery():
     m = net(torch.float32, "cpu")
     m.eval()
