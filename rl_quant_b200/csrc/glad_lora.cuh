@@ -49,6 +49,7 @@ struct Params {
   float scale_value;
   int M, K, N, r, L, index64, cluster;
   int halves;           // a tile of the plan (32 rows) is taken as two of 16
+  int half;             // some address off 4 bytes
 };
 
 struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
@@ -60,6 +61,7 @@ struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
   int M, K, r, L, cluster;
   uint32_t pitch;       // of x in bytes, where it fits
   int blocks;
+  int half;             // some address of x off 4 bytes
 };
 struct OuterPair {
   OuterParams of[2];
@@ -108,41 +110,7 @@ __device__ __forceinline__ void split4(const float4& v, float4& hi, float4& lo) 
   split(v.w, hi.w, lo.w);
 }
 
-// n adjacent elements as 32-bit words (16-bit types: two a word), those at or past `live` zero. VEC: live is 0 or at least n, and
-// the address on the boundary of the access.
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void load_n(const T* p, int live, uint32_t (&w)[N * (int)sizeof(T) / 4]) {
-  constexpr int W = N * (int)sizeof(T) / 4;
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = 0;
-    if (live > 0) {
-      if constexpr (W == 1) w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-      else if constexpr (W == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x, w[1] = v.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < W; i += 4) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
-          w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        w[i] = i < live ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-      } else {
-        const uint32_t lo = 2 * i < live ? reinterpret_cast<const uint16_t*>(p)[2 * i] : 0u;
-        const uint32_t hi = 2 * i + 1 < live ? reinterpret_cast<const uint16_t*>(p)[2 * i + 1] : 0u;
-        w[i] = lo | hi << 16;
-      }
-    }
-  }
-}
-// Element e of such words as fp32.
+// Element e of 32-bit words (16-bit types: two a word) as fp32.
 template <typename T, int W>
 __device__ __forceinline__ float elem(const uint32_t (&w)[W], int e) {
   if constexpr (sizeof(T) == 4) {
@@ -311,245 +279,6 @@ __device__ __forceinline__ float kept(float v) {
     return v;
   }
 }
-template <typename T>
-__device__ __forceinline__ float value_kept(float k) {
-  if constexpr (kPairs<T>) return __uint_as_float(__float_as_uint(k) << 16) + __uint_as_float(__float_as_uint(k) & 0xffff0000u);
-  else return k;
-}
-
-template <int RT, int MT>
-constexpr size_t smem_bytes() {
-  constexpr size_t u = (size_t)(kWarps + 1) * 16 * MT * RT * sizeof(float);
-  return u > kScanRows * 2 ? u : kScanRows * 2;
-}
-
-// For tensors off the 16-byte boundaries: operands straight from memory, element by element.
-// RT: the rank, rounded up to 16, 32, 64 or 128; 16 rows a tile.
-template <typename T, int RT, bool TRANS>
-__global__ void __launch_bounds__(kThreads, RT == 128 ? 1 : 2) lora_any_kernel(const Params p) {
-  constexpr int MT = 1;
-  constexpr bool VEC = false;
-  constexpr int R = 16 * MT, NT = RT / 8, EL = 16 / (int)sizeof(T), CH = 4 * EL;
-  constexpr int E = RT / 4, ST = E / 2;               // ranks of a lane as an operand of y, and their instructions
-  extern __shared__ __align__(16) float sm[];
-  float* part = sm;                                   // this block's part of u, [R][RT]
-  float* red = sm + R * RT;                           // [warps][R][RT]; then u as split operands
-  __shared__ int rows[R];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-  const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
-  grid_dep_wait();
-  int adapter;
-  const int n = find_rows<R>(p, tile, rows, adapter, sm);
-  if (n == 0) return;                                 // the whole cluster
-
-  if (adapter >= 0) {
-    const T* xr[2 * MT];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) xr[i] = static_cast<const T*>(p.x) + (int64_t)rows[g + 8 * i] * p.ldx;
-    const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
-    float acc[MT][NT][4] = {};
-    for (int k0 = (rank * kWarps + warp) * CH; k0 < p.K; k0 += C * kWarps * CH) {
-      const int k = k0 + q * EL, live = p.K - k;
-      uint32_t xa[2 * MT][4];
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) load_n<T, EL, VEC>(xr[i] + k, live, xa[i]);
-      uint32_t wb[NT][4];
-      if constexpr (!TRANS) {
-        // instruction column g of tile t: rank 8 t + g
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          load_n<T, EL, VEC>(w1 + (int64_t)(8 * t + g) * p.K + k, 8 * t + g < p.r ? live : 0, wb[t]);
-      } else {
-        // instruction column g of tile t: rank NT g + t, adjacent in a row of B
-        constexpr int W = NT * (int)sizeof(T) / 4;
-        uint32_t raw[EL][W];
-#pragma unroll
-        for (int e = 0; e < EL; ++e)
-          load_n<T, NT, VEC>(w1 + (int64_t)(k + e) * p.r + g * NT, e < live ? p.r - g * NT : 0, raw[e]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if constexpr (sizeof(T) == 4) wb[t][w] = raw[w][t];
-            else wb[t][w] = pair_of(raw[2 * w][t >> 1], raw[2 * w + 1][t >> 1], t);
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if constexpr (sizeof(T) == 4) {
-            float4 ah, al;
-            split4(make_float4(__uint_as_float(xa[2 * i][2 * j]), __uint_as_float(xa[2 * i + 1][2 * j]),
-                               __uint_as_float(xa[2 * i][2 * j + 1]), __uint_as_float(xa[2 * i + 1][2 * j + 1])), ah, al);
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              mma_split(acc[i][t], ah, al, __uint_as_float(wb[t][2 * j]), __uint_as_float(wb[t][2 * j + 1]));
-          } else {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              mma_16<T>(acc[i][t], xa[2 * i][2 * j], xa[2 * i + 1][2 * j], xa[2 * i][2 * j + 1], xa[2 * i + 1][2 * j + 1],
-                        wb[t][2 * j], wb[t][2 * j + 1]);
-          }
-        }
-      }
-    }
-    float* mine = red + warp * R * RT;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = 2 * q + (c & 1), at = TRANS ? col * NT + t : 8 * t + col;
-          mine[(16 * i + g + 8 * (c >> 1)) * RT + at] = acc[i][t][c];
-        }
-    __syncthreads();
-    for (int i = tid; i < R * RT; i += kThreads) {
-      float s = red[i];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) s += red[w * R * RT + i];
-      part[i] = s;
-    }
-  }
-  if (C > 1) cluster_sync_all();
-  else __syncthreads();
-  if (adapter >= 0) {
-    const float s = p.scale ? p.scale[adapter] : p.scale_value;
-    const uint32_t here = smem_u32(part);
-    float* whole = red;                                // [R][RT]
-    for (int i = tid; i < R * RT; i += kThreads) {
-      float v;
-      if (C > 1) {
-        v = ld_cluster(mapa_shared(here + 4 * i, 0));
-        for (int c = 1; c < C; ++c) v += ld_cluster(mapa_shared(here + 4 * i, c));
-      } else {
-        v = part[i];
-      }
-      v *= s;
-      whole[i] = v;
-      const int row = i / RT, at = i % RT;
-      if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = kept<T>(v);
-    }
-  }
-  if (C > 1) cluster_sync_all();                       // nobody reads another block's part any more
-  else __syncthreads();
-  if (p.y == nullptr) return;
-  // u as the operand of instruction j: ranks E q + 2 j and E q + 2 j + 1 of rows g and g + 8, in two parts
-  float4* frag = reinterpret_cast<float4*>(red + R * RT);   // [MT][ST][32][2]
-  if (adapter >= 0) {
-    for (int i = tid; i < MT * ST * 32; i += kThreads) {
-      const int l = i & 31, j = (i >> 5) % ST, m = (i >> 5) / ST;
-      const float* v = red + (16 * m + (l >> 2)) * RT + (l & 3) * E + 2 * j;
-      split4(make_float4(v[0], v[8 * RT], v[1], v[8 * RT + 1]), frag[2 * i], frag[2 * i + 1]);
-    }
-  }
-  __syncthreads();
-
-  constexpr int TL = EL, CW = 2 * TL, BW = 8 * TL;     // tiles, a lane's adjacent columns, columns of a step
-  const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(adapter < 0 ? 0 : adapter) * p.N * p.r;
-  for (int n0 = (rank * kWarps + warp) * BW; n0 < p.N; n0 += C * kWarps * BW) {
-    const int col = n0 + q * CW;
-    uint32_t bw[2 * MT][2][4];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool on = p.base != nullptr && g + 8 * i < n;
-        load_n<T, EL, VEC>(static_cast<const T*>(p.base) + (on ? (int64_t)rows[g + 8 * i] * p.ldb + col + h * EL : 0),
-                           on ? p.N - col - h * EL : 0, bw[i][h]);
-      }
-    float c[MT][TL][4] = {};
-    if (adapter >= 0) {
-      if constexpr (!TRANS) {
-        // instruction column g of tile t: output column CW (g / 2) + 2 t + g % 2
-        constexpr int PE = E < EL ? E : EL, PIECES = E / PE;
-#pragma unroll 1
-        for (int pi = 0; pi < PIECES; ++pi) {
-          uint32_t wv[TL][PE * sizeof(T) / 4];
-          const int from = q * E + pi * PE;
-#pragma unroll
-          for (int t = 0; t < TL; ++t) {
-            const int o = n0 + (g >> 1) * CW + 2 * t + (g & 1);
-            load_n<T, PE, VEC>(w2 + (int64_t)(o < p.N ? o : 0) * p.r + from, o < p.N ? p.r - from : 0, wv[t]);
-          }
-#pragma unroll
-          for (int s = 0; s < PE / 2; ++s) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const float4* f = frag + 2 * ((i * ST + pi * (PE / 2) + s) * 32 + lane);
-              const float4 ah = f[0], al = f[1];
-#pragma unroll
-              for (int t = 0; t < TL; ++t) {
-                const float b0 = elem<T>(wv[t], 2 * s), b1 = elem<T>(wv[t], 2 * s + 1);
-                if constexpr (sizeof(T) == 4) {
-                  mma_split(c[i][t], ah, al, b0, b1);
-                } else {
-                  mma_tf32(c[i][t], al, b0, b1);
-                  mma_tf32(c[i][t], ah, b0, b1);
-                }
-              }
-            }
-          }
-        }
-      } else {
-        // instruction column g of tile t: output column TL g + t, adjacent in a row of A
-        const int at = n0 + g * TL;
-#pragma unroll 2
-        for (int s = 0; s < ST; ++s) {
-          const int from = q * E + 2 * s;
-          uint32_t w0[4], w1v[4];
-          load_n<T, EL, VEC>(w2 + (int64_t)(from < p.r ? from : 0) * p.N + at, from < p.r ? p.N - at : 0, w0);
-          load_n<T, EL, VEC>(w2 + (int64_t)(from + 1 < p.r ? from + 1 : 0) * p.N + at, from + 1 < p.r ? p.N - at : 0, w1v);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const float4* f = frag + 2 * ((i * ST + s) * 32 + lane);
-            const float4 ah = f[0], al = f[1];
-#pragma unroll
-            for (int t = 0; t < TL; ++t) {
-              const float b0 = elem<T>(w0, t), b1 = elem<T>(w1v, t);
-              if constexpr (sizeof(T) == 4) {
-                mma_split(c[i][t], ah, al, b0, b1);
-              } else {
-                mma_tf32(c[i][t], al, b0, b1);
-                mma_tf32(c[i][t], ah, b0, b1);
-              }
-            }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      if (g + 8 * i >= n) continue;
-      T* y = static_cast<T*>(p.y) + (int64_t)rows[g + 8 * i] * p.N + col;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float o[EL];
-#pragma unroll
-        for (int e = 0; e < EL; ++e) {
-          const int l = h * EL + e;                    // the lane's column
-          const int t = TRANS ? l % TL : l >> 1, odd = TRANS ? l / TL : l & 1;
-          o[e] = c[i >> 1][t][2 * (i & 1) + odd] + elem<T>(bw[i][h], e);
-        }
-        if constexpr (VEC) {
-          if (col + h * EL < p.N) {
-            if constexpr (sizeof(T) == 4)
-              *reinterpret_cast<float4*>(y + h * EL) = make_float4(o[0], o[1], o[2], o[3]);
-            else
-              *reinterpret_cast<uint4*>(y + h * EL) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
-                                                                 pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < EL; ++e)
-            if (col + h * EL + e < p.N) y[h * EL + e] = from_f<T>(o[e]);
-        }
-      }
-    }
-  }
-}
-
 // The warps' parts of a gradient tile, [RT][BW] each `step` floats apart, added up and, over the cluster, written.
 template <typename T, int RT, int BW>
 __device__ __forceinline__ void outer_end(const OuterParams& p, float* part, const float* red, int step, int a, int r0, int n0,
@@ -581,71 +310,7 @@ __device__ __forceinline__ void outer_end(const OuterParams& p, float* part, con
   if (C > 1) cluster_sync_all();
 }
 
-// RT: ranks of a block, 16 or 32 (blockIdx.z: which). A cluster shares 8 EL columns of one adapter's gradient; its warps split
-// the rows, and the parts are added in a fixed order. For tensors off the 16-byte boundaries.
-template <typename T, int RT>
-__global__ void __launch_bounds__(kThreads, 2) outer_any_kernel(const OuterParams p) {
-  constexpr bool VEC = false;
-  constexpr int EL = 16 / (int)sizeof(T), TL = EL, BW = 8 * TL, RM = RT / 16;
-  extern __shared__ __align__(16) float sm[];
-  float* part = sm;                                    // [RT][BW]
-  float* red = sm + RT * BW;                           // [warps][RT][BW]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-  const int C = p.cluster, rank = (int)blockIdx.x % C, n0 = (int)blockIdx.x / C * BW;
-  const int a = blockIdx.y, r0 = blockIdx.z * RT;
-  grid_dep_wait();
-  const Plan plan{p.plan, p.L, p.M};
-  const int from = p.plan ? plan.first(a) : 0, rows = p.plan ? plan.first(a + 1) - from : p.M;
-  const int at = n0 + g * EL, live = p.K - at;
-  float acc[RM][TL][4] = {};
-#pragma unroll 2
-  for (int i0 = (rank * kWarps + warp) * 8; i0 < rows; i0 += C * kWarps * 8) {
-    uint32_t xw[2][4];
-    float4 v[RM];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = i0 + q + 4 * h;
-      const bool on = i < rows;
-      const int m = !on ? 0 : p.plan ? plan.row(from + i) : i;
-      load_n<T, EL, VEC>(static_cast<const T*>(p.x) + (int64_t)m * p.ldx + at, on ? live : 0, xw[h]);
-      const float* vr = p.v + (int64_t)m * p.r;
-#pragma unroll
-      for (int k = 0; k < RM; ++k) {
-        const int lo = r0 + 16 * k + g, hi = lo + 8;
-        const float v0 = on && lo < p.r ? value_kept<T>(vr[lo]) : 0.0f, v1 = on && hi < p.r ? value_kept<T>(vr[hi]) : 0.0f;
-        if (h == 0) v[k].x = v0, v[k].y = v1;
-        else v[k].z = v0, v[k].w = v1;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < RM; ++k) {
-      float4 ah, al;
-      split4(v[k], ah, al);
-#pragma unroll
-      for (int t = 0; t < TL; ++t) {
-        const float b0 = elem<T>(xw[0], t), b1 = elem<T>(xw[1], t);
-        if constexpr (sizeof(T) == 4) {
-          mma_split(acc[k][t], ah, al, b0, b1);
-        } else {
-          mma_tf32(acc[k][t], al, b0, b1);
-          mma_tf32(acc[k][t], ah, b0, b1);
-        }
-      }
-    }
-  }
-  float* mine = red + warp * RT * BW;
-#pragma unroll
-  for (int k = 0; k < RM; ++k)
-#pragma unroll
-    for (int t = 0; t < TL; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        mine[(16 * k + g + 8 * (c >> 1)) * BW + (2 * q + (c & 1)) * TL + t] = acc[k][t][c];
-  __syncthreads();
-  outer_end<T, RT, BW>(p, part, red, RT * BW, a, r0, n0, rank, C);
-}
-
-// ---- the same from asynchronously filled rings ---------------------------------------------------
+// ---- rings of asynchronous copies ---------------------------------------------------------------
 // Every warp copies what it needs next, by itself: 16-byte copies into a ring of its own while it works on the stage before, so
 // the bytes in flight (up to 100 KB an SM) do not depend on registers or on other warps. The pieces are placed so that a
 // fragment's reads touch every bank once.
@@ -691,6 +356,41 @@ __device__ __forceinline__ void copy_rows(int lane, uint32_t dst, const T* src, 
       const int row = id / (2 * COUNT), c = id % (2 * COUNT);
       const bool live = row < there && c * (EL / 2) < ranks;
       copy8(dst + P::at(row) * PITCH + 8 * c, src + (live ? (int64_t)row * r + c * (EL / 2) : 0), live);
+    }
+  }
+}
+
+// The same for tensors off the 16-byte boundaries, one word of 4 bytes a lane: by asynchronous copies where every address is on 4 bytes
+// (half == false), else, for 16-bit elements, by two loads and a store. `left` elements are there from src on (null: none).
+template <typename T>
+struct Word {
+  uint32_t dst;
+  const T* src;
+  int left;
+};
+template <typename T, int COUNT, typename F>
+__device__ __forceinline__ void copy_words(bool half, const T* any, F&& f) {
+  constexpr int PER = 4 / (int)sizeof(T), BATCH = COUNT < 16 ? COUNT : 16;
+  if (!half || sizeof(T) == 4) {
+#pragma unroll 4
+    for (int i = 0; i < COUNT; ++i) {
+      const Word<T> w = f(i);
+      const int bytes = w.src ? max(0, min(PER, w.left)) * (int)sizeof(T) : 0;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(w.dst), "l"(bytes ? w.src : any), "r"(bytes) : "memory");
+    }
+  } else {
+#pragma unroll 1
+    for (int i0 = 0; i0 < COUNT; i0 += BATCH) {
+      uint32_t v[BATCH], at[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const Word<T> w = f(i0 + i);
+        const uint16_t* u = reinterpret_cast<const uint16_t*>(w.src);
+        const uint32_t lo = w.src && w.left > 0 ? __ldg(u) : 0u, hi = w.src && w.left > 1 ? __ldg(u + 1) : 0u;
+        v[i] = lo | hi << 16, at[i] = w.dst;
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at[i]), "r"(v[i]) : "memory");
     }
   }
 }
@@ -765,7 +465,8 @@ struct NPlace {
   }
 };
 
-template <typename T, int RT, int MT, bool TRANS>
+// RT: the rank, rounded up to 16, 32, 64 or 128; 16 MT rows a tile. RAGGED: some address off 16 bytes.
+template <typename T, int RT, int MT, bool TRANS, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const Params p) {
   using L = Ring<T, RT, MT>;
   constexpr int SZ = L::SZ, R = L::R, NT = RT / 8, EL = 16 / SZ, CH = 8 * EL, S1 = L::kStages, S2 = L::kSlots;
@@ -801,7 +502,29 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
     const T* wp = TRANS ? w1 + (int64_t)w0 * CH * p.r : w1 + (int64_t)(lane >> 3) * p.K + w0 * CH + (lane & 7) * EL;
     int from = w0 * CH, slot = 0;
     auto fetch = [&]() {
-      if (from < p.K) {
+      if (from < p.K && RAGGED) {
+        // a line of a row's 128 bytes at a time
+        const uint32_t at = ring + slot * L::kStage1, wat = at + R * 128;
+        const int e = lane * (4 / SZ);
+        copy_words<T, R>(p.half, static_cast<const T*>(p.x), [&](int row) {
+          return Word<T>{at + row * 128 + swap(lane >> 2, row) + 4 * (lane & 3),
+                         row < n ? static_cast<const T*>(p.x) + (int64_t)rows[row] * p.ldx + from + e : nullptr, p.K - from - e};
+        });
+        if constexpr (!TRANS) {
+          copy_words<T, RT>(p.half, w1, [&](int row) {
+            return Word<T>{wat + row * 128 + swap(lane >> 2, row) + 4 * (lane & 3),
+                           row < p.r ? w1 + (int64_t)row * p.K + from + e : nullptr, p.K - from - e};
+          });
+        } else {
+          constexpr int WPR = RT * SZ / 4;             // words of a row
+          copy_words<T, CH * WPR / 32>(p.half, w1, [&](int i) {
+            const int id = lane + 32 * i, row = id / WPR, rk = id % WPR * (4 / SZ);
+            return Word<T>{wat + KPlace<EL>::at(row) * (RT * SZ) + id % WPR * 4,
+                           from + row < p.K ? w1 + (int64_t)(from + row) * p.r + rk : nullptr, p.r - rk};
+          });
+        }
+        from += W * CH;
+      } else if (from < p.K) {
         const uint32_t at = ring + slot * L::kStage1, to = at + (lane >> 3) * 128 + swap(lane & 7, lane >> 3), wat = at + R * 128;
         const bool whole = from + CH <= p.K && n == R, live = from + (lane & 7) * EL < p.K;
 #pragma unroll
@@ -909,7 +632,15 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
   auto fetch2 = [&]() {
     if (next_n < p.N) {
       if (next_piece == 0) {
-        if (p.base != nullptr) {
+        if (p.base != nullptr && RAGGED) {
+          const uint32_t at = ring + b_slot * L::kSlot + L::kW2;
+          const T* src = static_cast<const T*>(p.base);
+          const int col = next_n + lane * (4 / SZ);
+          copy_words<T, R>(p.half, src, [&](int row) {
+            return Word<T>{at + row * 128 + swap(lane >> 2, row) + 4 * (lane & 3), row < n ? src + base_at[row] + col : nullptr,
+                           p.N - col};
+          });
+        } else if (p.base != nullptr) {
           const uint32_t at = ring + b_slot * L::kSlot + L::kW2 + (lane >> 3) * 128 + swap(lane & 7, lane >> 3);
           const int col = next_n + (lane & 7) * EL;
           const T* src = static_cast<const T*>(p.base);
@@ -928,7 +659,21 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
       }
       if (any) {
         const uint32_t at = ring + w_slot * L::kSlot;
-        if constexpr (!TRANS) {
+        if constexpr (RAGGED && !TRANS) {
+          constexpr int WPR = PB / 4;
+          copy_words<T, BW * WPR / 32>(p.half, w2, [&](int i) {
+            const int id = lane + 32 * i, row = id / WPR, rk = next_piece * PR + id % WPR * (4 / SZ);
+            return Word<T>{at + NPlace<EL>::at(row) * PB + id % WPR * 4,
+                           next_n + row < p.N ? w2 + (int64_t)(next_n + row) * p.r + rk : nullptr, p.r - rk};
+          });
+        } else if constexpr (RAGGED) {
+          const int col = next_n + lane * (4 / SZ);
+          copy_words<T, PR>(p.half, w2, [&](int row) {
+            const int rk = next_piece * PR + row;
+            return Word<T>{at + row * 128 + (((lane >> 2) ^ (row / E)) * 16) + 4 * (lane & 3),
+                           rk < p.r ? w2 + (int64_t)rk * p.N + col : nullptr, p.N - col};
+          });
+        } else if constexpr (!TRANS) {
           copy_rows<T, PB / 16, BW, PB, NPlace<EL>>(lane, at, w2 + (int64_t)next_n * p.r + (next_piece * PR < p.r ? next_piece * PR : 0),
                                                     p.r, p.r - next_piece * PR, p.N - next_n);
         } else {
@@ -1087,8 +832,9 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
         for (int h = 0; h < 2; ++h) {                  // a lane's columns: pieces q and q + 4
           if (n0 + (q + 4 * h) * EL >= p.N) continue;
           T* y = yp[i] + n0 + 4 * h * EL;
+          const uint32_t here = at + row * 128 + swap(q + 4 * h, row);
           uint32_t bw[4] = {0, 0, 0, 0};
-          if (p.base != nullptr) lds(at + row * 128 + swap(q + 4 * h, row), bw);
+          if (p.base != nullptr) lds(here, bw);
           float o[EL];
 #pragma unroll
           for (int e = 0; e < EL; ++e) {
@@ -1096,11 +842,37 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
             const float v = c[i >> 1][t][2 * (i & 1) + odd], b = elem<T>(bw, e);
             o[e] = kHalves<T> ? fmaf(v, factor, b) : v + b;
           }
+          uint4 bits;
           if constexpr (SZ == 4)
-            *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
+            bits = make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
           else
-            *reinterpret_cast<uint4*>(y) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
-                                                      pack2<T>(o[6], o[7]));
+            bits = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+          if constexpr (RAGGED)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(here), "r"(bits.x), "r"(bits.y), "r"(bits.z), "r"(bits.w)
+                         : "memory");
+          else
+            *reinterpret_cast<uint4*>(y) = bits;
+        }
+      }
+      if constexpr (RAGGED) {                          // in place of base, and from there by rows
+        __syncwarp();
+        const int left = p.N - n0 - lane * (4 / SZ);
+#pragma unroll 4
+        for (int row = 0; row < n; ++row) {
+          uint32_t w[1];
+          lds(at + row * 128 + swap(lane >> 2, row) + 4 * (lane & 3), w);
+          T* y = static_cast<T*>(p.y) + (int64_t)rows[row] * p.N + n0 + lane * (4 / SZ);
+          if constexpr (SZ == 4) {
+            if (left > 0) *reinterpret_cast<uint32_t*>(y) = w[0];
+          } else {
+            uint16_t* u = reinterpret_cast<uint16_t*>(y);
+            if (!p.half && left > 1) {
+              *reinterpret_cast<uint32_t*>(y) = w[0];
+            } else {
+              if (left > 0) u[0] = (uint16_t)w[0];
+              if (left > 1) u[1] = (uint16_t)(w[0] >> 16);
+            }
+          }
         }
       }
       pi = 0;
@@ -1122,8 +894,10 @@ struct OuterRing {
   static_assert(RT * BW * 4 <= kBytes, "a warp's part of the gradient fits into its ring");
 };
 
-// Two gradients in one launch: the first blocks are of the first.
-template <typename T, int RT>
+// out[a] = sum over a's rows of v[m]^T x[m], two gradients in one launch: the first blocks are of the first. RT: ranks of a block, 16 or
+// 32 (blockIdx.z: which). A cluster shares 128 bytes of columns of an adapter's gradient; its warps split the rows, and
+// the parts are added in a fixed order.
+template <typename T, int RT, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constant__ OuterPair pair) {
   using L = OuterRing<T, RT>;
   const int second = (int)blockIdx.x >= pair.of[0].blocks;
@@ -1157,19 +931,34 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
       group += W * 16;
       next = index_of(group);
       const uint32_t at = ring + slot * L::kStage;
+      if constexpr (RAGGED) {
+        const T* x = static_cast<const T*>(p.x);
+        const int col = n0 + lane * (4 / (int)sizeof(T));
+        copy_words<T, 16>(p.half, x, [&](int row) {
+          const int m = __shfl_sync(0xffffffffu, mine, row), turn = kPairs<T> ? row >> 1 & 3 : row & 3;
+          return Word<T>{at + row * 128 + (((lane >> 2) ^ (2 * turn)) * 16) + 4 * (lane & 3),
+                         m >= 0 ? x + (int64_t)m * p.ldx + col : nullptr, p.K - col};
+        });
+        copy_words<float, RT / 2>(false, p.v, [&](int i) {
+          const int id = lane + 32 * i, row = id / RT, rk = id % RT, m = __shfl_sync(0xffffffffu, mine, row);
+          return Word<float>{at + 2048 + row * L::kPitch + 4 * rk, m >= 0 ? p.v + (int64_t)m * p.r + r0 + rk : nullptr,
+                             p.r - r0 - rk};
+        });
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = (lane >> 3) + 4 * j;
-        const int m = __shfl_sync(0xffffffffu, mine, row);
-        const int turn = kPairs<T> ? row >> 1 & 3 : row & 3;           // a fragment's four rows at four places
-        copy16(at + row * 128 + (((lane & 7) ^ (2 * turn)) * 16), xc + (uint64_t)(uint32_t)max(m, 0) * p.pitch, in && m >= 0);
-      }
+        for (int j = 0; j < 4; ++j) {
+          const int row = (lane >> 3) + 4 * j;
+          const int m = __shfl_sync(0xffffffffu, mine, row);
+          const int turn = kPairs<T> ? row >> 1 & 3 : row & 3;         // a fragment's four rows at four places
+          copy16(at + row * 128 + (((lane & 7) ^ (2 * turn)) * 16), xc + (uint64_t)(uint32_t)max(m, 0) * p.pitch, in && m >= 0);
+        }
 #pragma unroll
-      for (int j = 0; j < 16 / VS; ++j) {
-        const int row = lane / VC + VS * j;
-        const int m = __shfl_sync(0xffffffffu, mine, row);
-        copy16(at + 2048 + row * L::kPitch + 16 * (lane % VC), vc + (uint64_t)(uint32_t)max(m, 0) * (uint32_t)(4 * p.r),
-               v_in && m >= 0);
+        for (int j = 0; j < 16 / VS; ++j) {
+          const int row = lane / VC + VS * j;
+          const int m = __shfl_sync(0xffffffffu, mine, row);
+          copy16(at + 2048 + row * L::kPitch + 16 * (lane % VC), vc + (uint64_t)(uint32_t)max(m, 0) * (uint32_t)(4 * p.r),
+                 v_in && m >= 0);
+        }
       }
     }
     slot = slot + 1 == S ? 0 : slot + 1;
@@ -1298,27 +1087,27 @@ inline int64_t max_tiles(int64_t M, int L, int r, bool indexed, bool planned) {
   return all < M ? all : M;
 }
 
-template <typename T, int RT, int MT, bool TRANS>
+template <typename T, int RT, int MT, bool TRANS, bool RAGGED>
 cudaError_t launch_ring(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
   // blocks of a tile: while the tiles alone do not fill the GPU's places
   const int places = (RT == 16 ? 2 : 1) * num_sms();
   p.cluster = 1;
   while (p.cluster < 8 && likely * p.cluster * 2 <= places) p.cluster *= 2;
-  return launch_clusters<lora_kernel<T, RT, MT, TRANS>>(p, dim3((unsigned)(tiles * p.cluster)), Ring<T, RT, MT>::kSmem, st);
+  return launch_clusters<lora_kernel<T, RT, MT, TRANS, RAGGED>>(p, dim3((unsigned)(tiles * p.cluster)), Ring<T, RT, MT>::kSmem, st);
 }
-template <typename T, int RT, bool TRANS>
-cudaError_t launch_any(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
-  p.cluster = 1;
-  while (p.cluster < 8 && likely * p.cluster * 2 <= 2 * num_sms()) p.cluster *= 2;
-  return launch_clusters<lora_any_kernel<T, RT, TRANS>>(p, dim3((unsigned)(tiles * p.cluster)), smem_bytes<RT, 1>(), st);
-}
-
-// Whether every access of the ring kernels is on its boundary.
+// Whether every address is on 16 bytes (rows of ranks on 8).
 template <typename T>
 bool aligned(const Params& p) {
   constexpr int EL = 16 / (int)sizeof(T);
   return p.K % EL == 0 && p.N % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && on(p.w1, 16) && on(p.w2, 16) &&
          on(p.base, 16) && (p.M <= 1 || p.ldb % EL == 0) && on(p.y, 16) && p.r % (EL / 2) == 0;
+}
+
+// Whether some address is off 4 bytes.
+template <typename T>
+bool off_words(const Params& p) {
+  return sizeof(T) == 2 && (p.K % 2 || p.N % 2 || p.r % 2 || !on(p.x, 4) || (p.M > 1 && p.ldx % 2) || !on(p.w1, 4) || !on(p.w2, 4) ||
+                            !on(p.base, 4) || (p.M > 1 && p.ldb % 2) || !on(p.y, 4));
 }
 
 template <typename T, bool TRANS>
@@ -1329,22 +1118,27 @@ cudaError_t run_as(const Params& p, cudaStream_t st) {
   int64_t likely = (p.M + R - 1) / R + (indexed ? p.L - 1 : 0);
   if (likely > p.M) likely = p.M;
   if (aligned<T>(p)) {
-    if (p.r <= 16) return R == 32 ? launch_ring<T, 16, 2, TRANS>(p, tiles, likely, st) : launch_ring<T, 16, 1, TRANS>(p, tiles, likely, st);
-    if (p.r <= 32) return R == 32 ? launch_ring<T, 32, 2, TRANS>(p, tiles, likely, st) : launch_ring<T, 32, 1, TRANS>(p, tiles, likely, st);
-    if (p.r <= 64) return R == 32 ? launch_ring<T, 64, 2, TRANS>(p, tiles, likely, st) : launch_ring<T, 64, 1, TRANS>(p, tiles, likely, st);
-    return launch_ring<T, 128, 1, TRANS>(p, tiles, likely, st);
+#define GLAD_LORA(RT) \
+  return R == 32 ? launch_ring<T, RT, 2, TRANS, false>(p, tiles, likely, st) : launch_ring<T, RT, 1, TRANS, false>(p, tiles, likely, st)
+    if (p.r <= 16) GLAD_LORA(16);
+    if (p.r <= 32) GLAD_LORA(32);
+    if (p.r <= 64) GLAD_LORA(64);
+#undef GLAD_LORA
+    return launch_ring<T, 128, 1, TRANS, false>(p, tiles, likely, st);
   }
   // 16 rows a tile: the plan's tiles of 32 in two
   Params h = p;
+  h.half = off_words<T>(p);
   h.halves = R == 32 && p.plan != nullptr;
   int64_t all = tiles;
   if (h.halves) all = 2 * tiles;
   else if (!indexed) all = (p.M + 15) / 16;
   else if (!p.plan && p.M > kSelfRows) all = (p.M + 15) / 16 + p.L;
-  if (p.r <= 16) return launch_any<T, 16, TRANS>(h, all, likely, st);
-  if (p.r <= 32) return launch_any<T, 32, TRANS>(h, all, likely, st);
-  if (p.r <= 64) return launch_any<T, 64, TRANS>(h, all, likely, st);
-  return launch_any<T, 128, TRANS>(h, all, likely, st);
+  likely = all < likely * (R / 16) ? all : likely * (R / 16);
+  if (p.r <= 16) return launch_ring<T, 16, 1, TRANS, true>(h, all, likely, st);
+  if (p.r <= 32) return launch_ring<T, 32, 1, TRANS, true>(h, all, likely, st);
+  if (p.r <= 64) return launch_ring<T, 64, 1, TRANS, true>(h, all, likely, st);
+  return launch_ring<T, 128, 1, TRANS, true>(h, all, likely, st);
 }
 template <typename T>
 cudaError_t run(Params p, bool trans, cudaStream_t st) {
@@ -1364,6 +1158,7 @@ cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
     OuterParams& p = pair.of[i];
     tiles += (int64_t)((p.K + BW - 1) / BW) * p.L * ranks;
     p.pitch = (uint32_t)(p.ldx * (int64_t)sizeof(T));
+    p.half = sizeof(T) == 2 && (p.K % 2 || !on(p.x, 4) || (p.M > 1 && p.ldx % 2));
     ring = ring && p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && p.ldx < (int64_t)1 << 29 && on(p.v, 16);
   }
   // blocks of a tile: while every warp keeps a few groups of 16 rows and the tiles alone do not fill the GPU
@@ -1376,19 +1171,12 @@ cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
     blocks += (unsigned)pair.of[i].blocks;
   }
   pair.cluster = C;
-  if (ring) {
-    const dim3 grid(blocks, (unsigned)first.L, (unsigned)ranks);
-    return RT == 16 ? launch_clusters<outer_kernel<T, 16>>(pair, grid, OuterRing<T, 16>::kSmem, st)
-                    : launch_clusters<outer_kernel<T, 32>>(pair, grid, OuterRing<T, 32>::kSmem, st);
-  }
-  const size_t smem = (size_t)(kWarps + 1) * RT * BW * sizeof(float);
-  cudaError_t e = cudaSuccess;
-  for (int i = 0; i < count && e == cudaSuccess; ++i) {
-    const dim3 grid((unsigned)pair.of[i].blocks, (unsigned)first.L, (unsigned)ranks);
-    e = RT == 16 ? launch_clusters<outer_any_kernel<T, 16>>(pair.of[i], grid, smem, st)
-                 : launch_clusters<outer_any_kernel<T, 32>>(pair.of[i], grid, smem, st);
-  }
-  return e;
+  const dim3 grid(blocks, (unsigned)first.L, (unsigned)ranks);
+  if (RT == 16)
+    return ring ? launch_clusters<outer_kernel<T, 16, false>>(pair, grid, OuterRing<T, 16>::kSmem, st)
+                : launch_clusters<outer_kernel<T, 16, true>>(pair, grid, OuterRing<T, 16>::kSmem, st);
+  return ring ? launch_clusters<outer_kernel<T, 32, false>>(pair, grid, OuterRing<T, 32>::kSmem, st)
+              : launch_clusters<outer_kernel<T, 32, true>>(pair, grid, OuterRing<T, 32>::kSmem, st);
 }
 
 }  // namespace lora
