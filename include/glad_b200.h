@@ -449,7 +449,7 @@ int glad_w4_linear_forward(const GladW4Weight* w, const void* x, int x_dtype, in
                            const float* x_scale, int x_scale_rows, int x_scale_groups, const void* bias, void* y,
                            int y_dtype, void* stream);
 
-/* Device-side status word of glad_w4_linear_forward on the current device: 0, or
+/* Device-side status word of glad_w4_linear_forward (and of glad_lora_forward and _backward) on the current device: 0, or
  * GLAD_DEVERR_* bits when a bounded wait inside a kernel ran out since the last
  * call of this function, in which case that call's outputs are not valid; reads
  * and clears it in one step and returns GLAD_ERR_DEVICE when it was not 0. One word for the
@@ -483,11 +483,19 @@ int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t 
 /* Its backward pass: du[m] = scale[i] * b[i]^T dy[m], dx[m] = a[i]^T du[m] (contiguous),
  * da[i] = sum over i's rows of du[m] x[m]^T, db[i] = the same of dy[m] u[m]^T; the gradient of base is dy. dx, da, db of x's type,
  * each NULL: not wanted; da needs x and du (4 bytes [M, r] of workspace), db needs u; an index needs the
- * forward pass's plan. Sums have a fixed order: the same call gives the same bits. Adapters without rows get zeros.    */
+ * forward pass's plan. Sums have a fixed order: the same call gives the same bits. Adapters without rows get zeros. The workspace
+ * (16-byte aligned, its size may be 0) holds the adapters transposed for large calls; without it they take the
+ * kernel of small ones. Large calls of both directions wait, with a bound, for the tensor core: a wait that runs out is told by
+ * glad_w4_linear_status, and that call's outputs are not valid.  */
 int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, int64_t M, int64_t K, const void* a,
                        const void* b, int64_t N, int L, int r, const void* index, int index_bytes, const void* plan,
                        const float* scale, float scale_value, const float* u, float* du, void* dx, void* da, void* db,
-                       void* stream);
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t glad_lora_backward_workspace_size(int64_t M, int64_t K, int64_t N, int L, int r, int dtype, int indexed);
+
+/* Test hook of the status word: with hold 1 the tensor-core kernel's barriers wait for an arrival that never comes, for
+ * `limit_ns` nanoseconds (at most, and 0 for, the normal 2 s). (0, 0) restores normal operation. Process-wide. */
+int glad_debug_lora_wait(uint32_t hold, uint64_t limit_ns);
 
 /* ---- log probabilities of given tokens (no counterpart in the reference) -------
  * Rows of logits x [rows, cols] (f32, f16 or bf16, row stride ldx >= cols elements), a token

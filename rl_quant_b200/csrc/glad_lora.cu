@@ -1,12 +1,19 @@
 // C entries of the low-rank adapters (glad_lora.cuh), and the order of rows by adapter that larger calls need.
 #include "glad_lora.cuh"
 
+#include <atomic>
+
 namespace glad {
+cudaError_t w4_status_word(uint32_t** word);          // glad_w4.cu: the device's status word
+
 namespace lora {
 
 extern template cudaError_t run<__half>(Params, bool, cudaStream_t);
 extern template cudaError_t run<__nv_bfloat16>(Params, bool, cudaStream_t);
 extern template cudaError_t run<float>(Params, bool, cudaStream_t);
+extern template bool wants_transposed<__half>(const Params&);
+extern template bool wants_transposed<__nv_bfloat16>(const Params&);
+extern template bool wants_transposed<float>(const Params&);
 extern template cudaError_t run_outer<__half>(OuterPair, int, cudaStream_t);
 extern template cudaError_t run_outer<__nv_bfloat16>(OuterPair, int, cudaStream_t);
 extern template cudaError_t run_outer<float>(OuterPair, int, cudaStream_t);
@@ -126,6 +133,36 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   }
 }
 
+// dst[l] = src[l]^T for two sets of matrices of 16-bit elements, [rows, cols] each, in one launch: 64 x 64 elements a block.
+struct Transposes {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int rows[2], cols[2];
+};
+__global__ void __launch_bounds__(256) transpose_kernel(const Transposes p) {
+  __shared__ uint16_t tile[64][66];
+  const int which = blockIdx.z & 1, rows = p.rows[which], cols = p.cols[which];
+  const int64_t at = (int64_t)(blockIdx.z >> 1) * rows * cols;
+  const int tall = rows > cols;                         // the long side runs along blockIdx.x
+  const int r0 = (tall ? blockIdx.x : blockIdx.y) * 64, c0 = (tall ? blockIdx.y : blockIdx.x) * 64;
+  if (r0 >= rows || c0 >= cols) return;
+  grid_dep_wait();
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int i = y; i < 64; i += 4)
+    if (r0 + i < rows && c0 + x < cols) tile[i][x] = p.src[which][at + (int64_t)(r0 + i) * cols + c0 + x];
+  __syncthreads();
+  for (int i = y; i < 64; i += 4)
+    if (c0 + i < cols && r0 + x < rows) p.dst[which][at + (int64_t)(c0 + i) * rows + r0 + x] = tile[x][i];
+}
+
+std::atomic<uint32_t> g_hold{0}, g_wait_ns{2000000000u};
+
+// What the tensor-core kernel needs beside the operands.
+cudaError_t tensor_setup(Params& p) {
+  p.wait_ns = g_wait_ns, p.hold = g_hold;
+  return w4_status_word(&p.status);
+}
+
 template <typename F>
 cudaError_t for_type(int dtype, F&& f) {
   if (dtype == GLAD_DTYPE_F16) return f(__half());
@@ -145,14 +182,14 @@ const char* shape_wrong(int dtype, int64_t M, int64_t K, int64_t N, int L, int r
   return nullptr;
 }
 
-int64_t plan_words(int64_t M, int L) { return 3 + L + M + 2 * max_tiles(M, L, kMaxRank, true, true); }
+int64_t plan_words(int64_t M, int L) { return 3 + L + M + 2 * max_tiles(M, L, 16, true, true); }
 
-cudaError_t make_plan(const void* index, int index_bytes, int64_t M, int L, int r, void* plan, cudaStream_t st) {
+cudaError_t make_plan(const void* index, int index_bytes, int64_t M, int L, int r, bool wide16, void* plan, cudaStream_t st) {
   static size_t limit[64] = {};
   // counting warps: 256 rows each if possible, which they hold in registers; as many as shared memory has counters for
   int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
   if (M < 256 * warps) warps = (int)((M + 255) / 256);
-  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true)};
+  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true, wide16)};
   const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
   const cudaError_t e = allow_smem(plan_kernel, smem, limit);
   if (e != cudaSuccess) return e;
@@ -195,15 +232,30 @@ int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t 
   p.x = x, p.ldx = ldx, p.M = (int)M, p.K = (int)K, p.N = (int)N, p.w1 = a, p.w2 = b, p.L = L, p.r = r;
   p.index = index, p.index64 = index_bytes == 8, p.plan = static_cast<const int32_t*>(plan);
   p.scale = scale, p.scale_value = scale_value, p.base = base, p.ldb = base ? ldb : 0, p.y = y, p.u = u;
-  cudaError_t e = plan ? make_plan(index, index_bytes, M, L, r, plan, (cudaStream_t)stream) : cudaSuccess;
+  cudaError_t e = tensor_setup(p);
+  if (plan && e == cudaSuccess) e = make_plan(index, index_bytes, M, L, r, dtype != GLAD_DTYPE_F32, plan, (cudaStream_t)stream);
   if (e == cudaSuccess) e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, false, (cudaStream_t)stream); });
   return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
+}
+
+size_t glad_lora_backward_workspace_size(int64_t M, int64_t K, int64_t N, int L, int r, int dtype, int indexed) {
+  if (M < 1 || K < 1 || N < 1 || L < 1 || L > kMaxAdapters || r < 1 || r > kMaxRank) return 0;
+  if (r % 8 || !tensor_sized(M, L, r, indexed != 0, dtype != GLAD_DTYPE_F32)) return 0;
+  return (size_t)L * (size_t)r * (size_t)(K + N) * 2;
+}
+
+int glad_debug_lora_wait(uint32_t hold, uint64_t limit_ns) {
+  if (hold > 1 || limit_ns > 2000000000ull)
+    return set_last_error(GLAD_ERR_INVALID_ARG, "glad_debug_lora_wait: hold above 1 or limit_ns above 2 s");
+  g_hold = hold;
+  g_wait_ns = limit_ns ? (uint32_t)limit_ns : 2000000000u;
+  return GLAD_OK;
 }
 
 int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, int64_t M, int64_t K, const void* a,
                        const void* b, int64_t N, int L, int r, const void* index, int index_bytes, const void* plan,
                        const float* scale, float scale_value, const float* u, float* du, void* dx, void* da, void* db,
-                       void* stream) {
+                       void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "glad_lora_backward";
   const char* why = shape_wrong(dtype, M, K, N, L, r, index, index_bytes);
   if (why) return bad(who, why);
@@ -230,7 +282,24 @@ int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, i
     p.x = dy, p.ldx = lddy, p.M = (int)M, p.K = (int)N, p.N = (int)K, p.w1 = b, p.w2 = a, p.L = L, p.r = r;
     p.index = index, p.index64 = index_bytes == 8, p.plan = static_cast<const int32_t*>(plan);
     p.scale = scale, p.scale_value = scale_value, p.y = dx, p.u = da ? du : nullptr;
-    e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, true, st); });
+    e = tensor_setup(p);
+    const size_t need = glad_lora_backward_workspace_size(M, K, N, L, r, dtype, index != nullptr);
+    bool transposed = false;
+    for_type(dtype, [&](auto t) {
+      transposed = need && workspace && workspace_bytes >= need && on(workspace, 16) && wants_transposed<decltype(t)>(p);
+      return cudaSuccess;
+    });
+    if (transposed && e == cudaSuccess) {              // b [L, N, r] -> [L, r, N], a [L, r, K] -> [L, K, r]
+      Transposes t{};
+      uint16_t* ws = static_cast<uint16_t*>(workspace);
+      t.src[0] = static_cast<const uint16_t*>(b), t.dst[0] = ws, t.rows[0] = (int)N, t.cols[0] = r;
+      t.src[1] = static_cast<const uint16_t*>(a), t.dst[1] = ws + (size_t)L * r * N, t.rows[1] = r, t.cols[1] = (int)K;
+      const int64_t longest = N > K ? N : K;
+      const unsigned wide = longest <= kMaxRank ? kMaxRank / 64 : (unsigned)((longest + 63) / 64);
+      e = launch_k(transpose_kernel, dim3(wide, kMaxRank / 64, 2 * L), dim3(256), 0, st, true, t);
+      p.w1 = t.dst[0], p.w2 = t.dst[1];
+    }
+    if (e == cudaSuccess) e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, !transposed, st); });
   }
   // db first: dy has just been read
   OuterPair pair{};

@@ -12,6 +12,8 @@
 // u is fp32 and stays so: as an operand it is split into two tf32 numbers (22 bits). Inputs of 16 bits are exact in tf32;
 // fp32 inputs are split the same way, three products each.
 #pragma once
+#include <utility>
+
 #include "glad_elem.cuh"
 #include "tc05.cuh"
 
@@ -48,8 +50,11 @@ struct Params {
   int64_t ldx, ldb;
   float scale_value;
   int M, K, N, r, L, index64, cluster;
-  int halves;           // a tile of the plan (32 rows) is taken as two of 16
+  int split;            // tiles of the kernel in a tile of the plan
   int half;             // some address off 4 bytes
+  // of the tensor-core kernel: the device's status word, the longest wait, and arrivals to wait for that never come (tests)
+  uint32_t* status;
+  uint32_t wait_ns, hold;
 };
 
 struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
@@ -150,11 +155,11 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
     if (tid < n) rows[tid] = tile * R + tid;
   } else if (p.plan != nullptr) {
     const Plan plan{p.plan, p.L, p.M};
-    const int whole = p.halves ? tile >> 1 : tile;
+    const int whole = tile / p.split;
     if (whole >= plan.tiles()) return 0;
     const int2 t = plan.tile(whole);
     adapter = t.x;
-    const int from = t.y + (p.halves ? (tile & 1) * R : 0);
+    const int from = t.y + tile % p.split * R;
     n = min(R, plan.first((adapter < 0 ? p.L : adapter) + 1) - from);
     if (n <= 0) return 0;
     if (tid < n) rows[tid] = plan.row(from + tid);
@@ -267,6 +272,13 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
   const float2 f = __half22float2(h);
   const __half2 l = __floats2half2_rn(fmaxf(a - f.x, -3e38f), fmaxf(b - f.y, -3e38f));
   lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// A row's power of two and its inverse: brings its largest number (as bits) to 2^14, so that the lower halves reach 2^-38 of it.
+__device__ __forceinline__ void row_power(uint32_t most, float& up, float& down) {
+  int e = 14 - ((int)(most >> 23) - 127);
+  if (most == 0 || most >= 0x7f800000u) e = 0;
+  e = min(max(e, -126), 126);
+  up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 // u and du as they are kept: the two bf16 numbers side by side, or fp32.
 template <typename T>
@@ -726,15 +738,11 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
     }
     __syncthreads();
     if constexpr (kHalves<T>) {
-      // a row's power of two: its largest number to 2^14, so that the lower halves reach 2^-38 of it
       for (int row = warp; row < R; row += kWarps) {
         float most = 0.0f;
         for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(whole[row * RT + i]));
         const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-        int e = 14 - ((int)(bits >> 23) - 127);
-        if (bits == 0 || bits >= 0x7f800000u) e = 0;
-        e = min(max(e, -126), 126);
-        if (lane == 0) up[row] = __uint_as_float((uint32_t)(127 + e) << 23), down[row] = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (lane == 0) row_power(bits, up[row], down[row]);
       }
       __syncthreads();
     }
@@ -1041,6 +1049,293 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
                        L::kBytes / 4, a, r0, n0, rank, C);
 }
 
+// ---- many rows an adapter, ranks above 32: both products on the tensor core's own memory -------------
+// At these ranks mma.sync is the bound (8192 rows 4096 -> 4096 bf16: rank 128 159 us with the rings, @T128@ here; rank 64 @R64@ and
+// @T64@), and a tile of 32 rows reads the adapter too often. So: tiles of 128 rows, u summed in tensor memory by tcgen05 while
+// all warps keep four stages of x and A in flight, then u as two 16-bit numbers (as in the rings) times 128 columns of B
+// a step, base and y through shared memory. Operands lie K-major with the 128-byte swizzle; the backward pass
+// gets its adapters transposed first (transpose_kernel), which are small.
+template <int RT>
+struct Tc {
+  static constexpr int kStages = 4, kStage = 128 * 128 + RT * 128, NB = RT / 64;       // NB: blocks of 64 ranks
+  static constexpr int kPart = 128 * RT * 4, kB = NB * 16384, kBase = 32768;
+  // first product: the ring; sums: [part][u]; second: [B, two][base, two]; u's operand behind all of them
+  static constexpr int kBaseAt = 2 * kB, kA = 2 * kB + 2 * kBase;
+  static constexpr int kSmem = kA + 2 * NB * 16384 + 1024;
+  static_assert(kStages * kStage <= kA && 2 * kPart <= kA, "u's operand lies behind what is read while it is written");
+};
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {      // rows of 128 bytes, piece i of row r at i ^ (r & 7)
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ int turned(int piece, int row) { return (piece ^ (row & 7)) * 16; }
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+// Waits for the products behind a phase; after one wait that ran out no other one waits, the bit is set and the kernel ends as usual.
+__device__ __forceinline__ void tc_wait(uint64_t* bar, uint32_t parity, const Params& p, bool& dead) {
+  if (dead || mbar_try_wait(bar, parity)) return;
+  if (mbar_wait_bounded(bar, parity, p.wait_ns)) return;
+  dead = true;
+  atomicOr(p.status, kDevErrMmaTimeout);
+}
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
+  using L = Tc<RT>;
+  constexpr int R = 128, S = L::kStages, NB = L::NB;
+  constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+  constexpr uint32_t kFirst = idesc_f16(128, RT) | kType, kSecond = idesc_f16(128, 128) | kType;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int rows[R];
+  __shared__ float up[R], down[R];
+  __shared__ __align__(8) uint64_t full[S], done[2], drain;
+  __shared__ uint32_t tmem_at;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
+  grid_dep_wait();
+  int adapter;
+  const int n = find_rows<R>(p, tile, rows, adapter, smem);
+  if (n == 0) return;                                 // the whole cluster
+  const bool any = adapter >= 0;
+  if (warp == 0) tmem_alloc(&tmem_at, 512);
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&full[i], 1 + p.hold);
+    mbar_init(&done[0], 1 + p.hold);
+    mbar_init(&done[1], 1 + p.hold);
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at, base_addr = smem_u32(smem);
+  bool dead = false;
+
+  if (any) {
+    const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
+    const int row0 = tid >> 3, c = tid & 7;
+    const T* xp[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xp[j] = static_cast<const T*>(p.x) + (int64_t)rows[row0 + 32 * j] * p.ldx + c * 8;
+    const int chunks = (p.K + 63) / 64, mine = rank < chunks ? (chunks - rank + C - 1) / C : 0;
+    auto fetch = [&](int i) {
+      if (i < mine) {
+        const int k = (rank + i * C) * 64;
+        const bool live = k + c * 8 < p.K;
+        const uint32_t at = base_addr + i % S * L::kStage;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = row0 + 32 * j;
+          const bool in = live && row < n;
+          copy16(at + row * 128 + turned(c, row), in ? xp[j] + k : static_cast<const T*>(p.x), in);
+        }
+#pragma unroll
+        for (int j = 0; j < RT / 32; ++j) {
+          const int row = row0 + 32 * j;
+          const bool in = live && row < p.r;
+          copy16(at + 16384 + row * 128 + turned(c, row), in ? w1 + (int64_t)row * p.K + k + c * 8 : w1, in);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) fetch(i);
+    for (int i = 0; i < mine; ++i) {
+      cp_async_wait_group<S - 2>();
+      fence_async_smem();
+      __syncthreads();
+      if (warp == 0) {
+        tc_fence_after();
+        const uint32_t at = base_addr + i % S * L::kStage;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_f16_warp(tmem, desc_sw128(at) + 2 * k, desc_sw128(at + 16384) + 2 * k, kFirst, i > 0 || k > 0 ? 1u : 0u);
+        mma_commit_warp(&full[i % S]);
+      }
+      if (i > 0) tc_wait(&full[(i - 1) % S], ((i - 1) / S) & 1, p, dead);      // its stage is filled next
+      fetch(i + S - 1);
+    }
+    if (mine > 0) tc_wait(&full[(mine - 1) % S], ((mine - 1) / S) & 1, p, dead);
+    cp_async_wait_all();
+    tc_fence_after();
+    __syncthreads();
+    // this block's part of u: row 32 (warp % 4) + lane, half of the ranks
+    const int row = (warp & 3) * 32 + lane;
+#pragma unroll 1
+    for (int col = (warp >> 2) * (RT / 2); col < ((warp >> 2) + 1) * (RT / 2); col += 16) {
+      uint32_t v[16] = {};
+      if (mine > 0) {
+        tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + col, v);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(smem + row * RT * 4 + turned(col / 4 + i, row)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+    tc_fence_before();
+  }
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  if (any) {
+    const float s = p.scale ? p.scale[adapter] : p.scale_value;
+    uint8_t* whole = smem + L::kPart;
+    for (int i = tid; i < R * RT / 4; i += kThreads) {
+      const int row = i / (RT / 4), piece = i % (RT / 4), at = row * RT * 4 + turned(piece, row);
+      float4 v = ld_cluster4(mapa_shared(base_addr + at, 0));
+      for (int c = 1; c < C; ++c) {
+        const float4 o = ld_cluster4(mapa_shared(base_addr + at, c));
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      v.x *= s, v.y *= s, v.z *= s, v.w *= s;
+      *reinterpret_cast<float4*>(whole + at) = v;
+      if (p.u && rank == 0 && row < n) {
+        float* u = p.u + (int64_t)rows[row] * p.r + 4 * piece;
+        const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * piece + e < p.r) u[e] = kept<T>(f[e]);
+      }
+    }
+    __syncthreads();
+    if constexpr (kHalves<T>) {                        // a row's power of two, as in the rings
+      const int row = tid >> 1;
+      float most = 0.0f;
+      for (int i = 0; i < RT / 8; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(whole + row * RT * 4 + turned((tid & 1) * (RT / 8) + i, row));
+        most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+      }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      row_power(__float_as_uint(most), up[row], down[row]);
+      __syncthreads();
+    }
+    for (int i = tid; i < R * RT / 8; i += kThreads) {
+      const int row = i / (RT / 8), c8 = i % (RT / 8);
+      const float4 a = *reinterpret_cast<const float4*>(whole + row * RT * 4 + turned(2 * c8, row));
+      const float4 b = *reinterpret_cast<const float4*>(whole + row * RT * 4 + turned(2 * c8 + 1, row));
+      uint4 hi, lo;
+      if constexpr (kHalves<T>) {
+        const float f = up[row];
+        split_f16(a.x * f, a.y * f, hi.x, lo.x), split_f16(a.z * f, a.w * f, hi.y, lo.y);
+        split_f16(b.x * f, b.y * f, hi.z, lo.z), split_f16(b.z * f, b.w * f, hi.w, lo.w);
+      } else {
+        split_bf16(a.x, a.y, hi.x, lo.x), split_bf16(a.z, a.w, hi.y, lo.y);
+        split_bf16(b.x, b.y, hi.z, lo.z), split_bf16(b.z, b.w, hi.w, lo.w);
+      }
+      uint8_t* at = smem + L::kA + c8 / 8 * 16384 + row * 128 + turned(c8 & 7, row);
+      *reinterpret_cast<uint4*>(at) = hi;
+      *reinterpret_cast<uint4*>(at + NB * 16384) = lo;
+    }
+    fence_async_smem();
+  }
+  if (C > 1) cluster_sync_all();                       // nobody reads another block's part any more
+  else __syncthreads();
+
+  const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(any ? adapter : 0) * p.N * p.r;
+  const int tiles = (p.N + 127) / 128, steps = p.y != nullptr && rank < tiles ? (tiles - rank + C - 1) / C : 0;
+  auto fetch2 = [&](int j) {
+    if (j < steps) {
+      const int n0 = (rank + j * C) * 128;
+      if (any) {
+        const uint32_t at = base_addr + (j & 1) * L::kB;
+        const int row0 = tid >> 3, c = tid & 7;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = row0 + 32 * i, rk = 64 * b + 8 * c;
+            const bool in = n0 + row < p.N && rk < p.r;
+            copy16(at + b * 16384 + row * 128 + turned(c, row), in ? w2 + (int64_t)(n0 + row) * p.r + rk : w2, in);
+          }
+      }
+      if (p.base != nullptr) {
+        const uint32_t at = base_addr + L::kBaseAt + (j & 1) * L::kBase;
+        const int row0 = tid >> 4, c = tid & 15;
+        const T* base = static_cast<const T*>(p.base);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = row0 + 16 * i;
+          const bool in = row < n && n0 + 8 * c < p.N;
+          copy16(at + row * 256 + turned(c, row), in ? base + (int64_t)rows[row] * p.ldb + n0 + 8 * c : base, in);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  fetch2(0);
+  for (int j = 0; j < steps; ++j) {
+    fetch2(j + 1);
+    cp_async_wait_group<1>();
+    fence_async_smem();
+    __syncthreads();
+    const uint32_t d = tmem + 128 + (j & 1) * 128;
+    if (any) {
+      if (warp == 0) {
+        tc_fence_after();
+        const uint32_t a = base_addr + L::kA, b = base_addr + (j & 1) * L::kB;
+#pragma unroll
+        for (int half = 1; half >= 0; --half)          // the smaller numbers first
+#pragma unroll
+          for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_f16_warp(d, desc_sw128(a + (half * NB + blk) * 16384) + 2 * k, desc_sw128(b + blk * 16384) + 2 * k, kSecond,
+                           half == 1 && blk == 0 && k == 0 ? 0u : 1u);
+        mma_commit_warp(&done[j & 1]);
+      }
+      tc_wait(&done[j & 1], (j >> 1) & 1, p, dead);
+      __syncwarp();
+      tc_fence_after();
+    }
+    {
+      const int row = (warp & 3) * 32 + lane;
+      const float f = kHalves<T> && any ? down[row] : 1.0f;
+      uint8_t* line = smem + L::kBaseAt + (j & 1) * L::kBase + row * 256;
+#pragma unroll 1
+      for (int col = (warp >> 2) * 64; col < (warp >> 2) * 64 + 64; col += 16) {
+        uint32_t v[16] = {};
+        if (any) {
+          tmem_ld16(d + ((uint32_t)((warp & 3) * 32) << 16) + col, v);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4* at = reinterpret_cast<uint4*>(line + turned(col / 8 + h, row));
+          const uint4 b = p.base != nullptr ? *at : make_uint4(0, 0, 0, 0);
+          const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[e] = pack2<T>(fmaf(__uint_as_float(v[8 * h + 2 * e]), f, elem<T>(bw, 2 * e)),
+                            fmaf(__uint_as_float(v[8 * h + 2 * e + 1]), f, elem<T>(bw, 2 * e + 1)));
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      tc_fence_before();
+    }
+    __syncthreads();
+    const int n0 = (rank + j * C) * 128, c = tid & 15;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = (tid >> 4) + 16 * i;
+      if (row < n && n0 + 8 * c < p.N)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + (int64_t)rows[row] * p.N + n0 + 8 * c) =
+            *reinterpret_cast<const uint4*>(smem + L::kBaseAt + (j & 1) * L::kBase + row * 256 + turned(c, row));
+    }
+    __syncthreads();
+  }
+  cp_async_wait_all();
+  if (dead) {                                          // products may still be on their way: they take microseconds
+    if (warp == 0) mma_commit_warp(&drain);
+    mbar_wait_bounded(&drain, 0, 10000000);
+  }
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
 // Allows a kernel its dynamic shared memory, once a device (the call costs as much as a launch). `limit`: 0 or what was allowed.
 template <typename K>
 cudaError_t allow_smem(K* kernel, size_t smem, size_t (&limit)[64]) {
@@ -1074,13 +1369,21 @@ cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st)
   return cudaLaunchKernelEx(&cfg, Kernel, p);
 }
 
-// Rows of a tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
-inline int tile_rows(int64_t M, int L, int r, bool indexed) {
-  if (r > 64) return 16;
-  return M > 16 * (int64_t)(indexed ? L : 1) ? 32 : 16;
+// Whether the tensor-core kernel takes the call (if every address is on 16 bytes): 16-bit rows, ranks above 32, and half a tile of rows
+// an adapter on average.
+inline bool tensor_sized(int64_t M, int L, int r, bool indexed, bool wide16) {
+  return wide16 && r > 32 && M >= 64 * (int64_t)(indexed ? L : 1);
 }
-inline int64_t max_tiles(int64_t M, int L, int r, bool indexed, bool planned) {
-  const int R = tile_rows(M, L, r, indexed);
+// Rows of a ring kernel's tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
+inline int ring_rows(int64_t M, int L, int r, bool indexed) {
+  return r <= 64 && M > 16 * (int64_t)(indexed ? L : 1) ? 32 : 16;
+}
+// Rows of a tile of the plan: the larger of what the kernels of both directions may take.
+inline int tile_rows(int64_t M, int L, int r, bool indexed, bool wide16) {
+  return tensor_sized(M, L, r, indexed, wide16) ? 128 : ring_rows(M, L, r, indexed);
+}
+// Clusters for tiles of R rows.
+inline int64_t max_tiles(int64_t M, int L, int R, bool indexed, bool planned) {
   if (!indexed) return (M + R - 1) / R;
   if (!planned && M <= kSelfRows) return M;
   const int64_t all = (M + R - 1) / R + L + 1;
@@ -1110,39 +1413,58 @@ bool off_words(const Params& p) {
                             !on(p.base, 4) || (p.M > 1 && p.ldb % 2) || !on(p.y, 4));
 }
 
+template <typename T, int RT>
+cudaError_t launch_tc(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
+  p.cluster = 1;
+  while (p.cluster < 4 && likely * p.cluster * 2 <= num_sms()) p.cluster *= 2;     // clusters of 8 such blocks leave SMs empty
+  return launch_clusters<lora_tc_kernel<T, RT>>(p, dim3((unsigned)(tiles * p.cluster)), Tc<RT>::kSmem, st);
+}
+
 template <typename T, bool TRANS>
-cudaError_t run_as(const Params& p, cudaStream_t st) {
-  const bool indexed = p.index != nullptr;
-  const int R = tile_rows(p.M, p.L, p.r, indexed);
-  const int64_t tiles = max_tiles(p.M, p.L, p.r, indexed, p.plan != nullptr);
-  int64_t likely = (p.M + R - 1) / R + (indexed ? p.L - 1 : 0);
-  if (likely > p.M) likely = p.M;
-  if (aligned<T>(p)) {
-#define GLAD_LORA(RT) \
-  return R == 32 ? launch_ring<T, RT, 2, TRANS, false>(p, tiles, likely, st) : launch_ring<T, RT, 1, TRANS, false>(p, tiles, likely, st)
+cudaError_t run_as(Params p, cudaStream_t st) {
+  const bool indexed = p.index != nullptr, planned = p.plan != nullptr;
+  const int whole = tile_rows(p.M, p.L, p.r, indexed, sizeof(T) == 2);
+  const bool on16 = aligned<T>(p);
+  auto tiles_of = [&](int R) {             // and how many of them are likely to have rows
+    p.split = planned ? whole / R : 1;
+    const int64_t tiles = planned ? max_tiles(p.M, p.L, whole, indexed, true) * p.split : max_tiles(p.M, p.L, R, indexed, false);
+    int64_t likely = (p.M + R - 1) / R + (indexed ? p.L - 1 : 0);
+    if (likely > p.M) likely = p.M;
+    return std::pair<int64_t, int64_t>(tiles, likely < tiles ? likely : tiles);
+  };
+  if constexpr (!TRANS && sizeof(T) == 2) {
+    if (on16 && p.r % 8 == 0 && tensor_sized(p.M, p.L, p.r, indexed, true)) {
+      const auto t = tiles_of(128);
+      return p.r <= 64 ? launch_tc<T, 64>(p, t.first, t.second, st) : launch_tc<T, 128>(p, t.first, t.second, st);
+    }
+  }
+  const int R = on16 ? ring_rows(p.M, p.L, p.r, indexed) : 16;
+  const auto t = tiles_of(R);
+  if (on16) {
+#define GLAD_LORA(RT)                                                                        \
+  return R == 32 ? launch_ring<T, RT, 2, TRANS, false>(p, t.first, t.second, st) \
+                 : launch_ring<T, RT, 1, TRANS, false>(p, t.first, t.second, st)
     if (p.r <= 16) GLAD_LORA(16);
     if (p.r <= 32) GLAD_LORA(32);
     if (p.r <= 64) GLAD_LORA(64);
 #undef GLAD_LORA
-    return launch_ring<T, 128, 1, TRANS, false>(p, tiles, likely, st);
+    return launch_ring<T, 128, 1, TRANS, false>(p, t.first, t.second, st);
   }
-  // 16 rows a tile: the plan's tiles of 32 in two
-  Params h = p;
-  h.half = off_words<T>(p);
-  h.halves = R == 32 && p.plan != nullptr;
-  int64_t all = tiles;
-  if (h.halves) all = 2 * tiles;
-  else if (!indexed) all = (p.M + 15) / 16;
-  else if (!p.plan && p.M > kSelfRows) all = (p.M + 15) / 16 + p.L;
-  likely = all < likely * (R / 16) ? all : likely * (R / 16);
-  if (p.r <= 16) return launch_ring<T, 16, 1, TRANS, true>(h, all, likely, st);
-  if (p.r <= 32) return launch_ring<T, 32, 1, TRANS, true>(h, all, likely, st);
-  if (p.r <= 64) return launch_ring<T, 64, 1, TRANS, true>(h, all, likely, st);
-  return launch_ring<T, 128, 1, TRANS, true>(h, all, likely, st);
+  p.half = off_words<T>(p);
+  if (p.r <= 16) return launch_ring<T, 16, 1, TRANS, true>(p, t.first, t.second, st);
+  if (p.r <= 32) return launch_ring<T, 32, 1, TRANS, true>(p, t.first, t.second, st);
+  if (p.r <= 64) return launch_ring<T, 64, 1, TRANS, true>(p, t.first, t.second, st);
+  return launch_ring<T, 128, 1, TRANS, true>(p, t.first, t.second, st);
 }
+// trans: w1 is B [L, K, r] and w2 A [L, r, N], else A [L, r, K] and B [L, N, r].
 template <typename T>
 cudaError_t run(Params p, bool trans, cudaStream_t st) {
   return trans ? run_as<T, true>(p, st) : run_as<T, false>(p, st);
+}
+// Whether a backward call goes to the tensor-core kernel once its adapters are transposed.
+template <typename T>
+bool wants_transposed(const Params& p) {
+  return sizeof(T) == 2 && p.r % 8 == 0 && tensor_sized(p.M, p.L, p.r, p.index != nullptr, true) && aligned<T>(p);
 }
 
 // One or two gradients (count).

@@ -5,5 +5,6 @@ namespace glad {
 namespace lora {
 template cudaError_t run<float>(Params, bool, cudaStream_t);
 template cudaError_t run_outer<float>(OuterPair, int, cudaStream_t);
+template bool wants_transposed<float>(const Params&);
 }  // namespace lora
 }  // namespace glad

@@ -1139,6 +1139,19 @@ bool shape_ok(int K, int N, int group) {
 int units(int K) { return (K + 127) / 128; }
 
 }  // namespace
+
+// The status word of the current device, for the kernels of other files that report through it.
+cudaError_t w4_status_word(uint32_t** word) {
+  static void* cache[64] = {};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (cache[dev] == nullptr) {
+    const cudaError_t e = cudaGetSymbolAddress(&cache[dev], g_w4_status);
+    if (e != cudaSuccess) return e;
+  }
+  *word = static_cast<uint32_t*>(cache[dev]);
+  return cudaSuccess;
+}
 }  // namespace glad
 
 using namespace glad;

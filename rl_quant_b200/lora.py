@@ -84,24 +84,32 @@ class _LoRA(torch.autograd.Function):
             d2 = _rows(dy)
             M, n = d2.shape
             L, r, K = a.shape
-            xp = dxp = dap = dbp = up = dup = ip = plan = None
+            xp = dxp = dap = dbp = up = dup = ip = plan = wsp = None
             ldx = ib = 0
+            lib, code = N.load(), _CODE[dy.dtype]
+            # one buffer: du, then the adapters transposed (large calls)
+            first = 4 * M * r + 15 & -16 if need_a else 0
+            ws_bytes = lib.glad_lora_backward_workspace_size(M, K, n, L, r, code, index is not None) if need_x or need_a else 0
+            if first or ws_bytes:
+                ws = torch.empty(first + ws_bytes, dtype=torch.uint8, device=dy.device)
+                dup = ws.data_ptr()
+                wsp = dup + first
             if need_x:
                 dx = dy.new_empty(ctx.x_shape)
                 dxp = dx.data_ptr()
             if need_a:
                 x2 = _rows(x)
                 xp, ldx = x2.data_ptr(), x2.stride(0)
-                da, du = torch.empty_like(a), dy.new_empty((M, r), dtype=torch.float32)
-                dap, dup = da.data_ptr(), du.data_ptr()
+                da = torch.empty_like(a)
+                dap = da.data_ptr()
             if need_b:
                 db = torch.empty_like(b)
                 dbp, up = db.data_ptr(), kept.data_ptr() + ctx.plan_bytes
             if index is not None:
                 ip, ib, plan = index.data_ptr(), index.element_size(), kept.data_ptr()
-            rc = N.on_device(N.load().glad_lora_backward, dy.device.index, d2.data_ptr(), _CODE[dy.dtype], d2.stride(0), xp,
+            rc = N.on_device(lib.glad_lora_backward, dy.device.index, d2.data_ptr(), code, d2.stride(0), xp,
                              ldx, M, K, a.data_ptr(), b.data_ptr(), n, L, r, ip, ib, plan,
-                             None if scale is None else scale.data_ptr(), ctx.scale, up, dup, dxp, dap, dbp)
+                             None if scale is None else scale.data_ptr(), ctx.scale, up, dup, dxp, dap, dbp, wsp, ws_bytes)
             if rc:
                 N.check(rc, "lora_linear backward")
         return dx, da, db, None, None, dy if need_base else None
@@ -114,7 +122,8 @@ def lora_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.
     x [..., K], a [L, r, K], b [L, N, r] and base have one type, float32, float16 or bfloat16; rows of x and base may have any
     stride. index [...] int64 or int32 names the adapter of each row of x; outside 0..L-1 (by custom -1) the row has none. None:
     adapter 0 for all (L = 1). scale a number, or float32 [L]. r up to 128, L up to 16384. Differentiable in x, a, b and
-    base (backward mode). Sums are float32 and the result is rounded once."""
+    base (backward mode). Sums are float32 and the result is rounded once. Large calls of high rank wait for the tensor core with a
+    bound; ``w4_status`` tells of a wait that ran out."""
     dt, shape, dev, a_shape, b_shape = x.dtype, x.shape, x.device, a.shape, b.shape
     if dt not in _CODE:
         raise TypeError(f"x is {dt}; expected float32, float16 or bfloat16")

@@ -290,16 +290,16 @@ class InferenceRunner:
         return pipe(host_obs, out)
 
     def check_status(self) -> None:
-        """Raise ``DeviceStatusError`` if any fused forward or 4-bit layer launched since the previous
+        """Raise ``DeviceStatusError`` if any fused forward, 4-bit layer or adapter launched since the previous
         check (directly or by a captured graph's replay) reported that a bounded
         device-side wait ran out; its outputs are then not valid. Reads and clears the
         status word of every workspace (one host synchronisation): call it once per PPO
-        iteration, as ``accelerate_runner`` does before each update. 4-bit layers share one
+        iteration, as ``accelerate_runner`` does before each update. 4-bit layers and adapters share one
         word a device: every runner with such layers is told of each failure there once."""
         for f in (self._fused, self._fused_critic, self._fused_ac):
             if f is not None:
                 f.check_status()
-        if any(isinstance(m, w4linear.W4Linear) for m in self.model.modules()):
+        if any(isinstance(m, (w4linear.W4Linear, LoRALinear)) for m in self.model.modules()):
             with w4linear.w4_status_reader(self.__dict__.setdefault("_w4_told", {})):
                 w4linear.w4_status(self._device())
 

@@ -188,8 +188,8 @@ def w4_status_reader(told: dict[int, int]):
 
 
 def w4_status(device=None) -> int:
-    """Device status bits of the w4_linear calls on ``device`` since this reader's last call (0: fine); where a bounded
-    wait inside a kernel ran out, raises ``DeviceStatusError``. The word is the device's: a failure of anyone's kernels
+    """Device status bits of the w4_linear and lora_linear calls on ``device`` since this reader's last call (0: fine); where a
+    bounded wait inside a kernel ran out, raises ``DeviceStatusError``. The word is the device's: a failure of anyone's kernels
     is told to every reader once. Covers the work before it in the current stream, which it synchronises."""
     from .fused import DeviceStatusError
     index = device if isinstance(device, int) or device is None else torch.device(device).index
@@ -208,7 +208,7 @@ def w4_status(device=None) -> int:
         told = _told if told is None else told
         known, told[index] = told.get(index, 0), count
     if known != count:
-        raise DeviceStatusError(f"w4_linear: device status {bits:#x}")
+        raise DeviceStatusError(f"w4_linear or lora_linear: device status {bits:#x}")
     return 0
 
 

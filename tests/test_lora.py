@@ -1,8 +1,9 @@
 """lora_linear and its gradients against the formula in 64 bits.
 
 Tolerances, fixed before the first run. One matrix instruction adds up to 17 terms aligned to the largest, each off by at most
-2^-24 of it: 2^-20 of the running sum of magnitudes. A warp runs at most K / 64 + 2 of them for u (the 16-bit products are
-exact; split fp32 ones are off by 2^-20), and the joins of warps and blocks add at most 16 roundings: so u is off by (K / 64 + 20) 2^-20 sum |x| |A|.
+2^-24 of it: 2^-20 of the running sum of magnitudes. A warp runs at most K / 64 + 2 of them for u, the tensor-core kernel (16-bit rows, ranks above 32) at most K / 16 (the 16-bit
+products are exact; split fp32 ones are off by 2^-20), and the joins of warps and blocks add at most 16 roundings: so u is off by
+(K / 64 + 20) 2^-20 sum |x| |A|, or K / 16 for K / 64.
 In y each term of u counts with its own error, splitting u is off by 2^-21 (two tf32 numbers) or 2^-17 (two bf16 ones beside
 bf16 rows), and at most 3 r / 8 + 2 instructions follow; the rounding to the type is half a step. The gradients are the same sums with other operands; rows of an adapter take the place of K.
 Inputs of one sign make the sums of magnitudes the sums themselves."""
@@ -66,7 +67,8 @@ def ref(x, a, b, i, scale, base, dy):
         s = float(scale[j]) if isinstance(scale, torch.Tensor) else scale
         U, V = s * X @ A.T, s * G @ B
         U1, V1 = s * X.abs() @ A.abs().T, s * G.abs() @ B.abs()
-        eU, eV = (k / 64 + 21) * S * U1, (n / 64 + 21) * S * V1
+        per = 16 if r > 32 and x.dtype != torch.float32 else 64
+        eU, eV = (k / per + 21) * S * U1, (n / per + 21) * S * V1
         split = 8 if x.dtype == torch.bfloat16 else 1
         more, many = (3 * r / 8 + 2 + split) * S, (3 * len(rows) / 8 + 19 + split) * S
         out[0][0][rows] += U @ B.T
@@ -111,7 +113,10 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (64, 512, 1024, 16, 64), (33, 96, 64, 32, 2), (40, 1002, 777, 9, 5), (256, 264, 136, 24, 3), (257, 64, 72, 64, 3),
          (300, 200, 320, 48, 1), (300, 72, 64, 100, 2), (130, 128, 128, 128, 2), (1000, 48, 40, 16, 130), (2050, 520, 264, 16, 2),
          (600, 1024, 1024, 33, 1),
-         (8192, 32, 24, 16, 512), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3)]
+         (8192, 32, 24, 16, 512), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3),
+         # tiles of 128 rows on the tensor core's memory: one and several, odd counts of chunks and of columns, empty adapters
+         (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
+         (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3)]
 
 
 @gpu
@@ -198,10 +203,11 @@ def test_some_gradients_only(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("r", [16, 64])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_rows_keep_to_themselves(dtype):
+def test_rows_keep_to_themselves(dtype, r):
     """A NaN or an infinity in a row of x or of base stays in that row; in an adapter, in its rows."""
-    x, a, b, i, scale, base, dy = make(90, 96, 80, 16, 4, dtype, 7)
+    x, a, b, i, scale, base, dy = make(90, 96, 80, 16, 4, dtype, 7) if r == 16 else make(290, 96, 80, r, 4, dtype, 7)
     want = lora_linear(x, a, b, i, scale, base)
     i[5], i[9] = 1, -1
     want = lora_linear(x, a, b, i, scale, base)
@@ -209,7 +215,7 @@ def test_rows_keep_to_themselves(dtype):
     bad[5, 3] = math.nan
     bad[9] = math.inf                      # a row without an adapter
     got = lora_linear(bad, a, b, i, scale, base)
-    keep = torch.ones(90, dtype=torch.bool)
+    keep = torch.ones(len(x), dtype=torch.bool)
     keep[5] = False
     assert torch.equal(got[keep], want[keep]) and got[5].isnan().all()
     ab = a.clone()
@@ -227,8 +233,8 @@ def test_rows_keep_to_themselves(dtype):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_repeats_streams_and_graphs(dtype):
-    for m in (30, 700):
-        x, a, b, i, scale, base, dy = make(m, 256, 192, 16, 5, dtype, 8)
+    for m, r in ((30, 16), (700, 16), (700, 64)):
+        x, a, b, i, scale, base, dy = make(m, 256, 192, r, 5, dtype, 8)
         leaves = [t.clone().requires_grad_() for t in (x, a, b)]
 
         def once():
@@ -253,6 +259,48 @@ def test_repeats_streams_and_graphs(dtype):
                 graph.replay()
             assert torch.equal(y1, lora_linear(x, a, b, i.flip(0), scale, base))
             assert torch.equal(y2, lora_linear(x, a, b, i.flip(0), 2.0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_ranges_of_the_split(dtype):
+    """Rows of u of very different magnitudes, and of one large number beside small ones: rows keep their relative accuracy."""
+    for m, r in ((40, 16), (300, 64), (300, 128)):
+        x, a, b, i, scale, base, dy = make(m, 256, 128, r, 1, dtype, 11, sign=True, base=False, index=None)
+        x = x * torch.logspace(-3, 2, m).to(dtype).cuda()[:, None]
+        a = a.clone()
+        a[:, 1::2] *= 2.0 ** -9
+        check(x, a, b, i, scale, base, dy * torch.logspace(0, -3, m).to(dtype).cuda()[:, None])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_waits_that_run_out(dtype):
+    """Arrivals that never come (a host switch) and a limit of a millisecond: the kernel gives up, says so in the status word, and
+    the next calls are what they were."""
+    from rl_quant_b200 import DeviceStatusError, w4_status
+    from rl_quant_b200 import _native as N
+    lib = N.load()
+    x, a, b, i, scale, base, dy = make(600, 512, 384, 64, 2, dtype, 12)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+
+    def once():
+        y = lora_linear(*leaves, i, scale, base)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    want = once()
+    assert w4_status() == 0
+    N.check(lib.glad_debug_lora_wait(1, 1_000_000))
+    try:
+        once()
+        torch.cuda.synchronize()
+    finally:
+        N.check(lib.glad_debug_lora_wait(0, 0))
+    with pytest.raises(DeviceStatusError):
+        w4_status()
+    assert w4_status() == 0
+    for _ in range(2):
+        assert all(torch.equal(u, v) for u, v in zip(once(), want))
+    assert w4_status() == 0
 
 
 @gpu
@@ -435,6 +483,9 @@ def test_refusals():
             (dict(), RuntimeError, "CUDA")):
         with pytest.raises(kind, match=what):
             call(**bad)
+    from rl_quant_b200 import _native as N
+    lib = N.load()
+    assert lib.glad_debug_lora_wait(2, 0) == lib.glad_debug_lora_wait(1, 2_000_000_001) == N.GLAD_ERR_INVALID_ARG
     big = torch.zeros(1, 8).expand(lora_mod.MAX_SIZE + 1, 8)
     with pytest.raises(ValueError, match="rows"):
         lora_linear(big, a[:1], b[:1])
