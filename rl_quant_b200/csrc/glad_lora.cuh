@@ -1057,12 +1057,15 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
 // gets its adapters transposed first (transpose_kernel), which are small.
 template <int RT>
 struct Tc {
-  static constexpr int kStages = 4, kStage = 128 * 128 + RT * 128, NB = RT / 64;       // NB: blocks of 64 ranks
+  // a stage: 128 inputs of 128 rows of x and of A, in two blocks of 64 (128 bytes) each
+  static constexpr int kStages = 3, kBlock = 128 * 128 + RT * 128, kStage = 2 * kBlock, NB = RT / 64;  // NB: blocks of 64 ranks
   static constexpr int kPart = 128 * RT * 4, kB = NB * 16384, kBase = 32768;
-  // first product: the ring; sums: [part][u]; second: [B, two][base, two]; u's operand behind all of them
-  static constexpr int kBaseAt = 2 * kB, kA = 2 * kB + 2 * kBase;
-  static constexpr int kSmem = kA + 2 * NB * 16384 + 1024;
-  static_assert(kStages * kStage <= kA && 2 * kPart <= kA, "u's operand lies behind what is read while it is written");
+  // first the ring; then [B, two][base, two][u's operand], and this block's part of u behind it or, where that is too much, over base
+  static constexpr int kBaseAt = 2 * kB, kA = 2 * kB + 2 * kBase, kBehind = kA + 2 * NB * 16384;
+  static constexpr bool kApart = RT == 64;
+  static constexpr int kPartAt = kApart ? kBehind : kBaseAt, kEnd = kApart ? kBehind + kPart : kBehind;
+  static constexpr int kSmem = (kStages * kStage > kEnd ? kStages * kStage : kEnd) + 1024;
+  static_assert(kPart <= 2 * kBase, "over base");
 };
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {      // rows of 128 bytes, piece i of row r at i ^ (r & 7)
@@ -1073,6 +1076,23 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ void st_cluster4(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_cluster1(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+// 32 consecutive columns of a warp's lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
 }
 // Waits for the products behind a phase; after one wait that ran out no other one waits, the bit is set and the kernel ends as usual.
 __device__ __forceinline__ void tc_wait(uint64_t* bar, uint32_t parity, const Params& p, bool& dead) {
@@ -1091,7 +1111,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int rows[R];
-  __shared__ float up[R], down[R];
+  __shared__ float down[kHalves<T> ? R : 1];          // what the rows of u were divided by
   __shared__ __align__(8) uint64_t full[S], done[2], drain;
   __shared__ uint32_t tmem_at;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -1115,29 +1135,68 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
   const uint32_t tmem = tmem_at, base_addr = smem_u32(smem);
   bool dead = false;
 
+  const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(any ? adapter : 0) * p.N * p.r;
+  const int tiles = (p.N + 127) / 128, steps = p.y != nullptr && rank < tiles ? (tiles - rank + C - 1) / C : 0;
+  auto fetch_b = [&](int j) {
+    if (j < steps && any) {
+      const int n0 = (rank + j * C) * 128, row0 = tid >> 3, c = tid & 7;
+      const uint32_t at = base_addr + (j & 1) * L::kB + row0 * 128 + turned(c, row0);
+      const T* src = w2 + (int64_t)(n0 + row0) * p.r + 8 * c;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = n0 + row0 + 32 * i < p.N && 64 * b + 8 * c < p.r;
+          copy16(at + b * 16384 + i * 4096, in ? src + (int64_t)(32 * i) * p.r + 64 * b : w2, in);
+        }
+    }
+    cp_async_commit();
+  };
+  auto fetch_base = [&](int j) {
+    if (j < steps && p.base != nullptr) {
+      const int n0 = (rank + j * C) * 128, row0 = tid >> 4, c = tid & 15;
+      const uint32_t at = base_addr + L::kBaseAt + (j & 1) * L::kBase + row0 * 256;
+      const T* base = static_cast<const T*>(p.base);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = row0 + 16 * i;
+        const bool in = row < n && n0 + 8 * c < p.N;
+        copy16(at + i * 4096 + turned(c, row), in ? base + (int64_t)rows[row] * p.ldb + n0 + 8 * c : base, in);
+      }
+    }
+    cp_async_commit();
+  };
   if (any) {
     const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
     const int row0 = tid >> 3, c = tid & 7;
     const T* xp[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) xp[j] = static_cast<const T*>(p.x) + (int64_t)rows[row0 + 32 * j] * p.ldx + c * 8;
-    const int chunks = (p.K + 63) / 64, mine = rank < chunks ? (chunks - rank + C - 1) / C : 0;
+    const int chunks = (p.K + 127) / 128, mine = rank < chunks ? (chunks - rank + C - 1) / C : 0;
     auto fetch = [&](int i) {
       if (i < mine) {
-        const int k = (rank + i * C) * 64;
-        const bool live = k + c * 8 < p.K;
-        const uint32_t at = base_addr + i % S * L::kStage;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = row0 + 32 * j;
-          const bool in = live && row < n;
-          copy16(at + row * 128 + turned(c, row), in ? xp[j] + k : static_cast<const T*>(p.x), in);
-        }
+        for (int b = 0; b < 2; ++b) {
+          const int k = (rank + i * C) * 128 + 64 * b;
+          const bool live = k + c * 8 < p.K;
+          const uint32_t at = base_addr + i % S * L::kStage + b * L::kBlock + row0 * 128 + turned(c, row0);   // 32 rows on: the same turn
+          if (k + 64 <= p.K && n == R && p.r == RT) {
 #pragma unroll
-        for (int j = 0; j < RT / 32; ++j) {
-          const int row = row0 + 32 * j;
-          const bool in = live && row < p.r;
-          copy16(at + 16384 + row * 128 + turned(c, row), in ? w1 + (int64_t)row * p.K + k + c * 8 : w1, in);
+            for (int j = 0; j < 4; ++j) copy16(at + j * 4096, xp[j] + k);
+#pragma unroll
+            for (int j = 0; j < RT / 32; ++j) copy16(at + 16384 + j * 4096, w1 + (int64_t)(row0 + 32 * j) * p.K + k + c * 8);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool in = live && row0 + 32 * j < n;
+              copy16(at + j * 4096, in ? xp[j] + k : static_cast<const T*>(p.x), in);
+            }
+#pragma unroll
+            for (int j = 0; j < RT / 32; ++j) {
+              const bool in = live && row0 + 32 * j < p.r;
+              copy16(at + 16384 + j * 4096, in ? w1 + (int64_t)(row0 + 32 * j) * p.K + k + c * 8 : w1, in);
+            }
+          }
         }
       }
       cp_async_commit();
@@ -1152,8 +1211,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
         tc_fence_after();
         const uint32_t at = base_addr + i % S * L::kStage;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_f16_warp(tmem, desc_sw128(at) + 2 * k, desc_sw128(at + 16384) + 2 * k, kFirst, i > 0 || k > 0 ? 1u : 0u);
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16_warp(tmem, desc_sw128(at + b * L::kBlock) + 2 * k, desc_sw128(at + b * L::kBlock + 16384) + 2 * k, kFirst,
+                         i > 0 || b > 0 || k > 0 ? 1u : 0u);
         mma_commit_warp(&full[i % S]);
       }
       if (i > 0) tc_wait(&full[(i - 1) % S], ((i - 1) / S) & 1, p, dead);      // its stage is filled next
@@ -1163,6 +1225,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
     cp_async_wait_all();
     tc_fence_after();
     __syncthreads();
+    fetch_b(0);                                        // the ring is read no more
+    fetch_b(1);
+    if (L::kApart) fetch_base(0);
     // this block's part of u: row 32 (warp % 4) + lane, half of the ranks
     const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
@@ -1174,145 +1239,129 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint4*>(smem + row * RT * 4 + turned(col / 4 + i, row)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        *reinterpret_cast<uint4*>(smem + L::kPartAt + row * RT * 4 + turned(col / 4 + i, row)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     }
     tc_fence_before();
   }
   if (C > 1) cluster_sync_all();
   else __syncthreads();
   if (any) {
+    // every block adds up its share of the rows, eight ranks a lane, and sends the operand to all
     const float s = p.scale ? p.scale[adapter] : p.scale_value;
-    uint8_t* whole = smem + L::kPart;
-    for (int i = tid; i < R * RT / 4; i += kThreads) {
-      const int row = i / (RT / 4), piece = i % (RT / 4), at = row * RT * 4 + turned(piece, row);
-      float4 v = ld_cluster4(mapa_shared(base_addr + at, 0));
-      for (int c = 1; c < C; ++c) {
-        const float4 o = ld_cluster4(mapa_shared(base_addr + at, c));
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-      }
-      v.x *= s, v.y *= s, v.z *= s, v.w *= s;
-      *reinterpret_cast<float4*>(whole + at) = v;
-      if (p.u && rank == 0 && row < n) {
-        float* u = p.u + (int64_t)rows[row] * p.r + 4 * piece;
-        const float f[4] = {v.x, v.y, v.z, v.w};
+    const int share = (R + C - 1) / C;
+    for (int from = 0; from < share * (RT / 8); from += kThreads) {
+      const int i = from + tid, row = rank * share + i / (RT / 8), c8 = i % (RT / 8);
+      const bool in = i < share * (RT / 8) && row < R;
+      float f[8] = {};
+      if (in) {
+        const uint32_t line = base_addr + L::kPartAt + row * RT * 4;
+        for (int c = 0; c < C; c += 4) {               // in order, four blocks' parts on their way
+          float4 o[8] = {};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (4 * piece + e < p.r) u[e] = kept<T>(f[e]);
-      }
-    }
-    __syncthreads();
-    if constexpr (kHalves<T>) {                        // a row's power of two, as in the rings
-      const int row = tid >> 1;
-      float most = 0.0f;
-      for (int i = 0; i < RT / 8; ++i) {
-        const float4 v = *reinterpret_cast<const float4*>(whole + row * RT * 4 + turned((tid & 1) * (RT / 8) + i, row));
-        most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-      }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      row_power(__float_as_uint(most), up[row], down[row]);
-      __syncthreads();
-    }
-    for (int i = tid; i < R * RT / 8; i += kThreads) {
-      const int row = i / (RT / 8), c8 = i % (RT / 8);
-      const float4 a = *reinterpret_cast<const float4*>(whole + row * RT * 4 + turned(2 * c8, row));
-      const float4 b = *reinterpret_cast<const float4*>(whole + row * RT * 4 + turned(2 * c8 + 1, row));
-      uint4 hi, lo;
-      if constexpr (kHalves<T>) {
-        const float f = up[row];
-        split_f16(a.x * f, a.y * f, hi.x, lo.x), split_f16(a.z * f, a.w * f, hi.y, lo.y);
-        split_f16(b.x * f, b.y * f, hi.z, lo.z), split_f16(b.z * f, b.w * f, hi.w, lo.w);
-      } else {
-        split_bf16(a.x, a.y, hi.x, lo.x), split_bf16(a.z, a.w, hi.y, lo.y);
-        split_bf16(b.x, b.y, hi.z, lo.z), split_bf16(b.z, b.w, hi.w, lo.w);
-      }
-      uint8_t* at = smem + L::kA + c8 / 8 * 16384 + row * 128 + turned(c8 & 7, row);
-      *reinterpret_cast<uint4*>(at) = hi;
-      *reinterpret_cast<uint4*>(at + NB * 16384) = lo;
-    }
-    fence_async_smem();
-  }
-  if (C > 1) cluster_sync_all();                       // nobody reads another block's part any more
-  else __syncthreads();
-
-  const T* w2 = static_cast<const T*>(p.w2) + (int64_t)(any ? adapter : 0) * p.N * p.r;
-  const int tiles = (p.N + 127) / 128, steps = p.y != nullptr && rank < tiles ? (tiles - rank + C - 1) / C : 0;
-  auto fetch2 = [&](int j) {
-    if (j < steps) {
-      const int n0 = (rank + j * C) * 128;
-      if (any) {
-        const uint32_t at = base_addr + (j & 1) * L::kB;
-        const int row0 = tid >> 3, c = tid & 7;
+          for (int e = 0; e < 4; ++e)
+            if (c + e < C) {
+              const uint32_t at = mapa_shared(line, c + e);
+              o[2 * e] = ld_cluster4(at + turned(2 * c8, row)), o[2 * e + 1] = ld_cluster4(at + turned(2 * c8 + 1, row));
+            }
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = row0 + 32 * i, rk = 64 * b + 8 * c;
-            const bool in = n0 + row < p.N && rk < p.r;
-            copy16(at + b * 16384 + row * 128 + turned(c, row), in ? w2 + (int64_t)(n0 + row) * p.r + rk : w2, in);
+          for (int e = 0; e < 4; ++e) {
+            f[0] += o[2 * e].x, f[1] += o[2 * e].y, f[2] += o[2 * e].z, f[3] += o[2 * e].w;
+            f[4] += o[2 * e + 1].x, f[5] += o[2 * e + 1].y, f[6] += o[2 * e + 1].z, f[7] += o[2 * e + 1].w;
           }
-      }
-      if (p.base != nullptr) {
-        const uint32_t at = base_addr + L::kBaseAt + (j & 1) * L::kBase;
-        const int row0 = tid >> 4, c = tid & 15;
-        const T* base = static_cast<const T*>(p.base);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = row0 + 16 * i;
-          const bool in = row < n && n0 + 8 * c < p.N;
-          copy16(at + row * 256 + turned(c, row), in ? base + (int64_t)rows[row] * p.ldb + n0 + 8 * c : base, in);
+        for (int e = 0; e < 8; ++e) f[e] *= s;
+        if (p.u && row < n && 8 * c8 < p.r) {
+          float4* u = reinterpret_cast<float4*>(p.u + (int64_t)rows[row] * p.r + 8 * c8);
+          u[0] = make_float4(kept<T>(f[0]), kept<T>(f[1]), kept<T>(f[2]), kept<T>(f[3]));
+          u[1] = make_float4(kept<T>(f[4]), kept<T>(f[5]), kept<T>(f[6]), kept<T>(f[7]));
+        }
+      }
+      uint4 hi, lo;
+      float back = 1.0f;
+      if constexpr (kHalves<T>) {                      // a row's power of two, as in the rings
+        float most = 0.0f, to;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]));
+#pragma unroll
+        for (int d = 1; d < RT / 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        row_power(__float_as_uint(most), to, back);
+        split_f16(f[0] * to, f[1] * to, hi.x, lo.x), split_f16(f[2] * to, f[3] * to, hi.y, lo.y);
+        split_f16(f[4] * to, f[5] * to, hi.z, lo.z), split_f16(f[6] * to, f[7] * to, hi.w, lo.w);
+      } else {
+        split_bf16(f[0], f[1], hi.x, lo.x), split_bf16(f[2], f[3], hi.y, lo.y);
+        split_bf16(f[4], f[5], hi.z, lo.z), split_bf16(f[6], f[7], hi.w, lo.w);
+      }
+      if (in) {
+        const uint32_t at = base_addr + L::kA + c8 / 8 * 16384 + row * 128 + turned(c8 & 7, row);
+        for (int c = 0; c < C; ++c) {
+          const uint32_t to = mapa_shared(at, c);
+          st_cluster4(to, hi);
+          st_cluster4(to + NB * 16384, lo);
+          if (kHalves<T> && c8 == 0) st_cluster1(mapa_shared(smem_u32(&down[kHalves<T> ? row : 0]), c), back);
         }
       }
     }
-    cp_async_commit();
+  }
+  if (C > 1) cluster_sync_all();                       // u is there, and nobody reads another block's part any more
+  else __syncthreads();
+
+  // The products of step j, behind those of the step before.
+  auto issue = [&](int j) {
+    if (j < steps && any && warp == 0) {
+      tc_fence_after();
+      const uint32_t d = tmem + 128 + (j & 1) * 128, a = base_addr + L::kA, b = base_addr + (j & 1) * L::kB;
+#pragma unroll
+      for (int half = 1; half >= 0; --half)            // the smaller numbers first
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16_warp(d, desc_sw128(a + (half * NB + blk) * 16384) + 2 * k, desc_sw128(b + blk * 16384) + 2 * k, kSecond,
+                         half == 1 && blk == 0 && k == 0 ? 0u : 1u);
+      mma_commit_warp(&done[j & 1]);
+    }
   };
-  fetch2(0);
+  if (!any) fetch_b(0), fetch_b(1);
+  if (!any || !L::kApart) fetch_base(0);
+  fetch_base(1);
+  cp_async_wait_group<3>();
+  fence_async_smem();
+  __syncthreads();
+  issue(0);
   for (int j = 0; j < steps; ++j) {
-    fetch2(j + 1);
-    cp_async_wait_group<1>();
+    cp_async_wait_group<1>();                          // all but base of the next step
     fence_async_smem();
     __syncthreads();
-    const uint32_t d = tmem + 128 + (j & 1) * 128;
+    issue(j + 1);
     if (any) {
-      if (warp == 0) {
-        tc_fence_after();
-        const uint32_t a = base_addr + L::kA, b = base_addr + (j & 1) * L::kB;
-#pragma unroll
-        for (int half = 1; half >= 0; --half)          // the smaller numbers first
-#pragma unroll
-          for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_f16_warp(d, desc_sw128(a + (half * NB + blk) * 16384) + 2 * k, desc_sw128(b + blk * 16384) + 2 * k, kSecond,
-                           half == 1 && blk == 0 && k == 0 ? 0u : 1u);
-        mma_commit_warp(&done[j & 1]);
-      }
       tc_wait(&done[j & 1], (j >> 1) & 1, p, dead);
       __syncwarp();
       tc_fence_after();
     }
+    fetch_b(j + 2);                                    // its place is read no more
     {
       const int row = (warp & 3) * 32 + lane;
-      const float f = kHalves<T> && any ? down[row] : 1.0f;
+      const float f = kHalves<T> && any ? down[kHalves<T> ? row : 0] : 1.0f;
+      const uint32_t d = tmem + 128 + (j & 1) * 128 + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * 64;
       uint8_t* line = smem + L::kBaseAt + (j & 1) * L::kBase + row * 256;
-#pragma unroll 1
-      for (int col = (warp >> 2) * 64; col < (warp >> 2) * 64 + 64; col += 16) {
-        uint32_t v[16] = {};
-        if (any) {
-          tmem_ld16(d + ((uint32_t)((warp & 3) * 32) << 16) + col, v);
-          tmem_ld_wait();
-        }
+      uint32_t v[2][32] = {};
+      if (any) {
+        tmem_ld32(d, v[0]);
+        tmem_ld32(d + 32, v[1]);
+        tmem_ld_wait();
+      }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4* at = reinterpret_cast<uint4*>(line + turned(col / 8 + h, row));
-          const uint4 b = p.base != nullptr ? *at : make_uint4(0, 0, 0, 0);
-          const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-          uint32_t o[4];
+      for (int h = 0; h < 8; ++h) {
+        uint4* at = reinterpret_cast<uint4*>(line + turned((warp >> 2) * 8 + h, row));
+        const uint4 b = p.base != nullptr ? *at : make_uint4(0, 0, 0, 0);
+        const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+        uint32_t o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[e] = pack2<T>(fmaf(__uint_as_float(v[8 * h + 2 * e]), f, elem<T>(bw, 2 * e)),
-                            fmaf(__uint_as_float(v[8 * h + 2 * e + 1]), f, elem<T>(bw, 2 * e + 1)));
-          *at = make_uint4(o[0], o[1], o[2], o[3]);
-        }
+        for (int e = 0; e < 4; ++e)
+          o[e] = pack2<T>(fmaf(__uint_as_float(v[h / 4][h % 4 * 8 + 2 * e]), f, elem<T>(bw, 2 * e)),
+                          fmaf(__uint_as_float(v[h / 4][h % 4 * 8 + 2 * e + 1]), f, elem<T>(bw, 2 * e + 1)));
+        *at = make_uint4(o[0], o[1], o[2], o[3]);
       }
       tc_fence_before();
     }
@@ -1326,6 +1375,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
             *reinterpret_cast<const uint4*>(smem + L::kBaseAt + (j & 1) * L::kBase + row * 256 + turned(c, row));
     }
     __syncthreads();
+    fetch_base(j + 2);
   }
   cp_async_wait_all();
   if (dead) {                                          // products may still be on their way: they take microseconds
@@ -1346,6 +1396,32 @@ cudaError_t allow_smem(K* kernel, size_t smem, size_t (&limit)[64]) {
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess && dev < 64) limit[dev] = smem;
   return e;
+}
+
+// Clusters of n such blocks that the GPU holds at once. They are placed within groups of SMs, so that fewer blocks fit in
+// larger ones: 16 clusters of 8 take two rounds (512 rows 4096 -> 4096 rank 64 bf16: @R16X8@ us, 16 of 4 @R16X4@).
+template <auto Kernel>
+int clusters_at_once(int n, size_t smem) {
+  static int cache[64][9] = {};                        // plus one
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  if (cache[dev][n] == 0) {
+    static size_t limit[64] = {};
+    if (allow_smem(Kernel, smem, limit) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)n, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int most = 0;
+    if (cudaOccupancyMaxActiveClusters(&most, Kernel, &cfg) != cudaSuccess) most = 0;
+    cache[dev][n] = most + 1;
+  }
+  return cache[dev][n] - 1;
 }
 
 template <auto Kernel, typename P>
@@ -1392,11 +1468,12 @@ inline int64_t max_tiles(int64_t M, int L, int R, bool indexed, bool planned) {
 
 template <typename T, int RT, int MT, bool TRANS, bool RAGGED>
 cudaError_t launch_ring(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
-  // blocks of a tile: while the tiles alone do not fill the GPU's places
-  const int places = (RT == 16 ? 2 : 1) * num_sms();
+  // blocks of a tile: as many as the GPU holds at once
+  constexpr auto kernel = lora_kernel<T, RT, MT, TRANS, RAGGED>;
+  constexpr size_t smem = Ring<T, RT, MT>::kSmem;
   p.cluster = 1;
-  while (p.cluster < 8 && likely * p.cluster * 2 <= places) p.cluster *= 2;
-  return launch_clusters<lora_kernel<T, RT, MT, TRANS, RAGGED>>(p, dim3((unsigned)(tiles * p.cluster)), Ring<T, RT, MT>::kSmem, st);
+  while (p.cluster < 8 && likely <= clusters_at_once<kernel>(2 * p.cluster, smem)) p.cluster *= 2;
+  return launch_clusters<kernel>(p, dim3((unsigned)(tiles * p.cluster)), smem, st);
 }
 // Whether every address is on 16 bytes (rows of ranks on 8).
 template <typename T>
@@ -1415,9 +1492,14 @@ bool off_words(const Params& p) {
 
 template <typename T, int RT>
 cudaError_t launch_tc(Params p, int64_t tiles, int64_t likely, cudaStream_t st) {
-  p.cluster = 1;
-  while (p.cluster < 4 && likely * p.cluster * 2 <= num_sms()) p.cluster *= 2;     // clusters of 8 such blocks leave SMs empty
-  return launch_clusters<lora_tc_kernel<T, RT>>(p, dim3((unsigned)(tiles * p.cluster)), Tc<RT>::kSmem, st);
+  // blocks of a tile: as many as the GPU holds at once, and no more than shorten a block's work
+  constexpr auto kernel = lora_tc_kernel<T, RT>;
+  constexpr size_t smem = Tc<RT>::kSmem;
+  auto steps = [&](int c) { return ((p.K + 127) / 128 + c - 1) / c + ((p.N + 127) / 128 + c - 1) / c; };
+  p.cluster = 8;
+  while (p.cluster > 1 && likely > clusters_at_once<kernel>(p.cluster, smem)) --p.cluster;
+  while (p.cluster > 1 && steps(p.cluster - 1) == steps(p.cluster)) --p.cluster;
+  return launch_clusters<kernel>(p, dim3((unsigned)(tiles * p.cluster)), smem, st);
 }
 
 template <typename T, bool TRANS>
@@ -1433,7 +1515,7 @@ cudaError_t run_as(Params p, cudaStream_t st) {
     return std::pair<int64_t, int64_t>(tiles, likely < tiles ? likely : tiles);
   };
   if constexpr (!TRANS && sizeof(T) == 2) {
-    if (on16 && p.r % 8 == 0 && tensor_sized(p.M, p.L, p.r, indexed, true)) {
+    if (on16 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, p.L, p.r, indexed, true)) {
       const auto t = tiles_of(128);
       return p.r <= 64 ? launch_tc<T, 64>(p, t.first, t.second, st) : launch_tc<T, 128>(p, t.first, t.second, st);
     }
@@ -1464,7 +1546,7 @@ cudaError_t run(Params p, bool trans, cudaStream_t st) {
 // Whether a backward call goes to the tensor-core kernel once its adapters are transposed.
 template <typename T>
 bool wants_transposed(const Params& p) {
-  return sizeof(T) == 2 && p.r % 8 == 0 && tensor_sized(p.M, p.L, p.r, p.index != nullptr, true) && aligned<T>(p);
+  return sizeof(T) == 2 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, p.L, p.r, p.index != nullptr, true) && aligned<T>(p);
 }
 
 // One or two gradients (count).
