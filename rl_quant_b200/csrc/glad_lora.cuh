@@ -145,7 +145,7 @@ __device__ __forceinline__ int adapter_of(const Params& p, int m) {
 
 // The rows of this cluster's tile into rows[0 .. n); returns n (0: nothing to do) and the adapter. `scratch` is shared memory for
 // kScanRows short numbers.
-template <int R>
+template <int R, int NT = kThreads>
 __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, int& adapter, void* scratch) {
   const int tid = threadIdx.x;
   int n;
@@ -165,12 +165,12 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
     if (tid < n) rows[tid] = plan.row(from + tid);
   } else if (p.M > kSelfRows) {
     // Count the rows of every adapter, look the tile up among their tiles, and collect the adapter's rows from the tile's first on.
-    __shared__ int cnt[kScanAdapters + 1], sums[kWarps], found[2];
+    __shared__ int cnt[kScanAdapters + 1], sums[NT / 32], found[2];
     uint16_t* of = static_cast<uint16_t*>(scratch);
     const int lane = tid & 31, G = p.L + 1;
-    for (int i = tid; i < G; i += kThreads) cnt[i] = 0;
+    for (int i = tid; i < G; i += NT) cnt[i] = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < p.M; i0 += kThreads) {
+    for (int i0 = 0; i0 < p.M; i0 += NT) {
       const int i = i0 + tid;
       int a = -1;
       if (i < p.M) {
@@ -207,7 +207,7 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
     if (a < 0) return 0;
     adapter = a == p.L ? -1 : a;
     n = min(R, cnt[a] - first);
-    const int run = (p.M + kThreads - 1) / kThreads, lo = tid * run, hi = min(p.M, lo + run);
+    const int run = (p.M + NT - 1) / NT, lo = tid * run, hi = min(p.M, lo + run);
     int mine = 0;
     for (int i = lo; i < hi; ++i) mine += of[i] == a;
     int at = mine;
@@ -228,7 +228,7 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
         }
   } else {
     // One cluster a row: it is the tile's where R, 2 R, ... rows of the same adapter (none) come before it.
-    __shared__ int of[kSelfRows], counts[kWarps];
+    __shared__ int of[kSelfRows], counts[NT / 32];
     if (tid < p.M) of[tid] = adapter_of(p, tid);
     __syncthreads();
     adapter = of[tile];
@@ -239,7 +239,7 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
     if ((tid & 31) == 0) counts[tid >> 5] = __popc(votes);
     __syncthreads();
     int at = __popc(votes & ((1u << (tid & 31)) - 1)), all = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < NT / 32; ++w) {
       if (w < tid >> 5) at += counts[w];
       all += counts[w];
     }
@@ -1058,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
 template <int RT>
 struct Tc {
   // a stage: 128 inputs of 128 rows of x and of A, in two blocks of 64 (128 bytes) each
-  static constexpr int kStages = 3, kBlock = 128 * 128 + RT * 128, kStage = 2 * kBlock, NB = RT / 64;  // NB: blocks of 64 ranks
+  static constexpr int kThreads = 512, kStages = RT == 64 ? 4 : 3, kBlock = 128 * 128 + RT * 128, kStage = 2 * kBlock, NB = RT / 64;  // NB: blocks of 64 ranks
   static constexpr int kPart = 128 * RT * 4, kB = NB * 16384, kBase = 32768;
   // first the ring; then [B, two][base, two][u's operand], and this block's part of u behind it or, where that is too much, over base
   static constexpr int kBaseAt = 2 * kB, kA = 2 * kB + 2 * kBase, kBehind = kA + 2 * NB * 16384;
@@ -1094,6 +1094,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 256;" ::"r"(half + 1) : "memory"); }
 // Waits for the products behind a phase; after one wait that ran out no other one waits, the bit is set and the kernel ends as usual.
 __device__ __forceinline__ void tc_wait(uint64_t* bar, uint32_t parity, const Params& p, bool& dead) {
   if (dead || mbar_try_wait(bar, parity)) return;
@@ -1103,22 +1104,23 @@ __device__ __forceinline__ void tc_wait(uint64_t* bar, uint32_t parity, const Pa
 }
 
 template <typename T, int RT>
-__global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
+__global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Params p) {
   using L = Tc<RT>;
-  constexpr int R = 128, S = L::kStages, NB = L::NB;
+  constexpr int NTH = L::kThreads, R = 128, S = L::kStages, NB = L::NB;
   constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   constexpr uint32_t kFirst = idesc_f16(128, RT) | kType, kSecond = idesc_f16(128, 128) | kType;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int rows[R];
   __shared__ float down[kHalves<T> ? R : 1];          // what the rows of u were divided by
-  __shared__ __align__(8) uint64_t full[S], done[2], drain;
+  __shared__ __align__(8) uint64_t full[S], done[2], drain[2];
   __shared__ uint32_t tmem_at;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int half = warp >> 3, hw = warp & 7, ht = tid & 255;            // two halves of 8 warps take the second product's steps in turn
   const int C = p.cluster, rank = (int)blockIdx.x % C, tile = (int)blockIdx.x / C;
   grid_dep_wait();
   int adapter;
-  const int n = find_rows<R>(p, tile, rows, adapter, smem);
+  const int n = find_rows<R, NTH>(p, tile, rows, adapter, smem);
   if (n == 0) return;                                 // the whole cluster
   const bool any = adapter >= 0;
   if (warp == 0) tmem_alloc(&tmem_at, 512);
@@ -1126,7 +1128,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1 + p.hold);
     mbar_init(&done[0], 1 + p.hold);
     mbar_init(&done[1], 1 + p.hold);
-    mbar_init(&drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -1139,8 +1142,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
   const int tiles = (p.N + 127) / 128, steps = p.y != nullptr && rank < tiles ? (tiles - rank + C - 1) / C : 0;
   auto fetch_b = [&](int j) {
     if (j < steps && any) {
-      const int n0 = (rank + j * C) * 128, row0 = tid >> 3, c = tid & 7;
-      const uint32_t at = base_addr + (j & 1) * L::kB + row0 * 128 + turned(c, row0);
+      const int n0 = (rank + j * C) * 128, row0 = ht >> 3, c = ht & 7;
+      const uint32_t at = base_addr + half * L::kB + row0 * 128 + turned(c, row0);
       const T* src = w2 + (int64_t)(n0 + row0) * p.r + 8 * c;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -1154,8 +1157,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
   };
   auto fetch_base = [&](int j) {
     if (j < steps && p.base != nullptr) {
-      const int n0 = (rank + j * C) * 128, row0 = tid >> 4, c = tid & 15;
-      const uint32_t at = base_addr + L::kBaseAt + (j & 1) * L::kBase + row0 * 256;
+      const int n0 = (rank + j * C) * 128, row0 = ht >> 4, c = ht & 15;
+      const uint32_t at = base_addr + L::kBaseAt + half * L::kBase + row0 * 256;
       const T* base = static_cast<const T*>(p.base);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1169,9 +1172,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
   if (any) {
     const T* w1 = static_cast<const T*>(p.w1) + (int64_t)adapter * p.r * p.K;
     const int row0 = tid >> 3, c = tid & 7;
-    const T* xp[4];
+    const T* xp[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xp[j] = static_cast<const T*>(p.x) + (int64_t)rows[row0 + 32 * j] * p.ldx + c * 8;
+    for (int j = 0; j < 2; ++j) xp[j] = static_cast<const T*>(p.x) + (int64_t)rows[row0 + 64 * j] * p.ldx + c * 8;
     const int chunks = (p.K + 127) / 128, mine = rank < chunks ? (chunks - rank + C - 1) / C : 0;
     auto fetch = [&](int i) {
       if (i < mine) {
@@ -1179,22 +1182,22 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
         for (int b = 0; b < 2; ++b) {
           const int k = (rank + i * C) * 128 + 64 * b;
           const bool live = k + c * 8 < p.K;
-          const uint32_t at = base_addr + i % S * L::kStage + b * L::kBlock + row0 * 128 + turned(c, row0);   // 32 rows on: the same turn
+          const uint32_t at = base_addr + i % S * L::kStage + b * L::kBlock + row0 * 128 + turned(c, row0);   // 64 rows on: the same turn
           if (k + 64 <= p.K && n == R && p.r == RT) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) copy16(at + j * 4096, xp[j] + k);
+            for (int j = 0; j < 2; ++j) copy16(at + j * 8192, xp[j] + k);
 #pragma unroll
-            for (int j = 0; j < RT / 32; ++j) copy16(at + 16384 + j * 4096, w1 + (int64_t)(row0 + 32 * j) * p.K + k + c * 8);
+            for (int j = 0; j < RT / 64; ++j) copy16(at + 16384 + j * 8192, w1 + (int64_t)(row0 + 64 * j) * p.K + k + c * 8);
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool in = live && row0 + 32 * j < n;
-              copy16(at + j * 4096, in ? xp[j] + k : static_cast<const T*>(p.x), in);
+            for (int j = 0; j < 2; ++j) {
+              const bool in = live && row0 + 64 * j < n;
+              copy16(at + j * 8192, in ? xp[j] + k : static_cast<const T*>(p.x), in);
             }
 #pragma unroll
-            for (int j = 0; j < RT / 32; ++j) {
-              const bool in = live && row0 + 32 * j < p.r;
-              copy16(at + 16384 + j * 4096, in ? w1 + (int64_t)(row0 + 32 * j) * p.K + k + c * 8 : w1, in);
+            for (int j = 0; j < RT / 64; ++j) {
+              const bool in = live && row0 + 64 * j < p.r;
+              copy16(at + 16384 + j * 8192, in ? w1 + (int64_t)(row0 + 64 * j) * p.K + k + c * 8 : w1, in);
             }
           }
         }
@@ -1225,13 +1228,12 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
     cp_async_wait_all();
     tc_fence_after();
     __syncthreads();
-    fetch_b(0);                                        // the ring is read no more
-    fetch_b(1);
-    if (L::kApart) fetch_base(0);
-    // this block's part of u: row 32 (warp % 4) + lane, half of the ranks
+    fetch_b(half);                                     // the ring is read no more
+    if (L::kApart) fetch_base(half);
+    // this block's part of u: row 32 (warp % 4) + lane, a quarter of the ranks
     const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
-    for (int col = (warp >> 2) * (RT / 2); col < ((warp >> 2) + 1) * (RT / 2); col += 16) {
+    for (int col = (warp >> 2) * (RT / 4); col < ((warp >> 2) + 1) * (RT / 4); col += 16) {
       uint32_t v[16] = {};
       if (mine > 0) {
         tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + col, v);
@@ -1249,7 +1251,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
     // every block adds up its share of the rows, eight ranks a lane, and sends the operand to all
     const float s = p.scale ? p.scale[adapter] : p.scale_value;
     const int share = (R + C - 1) / C;
-    for (int from = 0; from < share * (RT / 8); from += kThreads) {
+    for (int from = 0; from < share * (RT / 8); from += NTH) {
       const int i = from + tid, row = rank * share + i / (RT / 8), c8 = i % (RT / 8);
       const bool in = i < share * (RT / 8) && row < R;
       float f[8] = {};
@@ -1306,81 +1308,73 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tc_kernel(const Params p) {
   if (C > 1) cluster_sync_all();                       // u is there, and nobody reads another block's part any more
   else __syncthreads();
 
-  // The products of step j, behind those of the step before.
-  auto issue = [&](int j) {
-    if (j < steps && any && warp == 0) {
-      tc_fence_after();
-      const uint32_t d = tmem + 128 + (j & 1) * 128, a = base_addr + L::kA, b = base_addr + (j & 1) * L::kB;
-#pragma unroll
-      for (int half = 1; half >= 0; --half)            // the smaller numbers first
-#pragma unroll
-        for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16_warp(d, desc_sw128(a + (half * NB + blk) * 16384) + 2 * k, desc_sw128(b + blk * 16384) + 2 * k, kSecond,
-                         half == 1 && blk == 0 && k == 0 ? 0u : 1u);
-      mma_commit_warp(&done[j & 1]);
-    }
-  };
-  if (!any) fetch_b(0), fetch_b(1);
-  if (!any || !L::kApart) fetch_base(0);
-  fetch_base(1);
-  cp_async_wait_group<3>();
-  fence_async_smem();
-  __syncthreads();
-  issue(0);
-  for (int j = 0; j < steps; ++j) {
-    cp_async_wait_group<1>();                          // all but base of the next step
+  if (!any) fetch_b(half);
+  if (!any || !L::kApart) fetch_base(half);
+  const uint32_t d = tmem + 128 + half * 128;
+  for (int j = half; j < steps; j += 2) {
+    cp_async_wait_group<1>();                          // B; base may be on its way
     fence_async_smem();
-    __syncthreads();
-    issue(j + 1);
+    half_sync(half);
     if (any) {
-      tc_wait(&done[j & 1], (j >> 1) & 1, p, dead);
+      if (hw == 0) {
+        tc_fence_after();
+        const uint32_t a = base_addr + L::kA, b = base_addr + half * L::kB;
+#pragma unroll
+        for (int part = 1; part >= 0; --part)          // the smaller numbers first
+#pragma unroll
+          for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_f16_warp(d, desc_sw128(a + (part * NB + blk) * 16384) + 2 * k, desc_sw128(b + blk * 16384) + 2 * k, kSecond,
+                           part == 1 && blk == 0 && k == 0 ? 0u : 1u);
+        mma_commit_warp(&done[half]);
+      }
+      tc_wait(&done[half], (j >> 1) & 1, p, dead);
       __syncwarp();
       tc_fence_after();
     }
-    fetch_b(j + 2);                                    // its place is read no more
-    {
-      const int row = (warp & 3) * 32 + lane;
-      const float f = kHalves<T> && any ? down[kHalves<T> ? row : 0] : 1.0f;
-      const uint32_t d = tmem + 128 + (j & 1) * 128 + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * 64;
-      uint8_t* line = smem + L::kBaseAt + (j & 1) * L::kBase + row * 256;
-      uint32_t v[2][32] = {};
-      if (any) {
-        tmem_ld32(d, v[0]);
-        tmem_ld32(d + 32, v[1]);
-        tmem_ld_wait();
-      }
-#pragma unroll
-      for (int h = 0; h < 8; ++h) {
-        uint4* at = reinterpret_cast<uint4*>(line + turned((warp >> 2) * 8 + h, row));
-        const uint4 b = p.base != nullptr ? *at : make_uint4(0, 0, 0, 0);
-        const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = pack2<T>(fmaf(__uint_as_float(v[h / 4][h % 4 * 8 + 2 * e]), f, elem<T>(bw, 2 * e)),
-                          fmaf(__uint_as_float(v[h / 4][h % 4 * 8 + 2 * e + 1]), f, elem<T>(bw, 2 * e + 1)));
-        *at = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-      tc_fence_before();
+    fetch_b(j + 2);
+    cp_async_wait_group<1>();                          // base
+    half_sync(half);
+    const int row = (warp & 3) * 32 + lane;
+    const float f = kHalves<T> && any ? down[kHalves<T> ? row : 0] : 1.0f;
+    uint8_t* line = smem + L::kBaseAt + half * L::kBase + row * 256;
+    uint32_t v[2][32] = {};
+    if (any) {
+      const uint32_t at = d + ((uint32_t)((warp & 3) * 32) << 16) + (hw >> 2) * 64;
+      tmem_ld32(at, v[0]);
+      tmem_ld32(at + 32, v[1]);
+      tmem_ld_wait();
     }
-    __syncthreads();
-    const int n0 = (rank + j * C) * 128, c = tid & 15;
+#pragma unroll
+    for (int h = 0; h < 8; ++h) {
+      uint4* at = reinterpret_cast<uint4*>(line + turned((hw >> 2) * 8 + h, row));
+      const uint4 b = p.base != nullptr ? *at : make_uint4(0, 0, 0, 0);
+      const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[e] = pack2<T>(fmaf(__uint_as_float(v[h / 4][h % 4 * 8 + 2 * e]), f, elem<T>(bw, 2 * e)),
+                        fmaf(__uint_as_float(v[h / 4][h % 4 * 8 + 2 * e + 1]), f, elem<T>(bw, 2 * e + 1)));
+      *at = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    tc_fence_before();
+    half_sync(half);
+    const int n0 = (rank + j * C) * 128, c = ht & 15;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = (tid >> 4) + 16 * i;
+      const int row = (ht >> 4) + 16 * i;
       if (row < n && n0 + 8 * c < p.N)
         *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + (int64_t)rows[row] * p.N + n0 + 8 * c) =
-            *reinterpret_cast<const uint4*>(smem + L::kBaseAt + (j & 1) * L::kBase + row * 256 + turned(c, row));
+            *reinterpret_cast<const uint4*>(smem + L::kBaseAt + half * L::kBase + row * 256 + turned(c, row));
     }
-    __syncthreads();
+    half_sync(half);
     fetch_base(j + 2);
   }
   cp_async_wait_all();
   if (dead) {                                          // products may still be on their way: they take microseconds
-    if (warp == 0) mma_commit_warp(&drain);
-    mbar_wait_bounded(&drain, 0, 10000000);
+    if (hw == 0) mma_commit_warp(&drain[half]);
+    mbar_wait_bounded(&drain[half], 0, 10000000);
   }
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 512);
@@ -1400,7 +1394,7 @@ cudaError_t allow_smem(K* kernel, size_t smem, size_t (&limit)[64]) {
 
 // Clusters of n such blocks that the GPU holds at once. They are placed within groups of SMs, so that fewer blocks fit in
 // larger ones: 16 clusters of 8 take two rounds (512 rows 4096 -> 4096 rank 64 bf16: @R16X8@ us, 16 of 4 @R16X4@).
-template <auto Kernel>
+template <auto Kernel, int NT = kThreads>
 int clusters_at_once(int n, size_t smem) {
   static int cache[64][9] = {};                        // plus one
   int dev = 0;
@@ -1410,7 +1404,7 @@ int clusters_at_once(int n, size_t smem) {
     if (allow_smem(Kernel, smem, limit) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(NT);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1424,14 +1418,14 @@ int clusters_at_once(int n, size_t smem) {
   return cache[dev][n] - 1;
 }
 
-template <auto Kernel, typename P>
+template <auto Kernel, int NT = kThreads, typename P>
 cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st) {
   static size_t limit[64] = {};
   const cudaError_t e = allow_smem(Kernel, smem, limit);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -1497,9 +1491,9 @@ cudaError_t launch_tc(Params p, int64_t tiles, int64_t likely, cudaStream_t st) 
   constexpr size_t smem = Tc<RT>::kSmem;
   auto steps = [&](int c) { return ((p.K + 127) / 128 + c - 1) / c + ((p.N + 127) / 128 + c - 1) / c; };
   p.cluster = 8;
-  while (p.cluster > 1 && likely > clusters_at_once<kernel>(p.cluster, smem)) --p.cluster;
+  while (p.cluster > 1 && likely > clusters_at_once<kernel, Tc<RT>::kThreads>(p.cluster, smem)) --p.cluster;
   while (p.cluster > 1 && steps(p.cluster - 1) == steps(p.cluster)) --p.cluster;
-  return launch_clusters<kernel>(p, dim3((unsigned)(tiles * p.cluster)), smem, st);
+  return launch_clusters<kernel, Tc<RT>::kThreads>(p, dim3((unsigned)(tiles * p.cluster)), smem, st);
 }
 
 template <typename T, bool TRANS>
