@@ -1050,11 +1050,15 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
 }
 
 // ---- many rows an adapter, ranks above 32: both products on the tensor core's own memory -------------
-// At these ranks mma.sync is the bound (8192 rows 4096 -> 4096 bf16: rank 128 159 us with the rings, @T128@ here; rank 64 @R64@ and
-// @T64@), and a tile of 32 rows reads the adapter too often. So: tiles of 128 rows, u summed in tensor memory by tcgen05 while
-// all warps keep four stages of x and A in flight, then u as two 16-bit numbers (as in the rings) times 128 columns of B
-// a step, base and y through shared memory. Operands lie K-major with the 128-byte swizzle; the backward pass
-// gets its adapters transposed first (transpose_kernel), which are small.
+// At these ranks mma.sync is the bound (8192 rows 4096 -> 4096 bf16: rank 64 73 us with the rings, rank 128 157), and a tile of 32 rows
+// reads the adapter too often. So: tiles of 128 rows, u summed in tensor memory by tcgen05 while all warps keep three or four stages of x
+// and A in flight; every block of the cluster adds up its share of u's rows and sends them, as two 16-bit numbers each (as in the
+// rings), to the others; then u times 128 columns of B a step, base and y through shared memory. Two halves of eight warps take these steps
+// in turn, so that one's stores go out while the other computes (one group of eight: rank 64 54 us, rank 128 61; with base and y as
+// bulk copies of 256 bytes a row 67 and 72: issuing them took 3500 cycles a step). Operands lie K-major with the 128-byte
+// swizzle; the backward pass gets its adapters transposed first (transpose_kernel), which are small.
+// 8192 rows rank 64 51 us, rank 128 56, both 201 MB at least: 3.9 and 3.6 TB/s. Bound: the way into and out of an SM, 35 bytes a cycle
+// in either phase; with few tiles latency (256 rows rank 64 17 us: launch 3, rows and setup 2, x and A 4, u 5, columns 3).
 template <int RT>
 struct Tc {
   // a stage: 128 inputs of 128 rows of x and of A, in two blocks of 64 (128 bytes) each
@@ -1393,7 +1397,7 @@ cudaError_t allow_smem(K* kernel, size_t smem, size_t (&limit)[64]) {
 }
 
 // Clusters of n such blocks that the GPU holds at once. They are placed within groups of SMs, so that fewer blocks fit in
-// larger ones: 16 clusters of 8 take two rounds (512 rows 4096 -> 4096 rank 64 bf16: @R16X8@ us, 16 of 4 @R16X4@).
+// larger ones: 16 clusters of 8 take two rounds (rings, 512 rows 4096 -> 4096 rank 64 bf16: 25.9 us, 16 of 4 16.5).
 template <auto Kernel, int NT = kThreads>
 int clusters_at_once(int n, size_t smem) {
   static int cache[64][9] = {};                        // plus one
@@ -1439,10 +1443,12 @@ cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st)
   return cudaLaunchKernelEx(&cfg, Kernel, p);
 }
 
-// Whether the tensor-core kernel takes the call (if every address is on 16 bytes): 16-bit rows, ranks above 32, and half a tile of rows
-// an adapter on average.
+// Whether the tensor-core kernel takes the call (if every address is on 16 bytes): 16-bit rows, ranks above 32, 1024 rows or more and half
+// a tile an adapter on average. Both sides, us, 4096 -> 4096 bf16, this kernel and the rings: rank 64, one adapter, 256 rows 17.5 and
+// 13.5, 1024 17.9 and 16.8, 2048 22.1 and 23.5, 8192 51 and 73; 1024 rows and 8 adapters 20.5 and 26.1, 8192 and 16 88 and 112.
+// Rank 128: 256 rows 22.8 and 17.0, 1024 23.3 and 24.4, 8192 56 and 157; 1024 rows and 8 adapters 28.2 and 29.5.
 inline bool tensor_sized(int64_t M, int L, int r, bool indexed, bool wide16) {
-  return wide16 && r > 32 && M >= 64 * (int64_t)(indexed ? L : 1);
+  return wide16 && r > 32 && M >= 1024 && M >= 64 * (int64_t)(indexed ? L : 1);
 }
 // Rows of a ring kernel's tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
 inline int ring_rows(int64_t M, int L, int r, bool indexed) {

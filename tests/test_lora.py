@@ -116,7 +116,8 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (8192, 32, 24, 16, 512), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3),
          # tiles of 128 rows on the tensor core's memory: one and several, odd counts of chunks and of columns, empty adapters
          (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
-         (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3)]
+         (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1100, 4096, 264, 64, 2),
+         (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3)]
 
 
 @gpu
@@ -281,7 +282,7 @@ def test_waits_that_run_out(dtype):
     from rl_quant_b200 import DeviceStatusError, w4_status
     from rl_quant_b200 import _native as N
     lib = N.load()
-    x, a, b, i, scale, base, dy = make(600, 512, 384, 64, 2, dtype, 12)
+    x, a, b, i, scale, base, dy = make(1100, 512, 384, 64, 2, dtype, 12)
     leaves = [t.clone().requires_grad_() for t in (x, a, b)]
 
     def once():
