@@ -133,26 +133,38 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   }
 }
 
-// dst[l] = src[l]^T for two sets of matrices of 16-bit elements, [rows, cols] each, in one launch: 64 x 64 elements a block.
+// dst[l] = src[l]^T for two sets of matrices of 16-bit elements, [rows, cols] each (multiples of 8, on 16 bytes), in one launch:
+// 64 x 64 elements a block, 16 bytes a lane in and out.
 struct Transposes {
   const uint16_t* src[2];
   uint16_t* dst[2];
   int rows[2], cols[2];
 };
 __global__ void __launch_bounds__(256) transpose_kernel(const Transposes p) {
-  __shared__ uint16_t tile[64][66];
+  __shared__ __align__(16) uint16_t tile[64][72];       // [column][row]
   const int which = blockIdx.z & 1, rows = p.rows[which], cols = p.cols[which];
   const int64_t at = (int64_t)(blockIdx.z >> 1) * rows * cols;
   const int tall = rows > cols;                         // the long side runs along blockIdx.x
   const int r0 = (tall ? blockIdx.x : blockIdx.y) * 64, c0 = (tall ? blockIdx.y : blockIdx.x) * 64;
   if (r0 >= rows || c0 >= cols) return;
   grid_dep_wait();
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4)
-    if (r0 + i < rows && c0 + x < cols) tile[i][x] = p.src[which][at + (int64_t)(r0 + i) * cols + c0 + x];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = (threadIdx.x >> 3) + 32 * j, c = (threadIdx.x & 7) * 8;
+    if (r0 + row < rows && c0 + c < cols) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p.src[which] + at + (int64_t)(r0 + row) * cols + c0 + c);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tile[c + e][row] = (uint16_t)(w[e >> 1] >> 16 * (e & 1));
+    }
+  }
   __syncthreads();
-  for (int i = y; i < 64; i += 4)
-    if (c0 + i < cols && r0 + x < rows) p.dst[which][at + (int64_t)(c0 + i) * rows + r0 + x] = tile[x][i];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int col = (threadIdx.x >> 3) + 32 * j, r = (threadIdx.x & 7) * 8;
+    if (c0 + col < cols && r0 + r < rows)
+      *reinterpret_cast<uint4*>(p.dst[which] + at + (int64_t)(c0 + col) * rows + r0 + r) = *reinterpret_cast<const uint4*>(&tile[col][r]);
+  }
 }
 
 std::atomic<uint32_t> g_hold{0}, g_wait_ns{2000000000u};
