@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(256) transpose_kernel(const Transposes p) {
 std::atomic<uint32_t> g_hold{0}, g_wait_ns{2000000000u};
 
 // What the tensor-core kernel needs beside the operands.
-cudaError_t tensor_setup(Params& p) {
+template <typename P>
+cudaError_t tensor_setup(P& p) {
   p.wait_ns = g_wait_ns, p.hold = g_hold;
   return w4_status_word(&p.status);
 }
@@ -323,6 +324,7 @@ int glad_lora_backward(const void* dy, int dtype, int64_t lddy, const void* x, i
   };
   if (db) add(dy, lddy, u, db, N, 1, r);
   if (da) add(x, ldx, du, da, K, K, 1);
+  if (count && e == cudaSuccess) e = tensor_setup(pair);
   if (count && e == cudaSuccess)
     e = for_type(dtype, [&](auto t) { return run_outer<decltype(t)>(pair, count, st); });
   return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);

@@ -71,6 +71,8 @@ struct OuterParams {    // out[a] = sum over a's rows of v[m]^T x[m]
 struct OuterPair {
   OuterParams of[2];
   int cluster;
+  uint32_t* status;     // of the tensor-core kernel, as above
+  uint32_t wait_ns, hold;
 };
 
 __device__ __forceinline__ float tf32(float v) {
@@ -1100,7 +1102,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 256;" ::"r"(half + 1) : "memory"); }
 // Waits for the products behind a phase; after one wait that ran out no other one waits, the bit is set and the kernel ends as usual.
-__device__ __forceinline__ void tc_wait(uint64_t* bar, uint32_t parity, const Params& p, bool& dead) {
+template <typename P>
+__device__ __forceinline__ void tc_wait(uint64_t* bar, uint32_t parity, const P& p, bool& dead) {
   if (dead || mbar_try_wait(bar, parity)) return;
   if (mbar_wait_bounded(bar, parity, p.wait_ns)) return;
   dead = true;
@@ -1384,6 +1387,189 @@ __global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Para
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
+// The gradients of adapters by tcgen05: out[a] = sum over a's rows of v[m]^T x[m] for 256 columns of x a block, both operands with the
+// rows as k: 128 bytes of a row side by side (swizzled), 8 rows a group. 64 rows a stage: x by asynchronous copies, v (two bf16
+// numbers each) through registers, taken apart on the way. A cluster's blocks take stages in turn and add up in a fixed order.
+// Bound: the steps of a stage one after the other (copies there, products issued, the last ones done: 1700 cycles at rank 64, 2000 at 128,
+// products alone 512). 8192 rows rank 64, both gradients of 4096 columns, 42 us: 3.2 TB/s. (Rows in core matrices of 16 bytes
+// instead of 128 took 2800 cycles a stage: every 16 bytes are a write of their own.)
+template <int RT>
+struct OuterTc {
+  static constexpr int kThreads = 512, BW = 256, kRows = 64, kStages = 4;
+  static constexpr int kBlock = kRows * 128;                           // of 64 columns
+  static constexpr int kX = BW / 64 * kBlock, kHalf = RT / 64 * kBlock, kV = 2 * kHalf;
+  static constexpr int kNeed = kStages * kX + 2 * kV, kSmem = kNeed + 1024;
+  static constexpr int kByRank = RT + 4, kByCol = BW + 4;              // pitch of the sums in floats: [BW][kByRank] or [RT][kByCol]
+  static_assert(BW * kByRank * 4 <= kNeed && RT * kByCol * 4 <= kNeed, "the sums lie over all of it");
+};
+__device__ __forceinline__ uint64_t desc_rows(uint32_t saddr) {         // blocks of 64 columns by 64 rows, groups of 8 rows
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(OuterTc<RT>::kThreads, 1) outer_tc_kernel(const __grid_constant__ OuterPair pair) {
+  using L = OuterTc<RT>;
+  static_assert(kPairs<T>, "v comes as two numbers of the type of x");
+  constexpr int S = L::kStages, BW = L::BW, NTH = L::kThreads, KR = L::kRows;
+  constexpr int VI = RT / 8, VROWS = NTH / VI < KR ? NTH / VI : KR, VP = KR / VROWS;      // pieces of a row of v, rows a pass, passes
+  constexpr uint32_t kDesc = idesc_f16(128, RT) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16);
+  const int second = (int)blockIdx.x >= pair.of[0].blocks;
+  const OuterParams& p = pair.of[second];
+  const int block = (int)blockIdx.x - (second ? pair.of[0].blocks : 0);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full[S], drain;
+  __shared__ uint32_t tmem_at;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int C = p.cluster, rank = block % C, n0 = block / C * BW, a = blockIdx.y;
+  grid_dep_wait();                                     // tensor memory is not held while others may need it
+  if (warp == 0) tmem_alloc(&tmem_at, 2 * RT);
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&full[i], 1 + pair.hold);
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at, base = smem_u32(smem);
+  bool dead = false;
+  const Plan plan{p.plan, p.L, p.M};
+  const int from = p.plan ? plan.first(a) : 0, rows = p.plan ? plan.first(a + 1) - from : p.M;
+  const int chunks = (rows + KR - 1) / KR, mine = rank < chunks ? (chunks - rank + C - 1) / C : 0;
+  auto row_of = [&](int i, int at) {                   // of the block's chunk i; -1: none
+    at += (rank + i * C) * KR;
+    return i < mine && at < rows ? p.plan ? plan.row(from + at) : at : -1;
+  };
+  // x: a warp's lanes hold a row's 256 columns, rows warp + 16 j; their numbers a chunk ahead
+  const bool in = n0 + lane * 8 < p.K;
+  const T* xc = static_cast<const T*>(p.x) + (in ? n0 + lane * 8 : 0);
+  int xr[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) xr[j] = row_of(0, warp + 16 * j);
+  auto fetch = [&](int i) {
+    if (i < mine) {
+      const uint32_t at = base + i % S * L::kX + (lane >> 3) * L::kBlock + warp * 128 + turned(lane & 7, warp);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copy16(at + j * 2048, xc + (int64_t)max(xr[j], 0) * p.ldx, in && xr[j] >= 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xr[j] = row_of(i + 1, warp + 16 * j);
+    }
+    cp_async_commit();
+  };
+  // v: eight ranks of a row a thread, rows v0 + VROWS j
+  const int v8 = tid % VI, v0 = tid / VI;
+  const bool v_in = 8 * v8 < p.r && v0 < VROWS;
+  int vr[VP];
+  uint4 v[VP][2];
+#pragma unroll
+  for (int j = 0; j < VP; ++j) vr[j] = v_in ? row_of(0, v0 + VROWS * j) : -1;
+  auto read = [&](int i) {                             // chunk i, whose row numbers are there
+#pragma unroll
+    for (int j = 0; j < VP; ++j) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.v + (int64_t)max(vr[j], 0) * p.r + 8 * v8);
+      v[j][0] = vr[j] >= 0 ? src[0] : make_uint4(0, 0, 0, 0);
+      v[j][1] = vr[j] >= 0 ? src[1] : make_uint4(0, 0, 0, 0);
+      vr[j] = v_in ? row_of(i + 1, v0 + VROWS * j) : -1;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i);
+  read(0);
+  for (int i = 0; i < mine; ++i) {
+    const int vat = S * L::kX + (i & 1) * L::kV;
+    if (v0 < VROWS) {
+#pragma unroll
+      for (int j = 0; j < VP; ++j) {
+        uint8_t* at = smem + vat + (v8 >> 3) * L::kBlock + (v0 + VROWS * j) * 128 + turned(v8 & 7, v0 + VROWS * j);
+        const uint4 f = v[j][0], g = v[j][1];
+        *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(f.x, f.y, 0x5410), __byte_perm(f.z, f.w, 0x5410),
+                                                   __byte_perm(g.x, g.y, 0x5410), __byte_perm(g.z, g.w, 0x5410));
+        *reinterpret_cast<uint4*>(at + L::kHalf) = make_uint4(__byte_perm(f.x, f.y, 0x7632), __byte_perm(f.z, f.w, 0x7632),
+                                                              __byte_perm(g.x, g.y, 0x7632), __byte_perm(g.z, g.w, 0x7632));
+      }
+    }
+    read(i + 1);
+    cp_async_wait_group<S - 2>();
+    fence_async_smem();
+    __syncthreads();
+    if (warp == 0) {
+      tc_fence_after();
+      const uint32_t xs = base + i % S * L::kX, vs = base + vat;
+#pragma unroll
+      for (int half = 1; half >= 0; --half)            // the smaller numbers first
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int k = 0; k < KR / 16; ++k)
+            mma_f16_warp(tmem + c * RT, desc_rows(xs + c * 2 * L::kBlock + k * 2048), desc_rows(vs + half * L::kHalf + k * 2048), kDesc, i > 0 || half == 0 || k > 0 ? 1u : 0u);
+      mma_commit_warp(&full[i % S]);
+    }
+    if (i > 0) tc_wait(&full[(i - 1) % S], ((i - 1) / S) & 1, pair, dead);       // its stage, and its v, are filled next
+    fetch(i + S - 1);
+  }
+  if (mine > 0) tc_wait(&full[(mine - 1) % S], ((mine - 1) / S) & 1, pair, dead);
+  cp_async_wait_all();
+  tc_fence_after();
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem);
+  const bool by_rank = p.step_r == 1;                  // else columns lie side by side
+  {
+    const int c = (warp >> 2) & 1, col = c * 128 + (warp & 3) * 32 + lane;
+#pragma unroll 1
+    for (int k = (warp >> 3) * (RT / 2); k < ((warp >> 3) + 1) * (RT / 2); k += 16) {
+      uint32_t w[16] = {};
+      if (mine > 0) {
+        tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c * RT + k, w);
+        tmem_ld_wait();
+      }
+      if (by_rank) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(part + col * L::kByRank + k + 4 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[(k + e) * L::kByCol + col] = __uint_as_float(w[e]);
+      }
+    }
+  }
+  tc_fence_before();
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  // eight adjacent numbers of the gradient a thread
+  T* out = static_cast<T*>(p.out) + (int64_t)a * p.r * p.K;
+  for (int i = rank * NTH + tid; i < RT * BW / 8; i += C * NTH) {
+    const int k = by_rank ? i % VI * 8 : i / (BW / 8), col = by_rank ? i / VI : i % (BW / 8) * 8;
+    const uint32_t at = base + 4 * (by_rank ? col * L::kByRank + k : k * L::kByCol + col);
+    float f[8] = {};
+    for (int c0 = 0; c0 < C; c0 += 4) {                // in order, four blocks' parts on their way
+      float4 o[8] = {};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c0 + e < C) {
+          const uint32_t src = mapa_shared(at, c0 + e);
+          o[2 * e] = ld_cluster4(src), o[2 * e + 1] = ld_cluster4(src + 16);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[0] += o[2 * e].x, f[1] += o[2 * e].y, f[2] += o[2 * e].z, f[3] += o[2 * e].w;
+        f[4] += o[2 * e + 1].x, f[5] += o[2 * e + 1].y, f[6] += o[2 * e + 1].z, f[7] += o[2 * e + 1].w;
+      }
+    }
+    if (k < p.r && n0 + col < p.K)
+      *reinterpret_cast<uint4*>(out + k * p.step_r + (int64_t)(n0 + col) * p.step_k) =
+          make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+  }
+  if (C > 1) cluster_sync_all();
+  if (dead) {                                          // products may still be on their way: they take microseconds
+    if (warp == 0) mma_commit_warp(&drain);
+    mbar_wait_bounded(&drain, 0, 10000000);
+  }
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 2 * RT);
+}
+
 // Allows a kernel its dynamic shared memory, once a device (the call costs as much as a launch). `limit`: 0 or what was allowed.
 template <typename K>
 cudaError_t allow_smem(K* kernel, size_t smem, size_t (&limit)[64]) {
@@ -1549,6 +1735,32 @@ bool wants_transposed(const Params& p) {
   return sizeof(T) == 2 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, p.L, p.r, p.index != nullptr, true) && aligned<T>(p);
 }
 
+// Whether the gradients of adapters go to the tensor-core kernel: bf16, whose v is kept as two numbers of the type of x (fp16's is fp32: its
+// sums over rows have no factor in common that would bring v into range), multiples of 8 ranks above 16. Backward passes 4096 ->
+// 4096 with the rings and with this kernel, us: rank 16, 8192 rows 65 and 76, 1024 rows and 16 adapters 42.6 and 42.7; rank 32, 87 and 88,
+// 65 and 48; rank 64, 117 and 88, 127 and 74; rank 128, 197 and 106, 221 and 101; 64 rows rank 32 13.3 and 14.9, rank 64 21.2 and 20.4.
+inline bool outer_sized(int r) { return r > 16; }
+
+template <typename T, int RT>
+cudaError_t launch_outer_tc(OuterPair pair, int count, int64_t rows, cudaStream_t st) {
+  constexpr auto kernel = outer_tc_kernel<T, RT>;
+  constexpr size_t smem = OuterTc<RT>::kSmem;
+  constexpr int BW = OuterTc<RT>::BW;
+  int64_t tiles = 0;
+  for (int i = 0; i < count; ++i) tiles += (int64_t)((pair.of[i].K + BW - 1) / BW) * pair.of[i].L;
+  // blocks of a tile: as many as the GPU holds at once, two stages of rows each or more
+  int C = 1;
+  while (C < 8 && rows >= (int64_t)C * 4 * OuterTc<RT>::kRows && tiles <= clusters_at_once<kernel, OuterTc<RT>::kThreads>(2 * C, smem)) C *= 2;
+  unsigned blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    pair.of[i].cluster = C;
+    pair.of[i].blocks = (pair.of[i].K + BW - 1) / BW * C;
+    blocks += (unsigned)pair.of[i].blocks;
+  }
+  pair.cluster = C;
+  return launch_clusters<kernel, OuterTc<RT>::kThreads>(pair, dim3(blocks, (unsigned)pair.of[0].L), smem, st);
+}
+
 // One or two gradients (count).
 template <typename T>
 cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
@@ -1557,13 +1769,19 @@ cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
   const int RT = first.r <= 16 ? 16 : 32, ranks = (first.r + RT - 1) / RT;
   const int64_t rows = first.plan ? (first.M + first.L - 1) / first.L : first.M;       // of an adapter, on average
   int64_t tiles = 0;
-  bool ring = first.r % 4 == 0;
+  bool ring = first.r % 4 == 0, wide = true;
   for (int i = 0; i < count; ++i) {
     OuterParams& p = pair.of[i];
     tiles += (int64_t)((p.K + BW - 1) / BW) * p.L * ranks;
+    wide = wide && on(p.out, 16);
     p.pitch = (uint32_t)(p.ldx * (int64_t)sizeof(T));
     p.half = sizeof(T) == 2 && (p.K % 2 || !on(p.x, 4) || (p.M > 1 && p.ldx % 2));
     ring = ring && p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && p.ldx < (int64_t)1 << 29 && on(p.v, 16);
+  }
+  if constexpr (kPairs<T>) {
+    if (ring && wide && first.r % 8 == 0 && outer_sized(first.r)) {
+      return first.r <= 64 ? launch_outer_tc<T, 64>(pair, count, rows, st) : launch_outer_tc<T, 128>(pair, count, rows, st);
+    }
   }
   // blocks of a tile: while every warp keeps a few groups of 16 rows and the tiles alone do not fill the GPU
   int C = 1;

@@ -117,7 +117,8 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          # tiles of 128 rows on the tensor core's memory: one and several, odd counts of chunks and of columns, empty adapters
          (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
          (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1100, 4096, 264, 64, 2),
-         (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3)]
+         (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3), (5000, 520, 264, 24, 1),
+         (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3)]
 
 
 @gpu
