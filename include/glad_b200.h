@@ -506,8 +506,8 @@ int glad_debug_lora_wait(uint32_t hold, uint64_t limit_ns);
  *     columns and log probabilities, largest first, the lower column first among equals
  *   stats [rows, 2]: what the backward pass reads                   (NULL: not wanted)
  * Logits of -inf have probability 0 and add nothing to the entropy; a row of nothing else has log probability
- * -inf, entropy 0 and no gradient. A row whose token is ignore_index is not read: its
- * outputs are 0 (top_index -1), its gradient 0. Any other token outside [0, cols) gives NaN,
+ * -inf, entropy 0 and no gradient. A row whose token is ignore_index counts for
+ * nothing, whatever it holds: its outputs are 0 (top_index -1), its gradient 0. Any other token outside [0, cols) gives NaN,
  * as does a NaN or +inf in the row. All f32 but top_index (i64).               */
 int glad_token_log_probs(const void* logits, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, const void* tokens,
                          int token_bytes, int64_t ignore_index, float temperature, int top, float* log_prob,

