@@ -30,7 +30,7 @@ struct PlanParams {
 
 // A stable counting sort by one block: the first `warps` warps count the adapters of a run of rows each, the counts are added up by
 // adapter, then by warp, and the warps place their rows. Rows of an adapter stay in order, so sums over them repeat. Latency: three
-// passes over the index by one block (300 rows, 5 adapters: 6 us).
+// passes over the index by one block (300 rows, 5 adapters: 9.6 us with cold caches).
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   extern __shared__ int32_t sh[];
   const int G = p.L + 1;                                // groups: adapters, then the rows without one

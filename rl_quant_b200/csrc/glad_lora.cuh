@@ -913,7 +913,7 @@ struct OuterRing {
 // out[a] = sum over a's rows of v[m]^T x[m], two gradients in one launch: the first blocks are of the first. RT: ranks of a block, 16 or
 // 32 (blockIdx.z: which). A cluster shares 128 bytes of columns of an adapter's gradient; its warps split the rows, and
 // the parts are added in a fixed order. Bound: at one block of ranks the bytes of x and dy, which every other one reads again (8192 rows
-// 4096 -> 4096 rank 16 bf16, both gradients, 30 us, 134 MB: 4.5 TB/s); with few rows an adapter the blocks' latency.
+// 4096 -> 4096 rank 16 bf16, both gradients, 32 us with cold caches, 134 MB: 4.2 TB/s); with few rows an adapter the blocks' latency.
 template <typename T, int RT, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constant__ OuterPair pair) {
   using L = OuterRing<T, RT>;
@@ -1067,7 +1067,7 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
 // bulk copies of 256 bytes a row 67 and 72: issuing them took 3500 cycles a step). Operands lie K-major with the 128-byte
 // swizzle; the backward pass gets its adapters transposed first (transpose_kernel), which are small.
 // 8192 rows rank 64 51 us, rank 128 56, both 201 MB at least: 3.9 and 3.6 TB/s. Bound: the way into and out of an SM, 35 bytes a cycle
-// in either phase; with few tiles latency (256 rows rank 64 17 us: launch 3, rows and setup 2, x and A 4, u 5, columns 3).
+// in either phase; with few tiles latency (256 rows rank 64 17 us: launch, rows and setup 5, the rest x and A, u and columns alike).
 template <int RT>
 struct Tc {
   // a stage: 128 inputs of 128 rows of x and of A, in two blocks of 64 (128 bytes) each
