@@ -118,7 +118,9 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
          (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1100, 4096, 264, 64, 2),
          (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3), (5000, 520, 264, 24, 1),
-         (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3)]
+         (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3),
+         # as many rows and ranks, off the 16 bytes: the other kernel on the same tiles
+         (1200, 72, 64, 100, 2), (1100, 73, 65, 64, 2), (1030, 70, 68, 40, 3)]
 
 
 @gpu
@@ -192,8 +194,9 @@ def test_index(m, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-def test_some_gradients_only(dtype):
-    x, a, b, i, scale, base, dy = make(70, 64, 96, 16, 3, dtype, 6)
+@pytest.mark.parametrize("size", [(70, 64, 96, 16, 3), (1100, 64, 96, 64, 3), (1100, 520, 72, 128, 1)])
+def test_some_gradients_only(size, dtype):
+    x, a, b, i, scale, base, dy = make(*size, dtype, 6, index=None if size[4] == 1 else "mixed")
     want = ref(x, a, b, i, scale, base, dy)[1:]
     for use in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1)):
         leaves = [t.clone().requires_grad_(bool(u)) for t, u in zip((x, a, b), use)]
@@ -209,7 +212,7 @@ def test_some_gradients_only(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_keep_to_themselves(dtype, r):
     """A NaN or an infinity in a row of x or of base stays in that row; in an adapter, in its rows."""
-    x, a, b, i, scale, base, dy = make(90, 96, 80, 16, 4, dtype, 7) if r == 16 else make(290, 96, 80, r, 4, dtype, 7)
+    x, a, b, i, scale, base, dy = make(90, 96, 80, 16, 4, dtype, 7) if r == 16 else make(1290, 96, 80, r, 4, dtype, 7)
     want = lora_linear(x, a, b, i, scale, base)
     i[5], i[9] = 1, -1
     want = lora_linear(x, a, b, i, scale, base)
@@ -235,7 +238,7 @@ def test_rows_keep_to_themselves(dtype, r):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_repeats_streams_and_graphs(dtype):
-    for m, r in ((30, 16), (700, 16), (700, 64)):
+    for m, r in ((30, 16), (700, 16), (700, 64), (1100, 64)):
         x, a, b, i, scale, base, dy = make(m, 256, 192, r, 5, dtype, 8)
         leaves = [t.clone().requires_grad_() for t in (x, a, b)]
 
@@ -267,7 +270,7 @@ def test_repeats_streams_and_graphs(dtype):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_ranges_of_the_split(dtype):
     """Rows of u of very different magnitudes, and of one large number beside small ones: rows keep their relative accuracy."""
-    for m, r in ((40, 16), (300, 64), (300, 128)):
+    for m, r in ((40, 16), (300, 64), (300, 128), (1100, 64), (1030, 128)):
         x, a, b, i, scale, base, dy = make(m, 256, 128, r, 1, dtype, 11, sign=True, base=False, index=None)
         x = x * torch.logspace(-3, 2, m).to(dtype).cuda()[:, None]
         a = a.clone()
