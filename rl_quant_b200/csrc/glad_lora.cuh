@@ -1090,6 +1090,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st_cluster4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -1242,8 +1244,6 @@ __global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Para
     cp_async_wait_all();
     tc_fence_after();
     __syncthreads();
-    fetch_b(half);                                     // the ring is read no more
-    if (L::kApart) fetch_base(half);
     // this block's part of u: row 32 (warp % 4) + lane, a quarter of the ranks
     const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
@@ -1259,7 +1259,11 @@ __global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Para
     }
     tc_fence_before();
   }
-  if (C > 1) cluster_sync_all();
+  // the first operands of the second product are on their way while the others' parts are waited for
+  if (C > 1) cluster_arrive();
+  if (any) fetch_b(half);
+  if (any && L::kApart) fetch_base(half);
+  if (C > 1) cluster_wait();
   else __syncthreads();
   if (any) {
     // every block adds up its share of the rows, eight ranks a lane, and sends the operand to all
