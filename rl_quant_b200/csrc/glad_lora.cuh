@@ -1275,19 +1275,17 @@ __global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Para
       float f[8] = {};
       if (in) {
         const uint32_t line = base_addr + L::kPartAt + row * RT * 4;
-        for (int c = 0; c < C; c += 4) {               // in order, four blocks' parts on their way
-          float4 o[8] = {};
+        float4 o[16] = {};                             // all blocks' parts on their way
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < C) {
-              const uint32_t at = mapa_shared(line, c + e);
-              o[2 * e] = ld_cluster4(at + turned(2 * c8, row)), o[2 * e + 1] = ld_cluster4(at + turned(2 * c8 + 1, row));
-            }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[0] += o[2 * e].x, f[1] += o[2 * e].y, f[2] += o[2 * e].z, f[3] += o[2 * e].w;
-            f[4] += o[2 * e + 1].x, f[5] += o[2 * e + 1].y, f[6] += o[2 * e + 1].z, f[7] += o[2 * e + 1].w;
+        for (int c = 0; c < 8; ++c)
+          if (c < C) {
+            const uint32_t at = mapa_shared(line, c);
+            o[2 * c] = ld_cluster4(at + turned(2 * c8, row)), o[2 * c + 1] = ld_cluster4(at + turned(2 * c8 + 1, row));
           }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          f[0] += o[2 * c].x, f[1] += o[2 * c].y, f[2] += o[2 * c].z, f[3] += o[2 * c].w;
+          f[4] += o[2 * c + 1].x, f[5] += o[2 * c + 1].y, f[6] += o[2 * c + 1].z, f[7] += o[2 * c + 1].w;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= s;
