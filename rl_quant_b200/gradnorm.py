@@ -135,8 +135,8 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
     """``(clipped, norm)``: every tensor of ``grads`` times min(1, max_norm / (norm + 1e-6)), in its own type, in new tensors
-    or in those of ``out`` (shapes, types and strides of the gradients; their memory is shared with no other tensor of the call, but out[i]
-    may be grads[i])."""
+    or in those of ``out`` (shapes, types and strides of the gradients, which then leave no gaps in memory; their memory is shared with
+    no other tensor of the call, but out[i] may be grads[i])."""
     kind, max_norm, grads = _kind(norm_type), _max_norm(max_norm), _tensors(grads, "grads")
     given = None if out is None else _tensors(out, "out")
     if given is not None and len(given) != len(grads):

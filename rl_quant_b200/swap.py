@@ -99,7 +99,7 @@ def select_lora(swapped: dict[str, LoRALinear], index) -> None:
 
 
 def restore_lora(model: nn.Module, swapped: dict[str, LoRALinear]) -> None:
-    """Put the layers below the adapters back, with the swapped modules' train/eval flag."""
+    """Put the layers below the adapters back, with the swapped modules' train/eval flag (and frozen, where they were)."""
     for path, mod in swapped.items():
         set_module(model, path, mod.base.train(mod.training))
 

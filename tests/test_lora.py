@@ -267,6 +267,38 @@ def test_repeats_streams_and_graphs(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,r", [(300, 16), (1100, 64), (9000, 32)])
+def test_captured_training(m, r, dtype):
+    """Forward and backward pass in one graph, replayed twice on other rows, adapters and gradients; two graphs of one pool in turn."""
+    x, a, b, i, scale, base, dy = make(m, 136, 72, r, 3, dtype, 13)
+    x2, a2, b2, i2, _, base2, dy2 = make(m, 136, 72, r, 3, dtype, 14)
+
+    def once(x, a, b, i, base, dy):
+        leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+        y = lora_linear(*leaves, i, scale, base)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    held = [t.clone() for t in (x, a, b, i, base, dy)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once(*held)
+    torch.cuda.current_stream().wait_stream(s)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once(*held)
+    with torch.cuda.graph(other, pool=graph.pool()):
+        got2 = once(*held)
+    for given in ((x2, a2, b2, i2, base2, dy2), (x, a, b, i, base, dy)):
+        for h, t in zip(held, given):
+            h.copy_(t)
+        want = once(*given)
+        for g, outs in ((graph, got), (graph, got), (other, got2)):
+            g.replay()
+            assert all(torch.equal(u, v) for u, v in zip(outs, want))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_ranges_of_the_split(dtype):
     """Rows of u of very different magnitudes, and of one large number beside small ones: rows keep their relative accuracy."""
@@ -342,13 +374,18 @@ def test_empty_and_large_offsets():
     m = 70000
     big = torch.zeros(m, 32768, dtype=torch.bfloat16, device="cuda")
     big[m - 1] = 1.0
-    a, b = torch.full((1, 16, 32768), 2.0 ** -15, dtype=torch.bfloat16, device="cuda"), torch.ones(1, 64, 16, dtype=torch.bfloat16,
-                                                                                                   device="cuda")
-    y = lora_linear(big, a, b)
-    assert (y[m - 1] == 16.0).all() and not y[:m - 1].any()
-    leaf = a.clone().requires_grad_()
-    da, = torch.autograd.grad(lora_linear(big, leaf, b), leaf, torch.ones(m, 64, dtype=torch.bfloat16, device="cuda"))
-    assert (da == 64.0).all()
+    one = lambda *s: torch.ones(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    for r in (16, 64):
+        a, b = one(1, r, 32768) * 2.0 ** -15, one(1, 64, r)
+        y = lora_linear(big, a, b)
+        assert (y[m - 1] == r).all() and not y[:m - 1].any()
+        leaf = a.clone().requires_grad_()
+        da, = torch.autograd.grad(lora_linear(big, leaf, b), leaf, one(m, 64))
+        assert (da == 64.0).all()
+    # outputs whose offsets do
+    for r in (16, 64):
+        y = lora_linear(big[:, :64], one(1, r, 64) / 64, one(1, 32768, r), base=big)
+        assert (y[m - 1] == r + 1).all() and not y[:m - 1].any()
 
 
 def net(dtype, device):
