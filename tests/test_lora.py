@@ -299,6 +299,31 @@ def test_captured_training(m, r, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("m,r", [(300, 16), (1100, 64), (2000, 128)])
+def test_two_at_once(m, r):
+    """Calls on two streams whose kernels share the GPU."""
+    sets = [make(m, 520, 264, r, 3, torch.bfloat16, 15 + j) for j in range(2)]
+
+    def once(x, a, b, i, scale, base, dy):
+        leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+        y = lora_linear(*leaves, i, scale, base)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    want = [once(*q) for q in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(once(*sets[j]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for g in got[j]:
+            assert all(torch.equal(u, v) for u, v in zip(g, want[j]))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_ranges_of_the_split(dtype):
     """Rows of u of very different magnitudes, and of one large number beside small ones: rows keep their relative accuracy."""
