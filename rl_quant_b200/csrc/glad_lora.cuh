@@ -1066,7 +1066,7 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const __grid_constan
 // in turn, so that one's stores go out while the other computes (one group of eight: rank 64 54 us, rank 128 61; with base and y as
 // bulk copies of 256 bytes a row 67 and 72: issuing them took 3500 cycles a step). Operands lie K-major with the 128-byte
 // swizzle; the backward pass gets its adapters transposed first (transpose_kernel), which are small.
-// 8192 rows rank 64 51 us, rank 128 56, both 201 MB at least: 3.9 and 3.6 TB/s. Bound: the way into and out of an SM, 35 bytes a cycle
+// 8192 rows rank 64 50 us, rank 128 56, both 201 MB at least: 4.0 and 3.6 TB/s. Bound: the way into and out of an SM, 35 bytes a cycle
 // in either phase; with few tiles latency (256 rows rank 64 17 us: launch, rows and setup 5, the rest x and A, u and columns alike).
 template <int RT>
 struct Tc {
