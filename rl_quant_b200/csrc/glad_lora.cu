@@ -198,12 +198,13 @@ const char* shape_wrong(int dtype, int64_t M, int64_t K, int64_t N, int L, int r
 
 int64_t plan_words(int64_t M, int L) { return 3 + L + M + 2 * max_tiles(M, L, 16, true, true); }
 
-cudaError_t make_plan(const void* index, int index_bytes, int64_t M, int L, int r, bool wide16, void* plan, cudaStream_t st) {
+cudaError_t make_plan(const void* index, int index_bytes, int64_t M, int64_t sides, int L, int r, bool wide16, void* plan,
+                      cudaStream_t st) {
   static size_t limit[64] = {};
   // counting warps: 256 rows each if possible, which they hold in registers; as many as shared memory has counters for
   int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
   if (M < 256 * warps) warps = (int)((M + 255) / 256);
-  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, L, r, true, wide16)};
+  const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, sides, L, r, true, wide16)};
   const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
   const cudaError_t e = allow_smem(plan_kernel, smem, limit);
   if (e != cudaSuccess) return e;
@@ -247,14 +248,14 @@ int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t 
   p.index = index, p.index64 = index_bytes == 8, p.plan = static_cast<const int32_t*>(plan);
   p.scale = scale, p.scale_value = scale_value, p.base = base, p.ldb = base ? ldb : 0, p.y = y, p.u = u;
   cudaError_t e = tensor_setup(p);
-  if (plan && e == cudaSuccess) e = make_plan(index, index_bytes, M, L, r, dtype != GLAD_DTYPE_F32, plan, (cudaStream_t)stream);
+  if (plan && e == cudaSuccess) e = make_plan(index, index_bytes, M, K + N, L, r, dtype != GLAD_DTYPE_F32, plan, (cudaStream_t)stream);
   if (e == cudaSuccess) e = for_type(dtype, [&](auto t) { return run<decltype(t)>(p, false, (cudaStream_t)stream); });
   return e == cudaSuccess ? GLAD_OK : cuda_bad(who, e);
 }
 
 size_t glad_lora_backward_workspace_size(int64_t M, int64_t K, int64_t N, int L, int r, int dtype, int indexed) {
   if (M < 1 || K < 1 || N < 1 || L < 1 || L > kMaxAdapters || r < 1 || r > kMaxRank) return 0;
-  if (r % 8 || !tensor_sized(M, L, r, indexed != 0, dtype != GLAD_DTYPE_F32)) return 0;
+  if (r % 8 || !tensor_sized(M, K + N, L, r, indexed != 0, dtype != GLAD_DTYPE_F32)) return 0;
   return (size_t)L * (size_t)r * (size_t)(K + N) * 2;
 }
 

@@ -1640,20 +1640,22 @@ cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st)
   return cudaLaunchKernelEx(&cfg, Kernel, p);
 }
 
-// Whether the tensor-core kernel takes the call (if every address is on 16 bytes): 16-bit rows, ranks above 32, 1024 rows or more and half
-// a tile an adapter on average. Both sides, us, 4096 -> 4096 bf16, this kernel and the rings: rank 64, one adapter, 256 rows 17.5 and
-// 13.5, 1024 17.9 and 16.8, 2048 22.1 and 23.5, 8192 51 and 73; 1024 rows and 8 adapters 20.5 and 26.1, 8192 and 16 88 and 112.
-// Rank 128: 256 rows 22.8 and 17.0, 1024 23.3 and 24.4, 8192 56 and 157; 1024 rows and 8 adapters 28.2 and 29.5.
-inline bool tensor_sized(int64_t M, int L, int r, bool indexed, bool wide16) {
-  return wide16 && r > 32 && M >= 1024 && M >= 64 * (int64_t)(indexed ? L : 1);
+// Whether the tensor-core kernel takes the call (if every address is on 16 bytes; sides: inputs and outputs together): 16-bit rows, ranks
+// above 32, half a tile an adapter on average, 1024 rows or more and, above rank 64, 4096 or 2^23 elements of x and y.
+// Both sides, us, bf16, this kernel and the rings. Rank 64, 4096 -> 4096, one adapter: 256 rows 17.5 and 13.5, 1024 17.9 and 16.8, 2048 22
+// and 24, 8192 50 and 73; 8 adapters, 1024 rows 20.5 and 26.1; 16, 8192 rows 88 and 112; 512 -> 512, 1024 rows 10.1 and 12.0. Rank
+// 128, 4096 -> 4096: 256 rows 22.8 and 17.0, 1024 23.3 and 24.4, 8192 56 and 157; 1024 -> 1024, 1024 rows 16.2 and 11.5, 2048 16.0 and
+// 13.7, 4096 16.9 and 26.4; 512 -> 512, 2048 rows 13.0 and 9.3, 4096 14.0 and 17.6.
+inline bool tensor_sized(int64_t M, int64_t sides, int L, int r, bool indexed, bool wide16) {
+  return wide16 && r > 32 && M >= 1024 && M >= 64 * (int64_t)(indexed ? L : 1) && (r <= 64 || M >= 4096 || M * sides >= 1 << 23);
 }
 // Rows of a ring kernel's tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
 inline int ring_rows(int64_t M, int L, int r, bool indexed) {
   return r <= 64 && M > 16 * (int64_t)(indexed ? L : 1) ? 32 : 16;
 }
 // Rows of a tile of the plan: the larger of what the kernels of both directions may take.
-inline int tile_rows(int64_t M, int L, int r, bool indexed, bool wide16) {
-  return tensor_sized(M, L, r, indexed, wide16) ? 128 : ring_rows(M, L, r, indexed);
+inline int tile_rows(int64_t M, int64_t sides, int L, int r, bool indexed, bool wide16) {
+  return tensor_sized(M, sides, L, r, indexed, wide16) ? 128 : ring_rows(M, L, r, indexed);
 }
 // Clusters for tiles of R rows.
 inline int64_t max_tiles(int64_t M, int L, int R, bool indexed, bool planned) {
@@ -1702,7 +1704,7 @@ cudaError_t launch_tc(Params p, int64_t tiles, int64_t likely, cudaStream_t st) 
 template <typename T, bool TRANS>
 cudaError_t run_as(Params p, cudaStream_t st) {
   const bool indexed = p.index != nullptr, planned = p.plan != nullptr;
-  const int whole = tile_rows(p.M, p.L, p.r, indexed, sizeof(T) == 2);
+  const int whole = tile_rows(p.M, (int64_t)p.K + p.N, p.L, p.r, indexed, sizeof(T) == 2);
   const bool on16 = aligned<T>(p);
   auto tiles_of = [&](int R) {             // and how many of them are likely to have rows
     p.split = planned ? whole / R : 1;
@@ -1712,7 +1714,7 @@ cudaError_t run_as(Params p, cudaStream_t st) {
     return std::pair<int64_t, int64_t>(tiles, likely < tiles ? likely : tiles);
   };
   if constexpr (!TRANS && sizeof(T) == 2) {
-    if (on16 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, p.L, p.r, indexed, true)) {
+    if (on16 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, (int64_t)p.K + p.N, p.L, p.r, indexed, true)) {
       const auto t = tiles_of(128);
       return p.r <= 64 ? launch_tc<T, 64>(p, t.first, t.second, st) : launch_tc<T, 128>(p, t.first, t.second, st);
     }
@@ -1743,7 +1745,8 @@ cudaError_t run(Params p, bool trans, cudaStream_t st) {
 // Whether a backward call goes to the tensor-core kernel once its adapters are transposed.
 template <typename T>
 bool wants_transposed(const Params& p) {
-  return sizeof(T) == 2 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, p.L, p.r, p.index != nullptr, true) && aligned<T>(p);
+  return sizeof(T) == 2 && p.r % 8 == 0 && on(p.u, 16) && tensor_sized(p.M, (int64_t)p.K + p.N, p.L, p.r, p.index != nullptr, true) &&
+         aligned<T>(p);
 }
 
 // Whether the gradients of adapters go to the tensor-core kernel: bf16, whose v is kept as two numbers of the type of x (fp16's is fp32: its

@@ -84,7 +84,14 @@ def close(got, want, dtype):
     value, bound = want
     assert got.dtype == dtype and got.shape == value.shape
     tol = bound + half_step(dtype) * (value.abs() + bound) + tiny(dtype)
-    worst = ((got.double() - value).abs() - tol).max() if got.numel() else torch.tensor(0.0)
+    # From half a step above the type's largest number on (fp16: 65520) rounding to nearest gives infinity: expected there, and allowed
+    # where the bound reaches that far.
+    edge = float(torch.finfo(dtype).max) * (1 + torch.finfo(dtype).eps / 4)
+    infinite = got.double() == torch.sign(value) * math.inf
+    assert infinite[value.abs() - bound > edge].all()
+    value = torch.where(infinite & (value.abs() + bound >= edge), got.double(), value)
+    off = torch.where(got.double() == value, 0.0, (got.double() - value).abs() - tol)
+    worst = off.max() if got.numel() else torch.tensor(0.0)
     assert float(worst) <= 0.0, float(worst)
 
 
@@ -120,7 +127,8 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3), (5000, 520, 264, 24, 1),
          (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3),
          # as many rows and ranks, off the 16 bytes: the other kernel on the same tiles
-         (1200, 72, 64, 100, 2), (1100, 73, 65, 64, 2), (1030, 70, 68, 40, 3)]
+         (1200, 72, 64, 100, 2), (1100, 73, 65, 64, 2), (1030, 70, 68, 40, 3),
+         (4100, 136, 72, 128, 5), (4100, 70, 72, 100, 2), (1100, 4096, 4096, 72, 3)]
 
 
 @gpu
@@ -194,7 +202,7 @@ def test_index(m, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("size", [(70, 64, 96, 16, 3), (1100, 64, 96, 64, 3), (1100, 520, 72, 128, 1)])
+@pytest.mark.parametrize("size", [(70, 64, 96, 16, 3), (1100, 64, 96, 64, 3), (4100, 520, 72, 128, 1)])
 def test_some_gradients_only(size, dtype):
     x, a, b, i, scale, base, dy = make(*size, dtype, 6, index=None if size[4] == 1 else "mixed")
     want = ref(x, a, b, i, scale, base, dy)[1:]
@@ -299,7 +307,7 @@ def test_captured_training(m, r, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("m,r", [(300, 16), (1100, 64), (2000, 128)])
+@pytest.mark.parametrize("m,r", [(300, 16), (1100, 64), (4100, 128)])
 def test_two_at_once(m, r):
     """Calls on two streams whose kernels share the GPU."""
     sets = [make(m, 520, 264, r, 3, torch.bfloat16, 15 + j) for j in range(2)]
@@ -327,7 +335,7 @@ def test_two_at_once(m, r):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_ranges_of_the_split(dtype):
     """Rows of u of very different magnitudes, and of one large number beside small ones: rows keep their relative accuracy."""
-    for m, r in ((40, 16), (300, 64), (300, 128), (1100, 64), (1030, 128)):
+    for m, r in ((40, 16), (300, 64), (300, 128), (1100, 64), (4130, 128)):
         x, a, b, i, scale, base, dy = make(m, 256, 128, r, 1, dtype, 11, sign=True, base=False, index=None)
         x = x * torch.logspace(-3, 2, m).to(dtype).cuda()[:, None]
         a = a.clone()
