@@ -261,8 +261,8 @@ __device__ __forceinline__ int find_rows(const Params& p, int tile, int* rows, i
 }
 
 // fp32 numbers as an operand beside rows of T, whose products should run at the rate of T: two bf16 numbers (16 bits) for bf16;
-// two fp16 numbers (22 bits) for fp16 where a power of two can bring them into its range: u, by row (kHalves). Else two
-// tf32 numbers (22 bits), at half the rate: fp32, and fp16's sums over rows, which have no factor in common.
+// two fp16 numbers (22 bits) for fp16 where a power of two can bring them into its range: u, by row, and
+// outer_tc_kernel's v, by rank (kHalves). Else two tf32 numbers (22 bits), at half the rate: fp32, and fp16's v in outer_kernel.
 template <typename T>
 constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
 template <typename T>
@@ -1398,8 +1398,9 @@ __global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Para
 }
 
 // The gradients of adapters by tcgen05: out[a] = sum over a's rows of v[m]^T x[m] for 256 columns of x a block, both operands with the
-// rows as k: 128 bytes of a row side by side (swizzled), 8 rows a group. 64 rows a stage: x by asynchronous copies, v (two bf16
-// numbers each) through registers, taken apart on the way. A cluster's blocks take stages in turn and add up in a fixed order.
+// rows as k: 128 bytes of a row side by side (swizzled), 8 rows a group. 64 rows a stage: x by asynchronous copies, v through registers,
+// taken apart on the way: bf16's two numbers as they are kept; fp16's split in two by a power of two for each rank, from the largest v of
+// the block's rows (read once before: the backward pass of 8192 rows rank 128 takes 141 us, bf16's 106), which leaves an error of 2^-22 of a number or 2^-39 of the largest. A cluster's blocks take stages in turn and add up in a fixed order.
 // Bound: the steps of a stage one after the other (copies there, products issued, the last ones done: 1700 cycles at rank 64, 2000 at 128,
 // products alone 512). 8192 rows rank 64, both gradients of 4096 columns, 42 us: 3.2 TB/s. (Rows in core matrices of 16 bytes
 // instead of 128 took 2800 cycles a stage: every 16 bytes are a write of their own.)
@@ -1420,17 +1421,17 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t saddr) {         // block
 template <typename T, int RT>
 __global__ void __launch_bounds__(OuterTc<RT>::kThreads, 1) outer_tc_kernel(const __grid_constant__ OuterPair pair) {
   using L = OuterTc<RT>;
-  static_assert(kPairs<T>, "v comes as two numbers of the type of x");
   constexpr int S = L::kStages, BW = L::BW, NTH = L::kThreads, KR = L::kRows;
   constexpr int VI = RT / 8, VROWS = NTH / VI < KR ? NTH / VI : KR, VP = KR / VROWS;      // pieces of a row of v, rows a pass, passes
-  constexpr uint32_t kDesc = idesc_f16(128, RT) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16);
+  constexpr uint32_t kDesc = idesc_f16(128, RT) | (kPairs<T> ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16);
   const int second = (int)blockIdx.x >= pair.of[0].blocks;
   const OuterParams& p = pair.of[second];
   const int block = (int)blockIdx.x - (second ? pair.of[0].blocks : 0);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[S], drain;
-  __shared__ uint32_t tmem_at;
+  __shared__ uint32_t tmem_at, most[kHalves<T> ? RT : 1];
+  __shared__ float down[kHalves<T> ? RT : 1];          // what the ranks of v were divided by
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int C = p.cluster, rank = block % C, n0 = block / C * BW, a = blockIdx.y;
   grid_dep_wait();                                     // tensor memory is not held while others may need it
@@ -1486,6 +1487,33 @@ __global__ void __launch_bounds__(OuterTc<RT>::kThreads, 1) outer_tc_kernel(cons
   };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) fetch(i);
+  float up[8];
+  if constexpr (kHalves<T>) {                          // a rank's power of two, from the block's rows
+    for (int k = tid; k < RT; k += NTH) most[k] = 0;
+    __syncthreads();
+    uint32_t top[8] = {};
+#pragma unroll 2
+    for (int i = 0; i < mine; ++i)
+#pragma unroll
+      for (int j = 0; j < VP; ++j) {
+        const int row = v_in ? row_of(i, v0 + VROWS * j) : -1;
+        const uint4* src = reinterpret_cast<const uint4*>(p.v + (int64_t)max(row, 0) * p.r + 8 * v8);
+        const uint4 f = row >= 0 ? src[0] : make_uint4(0, 0, 0, 0), g = row >= 0 ? src[1] : make_uint4(0, 0, 0, 0);
+        const uint32_t w[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top[e] = max(top[e], w[e] & 0x7fffffffu);
+      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (top[e]) atomicMax(&most[8 * v8 + e], top[e]);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float back;
+      row_power(most[8 * v8 + e], up[e], back);
+      if (v0 == 0) down[8 * v8 + e] = back;
+    }
+  }
   read(0);
   for (int i = 0; i < mine; ++i) {
     const int vat = S * L::kX + (i & 1) * L::kV;
@@ -1494,10 +1522,20 @@ __global__ void __launch_bounds__(OuterTc<RT>::kThreads, 1) outer_tc_kernel(cons
       for (int j = 0; j < VP; ++j) {
         uint8_t* at = smem + vat + (v8 >> 3) * L::kBlock + (v0 + VROWS * j) * 128 + turned(v8 & 7, v0 + VROWS * j);
         const uint4 f = v[j][0], g = v[j][1];
-        *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(f.x, f.y, 0x5410), __byte_perm(f.z, f.w, 0x5410),
-                                                   __byte_perm(g.x, g.y, 0x5410), __byte_perm(g.z, g.w, 0x5410));
-        *reinterpret_cast<uint4*>(at + L::kHalf) = make_uint4(__byte_perm(f.x, f.y, 0x7632), __byte_perm(f.z, f.w, 0x7632),
-                                                              __byte_perm(g.x, g.y, 0x7632), __byte_perm(g.z, g.w, 0x7632));
+        uint4 hi, lo;
+        if constexpr (kHalves<T>) {
+          auto two = [&](uint32_t a, uint32_t b, int e, uint32_t& h, uint32_t& l) {
+            split_f16(__uint_as_float(a) * up[e], __uint_as_float(b) * up[e + 1], h, l);
+          };
+          two(f.x, f.y, 0, hi.x, lo.x), two(f.z, f.w, 2, hi.y, lo.y), two(g.x, g.y, 4, hi.z, lo.z), two(g.z, g.w, 6, hi.w, lo.w);
+        } else {
+          hi = make_uint4(__byte_perm(f.x, f.y, 0x5410), __byte_perm(f.z, f.w, 0x5410), __byte_perm(g.x, g.y, 0x5410),
+                          __byte_perm(g.z, g.w, 0x5410));
+          lo = make_uint4(__byte_perm(f.x, f.y, 0x7632), __byte_perm(f.z, f.w, 0x7632), __byte_perm(g.x, g.y, 0x7632),
+                          __byte_perm(g.z, g.w, 0x7632));
+        }
+        *reinterpret_cast<uint4*>(at) = hi;
+        *reinterpret_cast<uint4*>(at + L::kHalf) = lo;
       }
     }
     read(i + 1);
@@ -1534,6 +1572,9 @@ __global__ void __launch_bounds__(OuterTc<RT>::kThreads, 1) outer_tc_kernel(cons
         tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c * RT + k, w);
         tmem_ld_wait();
       }
+      if constexpr (kHalves<T>)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * down[k + e]);
       if (by_rank) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -1749,10 +1790,10 @@ bool wants_transposed(const Params& p) {
          aligned<T>(p);
 }
 
-// Whether the gradients of adapters go to the tensor-core kernel: bf16, whose v is kept as two numbers of the type of x (fp16's is fp32: its
-// sums over rows have no factor in common that would bring v into range), multiples of 8 ranks above 16. Backward passes 4096 ->
-// 4096 with the rings and with this kernel, us: rank 16, 8192 rows 65 and 76, 1024 rows and 16 adapters 42.6 and 42.7; rank 32, 87 and 88,
-// 65 and 48; rank 64, 117 and 88, 127 and 74; rank 128, 197 and 106, 221 and 101; 64 rows rank 32 13.3 and 14.9, rank 64 21.2 and 20.4.
+// Whether the gradients of adapters go to the tensor-core kernel: 16-bit rows, multiples of 8 ranks above 16. Backward passes 4096 -> 4096
+// with the rings and with this kernel, us, bf16: rank 16, 8192 rows 65 and 76, 1024 rows and 16 adapters 42.6 and 42.7; rank 32, 87
+// and 88, 65 and 48; rank 64, 117 and 88, 127 and 74; rank 128, 197 and 106, 221 and 101; 64 rows rank 32 13.3 and 14.9, rank 64 21.2 and
+// 20.4. fp16: rank 32, 8192 rows 110 and 107, 1024 rows and 16 adapters 65 and 55; rank 128 289 and 141, 224 and 110.
 inline bool outer_sized(int r) { return r > 16; }
 
 template <typename T, int RT>
@@ -1792,7 +1833,7 @@ cudaError_t run_outer(OuterPair pair, int count, cudaStream_t st) {
     p.half = sizeof(T) == 2 && (p.K % 2 || !on(p.x, 4) || (p.M > 1 && p.ldx % 2));
     ring = ring && p.K % EL == 0 && on(p.x, 16) && (p.M <= 1 || p.ldx % EL == 0) && p.ldx < (int64_t)1 << 29 && on(p.v, 16);
   }
-  if constexpr (kPairs<T>) {
+  if constexpr (sizeof(T) == 2) {
     if (ring && wide && first.r % 8 == 0 && outer_sized(first.r)) {
       return first.r <= 64 ? launch_outer_tc<T, 64>(pair, count, rows, st) : launch_outer_tc<T, 128>(pair, count, rows, st);
     }

@@ -4,6 +4,8 @@ Tolerances, fixed before the first run. One matrix instruction adds up to 17 ter
 2^-24 of it: 2^-20 of the running sum of magnitudes. A warp runs at most K / 64 + 2 of them for u, the tensor-core kernel (16-bit rows, ranks above 32) at most K / 16 (the 16-bit
 products are exact; split fp32 ones are off by 2^-20), and the joins of warps and blocks add at most 16 roundings: so u is off by
 (K / 64 + 20) 2^-20 sum |x| |A|, or K / 16 for K / 64.
+(The gradients of fp16 rows above rank 16 split u and du by a power of two a rank: 2^-22 of each, or 2^-39 of the rank's largest, which
+the instructions' 2^-20 of the sum of magnitudes covers where no row's share is 2^-19 of what its neighbours' largest would give it.)
 In y each term of u counts with its own error, splitting u is off by 2^-21 (two tf32 numbers) or 2^-17 (two bf16 ones beside
 bf16 rows), and at most 3 r / 8 + 2 instructions follow; the rounding to the type is half a step. The gradients are the same sums with other operands; rows of an adapter take the place of K.
 Inputs of one sign make the sums of magnitudes the sums themselves."""
