@@ -1750,7 +1750,8 @@ cudaError_t run_as(Params p, cudaStream_t st) {
   auto tiles_of = [&](int R) {             // and how many of them are likely to have rows
     p.split = planned ? whole / R : 1;
     const int64_t tiles = planned ? max_tiles(p.M, p.L, whole, indexed, true) * p.split : max_tiles(p.M, p.L, R, indexed, false);
-    int64_t likely = (p.M + R - 1) / R + (indexed ? p.L - 1 : 0);
+    // an adapter of more rows than a tile leaves half of its last one empty on average; where most have fewer, each is a tile
+    int64_t likely = (p.M + R - 1) / R + (!indexed ? 0 : p.M >= (int64_t)R * p.L ? p.L / 2 : p.L - 1);
     if (likely > p.M) likely = p.M;
     return std::pair<int64_t, int64_t>(tiles, likely < tiles ? likely : tiles);
   };
