@@ -130,7 +130,7 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3),
          # as many rows and ranks, off the 16 bytes: the other kernel on the same tiles
          (1200, 72, 64, 100, 2), (1100, 73, 65, 64, 2), (1030, 70, 68, 40, 3),
-         (4100, 136, 72, 128, 5), (4100, 70, 72, 100, 2), (1100, 4096, 4096, 72, 3)]
+         (4100, 136, 72, 128, 5), (128, 96, 72, 16, 4), (256, 72, 64, 64, 3), (200, 73, 64, 16, 2), (4100, 70, 72, 100, 2), (1100, 4096, 4096, 72, 3)]
 
 
 @gpu
