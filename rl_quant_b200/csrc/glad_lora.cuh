@@ -1696,13 +1696,18 @@ cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st)
 inline bool tensor_sized(int64_t M, int64_t sides, int L, int r, bool indexed, bool wide16) {
   return wide16 && r > 32 && M >= 1024 && M >= 64 * (int64_t)(indexed ? L : 1) && (r <= 64 || M >= 4096 || M * sides >= 1 << 23);
 }
-// Rows of a ring kernel's tile: 16 where an adapter has no more on average, or where 32 need too much shared memory.
-inline int ring_rows(int64_t M, int L, int r, bool indexed) {
-  return r <= 64 && M > 16 * (int64_t)(indexed ? L : 1) ? 32 : 16;
+// Rows of a ring kernel's tile: 32 need half of the reads of the adapters, 16 half of the shared memory and leave a block half of the
+// work: 16 where an adapter has no more on average, above rank 64, and while the GPU holds two or more blocks of each tile at once
+// (four at 32 bits or up to rank 16). 32 rows and 16, us, 4096 -> 4096 bf16: rank 16, one adapter, 64 rows 6.8 and 5.1, 512 8.8 and 6.7, 1000
+// 9.2 and 8.3, rank 8 1500 12.8 and 14.1; rank 64, 128 rows 13.5 and 9.2, 512 16.5 and 11.2, 1000 of 4 adapters 26.2 and 18.6; f32, rank
+// 64, 200 rows of 2 25.2 and 17.8, 1000 40.8 and 46.9.
+inline int ring_rows(int64_t M, int L, int r, bool indexed, bool wide16) {
+  const bool few = M / 16 + (indexed ? L / 2 : 0) <= (r <= 16 || wide16 ? 72 : 36);
+  return r <= 64 && M > 16 * (int64_t)(indexed ? L : 1) && !few ? 32 : 16;
 }
 // Rows of a tile of the plan: the larger of what the kernels of both directions may take.
 inline int tile_rows(int64_t M, int64_t sides, int L, int r, bool indexed, bool wide16) {
-  return tensor_sized(M, sides, L, r, indexed, wide16) ? 128 : ring_rows(M, L, r, indexed);
+  return tensor_sized(M, sides, L, r, indexed, wide16) ? 128 : ring_rows(M, L, r, indexed, wide16);
 }
 // Clusters for tiles of R rows.
 inline int64_t max_tiles(int64_t M, int L, int R, bool indexed, bool planned) {
@@ -1756,8 +1761,10 @@ cudaError_t run_as(Params p, cudaStream_t st) {
   auto tiles_of = [&](int R) {             // and how many of them are likely to have rows
     p.split = planned ? whole / R : 1;
     const int64_t tiles = planned ? max_tiles(p.M, p.L, whole, indexed, true) * p.split : max_tiles(p.M, p.L, R, indexed, false);
-    // an adapter of more rows than a tile leaves half of its last one empty on average; where most have fewer, each is a tile
-    int64_t likely = (p.M + R - 1) / R + (!indexed ? 0 : p.M >= (int64_t)R * p.L ? p.L / 2 : p.L - 1);
+    // an adapter of many tiles leaves half of its last one empty on average, one of one or two more than that; where most have fewer rows
+    // than a tile, each is one
+    const int64_t all = (int64_t)R * p.L;
+    int64_t likely = (p.M + R - 1) / R + (!indexed ? 0 : p.M >= 2 * all ? p.L / 2 : p.M >= all ? 3 * p.L / 4 : p.L - 1);
     if (likely > p.M) likely = p.M;
     return std::pair<int64_t, int64_t>(tiles, likely < tiles ? likely : tiles);
   };
@@ -1767,7 +1774,7 @@ cudaError_t run_as(Params p, cudaStream_t st) {
       return p.r <= 64 ? launch_tc<T, 64>(p, t.first, t.second, st) : launch_tc<T, 128>(p, t.first, t.second, st);
     }
   }
-  const int R = on16 ? ring_rows(p.M, p.L, p.r, indexed) : 16;
+  const int R = on16 ? ring_rows(p.M, p.L, p.r, indexed, sizeof(T) == 2) : 16;
   const auto t = tiles_of(R);
   if (on16) {
 #define GLAD_LORA(RT)                                                                        \
