@@ -473,7 +473,7 @@ int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
  * backward pass reads (bf16 rows: two bf16 numbers, u's sum). r 1..128, L up to 16384, M, K and N up to 2^24. u and the sums are f32, y is rounded once.
  * Infinite inputs give infinite or NaN outputs in their rows.
  * plan: glad_lora_plan_size(M, L) bytes (16-byte aligned) that the call fills with the order of the rows by adapter;
- * needed with an index where a backward pass follows, for more than 8192 rows, and for more than 256 with more than 512
+ * needed with an index where a backward pass follows, for more than 4096 rows, and for more than 256 with more than 512
  * adapters; else it may be NULL.  */
 size_t glad_lora_plan_size(int64_t M, int L);
 int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const void* a, const void* b, int64_t N,

@@ -239,7 +239,7 @@ int glad_lora_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t 
       !on(plan, 16))
     return bad(who, "a tensor is not element-aligned");
   if (index && !plan && M > kSelfRows && (M > kScanRows || L > kScanAdapters))
-    return bad(who, "so many rows (more than 256, with more than 512 adapters; more than 8192) with an index need a plan");
+    return bad(who, "so many rows (more than 256, with more than 512 adapters; more than 4096) with an index need a plan");
   if (!index) plan = nullptr;
   if (plan && plan_bytes < glad_lora_plan_size(M, L))
     return set_last_error(GLAD_ERR_WORKSPACE, "glad_lora_forward: a plan of glad_lora_plan_size bytes is required");

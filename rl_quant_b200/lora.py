@@ -23,7 +23,7 @@ MAX_SIZE = 1 << 24           # rows, inputs, outputs
 
 def _needs_plan(M, L):
     """Whether a forward pass alone needs the order of the rows by adapter laid down first."""
-    return M > 8192 or (M > 256 and L > 512)
+    return M > 4096 or (M > 256 and L > 512)
 
 
 def _rows(t):

@@ -122,7 +122,7 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (64, 512, 1024, 16, 64), (33, 96, 64, 32, 2), (40, 1002, 777, 9, 5), (256, 264, 136, 24, 3), (257, 64, 72, 64, 3),
          (300, 200, 320, 48, 1), (300, 72, 64, 100, 2), (130, 128, 128, 128, 2), (1000, 48, 40, 16, 130), (2050, 520, 264, 16, 2),
          (600, 1024, 1024, 33, 1),
-         (8192, 32, 24, 16, 512), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3),
+         (8192, 32, 24, 16, 512), (4096, 32, 24, 16, 512), (4097, 40, 24, 8, 3), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3),
          # tiles of 128 rows on the tensor core's memory: one and several, odd counts of chunks and of columns, empty adapters
          (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
          (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1100, 4096, 264, 64, 2),
