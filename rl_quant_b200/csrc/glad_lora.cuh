@@ -1689,22 +1689,25 @@ cudaError_t launch_clusters(const P& p, dim3 grid, size_t smem, cudaStream_t st)
   return cudaLaunchKernelEx(&cfg, Kernel, p);
 }
 
+// Whether tiles of 16 rows are so few that the GPU holds `blocks` blocks or more of each at once (on 148 SMs).
+inline bool few_tiles(int64_t M, int L, bool indexed, int blocks) { return M / 16 + (indexed ? L / 2 : 0) <= 144 / blocks; }
 // Whether the tensor-core kernel takes the call (if every address is on 16 bytes; sides: inputs and outputs together): 16-bit rows, ranks
-// above 32, half a tile an adapter on average, 1024 rows or more and, above rank 64, 4096 or 2^23 elements of x and y.
-// Both sides, us, bf16, this kernel and the rings. Rank 64, 4096 -> 4096, one adapter: 256 rows 17.5 and 13.5, 1024 17.9 and 16.8, 2048 22
-// and 24, 8192 50 and 73; 8 adapters, 1024 rows 20.5 and 26.1; 16, 8192 rows 88 and 112; 512 -> 512, 1024 rows 10.1 and 12.0. Rank
-// 128, 4096 -> 4096: 256 rows 22.8 and 17.0, 1024 23.3 and 24.4, 8192 56 and 157; 1024 -> 1024, 1024 rows 16.2 and 11.5, 2048 16.0 and
+// above 32, half a tile an adapter on average, and more tiles than the rings hold in 16 rows or, above rank 64, 4096 rows or 1024 and
+// 2^23 elements of x and y. Both sides, us, bf16, this kernel and the rings. Rank 64, 4096 -> 4096, one adapter: 256 rows 17.5 and
+// 11.0, 1024 17.9 and 15.6, 2048 22 and 24, 8192 50 and 73; 8 adapters, 1024 rows 20.5 and 18.9, 16, 8192 rows 66 and 112. Rank 128,
+// 4096 -> 4096: 256 rows 22.8 and 17.0, 1024 23.3 and 24.4, 8192 56 and 157; 1024 -> 1024, 1024 rows 16.2 and 11.5, 2048 16.0 and
 // 13.7, 4096 16.9 and 26.4; 512 -> 512, 2048 rows 13.0 and 9.3, 4096 14.0 and 17.6.
 inline bool tensor_sized(int64_t M, int64_t sides, int L, int r, bool indexed, bool wide16) {
-  return wide16 && r > 32 && M >= 1024 && M >= 64 * (int64_t)(indexed ? L : 1) && (r <= 64 || M >= 4096 || M * sides >= 1 << 23);
+  if (!wide16 || r <= 32 || M < 64 * (int64_t)(indexed ? L : 1)) return false;
+  return r <= 64 ? !few_tiles(M, L, indexed, 2) : M >= 4096 || (M >= 1024 && M * sides >= 1 << 23);
 }
 // Rows of a ring kernel's tile: 32 need half of the reads of the adapters, 16 half of the shared memory and leave a block half of the
-// work: 16 where an adapter has no more on average, above rank 64, and while the GPU holds two or more blocks of each tile at once
-// (four at 32 bits or up to rank 16). 32 rows and 16, us, 4096 -> 4096 bf16: rank 16, one adapter, 64 rows 6.8 and 5.1, 512 8.8 and 6.7, 1000
+// work: 16 where an adapter has no more on average, above rank 64, and while the GPU holds several blocks of each tile at once
+// (two, four at 32 bits above rank 16; up to rank 16 an SM holds two blocks). 32 rows and 16, us, 4096 -> 4096 bf16: rank 16, one adapter, 64 rows 6.8 and 5.1, 512 8.8 and 6.7, 1000
 // 9.2 and 8.3, rank 8 1500 12.8 and 14.1; rank 64, 128 rows 13.5 and 9.2, 512 16.5 and 11.2, 1000 of 4 adapters 26.2 and 18.6; f32, rank
 // 64, 200 rows of 2 25.2 and 17.8, 1000 40.8 and 46.9.
 inline int ring_rows(int64_t M, int L, int r, bool indexed, bool wide16) {
-  const bool few = M / 16 + (indexed ? L / 2 : 0) <= (r <= 16 || wide16 ? 72 : 36);
+  const bool few = few_tiles(M, L, indexed, r <= 16 || wide16 ? 2 : 4);
   return r <= 64 && M > 16 * (int64_t)(indexed ? L : 1) && !few ? 32 : 16;
 }
 // Rows of a tile of the plan: the larger of what the kernels of both directions may take.

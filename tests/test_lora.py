@@ -125,11 +125,11 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (8192, 32, 24, 16, 512), (4096, 32, 24, 16, 512), (4097, 40, 24, 8, 3), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3),
          # tiles of 128 rows on the tensor core's memory: one and several, odd counts of chunks and of columns, empty adapters
          (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
-         (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1100, 4096, 264, 64, 2),
+         (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1300, 4096, 264, 64, 2), (1300, 64, 64, 64, 1), (1297, 72, 136, 40, 1),
          (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3), (5000, 520, 264, 24, 1),
          (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3),
          # as many rows and ranks, off the 16 bytes: the other kernel on the same tiles
-         (1200, 72, 64, 100, 2), (1100, 73, 65, 64, 2), (1030, 70, 68, 40, 3),
+         (1200, 72, 64, 100, 2), (1300, 73, 65, 64, 2), (1330, 70, 68, 40, 3),
          (4100, 136, 72, 128, 5), (128, 96, 72, 16, 4), (256, 72, 64, 64, 3), (200, 73, 64, 16, 2), (4100, 70, 72, 100, 2), (1100, 4096, 4096, 72, 3)]
 
 
@@ -204,7 +204,7 @@ def test_index(m, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("size", [(70, 64, 96, 16, 3), (1100, 64, 96, 64, 3), (4100, 520, 72, 128, 1)])
+@pytest.mark.parametrize("size", [(70, 64, 96, 16, 3), (1300, 64, 96, 64, 3), (4100, 520, 72, 128, 1)])
 def test_some_gradients_only(size, dtype):
     x, a, b, i, scale, base, dy = make(*size, dtype, 6, index=None if size[4] == 1 else "mixed")
     want = ref(x, a, b, i, scale, base, dy)[1:]
@@ -248,7 +248,7 @@ def test_rows_keep_to_themselves(dtype, r):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_repeats_streams_and_graphs(dtype):
-    for m, r in ((30, 16), (700, 16), (700, 64), (1100, 64)):
+    for m, r in ((30, 16), (700, 16), (700, 64), (1300, 64)):
         x, a, b, i, scale, base, dy = make(m, 256, 192, r, 5, dtype, 8)
         leaves = [t.clone().requires_grad_() for t in (x, a, b)]
 
@@ -278,7 +278,7 @@ def test_repeats_streams_and_graphs(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,r", [(300, 16), (1100, 64), (9000, 32)])
+@pytest.mark.parametrize("m,r", [(300, 16), (1300, 64), (9000, 32)])
 def test_captured_training(m, r, dtype):
     """Forward and backward pass in one graph, replayed twice on other rows, adapters and gradients; two graphs of one pool in turn."""
     x, a, b, i, scale, base, dy = make(m, 136, 72, r, 3, dtype, 13)
@@ -309,7 +309,7 @@ def test_captured_training(m, r, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("m,r", [(300, 16), (1100, 64), (4100, 128)])
+@pytest.mark.parametrize("m,r", [(300, 16), (1300, 64), (4100, 128)])
 def test_two_at_once(m, r):
     """Calls on two streams whose kernels share the GPU."""
     sets = [make(m, 520, 264, r, 3, torch.bfloat16, 15 + j) for j in range(2)]
@@ -337,7 +337,7 @@ def test_two_at_once(m, r):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_ranges_of_the_split(dtype):
     """Rows of u of very different magnitudes, and of one large number beside small ones: rows keep their relative accuracy."""
-    for m, r in ((40, 16), (300, 64), (300, 128), (1100, 64), (4130, 128)):
+    for m, r in ((40, 16), (300, 64), (300, 128), (1300, 64), (4130, 128)):
         x, a, b, i, scale, base, dy = make(m, 256, 128, r, 1, dtype, 11, sign=True, base=False, index=None)
         x = x * torch.logspace(-3, 2, m).to(dtype).cuda()[:, None]
         a = a.clone()
@@ -353,7 +353,7 @@ def test_waits_that_run_out(dtype):
     from rl_quant_b200 import DeviceStatusError, w4_status
     from rl_quant_b200 import _native as N
     lib = N.load()
-    x, a, b, i, scale, base, dy = make(1100, 512, 384, 64, 2, dtype, 12)
+    x, a, b, i, scale, base, dy = make(1300, 512, 384, 64, 2, dtype, 12)
     leaves = [t.clone().requires_grad_() for t in (x, a, b)]
 
     def once():
