@@ -772,6 +772,7 @@ __global__ void __launch_bounds__(256) logp_grad_warp_kernel(const LogpGradParam
   bool none;
   const RowGrad rg = row_grad(p, mine < p.rows ? mine : p.rows - 1, tok, none);
   none |= mine >= p.rows;
+  const uint32_t empty = __ballot_sync(0xffffffffu, none);
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     if (row0 + r >= p.rows) break;
@@ -781,7 +782,12 @@ __global__ void __launch_bounds__(256) logp_grad_warp_kernel(const LogpGradParam
                      __shfl_sync(0xffffffffu, rg.a, from), __shfl_sync(0xffffffffu, rg.b, from)};
     float f[E];
     h[r].floats(f);
-    of.over(f);
+    if (empty >> from & 1) {                            // 0 whatever the row holds: an infinity would make NaN of it
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = 0.0f;
+    } else {
+      of.over(f);
+    }
     if constexpr (VEC) {
 #pragma unroll
       for (int j = 0; j < E / EL; ++j) {

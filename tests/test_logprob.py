@@ -196,6 +196,34 @@ def test_bad_rows(cols, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [40, 100, 300, 1000, 1500])
+def test_ignored_rows_have_no_gradient(cols, dtype):
+    """Whatever an ignored row holds: its gradient is 0, and its neighbours' is what it is beside clean rows."""
+    x, tok = make(20, cols, dtype, 13)
+    fills = {1: [math.inf] * cols, 3: [-math.inf] * cols, 4: [math.nan] * cols, 6: [math.inf, math.nan] * (cols // 2), 9: [math.inf, -math.inf] * (cols // 2),
+             10: [torch.finfo(dtype).max] * cols, 12: [torch.finfo(dtype).min] * cols, 19: None}
+    bad = x.clone()
+    for row, fill in fills.items():
+        tok[row] = -100
+        if fill is None:
+            bad[row, cols - 1] = math.inf          # one logit that overflowed
+        else:
+            bad[row] = torch.tensor(fill)
+    rng = torch.Generator().manual_seed(14)
+    g, gh, gt = (torch.randn(*s, generator=rng).cuda() for s in ((20,), (20,), (20, 3)))
+    for use in ((1, 0, 0), (0, 1, 0), (1, 1, 1)):
+        grads = []
+        for v in (bad, x):
+            leaf = v.clone().requires_grad_()
+            out = token_log_probs(leaf, tok, entropy=True, top=3)
+            outs = [o for o, u in zip((out.log_prob, out.entropy, out.top_log_prob), use) if u]
+            grads += torch.autograd.grad(outs, leaf, [t for t, u in zip((g, gh, gt), use) if u])
+        assert not grads[0][list(fills)].any()     # neither a number nor NaN
+        assert torch.equal(*grads) and grads[0].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 1), (5, 31), (64, 256), (3, 1025), (700, 1000), (40, 4097), (2, 128001), (300, 8200)])
 def test_backward(shape, dtype):
     x, tok = make(*shape, dtype, 6)
