@@ -30,7 +30,7 @@ struct LogpGradParams {
   const void* tokens;
   int64_t ldx, rows, ignore;
   int cols, top, tok64, chunks;
-  float inv_t;
+  float inv_t, low;
   const float* entropy;
   const float2* stats;
   const int64_t* top_index;
@@ -709,11 +709,12 @@ __global__ void __launch_bounds__(kRowThreads) logp_row_kernel(const LogpParams 
 
 // ---- gradient ----------------------------------------------------------------------------------
 // A row's gradient without the given columns' own terms: with d = x - m, p = 2^(k d + c) and ln p + H = d / T + H - ln S it is
-// p (a d + b), a = -gh / T^2, b = -(gh (H - ln S) + G) / T.
+// p (a d + b), a = -gh / T^2, b = -(gh (H - ln S) + G) / T. d ends at `low`, where p is 2^-200 of the largest and less, which is
+// 0 here: beyond it a d would reach infinity for masked logits at small T, and 0 times that is NaN.
 struct RowGrad {
-  float m, k, c, a, b;
+  float m, k, c, a, b, low;
   __device__ __forceinline__ float at(float x) const {
-    const float d = below(x, m);
+    const float d = fmaxf(x - m, low);
     return exp2_fast(fmaf(d, k, c)) * fmaf(d, a, b);
   }
   // of N logits, in place
@@ -724,7 +725,7 @@ struct RowGrad {
     for (int e = 0; e < N; e += 2) {
       float x, y;
       apart(two(f[e], f[e + 1]) + minus, x, y);
-      const Two d = two(fmaxf(x, -1e30f), fmaxf(y, -1e30f));
+      const Two d = two(fmaxf(x, low), fmaxf(y, low));
       apart(fma2(d, kk, cc), x, y);
       apart(two(exp2_fast(x), exp2_fast(y)) * fma2(d, aa, bb), f[e], f[e + 1]);
     }
@@ -741,8 +742,9 @@ __device__ __forceinline__ RowGrad row_grad(const LogpGradParams& p, int64_t row
   if (!given_in(tok, p.cols) && p.g) G = NAN;
   if (p.gt)
     for (int i = 0; i < p.top; ++i) G += p.gt[row * p.top + i];
-  if (none) return RowGrad{0.0f, 1.0f, -INFINITY, 0.0f, 0.0f};
-  return RowGrad{st.x, p.inv_t * kLog2e, -st.y * kLog2e, -gh * p.inv_t, p.gh ? fmaf(-gh, H - st.y, -G * p.inv_t) : -G * p.inv_t};
+  if (none) return RowGrad{0.0f, 1.0f, -INFINITY, 0.0f, 0.0f, p.low};
+  return RowGrad{st.x, p.inv_t * kLog2e, -st.y * kLog2e, -gh * p.inv_t, p.gh ? fmaf(-gh, H - st.y, -G * p.inv_t) : -G * p.inv_t,
+                 p.low};
 }
 // Column number i of the row's given ones (the top alternatives where they have gradients, then the token) again, with its own terms.
 template <typename T>
@@ -779,7 +781,7 @@ __global__ void __launch_bounds__(256) logp_grad_warp_kernel(const LogpGradParam
     T* dx = static_cast<T*>(p.dx) + (row0 + r) * p.cols;
     const int from = r * LR;
     const RowGrad of{__shfl_sync(0xffffffffu, rg.m, from), p.inv_t * kLog2e, __shfl_sync(0xffffffffu, rg.c, from),
-                     __shfl_sync(0xffffffffu, rg.a, from), __shfl_sync(0xffffffffu, rg.b, from)};
+                     __shfl_sync(0xffffffffu, rg.a, from), __shfl_sync(0xffffffffu, rg.b, from), p.low};
     float f[E];
     h[r].floats(f);
     if (empty >> from & 1) {                            // 0 whatever the row holds: an infinity would make NaN of it
@@ -989,7 +991,7 @@ int glad_token_log_probs_backward(const void* logits, int x_dtype, int64_t ldx, 
     return bad(who, "a tensor is not element-aligned");
   LogpGradParams p{};
   p.x = logits, p.ldx = ldx, p.rows = rows, p.cols = (int)cols, p.tokens = tokens, p.tok64 = token_bytes == 8;
-  p.ignore = ignore_index, p.inv_t = 1.0f / temperature, p.top = top;
+  p.ignore = ignore_index, p.inv_t = 1.0f / temperature, p.top = top, p.low = -200.0f / (p.inv_t * kLog2e);
   p.stats = reinterpret_cast<const float2*>(stats), p.entropy = entropy, p.top_index = top_index;
   p.g = d_log_prob, p.gh = d_entropy, p.gt = d_top, p.dx = d_logits;
   return for_type(x_dtype, [&](auto t) {

@@ -224,6 +224,37 @@ def test_ignored_rows_have_no_gradient(cols, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [40, 200, 1000, 1500])
+@pytest.mark.parametrize("T", [1e-6, 1e-3, 1e-2, 1e3])
+def test_masked_columns_have_no_gradient(T, cols, dtype):
+    """Masked by -inf or by the type's lowest value, at any temperature and any size of the entropy's gradient (a loss scale): 0 there,
+    the formula's elsewhere. Logits are of the temperature's size, so that the distribution is not one column's. Results beyond the type
+    are infinite as rounding makes them."""
+    x, tok = make(12, cols, dtype, 15, 2.0)
+    x = (x.float() * T).to(dtype)
+    rng = torch.Generator().manual_seed(16)
+    mask = (torch.rand(12, cols, generator=rng) < 0.3).cuda()
+    mask[torch.arange(12), tok] = False
+    x[mask] = -math.inf
+    x[6:][mask[6:]] = torch.finfo(dtype).min
+    g = torch.randn(12, generator=rng).cuda()
+    r = Ref(x, T)
+    edge = float(torch.finfo(dtype).max) * (1 + torch.finfo(dtype).eps / 4)
+    for size in (1e-3, 1.0, 400.0, 65536.0):
+        gh = torch.full((12,), size, device="cuda")
+        for use in ((0, 1), (1, 1)):
+            leaf = x.clone().requires_grad_()
+            out = token_log_probs(leaf, tok, temperature=T, entropy=True)
+            outs = [o for o, u in zip((out.log_prob, out.entropy), use) if u]
+            d, = torch.autograd.grad(outs, leaf, [t for t, u in zip((g, gh), use) if u])
+            assert not d[mask].any() and not d.isnan().any()
+            want, err = r.grad(tok, g if use[0] else None, gh)
+            near = (d.double() - want).abs() <= err + half_step(dtype) * (want.abs() + err) + tiny(dtype)
+            assert (near | ((d.double() == torch.sign(want) * math.inf) & (want.abs() + err >= edge))).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 1), (5, 31), (64, 256), (3, 1025), (700, 1000), (40, 4097), (2, 128001), (300, 8200)])
 def test_backward(shape, dtype):
     x, tok = make(*shape, dtype, 6)
