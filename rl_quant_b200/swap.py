@@ -78,11 +78,15 @@ def restore_norm(model: nn.Module, originals: dict[str, nn.RMSNorm]) -> None:
 def apply_lora(model: nn.Module, paths: list[str], rank: int = 16, adapters: int = 1, alpha: float | None = None,
                freeze: bool = True) -> dict[str, LoRALinear]:
     """Put ``adapters`` low-rank adapters over each of the named linear layers (nn.Linear, QuantLinear, W4Linear); returns the
-    new layers by path. All or none."""
+    new layers by path. All or none. Layers that their parent computes by itself from their weight (in nn.MultiheadAttention and
+    nn.TransformerEncoderLayer) are refused."""
     swapped: dict[str, LoRALinear] = {}
     for path in paths:
         lin = get_module(model, path)
         assert isinstance(lin, (nn.Linear, QuantLinear, W4Linear)), f"{path} is not a linear layer: {type(lin)}"
+        parent = get_module(model, path.rpartition(".")[0])
+        if isinstance(parent, (nn.MultiheadAttention, nn.TransformerEncoderLayer)):
+            raise ValueError(f"{path}: {type(parent).__name__} reads the layer's weight itself, adapters over it would not be applied")
         swapped[path] = LoRALinear(lin, rank, adapters, alpha, freeze=False)
     for path, mod in swapped.items():
         if freeze:

@@ -540,6 +540,22 @@ def test_module_surgery():
     assert m[0] is lin and not lin.training
 
 
+def test_layers_that_their_parent_computes_itself():
+    """nn.MultiheadAttention and nn.TransformerEncoderLayer read weights of layers below instead of calling them: adapters over those would
+    end in the next forward, so the swap refuses them, all or none."""
+    m = nn.Sequential(nn.Linear(32, 32), nn.MultiheadAttention(32, 4), nn.TransformerEncoderLayer(32, 4, 64)).eval()
+    x = torch.randn(5, 2, 32, generator=torch.Generator().manual_seed(0))
+
+    def run():
+        h = m[0](x)
+        return m[2](m[1](h, h, h)[0])
+    before = run().detach()
+    for bad in ("1.out_proj", "2.linear1", "2.linear2", "2.self_attn.out_proj"):
+        with pytest.raises(ValueError, match="reads the layer's weight"):
+            swap.apply_lora(m, ["0", bad], rank=4)
+    assert type(m[0]) is nn.Linear and m[0].weight.requires_grad and torch.equal(run(), before)
+
+
 def test_refusals():
     x, a, b = torch.zeros(3, 8), torch.zeros(2, 4, 8), torch.zeros(2, 5, 4)
     i = torch.zeros(3, dtype=torch.int64)
