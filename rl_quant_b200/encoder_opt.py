@@ -9,7 +9,8 @@ The patched ``_encode_terrain`` is the reference's algebraic rewrite
 Without autograd it runs the fused sm_100a encoder in encoder-only mode
 (glad_actor_forward for the actor observation group, glad_critic_forward for
 the critic group): conv chain, pooling, query, top-32, attention. With autograd (PPO update) it runs the same rewrite in float torch
-ops on the model's own parameters, as the reference does.
+ops on the model's own parameters, as the reference does. With adapters over a
+layer of the encoder both take the model's own ``_encode_terrain``, which calls the layers.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ import torch
 import torch.nn.functional as F
 
 from .fused import FusedActor, FusedCritic
+from .lora import LoRALinear
 
 
 def _encode_terrain_float(self, obs):
@@ -70,7 +72,17 @@ def _gumbel_noise(logit_shape, device, dtype=torch.float16):
     return (-torch.log(-torch.log(u + 1e-10) + 1e-10)).float()
 
 
+def _has_adapters(self, obs):
+    """Whether a layer that encodes this observation group has adapters."""
+    actor = obs.shape[1] - self.L * self.W * self.coord_dim == self.actor_proprio_dim
+    layers = (self.actor_proprio_embedding if actor else self.critic_proprio_embedding, self.global_pool_selector,
+              self.query_projector, self.topk_scorer)
+    return any(isinstance(m, LoRALinear) for m in layers)
+
+
 def _encode_terrain_opt(self, obs):
+    if _has_adapters(self, obs):
+        return self._encode_terrain_orig(obs)
     if torch.is_grad_enabled():
         return _encode_terrain_float(self, obs)
     n_map = self.L * self.W * self.coord_dim

@@ -12,6 +12,7 @@ import torch.nn as nn
 
 from . import _native as N
 from .qconv import QuantCNN
+from .lora import LoRALinear
 from .qlinear import QuantLinear
 
 MLP_PATHS = ("actor.0", "actor.2", "actor.4", "actor.6")
@@ -65,6 +66,13 @@ def obs_norm_struct(norm, width: int) -> N.GladObsNorm:
     return N.GladObsNorm(mean.data_ptr(), var.data_ptr(), float(norm.eps), width)
 
 
+def refuse_adapters(model: nn.Module, *paths: str) -> None:
+    """The kernels read these layers' weights, which leaves adapters over them out."""
+    for p in paths:
+        if isinstance(model.get_submodule(p), LoRALinear):
+            raise FusedUnsupported(f"{p} has adapters")
+
+
 def model_act_mode(model: nn.Module) -> str:
     modes = {m.act_mode for m in model.modules() if isinstance(m, QuantLinear)}
     if len(modes) != 1 or not modes <= {"static", "dynamic"}:
@@ -88,6 +96,7 @@ class FusedActor:
         for p in ("actor_proprio_embedding", "query_projector") + (MLP_PATHS if need_mlp else ()):
             if not isinstance(model.get_submodule(p), QuantLinear):
                 raise FusedUnsupported(f"{p} is not a QuantLinear (swap.apply the qrt INT8 paths)")
+        refuse_adapters(model, "global_pool_selector", "topk_scorer")
         if model.actor_proprio_embedding.in_features != 96:
             raise FusedUnsupported("the fused encoder is built for a 96-wide actor proprio")
         if getattr(model, "num_heads", 16) != 16 or getattr(model, "mha_dim", 64) != 64:
@@ -206,6 +215,7 @@ class FusedCritic:
         self.use_actor_emb = self.P == int(model.actor_proprio_dim)
         if self.use_actor_emb and not isinstance(model.actor_proprio_embedding, QuantLinear):
             raise FusedUnsupported("actor_proprio_embedding must be a QuantLinear")
+        refuse_adapters(model, "global_pool_selector", "topk_scorer", *([] if self.use_actor_emb else ["critic_proprio_embedding"]))
         self.act_mode = model_act_mode(model)
         self._ws: dict[tuple, torch.Tensor] = {}
 

@@ -514,6 +514,43 @@ def test_runner_with_adapters(mode):
         bare.sync_weights_from(master)
 
 
+@gpu
+@pytest.mark.parametrize("path", ["topk_scorer", "global_pool_selector", "critic_proprio_embedding", "query_projector",
+                                  "actor_proprio_embedding"])
+def test_adapters_over_the_encoder(path, golden_weights):
+    """Layers that the fused forwards and the patched encoder read themselves: with adapters the policy runs op by op, and the adapters count, in
+    the rollout and in the update."""
+    from gpu_util import golden_model
+    from rl_quant_b200 import InferenceRunner
+    from rl_quant_b200.fused import FusedActor, FusedCritic, FusedUnsupported
+    from rl_quant_b200.synthetic import glad_obs_pair
+    m, _ = golden_model(golden_weights)
+    po, co = (t.cuda().half() for t in glad_obs_pair(12, seed=3))
+    heads = [(m.actor, po), (m.critic, co)]
+    with torch.no_grad():
+        before = [f(m._encode_terrain_orig(o)[0]) for f, o in heads]
+    layers = swap.apply_lora(m, [path], rank=4)
+    nn.init.normal_(layers[path].lora_b, std=0.5)
+    adapted = [path != "critic_proprio_embedding", path != "actor_proprio_embedding"]      # the observation groups that it encodes
+    with pytest.warns(UserWarning, match="op by op"):
+        run = InferenceRunner(m, mode="eager", with_critic=True)
+    assert [run._fused is None, run._fused_critic is None] == adapted
+    with torch.no_grad():
+        want = [f(m._encode_terrain_orig(o)[0]) for f, o in heads]
+        assert [not torch.equal(a, b) for a, b in zip(want, before)] == adapted
+        for got in ([run.act(po), run.evaluate(co)], [f(m._encode_terrain(o)[0]) for f, o in heads]):
+            assert all(torch.equal(a, b) for a, b, on in zip(got, want, adapted) if on)
+    make = FusedCritic if path == "critic_proprio_embedding" else FusedActor
+    with pytest.raises(FusedUnsupported):
+        make(m, need_mlp=False)
+    # the update: a gradient for the adapters (the scorer has one in train mode only)
+    m.train()
+    m.map_cnn.eval()
+    f, o = heads[path == "critic_proprio_embedding"]
+    f(m._encode_terrain(o)[0]).float().square().sum().backward()
+    assert layers[path].lora_a.grad is not None and layers[path].lora_b.grad.any()
+
+
 def test_module_surgery():
     m = net(torch.float32, "cpu")
     m.eval()
