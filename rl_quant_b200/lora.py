@@ -190,7 +190,8 @@ class LoRALinear(nn.Module):
     ``forward(x)`` is the layer's output plus each row's adapter, times alpha / rank.
 
     ``select(index)`` names the adapters of the rows from then on (int tensor of x's leading dimensions, or a number for all rows; -1:
-    none). Parameters ``lora_a`` [L, r, K] (random) and ``lora_b`` [L, N, r] (zeros, so a new adapter changes nothing);
+    none). The tensor is kept, not copied: new values in it count from the next call on, a captured one's too, while another selection
+    needs another capture (an ``InferenceRunner`` makes it by itself). Parameters ``lora_a`` [L, r, K] (random) and ``lora_b`` [L, N, r] (zeros, so a new adapter changes nothing);
     the layer below, ``base``, is kept as it is, and its Parameters are frozen where ``freeze`` is set. Rows are float32, float16 or
     bfloat16; where the layer's output type is not the adapters' own, rows and adapters are cast to it for the call."""
 

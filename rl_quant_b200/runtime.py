@@ -5,6 +5,8 @@ Modes (qrt/runtime.py:34-37, 83-84):
       (batch, dtype, device) in a CUDA graph with static input/output buffers;
       each call copies the observations in and replays.
   "eager": the fused forward is launched directly each call.
+A captured forward belongs to the adapters that were selected (``LoRALinear.select``): another number or another index tensor is
+captured anew, new values in the same tensor are read by the next call.
 
 The fused path needs the qrt full-mode layout (QuantCNN + QuantLinear on the
 encoder and actor MLP). A model without it runs ``act_inference`` op by op.
@@ -125,6 +127,7 @@ class InferenceRunner:
         self.with_critic = with_critic
         self.clone_outputs = clone_outputs
         self._quant_layers = [m for m in model.modules() if m is not model and hasattr(m, "requantize_")]
+        self._adapters = [m for m in model.modules() if isinstance(m, LoRALinear)]
         try:
             self._fused = FusedActor(model)
         except FusedUnsupported as e:
@@ -185,10 +188,15 @@ class InferenceRunner:
         enc, _, _, _ = (enc_fn or m._encode_terrain)(c)
         return m.critic(enc)
 
+    def _selection(self) -> tuple:
+        """What a captured forward holds of the adapters that are selected: a number, or the place of an index tensor."""
+        at = [m.index for m in self._adapters]
+        return tuple((i.data_ptr(), i.shape, i.stride(), i.dtype) if isinstance(i, torch.Tensor) else i for i in at)
+
     def _call(self, key, fn, *xs):
         if self.mode == "eager":
             return fn(*xs)
-        k = (key,) + tuple((tuple(x.shape), x.dtype, x.device) for x in xs)
+        k = (key,) + tuple((tuple(x.shape), x.dtype, x.device) for x in xs) + self._selection()
         g = self._graphs.get(k)
         if g is None:
             static = tuple(x.clone() for x in xs)
@@ -282,7 +290,7 @@ class InferenceRunner:
             x = host_obs.to(dev, non_blocking=True)
             out.copy_(self._act_fn(x), non_blocking=True)
             return out
-        k = ("act", tuple(host_obs.shape), host_obs.dtype, dev)
+        k = ("act", tuple(host_obs.shape), host_obs.dtype, dev) + self._selection()
         pipe = self._pipes.get(k)
         if pipe is None:
             pipe = _HostPipe(lambda st: self._new_graph(self._act_fn, st), host_obs.to(dev), self.host_lanes)

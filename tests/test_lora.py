@@ -551,6 +551,39 @@ def test_adapters_over_the_encoder(path, golden_weights):
     assert layers[path].lora_a.grad is not None and layers[path].lora_b.grad.any()
 
 
+@gpu
+@pytest.mark.parametrize("mode", ["eager", "manual-graph", "max-autotune"])
+def test_runner_follows_the_selection(mode):
+    """Numbers, index tensors and none, selected between calls of one runner: each call is of the adapters selected then. New values in the
+    same tensor need no new capture."""
+    from rl_quant_b200 import InferenceRunner, build_glad
+    from rl_quant_b200.synthetic import glad_obs_pair
+    torch.manual_seed(0)
+    m = build_glad().cuda().half().eval()
+    layers = swap.apply_lora(m, ["actor.0", "critic.2"], rank=8, adapters=3)
+    for mod in layers.values():
+        nn.init.normal_(mod.lora_b, std=0.1)
+    with pytest.warns(UserWarning, match="op by op"):
+        run = InferenceRunner(m, mode=mode, with_critic=True)
+    po, co = (t.cuda().half() for t in glad_obs_pair(10, seed=5))
+    host = po.cpu().pin_memory()
+    task = torch.tensor([0, 1, 2, -1, 0], device="cuda").repeat(2)
+    seen = []
+    for index in (0, 2, task, task.flip(0).contiguous(), task.int(), None, 2, task):
+        swap.select_lora(layers, index)
+        with torch.no_grad():
+            want = m.act_inference({"policy_obs": po})[0], m.evaluate(co)
+        got = run.act(po).clone(), run.evaluate(co).clone()
+        out = run.act_host(host)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(out, want[0].float().cpu())
+        seen.append(want[0].clone())
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[2], seen[3]) and torch.equal(seen[1], seen[6])
+    graphs = len(run._graphs)
+    task.copy_(task.flip(0))
+    assert torch.equal(run.act(po), seen[3]) and len(run._graphs) == graphs
+
+
 def test_module_surgery():
     m = net(torch.float32, "cpu")
     m.eval()
