@@ -190,7 +190,8 @@ int glad_qlinear_forward(const GladQLinear* L, int act_mode, const void* x, int 
  * runtime.py:98-99): _encode_terrain_opt (qrt/encoder_opt.py:41-123) over
  * QuantCNN/QuantLinear, then the INT8 actor MLP. obs [B, 96+2079] (f32 or
  * f16, row stride ld_obs elements) -> mean f32 [B,29]. With mean_out NULL
- * only the encoder runs (aux->encoded must then be set).
+ * only the encoder runs (aux->encoded must then be set); the MLP's layers may then be
+ * unset, each as a whole, but where aux->act_scales is wanted.
  * `topk_noise` (NULL or f32 [B,187]) is added to the top-k logits before
  * selection (the Gumbel term of train-mode rollouts, qrt/encoder_opt.py:87-91). */
 size_t glad_actor_workspace_size(int64_t B);
@@ -280,7 +281,7 @@ int glad_critic_forward(const GladCriticWeights* w, const void* obs, int obs_dty
  * glad_actor_forward_train) instead of read from memory, as the reference's
  * train-mode critic draws its own (qrt/integration.py:212-216,
  * qrt/encoder_opt.py:87-91); the call adds one to the device word
- * *gumbel_offset. value_out NULL runs the encoder only (aux->encoded set).   */
+ * *gumbel_offset. value_out NULL runs the encoder only (aux->encoded set; the MLP may be unset). */
 int glad_critic_forward_train(const GladCriticWeights* w, const void* obs, int obs_dtype, int64_t B,
                               int64_t ld_obs, int act_mode, uint64_t gumbel_seed,
                               unsigned long long* gumbel_offset, float* value_out, const GladActorAux* aux,

@@ -514,8 +514,11 @@ int actor_forward_impl(const GladActorWeights* w, const void* obs, int obs_dtype
   if ((rc = check_ql(&w->proprio_emb, "actor_proprio_embedding", 96, 64, false))) return rc;
   if ((rc = check_ql(&w->query_proj, "query_projector", 128, 64))) return rc;
   const int mk[4] = {224, 512, 256, 128}, mn[4] = {512, 256, 128, kActions};
-  for (int i = 0; i < 4; ++i)
-    if ((rc = check_ql(&w->mlp[i], "actor MLP layer", mk[i], mn[i]))) return rc;
+  const bool mlp = mean_out || dual || (aux && aux->act_scales);
+  for (int i = 0; i < 4; ++i) {        // an encoder-only call takes layers that are not there (but reads the first one's alpha and beta)
+    const GladQLinear& L = w->mlp[i];
+    if ((mlp || L.w8 || L.alpha || L.beta) && (rc = check_ql(&L, "actor MLP layer", mk[i], mn[i]))) return rc;
+  }
   if (!w->gps_w || !w->gps_b || !w->scorer_w || !w->scorer_b || !w->mha_in_w || !w->mha_in_b ||
       !w->mha_out_w || !w->mha_out_b)
     return fail(GLAD_ERR_INVALID_ARG, "fp16 encoder weights must be set");
@@ -750,7 +753,7 @@ int critic_forward_impl(const GladCriticWeights* w, const void* obs, int obs_dty
   if ((rc = check_norm(w->obs_norm, P + kMap, obs_dtype))) return rc;
   if ((rc = check_ql(&w->query_proj, "query_projector", 128, 64))) return rc;
   const int hk[4] = {128 + P, 512, 256, 128}, hn[4] = {512, 256, 128, 1};
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4 && value_out; ++i) {
     const GladLinear16& L = w->mlp[i];
     if (!L.weight || L.in_features != hk[i] || L.out_features != hn[i])
       return fail(GLAD_ERR_INVALID_ARG, "critic MLP layer %d must be %d -> %d", i, hk[i], hn[i]);

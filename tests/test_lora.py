@@ -584,6 +584,56 @@ def test_runner_follows_the_selection(mode):
     assert torch.equal(run.act(po), seen[3]) and len(run._graphs) == graphs
 
 
+@gpu
+@pytest.mark.parametrize("paths", [["actor.4"], ["actor.0", "actor.6"], ["critic.2"]])
+def test_adapters_over_the_quantised_policy(paths, golden_weights):
+    """The int8 policy with adapters over QuantLinear layers of its MLP (or over the critic's): the fused encoder still runs, the MLP op by
+    op, in the rollout and in the update; weights synchronised from a master are requantised below the adapters."""
+    from gpu_util import golden_model
+    from rl_quant_b200 import InferenceRunner, QuantLinear, build_glad
+    from rl_quant_b200.synthetic import glad_obs_pair
+    m, _ = golden_model(golden_weights)
+    po, co = (t.cuda().half() for t in glad_obs_pair(20, seed=7))
+    head, obs = (m.critic, co) if paths[0].startswith("critic") else (m.actor, po)
+    with torch.no_grad():
+        enc = m._encode_terrain(obs)[0].clone()
+        before = head(enc)
+    m.__dict__.pop("_glad_fused", None)
+    layers = swap.apply_lora(m, paths, rank=8, adapters=2)
+    for mod in layers.values():
+        assert isinstance(mod.base, nn.Linear if head is m.critic else QuantLinear)
+    task = torch.arange(20, device="cuda") % 3 - 1
+    swap.select_lora(layers, task)
+    for mode in ("eager", "manual-graph"):
+        with pytest.warns(UserWarning, match="op by op"):
+            run = InferenceRunner(m, mode=mode, with_critic=True)
+        act = run.evaluate if head is m.critic else run.act
+        with torch.no_grad():
+            assert torch.equal(m._encode_terrain(obs)[0], enc)       # the same kernels, bit for bit
+            if head is m.actor:
+                assert torch.equal(act(obs), before)                 # new adapters change nothing
+            for mod in layers.values():
+                nn.init.normal_(mod.lora_b, std=0.2)
+            got = act(obs).clone()
+            assert torch.equal(got, head(enc) if head is m.actor else head(m._encode_terrain_orig(obs)[0]))
+            swap.select_lora(layers, None)
+            assert not torch.equal(act(obs), got) and (head is m.critic or torch.equal(act(obs), before))
+            swap.select_lora(layers, task)
+            for mod in layers.values():
+                mod.lora_b.zero_()
+    head(m._encode_terrain(obs)[0]).float().square().sum().backward()
+    for mod in layers.values():
+        assert mod.lora_b.grad.any() and mod.base.weight.grad is None
+    master = build_glad(seed=1).cuda()
+    run.sync_weights_from(master)
+    for p, mod in layers.items():
+        assert torch.equal(mod.base.weight, master.get_submodule(p).weight.half())
+        if isinstance(mod.base, QuantLinear):
+            w8 = mod.base.w8.clone()
+            mod.base.requantize_()
+            assert torch.equal(mod.base.w8, w8) and w8.any()
+
+
 def test_module_surgery():
     m = net(torch.float32, "cpu")
     m.eval()
