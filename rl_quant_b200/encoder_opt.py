@@ -82,6 +82,8 @@ def _has_adapters(self, obs):
 
 def _encode_terrain_opt(self, obs):
     if _has_adapters(self, obs):
+        if not torch.is_grad_enabled():         # float32 rows too, as the fused encoder takes them
+            obs = obs.to(next(self.map_cnn.parameters()).dtype)
         return self._encode_terrain_orig(obs)
     if torch.is_grad_enabled():
         return _encode_terrain_float(self, obs)

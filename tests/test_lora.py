@@ -585,6 +585,23 @@ def test_runner_follows_the_selection(mode):
 
 
 @gpu
+def test_adapters_over_the_encoder_take_float32_observations(golden_weights):
+    """As the fused encoder does: the rows are rounded to the copy's type."""
+    from gpu_util import golden_model
+    from rl_quant_b200 import InferenceRunner
+    from rl_quant_b200.synthetic import glad_obs_pair
+    m, _ = golden_model(golden_weights)
+    nn.init.normal_(swap.apply_lora(m, ["topk_scorer"], rank=4)["topk_scorer"].lora_b, std=0.5)
+    with pytest.warns(UserWarning, match="op by op"):
+        run = InferenceRunner(m, mode="manual-graph", normalize=False)
+    po, co = (t.cuda() for t in glad_obs_pair(12, seed=3))
+    assert torch.equal(run.act(po), run.act(po.half()))
+    with torch.no_grad():
+        for o in (po, co):
+            assert all(torch.equal(a, b) for a, b in zip(m._encode_terrain(o), m._encode_terrain(o.half())))
+
+
+@gpu
 @pytest.mark.parametrize("paths", [["actor.4"], ["actor.0", "actor.6"], ["critic.2"]])
 def test_adapters_over_the_quantised_policy(paths, golden_weights):
     """The int8 policy with adapters over QuantLinear layers of its MLP (or over the critic's): the fused encoder still runs, the MLP op by
