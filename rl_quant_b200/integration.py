@@ -14,7 +14,9 @@ What it does (qrt/integration.py:94-247):
   * ``alg.update`` is wrapped so every PPO iteration first checks the device
     status of the rollout's fused forwards (``InferenceRunner.check_status``,
     raising ``DeviceStatusError`` if a bounded device-side wait ran out) and
-    ends with ``sync_weights_from`` (one graphed cast-copy + requantisation).
+    ends with ``sync_weights_from`` (one graphed cast-copy + requantisation);
+  * adapters of the policy (``swap.apply_lora`` before this call) are in the copy
+    too, and every rollout call takes the selection that the policy's have then.
 
 Training-side options of the reference (``accelerate_update``,
 ``update_amp``, ``cocalib``) concern the PPO update, which is outside this
@@ -33,6 +35,7 @@ from torch.distributions import Normal
 from . import calib as _calib
 from . import swap as _swap
 from .encoder_opt import patch_encoder
+from .lora import LoRALinear
 from .qconv import calib_cnn_scale, swap_cnn
 from .runtime import InferenceRunner
 
@@ -101,6 +104,12 @@ class QRTAccelerator:
         self._runner = InferenceRunner(infer, mode=mode, with_critic=True, normalize=False)
         self._sync_runner = self._runner
 
+        adapters = [(m, infer.get_submodule(p)) for p, m in self.policy.named_modules() if isinstance(m, LoRALinear)]
+
+        def follow():
+            for mine, theirs in adapters:
+                theirs.index = mine.index
+
         policy = self.policy
         self._orig_ud = policy.update_distribution
         self._orig_eval = policy.evaluate
@@ -115,12 +124,14 @@ class QRTAccelerator:
 
         def update_distribution_qrt(self_p, actor_obs):
             if torch.is_inference_mode_enabled():
+                follow()
                 _make_dist(self_p, run.act(actor_obs).float())
             else:
                 acc._orig_ud(actor_obs)
 
         def evaluate_qrt(self_p, obs, **kwargs):
             if torch.is_inference_mode_enabled():
+                follow()
                 co = self_p.critic_obs_normalizer(self_p.get_critic_obs(obs))
                 return run.evaluate(co.half()).float()
             return acc._orig_eval(obs, **kwargs)
@@ -139,6 +150,7 @@ class QRTAccelerator:
             def act_fused(obs):
                 if policy.is_recurrent:
                     return acc._orig_act(obs)
+                follow()
                 # raw groups; the master's normalisers run inside the kernels' row loads
                 ao = policy.get_actor_obs(obs)
                 co = policy.get_critic_obs(obs)

@@ -651,6 +651,57 @@ def test_adapters_over_the_quantised_policy(paths, golden_weights):
             assert torch.equal(mod.base.w8, w8) and w8.any()
 
 
+@gpu
+@pytest.mark.parametrize("paths", [["actor.4", "critic.0"], ["topk_scorer", "actor.0"]])
+def test_accelerated_policy_with_adapters(paths):
+    """accelerate_runner over a policy with adapters: rollouts are of the adapters that the policy has selected then, and of its current
+    weights after an update."""
+    import types
+
+    from rl_quant_b200 import accelerate_runner, build_glad
+    from rl_quant_b200.synthetic import glad_obs_pair
+    torch.manual_seed(0)
+    policy = build_glad().cuda().eval()
+    layers = swap.apply_lora(policy, paths, rank=8, adapters=3)
+    for mod in layers.values():
+        nn.init.normal_(mod.lora_b, std=0.3)
+    obs = dict(zip(("policy_obs", "critic_obs"), (t.cuda() for t in glad_obs_pair(32, seed=6))))
+    alg = types.SimpleNamespace(policy=policy, act=lambda o: None, update=lambda: {})
+    with pytest.warns(UserWarning, match="op by op"):
+        acc = accelerate_runner(types.SimpleNamespace(alg=alg, device="cuda", env=None), calib_obs=[obs], let_steps=5, mode="manual-graph",
+                                rollout_training=False, verbose=False)
+    inner = {p: acc.infer.get_submodule(p) for p in paths}
+    assert all(isinstance(m, LoRALinear) for m in inner.values())
+    seen = []
+    task = torch.arange(32, device="cuda") % 4 - 1
+    for index in (0, 2, task, None):
+        if isinstance(index, torch.Tensor) and "topk_scorer" in paths:
+            layers["actor.0"].select(index)               # the scorer's rows are those of a map
+        else:
+            swap.select_lora(layers, index)
+        with torch.inference_mode():
+            policy.update_distribution(policy.get_actor_obs(obs))
+            mean, value = policy.action_mean.clone(), policy.evaluate(obs).clone()
+            float_mean = policy.actor(acc._orig_ud.__self__._encode_terrain(policy.get_actor_obs(obs))[0])
+        seen.append(mean)
+        # the copy's int8 layers and 16-bit rows: a few percent, other adapters change more than that
+        assert float((mean - float_mean).norm() / float_mean.norm()) < 0.1
+        assert float((value - acc._orig_eval(obs)).norm() / acc._orig_eval(obs).norm()) < 0.1
+        assert all(m.index is layers[p].index for p, m in inner.items())
+    assert all(float((a - b).norm() / b.norm()) > 0.2 for a, b in zip(seen, seen[1:]))
+    swap.select_lora(layers, 0)
+    with torch.no_grad():
+        for mod in layers.values():
+            mod.lora_b.mul_(-1.0)
+    alg.update()
+    with torch.inference_mode():
+        policy.update_distribution(policy.get_actor_obs(obs))
+    assert not torch.equal(policy.action_mean, seen[0])
+    for p, m in inner.items():
+        assert torch.equal(m.lora_b, layers[p].lora_b.half())
+    acc.detach()
+
+
 def test_module_surgery():
     m = net(torch.float32, "cpu")
     m.eval()
