@@ -22,6 +22,13 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 
+// Counting warps, as many as shared memory has counters for, and its size with them, which is largest at the most adapters.
+constexpr int plan_warps(int L) { return L < 1024 ? 32 : L < 4096 ? 8 : 2; }
+constexpr size_t plan_smem(int warps, int L) { return (size_t)(warps * (L + 1) + L + 2) * 4; }
+constexpr size_t kPlanSmem = plan_smem(plan_warps(kMaxAdapters), kMaxAdapters);
+static_assert(kPlanSmem >= plan_smem(plan_warps(1023), 1023) && kPlanSmem >= plan_smem(plan_warps(4095), 4095) && kPlanSmem <= 226 * 1024,
+              "the most of any call");
+
 struct PlanParams {
   const void* index;
   int32_t* plan;
@@ -201,14 +208,14 @@ int64_t plan_words(int64_t M, int L) { return 3 + L + M + 2 * max_tiles(M, L, 16
 cudaError_t make_plan(const void* index, int index_bytes, int64_t M, int64_t sides, int L, int r, bool wide16, void* plan,
                       cudaStream_t st) {
   static size_t limit[64] = {};
-  // counting warps: 256 rows each if possible, which they hold in registers; as many as shared memory has counters for
-  int warps = L < 1024 ? 32 : L < 4096 ? 8 : 2;
+  // 256 rows a counting warp if possible, which it holds in registers
+  int warps = plan_warps(L);
   if (M < 256 * warps) warps = (int)((M + 255) / 256);
   const PlanParams p{index, static_cast<int32_t*>(plan), (int)M, L, index_bytes == 8, warps, tile_rows(M, sides, L, r, true, wide16)};
-  const size_t smem = (size_t)(warps * (L + 1) + L + 2) * 4;
-  const cudaError_t e = allow_smem(plan_kernel, smem, limit);
+  // the most of any call, so that the first calls of two threads allow the same whichever comes last
+  const cudaError_t e = allow_smem(plan_kernel, kPlanSmem, limit);
   if (e != cudaSuccess) return e;
-  return launch_k(plan_kernel, dim3(1), dim3(kPlanThreads), smem, st, true, p);
+  return launch_k(plan_kernel, dim3(1), dim3(kPlanThreads), plan_smem(warps, L), st, true, p);
 }
 
 }  // namespace
