@@ -88,10 +88,11 @@ __device__ __forceinline__ float tf32(float v) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
   return __uint_as_float(r);
 }
-// v = hi + lo, 11 bits each. Where hi is infinite, lo is finite (the difference would be a NaN).
+// v = hi + lo, 11 bits each. Of an infinite v, lo is finite (the difference would be a NaN): the least that a finite v has, half a step of
+// the largest number, so that products with it do not overflow beside the infinite ones. The 16-bit splits below alike.
 __device__ __forceinline__ void split(float v, float& hi, float& lo) {
   hi = tf32(v);
-  lo = tf32(fmaxf(v - hi, -3e38f));
+  lo = tf32(fmaxf(v - hi, -1.7e35f));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const float4& a, float b0, float b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -279,14 +280,14 @@ __device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint3
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   const float2 f = __bfloat1622float2(h);
-  const __nv_bfloat162 l = __floats2bfloat162_rn(fmaxf(a - f.x, -3e38f), fmaxf(b - f.y, -3e38f));    // as in split()
+  const __nv_bfloat162 l = __floats2bfloat162_rn(fmaxf(a - f.x, -6.7e35f), fmaxf(b - f.y, -6.7e35f));
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(a, b);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(fmaxf(a - f.x, -3e38f), fmaxf(b - f.y, -3e38f));
+  const __half2 l = __floats2half2_rn(fmaxf(a - f.x, -16.0f), fmaxf(b - f.y, -16.0f));
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // A row's power of two and its inverse: brings its largest number (as bits) to 2^14, so that the lower halves reach 2^-38 of it.
@@ -747,9 +748,9 @@ __global__ void __launch_bounds__(kThreads, RT == 16 ? 2 : 1) lora_kernel(const 
       } else {
         v = part[i];
       }
-      v *= s;
-      whole[i] = v;
       const int row = i / RT, at = i % RT;
+      v = at < p.r ? v * s : 0.0f;                     // behind the ranks: 0 times an infinite x
+      whole[i] = v;
       if (p.u && rank == 0 && row < n && at < p.r) p.u[(int64_t)rows[row] * p.r + at] = kept<T>(v);
     }
     __syncthreads();
@@ -1296,7 +1297,7 @@ __global__ void __launch_bounds__(Tc<RT>::kThreads, 1) lora_tc_kernel(const Para
           f[4] += o[2 * c + 1].x, f[5] += o[2 * c + 1].y, f[6] += o[2 * c + 1].z, f[7] += o[2 * c + 1].w;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= s;
+        for (int e = 0; e < 8; ++e) f[e] = 8 * c8 < p.r ? f[e] * s : 0.0f;      // as in the rings
         if (p.u && row < n && 8 * c8 < p.r) {
           float4* u = reinterpret_cast<float4*>(p.u + (int64_t)rows[row] * p.r + 8 * c8);
           u[0] = make_float4(kept<T>(f[0]), kept<T>(f[1]), kept<T>(f[2]), kept<T>(f[3]));

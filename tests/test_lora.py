@@ -246,6 +246,40 @@ def test_rows_keep_to_themselves(dtype, r):
 
 
 @gpu
+@pytest.mark.parametrize("size", [(90, 96, 80, 16), (90, 97, 81, 15), (300, 96, 80, 128), (300, 96, 80, 72),
+                                  (1290, 96, 80, 64), (1290, 96, 80, 40), (4130, 96, 80, 128), (4130, 96, 80, 104)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinities_of_16_bit_rows(size, dtype):
+    """Positive numbers with an infinity in a row of x and in one of dy: infinite, not NaN, where u and du are, although they are taken as
+    pairs of 16-bit numbers; the other rows and adapters as without."""
+    m, k, n, r = size
+    x, a, b, i, scale, base, dy = make(m, k, n, r, 3, dtype, 17, sign=True)
+    a, b = a + 2.0 ** -10, b + 2.0 ** -10                # no zeros, which times an infinity are NaN
+    x, dy = x + 2.0 ** -10, dy + 2.0 ** -10
+    i[5], i[7] = 1, 2
+    clean = [t.clone().requires_grad_() for t in (x, a, b)]
+    want = lora_linear(*clean, i, scale, base)
+    want = [want.detach(), *torch.autograd.grad(want, clean, dy)]
+    x, dy = x.clone(), dy.clone()
+    x[5, 3] = math.inf
+    dy[7, 4] = math.inf
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    y = lora_linear(*leaves, i, scale, base)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    for j, (g, w) in enumerate(zip(got, want)):
+        hit, past = torch.zeros_like(g, dtype=torch.bool), torch.zeros_like(g, dtype=torch.bool)
+        if j < 2:
+            hit[5 + 2 * j] = True                        # y of the one row, dx of the other
+        elif j == 2:
+            hit[2], past[1, :, 3] = True, True           # du of row 7; the column of x, times a pair that may have both signs
+        else:
+            hit[1], past[2, 4] = True, True              # u of row 5; the column of dy
+        assert (g[hit] == math.inf).all() and not torch.isfinite(g[past]).any(), j
+        hit |= past
+        assert torch.equal(g[~hit], w[~hit]), j
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_repeats_streams_and_graphs(dtype):
     for m, r in ((30, 16), (700, 16), (700, 64), (1300, 64)):
