@@ -1,6 +1,6 @@
 """lora_linear and its gradients against the formula in 64 bits.
 
-Tolerances, fixed before the first run. One matrix instruction adds up to 17 terms aligned to the largest, each off by at most
+Tolerances, from the arithmetic of the kernels. One matrix instruction adds up to 17 terms aligned to the largest, each off by at most
 2^-24 of it: 2^-20 of the running sum of magnitudes. A warp runs at most K / 64 + 2 of them for u, the tensor-core kernel (16-bit rows, ranks above 32) at most K / 16 (the 16-bit
 products are exact; split fp32 ones are off by 2^-20), and the joins of warps and blocks add at most 16 roundings: so u is off by
 (K / 64 + 20) 2^-20 sum |x| |A|, or K / 16 for K / 64.
@@ -123,12 +123,13 @@ SIZES = [(1, 64, 64, 16, 1), (1, 4096, 512, 16, 3), (5, 1, 1, 1, 2), (7, 33, 65,
          (300, 200, 320, 48, 1), (300, 72, 64, 100, 2), (130, 128, 128, 128, 2), (1000, 48, 40, 16, 130), (2050, 520, 264, 16, 2),
          (600, 1024, 1024, 33, 1),
          (8192, 32, 24, 16, 512), (4096, 32, 24, 16, 512), (4097, 40, 24, 8, 3), (8200, 24, 32, 8, 7), (400, 16, 16, 16, 600), (1500, 64, 64, 64, 3),
-         # tiles of 128 rows on the tensor core's memory: one and several, odd counts of chunks and of columns, empty adapters
+         # high ranks: one and several tiles of any height, odd counts of chunks and of columns, empty adapters (TC_SIZES below are
+         # those that the tensor-core kernel takes)
          (64, 64, 64, 64, 1), (129, 72, 136, 40, 1), (700, 4096, 264, 64, 2), (300, 520, 1032, 128, 1), (2000, 1000, 504, 96, 9),
          (513, 2048, 2048, 128, 4), (3000, 192, 320, 80, 3), (1024, 64, 64, 64, 1), (1025, 72, 136, 40, 1), (1300, 4096, 264, 64, 2), (1300, 64, 64, 64, 1), (1297, 72, 136, 40, 1),
          (1300, 520, 1032, 128, 1), (1030, 128, 640, 128, 16), (9000, 64, 48, 64, 3), (5000, 520, 264, 24, 1),
          (700, 1032, 264, 32, 40), (1000, 776, 1000, 128, 3),
-         # as many rows and ranks, off the 16 bytes: the other kernel on the same tiles
+         # as many rows and ranks, off the 16 bytes
          (1200, 72, 64, 100, 2), (1300, 73, 65, 64, 2), (1330, 70, 68, 40, 3),
          (4100, 136, 72, 128, 5), (128, 96, 72, 16, 4), (256, 72, 64, 64, 3), (200, 73, 64, 16, 2), (4100, 70, 72, 100, 2), (1100, 4096, 4096, 72, 3)]
 
@@ -142,6 +143,43 @@ def test_sizes(size, dtype):
         if index == "one" and L == 1:
             index = None
         check(*make(m, k, n, r, L, dtype, seed, sign, base, index))
+
+
+# Calls that the tensor-core kernel takes, forward and backward: few and many adapters (some without rows), ranks that are no power of two, inputs and outputs
+# of several chunks of 128 and a rest, or of less than one.
+TC_SIZES = [(4100, 136, 72, 80, 9), (4096, 264, 392, 96, 16), (5200, 648, 904, 128, 40), (4200, 72, 136, 104, 1), (1100, 4096, 4096, 128, 2),
+            (1030, 4104, 4104, 96, 3), (4099, 2184, 136, 72, 12), (8000, 136, 1544, 128, 33), (4224, 128, 128, 120, 66),
+            (1300, 392, 264, 64, 9), (2700, 1032, 776, 56, 40), (1500, 8, 8, 40, 5), (1280, 1000, 1160, 48, 20), (1177, 264, 136, 64, 1)]
+
+
+def test_sizes_of_the_tensor_core_kernel():
+    """The workspace of the backward pass, for the adapters transposed, tells which kernel takes a call."""
+    from rl_quant_b200 import _native as N
+    size = N.load().glad_lora_backward_workspace_size
+    for m, k, n, r, L in TC_SIZES:
+        for code in (N.DTYPE_F16, N.DTYPE_BF16):
+            assert size(m, k, n, L, r, code, L > 1) == 2 * L * r * (k + n)
+        assert size(m, k, n, L, r, N.DTYPE_F32, L > 1) == 0
+    # the borders: rows, rank, rows an adapter, ranks off 8
+    few, many = 1024, 4096
+    for at in ((1160, 72, 72, 64, 1), (few, 4096, 4000, 128, 1), (many - 1, 136, 72, 128, 1), (1300, 72, 72, 32, 1), (2700, 72, 72, 64, 43),
+               (4100, 72, 72, 100, 1)):
+        m, k, n, r, L = at
+        assert size(m, k, n, L, r, N.DTYPE_BF16, L > 1) == 0, at
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", TC_SIZES)
+def test_tensor_core_kernel(size, dtype):
+    m, k, n, r, L = size
+    for seed, (sign, base, index) in enumerate(((True, False, "mixed"), (False, True, "runs"), (False, True, "one"))):
+        if L == 1:
+            index = None
+        data = make(m, k, n, r, L, dtype, 20 + seed, sign, base, index)
+        if index == "mixed" and L > 4:
+            data[3][data[3] % 3 == 1] = 0                # a third of the adapters without rows
+        check(*data)
 
 
 @gpu
