@@ -1,8 +1,8 @@
 """grad_norm / clip_grads / clip_grads_ / clip_grad_norm_ against the formula in 64 bits.
 
-Tolerances, fixed before the first run: a thread adds at most 128 squares of a chunk in four running sums (33 roundings
-of 2^-24 each, and 2 to join them), the rest is 64-bit; the root halves that and its rounding to float32 adds one: NORM2 = 20 *
-2^-24, and 37 * 2^-24 for the sum of magnitudes. The maximum is exact. The coefficient adds three roundings, the product one."""
+Tolerances: they allow a thread batches of up to 128 squares in four running sums (33 roundings
+of 2^-24 each, and 2 to join them), the rest in 64 bits; the root halves that and its rounding to float32 adds one: NORM2 = 20 *
+2^-24, and 37 * 2^-24 for the sum of magnitudes (test_bounds_of_the_present_batch has those of the batches that the kernel takes). The maximum is exact. The coefficient adds three roundings, the product one."""
 import itertools
 import math
 
@@ -71,6 +71,21 @@ def test_sizes(sizes, types, p):
     ts = make(sizes, types, 1)
     check(ts, 0.25, p)
     check(make(sizes, types, 2), 1e9, p)
+
+
+@gpu
+@pytest.mark.parametrize("p", [2.0, 1.0])
+@pytest.mark.parametrize("types", [[t] for t in TYPES] + [TYPES])
+def test_bounds_of_the_present_batch(types, p):
+    """A thread adds at most 32 values (16 of float32) in four running sums before they become 64-bit: 8 roundings of a sum's squares, 7 of
+    its magnitudes, 2 to join the four, the root halves them and its rounding to float32 adds one: 6 * 2^-24, and 10 for the magnitudes; one
+    more of each covers the 64-bit sums. Values whose squares round the same way are among them."""
+    bound = {2.0: 7 * U, 1.0: 11 * U}[p]
+    sets = [make(sizes, types, 11) for sizes in ([100_003], [2048, 33, 4095], [1_000_001, 17, 262_144])]
+    same = [torch.full((70_001,), 1.0 + 2 ** -k, dtype=t, device="cuda") for t in types for k in (3, 6, 7)]
+    for ts in sets + [same]:
+        n = ref_norm(ts, p)
+        assert abs(float(grad_norm(ts, p)) - n) <= bound * n
 
 
 @gpu
