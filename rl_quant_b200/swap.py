@@ -109,7 +109,7 @@ def restore_lora(model: nn.Module, swapped: dict[str, LoRALinear]) -> None:
 
 
 def restore(model: nn.Module, swapped: dict[str, nn.Module]) -> None:
-    """Put plain nn.Linear shells (holding the same Parameters) back."""
+    """Put plain nn.Linear shells (holding the same Parameters) back; below adapters, where the layers have got some since."""
     for path, q in swapped.items():
         lin = nn.Linear(q.in_features, q.out_features, bias=q.bias is not None,
                         device=q.weight.device, dtype=q.weight.dtype)
@@ -117,7 +117,8 @@ def restore(model: nn.Module, swapped: dict[str, nn.Module]) -> None:
         if q.bias is not None:
             lin.bias = q.bias
         lin.train(q.training)
-        set_module(model, path, lin)
+        top = get_module(model, path)
+        set_module(model, f"{path}.base" if isinstance(top, LoRALinear) else path, lin)
 
 
 def refresh(swapped: dict[str, QuantLinear]) -> None:

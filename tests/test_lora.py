@@ -862,6 +862,18 @@ def test_module_surgery():
     assert m[0] is lin and not lin.training
 
 
+def test_restore_below_adapters():
+    """Plain layers put back for quantised ones come below the adapters that were put over those since."""
+    m = net(torch.float32, "cpu").eval()
+    weight = m[0].weight
+    q = swap.apply(m, {"0": {"bits": 4, "group": 32}})
+    layers = swap.apply_lora(m, ["0"], rank=4)
+    swap.restore(m, q)
+    assert m[0] is layers["0"] and type(m[0].base) is nn.Linear and m[0].base.weight is weight and not m[0].base.training
+    swap.restore_lora(m, layers)
+    assert type(m[0]) is nn.Linear and m[0].weight is weight
+
+
 def test_layers_that_their_parent_computes_itself():
     """nn.MultiheadAttention and nn.TransformerEncoderLayer read weights of layers below instead of calling them: adapters over those would
     end in the next forward, so the swap refuses them, all or none."""
