@@ -471,7 +471,8 @@ int glad_debug_w4_wait(uint32_t hold, uint64_t limit_ns);
  *   u[m] = scale[i] * a[i] x[m],   y[m] = base[m] + b[i] u[m],   i = index[m]
  * index (i32 or i64, index_bytes 4 or 8; NULL: adapter 0 for all, L = 1) outside [0, L): no adapter, y = base.
  * base [M, N] (row stride ldb, NULL: zeros) and y (contiguous) have x's type; u [M, r] (4 bytes each) or NULL is what the
- * backward pass reads (bf16 rows: two bf16 numbers, u's sum). r 1..128, L up to 16384, M, K and N up to 2^24. u and the sums are f32, y is rounded once.
+ * backward pass reads (f32; bf16 rows: two bf16 numbers whose sum it is). r 1..128, L up to 16384, M, K and N up to 2^24. Sums are f32, y
+ * is rounded once; in the second product (and in the gradients) u counts with 16 bits beside bf16 rows, with 22 beside others.
  * Infinite inputs give infinite or NaN outputs in their rows.
  * plan: glad_lora_plan_size(M, L) bytes (16-byte aligned) that the call fills with the order of the rows by adapter;
  * needed with an index where a backward pass follows, for more than 4096 rows, and for more than 256 with more than 512
@@ -506,7 +507,8 @@ int glad_debug_lora_wait(uint32_t hold, uint64_t limit_ns);
  *   top_index, top_log_prob [rows, top]: the `top` (0..32, at most cols) largest logits'
  *     columns and log probabilities, largest first, the lower column first among equals
  *   stats [rows, 2]: what the backward pass reads                   (NULL: not wanted)
- * Logits of -inf have probability 0 and add nothing to the entropy; a row of nothing else has log probability
+ * Logits of -inf have probability 0, add nothing to the entropy and have no gradient (but what the log probability of a given column
+ * has in itself, where that is masked); a row of nothing else has log probability
  * -inf, entropy 0 and no gradient. A row whose token is ignore_index counts for
  * nothing, whatever it holds: its outputs are 0 (top_index -1), its gradient 0. Any other token outside [0, cols) gives NaN,
  * as does a NaN or +inf in the row. All f32 but top_index (i64).               */

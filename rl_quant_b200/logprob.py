@@ -95,7 +95,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, temperature: flo
 
     logits float32, float16 or bfloat16, rows of any stride; tokens int64 or int32. ``log_prob`` [...], ``entropy`` [...] and
     ``top_log_prob`` [..., top] are float32 and differentiable in the logits (backward mode), ``top_index`` [..., top] int64:
-    the most likely first, the lower index first among equals. Logits of -inf are masked: probability 0, no gradient. A row that is
+    the most likely first, the lower index first among equals. Logits of -inf are masked: probability 0, no gradient (the token itself and
+    the alternatives keep their own term, as in torch: d log p_t / d x_t = (1 - p_t) / temperature). A row that is
     masked as a whole has log probability -inf, entropy 0 and no gradient. Rows whose token is ``ignore_index`` count as
     empty whatever they hold: their outputs are 0 (``top_index`` -1), their gradients 0. Any other token outside [0, V) gives NaN, in the row's gradient too."""
     N.refuse_tangents("token_log_probs", logits)

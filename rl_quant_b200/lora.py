@@ -122,7 +122,8 @@ def lora_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.
     x [..., K], a [L, r, K], b [L, N, r] and base have one type, float32, float16 or bfloat16; rows of x and base may have any
     stride. index [...] int64 or int32 names the adapter of each row of x; outside 0..L-1 (by custom -1) the row has none. None:
     adapter 0 for all (L = 1). scale a number, or float32 [L]. r up to 128, L up to 16384. Differentiable in x, a, b and
-    base (backward mode). Sums are float32 and the result is rounded once. Large calls of high rank wait for the tensor core with a
+    base (backward mode). Sums are float32 and the result is rounded once; A x (and B^T dy), between the two products, counts with 16
+    bits beside bfloat16 rows and with 22 beside others. Large calls of high rank wait for the tensor core with a
     bound; ``w4_status`` tells of a wait that ran out."""
     dt, shape, dev, a_shape, b_shape = x.dtype, x.shape, x.device, a.shape, b.shape
     if dt not in _CODE:
