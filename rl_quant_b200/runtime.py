@@ -425,7 +425,7 @@ class InferenceRunner:
         """Cast-copy every same-named parameter/buffer of ``src_model`` (the fp32
         master) into this copy, then requantise (qrt/runtime.py:224-271). A layer under
         adapters here takes the weights of a master without them; a master's adapters that
-        this copy lacks are an error."""
+        this copy lacks, or has of another number, rank or scale, are an error."""
         if self._sync_items is None:
             for p in self.model.parameters():
                 p.requires_grad_(False)
@@ -435,9 +435,16 @@ class InferenceRunner:
                 if isinstance(m, LoRALinear):       # the layer below under the name that it has without adapters
                     for name, t in list(m.base.named_parameters()) + list(m.base.named_buffers()):
                         dst.setdefault(f"{path}.{name}" if path else name, t)
+            here = dict(self.model.named_modules())
             for path, m in src_model.named_modules():
-                if isinstance(m, LoRALinear) and (f"{path}.lora_a" if path else "lora_a") not in dst:
+                if not isinstance(m, LoRALinear):
+                    continue
+                mine = here.get(path)
+                if not isinstance(mine, LoRALinear):
                     raise ValueError(f"{path}: the source has adapters, this copy has none")
+                if (mine.lora_a.shape, mine.lora_b.shape, mine.scale) != (m.lora_a.shape, m.lora_b.shape, m.scale):
+                    raise ValueError(f"{path}: the source has {m.adapters} adapters of rank {m.rank} and scale {m.scale:g}, this copy "
+                                     f"{mine.adapters} of rank {mine.rank} and scale {mine.scale:g}")
             items, keep = [], []
             for name, s in list(src_model.named_parameters()) + list(src_model.named_buffers()):
                 d = dst.get(name)

@@ -862,6 +862,23 @@ def test_module_surgery():
     assert m[0] is lin and not lin.training
 
 
+@pytest.mark.parametrize("other", [dict(rank=4), dict(adapters=2), dict(alpha=32.0)])
+def test_sync_refuses_other_adapters(other):
+    """A master's adapters of another rank, number or scale than the copy's: an error before anything is copied."""
+    from rl_quant_b200 import InferenceRunner, build_glad
+    common = dict(rank=8, adapters=3, alpha=16.0)
+    copy, master = build_glad(0), build_glad(1)
+    swap.apply_lora(copy, ["actor.0"], **common)
+    swap.apply_lora(master, ["actor.0"], **{**common, **other})
+    with pytest.warns(UserWarning, match="op by op"):
+        run = InferenceRunner(copy)
+    before = copy.actor[2].weight.clone()
+    for _ in range(2):
+        with pytest.raises(ValueError, match="actor.0: the source has"):
+            run.sync_weights_from(master)
+    assert torch.equal(copy.actor[2].weight, before)
+
+
 def test_restore_below_adapters():
     """Plain layers put back for quantised ones come below the adapters that were put over those since."""
     m = net(torch.float32, "cpu").eval()
